@@ -157,6 +157,7 @@ def _inputs(case, seed):
 def prepare(case, seed):
     state = _inputs(case, seed)
     state["case"] = case
+    state["flag"] = torch.zeros(1, dtype=torch.int32, device="cuda")  # the packs' error flag, one for a pipeline
     return state
 
 
@@ -233,19 +234,20 @@ def _calls(t, case):
     from pih_amd.linear import (adapter_backward, adapter_gemm, lm_head_loss, lm_head_loss_backward, router_backward,
                                 router_balance)
 
-    kind = case["kind"]
+    kind, flag = case["kind"], t["flag"]
     with engine_stream():
         if kind == "adapter":
-            return adapter_gemm(t["x"], t["a"], t["b"], t["scale"], t["offsets"], t["adapters"], base=t["base"])[0]
+            return adapter_gemm(t["x"], t["a"], t["b"], t["scale"], t["offsets"], t["adapters"], base=t["base"],
+                                flag=flag)[0]
         if kind == "adapter_grad":
             return adapter_backward(t["dy"], t["x"], t["a"], t["b"], t["scale"], t["offsets"], t["adapters"],
-                                    base=t["base"])[:3]
+                                    base=t["base"], flag=flag)[:3]
         if kind == "loss":
-            return lm_head_loss(t["x"], t["w"], t["target"])[:2]
+            return lm_head_loss(t["x"], t["w"], t["target"], flag=flag)[:2]
         if kind == "loss_grad":
-            return lm_head_loss_backward(t["x"], t["w"], t["target"], t["lse"], t["dloss"])[:2]
+            return lm_head_loss_backward(t["x"], t["w"], t["target"], t["lse"], t["dloss"], flag=flag)[:2]
         mode = abi.ROUTER_SQRT_SOFTPLUS if case["softplus"] else abi.ROUTER_SOFTMAX
-        loss, counts, mean, flag = router_balance(t["scores"], t["ids"], mode, t["coefficient"])
+        loss, counts, mean, _ = router_balance(t["scores"], t["ids"], mode, t["coefficient"], flag=flag)
         if not case["grad"]:
             return [loss, counts, mean]
         dscores, _ = router_backward(t["scores"], t["ids"], counts, mode, t["coefficient"], t["dloss"],
