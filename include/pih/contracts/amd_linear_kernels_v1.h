@@ -69,7 +69,16 @@
  *   launch_v41_block_dequant
  *                          the V4.1 wo_a e4m3 x block-scale -> bf16
  *                          dequantisation (weight_dequantize.cpp:17-50,
- *                          DequantizeWoATensor) on the device.
+ *                          DequantizeWoATensor) on the device;
+ *   query_adapter_backward_workspace, launch_adapter_gemm,
+ *   launch_adapter_backward, launch_lm_head_loss,
+ *   launch_lm_head_loss_backward, launch_router_balance,
+ *   launch_router_backward
+ *                          low-rank adapters on top of any projection's
+ *                          output, the LM head's softmax cross entropy, the
+ *                          router's balance loss and the gradients of all
+ *                          three (no reference counterpart: the reference
+ *                          serves one set of weights and does not train).
  *
  * Conventions are those of the reference's pack tables: one request pointer
  * in, pih_status_v1 by value out; a NULL request, wrong struct_size or wrong
@@ -114,12 +123,18 @@ extern "C" {
 #define PIH_AMD_WORKSPACE_ROUTE_PLAN_V1 1U
 #define PIH_AMD_WORKSPACE_BF16_GEMM_V1 2U
 #define PIH_AMD_WORKSPACE_W4A16_V1 3U
+#define PIH_AMD_WORKSPACE_ADAPTER_GEMM_V1 4U
+#define PIH_AMD_WORKSPACE_LM_HEAD_LOSS_V1 5U
+#define PIH_AMD_WORKSPACE_LM_HEAD_LOSS_BACKWARD_V1 6U
+#define PIH_AMD_WORKSPACE_ROUTER_BALANCE_V1 7U
 
 /* Scratch size query (host only; touches no device). */
 typedef struct pih_amd_workspace_query_v1 {
   uint32_t struct_size, abi_version;
   uint32_t kind;          /* PIH_AMD_WORKSPACE_* */
-  uint32_t m, n, k;       /* route plan: tokens, top_k, experts */
+  uint32_t m, n, k;       /* route plan and router balance: tokens, top_k,
+                             experts; LM-head loss: rows, vocabulary, hidden;
+                             adapter GEMM: rows, rank, k */
   uintptr_t bytes_u64;    /* host address the size is written to */
 } pih_amd_workspace_query_v1;
 
@@ -394,6 +409,141 @@ typedef struct pih_amd_v41_block_dequant_launch_v1 {
   uint32_t rows, columns, block, scale_storage;
 } pih_amd_v41_block_dequant_launch_v1;
 
+/* Low-rank adapters of many requests on top of a shared projection:
+ *   output[t, :] = bf16(base[t, :] + scale[a] * (input[t, :] . A[a]^T) . B[a]^T)
+ * for the rows of every segment: segment s is the rows
+ * segment_offsets[s] <= t < segment_offsets[s+1] (u32 [segments + 1],
+ * ascending; an empty segment is allowed) and has adapter a =
+ * segment_adapter[s] (u32 [segments]; 0xFFFFFFFF: none, output = base).
+ * Segments may share an adapter.  Rows outside every segment are neither
+ * read nor written.  A bf16 [adapters][rank][k], B bf16 [adapters][n][rank],
+ * scale f32 [adapters] (0: all 1).  base_bf16 may be the output itself (same
+ * stride) or 0 (the rows start from zero).  input, base and output rows are
+ * *_stride elements apart (k, n, n at least).
+ * rank a multiple of 8 up to 128; n, k and the strides multiples of 8; every
+ * address 16-byte aligned (the u32 and f32 arrays 4-byte).  The product with
+ * A is summed in fp32 and enters the second product as the sum of two bf16
+ * values (2^-16 relative), so the only rounding to bf16 is the output's.
+ * workspace: query_workspace(ADAPTER_GEMM, row_count, rank, k).
+ * Error bits: 1 an adapter id that is neither 0xFFFFFFFF nor below
+ * adapter_count (its rows are left unwritten), 2 offsets that descend or
+ * pass row_count (the segment is left out). */
+#define PIH_AMD_NO_ADAPTER_V1 0xFFFFFFFFU
+typedef struct pih_amd_adapter_gemm_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t input_bf16, a_bf16, b_bf16, scale_f32;
+  uintptr_t segment_offsets_u32, segment_adapter_u32;
+  uintptr_t base_bf16, output_bf16, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t row_count, segment_count, adapter_count, rank, n, k;
+  uint32_t input_stride, base_stride, output_stride;
+} pih_amd_adapter_gemm_launch_v1;
+
+/* Gradients of the above, for an upstream gradient dy of the output:
+ *   dx[t, :] = bf16(base[t, :] + scale[a] * (dy[t, :] . B[a]) . A[a])
+ *   da[a]    = scale[a] * sum over a's rows of (dy . B[a])^T . input
+ *   db[a]    = scale[a] * sum over a's rows of dy^T . (input . A[a]^T)
+ * base_bf16 (dx's own or 0) carries the shared projection's input gradient;
+ * da f32 [adapters][rank][k] and db f32 [adapters][n][rank] are written for
+ * every adapter, zero where it has no row.  dx rows outside every segment
+ * are left as they are.  Sums run in a fixed order: the same call gives the
+ * same bits.  Conditions, alignment and error bits are those of
+ * pih_amd_adapter_gemm_launch_v1.  query_adapter_backward_workspace writes
+ * the byte count that `workspace` needs (from row_count, segment_count,
+ * adapter_count, rank, n and k) to *required_bytes_u64, a host address. */
+typedef struct pih_amd_adapter_backward_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t output_grad_bf16, input_bf16, a_bf16, b_bf16, scale_f32;
+  uintptr_t segment_offsets_u32, segment_adapter_u32;
+  uintptr_t base_bf16, input_grad_bf16, a_grad_f32, b_grad_f32, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t required_bytes_u64;
+  uintptr_t error_flag_u32, stream;
+  uint32_t row_count, segment_count, adapter_count, rank, n, k;
+  uint32_t output_grad_stride, input_stride, base_stride, input_grad_stride;
+} pih_amd_adapter_backward_launch_v1;
+
+/* Softmax cross entropy of an LM head in pieces of the vocabulary, whose
+ * logits are never stored:
+ *   lse[t]  = log(sum over v of exp(input[t, :] . weight[v, :]))
+ *   loss[t] = lse[t] - input[t, :] . weight[target[t], :]
+ * input bf16 [rows][hidden], weight bf16 [vocab][hidden], target u32 [rows]
+ * (0xFFFFFFFF: the row has none, loss 0), loss f32 [rows], lse f32 [rows].
+ * -loss is the target's log-probability.  Logits, maxima and sums are fp32.
+ * hidden a multiple of 8, addresses 16-byte aligned (target, loss and lse
+ * 4-byte).  workspace: query_workspace(LM_HEAD_LOSS, rows, vocab, hidden).
+ * Error bits: 1 a target that is neither 0xFFFFFFFF nor below vocab (the row
+ * counts as one without), 4 a non-finite loss (stored). */
+#define PIH_AMD_NO_TARGET_V1 0xFFFFFFFFU
+typedef struct pih_amd_lm_head_loss_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t input_bf16, weight_bf16, target_u32;
+  uintptr_t loss_f32, lse_f32, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t rows, vocab, hidden;
+} pih_amd_lm_head_loss_launch_v1;
+
+/* Gradients of the above from lse (as launch_lm_head_loss wrote it) and the
+ * losses' upstream gradient f32 [rows]: with
+ *   g[t, v] = loss_grad[t] * (exp(logit[t, v] - lse[t]) - [v == target[t]])
+ * rounded to bf16 as the operand of both products,
+ *   input_grad  bf16 [rows][hidden]  = g . weight
+ *   weight_grad bf16 [vocab][hidden] = g^T . input   (address 0: left out)
+ * summed in fp32.  A row without a target gives zeros, whatever its input,
+ * lse and loss_grad hold.  Conditions are those of
+ * pih_amd_lm_head_loss_launch_v1; workspace:
+ * query_workspace(LM_HEAD_LOSS_BACKWARD, rows, vocab, hidden).
+ * Error bit 1 as above. */
+typedef struct pih_amd_lm_head_loss_backward_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t input_bf16, weight_bf16, target_u32, lse_f32, loss_grad_f32;
+  uintptr_t input_grad_bf16, weight_grad_bf16, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t rows, vocab, hidden;
+} pih_amd_lm_head_loss_backward_launch_v1;
+
+/* Balance loss of a router and its experts' route counts: with p[t, e] the
+ * row's affinities normalised to 1 (mode SOFTMAX: softmax of the scores;
+ * SQRT_SOFTPLUS: sqrt(softplus(score)) over its sum),
+ *   counts[e]        = routes of topk_ids that go to e          u32 [E]
+ *   mean_affinity[e] = 1/T sum over t of p[t, e]                f32 [E]
+ *   loss             = coefficient * E / (T * top_k) *
+ *                      sum over e of counts[e] * mean_affinity[e]   f32 [1]
+ * scores f32 [T, E], topk_ids u32 [T, top_k] (as launch_router_topk reads
+ * and writes them); limits as there.  Error bits: 1 a non-finite score (the
+ * row adds nothing to mean_affinity; its routes count), 2 an id >= E (not
+ * counted), 4 a row whose affinities sum to 0 (adds nothing).
+ * workspace: query_workspace(ROUTER_BALANCE, T, top_k, E). */
+typedef struct pih_amd_router_balance_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t scores_f32, topk_ids_u32;
+  uintptr_t loss_f32, counts_u32, mean_affinity_f32, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t token_count, expert_count, top_k, mode;
+  float coefficient;
+} pih_amd_router_balance_launch_v1;
+
+/* Gradient of the scores behind the balance loss (upstream loss_grad f32
+ * [1], 0: none; counts as launch_router_balance wrote them) and behind the
+ * weights of launch_router_topk (upstream topk_weights_grad f32 [T, top_k],
+ * 0: none; topk_ids as that entry wrote them, route_scale as it was given):
+ * scores_grad f32 [T, E], the sum of both.  The counts and the selection are
+ * constants of the differentiation.  A row with error bit 1 or 4 gets zeros,
+ * a route with error bit 2 (or an id a second time) adds its own term alone
+ * or none. */
+typedef struct pih_amd_router_backward_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t scores_f32, topk_ids_u32, counts_u32, loss_grad_f32;
+  uintptr_t topk_weights_grad_f32, scores_grad_f32;
+  uintptr_t error_flag_u32, stream;
+  uint32_t token_count, expert_count, top_k, mode;
+  float coefficient, route_scale;
+} pih_amd_router_backward_launch_v1;
+
 typedef struct pih_amd_linear_kernels_api_v1 {
   uint32_t struct_size;
   uint32_t contract_version;
@@ -436,6 +586,15 @@ typedef struct pih_amd_linear_kernels_api_v1 {
   pih_status_v1 (*launch_v41_linear)(const pih_amd_v41_linear_launch_v1*);
   pih_status_v1 (*launch_v41_fp4_to_fp8)(const pih_amd_v41_fp4_to_fp8_launch_v1*);
   pih_status_v1 (*launch_v41_block_dequant)(const pih_amd_v41_block_dequant_launch_v1*);
+  /* Adapters, LM-head loss and router balance with their gradients (the six
+   * structs above; no counterpart in the reference). */
+  pih_status_v1 (*launch_adapter_gemm)(const pih_amd_adapter_gemm_launch_v1*);
+  pih_status_v1 (*query_adapter_backward_workspace)(const pih_amd_adapter_backward_launch_v1*);
+  pih_status_v1 (*launch_adapter_backward)(const pih_amd_adapter_backward_launch_v1*);
+  pih_status_v1 (*launch_lm_head_loss)(const pih_amd_lm_head_loss_launch_v1*);
+  pih_status_v1 (*launch_lm_head_loss_backward)(const pih_amd_lm_head_loss_backward_launch_v1*);
+  pih_status_v1 (*launch_router_balance)(const pih_amd_router_balance_launch_v1*);
+  pih_status_v1 (*launch_router_backward)(const pih_amd_router_backward_launch_v1*);
 } pih_amd_linear_kernels_api_v1;
 
 #define PIH_AMD_ROUTE_PLAN_NOALLOC_MAX_SCRATCH_V1 (1ULL << 20)

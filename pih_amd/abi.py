@@ -239,6 +239,33 @@ LN["moe_layer"] = _struct("MoeLayer", _hdr(*_u("input_bf16", "topk_ids_u32", "to
                                           *_i("token_count", "top_k", "expert_count", "hidden_size",
                                               "intermediate_size", "weight_format", "scale_format",
                                               "activation_type"), ("swiglu_limit", F32)))
+LN["adapter_gemm"] = _struct("AdapterGemm", _hdr(
+    *_u("input_bf16", "a_bf16", "b_bf16", "scale_f32", "segment_offsets_u32", "segment_adapter_u32", "base_bf16",
+        "output_bf16", "workspace"), ("workspace_bytes", U64), *_u("error_flag_u32", "stream"),
+    *_i("row_count", "segment_count", "adapter_count", "rank", "n", "k", "input_stride", "base_stride",
+        "output_stride")))
+LN["adapter_backward"] = _struct("AdapterBackward", _hdr(
+    *_u("output_grad_bf16", "input_bf16", "a_bf16", "b_bf16", "scale_f32", "segment_offsets_u32",
+        "segment_adapter_u32", "base_bf16", "input_grad_bf16", "a_grad_f32", "b_grad_f32", "workspace"),
+    ("workspace_bytes", U64), *_u("required_bytes_u64", "error_flag_u32", "stream"),
+    *_i("row_count", "segment_count", "adapter_count", "rank", "n", "k", "output_grad_stride", "input_stride",
+        "base_stride", "input_grad_stride")))
+LN["lm_head_loss"] = _struct("LmHeadLoss", _hdr(
+    *_u("input_bf16", "weight_bf16", "target_u32", "loss_f32", "lse_f32", "workspace"), ("workspace_bytes", U64),
+    *_u("error_flag_u32", "stream"), *_i("rows", "vocab", "hidden")))
+LN["lm_head_loss_backward"] = _struct("LmHeadLossBackward", _hdr(
+    *_u("input_bf16", "weight_bf16", "target_u32", "lse_f32", "loss_grad_f32", "input_grad_bf16",
+        "weight_grad_bf16", "workspace"), ("workspace_bytes", U64), *_u("error_flag_u32", "stream"),
+    *_i("rows", "vocab", "hidden")))
+LN["router_balance"] = _struct("RouterBalance", _hdr(
+    *_u("scores_f32", "topk_ids_u32", "loss_f32", "counts_u32", "mean_affinity_f32", "workspace"),
+    ("workspace_bytes", U64), *_u("error_flag_u32", "stream"), *_i("token_count", "expert_count", "top_k", "mode"),
+    ("coefficient", F32)))
+LN["router_backward"] = _struct("RouterBackward", _hdr(
+    *_u("scores_f32", "topk_ids_u32", "counts_u32", "loss_grad_f32", "topk_weights_grad_f32", "scores_grad_f32",
+        "error_flag_u32", "stream"), *_i("token_count", "expert_count", "top_k", "mode"), ("coefficient", F32),
+    ("route_scale", F32)))
+NO_ADAPTER = NO_TARGET = 0xFFFFFFFF
 WEIGHT_FP8, WEIGHT_MXFP4 = 1, 2
 # pih_amd_w4a16_problem_v1: one entry of the grouped launch's host array
 W4A16_PROBLEM = _struct("W4a16Problem", _u("input_bf16", "qweight", "scales", "zeros", "output_bf16") +
@@ -253,7 +280,11 @@ LN_ORDER = [("query_workspace", "workspace_query"), ("launch_route_plan", "route
             ("launch_w4a16_grouped", "w4a16_grouped"), ("query_moe_layer_workspace", "moe_layer"),
             ("launch_moe_layer", "moe_layer"), ("launch_route_plan_noalloc", "route_plan"),
             ("launch_router_topk", "router_topk"), ("launch_v41_linear", "v41_linear"),
-            ("launch_v41_fp4_to_fp8", "v41_fp4_to_fp8"), ("launch_v41_block_dequant", "v41_block_dequant")]
+            ("launch_v41_fp4_to_fp8", "v41_fp4_to_fp8"), ("launch_v41_block_dequant", "v41_block_dequant"),
+            ("launch_adapter_gemm", "adapter_gemm"), ("query_adapter_backward_workspace", "adapter_backward"),
+            ("launch_adapter_backward", "adapter_backward"),
+            ("launch_lm_head_loss", "lm_head_loss"), ("launch_lm_head_loss_backward", "lm_head_loss_backward"),
+            ("launch_router_balance", "router_balance"), ("launch_router_backward", "router_backward")]
 LN_API = _struct("AmdLinearKernelsApi", [("struct_size", U32), ("contract_version", U32),
                                          ("identity", C.POINTER(Identity))] +
                  [(f, C.CFUNCTYPE(Status, C.POINTER(LN[s]))) for f, s in LN_ORDER])
@@ -320,6 +351,7 @@ OUTPUT_BF16, OUTPUT_F32, OUTPUT_SWIGLU_BF16, OUTPUT_SWIGLU_E4M3 = 1, 2, 3, 4
 ACTIVATION_E4M3, ACTIVATION_BF16 = 1, 2
 W4A16_SYMMETRIC, W4A16_ASYMMETRIC = 1, 2
 WORKSPACE_ROUTE_PLAN, WORKSPACE_BF16_GEMM, WORKSPACE_W4A16 = 1, 2, 3
+WORKSPACE_ADAPTER_GEMM, WORKSPACE_LM_HEAD_LOSS, WORKSPACE_LM_HEAD_LOSS_BACKWARD, WORKSPACE_ROUTER_BALANCE = 4, 5, 6, 7
 ROUTER_SOFTMAX, ROUTER_SQRT_SOFTPLUS = 1, 2
 
 

@@ -283,6 +283,89 @@ struct RouterTopkArgs {
 };
 St LaunchRouterTopk(const RouterTopkArgs& a);
 
+// Balance loss and route counts, and the scores' gradient (router_balance.hip)
+struct RouterBalanceArgs {
+  const float* scores = nullptr;       // [tokens, experts]
+  const uint32_t* ids = nullptr;       // [tokens, topk]
+  float* loss = nullptr;               // [1]
+  uint32_t* counts = nullptr;          // [experts]
+  float* mean = nullptr;               // [experts]
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  uint32_t* error_flag = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t tokens = 0, experts = 0, topk = 0;
+  uint32_t mode = kRouterSoftmax;
+  float coefficient = 0.0f;
+};
+St LaunchRouterBalance(const RouterBalanceArgs& a);
+uint64_t RouterBalanceWorkspaceBytes(uint32_t tokens, uint32_t topk, uint32_t experts);
+struct RouterBackwardArgs {
+  const float* scores = nullptr;
+  const uint32_t* ids = nullptr;
+  const uint32_t* counts = nullptr;      // [experts] with loss_grad
+  const float* loss_grad = nullptr;      // [1] (nullptr: none)
+  const float* weights_grad = nullptr;   // [tokens, topk] (nullptr: none)
+  float* scores_grad = nullptr;          // [tokens, experts]
+  uint32_t* error_flag = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t tokens = 0, experts = 0, topk = 0;
+  uint32_t mode = kRouterSoftmax;
+  float coefficient = 0.0f, scale = 1.0f;
+};
+St LaunchRouterBackward(const RouterBackwardArgs& a);
+
+// ------------------------------------------------- low-rank adapters
+// (adapter.hip) out rows = base + scale[a] (in . A[a]^T) . B[a]^T over
+// segments of rows, and the gradients
+struct AdapterArgs {
+  const uint16_t* x = nullptr;         // [rows, k]
+  const uint16_t* a = nullptr;         // [adapters, rank, k]
+  const uint16_t* b = nullptr;         // [adapters, n, rank]
+  const float* scale = nullptr;        // [adapters] (nullptr: 1)
+  const uint32_t* offsets = nullptr;   // [segments + 1]
+  const uint32_t* adapter = nullptr;   // [segments]
+  const uint16_t* base = nullptr;      // [rows, n], backward [rows, k] (nullptr: 0)
+  uint16_t* out = nullptr;             // [rows, n], backward the input's gradient [rows, k]
+  const uint16_t* dy = nullptr;        // backward: [rows, n]
+  float* da = nullptr;                 // backward: [adapters, rank, k]
+  float* db = nullptr;                 // backward: [adapters, n, rank]
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  uint32_t* error_flag = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t rows = 0, segments = 0, adapters = 0, rank = 0, n = 0, k = 0;
+  uint32_t x_stride = 0, base_stride = 0, out_stride = 0, dy_stride = 0;
+};
+St LaunchAdapterGemm(const AdapterArgs& a);
+St LaunchAdapterBackward(const AdapterArgs& a);
+uint64_t AdapterGemmWorkspaceBytes(uint32_t rows, uint32_t rank, uint32_t k);
+// 0 for a shape that the launcher refuses
+uint64_t AdapterBackwardWorkspaceBytes(const AdapterArgs& a);
+
+// ------------------------------------------------- LM-head cross entropy
+// (lm_head_loss.hip)
+struct LmHeadLossArgs {
+  const uint16_t* x = nullptr;         // [rows, hidden]
+  const uint16_t* w = nullptr;         // [vocab, hidden]
+  const uint32_t* target = nullptr;    // [rows], 0xffffffff: none
+  float* loss = nullptr;               // forward: [rows]
+  float* lse = nullptr;                // forward: written; backward: read
+  const float* loss_grad = nullptr;    // backward: [rows]
+  uint16_t* dx = nullptr;              // backward: [rows, hidden]
+  uint16_t* dw = nullptr;              // backward: [vocab, hidden] (nullptr: left out)
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  uint32_t* error_flag = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t rows = 0, vocab = 0, hidden = 0;
+};
+St LaunchLmHeadLoss(const LmHeadLossArgs& a);
+St LaunchLmHeadLossBackward(const LmHeadLossArgs& a);
+// 0 for a shape that the launcher refuses
+uint64_t LmHeadLossWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden);
+uint64_t LmHeadLossBackwardWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden);
+
 // --------------------------------------------------------------- MoE glue
 struct RoutePlanArgs {
   const uint32_t* topk_ids = nullptr;     // [tokens, topk]

@@ -40,6 +40,22 @@ St QueryWorkspace(const pih_amd_workspace_query_v1* r) {
     case PIH_AMD_WORKSPACE_W4A16_V1:
       bytes = W4a16WorkspaceBytes(r->m, r->n, r->k);
       break;
+    case PIH_AMD_WORKSPACE_ADAPTER_GEMM_V1:
+      bytes = AdapterGemmWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_LM_HEAD_LOSS_V1:
+      bytes = LmHeadLossWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_LM_HEAD_LOSS_BACKWARD_V1:
+      bytes = LmHeadLossBackwardWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_ROUTER_BALANCE_V1:
+      bytes = RouterBalanceWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
     default:
       return Invalid("workspace_query_kind_invalid");
   }
@@ -472,6 +488,154 @@ St W4a16Dequant(const pih_amd_w4a16_dequant_launch_v1* r) {
   return LaunchW4a16Dequant(a, Ptr<float>(r->output_f32));
 }
 
+St AdapterGemm(const pih_amd_adapter_gemm_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("adapter_gemm_request_invalid");
+  AdapterArgs a;
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.a = Ptr<const uint16_t>(r->a_bf16);
+  a.b = Ptr<const uint16_t>(r->b_bf16);
+  a.scale = Ptr<const float>(r->scale_f32);
+  a.offsets = Ptr<const uint32_t>(r->segment_offsets_u32);
+  a.adapter = Ptr<const uint32_t>(r->segment_adapter_u32);
+  a.base = Ptr<const uint16_t>(r->base_bf16);
+  a.out = Ptr<uint16_t>(r->output_bf16);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.rows = r->row_count;
+  a.segments = r->segment_count;
+  a.adapters = r->adapter_count;
+  a.rank = r->rank;
+  a.n = r->n;
+  a.k = r->k;
+  a.x_stride = r->input_stride;
+  a.base_stride = r->base_stride;
+  a.out_stride = r->output_stride;
+  return LaunchAdapterGemm(a);
+}
+
+AdapterArgs AdapterBackwardArgs(const pih_amd_adapter_backward_launch_v1* r) {
+  AdapterArgs a;
+  a.dy = Ptr<const uint16_t>(r->output_grad_bf16);
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.a = Ptr<const uint16_t>(r->a_bf16);
+  a.b = Ptr<const uint16_t>(r->b_bf16);
+  a.scale = Ptr<const float>(r->scale_f32);
+  a.offsets = Ptr<const uint32_t>(r->segment_offsets_u32);
+  a.adapter = Ptr<const uint32_t>(r->segment_adapter_u32);
+  a.base = Ptr<const uint16_t>(r->base_bf16);
+  a.out = Ptr<uint16_t>(r->input_grad_bf16);
+  a.da = Ptr<float>(r->a_grad_f32);
+  a.db = Ptr<float>(r->b_grad_f32);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.rows = r->row_count;
+  a.segments = r->segment_count;
+  a.adapters = r->adapter_count;
+  a.rank = r->rank;
+  a.n = r->n;
+  a.k = r->k;
+  a.dy_stride = r->output_grad_stride;
+  a.x_stride = r->input_stride;
+  a.base_stride = r->base_stride;
+  a.out_stride = r->input_grad_stride;
+  return a;
+}
+
+St QueryAdapterBackward(const pih_amd_adapter_backward_launch_v1* r) {
+  if (!HeaderOk(r, kAbi) || !r->required_bytes_u64) return Invalid("adapter_backward_query_invalid");
+  const uint64_t bytes = AdapterBackwardWorkspaceBytes(AdapterBackwardArgs(r));
+  if (bytes == 0) return Invalid("adapter_backward_shape_invalid");
+  *Ptr<uint64_t>(r->required_bytes_u64) = bytes;
+  return Ok();
+}
+
+St AdapterBackward(const pih_amd_adapter_backward_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("adapter_backward_request_invalid");
+  return LaunchAdapterBackward(AdapterBackwardArgs(r));
+}
+
+St LmHeadLoss(const pih_amd_lm_head_loss_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("lm_head_loss_request_invalid");
+  LmHeadLossArgs a;
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.w = Ptr<const uint16_t>(r->weight_bf16);
+  a.target = Ptr<const uint32_t>(r->target_u32);
+  a.loss = Ptr<float>(r->loss_f32);
+  a.lse = Ptr<float>(r->lse_f32);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.rows = r->rows;
+  a.vocab = r->vocab;
+  a.hidden = r->hidden;
+  return LaunchLmHeadLoss(a);
+}
+
+St LmHeadLossBackward(const pih_amd_lm_head_loss_backward_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("lm_head_loss_backward_request_invalid");
+  LmHeadLossArgs a;
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.w = Ptr<const uint16_t>(r->weight_bf16);
+  a.target = Ptr<const uint32_t>(r->target_u32);
+  a.lse = Ptr<float>(r->lse_f32);
+  a.loss_grad = Ptr<const float>(r->loss_grad_f32);
+  a.dx = Ptr<uint16_t>(r->input_grad_bf16);
+  a.dw = Ptr<uint16_t>(r->weight_grad_bf16);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.rows = r->rows;
+  a.vocab = r->vocab;
+  a.hidden = r->hidden;
+  return LaunchLmHeadLossBackward(a);
+}
+
+St RouterBalance(const pih_amd_router_balance_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("router_balance_request_invalid");
+  RouterBalanceArgs a;
+  a.scores = Ptr<const float>(r->scores_f32);
+  a.ids = Ptr<const uint32_t>(r->topk_ids_u32);
+  a.loss = Ptr<float>(r->loss_f32);
+  a.counts = Ptr<uint32_t>(r->counts_u32);
+  a.mean = Ptr<float>(r->mean_affinity_f32);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.tokens = r->token_count;
+  a.experts = r->expert_count;
+  a.topk = r->top_k;
+  a.mode = r->mode;
+  a.coefficient = r->coefficient;
+  return LaunchRouterBalance(a);
+}
+
+St RouterBackward(const pih_amd_router_backward_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("router_backward_request_invalid");
+  RouterBackwardArgs a;
+  a.scores = Ptr<const float>(r->scores_f32);
+  a.ids = Ptr<const uint32_t>(r->topk_ids_u32);
+  a.counts = Ptr<const uint32_t>(r->counts_u32);
+  a.loss_grad = Ptr<const float>(r->loss_grad_f32);
+  a.weights_grad = Ptr<const float>(r->topk_weights_grad_f32);
+  a.scores_grad = Ptr<float>(r->scores_grad_f32);
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.tokens = r->token_count;
+  a.experts = r->expert_count;
+  a.topk = r->top_k;
+  a.mode = r->mode;
+  a.coefficient = r->coefficient;
+  a.scale = r->route_scale;
+  return LaunchRouterBackward(a);
+}
+
 PIH_AMD_CONTAINED(CQueryWorkspace, QueryWorkspace, pih_amd_workspace_query_v1)
 PIH_AMD_CONTAINED(CRoutePlan, RoutePlan, pih_amd_route_plan_launch_v1)
 PIH_AMD_CONTAINED(CFp8Quant, Fp8Quant, pih_amd_fp8_quant_launch_v1)
@@ -493,12 +657,21 @@ PIH_AMD_CONTAINED(CRouterTopk, RouterTopk, pih_amd_router_topk_launch_v1)
 PIH_AMD_CONTAINED(CV41Linear, V41Linear, pih_amd_v41_linear_launch_v1)
 PIH_AMD_CONTAINED(CV41Fp4ToFp8, V41Fp4ToFp8, pih_amd_v41_fp4_to_fp8_launch_v1)
 PIH_AMD_CONTAINED(CV41BlockDequant, V41BlockDequant, pih_amd_v41_block_dequant_launch_v1)
+PIH_AMD_CONTAINED(CAdapterGemm, AdapterGemm, pih_amd_adapter_gemm_launch_v1)
+PIH_AMD_CONTAINED(CQueryAdapterBackward, QueryAdapterBackward, pih_amd_adapter_backward_launch_v1)
+PIH_AMD_CONTAINED(CAdapterBackward, AdapterBackward, pih_amd_adapter_backward_launch_v1)
+PIH_AMD_CONTAINED(CLmHeadLoss, LmHeadLoss, pih_amd_lm_head_loss_launch_v1)
+PIH_AMD_CONTAINED(CLmHeadLossBackward, LmHeadLossBackward, pih_amd_lm_head_loss_backward_launch_v1)
+PIH_AMD_CONTAINED(CRouterBalance, RouterBalance, pih_amd_router_balance_launch_v1)
+PIH_AMD_CONTAINED(CRouterBackward, RouterBackward, pih_amd_router_backward_launch_v1)
 
 const pih_amd_linear_kernels_api_v1 kContract = {
     sizeof(pih_amd_linear_kernels_api_v1), kAbi, &kIdentity, &CQueryWorkspace, &CRoutePlan,
     &CFp8Quant, &CFp8Gemm, &CMoeFp8Gemm, &CMoeMxfp4Gemm, &CMoeCombine, &CBf16Gemm, &CW4a16,
     &CSiluMul, &CSwiGlu, &CMxfp4Decode, &CW4a16Dequant, &CW4a16Grouped, &CQueryMoeLayer, &CMoeLayer,
-    &CRoutePlanNoAlloc, &CRouterTopk, &CV41Linear, &CV41Fp4ToFp8, &CV41BlockDequant};
+    &CRoutePlanNoAlloc, &CRouterTopk, &CV41Linear, &CV41Fp4ToFp8, &CV41BlockDequant,
+    &CAdapterGemm, &CQueryAdapterBackward, &CAdapterBackward, &CLmHeadLoss, &CLmHeadLossBackward, &CRouterBalance,
+    &CRouterBackward};
 
 pih_status_v1 BindOrigin(const char* path) noexcept {
   return ToAbi(path && path[0] == '/' ? Ok() : Invalid("bind_origin_path_not_absolute"));

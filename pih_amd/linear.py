@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import abi
-from .device import error_flag, ptr, stream_handle
+from .device import error_flag, ptr, rows_ptr, same_device, stream_handle
 
 
 class KernelError(RuntimeError):
@@ -493,3 +493,202 @@ def v41_block_dequant(source: torch.Tensor, scales: torch.Tensor, block: int, ou
                     scale_storage=storage)
     _check(_ln().call("launch_v41_block_dequant", r), "v41_block_dequant")
     return out, flag
+
+
+# ------------------------------------ adapters, LM-head loss, router balance
+def _workspace(kind: int, m: int, n: int, k: int, device) -> torch.Tensor:
+    out = abi.C.c_uint64()
+    q = abi.request(abi.LN["workspace_query"], kind=kind, m=m, n=n, k=k, bytes_u64=abi.C.addressof(out))
+    _check(_ln().call("query_workspace", q), "query_workspace")
+    return torch.empty(out.value, dtype=torch.uint8, device=device)
+
+
+def _want(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(f"pih_amd: {what}")
+
+
+def _adapter_stacks(a, b, scale, offsets, adapters):
+    _want(a.dim() == 3 and b.dim() == 3 and a.shape[0] == b.shape[0] and a.shape[1] == b.shape[2],
+          "adapter stacks are A [adapters, rank, k] and B [adapters, n, rank]")
+    _want(a.dtype == b.dtype == torch.bfloat16, "adapter stacks are bfloat16")
+    _want(scale is None or (scale.dtype == torch.float32 and scale.shape == a.shape[:1]),
+          "adapter scales are float32 [adapters]")
+    _want(offsets.dtype == adapters.dtype == torch.int32 and adapters.dim() == 1 and
+          offsets.shape == (adapters.shape[0] + 1,),
+          "segment offsets are int32 [segments + 1], segment adapters int32 [segments]")
+    return a.shape[0], a.shape[1], b.shape[1], a.shape[2]
+
+
+def _rows(t, rows: int, cols: int, what: str) -> int:
+    _want(tuple(t.shape) == (rows, cols) and t.dtype == torch.bfloat16, f"{what} is bfloat16 [{rows}, {cols}]")
+    return t.stride(0) if rows > 1 else cols
+
+
+def adapter_gemm(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: Optional[torch.Tensor],
+                 offsets: torch.Tensor, adapters: torch.Tensor, base: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, flag: Optional[torch.Tensor] = None):
+    """Low-rank adapters of many requests on top of a shared projection's
+    output (``launch_adapter_gemm``): ``out[t] = base[t] + scale[i] *
+    (x[t] . a[i]^T) . b[i]^T`` for the rows ``offsets[s] <= t <
+    offsets[s + 1]`` of every segment ``s``, whose adapter is ``i =
+    adapters[s]`` (-1: none).  ``x`` [rows, k], ``base`` and ``out``
+    [rows, n] may be column slices of wider tensors; ``out`` may be ``base``
+    itself; ``base`` None starts from zero.  Rows outside every segment are
+    left as they are.  Returns (out, flag)."""
+    count, rank, n, k = _adapter_stacks(a, b, scale, offsets, adapters)
+    rows = x.shape[0]
+    xs = _rows(x, rows, k, "the adapters' input")
+    bs = 0 if base is None else _rows(base, rows, n, "the adapters' base")
+    if out is None:
+        out = torch.empty(rows, n, dtype=torch.bfloat16, device=x.device)
+    os = _rows(out, rows, n, "the adapters' output")
+    flag = error_flag() if flag is None else flag
+    same_device(x, a, b, scale, offsets, adapters, base, out, flag)
+    ws = _workspace(abi.WORKSPACE_ADAPTER_GEMM, rows, rank, k, x.device)
+    r = abi.request(abi.LN["adapter_gemm"], input_bf16=rows_ptr(x), a_bf16=ptr(a), b_bf16=ptr(b),
+                    scale_f32=ptr(scale), segment_offsets_u32=ptr(offsets), segment_adapter_u32=ptr(adapters),
+                    base_bf16=rows_ptr(base), output_bf16=rows_ptr(out), workspace=ptr(ws),
+                    workspace_bytes=ws.numel(), error_flag_u32=ptr(flag), stream=stream_handle(), row_count=rows,
+                    segment_count=adapters.shape[0], adapter_count=count, rank=rank, n=n, k=k, input_stride=xs,
+                    base_stride=bs, output_stride=os)
+    _check(_ln().call("launch_adapter_gemm", r), "adapter_gemm")
+    return out, flag
+
+
+def adapter_backward(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                     scale: Optional[torch.Tensor], offsets: torch.Tensor, adapters: torch.Tensor,
+                     base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                     flag: Optional[torch.Tensor] = None):
+    """Gradients of ``adapter_gemm`` for the upstream gradient ``dy`` [rows,
+    n] (``launch_adapter_backward``): (dx bf16 [rows, k], da f32 like ``a``,
+    db f32 like ``b``, flag).  ``base`` is the shared projection's gradient of
+    x, on top of which dx comes (``out`` may be ``base`` itself).  Segments
+    that share an adapter add up; an adapter without rows has zeros."""
+    count, rank, n, k = _adapter_stacks(a, b, scale, offsets, adapters)
+    rows = x.shape[0]
+    ys, xs = _rows(dy, rows, n, "the upstream gradient"), _rows(x, rows, k, "the adapters' input")
+    bs = 0 if base is None else _rows(base, rows, k, "the gradient's base")
+    if out is None:
+        out = torch.empty(rows, k, dtype=torch.bfloat16, device=x.device)
+    os = _rows(out, rows, k, "the input's gradient")
+    da = torch.empty(a.shape, dtype=torch.float32, device=x.device)
+    db = torch.empty(b.shape, dtype=torch.float32, device=x.device)
+    flag = error_flag() if flag is None else flag
+    same_device(dy, x, a, b, scale, offsets, adapters, base, out, flag)
+    need = abi.C.c_uint64()
+    r = abi.request(abi.LN["adapter_backward"], output_grad_bf16=rows_ptr(dy), input_bf16=rows_ptr(x), a_bf16=ptr(a),
+                    b_bf16=ptr(b), scale_f32=ptr(scale), segment_offsets_u32=ptr(offsets),
+                    segment_adapter_u32=ptr(adapters), base_bf16=rows_ptr(base), input_grad_bf16=rows_ptr(out),
+                    a_grad_f32=ptr(da), b_grad_f32=ptr(db), required_bytes_u64=abi.C.addressof(need),
+                    error_flag_u32=ptr(flag), stream=stream_handle(), row_count=rows,
+                    segment_count=adapters.shape[0], adapter_count=count, rank=rank, n=n, k=k,
+                    output_grad_stride=ys, input_stride=xs, base_stride=bs, input_grad_stride=os)
+    _check(_ln().call("query_adapter_backward_workspace", r), "query_adapter_backward_workspace")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+    r.workspace, r.workspace_bytes = ptr(ws), ws.numel()
+    _check(_ln().call("launch_adapter_backward", r), "adapter_backward")
+    return out, da, db, flag
+
+
+def _loss_inputs(x, weight, targets):
+    _want(x.dim() == 2 and weight.dim() == 2 and x.shape[1] == weight.shape[1] and
+          x.dtype == weight.dtype == torch.bfloat16, "the LM head is x [rows, hidden] . weight [vocab, hidden], bfloat16")
+    _want(targets.dtype == torch.int32 and targets.shape == x.shape[:1], "targets are int32 [rows]")
+    return x.shape[0], weight.shape[0], x.shape[1]
+
+
+def lm_head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                 flag: Optional[torch.Tensor] = None):
+    """Softmax cross entropy of an LM head without its logits
+    (``launch_lm_head_loss``): (loss f32 [rows], lse f32 [rows], flag) with
+    ``lse`` the log-sum-exp of a row's logits and ``-loss`` the target's
+    log-probability.  A target of -1 is none: loss 0."""
+    rows, vocab, hidden = _loss_inputs(x, weight, targets)
+    loss = torch.empty(rows, dtype=torch.float32, device=x.device)
+    lse = torch.empty(rows, dtype=torch.float32, device=x.device)
+    flag = error_flag() if flag is None else flag
+    same_device(x, weight, targets, flag)
+    ws = _workspace(abi.WORKSPACE_LM_HEAD_LOSS, rows, vocab, hidden, x.device)
+    r = abi.request(abi.LN["lm_head_loss"], input_bf16=ptr(x), weight_bf16=ptr(weight), target_u32=ptr(targets),
+                    loss_f32=ptr(loss), lse_f32=ptr(lse), workspace=ptr(ws), workspace_bytes=ws.numel(),
+                    error_flag_u32=ptr(flag), stream=stream_handle(), rows=rows, vocab=vocab, hidden=hidden)
+    _check(_ln().call("launch_lm_head_loss", r), "lm_head_loss")
+    return loss, lse, flag
+
+
+def lm_head_loss_backward(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
+                          dloss: torch.Tensor, weight_gradient: bool = True, flag: Optional[torch.Tensor] = None):
+    """Gradients of ``lm_head_loss`` for the losses' upstream gradient
+    ``dloss`` f32 [rows] (``launch_lm_head_loss_backward``): (dx bf16 like
+    ``x``, dweight bf16 like ``weight``, or None without
+    ``weight_gradient``, flag)."""
+    rows, vocab, hidden = _loss_inputs(x, weight, targets)
+    _want(lse.dtype == dloss.dtype == torch.float32 and lse.shape == dloss.shape == x.shape[:1],
+          "lse and dloss are float32 [rows]")
+    dx = torch.empty_like(x)
+    dw = torch.empty_like(weight) if weight_gradient else None
+    flag = error_flag() if flag is None else flag
+    same_device(x, weight, targets, lse, dloss, flag)
+    ws = _workspace(abi.WORKSPACE_LM_HEAD_LOSS_BACKWARD, rows, vocab, hidden, x.device)
+    r = abi.request(abi.LN["lm_head_loss_backward"], input_bf16=ptr(x), weight_bf16=ptr(weight),
+                    target_u32=ptr(targets), lse_f32=ptr(lse), loss_grad_f32=ptr(dloss), input_grad_bf16=ptr(dx),
+                    weight_grad_bf16=ptr(dw), workspace=ptr(ws), workspace_bytes=ws.numel(), error_flag_u32=ptr(flag),
+                    stream=stream_handle(), rows=rows, vocab=vocab, hidden=hidden)
+    _check(_ln().call("launch_lm_head_loss_backward", r), "lm_head_loss_backward")
+    return dx, dw, flag
+
+
+def _router_inputs(scores, topk_ids):
+    _want(scores.dim() == 2 and scores.dtype == torch.float32, "router scores are float32 [tokens, experts]")
+    _want(topk_ids.dim() == 2 and topk_ids.dtype == torch.int32 and topk_ids.shape[0] == scores.shape[0],
+          "expert ids are int32 [tokens, top_k]")
+    return scores.shape[0], scores.shape[1], topk_ids.shape[1]
+
+
+def router_balance(scores: torch.Tensor, topk_ids: torch.Tensor, mode: int, coefficient: float,
+                   flag: Optional[torch.Tensor] = None):
+    """A router's balance loss and its experts' load
+    (``launch_router_balance``): (loss f32 [1], counts int32 [experts], mean
+    affinity f32 [experts], flag) from the raw scores and the ids that
+    ``router_topk`` chose; ``mode`` as there."""
+    tokens, experts, topk = _router_inputs(scores, topk_ids)
+    dev = scores.device
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    counts = torch.empty(experts, dtype=torch.int32, device=dev)
+    mean = torch.empty(experts, dtype=torch.float32, device=dev)
+    flag = error_flag() if flag is None else flag
+    same_device(scores, topk_ids, flag)
+    ws = _workspace(abi.WORKSPACE_ROUTER_BALANCE, tokens, topk, experts, dev)
+    r = abi.request(abi.LN["router_balance"], scores_f32=ptr(scores), topk_ids_u32=ptr(topk_ids), loss_f32=ptr(loss),
+                    counts_u32=ptr(counts), mean_affinity_f32=ptr(mean), workspace=ptr(ws),
+                    workspace_bytes=ws.numel(), error_flag_u32=ptr(flag), stream=stream_handle(), token_count=tokens,
+                    expert_count=experts, top_k=topk, mode=mode, coefficient=coefficient)
+    _check(_ln().call("launch_router_balance", r), "router_balance")
+    return loss, counts, mean, flag
+
+
+def router_backward(scores: torch.Tensor, topk_ids: torch.Tensor, counts: Optional[torch.Tensor], mode: int,
+                    coefficient: float, dloss: Optional[torch.Tensor], dweights: Optional[torch.Tensor] = None,
+                    route_scale: float = 1.0, flag: Optional[torch.Tensor] = None):
+    """Gradient of the raw scores (``launch_router_backward``): (dscores f32
+    like ``scores``, flag), the sum of the balance loss's (``dloss`` f32 [1],
+    with ``counts`` of ``router_balance``) and the route weights'
+    (``dweights`` f32 [tokens, top_k], with ``router_topk``'s
+    ``route_scale``); either may be None."""
+    tokens, experts, topk = _router_inputs(scores, topk_ids)
+    _want(dloss is None or (dloss.dtype == torch.float32 and dloss.numel() == 1 and counts is not None and
+                            counts.dtype == torch.int32 and tuple(counts.shape) == (experts,)),
+          "dloss is float32 [1] and comes with counts int32 [experts]")
+    _want(dweights is None or (dweights.dtype == torch.float32 and dweights.shape == topk_ids.shape),
+          "dweights is float32 [tokens, top_k]")
+    dscores = torch.empty_like(scores)
+    flag = error_flag() if flag is None else flag
+    same_device(scores, topk_ids, counts, dloss, dweights, flag)
+    r = abi.request(abi.LN["router_backward"], scores_f32=ptr(scores), topk_ids_u32=ptr(topk_ids),
+                    counts_u32=ptr(counts), loss_grad_f32=ptr(dloss), topk_weights_grad_f32=ptr(dweights),
+                    scores_grad_f32=ptr(dscores), error_flag_u32=ptr(flag), stream=stream_handle(),
+                    token_count=tokens, expert_count=experts, top_k=topk, mode=mode, coefficient=coefficient,
+                    route_scale=route_scale)
+    _check(_ln().call("launch_router_backward", r), "router_backward")
+    return dscores, flag
