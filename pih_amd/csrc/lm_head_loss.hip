@@ -19,6 +19,7 @@
 // x of dw's product is a copy with those rows as zeros, so that nothing an
 // unused row holds (infinities, NaN) reaches dw.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "kernels.hpp"
@@ -155,6 +156,321 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
   }
 }
 
+// ------------------------------------------------ 256 x 256 tiles
+// C [m][n] = A . B^T for large products, four waves of 128 x 128 (one per
+// SIMD, 256 accumulator registers each).  A K step is 64 deep and moved into
+// LDS by DMA, two steps resident.  Two layouts of an operand:
+//   rows     [row][k] in memory: LDS rows of 128 bytes, 16-byte chunk c of row
+//            r in slot c ^ ((r >> 1) & 7); a fragment is one ds_read_b128
+//            (16 rows, one chunk each: all 64 banks once);
+//   columns  [k][row] in memory: LDS rows of 512 bytes (one k each), chunk c
+//            of k row r in slot c ^ 2 f(r), f(r) = (r & 3) + 4 (r >> 3 & 1); a
+//            fragment is two transposing reads (ds_read_b64_tr_b16: lane l of
+//            16 gives the address of 4 values of k row l / 4 and receives
+//            column l of the four rows), whose 8 k rows per half wave lie in
+//            different 32-byte slots.
+// The step's two 32-deep halves: while the MFMAs of the first run, the second
+// half's fragments are read; then one wait and one barrier (every wave has
+// read the step, and the next one has arrived), and while the MFMAs of the
+// second run, the next step's first fragments are read and the step after it
+// is sent for, into the buffer just freed.
+constexpr uint32_t TB = 256, KB = 64, kStageBytes = TB * KB * 2;  // one operand's step
+constexpr uint32_t kBigLds = 4 * kStageBytes;
+
+struct BigArgs {
+  const uint16_t* a;
+  const uint16_t* b;
+  uint32_t m, n, k;        // k a multiple of 64
+  uint32_t k_valid;        // columns layout of B: k rows that exist (the others repeat the last)
+  uint64_t lda, ldb;
+  void* out;
+  uint64_t ldo;
+  uint32_t m_tiles, n_tiles, splits;
+  uint64_t split_stride;   // kEpiAdd: elements between the splits' sums
+  const uint32_t* target;
+  const float* lse;
+  const float* up;
+  float2* stats;
+  float* target_logit;
+  uint32_t v0, vocab, first;
+};
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+
+__device__ __forceinline__ v4i join(v4s x, v4s y) {
+  const uint2 a = __builtin_bit_cast(uint2, x), b = __builtin_bit_cast(uint2, y);
+  return v4i{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
+}
+
+template <bool AT, bool BT, int EPI>
+__global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
+  __shared__ __align__(16) uint8_t smem[kBigLds];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const uint32_t lds0 = lds_addr(smem);
+
+  // tile: strips of 8 M tiles, M fastest, so that the 32 tiles an XCD works on
+  // are 8 x 4 (each operand tile is shared by several of them in its L2)
+  const uint32_t total = p.m_tiles * p.n_tiles * p.splits, per = (total + 7) / 8;
+  uint32_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || t >= total) return;
+  const uint32_t split = t % p.splits;
+  t /= p.splits;
+  const uint32_t strip = t / (8 * p.n_tiles), in_strip = t % (8 * p.n_tiles);
+  const uint32_t high = min(8u, p.m_tiles - strip * 8);
+  const uint32_t m0 = (strip * 8 + in_strip % high) * TB, n0 = in_strip / high * TB;
+  const uint32_t all_steps = p.k / KB, per_split = (all_steps + p.splits - 1) / p.splits;
+  const uint32_t s0 = split * per_split, s1 = min(s0 + per_split, all_steps);
+  if (s0 >= s1 && EPI != kEpiAdd) return;
+  const uint32_t steps = s1 > s0 ? s1 - s0 : 0;
+
+  // ---- DMA: instruction i of a wave moves 1 KB: rows 32 i + 8 wave + (l >> 3)
+  // of a rows layout, k rows 8 i + 2 wave + (l >> 5) of a columns layout
+  uint32_t off_a[8], off_b[8];
+  auto offsets = [&](auto T, uint32_t (&off)[8], uint32_t r0, uint32_t rows, uint64_t ld) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      if constexpr (decltype(T)::value) {
+        const uint32_t r = 8 * i + 2 * wave + (lane >> 5), f = (r & 3) + 4 * ((r >> 3) & 1);
+        const uint32_t c = min((r0 >> 3) + ((lane & 31) ^ (2 * f)), (rows - 1) >> 3);
+        off[i] = (uint32_t)(r * ld * 2) + (c << 4);
+      } else {
+        const uint32_t r = 32 * i + 8 * wave + (lane >> 3);
+        off[i] = (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+      }
+    }
+  };
+  offsets(std::bool_constant<AT>{}, off_a, m0, p.m, p.lda);
+  offsets(std::bool_constant<BT>{}, off_b, n0, p.n, p.ldb);
+  const uint8_t* const base_a = reinterpret_cast<const uint8_t*>(AT ? p.a : p.a + m0 * p.lda);
+  const uint8_t* const base_b = reinterpret_cast<const uint8_t*>(BT ? p.b : p.b + n0 * p.ldb);
+  auto source = [&](auto T, const uint8_t* base, uint64_t ld, uint32_t step) __attribute__((always_inline)) {
+    return uniform_ptr(base + (decltype(T)::value ? (uint64_t)step * KB * ld * 2 : (uint64_t)step * KB * 2));
+  };
+  // the part i of 8 of a step's DMAs, into buffer s
+  auto issue = [&](const uint8_t* sa, const uint8_t* sb, uint32_t s, uint32_t i, bool short_b,
+                   uint32_t step) __attribute__((always_inline)) {
+    const uint32_t lds = lds0 + s * 2 * kStageBytes + i * 4096 + wave * 1024;
+    dma16(sa, off_a[i], lds);
+    uint32_t ob = off_b[i];
+    if constexpr (BT) {
+      if (short_b) {
+        // k rows past the last repeat it (their factors in A are 0)
+        const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.k_valid - 1 - step * KB;
+        if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
+      }
+    }
+    dma16(sb, ob, lds + kStageBytes);
+  };
+  auto issue_all = [&](uint32_t step, uint32_t s) __attribute__((always_inline)) {
+    const uint8_t* sa = source(std::bool_constant<AT>{}, base_a, p.lda, step);
+    const uint8_t* sb = source(std::bool_constant<BT>{}, base_b, p.ldb, step);
+    const bool short_b = BT && (step + 1) * KB > p.k_valid;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) issue(sa, sb, s, i, short_b, step);
+  };
+
+  // ---- fragments: rows 16 i .. of the wave's 128, half q of the step
+  const uint32_t row_a = wm * 128 + lr, row_b = wn * 128 + lr;
+  auto frag = [&](auto T, uint32_t stage, uint32_t row, uint32_t i, uint32_t q) __attribute__((always_inline)) -> v4i {
+    const uint8_t* const at = smem + stage;
+    if constexpr (decltype(T)::value) {
+      const uint32_t r = 32 * q + 8 * lg + (lr >> 2), f = (lr >> 2) + 4 * (lg & 1);
+      const uint32_t first = (row & 128) + 16 * i;  // column of the fragment
+      const uint32_t byte = (2 * first + 8 * (lr & 3)) ^ (32 * f);
+      const uint8_t* const x = at + r * 512 + byte;
+      return join(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)x),
+                  __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x + 4 * 512)));
+    } else {
+      const uint32_t r = row + 16 * i;
+      return *reinterpret_cast<const v4i*>(at + r * 128 + (((4 * q + lg) ^ ((lr >> 1) & 7)) << 4));
+    }
+  };
+  v4f acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  v4i fa[2][8], fb[2][8];
+  // the sixteen of a half, three beside each group of eight MFMAs: B's first,
+  // which the next half's first group needs, and all of them two groups early
+  auto read_one = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
+    if (i < 8) fb[to][i] = frag(std::bool_constant<BT>{}, s * 2 * kStageBytes + kStageBytes, row_b, i, q);
+    else if (i < 16) fa[to][i - 8] = frag(std::bool_constant<AT>{}, s * 2 * kStageBytes, row_a, i - 8, q);
+  };
+  auto read_group = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t e = 3 * i; e < 3 * i + 3; ++e) read_one(s, q, to, e);
+  };
+  auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fb[from][j]),
+                                                          __builtin_bit_cast(v8bf, fa[from][i]), acc[i][j], 0, 0, 0);
+  };
+
+  if (steps) {
+    issue_all(s0, 0);
+    if (steps > 1) issue_all(s0 + 1, 1);
+    if (steps > 1) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(16));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_at_most(0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) read_one(0, 0, 0, i);
+    for (uint32_t j = 0; j < steps; ++j) {
+      const uint32_t s = j & 1;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        read_group(s, 1, 1, i);
+        multiply(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // this step read by this wave, the next one arrived for it; then by all
+      __builtin_amdgcn_s_waitcnt(0xC07F & vmcnt_at_most(0));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const bool more = j + 2 < steps;
+      const uint32_t step = s0 + j + 2;
+      const uint8_t* sa = source(std::bool_constant<AT>{}, base_a, p.lda, step);
+      const uint8_t* sb = source(std::bool_constant<BT>{}, base_b, p.ldb, step);
+      const bool short_b = BT && more && (step + 1) * KB > p.k_valid;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        if (j + 1 < steps) read_group(s ^ 1, 0, 0, i);
+        if (more) issue(sa, sb, s, i, short_b, step);
+        multiply(1, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F & vmcnt_at_most(0));
+    __syncthreads();
+  }
+
+  // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of the
+  // wave's quarter
+  const uint32_t wrow = m0 + wm * 128, wcol = n0 + wn * 128;
+  constexpr float kLog2e = 1.44269504088896340736f;
+  if constexpr (EPI == kEpiStats) {
+    // [n half][row]: maximum and sum
+    float2* const half = reinterpret_cast<float2*>(smem);
+    const bool whole = n0 + TB <= p.n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t row = wrow + 16 * i + lr;
+      const uint32_t target = row < p.m ? p.target[row] : kNoTarget;
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = -INFINITY;
+      }
+      const uint32_t at = target - wcol;
+      if (at < 128 && ((at >> 2) & 3) == lg && target < p.n) {
+        float v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v = (uint32_t)j == at >> 4 && (uint32_t)e == (at & 3) ? acc[i][j][e] : v;
+        p.target_logit[row] = v;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float from = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float part = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part += __builtin_amdgcn_exp2f((acc[i][j][e] - from) * kLog2e);
+        sum += part;
+      }
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (lg == 0) half[wn * TB + wm * 128 + 16 * i + lr] = float2{top, sum};
+    }
+    __syncthreads();
+    if (m0 + tid < p.m) {
+      const float2 x = half[tid], y = half[TB + tid];
+      const float top = fmaxf(x.x, y.x);
+      const float sx = x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * kLog2e);
+      const float sy = y.x == -INFINITY ? y.y : y.y * __builtin_amdgcn_exp2f((y.x - top) * kLog2e);
+      p.stats[(uint64_t)(m0 + tid) * p.n_tiles + n0 / TB] = float2{top, sx + sy};
+    }
+  } else if constexpr (EPI == kEpiAdd) {
+    float* const out = static_cast<float*>(p.out) + split * p.split_stride;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t row = wrow + 16 * i + lr;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t col = wcol + 16 * j + 4 * lg;
+        if (row < p.m && col < p.n) {
+          v4f* const o = reinterpret_cast<v4f*>(out + (uint64_t)row * p.ldo + col);
+          *o = p.first ? acc[i][j] : *o + acc[i][j];
+        }
+      }
+    }
+  } else {
+    // bf16 through the wave's own LDS, 16 rows x 256 bytes at a time, so that
+    // a store instruction writes whole lines of four rows
+    constexpr uint32_t kOutRow = 272;
+    uint8_t* const st = smem + wave * 16 * kOutRow;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t row = wrow + 16 * i + lr;
+      uint32_t target = kNoTarget;
+      float lse = 0.0f, up = 0.0f;
+      if constexpr (EPI == kEpiGrad) {
+        if (row < p.m) {
+          target = p.target[row];
+          lse = p.lse[row];
+          up = p.up[row];
+        }
+      }
+      const uint32_t at = target - p.v0 - wcol;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v4f v = acc[i][j];
+        if constexpr (EPI == kEpiGrad) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float g = __builtin_amdgcn_exp2f((v[e] - lse) * kLog2e);
+            if (at == 16u * j + 4 * lg + e) g -= 1.0f;
+            v[e] = target < p.vocab && wcol + 16 * j + 4 * lg + e < p.n ? up * g : 0.0f;
+          }
+        }
+        *reinterpret_cast<uint2*>(st + lr * kOutRow + j * 32 + lg * 8) =
+            uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 4; ++h) {
+        const uint32_t r = wrow + 16 * i + 4 * h + lg, c = wcol + 8 * lr;
+        const v4i o = *reinterpret_cast<const v4i*>(st + (4 * h + lg) * kOutRow + lr * 16);
+        // the rows of g up to a multiple of 64 and its columns up to the
+        // tile's end are written as zeros: the products with g read them
+        const bool in = EPI == kEpiGrad ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
+        if (in) *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c) = o;
+      }
+    }
+  }
+}
+
+template <bool AT, bool BT, int EPI>
+void launch_big(BigArgs p, hipStream_t s) {
+  p.m_tiles = (p.m + TB - 1) / TB;
+  p.n_tiles = (p.n + TB - 1) / TB;
+  if (p.splits == 0) p.splits = 1;
+  const uint32_t grid = (p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8;
+  hipLaunchKernelGGL((loss_big_kernel<AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
+}
+
 // A row's pairs joined, by a wave: lse = M + log(sum of s exp(m - M))
 __global__ __launch_bounds__(256) void loss_join_kernel(const float2* stats, const float* target_logit,
                                                         const uint32_t* target, float* loss, float* lse, uint32_t* err,
@@ -198,11 +514,13 @@ __global__ __launch_bounds__(256) void loss_live_rows_kernel(const uint16_t* x, 
   }
 }
 
-// dx: bf16 of the fp32 sums
-__global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, uint16_t* out, uint64_t count) {
+// dx: bf16 of the fp32 sums, the splits' added in order
+__global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, uint16_t* out, uint64_t count,
+                                                         uint32_t splits) {
   const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= count) return;
-  const v4f v = *reinterpret_cast<const v4f*>(sums + i);
+  v4f v = *reinterpret_cast<const v4f*>(sums + i);
+  for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(sums + s * count + i);
   *reinterpret_cast<uint2*>(out + i) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
 }
 
@@ -225,8 +543,11 @@ uint32_t piece_columns(uint32_t rows, uint32_t vocab) {
   return std::min(all, std::max(fit, 4096u));
 }
 
+// the 256 x 256 tiles take 64-deep steps
+bool big_takes(uint32_t hidden) { return hidden % KB == 0; }
+
 struct BackwardPlan {
-  uint32_t piece;
+  uint32_t piece, splits;
   uint64_t g, live, sums, bytes;
 };
 BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
@@ -236,7 +557,11 @@ BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   p.g = 0;
   p.live = p.g + padded(row_up * p.piece * 2);
   p.sums = p.live + padded(row_up * hidden * 2);
-  p.bytes = p.sums + padded((uint64_t)rows * hidden * 4);
+  // dx has few tiles: its contraction, a piece's columns, is split until
+  // there is a tile for every CU, at 1024 columns a split or more
+  const uint32_t tiles = ((rows + TB - 1) / TB) * ((hidden + TB - 1) / TB);
+  p.splits = big_takes(hidden) ? std::max<uint32_t>(1, std::min<uint32_t>(kCus / tiles, p.piece / 1024)) : 1;
+  p.bytes = p.sums + padded((uint64_t)p.splits * rows * hidden * 4);
   return p;
 }
 
@@ -274,7 +599,22 @@ St LaunchLmHeadLoss(const LmHeadLossArgs& a) {
   g.stats = static_cast<float2*>(a.workspace);
   g.target_logit = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) +
                                             padded((uint64_t)a.rows * g.stat_tiles * 8));
-  launch_gemm<false, false, kEpiStats>(g, a.stream);
+  if (big_takes(a.hidden)) {
+    BigArgs b{};
+    b.a = a.x;
+    b.b = a.w;
+    b.m = a.rows;
+    b.n = b.vocab = a.vocab;
+    b.k = a.hidden;
+    b.lda = b.ldb = a.hidden;
+    b.target = a.target;
+    b.stats = g.stats;
+    b.target_logit = g.target_logit;
+    launch_big<false, false, kEpiStats>(b, a.stream);
+    g.stat_tiles = (a.vocab + TB - 1) / TB;
+  } else {
+    launch_gemm<false, false, kEpiStats>(g, a.stream);
+  }
   hipLaunchKernelGGL(loss_join_kernel, dim3((a.rows + 3) / 4), dim3(256), 0, a.stream, g.stats, g.target_logit,
                      a.target, a.loss, a.lse, a.error_flag, a.rows, a.vocab, g.stat_tiles);
   return AfterLaunch("lm_head_loss_launch_failed");
@@ -302,6 +642,52 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
   for (uint32_t v0 = 0; v0 < a.vocab; v0 += plan.piece) {
     const uint32_t cols = std::min(plan.piece, a.vocab - v0);
     const uint16_t* const w = a.w + (uint64_t)v0 * a.hidden;
+    if (big_takes(a.hidden)) {
+      BigArgs b{};
+      b.a = live;
+      b.b = w;
+      b.m = a.rows;
+      b.n = cols;
+      b.k = a.hidden;
+      b.lda = b.ldb = a.hidden;
+      b.out = grad;
+      b.ldo = plan.piece;
+      b.target = a.target;
+      b.lse = a.lse;
+      b.up = a.loss_grad;
+      b.v0 = v0;
+      b.vocab = a.vocab;
+      launch_big<false, false, kEpiGrad>(b, a.stream);
+      if (a.dw) {
+        b = BigArgs{};
+        b.a = grad;
+        b.b = live;
+        b.m = cols;
+        b.n = a.hidden;
+        b.k = b.k_valid = row_up;
+        b.lda = plan.piece;
+        b.ldb = a.hidden;
+        b.out = a.dw + (uint64_t)v0 * a.hidden;
+        b.ldo = a.hidden;
+        launch_big<true, true, kEpiBf16>(b, a.stream);
+      }
+      b = BigArgs{};
+      b.a = grad;
+      b.b = w;
+      b.m = a.rows;
+      b.n = a.hidden;
+      b.k = (cols + KB - 1) / KB * KB;
+      b.k_valid = cols;
+      b.lda = plan.piece;
+      b.ldb = a.hidden;
+      b.out = sums;
+      b.ldo = a.hidden;
+      b.splits = plan.splits;
+      b.split_stride = (uint64_t)a.rows * a.hidden;
+      b.first = v0 == 0;
+      launch_big<false, true, kEpiAdd>(b, a.stream);
+      continue;
+    }
     GemmArgs g{};
     g.a = live;
     g.b = w;
@@ -345,7 +731,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
   }
   const uint64_t count = (uint64_t)a.rows * a.hidden;
   hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, a.stream, sums, a.dx,
-                     count);
+                     count, plan.splits);
   return AfterLaunch("lm_head_loss_backward_launch_failed");
 }
 
