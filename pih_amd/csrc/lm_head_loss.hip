@@ -203,6 +203,16 @@ __device__ __forceinline__ v4i join(v4s x, v4s y) {
   return v4i{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
 }
 
+// c += a . b with c kept where it is: with all 256 accumulator registers in
+// use the compiler's own form moved them about, 518 moves beside 128 MFMAs.
+// Nothing else touches an accumulator within 63 MFMAs of its own; before the
+// results are read accumulators_settle() stands.
+__device__ __forceinline__ void mfma_in_place(v4f& c, v4i a, v4i b) {
+  asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// the cycles from the last MFMA to the first read of its result
+__device__ __forceinline__ void accumulators_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
 template <bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   __shared__ __align__(16) uint8_t smem[kBigLds];
@@ -306,9 +316,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   };
   auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fb[from][j]),
-                                                          __builtin_bit_cast(v8bf, fa[from][i]), acc[i][j], 0, 0, 0);
+    for (int j = 0; j < 8; ++j) mfma_in_place(acc[i][j], fb[from][j], fa[from][i]);
   };
 
   if (steps) {
@@ -320,33 +328,53 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     asm volatile("" ::: "memory");
 #pragma unroll
     for (uint32_t i = 0; i < 16; ++i) read_one(0, 0, 0, i);
-    for (uint32_t j = 0; j < steps; ++j) {
+    // kMore: the step after the next one exists and is sent for (kLast: it is
+    // the last one, whose k rows may be short); kNext: the next one exists
+    auto body = [&](uint32_t j, auto NEXT, auto MORE, auto LAST) __attribute__((always_inline)) {
+      constexpr bool kNext = decltype(NEXT)::value, kMore = decltype(MORE)::value, kLast = decltype(LAST)::value;
       const uint32_t s = j & 1;
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
+        // (the first MFMAs wait for every LDS read before them)
+        if (i == 0) {
+          multiply(0, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         read_group(s, 1, 1, i);
-        multiply(0, i);
+        if (i) multiply(0, i);
         __builtin_amdgcn_sched_barrier(0);
       }
       // this step read by this wave, the next one arrived for it; then by all
       __builtin_amdgcn_s_waitcnt(0xC07F & vmcnt_at_most(0));
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      const bool more = j + 2 < steps;
       const uint32_t step = s0 + j + 2;
-      const uint8_t* sa = source(std::bool_constant<AT>{}, base_a, p.lda, step);
-      const uint8_t* sb = source(std::bool_constant<BT>{}, base_b, p.ldb, step);
-      const bool short_b = BT && more && (step + 1) * KB > p.k_valid;
+      const uint8_t* sa = nullptr;
+      const uint8_t* sb = nullptr;
+      if constexpr (kMore) {
+        sa = source(std::bool_constant<AT>{}, base_a, p.lda, step);
+        sb = source(std::bool_constant<BT>{}, base_b, p.ldb, step);
+      }
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
-        if (j + 1 < steps) read_group(s ^ 1, 0, 0, i);
-        if (more) issue(sa, sb, s, i, short_b, step);
+        if constexpr (kNext) read_group(s ^ 1, 0, 0, i);
+        if constexpr (kMore) issue(sa, sb, s, i, kLast && (step + 1) * KB > p.k_valid, step);
         multiply(1, i);
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
+    };
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    uint32_t j = 0;
+#pragma unroll 1
+    for (; j + (BT ? 3 : 2) < steps; ++j) body(j, yes, yes, no);
+    if constexpr (BT)
+      if (j + 2 < steps) body(j++, yes, yes, yes);
+    if (j + 1 < steps) body(j++, yes, no, no);
+    body(j, no, no, no);
     __builtin_amdgcn_s_waitcnt(0xC07F & vmcnt_at_most(0));
     __syncthreads();
+    accumulators_settle();
   }
 
   // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of the
