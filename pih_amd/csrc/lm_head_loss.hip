@@ -156,10 +156,12 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
   }
 }
 
-// ------------------------------------------------ 256 x 256 tiles
-// C [m][n] = A . B^T for large products, four waves of 128 x 128 (one per
-// SIMD, 256 accumulator registers each).  A K step is 64 deep and moved into
-// LDS by DMA, two steps resident.  Two layouts of an operand:
+// ------------------------------------------------ tiles fed by DMA
+// C [m][n] = A . B^T in tiles of 256 columns and 256 or (few rows) 64 rows.
+// Four waves: 2 x 2 quarters of 128 x 128, one wave per SIMD with 256
+// accumulator registers, or 1 x 4 of 64 x 64.  A K step is 64 deep and moved
+// into LDS by DMA, two (64 rows: three) steps resident.  Two layouts of an
+// operand:
 //   rows     [row][k] in memory: LDS rows of 128 bytes, 16-byte chunk c of row
 //            r in slot c ^ ((r >> 1) & 7); a fragment is one ds_read_b128
 //            (16 rows, one chunk each: all 64 banks once);
@@ -172,10 +174,11 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
 // The step's two 32-deep halves: while the MFMAs of the first run, the second
 // half's fragments are read; then one wait and one barrier (every wave has
 // read the step, and the next one has arrived), and while the MFMAs of the
-// second run, the next step's first fragments are read and the step after it
-// is sent for, into the buffer just freed.
-constexpr uint32_t TB = 256, KB = 64, kStageBytes = TB * KB * 2;  // one operand's step
-constexpr uint32_t kBigLds = 4 * kStageBytes;
+// second run, the next step's first fragments are read and another step is
+// sent for, into the buffer just freed.  A block per CU walks its tiles; the
+// next tile's first steps are sent for before the results of this one are
+// worked on.
+constexpr uint32_t TB = 256, KB = 64;
 
 struct BigArgs {
   const uint16_t* a;
@@ -205,110 +208,155 @@ __device__ __forceinline__ v4i join(v4s x, v4s y) {
 
 // c += a . b with c kept where it is: with all 256 accumulator registers in
 // use the compiler's own form moved them about, 518 moves beside 128 MFMAs.
-// Nothing else touches an accumulator within 63 MFMAs of its own; before the
-// results are read accumulators_settle() stands.
+// The compiler does not see an MFMA in it, so the wait states are kept here: an
+// operand written by a vector instruction is read two states later (s_nop 1;
+// the matrix pipe is busy with the MFMA before meanwhile), an accumulator is
+// used again no sooner than 15 MFMAs on, and settle() stands between the MFMAs
+// and anything else that touches accumulators, tied to them by its operands.
 __device__ __forceinline__ void mfma_in_place(v4f& c, v4i a, v4i b) {
-  asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-// the cycles from the last MFMA to the first read of its result
-__device__ __forceinline__ void accumulators_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+template <int NB>
+__device__ __forceinline__ void settle(v4f (&c)[NB]) {
+  static_assert(NB == 4 || NB == 8, "blocks");
+  if constexpr (NB == 8)
+    asm volatile("s_nop 15\n\ts_nop 7"
+                 : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
+  else
+    asm volatile("s_nop 15\n\ts_nop 7" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]));
+}
 
-template <bool AT, bool BT, int EPI>
+template <int ROWS>
+struct BigShape {
+  static constexpr int WM = ROWS == 256 ? 2 : 1, WN = 4 / WM;        // waves
+  static constexpr int MB = ROWS / 16 / WM, NB = TB / 16 / WN;       // a wave's 16 x 16 blocks
+  static constexpr int ST = ROWS == 256 ? 2 : 3;                     // steps resident
+  static constexpr uint32_t kA = ROWS * KB * 2, kB = TB * KB * 2, kStage = kA + kB;
+  static constexpr int LA = ROWS / 32, LB = 8, NL = LA + LB;         // DMAs per wave and step
+  static constexpr uint32_t kOutRow = 16 * NB * 2 + 16;              // a wave's staged output row
+  static constexpr uint32_t kOut = ST * kStage;                      // 16 of them per wave
+  static constexpr uint32_t kMeta = kOut + 4 * 16 * kOutRow;         // per row: two tiles' targets, lse, up
+  static constexpr uint32_t kLds = kMeta + 2 * ROWS * 12;
+  static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+template <int ROWS, bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
-  __shared__ __align__(16) uint8_t smem[kBigLds];
+  using S = BigShape<ROWS>;
+  constexpr int MB = S::MB, NB = S::NB, ST = S::ST, LA = S::LA, LB = S::LB, NL = S::NL;
+  __shared__ __align__(16) uint8_t smem[S::kLds];
   const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
   const uint32_t lds0 = lds_addr(smem);
 
-  // tile: strips of 8 M tiles, M fastest, so that the 32 tiles an XCD works on
-  // are 8 x 4 (each operand tile is shared by several of them in its L2)
-  const uint32_t total = p.m_tiles * p.n_tiles * p.splits, per = (total + 7) / 8;
-  uint32_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per || t >= total) return;
-  const uint32_t split = t % p.splits;
-  t /= p.splits;
-  const uint32_t strip = t / (8 * p.n_tiles), in_strip = t % (8 * p.n_tiles);
-  const uint32_t high = min(8u, p.m_tiles - strip * 8);
-  const uint32_t m0 = (strip * 8 + in_strip % high) * TB, n0 = in_strip / high * TB;
+  // tiles: strips of 8 M tiles, M fastest, so that the 32 tiles an XCD works
+  // on are 8 x 4 (each operand tile is shared by several of them in its L2);
+  // the splits of a tile side by side
+  const uint32_t total = p.m_tiles * p.n_tiles * p.splits, per = (total + 7) / 8, stride = gridDim.x >> 3;
+  const uint32_t end = min(((blockIdx.x & 7) + 1) * per, total);
   const uint32_t all_steps = p.k / KB, per_split = (all_steps + p.splits - 1) / p.splits;
-  const uint32_t s0 = split * per_split, s1 = min(s0 + per_split, all_steps);
-  if (s0 >= s1 && EPI != kEpiAdd) return;
-  const uint32_t steps = s1 > s0 ? s1 - s0 : 0;
+  uint32_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  uint32_t m0, n0, split, s0, steps;
 
   // ---- DMA: instruction i of a wave moves 1 KB: rows 32 i + 8 wave + (l >> 3)
   // of a rows layout, k rows 8 i + 2 wave + (l >> 5) of a columns layout
-  uint32_t off_a[8], off_b[8];
-  auto offsets = [&](auto T, uint32_t (&off)[8], uint32_t r0, uint32_t rows, uint64_t ld) __attribute__((always_inline)) {
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      if constexpr (decltype(T)::value) {
-        const uint32_t r = 8 * i + 2 * wave + (lane >> 5), f = (r & 3) + 4 * ((r >> 3) & 1);
-        const uint32_t c = min((r0 >> 3) + ((lane & 31) ^ (2 * f)), (rows - 1) >> 3);
-        off[i] = (uint32_t)(r * ld * 2) + (c << 4);
-      } else {
-        const uint32_t r = 32 * i + 8 * wave + (lane >> 3);
-        off[i] = (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
-      }
+  uint32_t off_a[LA], off_b[LB];
+  const uint8_t* base_a;
+  const uint8_t* base_b;
+  auto offset = [&](auto T, uint32_t i, uint32_t r0, uint32_t rows, uint64_t ld) __attribute__((always_inline)) {
+    if constexpr (decltype(T)::value) {
+      const uint32_t r = 8 * i + 2 * wave + (lane >> 5), f = (r & 3) + 4 * ((r >> 3) & 1);
+      const uint32_t c = min((r0 >> 3) + ((lane & 31) ^ (2 * f)), (rows - 1) >> 3);
+      return (uint32_t)(r * ld * 2) + (c << 4);
+    } else {
+      const uint32_t r = 32 * i + 8 * wave + (lane >> 3);
+      return (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
     }
   };
-  offsets(std::bool_constant<AT>{}, off_a, m0, p.m, p.lda);
-  offsets(std::bool_constant<BT>{}, off_b, n0, p.n, p.ldb);
-  const uint8_t* const base_a = reinterpret_cast<const uint8_t*>(AT ? p.a : p.a + m0 * p.lda);
-  const uint8_t* const base_b = reinterpret_cast<const uint8_t*>(BT ? p.b : p.b + n0 * p.ldb);
   auto source = [&](auto T, const uint8_t* base, uint64_t ld, uint32_t step) __attribute__((always_inline)) {
     return uniform_ptr(base + (decltype(T)::value ? (uint64_t)step * KB * ld * 2 : (uint64_t)step * KB * 2));
   };
-  // the part i of 8 of a step's DMAs, into buffer s
+  constexpr std::bool_constant<AT> at{};
+  constexpr std::bool_constant<BT> bt{};
+  // DMA i of a step (A's first) into buffer s
   auto issue = [&](const uint8_t* sa, const uint8_t* sb, uint32_t s, uint32_t i, bool short_b,
                    uint32_t step) __attribute__((always_inline)) {
-    const uint32_t lds = lds0 + s * 2 * kStageBytes + i * 4096 + wave * 1024;
-    dma16(sa, off_a[i], lds);
-    uint32_t ob = off_b[i];
-    if constexpr (BT) {
-      if (short_b) {
-        // k rows past the last repeat it (their factors in A are 0)
-        const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.k_valid - 1 - step * KB;
-        if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
+    const uint32_t lds = lds0 + s * S::kStage + wave * 1024;
+    if (i < (uint32_t)LA) {
+      dma16(sa, off_a[i], lds + i * 4096);
+    } else {
+      i -= LA;
+      uint32_t ob = off_b[i];
+      if constexpr (BT) {
+        if (short_b) {
+          // k rows past the last repeat it (their factors in A are 0)
+          const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.k_valid - 1 - step * KB;
+          if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
+        }
+      }
+      dma16(sb, ob, lds + S::kA + i * 4096);
+    }
+  };
+  // tile t and its first steps sent for; its rows' targets and factors into
+  // half `which` of the panel (0 for a row that has no target: g is 0)
+  auto start = [&](uint32_t which) __attribute__((always_inline)) {
+    split = t % p.splits;
+    const uint32_t u = t / p.splits, strip = u / (8 * p.n_tiles), in_strip = u % (8 * p.n_tiles);
+    const uint32_t high = min(8u, p.m_tiles - strip * 8);
+    m0 = (strip * 8 + in_strip % high) * ROWS;
+    n0 = in_strip / high * TB;
+    s0 = min(split * per_split, all_steps);
+    steps = min(s0 + per_split, all_steps) - s0;
+    base_a = reinterpret_cast<const uint8_t*>(AT ? p.a : p.a + m0 * p.lda);
+    base_b = reinterpret_cast<const uint8_t*>(BT ? p.b : p.b + n0 * p.ldb);
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)LA; ++i) off_a[i] = offset(at, i, m0, p.m, p.lda);
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)LB; ++i) off_b[i] = offset(bt, i, n0, p.n, p.ldb);
+#pragma unroll
+    for (uint32_t q = 0; q < (uint32_t)ST; ++q) {
+      if (q >= steps) break;
+      const uint8_t* sa = source(at, base_a, p.lda, s0 + q);
+      const uint8_t* sb = source(bt, base_b, p.ldb, s0 + q);
+      const bool short_b = BT && (s0 + q + 1) * KB > p.k_valid;
+#pragma unroll
+      for (uint32_t i = 0; i < (uint32_t)NL; ++i) issue(sa, sb, q, i, short_b, s0 + q);
+    }
+    if constexpr (EPI == kEpiStats || EPI == kEpiGrad) {
+      if (tid < ROWS) {
+        const uint32_t row = m0 + tid;
+        uint32_t* const meta = reinterpret_cast<uint32_t*>(smem + S::kMeta + which * ROWS * 12);
+        const uint32_t y = row < p.m ? p.target[row] : kNoTarget;
+        meta[tid] = y;
+        if constexpr (EPI == kEpiGrad) {
+          const bool live = y < p.vocab;
+          meta[ROWS + tid] = __float_as_uint(live ? p.lse[row] : 0.0f);
+          meta[2 * ROWS + tid] = __float_as_uint(live ? p.up[row] : 0.0f);
+        }
       }
     }
-    dma16(sb, ob, lds + kStageBytes);
-  };
-  auto issue_all = [&](uint32_t step, uint32_t s) __attribute__((always_inline)) {
-    const uint8_t* sa = source(std::bool_constant<AT>{}, base_a, p.lda, step);
-    const uint8_t* sb = source(std::bool_constant<BT>{}, base_b, p.ldb, step);
-    const bool short_b = BT && (step + 1) * KB > p.k_valid;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) issue(sa, sb, s, i, short_b, step);
   };
 
-  // ---- fragments: rows 16 i .. of the wave's 128, half q of the step
-  const uint32_t row_a = wm * 128 + lr, row_b = wn * 128 + lr;
-  auto frag = [&](auto T, uint32_t stage, uint32_t row, uint32_t i, uint32_t q) __attribute__((always_inline)) -> v4i {
-    const uint8_t* const at = smem + stage;
+  // ---- fragments: 16 rows of the wave's, half q of the step
+  auto frag = [&](auto T, uint32_t stage, uint32_t first, uint32_t q) __attribute__((always_inline)) -> v4i {
+    const uint8_t* const from = smem + stage;
     if constexpr (decltype(T)::value) {
       const uint32_t r = 32 * q + 8 * lg + (lr >> 2), f = (lr >> 2) + 4 * (lg & 1);
-      const uint32_t first = (row & 128) + 16 * i;  // column of the fragment
-      const uint32_t byte = (2 * first + 8 * (lr & 3)) ^ (32 * f);
-      const uint8_t* const x = at + r * 512 + byte;
+      const uint8_t* const x = from + r * 512 + ((2 * first + 8 * (lr & 3)) ^ (32 * f));
       return join(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)x),
                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x + 4 * 512)));
     } else {
-      const uint32_t r = row + 16 * i;
-      return *reinterpret_cast<const v4i*>(at + r * 128 + (((4 * q + lg) ^ ((lr >> 1) & 7)) << 4));
+      return *reinterpret_cast<const v4i*>(from + (first + lr) * 128 + (((4 * q + lg) ^ ((lr >> 1) & 7)) << 4));
     }
   };
-  v4f acc[8][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-
-  v4i fa[2][8], fb[2][8];
-  // the sixteen of a half, three beside each group of eight MFMAs: B's first,
-  // which the next half's first group needs, and all of them two groups early
+  v4f acc[MB][NB];
+  v4i fa[2][MB], fb[2][NB];
+  // the fragments of a half, three beside each group of NB MFMAs: B's first,
+  // which the next half's first group needs, and all of them a group or two
+  // early
   auto read_one = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
-    if (i < 8) fb[to][i] = frag(std::bool_constant<BT>{}, s * 2 * kStageBytes + kStageBytes, row_b, i, q);
-    else if (i < 16) fa[to][i - 8] = frag(std::bool_constant<AT>{}, s * 2 * kStageBytes, row_a, i - 8, q);
+    if (i < (uint32_t)NB) fb[to][i] = frag(bt, s * S::kStage + S::kA, wn * NB * 16 + 16 * i, q);
+    else if (i < (uint32_t)(NB + MB)) fa[to][i - NB] = frag(at, s * S::kStage, wm * MB * 16 + 16 * (i - NB), q);
   };
   auto read_group = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
@@ -316,187 +364,239 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   };
   auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mfma_in_place(acc[i][j], fb[from][j], fa[from][i]);
+    for (int j = 0; j < NB; ++j) mfma_in_place(acc[i][j], fb[from][j], fa[from][i]);
   };
-
-  if (steps) {
-    issue_all(s0, 0);
-    if (steps > 1) issue_all(s0 + 1, 1);
-    if (steps > 1) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(16));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_at_most(0));
+  uint32_t s;  // the buffer of the step being multiplied
+  // kNext: the next step exists, with kLeft further steps in flight behind it;
+  // kMore: step j + ST exists and is sent for (kLast: it is the last one,
+  // whose k rows may be short)
+  auto body = [&](uint32_t j, auto NEXT, auto LEFT, auto MORE, auto LAST) __attribute__((always_inline)) {
+    constexpr bool kNext = decltype(NEXT)::value, kMore = decltype(MORE)::value, kLast = decltype(LAST)::value;
+    const uint32_t ns = s + 1 == ST ? 0 : s + 1;
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
+      // (the first MFMAs wait for every LDS read before them)
+      if (i == 0) {
+        multiply(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      read_group(s, 1, 1, i);
+      if (i) multiply(0, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // this step read by this wave, the next one arrived for it; then by all
+    __builtin_amdgcn_s_waitcnt(kLdsRead & vmcnt_at_most(decltype(LEFT)::value * NL));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    const uint32_t step = s0 + j + ST;
+    const uint8_t* sa = nullptr;
+    const uint8_t* sb = nullptr;
+    if constexpr (kMore) {
+      sa = source(at, base_a, p.lda, step);
+      sb = source(bt, base_b, p.ldb, step);
+    }
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) read_one(0, 0, 0, i);
-    // kMore: the step after the next one exists and is sent for (kLast: it is
-    // the last one, whose k rows may be short); kNext: the next one exists
-    auto body = [&](uint32_t j, auto NEXT, auto MORE, auto LAST) __attribute__((always_inline)) {
-      constexpr bool kNext = decltype(NEXT)::value, kMore = decltype(MORE)::value, kLast = decltype(LAST)::value;
-      const uint32_t s = j & 1;
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        // (the first MFMAs wait for every LDS read before them)
-        if (i == 0) {
-          multiply(0, i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        read_group(s, 1, 1, i);
-        if (i) multiply(0, i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      // this step read by this wave, the next one arrived for it; then by all
-      __builtin_amdgcn_s_waitcnt(0xC07F & vmcnt_at_most(0));
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      const uint32_t step = s0 + j + 2;
-      const uint8_t* sa = nullptr;
-      const uint8_t* sb = nullptr;
+    for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
+      if constexpr (kNext) read_group(ns, 0, 0, i);
       if constexpr (kMore) {
-        sa = source(std::bool_constant<AT>{}, base_a, p.lda, step);
-        sb = source(std::bool_constant<BT>{}, base_b, p.ldb, step);
-      }
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        if constexpr (kNext) read_group(s ^ 1, 0, 0, i);
-        if constexpr (kMore) issue(sa, sb, s, i, kLast && (step + 1) * KB > p.k_valid, step);
-        multiply(1, i);
-        __builtin_amdgcn_sched_barrier(0);
+        for (uint32_t e = i * NL / MB; e < (i + 1) * NL / MB; ++e)
+          issue(sa, sb, s, e, kLast && (step + 1) * KB > p.k_valid, step);
       }
-    };
-    constexpr std::true_type yes;
-    constexpr std::false_type no;
-    uint32_t j = 0;
-#pragma unroll 1
-    for (; j + (BT ? 3 : 2) < steps; ++j) body(j, yes, yes, no);
-    if constexpr (BT)
-      if (j + 2 < steps) body(j++, yes, yes, yes);
-    if (j + 1 < steps) body(j++, yes, no, no);
-    body(j, no, no, no);
-    __builtin_amdgcn_s_waitcnt(0xC07F & vmcnt_at_most(0));
-    __syncthreads();
-    accumulators_settle();
-  }
+      multiply(1, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    s = ns;
+  };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  constexpr std::integral_constant<int, 0> none;
+  constexpr std::integral_constant<int, ST - 2> full;
 
-  // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of the
-  // wave's quarter
-  const uint32_t wrow = m0 + wm * 128, wcol = n0 + wn * 128;
-  constexpr float kLog2e = 1.44269504088896340736f;
-  if constexpr (EPI == kEpiStats) {
-    // [n half][row]: maximum and sum
-    float2* const half = reinterpret_cast<float2*>(smem);
-    const bool whole = n0 + TB <= p.n;
+  if (t >= end) return;
+  uint32_t which = 0;
+  start(which);
+  while (true) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t row = wrow + 16 * i + lr;
-      const uint32_t target = row < p.m ? p.target[row] : kNoTarget;
-      if (!whole) {
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = -INFINITY;
-      }
-      const uint32_t at = target - wcol;
-      if (at < 128 && ((at >> 2) & 3) == lg && target < p.n) {
-        float v = 0.0f;
+    for (int i = 0; i < MB; ++i) settle(acc[i]);
+    // (the stores of the tile before count too)
+    __builtin_amdgcn_s_waitcnt(kLdsRead & vmcnt_at_most(0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (steps) {
+      s = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v = (uint32_t)j == at >> 4 && (uint32_t)e == (at & 3) ? acc[i][j][e] : v;
-        p.target_logit[row] = v;
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float from = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float part = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) part += __builtin_amdgcn_exp2f((acc[i][j][e] - from) * kLog2e);
-        sum += part;
-      }
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      if (lg == 0) half[wn * TB + wm * 128 + 16 * i + lr] = float2{top, sum};
+      for (uint32_t i = 0; i < (uint32_t)(MB + NB); ++i) read_one(0, 0, 0, i);
+      uint32_t j = 0;
+#pragma unroll 1
+      for (; j + ST + (BT ? 1 : 0) < steps; ++j) body(j, yes, full, yes, no);
+      if constexpr (BT)
+        if (j + ST < steps) body(j++, yes, full, yes, yes);
+      if constexpr (ST == 3)
+        if (j + 2 < steps) body(j++, yes, std::integral_constant<int, 1>{}, no, no);
+      if (j + 1 < steps) body(j++, yes, none, no, no);
+      body(j, no, none, no, no);
     }
-    __syncthreads();
-    if (m0 + tid < p.m) {
-      const float2 x = half[tid], y = half[TB + tid];
-      const float top = fmaxf(x.x, y.x);
-      const float sx = x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * kLog2e);
-      const float sy = y.x == -INFINITY ? y.y : y.y * __builtin_amdgcn_exp2f((y.x - top) * kLog2e);
-      p.stats[(uint64_t)(m0 + tid) * p.n_tiles + n0 / TB] = float2{top, sx + sy};
+    const uint32_t cm = m0, cn = n0, csplit = split;
+    const uint32_t* const meta = reinterpret_cast<const uint32_t*>(smem + S::kMeta + which * ROWS * 12);
+    const bool more = t + stride < end;
+    which ^= 1;
+    if (more) {
+      // (every wave is past the barrier after its last read of a buffer)
+      t += stride;
+      start(which);
     }
-  } else if constexpr (EPI == kEpiAdd) {
-    float* const out = static_cast<float*>(p.out) + split * p.split_stride;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t row = wrow + 16 * i + lr;
+    for (int i = 0; i < MB; ++i) settle(acc[i]);
+
+    // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of
+    // the wave's part
+    const uint32_t lrow = wm * MB * 16, wrow = cm + lrow, wcol = cn + wn * NB * 16;
+    constexpr float kLog2e = 1.44269504088896340736f;
+    if constexpr (EPI == kEpiStats) {
+      // [column part][row]: maximum and sum
+      float2* const parts = reinterpret_cast<float2*>(smem + S::kOut);
+      static_assert(S::WN * ROWS * 8 <= 4 * 16 * S::kOutRow, "parts");
+      const bool whole = cn + TB <= p.n;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t col = wcol + 16 * j + 4 * lg;
-        if (row < p.m && col < p.n) {
-          v4f* const o = reinterpret_cast<v4f*>(out + (uint64_t)row * p.ldo + col);
-          *o = p.first ? acc[i][j] : *o + acc[i][j];
+      for (int i = 0; i < MB; ++i) {
+        const uint32_t target = meta[lrow + 16 * i + lr];
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = -INFINITY;
         }
-      }
-    }
-  } else {
-    // bf16 through the wave's own LDS, 16 rows x 256 bytes at a time, so that
-    // a store instruction writes whole lines of four rows
-    constexpr uint32_t kOutRow = 272;
-    uint8_t* const st = smem + wave * 16 * kOutRow;
+        const uint32_t place = target - wcol;
+        if (place < 16u * NB && ((place >> 2) & 3) == lg && target < p.n) {
+          float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t row = wrow + 16 * i + lr;
-      uint32_t target = kNoTarget;
-      float lse = 0.0f, up = 0.0f;
-      if constexpr (EPI == kEpiGrad) {
-        if (row < p.m) {
-          target = p.target[row];
-          lse = p.lse[row];
-          up = p.up[row];
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v = (uint32_t)j == place >> 4 && (uint32_t)e == (place & 3) ? acc[i][j][e] : v;
+          p.target_logit[wrow + 16 * i + lr] = v;
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float from = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          float part = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part += __builtin_amdgcn_exp2f((acc[i][j][e] - from) * kLog2e);
+          sum += part;
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lg == 0) parts[wn * ROWS + lrow + 16 * i + lr] = float2{top, sum};
       }
-      const uint32_t at = target - p.v0 - wcol;
+      __syncthreads();
+      if (tid < ROWS && cm + tid < p.m) {
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v4f v = acc[i][j];
-        if constexpr (EPI == kEpiGrad) {
+        for (int w = 0; w < S::WN; ++w) top = fmaxf(top, parts[w * ROWS + tid].x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float g = __builtin_amdgcn_exp2f((v[e] - lse) * kLog2e);
-            if (at == 16u * j + 4 * lg + e) g -= 1.0f;
-            v[e] = target < p.vocab && wcol + 16 * j + 4 * lg + e < p.n ? up * g : 0.0f;
+        for (int w = 0; w < S::WN; ++w) {
+          const float2 x = parts[w * ROWS + tid];
+          sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * kLog2e);
+        }
+        p.stats[(uint64_t)(cm + tid) * p.n_tiles + cn / TB] = float2{top, sum};
+      }
+    } else if constexpr (EPI == kEpiAdd) {
+      float* const out = static_cast<float*>(p.out) + csplit * p.split_stride;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const uint32_t row = wrow + 16 * i + lr;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const uint32_t col = wcol + 16 * j + 4 * lg;
+          if (row < p.m && col < p.n) {
+            v4f* const o = reinterpret_cast<v4f*>(out + (uint64_t)row * p.ldo + col);
+            *o = p.first ? acc[i][j] : *o + acc[i][j];
           }
         }
-        *reinterpret_cast<uint2*>(st + lr * kOutRow + j * 32 + lg * 8) =
-            uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
       }
+    } else {
+      // bf16 through the wave's own LDS, 16 rows at a time, so that a store
+      // instruction writes whole lines
+      constexpr uint32_t kLanes = 2 * NB, kRowsAt = 64 / kLanes;  // lanes per row, rows per instruction
+      uint8_t* const st = smem + S::kOut + wave * 16 * S::kOutRow;
+      const bool whole = cn + TB <= p.n;
 #pragma unroll
-      for (uint32_t h = 0; h < 4; ++h) {
-        const uint32_t r = wrow + 16 * i + 4 * h + lg, c = wcol + 8 * lr;
-        const v4i o = *reinterpret_cast<const v4i*>(st + (4 * h + lg) * kOutRow + lr * 16);
-        // the rows of g up to a multiple of 64 and its columns up to the
-        // tile's end are written as zeros: the products with g read them
-        const bool in = EPI == kEpiGrad ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
-        if (in) *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c) = o;
+      for (int i = 0; i < MB; ++i) {
+        if constexpr (EPI == kEpiGrad) {
+          const uint32_t at_row = lrow + 16 * i + lr, place = meta[at_row] - p.v0 - wcol;
+          const float shift = -__uint_as_float(meta[ROWS + at_row]) * kLog2e, up = __uint_as_float(meta[2 * ROWS + at_row]);
+          const bool here = place < 16u * NB;
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[i][j][e] = up * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, shift));
+          if (__builtin_amdgcn_ballot_w64(here)) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (place == 16u * j + 4 * lg + e) acc[i][j][e] -= up;
+          }
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const v4f v = acc[i][j];
+          *reinterpret_cast<uint2*>(st + lr * S::kOutRow + j * 32 + lg * 8) =
+              uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < 16 / kRowsAt; ++h) {
+          const uint32_t q = kRowsAt * h + lane / kLanes, r = wrow + 16 * i + q, c = wcol + 8 * (lane % kLanes);
+          const v4i o = *reinterpret_cast<const v4i*>(st + q * S::kOutRow + lane % kLanes * 16);
+          // the rows of g up to a multiple of 64 and its columns up to the
+          // tile's end are written as zeros: the products with g read them
+          const bool in = EPI == kEpiGrad ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
+          if (in) *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c) = o;
+        }
       }
     }
+    if (!more) return;
   }
 }
 
-template <bool AT, bool BT, int EPI>
-void launch_big(BigArgs p, hipStream_t s) {
-  p.m_tiles = (p.m + TB - 1) / TB;
+template <int ROWS, bool AT, bool BT, int EPI>
+void launch_rows(BigArgs p, hipStream_t s) {
+  p.m_tiles = (p.m + ROWS - 1) / ROWS;
   p.n_tiles = (p.n + TB - 1) / TB;
   if (p.splits == 0) p.splits = 1;
-  const uint32_t grid = (p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8;
-  hipLaunchKernelGGL((loss_big_kernel<AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
+  const uint32_t grid = std::min((p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8, kCus);
+  hipLaunchKernelGGL((loss_big_kernel<ROWS, AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
+}
+// products whose rows are the batch's: 64-row tiles while there is one of them
+template <bool AT, bool BT, int EPI>
+void launch_big(const BigArgs& p, hipStream_t s) {
+  if constexpr (!AT) {
+    if (p.m <= 64) {
+      launch_rows<64, AT, BT, EPI>(p, s);
+      return;
+    }
+  }
+  launch_rows<256, AT, BT, EPI>(p, s);
 }
 
 // A row's pairs joined, by a wave: lse = M + log(sum of s exp(m - M))
