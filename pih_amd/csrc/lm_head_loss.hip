@@ -384,8 +384,10 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       if (i) multiply(0, i);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // this step read by this wave, the next one arrived for it; then by all
-    __builtin_amdgcn_s_waitcnt(kLdsRead & vmcnt_at_most(decltype(LEFT)::value * NL));
+    // this step read by this wave, the next one arrived for it (the first ST
+    // had before the tile was begun); then by all
+    __builtin_amdgcn_s_waitcnt(kLdsRead);
+    if (j + 1 >= (uint32_t)ST) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(decltype(LEFT)::value * NL));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     const uint32_t step = s0 + j + ST;
@@ -416,6 +418,11 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   if (t >= end) return;
   uint32_t which = 0;
   start(which);
+  // a tile's first steps have arrived before it is begun; for the tiles after
+  // the first that is waited for ahead of the results' stores, which so drain
+  // while the next tile is multiplied
+  auto arrived = []() __attribute__((always_inline)) { __builtin_amdgcn_s_waitcnt(vmcnt_at_most(0)); };
+  arrived();
   while (true) {
 #pragma unroll
     for (int i = 0; i < MB; ++i)
@@ -423,8 +430,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < MB; ++i) settle(acc[i]);
-    // (the stores of the tile before count too)
-    __builtin_amdgcn_s_waitcnt(kLdsRead & vmcnt_at_most(0));
+    __builtin_amdgcn_s_waitcnt(kLdsRead);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (steps) {
@@ -455,6 +461,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
 
     // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of
     // the wave's part
+    if constexpr (EPI != kEpiGrad) arrived();
     const uint32_t lrow = wm * MB * 16, wrow = cm + lrow, wcol = cn + wn * NB * 16;
     constexpr float kLog2e = 1.44269504088896340736f;
     if constexpr (EPI == kEpiStats) {
@@ -513,18 +520,23 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         p.stats[(uint64_t)(cm + tid) * p.n_tiles + cn / TB] = float2{top, sum};
       }
     } else if constexpr (EPI == kEpiAdd) {
-      float* const out = static_cast<float*>(p.out) + csplit * p.split_stride;
+      float* const out = static_cast<float*>(p.out) + csplit * p.split_stride + wcol + 4 * lg;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
         const uint32_t row = wrow + 16 * i + lr;
+        v4f* const o = reinterpret_cast<v4f*>(out + (uint64_t)min(row, p.m - 1) * p.ldo);
+        v4f before[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          const uint32_t col = wcol + 16 * j + 4 * lg;
-          if (row < p.m && col < p.n) {
-            v4f* const o = reinterpret_cast<v4f*>(out + (uint64_t)row * p.ldo + col);
-            *o = p.first ? acc[i][j] : *o + acc[i][j];
-          }
+          before[j] = v4f{0.f, 0.f, 0.f, 0.f};
+          if (!p.first && wcol + 16 * j + 4 * lg < p.n) before[j] = o[4 * j];
         }
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          if (row < p.m && wcol + 16 * j + 4 * lg < p.n) o[4 * j] = before[j] + acc[i][j];
+        // (16 rows at a time: registers for no more)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       // bf16 through the wave's own LDS, 16 rows at a time, so that a store
@@ -557,6 +569,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
               for (int e = 0; e < 4; ++e)
                 if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = 0.0f;
           }
+          if (i == 0) arrived();
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
@@ -667,7 +680,7 @@ uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 // columns of a piece: 2^26 elements of g, in whole tiles
 uint32_t piece_columns(uint32_t rows, uint32_t vocab) {
   const uint32_t all = (vocab + 255) / 256 * 256;
-  const uint32_t fit = (uint32_t)std::min<uint64_t>((1ull << 26) / rows / 256 * 256, 32768);
+  const uint32_t fit = (uint32_t)std::min<uint64_t>((1ull << 26) / rows / 256 * 256, 65536);
   return std::min(all, std::max(fit, 4096u));
 }
 

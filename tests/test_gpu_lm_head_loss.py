@@ -127,14 +127,14 @@ def test_backward(eng, rows, vocab, hidden):
 
 
 def test_several_pieces_of_the_vocabulary(eng):
-    """More columns than a piece holds (32768 at these few rows), the last
+    """More columns than a piece holds (65536 at these few rows), the last
     piece a short one."""
     import torch
 
     from pih_amd.linear import lm_head_loss, lm_head_loss_backward
 
-    x, w, target, up = _case(3, 37, 32768 * 2 + 1003, 64)
-    target[0], target[1], target[2] = 32767, 32768, 32768 * 2 + 1002
+    x, w, target, up = _case(3, 37, 65536 * 2 + 1003, 64)
+    target[0], target[1], target[2] = 65535, 65536, 65536 * 2 + 1002
     _, _, lse, elog, loss, eloss, _, _ = _ref(x, w, target)
     args = [t.cuda() for t in (x, w, target)]
     got, glse, _ = lm_head_loss(*args)
