@@ -32,7 +32,6 @@ namespace {
 
 constexpr uint32_t kMaxRank = 128;
 constexpr uint32_t kMaxColumns = 1u << 20;
-constexpr uint32_t TR = 16;  // rows of a tile
 constexpr uint32_t kErrAdapter = 1u, kErrOffsets = 2u;
 constexpr uint32_t kNoAdapter = 0xffffffffu;
 
@@ -48,23 +47,24 @@ struct Tile {
   float scale;
 };
 
-// Tile `index` of the segments' 16-row tiles, in order; false past the last.
-// A segment whose offsets descend or pass the rows counts as empty.
-__device__ __forceinline__ bool find_tile(const Segments& p, uint32_t index, Tile& t, uint32_t* err) {
+// Tile `index` of the segments' tiles of `height` rows, in order; false past
+// the last.  A segment whose offsets descend or pass the rows counts as empty.
+__device__ __forceinline__ bool find_tile(const Segments& p, uint32_t height, uint32_t index, Tile& t, uint32_t* err) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t before = 0;
   for (uint32_t s0 = 0; s0 < p.segments; s0 += 64) {
     const uint32_t s = s0 + lane;
-    uint32_t lo = 0, hi = 0;
+    uint32_t lo = 0, hi = 0, adapter = kNoAdapter;
     if (s < p.segments) {
       lo = p.offsets[s];
       hi = p.offsets[s + 1];
+      adapter = p.adapter[s];
       if (hi < lo || hi > p.rows) {
         if (index == 0 && threadIdx.x < 64) atomicOr(err, kErrOffsets);
         hi = lo = 0;
       }
     }
-    const uint32_t n = (hi - lo + TR - 1) / TR;
+    const uint32_t n = (hi - lo + height - 1) / height;
     uint32_t upto = n;
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
@@ -78,9 +78,9 @@ __device__ __forceinline__ bool find_tile(const Segments& p, uint32_t index, Til
       const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), l);
       const uint32_t slo = (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
       const uint32_t shi = (uint32_t)__builtin_amdgcn_readlane((int)hi, l);
-      t.row0 = slo + (index - before - first) * TR;
-      t.rows = min(TR, shi - t.row0);
-      t.adapter = p.adapter[s0 + l];
+      t.row0 = slo + (index - before - first) * height;
+      t.rows = min(height, shi - t.row0);
+      t.adapter = (uint32_t)__builtin_amdgcn_readlane((int)adapter, l);
       t.scale = 1.0f;
       if (t.adapter < p.adapters) {
         if (p.scale) t.scale = p.scale[t.adapter];
@@ -94,19 +94,21 @@ __device__ __forceinline__ bool find_tile(const Segments& p, uint32_t index, Til
   return false;
 }
 
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+
 __device__ __forceinline__ v4i load16(const uint16_t* p) { return *reinterpret_cast<const v4i*>(p); }
 __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
-// eight values `stride` elements apart, those from `count` on as 0
-__device__ __forceinline__ v4i load_column(const uint16_t* p, uint64_t stride, uint32_t count) {
-  v4i v{0, 0, 0, 0};
-#pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) {
-    const uint32_t e = i < count ? p[i * stride] : 0u;
-    v[i / 2] |= (int)(e << (16 * (i & 1)));
-  }
-  return v;
+// An operand whose contraction runs over LDS rows: lane l of 16 points at 4
+// values of row l / 4 and receives value l % 4 of piece l / 4 of the four rows
+// (ds_read_b64_tr_b16); x: the lane's place in rows 0-3 of its eight.
+__device__ __forceinline__ v4i transposed(const uint8_t* x, uint32_t pitch) {
+  const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)x);
+  const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x + 4 * pitch));
+  const uint2 u = __builtin_bit_cast(uint2, a), v = __builtin_bit_cast(uint2, b);
+  return v4i{(int)u.x, (int)u.y, (int)v.x, (int)v.y};
 }
 // fp32 values as bf16 hi + lo, eight of them
 __device__ __forceinline__ void split8(const float* v, v4i& hi, v4i& lo) {
@@ -133,60 +135,131 @@ struct DownParams {
   uint32_t rank;
 };
 
-// One tile of rows times the rank columns of its adapter over a range of
-// cols.  The four waves take 128-column pieces in turn.
-template <int NJ, bool kColumns>
-__device__ void down_tile(const DownParams& p, const DownSide& d, const Tile& t, uint32_t split) {
-  __shared__ float sums[4][TR][NJ * 16 + 4];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = tid >> 6;
-  const uint32_t c0 = split * d.per_split, c1 = min(c0 + d.per_split, d.cols);
-  v4f acc[NJ];
+// One tile of 16 RB rows times the rank columns of its adapter over a range
+// of cols; the four waves take 128-column pieces in turn.  kColumns: 32 rows
+// of the weights (one contiguous piece of memory) go through the wave's LDS
+// and are read transposed.
+template <int NJ, int RB, bool kColumns>
+__device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d, const Tile& t, uint32_t split,
+                                          uint8_t* lds) {
+  constexpr uint32_t kSumRow = NJ * 16 + 4;
+  float* const sums = reinterpret_cast<float*>(lds);  // [4][16][kSumRow]
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t c0 = split * d.per_split, c1 = min(c0 + d.per_split, d.cols), rank = p.rank;
+  v4f acc[RB][NJ];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-  const uint16_t* const src = d.src + (uint64_t)(t.row0 + min(lr, t.rows - 1)) * d.stride;
-  const uint16_t* const w = d.w + (uint64_t)t.adapter * p.rank * d.cols;
-  for (uint32_t c = c0 + 128 * wave; c < c1; c += 512) {
+  for (int r = 0; r < RB; ++r)
 #pragma unroll
-    for (uint32_t q = 0; q < 4; ++q) {
-      const uint32_t at = c + 32 * q + 8 * lg;
-      v4i x{0, 0, 0, 0};
-      if (at < c1) x = load16(src + at);
+    for (int j = 0; j < NJ; ++j) acc[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  const uint16_t* src[RB];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint32_t row = min(16 * j + lr, p.rank - 1);
-        v4i a{0, 0, 0, 0};
-        if (at < c1) {
-          if constexpr (kColumns) a = load_column(w + (uint64_t)at * p.rank + row, p.rank, 8);
-          else a = load16(w + (uint64_t)row * d.cols + at);
+  for (int r = 0; r < RB; ++r) src[r] = d.src + (uint64_t)(t.row0 + min(16 * r + lr, t.rows - 1)) * d.stride;
+  const uint16_t* const w = d.w + (uint64_t)t.adapter * rank * d.cols;
+  if constexpr (!kColumns) {
+    const uint16_t* wr[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) wr[j] = w + (uint64_t)min(16 * j + lr, rank - 1) * d.cols;
+    for (uint32_t c = c0 + 128 * wave; c < c1; c += 512) {
+      // 128 columns together while registers hold them, else 32
+      constexpr int Q = NJ + RB <= 6 ? 4 : 2;
+#pragma unroll
+      for (uint32_t q0 = 0; q0 < 4; q0 += Q) {
+        v4i x[Q][RB], a[Q][NJ];
+#pragma unroll
+        for (uint32_t q = 0; q < Q; ++q) {
+          const uint32_t at = c + 32 * (q0 + q) + 8 * lg;
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            x[q][r] = v4i{0, 0, 0, 0};
+            if (at < c1) x[q][r] = load16(src[r] + at);
+          }
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            a[q][j] = v4i{0, 0, 0, 0};
+            if (at < c1) a[q][j] = load16(wr[j] + at);
+          }
         }
-        acc[j] = mfma(a, x, acc[j]);
+#pragma unroll
+        for (uint32_t q = 0; q < Q; ++q)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a[q][j], x[q][r], acc[r][j]);
       }
     }
+  } else {
+    // LDS rows of 2 rank + 16 bytes; 16-byte piece i of a lane is number
+    // 64 i + lane of the 4 rank pieces of 32 rows
+    const uint32_t pitch = 2 * rank + 16, per_row = rank / 8, pieces = 32 * per_row;
+    uint8_t* const st = lds + wave * 32 * (NJ * 32 + 16);
+    uint32_t put[NJ];
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) {
+      const uint32_t e = min(64 * i + lane, pieces - 1);
+      put[i] = e / per_row * pitch + e % per_row * 16;
+    }
+    for (uint32_t c = c0 + 128 * wave; c < c1; c += 512) {
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        const uint32_t cq = c + 32 * q;
+        if (cq >= c1) break;
+        const uint32_t at = cq + 8 * lg, valid = min(32u, c1 - cq) * per_row;
+        v4i x[RB], m[NJ];
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          x[r] = v4i{0, 0, 0, 0};
+          if (at < c1) x[r] = load16(src[r] + at);
+        }
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) {
+          m[i] = v4i{0, 0, 0, 0};
+          if (64u * i + lane < valid) m[i] = load16(w + (uint64_t)cq * rank + 8 * (64 * i + lane));
+        }
+#pragma unroll
+        for (int i = 0; i < NJ; ++i)
+          if (64u * i + lane < pieces) *reinterpret_cast<v4i*>(st + put[i]) = m[i];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const v4i a = transposed(st + (8 * lg + (lr >> 2)) * pitch + 32 * j + 8 * (lr & 3), pitch);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a, x[r], acc[r][j]);
+        }
+      }
+    }
+    __syncthreads();
   }
+  float* const out = d.out + ((uint64_t)split * p.seg.rows + t.row0) * rank;
 #pragma unroll
-  for (int j = 0; j < NJ; ++j)
+  for (int r = 0; r < RB; ++r) {
+    if (16u * r >= t.rows) break;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][lr][16 * j + 4 * lg + i] = acc[j][i];
-  __syncthreads();
-  float* const out = d.out + ((uint64_t)split * p.seg.rows + t.row0) * p.rank;
-  for (uint32_t i = tid; i < t.rows * p.rank; i += 256) {
-    const uint32_t r = i / p.rank, j = i % p.rank;
-    out[i] = (sums[0][r][j] + sums[1][r][j]) + (sums[2][r][j] + sums[3][r][j]);
+    for (int j = 0; j < NJ; ++j) *reinterpret_cast<v4f*>(sums + (wave * 16 + lr) * kSumRow + 16 * j + 4 * lg) = acc[r][j];
+    __syncthreads();
+    for (uint32_t i = tid; i < min(16u, t.rows - 16 * r) * (rank / 4); i += 256) {
+      const uint32_t row = i / (rank / 4), j = i % (rank / 4) * 4;
+      const float* const from = sums + row * kSumRow + j;
+      auto part = [&](uint32_t v) { return *reinterpret_cast<const v4f*>(from + v * 16 * kSumRow); };
+      *reinterpret_cast<v4f*>(out + (uint64_t)(16 * r + row) * rank + j) = (part(0) + part(1)) + (part(2) + part(3));
+    }
+    __syncthreads();
   }
 }
 
-template <int NJ, bool kBackward>
+template <int NJ, int RB, bool kBackward>
 __global__ __launch_bounds__(256) void adapter_down_kernel(DownParams p) {
+  constexpr uint32_t kSums = 4 * 16 * (NJ * 16 + 4) * 4, kStaged = kBackward ? 4 * 32 * (NJ * 32 + 16) : 0;
+  __shared__ __align__(16) uint8_t lds[kSums > kStaged ? kSums : kStaged];
   Tile t;
   const DownSide& d = p.side[blockIdx.z];
-  if (blockIdx.y >= d.splits || !find_tile(p.seg, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
+  if (blockIdx.y >= d.splits || !find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
   if constexpr (kBackward) {
     if (blockIdx.z) {
-      down_tile<NJ, true>(p, d, t, blockIdx.y);
+      down_tile<NJ, RB, true>(p, d, t, blockIdx.y, lds);
       return;
     }
   }
-  down_tile<NJ, false>(p, d, t, blockIdx.y);
+  down_tile<NJ, RB, false>(p, d, t, blockIdx.y, lds);
 }
 
 // -------------------------------------------------------------------- up
@@ -201,84 +274,139 @@ struct UpParams {
   uint32_t scaled;      // h holds the scale
 };
 
-// out rows of a tile: 64 columns at a time per wave.  Row rho of MFMA u holds
-// column 16 (rho >> 2) + 4 u + (rho & 3), so that a lane's results over the
-// four are 16 consecutive columns.
-template <int KJ, bool kColumns>
-__global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
-  __shared__ float hs[TR][KJ * 32 + 4];
+// out rows of a tile of 16 RB: 64 columns at a time per wave.  Row rho of MFMA
+// u holds column 16 (rho >> 2) + 4 u + (rho & 3), so that a lane's results over
+// the four are 16 consecutive columns.  kColumns: 32 weight rows of the 64
+// columns go through the wave's LDS and are read transposed.
+template <int KJ, int RB, bool kColumns>
+__device__ __forceinline__ void up_tile(const UpParams& p, uint32_t tile, uint32_t column, uint8_t* lds) {
+  constexpr uint32_t kRow = KJ * 32 + 4, kPitch = 128 + 16;
+  float* const hs = reinterpret_cast<float*>(lds);  // [16 RB][kRow]
   Tile t;
-  if (!find_tile(p.seg, blockIdx.x, t, p.err)) return;
+  if (!find_tile(p.seg, 16 * RB, tile, t, p.err)) return;
   if (t.adapter >= p.seg.adapters && t.adapter != kNoAdapter) return;
   const bool live = t.adapter != kNoAdapter;
   if (!live && p.base == p.out) return;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = tid >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), rank = p.rank;
   if (live) {
     const float s = p.scaled ? 1.0f : t.scale;
-    for (uint32_t i = tid; i < TR * KJ * 32; i += 256) {
-      const uint32_t r = i / (KJ * 32), j = i % (KJ * 32);
-      float v = 0.0f;
-      if (r < t.rows && j < p.rank)
-        for (uint32_t q = 0; q < p.splits; ++q) v += p.h[((uint64_t)q * p.seg.rows + t.row0 + r) * p.rank + j];
-      hs[r][j] = v * s;
+    for (uint32_t i = tid; i < 16 * RB * KJ * 8; i += 256) {
+      const uint32_t r = i / (KJ * 8), j = i % (KJ * 8) * 4;
+      v4f v{0.f, 0.f, 0.f, 0.f};
+      if (r < t.rows && j < rank) {
+        const float* from = p.h + (uint64_t)(t.row0 + r) * rank + j;
+        const uint64_t step = (uint64_t)p.seg.rows * rank;
+#pragma unroll 8
+        for (uint32_t q = 0; q < p.splits; ++q) v += *reinterpret_cast<const v4f*>(from + q * step);
+      }
+      *reinterpret_cast<v4f*>(hs + r * kRow + j) = v4f{v[0] * s, v[1] * s, v[2] * s, v[3] * s};
     }
   }
   __syncthreads();
-  v4i hi[KJ], lo[KJ];
+  v4i hi[RB][KJ], lo[RB][KJ];
 #pragma unroll
-  for (int q = 0; q < KJ; ++q)
-    if (live) split8(&hs[lr][32 * q + 8 * lg], hi[q], lo[q]);
-  const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * p.rank * p.cols;
-  const uint32_t g0 = (blockIdx.y * 4 + wave) * p.groups;
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int q = 0; q < KJ; ++q)
+      if (live) split8(hs + (16 * r + lr) * kRow + 32 * q + 8 * lg, hi[r][q], lo[r][q]);
+  const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * rank * p.cols;
+  uint8_t* const st = lds + 16 * RB * kRow * 4 + wave * 32 * kPitch;
+  const uint32_t g0 = (column * 4 + wave) * p.groups;
   for (uint32_t g = g0; g < g0 + p.groups; ++g) {
     const uint32_t c0 = g * 64;
     if (c0 >= p.cols) return;
-    const uint32_t row = t.row0 + lr;
-    const bool in = lr < t.rows;
-    v4i b[2];
+    v4i b[RB][2];
 #pragma unroll
-    for (uint32_t v = 0; v < 2; ++v) {
-      b[v] = v4i{0, 0, 0, 0};
-      const uint32_t c = c0 + 16 * lg + 8 * v;
-      if (p.base && in && c < p.cols) b[v] = load16(p.base + (uint64_t)row * p.base_stride + c);
-    }
-    v4f acc[4];
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) acc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t v = 0; v < 2; ++v) {
+        b[r][v] = v4i{0, 0, 0, 0};
+        const uint32_t c = c0 + 16 * lg + 8 * v;
+        if (p.base && 16 * r + lr < t.rows && c < p.cols)
+          b[r][v] = load16(p.base + (uint64_t)(t.row0 + 16 * r + lr) * p.base_stride + c);
+      }
+    v4f acc[RB][4];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) acc[r][u] = v4f{0.f, 0.f, 0.f, 0.f};
     if (live) {
+      if constexpr (!kColumns) {
+        v4i x[4][KJ];
 #pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
-        const uint32_t c = min(c0 + 16 * (lr >> 2) + 4 * u + (lr & 3), p.cols - 1);
+        for (uint32_t u = 0; u < 4; ++u) {
+          const uint16_t* const row = w + (uint64_t)min(c0 + 16 * (lr >> 2) + 4 * u + (lr & 3), p.cols - 1) * rank;
+#pragma unroll
+          for (int q = 0; q < KJ; ++q) {
+            const uint32_t j = 32 * q + 8 * lg;
+            x[u][q] = v4i{0, 0, 0, 0};
+            if (j < rank) x[u][q] = load16(row + j);
+          }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+          for (int q = 0; q < KJ; ++q)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+              acc[r][u] = mfma(x[u][q], lo[r][q], acc[r][u]);
+              acc[r][u] = mfma(x[u][q], hi[r][q], acc[r][u]);
+            }
+      } else {
 #pragma unroll
         for (int q = 0; q < KJ; ++q) {
-          const uint32_t j = 32 * q + 8 * lg;
-          v4i x{0, 0, 0, 0};
-          if (j < p.rank) {
-            if constexpr (kColumns) x = load_column(w + (uint64_t)j * p.cols + c, p.cols, 8);
-            else x = load16(w + (uint64_t)c * p.rank + j);
+          // instruction i: rows 32 q + 8 i + (lane >> 3), 8 columns a lane
+          const uint32_t c = c0 + 8 * (lane & 7);
+          v4i m[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t j = 32 * q + 8 * i + (lane >> 3);
+            m[i] = v4i{0, 0, 0, 0};
+            if (j < rank && c < p.cols) m[i] = load16(w + (uint64_t)j * p.cols + c);
           }
-          acc[u] = mfma(x, lo[q], acc[u]);
-          acc[u] = mfma(x, hi[q], acc[u]);
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)
+            *reinterpret_cast<v4i*>(st + (8 * i + (lane >> 3)) * kPitch + 16 * (lane & 7)) = m[i];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) {
+            const v4i x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * (lr & 3) + 4 * u), kPitch);
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+              acc[r][u] = mfma(x, lo[r][q], acc[r][u]);
+              acc[r][u] = mfma(x, hi[r][q], acc[r][u]);
+            }
+          }
         }
       }
     }
 #pragma unroll
-    for (uint32_t v = 0; v < 2; ++v) {
-      const uint32_t c = c0 + 16 * lg + 8 * v;
-      v4i o;
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t bits = (uint32_t)b[v][i];
-        const float y0 = acc[2 * v + i / 2][2 * (i & 1)], y1 = acc[2 * v + i / 2][2 * (i & 1) + 1];
-        o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y0, bf16_bits_to_f32(bits >> 16) + y1);
+      for (uint32_t v = 0; v < 2; ++v) {
+        const uint32_t c = c0 + 16 * lg + 8 * v;
+        v4i o;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const uint32_t bits = (uint32_t)b[r][v][i];
+          const float y0 = acc[r][2 * v + i / 2][2 * (i & 1)], y1 = acc[r][2 * v + i / 2][2 * (i & 1) + 1];
+          o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y0, bf16_bits_to_f32(bits >> 16) + y1);
+        }
+        // (without an adapter base goes through bit for bit, a -0 too)
+        if (16 * r + lr < t.rows && c < p.cols)
+          *reinterpret_cast<v4i*>(p.out + (uint64_t)(t.row0 + 16 * r + lr) * p.out_stride + c) = live ? o : b[r][v];
       }
-      // (without an adapter base goes through bit for bit, a -0 too)
-      if (in && c < p.cols) *reinterpret_cast<v4i*>(p.out + (uint64_t)row * p.out_stride + c) = live ? o : b[v];
-    }
   }
 }
 
+template <int KJ, int RB, bool kColumns>
+__global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
+  __shared__ __align__(16) uint8_t lds[16 * RB * (KJ * 32 + 4) * 4 + (kColumns ? 4 * 32 * 144 : 0)];
+  up_tile<KJ, RB, kColumns>(p, blockIdx.x, blockIdx.y, lds);
+}
+
 // ---------------------------------------------------- splits of a backward
+constexpr uint32_t kFinishRows = 16;
 struct FinishParams {
   Segments seg;
   const float* part[2];   // [splits][rows][rank]: x A^T, dy B
@@ -291,13 +419,14 @@ struct FinishParams {
 };
 __global__ __launch_bounds__(256) void adapter_finish_kernel(FinishParams p) {
   Tile t;
-  if (!find_tile(p.seg, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
+  if (!find_tile(p.seg, kFinishRows, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
   const uint32_t side = blockIdx.y;
-  for (uint32_t i = threadIdx.x; i < TR * p.rank; i += 256) {
-    const uint32_t r = i & (TR - 1), j = i / TR;
+  for (uint32_t i = threadIdx.x; i < kFinishRows * p.rank; i += 256) {
+    const uint32_t r = i & (kFinishRows - 1), j = i / kFinishRows;
     if (r >= t.rows) continue;
     const uint64_t row = t.row0 + r;
     float v = 0.0f;
+#pragma unroll 8
     for (uint32_t q = 0; q < p.splits[side]; ++q) v += p.part[side][((uint64_t)q * p.seg.rows + row) * p.rank + j];
     v *= t.scale;
     if (side) p.dh[row * p.rank + j] = v;
@@ -322,87 +451,134 @@ struct GradParams {
   uint32_t rank, row_pitch, splits;
 };
 
-// 64 columns (16 a wave) of one adapter's gradient over its rows, in blocks
-// of 32 rows at multiples of 32; with several splits, every splits-th block.
+// 64 columns of one adapter's gradient over its rows, in blocks of 32 rows at
+// multiples of 32; with several splits, every splits-th group of four blocks.
+// The four waves take the blocks of a group and add up in LDS, in order.  The
+// rows' 64 columns go through the wave's LDS and are read transposed.
 template <int NJ, bool kB>
-__device__ void grad_tile(const GradParams& p, const GradSide& d, uint32_t adapter) {
-  const uint32_t lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4, wave = threadIdx.x >> 6;
-  const uint32_t c0 = blockIdx.x * 64 + wave * 16;
+__device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d, uint32_t adapter, uint8_t* lds) {
+  constexpr uint32_t kPitch = 128 + 16, kSumRow = NJ * 16 + 4;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t c0 = blockIdx.x * 64;
   if (c0 >= d.cols) return;
-  v4f acc[NJ];
+  uint8_t* const st = lds + wave * 32 * kPitch;
+  v4f acc[4][NJ];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-  const uint32_t c = min(c0 + lr, d.cols - 1);
-  uint32_t turn = 0;
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[u][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  const uint32_t c = c0 + 8 * (lane & 7);
+  uint32_t turn = 0;  // of the block, modulo 4 splits
+  const uint32_t mine = 4 * blockIdx.y + wave;
   for (uint32_t s = 0; s < p.seg.segments; ++s) {
     if (p.seg.adapter[s] != adapter) continue;
     const uint32_t lo_row = p.seg.offsets[s], hi_row = p.seg.offsets[s + 1];
-    if (hi_row < lo_row || hi_row > p.seg.rows) continue;
-    for (uint32_t r0 = lo_row & ~31u; r0 < hi_row; r0 += 32) {
-      const bool mine = turn == blockIdx.y;
-      turn = turn + 1 == p.splits ? 0 : turn + 1;
-      if (!mine) continue;
-      const uint32_t r = r0 + 8 * lg;
-      v4i src{0, 0, 0, 0};
-      int mask[4];
+    if (hi_row <= lo_row || hi_row > p.seg.rows) continue;
+    const uint32_t first = lo_row / 32, blocks = (hi_row + 31) / 32 - first, all = 4 * p.splits;
+    for (uint32_t i = (mine + all - turn) % all; i < blocks; i += all) {
+      const uint32_t r0 = (first + i) * 32, r = r0 + 8 * lg;
+      v4i m[4];
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        const bool in = r + i >= lo_row && r + i < hi_row;
-        const uint32_t e = in ? d.src[(uint64_t)(r + i) * d.stride + c] : 0u;
-        src[i / 2] |= (int)(e << (16 * (i & 1)));
-        if (i & 1) mask[i / 2] |= in ? (int)0xffff0000 : 0;
-        else mask[i / 2] = in ? 0xffff : 0;
+      for (uint32_t q = 0; q < 4; ++q) {
+        const uint32_t row = r0 + 8 * q + (lane >> 3);
+        m[q] = v4i{0, 0, 0, 0};
+        if (row >= lo_row && row < hi_row && c < d.cols) m[q] = load16(d.src + (uint64_t)row * d.stride + c);
       }
+      v4i h[NJ], l[NJ], mask;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        mask[q] = (r + 2 * q >= lo_row && r + 2 * q < hi_row ? 0xffff : 0) |
+                  (r + 2 * q + 1 >= lo_row && r + 2 * q + 1 < hi_row ? (int)0xffff0000 : 0);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const uint64_t at = (uint64_t)min(16 * j + lr, p.rank - 1) * p.row_pitch + r;
-        v4i h = load16(d.hi + at), l = load16(d.lo + at);
+        h[j] = load16(d.hi + at) & mask;
+        l[j] = load16(d.lo + at) & mask;
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h[i] &= mask[i];
-          l[i] &= mask[i];
-        }
-        if constexpr (kB) {
-          acc[j] = mfma(l, src, acc[j]);
-          acc[j] = mfma(h, src, acc[j]);
-        } else {
-          acc[j] = mfma(src, l, acc[j]);
-          acc[j] = mfma(src, h, acc[j]);
+      for (uint32_t q = 0; q < 4; ++q)
+        *reinterpret_cast<v4i*>(st + (8 * q + (lane >> 3)) * kPitch + 16 * (lane & 7)) = m[q];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const v4i x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * u + 4 * (lr & 3)), kPitch);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if constexpr (kB) {
+            acc[u][j] = mfma(l[j], x, acc[u][j]);
+            acc[u][j] = mfma(h[j], x, acc[u][j]);
+          } else {
+            acc[u][j] = mfma(x, l[j], acc[u][j]);
+            acc[u][j] = mfma(x, h[j], acc[u][j]);
+          }
         }
       }
     }
+    turn = (turn + blocks) % all;
   }
-  float* const out = p.splits > 1 ? d.part + (uint64_t)blockIdx.y * p.seg.adapters * p.rank * d.cols : d.out;
+  // [64 columns][rank], the waves in order
+  float* const sums = reinterpret_cast<float*>(lds);
+  for (uint32_t v = 0; v < 4; ++v) {
+    __syncthreads();
+    if (wave != v) continue;
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    if constexpr (kB) {
-      // lane: column c0 + lr, ranks 16 j + 4 lg ..
-      const uint32_t rk = 16 * j + 4 * lg;
-      if (c0 + lr < d.cols && rk < p.rank)
-        *reinterpret_cast<v4f*>(out + ((uint64_t)adapter * d.cols + c0 + lr) * p.rank + rk) = acc[j];
-    } else {
-      const uint32_t rk = 16 * j + lr, cc = c0 + 4 * lg;
-      if (rk < p.rank && cc < d.cols)
-        *reinterpret_cast<v4f*>(out + ((uint64_t)adapter * p.rank + rk) * d.cols + cc) = acc[j];
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if constexpr (kB) {  // lane: column 16 u + lr, ranks 16 j + 4 lg ..
+          v4f* const o = reinterpret_cast<v4f*>(sums + (16 * u + lr) * kSumRow + 16 * j + 4 * lg);
+          *o = v ? *o + acc[u][j] : acc[u][j];
+        } else {  // lane: rank 16 j + lr, columns 16 u + 4 lg ..
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float* const o = sums + (16 * u + 4 * lg + e) * kSumRow + 16 * j + lr;
+            *o = v ? *o + acc[u][j][e] : acc[u][j][e];
+          }
+        }
+      }
+  }
+  __syncthreads();
+  float* const out = p.splits > 1 ? d.part + (uint64_t)blockIdx.y * p.seg.adapters * p.rank * d.cols : d.out;
+  const uint32_t cols = min(64u, d.cols - c0);
+  if constexpr (kB) {
+    // one contiguous piece: columns c0 .., rank values each
+    float* const o = out + ((uint64_t)adapter * d.cols + c0) * p.rank;
+    for (uint32_t i = tid; i < cols * (p.rank / 4); i += 256) {
+      const uint32_t col = i / (p.rank / 4), j = i % (p.rank / 4) * 4;
+      *reinterpret_cast<v4f*>(o + 4 * (uint64_t)i) = *reinterpret_cast<const v4f*>(sums + col * kSumRow + j);
+    }
+  } else {
+    for (uint32_t i = tid; i < p.rank * 16; i += 256) {
+      const uint32_t j = i / 16, col = i % 16 * 4;
+      if (col >= cols) continue;
+      const float* const from = sums + col * kSumRow + j;
+      *reinterpret_cast<v4f*>(out + ((uint64_t)adapter * p.rank + j) * d.cols + c0 + col) =
+          v4f{from[0], from[kSumRow], from[2 * kSumRow], from[3 * kSumRow]};
     }
   }
 }
 
 template <int NJ>
 __global__ __launch_bounds__(256) void adapter_grad_kernel(GradParams p) {
+  constexpr uint32_t kStaged = 4 * 32 * 144, kSums = 64 * (NJ * 16 + 4) * 4;
+  __shared__ __align__(16) uint8_t lds[kSums > kStaged ? kSums : kStaged];
   const uint32_t adapter = blockIdx.z >> 1;
-  if (blockIdx.z & 1) grad_tile<NJ, true>(p, p.side[1], adapter);
-  else grad_tile<NJ, false>(p, p.side[0], adapter);
+  if (blockIdx.z & 1) grad_tile<NJ, true>(p, p.side[1], adapter, lds);
+  else grad_tile<NJ, false>(p, p.side[0], adapter, lds);
 }
 
-// the splits of the gradients, in order
-__global__ __launch_bounds__(256) void adapter_grad_reduce_kernel(const float* part, float* out, uint64_t count,
-                                                                  uint32_t splits) {
-  const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+// the splits of the gradients, in order: of A, then (blocks from `first_b`
+// on) of B
+__global__ __launch_bounds__(256) void adapter_grad_reduce_kernel(GradParams p, uint32_t first_b) {
+  const uint32_t side = blockIdx.x >= first_b;
+  const uint64_t count = (uint64_t)p.seg.adapters * p.rank * p.side[side].cols;
+  const uint64_t i = ((uint64_t)(blockIdx.x - side * first_b) * 256 + threadIdx.x) * 4;
   if (i >= count) return;
-  v4f v = *reinterpret_cast<const v4f*>(part + i);
-  for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(part + s * count + i);
-  *reinterpret_cast<v4f*>(out + i) = v;
+  const float* const part = p.side[side].part + i;
+  v4f v = *reinterpret_cast<const v4f*>(part);
+#pragma unroll 4
+  for (uint32_t s = 1; s < p.splits; ++s) v += *reinterpret_cast<const v4f*>(part + s * count);
+  *reinterpret_cast<v4f*>(p.side[side].out + i) = v;
 }
 
 // ------------------------------------------------------------------ host
@@ -414,15 +590,17 @@ bool shape_ok(const AdapterArgs& a) {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
+// row blocks of 16 in a tile: four where segments have 64 rows on average
+uint32_t tile_blocks(const AdapterArgs& a) { return a.rows / 64 >= a.segments ? 4 : 1; }
 // tiles of the segments at most: every segment ends in at most one short one
-uint32_t tile_bound(const AdapterArgs& a) {
-  const uint64_t t = ((uint64_t)a.rows + (uint64_t)std::min(a.segments, a.rows) * (TR - 1)) / TR;
+uint32_t tile_bound(const AdapterArgs& a, uint32_t height) {
+  const uint64_t t = ((uint64_t)a.rows + (uint64_t)std::min(a.segments, a.rows) * (height - 1)) / height;
   return (uint32_t)std::min<uint64_t>(t, a.rows);
 }
-// K splits of the down product: up to two rounds of blocks, 256 columns each
-// at least; `tiles` 16-row tiles
+// K splits of the down product: four rounds of blocks, 256 columns each at
+// least
 uint32_t down_splits(uint32_t tiles, uint32_t cols) {
-  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, 512 / std::max(tiles, 1u)));
+  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, 1024 / std::max(tiles, 1u)));
 }
 uint32_t per_split(uint32_t cols, uint32_t splits) { return ((cols + splits - 1) / splits + 127) / 128 * 128; }
 
@@ -435,14 +613,17 @@ void with_pow2(uint32_t n, F&& f) {
 }
 
 template <bool kColumns>
-void launch_up(UpParams p, uint32_t tiles, hipStream_t s) {
+void launch_up(UpParams p, uint32_t tiles, uint32_t blocks, hipStream_t s) {
   // a wave takes several 64-column groups once the blocks fill the card
   const uint32_t all = (p.cols + 63) / 64;
   p.groups = std::max<uint32_t>(1, std::min<uint32_t>(8, (uint64_t)tiles * all / 4 / 1024));
   const dim3 grid(tiles, (all + 4 * p.groups - 1) / (4 * p.groups));
   with_pow2((p.rank + 31) / 32, [&](auto kj) {
     constexpr int KJ = decltype(kj)::value;
-    if constexpr (KJ <= 4) hipLaunchKernelGGL((adapter_up_kernel<KJ, kColumns>), grid, dim3(256), 0, s, p);
+    if constexpr (KJ <= 4) {
+      if (blocks == 4) hipLaunchKernelGGL((adapter_up_kernel<KJ, 4, kColumns>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((adapter_up_kernel<KJ, 1, kColumns>), grid, dim3(256), 0, s, p);
+    }
   });
 }
 
@@ -450,13 +631,25 @@ Segments segments_of(const AdapterArgs& a) {
   return Segments{a.offsets, a.adapter, a.scale, a.segments, a.rows, a.adapters};
 }
 
+template <bool kBackward>
+void launch_down(const DownParams& d, uint32_t tiles, uint32_t blocks, uint32_t splits, hipStream_t s) {
+  const dim3 grid(tiles, splits, kBackward ? 2 : 1);
+  with_pow2((d.rank + 15) / 16, [&](auto nj) {
+    constexpr int NJ = decltype(nj)::value;
+    if (blocks == 4) hipLaunchKernelGGL((adapter_down_kernel<NJ, 4, kBackward>), grid, dim3(256), 0, s, d);
+    else hipLaunchKernelGGL((adapter_down_kernel<NJ, 1, kBackward>), grid, dim3(256), 0, s, d);
+  });
+}
+
 struct BackwardPlan {
-  uint32_t tiles, splits[2], row_pitch, grad_splits;
+  uint32_t blocks, tiles, finish_tiles, splits[2], row_pitch, grad_splits;
   uint64_t part[2], dh, hi[2], lo[2], grads[2], bytes;
 };
 BackwardPlan backward_plan(const AdapterArgs& a) {
   BackwardPlan p{};
-  p.tiles = tile_bound(a);
+  p.blocks = tile_blocks(a);
+  p.tiles = tile_bound(a, 16 * p.blocks);
+  p.finish_tiles = tile_bound(a, kFinishRows);
   p.splits[0] = down_splits(p.tiles, a.k);
   p.splits[1] = down_splits(p.tiles, a.n);
   p.row_pitch = (a.rows + 31) / 32 * 32;
@@ -485,8 +678,8 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
 
 uint64_t AdapterGemmWorkspaceBytes(uint32_t rows, uint32_t rank, uint32_t k) {
   if (!rows || !rank || rank > kMaxRank || !k) return 0;
-  // as many splits as segments can lead to: at least rows / 16 tiles
-  return (uint64_t)down_splits((rows + TR - 1) / TR, k) * rows * rank * 4;
+  // as many splits as segments can lead to: rows / 64 tiles at least
+  return (uint64_t)down_splits((rows + 63) / 64, k) * rows * rank * 4;
 }
 
 uint64_t AdapterBackwardWorkspaceBytes(const AdapterArgs& a) { return shape_ok(a) ? backward_plan(a).bytes : 0; }
@@ -501,7 +694,7 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   if (!aligned16(a.x) || !aligned16(a.a) || !aligned16(a.b) || !aligned16(a.base) || !aligned16(a.out) ||
       !aligned4(a.scale) || !aligned4(a.offsets) || !aligned4(a.adapter) || !aligned4(a.error_flag))
     return Invalid("adapter_gemm_alignment_invalid");
-  const uint32_t tiles = tile_bound(a), splits = down_splits(tiles, a.k);
+  const uint32_t blocks = tile_blocks(a), tiles = tile_bound(a, 16 * blocks), splits = down_splits(tiles, a.k);
   if (a.workspace_bytes < AdapterGemmWorkspaceBytes(a.rows, a.rank, a.k) || !aligned16(a.workspace))
     return Invalid("adapter_gemm_workspace_invalid");
   St clean = RequireCleanLastError();
@@ -511,10 +704,7 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   d.side[0] = DownSide{a.x, a.a, static_cast<float*>(a.workspace), a.x_stride, a.k, per_split(a.k, splits), splits};
   d.err = a.error_flag;
   d.rank = a.rank;
-  with_pow2((a.rank + 15) / 16, [&](auto nj) {
-    hipLaunchKernelGGL((adapter_down_kernel<decltype(nj)::value, false>), dim3(tiles, splits), dim3(256), 0, a.stream,
-                       d);
-  });
+  launch_down<false>(d, tiles, blocks, splits, a.stream);
   UpParams u{};
   u.seg = d.seg;
   u.h = d.side[0].out;
@@ -527,7 +717,7 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   u.cols = a.n;
   u.base_stride = a.base_stride;
   u.out_stride = a.out_stride;
-  launch_up<false>(u, tiles, a.stream);
+  launch_up<false>(u, tiles, blocks, a.stream);
   return AfterLaunch("adapter_gemm_launch_failed");
 }
 
@@ -557,10 +747,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   d.side[1] = DownSide{a.dy,  a.b, f32(plan.part[1]), a.dy_stride, a.n, per_split(a.n, plan.splits[1]), plan.splits[1]};
   d.err = a.error_flag;
   d.rank = a.rank;
-  with_pow2((a.rank + 15) / 16, [&](auto nj) {
-    hipLaunchKernelGGL((adapter_down_kernel<decltype(nj)::value, true>),
-                       dim3(plan.tiles, std::max(plan.splits[0], plan.splits[1]), 2), dim3(256), 0, a.stream, d);
-  });
+  launch_down<true>(d, plan.tiles, plan.blocks, std::max(plan.splits[0], plan.splits[1]), a.stream);
   FinishParams f{};
   f.seg = d.seg;
   f.dh = f32(plan.dh);
@@ -573,7 +760,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   f.err = a.error_flag;
   f.rank = a.rank;
   f.row_pitch = plan.row_pitch;
-  hipLaunchKernelGGL(adapter_finish_kernel, dim3(plan.tiles, 2), dim3(256), 0, a.stream, f);
+  hipLaunchKernelGGL(adapter_finish_kernel, dim3(plan.finish_tiles, 2), dim3(256), 0, a.stream, f);
   UpParams u{};
   u.seg = d.seg;
   u.h = f.dh;
@@ -587,7 +774,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   u.base_stride = a.base_stride;
   u.out_stride = a.out_stride;
   u.scaled = 1;
-  launch_up<true>(u, plan.tiles, a.stream);
+  launch_up<true>(u, plan.tiles, plan.blocks, a.stream);
   GradParams g{};
   g.seg = d.seg;
   g.rank = a.rank;
@@ -601,12 +788,11 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
                        dim3((std::max(a.n, a.k) + 63) / 64, plan.grad_splits, 2 * a.adapters), dim3(256), 0, a.stream,
                        g);
   });
-  if (plan.grad_splits > 1)
-    for (int s = 0; s < 2; ++s) {
-      const uint64_t count = (uint64_t)a.adapters * a.rank * (s ? a.n : a.k);
-      hipLaunchKernelGGL(adapter_grad_reduce_kernel, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, a.stream,
-                         g.side[s].part, s ? a.db : a.da, count, plan.grad_splits);
-    }
+  if (plan.grad_splits > 1) {
+    auto blocks = [&](uint32_t cols) { return (uint32_t)(((uint64_t)a.adapters * a.rank * cols / 4 + 255) / 256); };
+    hipLaunchKernelGGL(adapter_grad_reduce_kernel, dim3(blocks(a.k) + blocks(a.n)), dim3(256), 0, a.stream, g,
+                       blocks(a.k));
+  }
   return AfterLaunch("adapter_backward_launch_failed");
 }
 
