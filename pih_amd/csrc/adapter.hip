@@ -32,6 +32,7 @@ namespace {
 
 constexpr uint32_t kMaxRank = 128;
 constexpr uint32_t kMaxColumns = 1u << 20;
+constexpr uint32_t kUpRows = 16;
 constexpr uint32_t kErrAdapter = 1u, kErrOffsets = 2u;
 constexpr uint32_t kNoAdapter = 0xffffffffu;
 
@@ -219,12 +220,14 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
 #pragma unroll
         for (int i = 0; i < NJ; ++i)
           if (64u * i + lane < pieces) *reinterpret_cast<v4i*>(st + put[i]) = m[i];
+        wave_lds_order();
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           const v4i a = transposed(st + (8 * lg + (lr >> 2)) * pitch + 32 * j + 8 * (lr & 3), pitch);
 #pragma unroll
           for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a, x[r], acc[r][j]);
         }
+        wave_lds_order();
       }
     }
     __syncthreads();
@@ -270,28 +273,108 @@ struct UpParams {
   const uint16_t* base;
   uint16_t* out;
   uint32_t* err;
-  uint32_t splits, rank, cols, base_stride, out_stride, groups;  // groups of 64 columns per wave
+  uint32_t splits, rank, cols, base_stride, out_stride, groups;  // groups per wave
   uint32_t scaled;      // h holds the scale
 };
 
-// out rows of a tile of 16 RB: 64 columns at a time per wave.  Row rho of MFMA
-// u holds column 16 (rho >> 2) + 4 u + (rho & 3), so that a lane's results over
-// the four are 16 consecutive columns.  kColumns: 32 weight rows of the 64
-// columns go through the wave's LDS and are read transposed.
-template <int KJ, int RB, bool kColumns>
-__device__ __forceinline__ void up_tile(const UpParams& p, uint32_t tile, uint32_t column, uint8_t* lds) {
+// out rows of a 16-row tile: 64 columns ("a group") at a time per wave, the
+// next group's loads under way.  Row rho of MFMA u holds column
+// 16 (rho >> 2) + 4 u + (rho & 3), so that a lane's results over the four are
+// 16 consecutive columns.  kColumns: the weights' rows of the 64 columns go
+// through the wave's LDS and are read transposed.
+template <int KJ, bool kColumns>
+__global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
   constexpr uint32_t kRow = KJ * 32 + 4, kPitch = 128 + 16;
-  float* const hs = reinterpret_cast<float*>(lds);  // [16 RB][kRow]
+  __shared__ __align__(16) float hs[kUpRows * kRow];
+  __shared__ __align__(16) uint8_t staged[kColumns ? 4 * 32 * kPitch : 16];
   Tile t;
-  if (!find_tile(p.seg, 16 * RB, tile, t, p.err)) return;
+  if (!find_tile(p.seg, kUpRows, blockIdx.x, t, p.err)) return;
   if (t.adapter >= p.seg.adapters && t.adapter != kNoAdapter) return;
   const bool live = t.adapter != kNoAdapter;
   if (!live && p.base == p.out) return;
   const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), rank = p.rank;
+  const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * rank * p.cols;
+  uint8_t* const st = staged + (kColumns ? wave * 32 * kPitch : 0);
+  const uint32_t row = t.row0 + min(lr, t.rows - 1);
+  const uint16_t* const base = p.base ? p.base + (uint64_t)row * p.base_stride : nullptr;
+  uint16_t* const out = p.out + (uint64_t)row * p.out_stride;
+  const bool mine = lr < t.rows;
+
+  struct Group {
+    v4i x[KJ][4], b[2];
+  };
+  auto load = [&](uint32_t g, Group& v) __attribute__((always_inline)) {
+    const uint32_t c0 = g * 64;
+#pragma unroll
+    for (int q = 0; q < KJ; ++q)
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        v.x[q][u] = v4i{0, 0, 0, 0};
+        if constexpr (kColumns) {
+          // weight rows 32 q + 8 u + (lane >> 3), 8 columns a lane
+          const uint32_t j = 32 * q + 8 * u + (lane >> 3), c = c0 + 8 * (lane & 7);
+          if (j < rank && c < p.cols) v.x[q][u] = load16(w + (uint64_t)j * p.cols + c);
+        } else {
+          const uint32_t j = 32 * q + 8 * lg, c = c0 + 16 * (lr >> 2) + 4 * u + (lr & 3);
+          if (j < rank && c < p.cols) v.x[q][u] = load16(w + (uint64_t)c * rank + j);
+        }
+      }
+#pragma unroll
+    for (uint32_t v2 = 0; v2 < 2; ++v2) {
+      v.b[v2] = v4i{0, 0, 0, 0};
+      const uint32_t c = c0 + 16 * lg + 8 * v2;
+      if (base && c < p.cols) v.b[v2] = load16(base + c);
+    }
+  };
+  v4i hi[KJ], lo[KJ];
+  auto finish = [&](uint32_t g, Group& v) __attribute__((always_inline)) {
+    const uint32_t c0 = g * 64;
+    v4f acc[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) acc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (live) {
+#pragma unroll
+      for (int q = 0; q < KJ; ++q) {
+        if constexpr (kColumns) {
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u)
+            *reinterpret_cast<v4i*>(st + (8 * u + (lane >> 3)) * kPitch + 16 * (lane & 7)) = v.x[q][u];
+          wave_lds_order();
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+          v4i x = v.x[q][u];
+          if constexpr (kColumns) x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * (lr & 3) + 4 * u), kPitch);
+          acc[u] = mfma(x, lo[q], acc[u]);
+          acc[u] = mfma(x, hi[q], acc[u]);
+        }
+        if constexpr (kColumns) wave_lds_order();
+      }
+    }
+#pragma unroll
+    for (uint32_t v2 = 0; v2 < 2; ++v2) {
+      const uint32_t c = c0 + 16 * lg + 8 * v2;
+      v4i o;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t bits = (uint32_t)v.b[v2][i];
+        const float y0 = acc[2 * v2 + i / 2][2 * (i & 1)], y1 = acc[2 * v2 + i / 2][2 * (i & 1) + 1];
+        o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y0, bf16_bits_to_f32(bits >> 16) + y1);
+      }
+      // (without an adapter base goes through bit for bit, a -0 too)
+      if (mine && c < p.cols) *reinterpret_cast<v4i*>(out + c) = live ? o : v.b[v2];
+    }
+  };
+
+  // the wave's groups: wave, wave + 4, .. of the block's
+  const uint32_t all = (p.cols + 63) / 64, end = min((blockIdx.y + 1) * 4 * p.groups, all);
+  uint32_t g = blockIdx.y * 4 * p.groups + wave;
+  Group even, odd;
+  load(g, even);
   if (live) {
     const float s = p.scaled ? 1.0f : t.scale;
-    for (uint32_t i = tid; i < 16 * RB * KJ * 8; i += 256) {
+    for (uint32_t i = tid; i < kUpRows * KJ * 8; i += 256) {
       const uint32_t r = i / (KJ * 8), j = i % (KJ * 8) * 4;
       v4f v{0.f, 0.f, 0.f, 0.f};
       if (r < t.rows && j < rank) {
@@ -304,105 +387,17 @@ __device__ __forceinline__ void up_tile(const UpParams& p, uint32_t tile, uint32
     }
   }
   __syncthreads();
-  v4i hi[RB][KJ], lo[RB][KJ];
 #pragma unroll
-  for (int r = 0; r < RB; ++r)
-#pragma unroll
-    for (int q = 0; q < KJ; ++q)
-      if (live) split8(hs + (16 * r + lr) * kRow + 32 * q + 8 * lg, hi[r][q], lo[r][q]);
-  const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * rank * p.cols;
-  uint8_t* const st = lds + 16 * RB * kRow * 4 + wave * 32 * kPitch;
-  const uint32_t g0 = (column * 4 + wave) * p.groups;
-  for (uint32_t g = g0; g < g0 + p.groups; ++g) {
-    const uint32_t c0 = g * 64;
-    if (c0 >= p.cols) return;
-    v4i b[RB][2];
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (uint32_t v = 0; v < 2; ++v) {
-        b[r][v] = v4i{0, 0, 0, 0};
-        const uint32_t c = c0 + 16 * lg + 8 * v;
-        if (p.base && 16 * r + lr < t.rows && c < p.cols)
-          b[r][v] = load16(p.base + (uint64_t)(t.row0 + 16 * r + lr) * p.base_stride + c);
-      }
-    v4f acc[RB][4];
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) acc[r][u] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      if constexpr (!kColumns) {
-        v4i x[4][KJ];
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) {
-          const uint16_t* const row = w + (uint64_t)min(c0 + 16 * (lr >> 2) + 4 * u + (lr & 3), p.cols - 1) * rank;
-#pragma unroll
-          for (int q = 0; q < KJ; ++q) {
-            const uint32_t j = 32 * q + 8 * lg;
-            x[u][q] = v4i{0, 0, 0, 0};
-            if (j < rank) x[u][q] = load16(row + j);
-          }
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-          for (int q = 0; q < KJ; ++q)
-#pragma unroll
-            for (int r = 0; r < RB; ++r) {
-              acc[r][u] = mfma(x[u][q], lo[r][q], acc[r][u]);
-              acc[r][u] = mfma(x[u][q], hi[r][q], acc[r][u]);
-            }
-      } else {
-#pragma unroll
-        for (int q = 0; q < KJ; ++q) {
-          // instruction i: rows 32 q + 8 i + (lane >> 3), 8 columns a lane
-          const uint32_t c = c0 + 8 * (lane & 7);
-          v4i m[4];
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t j = 32 * q + 8 * i + (lane >> 3);
-            m[i] = v4i{0, 0, 0, 0};
-            if (j < rank && c < p.cols) m[i] = load16(w + (uint64_t)j * p.cols + c);
-          }
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i)
-            *reinterpret_cast<v4i*>(st + (8 * i + (lane >> 3)) * kPitch + 16 * (lane & 7)) = m[i];
-#pragma unroll
-          for (uint32_t u = 0; u < 4; ++u) {
-            const v4i x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * (lr & 3) + 4 * u), kPitch);
-#pragma unroll
-            for (int r = 0; r < RB; ++r) {
-              acc[r][u] = mfma(x, lo[r][q], acc[r][u]);
-              acc[r][u] = mfma(x, hi[r][q], acc[r][u]);
-            }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (uint32_t v = 0; v < 2; ++v) {
-        const uint32_t c = c0 + 16 * lg + 8 * v;
-        v4i o;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t bits = (uint32_t)b[r][v][i];
-          const float y0 = acc[r][2 * v + i / 2][2 * (i & 1)], y1 = acc[r][2 * v + i / 2][2 * (i & 1) + 1];
-          o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y0, bf16_bits_to_f32(bits >> 16) + y1);
-        }
-        // (without an adapter base goes through bit for bit, a -0 too)
-        if (16 * r + lr < t.rows && c < p.cols)
-          *reinterpret_cast<v4i*>(p.out + (uint64_t)(t.row0 + 16 * r + lr) * p.out_stride + c) = live ? o : b[r][v];
-      }
+  for (int q = 0; q < KJ; ++q)
+    if (live) split8(hs + lr * kRow + 32 * q + 8 * lg, hi[q], lo[q]);
+  while (g < end) {
+    if (g + 4 < end) load(g + 4, odd);
+    finish(g, even);
+    if (g + 4 >= end) break;
+    if (g + 8 < end) load(g + 8, even);
+    finish(g + 4, odd);
+    g += 8;
   }
-}
-
-template <int KJ, int RB, bool kColumns>
-__global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
-  __shared__ __align__(16) uint8_t lds[16 * RB * (KJ * 32 + 4) * 4 + (kColumns ? 4 * 32 * 144 : 0)];
-  up_tile<KJ, RB, kColumns>(p, blockIdx.x, blockIdx.y, lds);
 }
 
 // ---------------------------------------------------- splits of a backward
@@ -499,6 +494,7 @@ __device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d
 #pragma unroll
       for (uint32_t q = 0; q < 4; ++q)
         *reinterpret_cast<v4i*>(st + (8 * q + (lane >> 3)) * kPitch + 16 * (lane & 7)) = m[q];
+      wave_lds_order();
 #pragma unroll
       for (uint32_t u = 0; u < 4; ++u) {
         const v4i x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * u + 4 * (lr & 3)), kPitch);
@@ -513,6 +509,7 @@ __device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d
           }
         }
       }
+      wave_lds_order();
     }
     turn = (turn + blocks) % all;
   }
@@ -597,10 +594,10 @@ uint32_t tile_bound(const AdapterArgs& a, uint32_t height) {
   const uint64_t t = ((uint64_t)a.rows + (uint64_t)std::min(a.segments, a.rows) * (height - 1)) / height;
   return (uint32_t)std::min<uint64_t>(t, a.rows);
 }
-// K splits of the down product: four rounds of blocks, 256 columns each at
-// least
+// K splits of the down product: two rounds of blocks, 256 columns each at
+// least (every block of the up product adds the splits again)
 uint32_t down_splits(uint32_t tiles, uint32_t cols) {
-  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, 1024 / std::max(tiles, 1u)));
+  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, 512 / std::max(tiles, 1u)));
 }
 uint32_t per_split(uint32_t cols, uint32_t splits) { return ((cols + splits - 1) / splits + 127) / 128 * 128; }
 
@@ -613,17 +610,14 @@ void with_pow2(uint32_t n, F&& f) {
 }
 
 template <bool kColumns>
-void launch_up(UpParams p, uint32_t tiles, uint32_t blocks, hipStream_t s) {
-  // a wave takes several 64-column groups once the blocks fill the card
-  const uint32_t all = (p.cols + 63) / 64;
-  p.groups = std::max<uint32_t>(1, std::min<uint32_t>(8, (uint64_t)tiles * all / 4 / 1024));
+void launch_up(UpParams p, const AdapterArgs& a) {
+  // a wave takes several groups once the blocks fill the card twice
+  const uint32_t tiles = tile_bound(a, kUpRows), all = (p.cols + 63) / 64;
+  p.groups = std::max<uint32_t>(1, std::min<uint32_t>(8, (uint64_t)tiles * all / 4 / 512));
   const dim3 grid(tiles, (all + 4 * p.groups - 1) / (4 * p.groups));
   with_pow2((p.rank + 31) / 32, [&](auto kj) {
     constexpr int KJ = decltype(kj)::value;
-    if constexpr (KJ <= 4) {
-      if (blocks == 4) hipLaunchKernelGGL((adapter_up_kernel<KJ, 4, kColumns>), grid, dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((adapter_up_kernel<KJ, 1, kColumns>), grid, dim3(256), 0, s, p);
-    }
+    if constexpr (KJ <= 4) hipLaunchKernelGGL((adapter_up_kernel<KJ, kColumns>), grid, dim3(256), 0, a.stream, p);
   });
 }
 
@@ -717,7 +711,7 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   u.cols = a.n;
   u.base_stride = a.base_stride;
   u.out_stride = a.out_stride;
-  launch_up<false>(u, tiles, blocks, a.stream);
+  launch_up<false>(u, a);
   return AfterLaunch("adapter_gemm_launch_failed");
 }
 
@@ -774,7 +768,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   u.base_stride = a.base_stride;
   u.out_stride = a.out_stride;
   u.scaled = 1;
-  launch_up<true>(u, plan.tiles, plan.blocks, a.stream);
+  launch_up<true>(u, a);
   GradParams g{};
   g.seg = d.seg;
   g.rank = a.rank;

@@ -261,6 +261,11 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
 constexpr int vmcnt_at_most(int n) { return ((n >> 4) << 14) | 0x0F70 | (n & 15); }
 constexpr int kLdsRead = 0xC07F;
 
+// Between LDS writes and reads of other lanes of the same wave: LDS takes a
+// wave's accesses in order, this keeps the compiler from reordering them (or
+// from forwarding a lane's own writes).
+__device__ __forceinline__ void wave_lds_order() { asm volatile("" ::: "memory"); }
+
 template <int kWidth>
 __device__ __forceinline__ float reduce_max_xor(float v) {
 #pragma unroll

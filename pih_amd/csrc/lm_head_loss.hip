@@ -577,6 +577,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
           *reinterpret_cast<uint2*>(st + lr * S::kOutRow + j * 32 + lg * 8) =
               uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
         }
+        wave_lds_order();
 #pragma unroll
         for (uint32_t h = 0; h < 16 / kRowsAt; ++h) {
           const uint32_t q = kRowsAt * h + lane / kLanes, r = wrow + 16 * i + q, c = wcol + 8 * (lane % kLanes);
@@ -586,6 +587,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
           const bool in = EPI == kEpiGrad ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
           if (in) *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c) = o;
         }
+        wave_lds_order();
       }
     }
     if (!more) return;

@@ -11,15 +11,20 @@
 // weights w_j = scale b_j / sum over the k selected (both modes) add
 //   b'_j scale / S (dw_j - sum_i dw_i b_i / S),  S = sum of the selected b.
 //
-// Both passes are one read of the scores (and one write): a wavefront per
-// row, lane l holds experts l, l + 64, ... as the top-k kernel does, the row
-// sums by xor shuffles.  The affinities' sums stay in each wave's registers
-// over its rows, are added over the block's waves in LDS and over the blocks
-// by the second launch, in a fixed order and in fp32; the counts are integer
-// adds, whose order does not show.
+// Both passes are one read of the scores (and one write); what costs is the
+// instructions beside it, so a row is 16 lanes (E <= 256), whose sums are four
+// in-register rotations for four rows at once, or 32 or 64 where a lane would
+// hold more than 16 values.  (A wave per row with its sums by wave shuffles:
+// 28 us for the gradient of 32768 x 256 scores, 62 us for the loss.)  A lane
+// holds 4 neighbouring experts of every 4 LANES.  The affinities' sums stay in
+// each lane's registers over its rows, are added over the block in LDS and over
+// the blocks by the second launch, in a fixed order and in fp32; the counts
+// are integer adds, whose order does not show.  The route weights' part of the
+// gradient is added up per row in LDS, since its places are any experts.
 //
 // Error bits: 1 non-finite score, 2 id >= E, 4 affinities that sum to 0.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "kernels.hpp"
@@ -27,98 +32,180 @@
 namespace pih_amd {
 namespace {
 
-constexpr uint32_t kMaxExperts = 1024, kMaxTopk = 32;
-constexpr uint32_t kWaves = 4;
-// rows per wave below which another block costs more than it saves
-constexpr uint32_t kBlocks = 256;
+constexpr uint32_t kMaxExperts = 1024, kMaxTopk = 32, kNoId = 0xffffffffu;
+constexpr uint32_t kWaves = 4;          // of the gradient's blocks
+constexpr uint32_t kBalanceWaves = 16;  // of the loss's, whose partial sums one block adds up:
+constexpr uint32_t kBlocks = 128;       // few and large
+constexpr float kLog2e = 1.44269504088896340736f;
 
-// b(s) and its derivative
+// log(1 + e) for e in [0, 1]: 2 atanh(z) with z = e / (2 + e) <= 1/3, its
+// series up to z^15 (the next term is 2^-27 of the sum at most)
+__device__ __forceinline__ float log1p01(float e) {
+  const float z = e * __builtin_amdgcn_rcpf(2.0f + e), y = z * z;
+  float s = 1.0f / 15.0f;
+  s = __builtin_fmaf(s, y, 1.0f / 13.0f);
+  s = __builtin_fmaf(s, y, 1.0f / 11.0f);
+  s = __builtin_fmaf(s, y, 1.0f / 9.0f);
+  s = __builtin_fmaf(s, y, 1.0f / 7.0f);
+  s = __builtin_fmaf(s, y, 1.0f / 5.0f);
+  s = __builtin_fmaf(s, y, 1.0f / 3.0f);
+  s = __builtin_fmaf(s, y, 1.0f);
+  return 2.0f * z * s;
+}
+
+// b(s) and its derivative.  2^(s log2 e) by the hardware exponential: off by
+// 2^-23 of itself and |s| 2^-24 from the exponent's rounding.
 template <int MODE>
 __device__ __forceinline__ void affinity(float s, float top, float& b, float& slope) {
   if constexpr (MODE == kRouterSoftmax) {
-    b = expf(s - top);
+    b = __builtin_amdgcn_exp2f((s - top) * kLog2e);
     slope = b;
   } else {
-    const float e = expf(-fabsf(s));  // <= 1
-    const float sp = fmaxf(s, 0.0f) + log1pf(e);
-    const float sig = s >= 0.0f ? 1.0f / (1.0f + e) : e / (1.0f + e);
-    b = sqrtf(sp);
+    const float e = __builtin_amdgcn_exp2f(-fabsf(s) * kLog2e);  // <= 1
+    const float sp = fmaxf(s, 0.0f) + log1p01(e);
+    const float sig = (s >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e);
+    b = __builtin_amdgcn_sqrtf(sp);
     // sigmoid / softplus tends to 1 where both underflow
-    slope = sp > 1e-30f ? 0.5f * sig / b : 0.5f * b;
+    slope = sp > 1e-30f ? 0.5f * sig * __builtin_amdgcn_rcpf(b) : 0.5f * b;
   }
 }
 
-// the row's b, b' and their sum; bits of what is wrong with it (then the sum
-// is 1 and every b is 0)
-template <int MODE, int PER>
-__device__ __forceinline__ uint32_t row_affinities(const float* s, uint32_t lane, uint32_t experts, float (&b)[PER],
-                                                   float (&slope)[PER], float& sum) {
-  float raw[PER], top = -INFINITY;
-  bool finite = true;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const uint32_t e = lane + 64u * j;
-    raw[j] = e < experts ? s[e] : 0.0f;
-    if (e < experts) {
-      finite &= __builtin_isfinite(raw[j]);
-      top = fmaxf(top, raw[j]);
-    }
-  }
-  const bool bad = __builtin_amdgcn_ballot_w64(!finite) != 0;
-  if constexpr (MODE == kRouterSoftmax) top = reduce_max_xor<64>(top);
-  float part = 0.0f;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const uint32_t e = lane + 64u * j;
-    b[j] = slope[j] = 0.0f;
-    if (e < experts && !bad) {
-      affinity<MODE>(raw[j], top, b[j], slope[j]);
-      part += b[j];
-    }
-  }
-  sum = reduce_sum_xor<64>(part);
-  if (bad || sum == 0.0f) {
-    sum = 1.0f;
-    return bad ? 1u : 4u;
-  }
-  return 0u;
+// the sum or maximum over a row's lanes, in every one of them
+template <int ROR>
+__device__ __forceinline__ float rotated(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + ROR, 0xf, 0xf, true));
+}
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
+  v += rotated<8>(v);
+  v += rotated<4>(v);
+  v += rotated<2>(v);
+  v += rotated<1>(v);
+  if constexpr (LANES > 16) v += __shfl_xor(v, 16, 64);
+  if constexpr (LANES > 32) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, rotated<8>(v));
+  v = fmaxf(v, rotated<4>(v));
+  v = fmaxf(v, rotated<2>(v));
+  v = fmaxf(v, rotated<1>(v));
+  if constexpr (LANES > 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+  if constexpr (LANES > 32) v = fmaxf(v, __shfl_xor(v, 32, 64));
+  return v;
 }
 
-template <int MODE, int PER>
-__global__ __launch_bounds__(64 * kWaves) void router_balance_kernel(const float* scores, const uint32_t* ids,
-                                                                     float* part_sum, uint32_t* part_count,
-                                                                     uint32_t* err, uint32_t tokens, uint32_t experts,
-                                                                     uint32_t topk) {
-  __shared__ float sums[kWaves][64 * PER];
-  __shared__ uint32_t counts[64 * PER];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  for (uint32_t e = tid; e < 64 * PER; e += 64 * kWaves) counts[e] = 0;
+// Row t of the wave's, LANES lanes of it: lane i holds experts 4 (LANES q + i)
+// + c, q < Q.  vec: rows are 16-byte aligned.
+template <int MODE, int LANES, int Q>
+struct Row {
+  static constexpr int N = 4 * Q;
+  float b[N], slope[N], top, sum;
+  uint32_t wrong;
+
+  static __device__ __forceinline__ uint32_t expert(int j) {
+    return 4 * (LANES * (j / 4) + (threadIdx.x & (LANES - 1))) + j % 4;
+  }
+  __device__ __forceinline__ void load(const float* s, uint32_t experts, bool vec) {
+    // (raw scores in slope)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const uint32_t e = expert(4 * q);
+      if (vec) {
+        v4f v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (e < experts) v = *reinterpret_cast<const v4f*>(s + e);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) slope[4 * q + c] = v[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) slope[4 * q + c] = e + c < experts ? s[e + c] : -INFINITY;
+      }
+    }
+  }
+  // the affinities, their derivatives and sum; what is wrong with the row
+  // (then the sum is 1 and every affinity 0)
+  __device__ __forceinline__ void work(uint32_t experts) {
+    float bad = 0.0f;
+    top = 0.0f;
+    if constexpr (MODE == kRouterSoftmax) {
+      top = slope[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j) top = fmaxf(top, slope[j]);
+      top = row_max<LANES>(top);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      // 0 for a finite score, else NaN
+      const float nan = slope[j] * 0.0f;
+      bad += expert(j) < experts ? nan : 0.0f;
+    }
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float s = slope[j];
+      affinity<MODE>(s, top, b[j], slope[j]);
+      // (outside the row: -inf, whose derivative is a NaN)
+      if (expert(j) >= experts) b[j] = slope[j] = 0.0f;
+      sum += b[j];
+    }
+    sum = row_sum<LANES>(sum);
+    wrong = row_sum<LANES>(bad) == 0.0f ? (sum == 0.0f ? 4u : 0u) : 1u;
+    if (wrong) {
+      sum = 1.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) b[j] = slope[j] = 0.0f;
+    }
+  }
+};
+
+template <int MODE, int LANES, int Q>
+__global__ __launch_bounds__(64 * kBalanceWaves) void router_balance_kernel(const float* scores, const uint32_t* ids,
+                                                                            float* part_sum, uint32_t* part_count,
+                                                                            uint32_t* err, uint32_t tokens,
+                                                                            uint32_t experts, uint32_t topk, bool vec) {
+  using R = Row<MODE, LANES, Q>;
+  constexpr uint32_t kRows = 64 / LANES, kAll = LANES * R::N;  // rows of a wave, experts held
+  constexpr uint32_t kParts = kBalanceWaves * kRows;
+  constexpr uint32_t kFold = kParts * kAll > 16384 ? 16384 / kAll : kParts;  // partial sums in LDS at a time
+  __shared__ float sums[kFold][kAll];
+  __shared__ uint32_t counts[kAll];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, part = wave * kRows + lane / LANES;
+  for (uint32_t e = tid; e < kAll; e += 64 * kBalanceWaves) counts[e] = 0;
   __syncthreads();
-  float acc[PER];
+  float acc[R::N];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
+  for (int j = 0; j < R::N; ++j) acc[j] = 0.0f;
   uint32_t bad = 0;
-  for (uint32_t t = blockIdx.x * kWaves + wave; t < tokens; t += gridDim.x * kWaves) {
-    if (lane < topk) {
-      const uint32_t id = ids[(uint64_t)t * topk + lane];
+  for (uint32_t t = blockIdx.x * kParts + part; t < tokens; t += gridDim.x * kParts) {
+    R row;
+    row.load(scores + (uint64_t)t * experts, experts, vec);
+    for (uint32_t k = tid & (LANES - 1); k < topk; k += LANES) {
+      const uint32_t id = ids[(uint64_t)t * topk + k];
       if (id < experts) atomicAdd(&counts[id], 1u);
       else bad |= 2u;
     }
-    float b[PER], slope[PER], sum;
-    bad |= row_affinities<MODE, PER>(scores + (uint64_t)t * experts, lane, experts, b, slope, sum);
-    const float inv = 1.0f / sum;
+    row.work(experts);
+    bad |= row.wrong;
+    const float inv = 1.0f / row.sum;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] += b[j] * inv;
+    for (int j = 0; j < R::N; ++j) acc[j] += row.b[j] * inv;
   }
+  // kFold parts at a time, each time added up by expert
+  float total = 0.0f;
+  for (uint32_t p0 = 0; p0 < kParts; p0 += kFold) {
+    __syncthreads();
+    if (part >= p0 && part < p0 + kFold) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) sums[wave][lane + 64u * j] = acc[j];
-  __syncthreads();
-  for (uint32_t e = tid; e < experts; e += 64 * kWaves) {
-    float v = sums[0][e];
-#pragma unroll
-    for (uint32_t w = 1; w < kWaves; ++w) v += sums[w][e];
-    part_sum[(uint64_t)blockIdx.x * experts + e] = v;
-    part_count[(uint64_t)blockIdx.x * experts + e] = counts[e];
+      for (int j = 0; j < R::N; ++j) sums[part - p0][R::expert(j)] = acc[j];
+    }
+    __syncthreads();
+    if (tid < experts)
+      for (uint32_t i = 0; i < kFold; ++i) total += sums[i][tid];
+  }
+  if (tid < experts) {
+    part_sum[(uint64_t)blockIdx.x * experts + tid] = total;
+    part_count[(uint64_t)blockIdx.x * experts + tid] = counts[tid];
   }
   if (bad) atomicOr(err, bad);
 }
@@ -136,6 +223,7 @@ __global__ __launch_bounds__(1024) void router_balance_finish_kernel(const float
   float v = 0.0f;
   uint32_t c = 0;
   if (part < parts)
+#pragma unroll 8
     for (uint32_t i = part; i < blocks; i += parts) {
       v += part_sum[(uint64_t)i * experts + e];
       c += part_count[(uint64_t)i * experts + e];
@@ -164,96 +252,126 @@ __global__ __launch_bounds__(1024) void router_balance_finish_kernel(const float
   }
 }
 
-template <int MODE, int PER>
+template <int MODE, int LANES, int Q>
 __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
     const float* scores, const uint32_t* ids, const uint32_t* counts, const float* loss_grad,
     const float* weights_grad, float* scores_grad, uint32_t* err, uint32_t tokens, uint32_t experts, uint32_t topk,
-    float weight, float scale) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  float g[PER];
+    float weight, float scale, bool vec) {
+  using R = Row<MODE, LANES, Q>;
+  constexpr uint32_t kRows = 64 / LANES, kAll = LANES * R::N, kRoutes = (kMaxTopk + LANES - 1) / LANES;
+  __shared__ __align__(16) float extra[kWaves * kRows][kAll];
+  const uint32_t lane = threadIdx.x & 63u, part = (threadIdx.x >> 6) * kRows + lane / LANES, i = lane & (LANES - 1);
+  float* const mine = extra[part];
+  float g[R::N];
   const float up = loss_grad ? *loss_grad * weight : 0.0f;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const uint32_t e = lane + 64u * j;
+  for (int j = 0; j < R::N; ++j) {
+    const uint32_t e = R::expert(j);
     g[j] = loss_grad && e < experts ? (float)counts[e] * up : 0.0f;
   }
   uint32_t bad = 0;
-  for (uint32_t t = blockIdx.x * kWaves + wave; t < tokens; t += gridDim.x * kWaves) {
-    float b[PER], slope[PER], sum;
-    const uint32_t wrong =
-        row_affinities<MODE, PER>(scores + (uint64_t)t * experts, lane, experts, b, slope, sum);
-    bad |= wrong;
-    const float inv = 1.0f / sum;
-    float dot = 0.0f;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) dot += g[j] * (b[j] * inv);
-    dot = reduce_sum_xor<64>(dot);
-    float d[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) d[j] = slope[j] * inv * (g[j] - dot);
-    uint32_t id = 0xffffffffu;
-    if (lane < topk) {
-      id = ids[(uint64_t)t * topk + lane];
-      if (id >= experts) {
-        bad |= 2u;
-        id = 0xffffffffu;
-      }
-    }
+  for (uint32_t t = blockIdx.x * kWaves * kRows + part; t < tokens; t += gridDim.x * kWaves * kRows) {
+    const float* const s = scores + (uint64_t)t * experts;
+    R row;
+    row.load(s, experts, vec);
+    // lane r of the row holds routes r, r + LANES, ..: id, upstream gradient, score
+    uint32_t id[kRoutes];
+    float dw[kRoutes], chosen[kRoutes];
     if (weights_grad) {
-      // lane r < k holds route r; its b comes from the lane that owns the expert
-      float dw = lane < topk && id != 0xffffffffu ? weights_grad[(uint64_t)t * topk + lane] : 0.0f;
-      float mine = 0.0f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const float v = __shfl(b[j], (int)(id & 63u), 64);
-        if (id != 0xffffffffu && (id >> 6) == (uint32_t)j) mine = v;
-      }
-      const float chosen = reduce_sum_xor<64>(mine);
-      const float scaled = chosen > 0.0f ? 1.0f / chosen : 0.0f;
-      const float back = reduce_sum_xor<64>(dw * (mine * scaled));
-      const float term = scale * scaled * (dw - back);
-      for (uint32_t r = 0; r < topk; ++r) {
-        const uint32_t rid = (uint32_t)__builtin_amdgcn_readlane((int)id, r);
-        if (rid == 0xffffffffu) continue;
-        const float v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, term), r));
-        if ((rid & 63u) == lane) {
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if ((rid >> 6) == (uint32_t)j) d[j] += slope[j] * v;
+      for (uint32_t r = 0; r < kRoutes; ++r) {
+        const uint32_t k = r * LANES + i;
+        id[r] = k < topk ? ids[(uint64_t)t * topk + k] : kNoId;
+        dw[r] = k < topk ? weights_grad[(uint64_t)t * topk + k] : 0.0f;
+        if (id[r] >= experts) {
+          if (k < topk) bad |= 2u;
+          id[r] = kNoId;
+          dw[r] = 0.0f;
         }
       }
-    }
-    float* out = scores_grad + (uint64_t)t * experts;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint32_t e = lane + 64u * j;
-      if (e < experts) out[e] = wrong ? 0.0f : d[j];
+      for (uint32_t r = 0; r < kRoutes; ++r) chosen[r] = id[r] != kNoId ? s[id[r]] : 0.0f;
+    } else {
+      for (uint32_t k = i; k < topk; k += LANES)
+        if (ids[(uint64_t)t * topk + k] >= experts) bad |= 2u;
+    }
+    row.work(experts);
+    bad |= row.wrong;
+    const float inv = 1.0f / row.sum;
+    float dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < R::N; ++j) dot += g[j] * (row.b[j] * inv);
+    dot = row_sum<LANES>(dot);
+    float d[R::N];
+#pragma unroll
+    for (int j = 0; j < R::N; ++j) d[j] = row.slope[j] * inv * (g[j] - dot);
+    if (weights_grad) {
+      float cb[kRoutes], cs[kRoutes], sum = 0.0f, back = 0.0f;
+#pragma unroll
+      for (uint32_t r = 0; r < kRoutes; ++r) {
+        affinity<MODE>(chosen[r], row.top, cb[r], cs[r]);
+        if (id[r] == kNoId || row.wrong) cb[r] = cs[r] = 0.0f;
+        sum += cb[r];
+        back += dw[r] * cb[r];
+      }
+      sum = row_sum<LANES>(sum);
+      back = row_sum<LANES>(back);
+      const float per = sum > 0.0f ? 1.0f / sum : 0.0f, mean = back * per;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) *reinterpret_cast<v4f*>(mine + R::expert(4 * q)) = v4f{0.f, 0.f, 0.f, 0.f};
+      wave_lds_order();
+#pragma unroll
+      for (uint32_t r = 0; r < kRoutes; ++r)
+        if (id[r] != kNoId) atomicAdd(mine + id[r], cs[r] * (scale * per * (dw[r] - mean)));
+      wave_lds_order();
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const v4f v = *reinterpret_cast<const v4f*>(mine + R::expert(4 * q));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) d[4 * q + c] += v[c];
+      }
+    }
+    float* const out = scores_grad + (uint64_t)t * experts;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const uint32_t e = R::expert(4 * q);
+      if (vec) {
+        if (e < experts) *reinterpret_cast<v4f*>(out + e) = v4f{d[4 * q], d[4 * q + 1], d[4 * q + 2], d[4 * q + 3]};
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (e + c < experts) out[e + c] = d[4 * q + c];
+      }
     }
   }
   if (bad) atomicOr(err, bad);
 }
 
-uint32_t balance_blocks(uint32_t tokens) { return std::min(kBlocks, (tokens + kWaves - 1) / kWaves); }
-
 bool shape_ok(uint32_t tokens, uint32_t topk, uint32_t experts) {
   return tokens && experts && experts <= kMaxExperts && topk && topk <= kMaxTopk && topk <= experts;
 }
 
+// lanes of a row and float4s a lane holds
 template <typename F>
-void with_per(uint32_t experts, F&& f) {
-  const uint32_t per = (experts + 63) / 64;
-  if (per <= 1) f(std::integral_constant<int, 1>{});
-  else if (per <= 2) f(std::integral_constant<int, 2>{});
-  else if (per <= 4) f(std::integral_constant<int, 4>{});
-  else if (per <= 8) f(std::integral_constant<int, 8>{});
-  else f(std::integral_constant<int, 16>{});
+void with_row(uint32_t experts, F&& f) {
+  if (experts <= 64) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 128) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
+  else if (experts <= 256) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+  else if (experts <= 512) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
 }
+uint32_t row_lanes(uint32_t experts) { return experts <= 256 ? 16 : experts <= 512 ? 32 : 64; }
+uint32_t balance_blocks(uint32_t tokens, uint32_t experts) {
+  const uint32_t rows = kBalanceWaves * 64 / row_lanes(experts);
+  return std::min(kBlocks, (tokens + rows - 1) / rows);
+}
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
 uint64_t RouterBalanceWorkspaceBytes(uint32_t tokens, uint32_t topk, uint32_t experts) {
   if (!shape_ok(tokens, topk, experts)) return 0;
-  return (uint64_t)balance_blocks(tokens) * experts * 8;
+  return (uint64_t)balance_blocks(tokens, experts) * experts * 8;
 }
 
 St LaunchRouterBalance(const RouterBalanceArgs& a) {
@@ -267,15 +385,16 @@ St LaunchRouterBalance(const RouterBalanceArgs& a) {
     return Invalid("router_balance_workspace_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
-  const uint32_t blocks = balance_blocks(a.tokens);
+  const uint32_t blocks = balance_blocks(a.tokens, a.experts);
+  const bool vec = a.experts % 4 == 0 && aligned16(a.scores);
   float* sums = static_cast<float*>(a.workspace);
   uint32_t* counts = reinterpret_cast<uint32_t*>(sums + (uint64_t)blocks * a.experts);
-  with_per(a.experts, [&](auto per) {
-    constexpr int PER = decltype(per)::value;
-    auto kernel = a.mode == kRouterSoftmax ? router_balance_kernel<kRouterSoftmax, PER>
-                                           : router_balance_kernel<kRouterSqrtSoftplus, PER>;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWaves), 0, a.stream, a.scores, a.ids, sums, counts,
-                       a.error_flag, a.tokens, a.experts, a.topk);
+  with_row(a.experts, [&](auto lanes, auto quads) {
+    constexpr int L = decltype(lanes)::value, Q = decltype(quads)::value;
+    auto kernel = a.mode == kRouterSoftmax ? router_balance_kernel<kRouterSoftmax, L, Q>
+                                           : router_balance_kernel<kRouterSqrtSoftplus, L, Q>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kBalanceWaves), 0, a.stream, a.scores, a.ids, sums, counts,
+                       a.error_flag, a.tokens, a.experts, a.topk, vec);
   });
   const float weight = (float)((double)a.coefficient * a.experts / ((double)a.tokens * a.topk));
   hipLaunchKernelGGL(router_balance_finish_kernel, dim3(1), dim3(1024), 0, a.stream, sums, counts, a.loss, a.counts,
@@ -295,13 +414,14 @@ St LaunchRouterBackward(const RouterBackwardArgs& a) {
   if (!clean.ok()) return clean;
   // of a score's own term: the loss's weight over T
   const float weight = (float)((double)a.coefficient * a.experts / ((double)a.tokens * a.tokens * a.topk));
-  const uint32_t blocks = std::min<uint32_t>(2048, (a.tokens + kWaves - 1) / kWaves);
-  with_per(a.experts, [&](auto per) {
-    constexpr int PER = decltype(per)::value;
-    auto kernel = a.mode == kRouterSoftmax ? router_backward_kernel<kRouterSoftmax, PER>
-                                           : router_backward_kernel<kRouterSqrtSoftplus, PER>;
+  const uint32_t rows = kWaves * 64 / row_lanes(a.experts), blocks = std::min<uint32_t>(2048, (a.tokens + rows - 1) / rows);
+  const bool vec = a.experts % 4 == 0 && aligned16(a.scores) && aligned16(a.scores_grad);
+  with_row(a.experts, [&](auto lanes, auto quads) {
+    constexpr int L = decltype(lanes)::value, Q = decltype(quads)::value;
+    auto kernel = a.mode == kRouterSoftmax ? router_backward_kernel<kRouterSoftmax, L, Q>
+                                           : router_backward_kernel<kRouterSqrtSoftplus, L, Q>;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWaves), 0, a.stream, a.scores, a.ids, a.counts, a.loss_grad,
-                       a.weights_grad, a.scores_grad, a.error_flag, a.tokens, a.experts, a.topk, weight, a.scale);
+                       a.weights_grad, a.scores_grad, a.error_flag, a.tokens, a.experts, a.topk, weight, a.scale, vec);
   });
   return AfterLaunch("router_backward_launch_failed");
 }

@@ -521,23 +521,25 @@ def _launch(entry: str, name: str, *fields) -> None:
 
 def _want(ok: bool, what: str) -> None:
     if not ok:
-        raise ValueError(f"pih_amd: {what}")
+        raise ValueError("pih_amd: " + what)
 
 
 def _adapter_stacks(a, b, scale, offsets, adapters):
-    _want(a.dim() == 3 and b.dim() == 3 and a.shape[0] == b.shape[0] and a.shape[1] == b.shape[2],
-          "adapter stacks are A [adapters, rank, k] and B [adapters, n, rank]")
-    _want(a.dtype == b.dtype == torch.bfloat16, "adapter stacks are bfloat16")
-    _want(scale is None or (scale.dtype == torch.float32 and scale.shape == a.shape[:1]),
+    _want(a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype == torch.bfloat16,
+          "adapter stacks are A [adapters, rank, k] and B [adapters, n, rank], bfloat16")
+    (count, rank, k), (other, n, inner) = a.shape, b.shape
+    _want(count == other and rank == inner, "adapter stacks are A [adapters, rank, k] and B [adapters, n, rank]")
+    _want(scale is None or (scale.dtype == torch.float32 and scale.shape == (count,)),
           "adapter scales are float32 [adapters]")
     _want(offsets.dtype == adapters.dtype == torch.int32 and adapters.dim() == 1 and
           offsets.shape == (adapters.shape[0] + 1,),
           "segment offsets are int32 [segments + 1], segment adapters int32 [segments]")
-    return a.shape[0], a.shape[1], b.shape[1], a.shape[2]
+    return count, rank, n, k
 
 
 def _rows(t, rows: int, cols: int, what: str) -> int:
-    _want(tuple(t.shape) == (rows, cols) and t.dtype == torch.bfloat16, f"{what} is bfloat16 [{rows}, {cols}]")
+    if t.shape != (rows, cols) or t.dtype != torch.bfloat16:
+        raise ValueError(f"pih_amd: {what} is bfloat16 [{rows}, {cols}]")
     return t.stride(0) if rows > 1 else cols
 
 
