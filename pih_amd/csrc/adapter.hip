@@ -23,6 +23,7 @@
 // MFMA operands: the weights (or the rows' side for da) come first, so that a
 // lane's four results are consecutive in memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "kernels.hpp"
@@ -32,7 +33,6 @@ namespace {
 
 constexpr uint32_t kMaxRank = 128;
 constexpr uint32_t kMaxColumns = 1u << 20;
-constexpr uint32_t kUpRows = 16;
 constexpr uint32_t kErrAdapter = 1u, kErrOffsets = 2u;
 constexpr uint32_t kNoAdapter = 0xffffffffu;
 
@@ -249,8 +249,15 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
   }
 }
 
+// blocks of the down kernel that a CU holds, by its registers (nj: 16-column
+// pieces of the rank)
+constexpr int down_occupancy(int nj, int rb) {
+  if (rb == 1) return nj <= 2 ? 6 : nj <= 4 ? 4 : 3;
+  return nj == 1 ? 4 : nj == 2 ? 3 : nj <= 4 ? 2 : 1;
+}
+
 template <int NJ, int RB, bool kBackward>
-__global__ __launch_bounds__(256) void adapter_down_kernel(DownParams p) {
+__global__ __launch_bounds__(256, down_occupancy(NJ, RB)) void adapter_down_kernel(DownParams p) {
   constexpr uint32_t kSums = 4 * 16 * (NJ * 16 + 4) * 4, kStaged = kBackward ? 4 * 32 * (NJ * 32 + 16) : 0;
   __shared__ __align__(16) uint8_t lds[kSums > kStaged ? kSums : kStaged];
   Tile t;
@@ -277,18 +284,22 @@ struct UpParams {
   uint32_t scaled;      // h holds the scale
 };
 
-// out rows of a 16-row tile: 64 columns ("a group") at a time per wave, the
+// out rows of a tile of 16 RB: 64 columns ("a group") at a time per wave, the
 // next group's loads under way.  Row rho of MFMA u holds column
-// 16 (rho >> 2) + 4 u + (rho & 3), so that a lane's results over the four are
-// 16 consecutive columns.  kColumns: the weights' rows of the 64 columns go
-// through the wave's LDS and are read transposed.
-template <int KJ, bool kColumns>
-__global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
+// 32 (u >> 1) + 8 (rho >> 2) + 4 (u & 1) + (rho & 3), so that a lane's results
+// of two MFMAs are 8 consecutive columns and its row's four lanes' 64 bytes.
+// kColumns: the weights' rows of the 64 columns go through the wave's LDS and
+// are read transposed.
+// blocks of the up kernel that a CU holds, by its registers
+constexpr int up_occupancy(int kj, int rb) { return kj == 1 ? (rb == 1 ? 4 : 3) : kj == 2 && rb == 1 ? 3 : 2; }
+
+template <int KJ, int RB, bool kColumns>
+__global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(UpParams p) {
   constexpr uint32_t kRow = KJ * 32 + 4, kPitch = 128 + 16;
-  __shared__ __align__(16) float hs[kUpRows * kRow];
+  __shared__ __align__(16) float hs[16 * RB * kRow];
   __shared__ __align__(16) uint8_t staged[kColumns ? 4 * 32 * kPitch : 16];
   Tile t;
-  if (!find_tile(p.seg, kUpRows, blockIdx.x, t, p.err)) return;
+  if (!find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err)) return;
   if (t.adapter >= p.seg.adapters && t.adapter != kNoAdapter) return;
   const bool live = t.adapter != kNoAdapter;
   if (!live && p.base == p.out) return;
@@ -296,13 +307,16 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), rank = p.rank;
   const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * rank * p.cols;
   uint8_t* const st = staged + (kColumns ? wave * 32 * kPitch : 0);
-  const uint32_t row = t.row0 + min(lr, t.rows - 1);
-  const uint16_t* const base = p.base ? p.base + (uint64_t)row * p.base_stride : nullptr;
-  uint16_t* const out = p.out + (uint64_t)row * p.out_stride;
-  const bool mine = lr < t.rows;
+  uint64_t base_row[RB], out_row[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const uint32_t row = t.row0 + min(16 * r + lr, t.rows - 1);
+    base_row[r] = (uint64_t)row * p.base_stride;
+    out_row[r] = (uint64_t)row * p.out_stride;
+  }
 
   struct Group {
-    v4i x[KJ][4], b[2];
+    v4i x[KJ][4], b[RB][2];
   };
   auto load = [&](uint32_t g, Group& v) __attribute__((always_inline)) {
     const uint32_t c0 = g * 64;
@@ -316,23 +330,27 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
           const uint32_t j = 32 * q + 8 * u + (lane >> 3), c = c0 + 8 * (lane & 7);
           if (j < rank && c < p.cols) v.x[q][u] = load16(w + (uint64_t)j * p.cols + c);
         } else {
-          const uint32_t j = 32 * q + 8 * lg, c = c0 + 16 * (lr >> 2) + 4 * u + (lr & 3);
+          const uint32_t j = 32 * q + 8 * lg, c = c0 + 32 * (u >> 1) + 8 * (lr >> 2) + 4 * (u & 1) + (lr & 3);
           if (j < rank && c < p.cols) v.x[q][u] = load16(w + (uint64_t)c * rank + j);
         }
       }
 #pragma unroll
-    for (uint32_t v2 = 0; v2 < 2; ++v2) {
-      v.b[v2] = v4i{0, 0, 0, 0};
-      const uint32_t c = c0 + 16 * lg + 8 * v2;
-      if (base && c < p.cols) v.b[v2] = load16(base + c);
-    }
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        v.b[r][h] = v4i{0, 0, 0, 0};
+        const uint32_t c = c0 + 32 * h + 8 * lg;
+        if (p.base && c < p.cols) v.b[r][h] = load16(p.base + base_row[r] + c);
+      }
   };
-  v4i hi[KJ], lo[KJ];
+  v4i hi[RB][KJ], lo[RB][KJ];
   auto finish = [&](uint32_t g, Group& v) __attribute__((always_inline)) {
     const uint32_t c0 = g * 64;
-    v4f acc[4];
+    v4f acc[RB][4];
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) acc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) acc[r][u] = v4f{0.f, 0.f, 0.f, 0.f};
     if (live) {
 #pragma unroll
       for (int q = 0; q < KJ; ++q) {
@@ -345,26 +363,33 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
           v4i x = v.x[q][u];
-          if constexpr (kColumns) x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * (lr & 3) + 4 * u), kPitch);
-          acc[u] = mfma(x, lo[q], acc[u]);
-          acc[u] = mfma(x, hi[q], acc[u]);
+          if constexpr (kColumns)
+            x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (32 * (u >> 1) + 8 * (lr & 3) + 4 * (u & 1)), kPitch);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            acc[r][u] = mfma(x, lo[r][q], acc[r][u]);
+            acc[r][u] = mfma(x, hi[r][q], acc[r][u]);
+          }
         }
         if constexpr (kColumns) wave_lds_order();
       }
     }
 #pragma unroll
-    for (uint32_t v2 = 0; v2 < 2; ++v2) {
-      const uint32_t c = c0 + 16 * lg + 8 * v2;
-      v4i o;
+    for (int r = 0; r < RB; ++r)
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t bits = (uint32_t)v.b[v2][i];
-        const float y0 = acc[2 * v2 + i / 2][2 * (i & 1)], y1 = acc[2 * v2 + i / 2][2 * (i & 1) + 1];
-        o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y0, bf16_bits_to_f32(bits >> 16) + y1);
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t c = c0 + 32 * h + 8 * lg;
+        v4i o;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const uint32_t bits = (uint32_t)v.b[r][h][i];
+          const v4f y = acc[r][2 * h + i / 2];
+          o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y[2 * (i & 1)],
+                                      bf16_bits_to_f32(bits >> 16) + y[2 * (i & 1) + 1]);
+        }
+        // (without an adapter base goes through bit for bit, a -0 too)
+        if (16 * r + lr < t.rows && c < p.cols) *reinterpret_cast<v4i*>(p.out + out_row[r] + c) = live ? o : v.b[r][h];
       }
-      // (without an adapter base goes through bit for bit, a -0 too)
-      if (mine && c < p.cols) *reinterpret_cast<v4i*>(out + c) = live ? o : v.b[v2];
-    }
   };
 
   // the wave's groups: wave, wave + 4, .. of the block's
@@ -374,7 +399,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
   load(g, even);
   if (live) {
     const float s = p.scaled ? 1.0f : t.scale;
-    for (uint32_t i = tid; i < kUpRows * KJ * 8; i += 256) {
+    for (uint32_t i = tid; i < 16 * RB * KJ * 8; i += 256) {
       const uint32_t r = i / (KJ * 8), j = i % (KJ * 8) * 4;
       v4f v{0.f, 0.f, 0.f, 0.f};
       if (r < t.rows && j < rank) {
@@ -388,8 +413,10 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(UpParams p) {
   }
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < KJ; ++q)
-    if (live) split8(hs + lr * kRow + 32 * q + 8 * lg, hi[q], lo[q]);
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int q = 0; q < KJ; ++q)
+      if (live) split8(hs + (16 * r + lr) * kRow + 32 * q + 8 * lg, hi[r][q], lo[r][q]);
   while (g < end) {
     if (g + 4 < end) load(g + 4, odd);
     finish(g, even);
@@ -594,10 +621,11 @@ uint32_t tile_bound(const AdapterArgs& a, uint32_t height) {
   const uint64_t t = ((uint64_t)a.rows + (uint64_t)std::min(a.segments, a.rows) * (height - 1)) / height;
   return (uint32_t)std::min<uint64_t>(t, a.rows);
 }
-// K splits of the down product: two rounds of blocks, 256 columns each at
-// least (every block of the up product adds the splits again)
-uint32_t down_splits(uint32_t tiles, uint32_t cols) {
-  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, 512 / std::max(tiles, 1u)));
+// K splits of the down product: what the card holds at once (a short second
+// round costs as much as a full one), 256 columns each at least
+uint32_t down_splits(uint32_t tiles, uint32_t cols, uint32_t rank, uint32_t blocks, uint32_t sides) {
+  const uint32_t held = kCus * down_occupancy((rank + 15) / 16, blocks);
+  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, held / std::max(sides * tiles, 1u)));
 }
 uint32_t per_split(uint32_t cols, uint32_t splits) { return ((cols + splits - 1) / splits + 127) / 128 * 128; }
 
@@ -611,13 +639,28 @@ void with_pow2(uint32_t n, F&& f) {
 
 template <bool kColumns>
 void launch_up(UpParams p, const AdapterArgs& a) {
-  // a wave takes several groups once the blocks fill the card twice
-  const uint32_t tiles = tile_bound(a, kUpRows), all = (p.cols + 63) / 64;
-  p.groups = std::max<uint32_t>(1, std::min<uint32_t>(8, (uint64_t)tiles * all / 4 / 512));
-  const dim3 grid(tiles, (all + 4 * p.groups - 1) / (4 * p.groups));
+  // column blocks for three rounds of what the card holds: a wave then takes
+  // several groups where there are many tiles, and the last round costs little
+  const uint32_t blocks = tile_blocks(a) == 4 && p.rank <= 64 ? 2 : 1;
+  const uint32_t tiles = tile_bound(a, 16 * blocks), all = (p.cols + 63) / 64;
   with_pow2((p.rank + 31) / 32, [&](auto kj) {
     constexpr int KJ = decltype(kj)::value;
-    if constexpr (KJ <= 4) hipLaunchKernelGGL((adapter_up_kernel<KJ, kColumns>), grid, dim3(256), 0, a.stream, p);
+    if constexpr (KJ <= 4) {
+      auto launch = [&](auto rb) {
+        constexpr int RB = decltype(rb)::value;
+        const uint32_t columns = std::max<uint32_t>(1, 3 * kCus * up_occupancy(KJ, RB) / tiles);
+        p.groups = std::max<uint32_t>(1, (all + 4 * columns - 1) / (4 * columns));
+        const dim3 grid(tiles, (all + 4 * p.groups - 1) / (4 * p.groups));
+        hipLaunchKernelGGL((adapter_up_kernel<KJ, RB, kColumns>), grid, dim3(256), 0, a.stream, p);
+      };
+      if constexpr (KJ <= 2) {
+        if (blocks == 2) {
+          launch(std::integral_constant<int, 2>{});
+          return;
+        }
+      }
+      launch(std::integral_constant<int, 1>{});
+    }
   });
 }
 
@@ -644,8 +687,8 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   p.blocks = tile_blocks(a);
   p.tiles = tile_bound(a, 16 * p.blocks);
   p.finish_tiles = tile_bound(a, kFinishRows);
-  p.splits[0] = down_splits(p.tiles, a.k);
-  p.splits[1] = down_splits(p.tiles, a.n);
+  p.splits[0] = down_splits(p.tiles, a.k, a.rank, p.blocks, 2);
+  p.splits[1] = down_splits(p.tiles, a.n, a.rank, p.blocks, 2);
   p.row_pitch = (a.rows + 31) / 32 * 32;
   // row splits of the gradients: two rounds of blocks, 256 rows each at least
   const uint64_t blocks = (uint64_t)a.adapters * ((a.n + 63) / 64 + (a.k + 63) / 64);
@@ -672,8 +715,9 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
 
 uint64_t AdapterGemmWorkspaceBytes(uint32_t rows, uint32_t rank, uint32_t k) {
   if (!rows || !rank || rank > kMaxRank || !k) return 0;
-  // as many splits as segments can lead to: rows / 64 tiles at least
-  return (uint64_t)down_splits((rows + 63) / 64, k) * rows * rank * 4;
+  // as many splits as any segments lead to: a tile per 64 or 16 rows at least
+  const uint32_t splits = std::max(down_splits((rows + 63) / 64, k, rank, 4, 1), down_splits((rows + 15) / 16, k, rank, 1, 1));
+  return (uint64_t)splits * rows * rank * 4;
 }
 
 uint64_t AdapterBackwardWorkspaceBytes(const AdapterArgs& a) { return shape_ok(a) ? backward_plan(a).bytes : 0; }
@@ -688,7 +732,8 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   if (!aligned16(a.x) || !aligned16(a.a) || !aligned16(a.b) || !aligned16(a.base) || !aligned16(a.out) ||
       !aligned4(a.scale) || !aligned4(a.offsets) || !aligned4(a.adapter) || !aligned4(a.error_flag))
     return Invalid("adapter_gemm_alignment_invalid");
-  const uint32_t blocks = tile_blocks(a), tiles = tile_bound(a, 16 * blocks), splits = down_splits(tiles, a.k);
+  const uint32_t blocks = tile_blocks(a), tiles = tile_bound(a, 16 * blocks);
+  const uint32_t splits = down_splits(tiles, a.k, a.rank, blocks, 1);
   if (a.workspace_bytes < AdapterGemmWorkspaceBytes(a.rows, a.rank, a.k) || !aligned16(a.workspace))
     return Invalid("adapter_gemm_workspace_invalid");
   St clean = RequireCleanLastError();
