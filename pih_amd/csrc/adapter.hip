@@ -16,9 +16,9 @@
 // is off by its own rounding only.
 //
 // The backward runs both downs (x A^T and dy B) in one launch, then sums the
-// splits once, into [row][rank] for the up product with A and into bf16 hi
-// and lo with the rows innermost for the gradients of A and B, whose
-// contraction runs over the rows.
+// splits once, into [row][rank] for the up product with A and into three bf16
+// parts (all 24 bits: these gradients are fp32) with the rows innermost for
+// the gradients of A and B, whose contraction runs over the rows.
 //
 // MFMA operands: the weights (or the rows' side for da) come first, so that a
 // lane's four results are consecutive in memory.
@@ -433,8 +433,7 @@ struct FinishParams {
   Segments seg;
   const float* part[2];   // [splits][rows][rank]: x A^T, dy B
   float* dh;              // [rows][rank], scaled
-  uint16_t* hi[2];        // [rank][row_pitch], scaled, bf16 hi ...
-  uint16_t* lo[2];        // ... and lo
+  uint16_t* parts[2];     // [3][rank][row_pitch], scaled: three bf16 that add up to the value
   uint32_t* err;
   uint32_t splits[2];
   uint32_t rank, row_pitch;
@@ -452,17 +451,20 @@ __global__ __launch_bounds__(256) void adapter_finish_kernel(FinishParams p) {
     for (uint32_t q = 0; q < p.splits[side]; ++q) v += p.part[side][((uint64_t)q * p.seg.rows + row) * p.rank + j];
     v *= t.scale;
     if (side) p.dh[row * p.rank + j] = v;
-    const uint32_t h = f32_to_bf16_bits(v);
-    p.hi[side][(uint64_t)j * p.row_pitch + row] = (uint16_t)h;
-    p.lo[side][(uint64_t)j * p.row_pitch + row] = (uint16_t)f32_to_bf16_bits(v - bf16_bits_to_f32(h));
+    uint16_t* const part = p.parts[side] + (uint64_t)j * p.row_pitch + row;
+#pragma unroll
+    for (uint32_t q = 0; q < 3; ++q) {
+      const uint32_t h = f32_to_bf16_bits(v);
+      part[(uint64_t)q * p.rank * p.row_pitch] = (uint16_t)h;
+      v -= bf16_bits_to_f32(h);
+    }
   }
 }
 
 // ------------------------------------------------- gradients of A and of B
 struct GradSide {
   const uint16_t* src;   // [rows][cols]: x for A, dy for B
-  const uint16_t* hi;    // [rank][row_pitch]
-  const uint16_t* lo;
+  const uint16_t* parts; // [3][rank][row_pitch]
   float* out;            // [adapters][rank][cols], or (B) [adapters][cols][rank]
   float* part;           // [splits] of those when the rows are split
   uint32_t stride, cols;
@@ -507,16 +509,16 @@ __device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d
         m[q] = v4i{0, 0, 0, 0};
         if (row >= lo_row && row < hi_row && c < d.cols) m[q] = load16(d.src + (uint64_t)row * d.stride + c);
       }
-      v4i h[NJ], l[NJ], mask;
+      v4i h[3][NJ], mask;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         mask[q] = (r + 2 * q >= lo_row && r + 2 * q < hi_row ? 0xffff : 0) |
                   (r + 2 * q + 1 >= lo_row && r + 2 * q + 1 < hi_row ? (int)0xffff0000 : 0);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const uint64_t at = (uint64_t)min(16 * j + lr, p.rank - 1) * p.row_pitch + r;
-        h[j] = load16(d.hi + at) & mask;
-        l[j] = load16(d.lo + at) & mask;
+        const uint16_t* const from = d.parts + (uint64_t)min(16 * j + lr, p.rank - 1) * p.row_pitch + r;
+#pragma unroll
+        for (uint32_t q = 0; q < 3; ++q) h[q][j] = load16(from + (uint64_t)q * p.rank * p.row_pitch) & mask;
       }
 #pragma unroll
       for (uint32_t q = 0; q < 4; ++q)
@@ -527,13 +529,8 @@ __device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d
         const v4i x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * u + 4 * (lr & 3)), kPitch);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          if constexpr (kB) {
-            acc[u][j] = mfma(l[j], x, acc[u][j]);
-            acc[u][j] = mfma(h[j], x, acc[u][j]);
-          } else {
-            acc[u][j] = mfma(x, l[j], acc[u][j]);
-            acc[u][j] = mfma(x, h[j], acc[u][j]);
-          }
+#pragma unroll
+          for (int q = 2; q >= 0; --q) acc[u][j] = kB ? mfma(h[q][j], x, acc[u][j]) : mfma(x, h[q][j], acc[u][j]);
         }
       }
       wave_lds_order();
@@ -680,7 +677,7 @@ void launch_down(const DownParams& d, uint32_t tiles, uint32_t blocks, uint32_t 
 
 struct BackwardPlan {
   uint32_t blocks, tiles, finish_tiles, splits[2], row_pitch, grad_splits;
-  uint64_t part[2], dh, hi[2], lo[2], grads[2], bytes;
+  uint64_t part[2], dh, parts[2], grads[2], bytes;
 };
 BackwardPlan backward_plan(const AdapterArgs& a) {
   BackwardPlan p{};
@@ -701,10 +698,7 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   };
   for (int s = 0; s < 2; ++s) p.part[s] = take((uint64_t)p.splits[s] * a.rows * a.rank * 4);
   p.dh = take((uint64_t)a.rows * a.rank * 4);
-  for (int s = 0; s < 2; ++s) {
-    p.hi[s] = take((uint64_t)a.rank * p.row_pitch * 2);
-    p.lo[s] = take((uint64_t)a.rank * p.row_pitch * 2);
-  }
+  for (int s = 0; s < 2; ++s) p.parts[s] = take(3ull * a.rank * p.row_pitch * 2);
   if (p.grad_splits > 1)
     for (int s = 0; s < 2; ++s) p.grads[s] = take((uint64_t)p.grad_splits * a.adapters * a.rank * (s ? a.n : a.k) * 4);
   p.bytes = at;
@@ -793,8 +787,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   for (int s = 0; s < 2; ++s) {
     f.part[s] = d.side[s].out;
     f.splits[s] = plan.splits[s];
-    f.hi[s] = u16(plan.hi[s]);
-    f.lo[s] = u16(plan.lo[s]);
+    f.parts[s] = u16(plan.parts[s]);
   }
   f.err = a.error_flag;
   f.rank = a.rank;
@@ -820,8 +813,8 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   g.row_pitch = plan.row_pitch;
   g.splits = plan.grad_splits;
   // da = dh^T x, db = dy^T h
-  g.side[0] = GradSide{a.x, f.hi[1], f.lo[1], a.da, f32(plan.grads[0]), a.x_stride, a.k};
-  g.side[1] = GradSide{a.dy, f.hi[0], f.lo[0], a.db, f32(plan.grads[1]), a.dy_stride, a.n};
+  g.side[0] = GradSide{a.x, f.parts[1], a.da, f32(plan.grads[0]), a.x_stride, a.k};
+  g.side[1] = GradSide{a.dy, f.parts[0], a.db, f32(plan.grads[1]), a.dy_stride, a.n};
   with_pow2((a.rank + 15) / 16, [&](auto nj) {
     hipLaunchKernelGGL((adapter_grad_kernel<decltype(nj)::value>),
                        dim3((std::max(a.n, a.k) + 63) / 64, plan.grad_splits, 2 * a.adapters), dim3(256), 0, a.stream,

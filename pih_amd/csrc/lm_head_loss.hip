@@ -10,10 +10,17 @@
 // row's pairs.  Backward: pieces of the vocabulary.  For a piece the logits
 // are computed again and leave as g, bf16 [rows][piece] in the workspace
 // (128 MB at most, so that it stays in the memory-side cache between its
-// writer and its two readers), then dw of the piece is g^T x, and dx grows by
-// g W_piece in fp32.  g is rounded to bf16 for the matrix cores: 2^-9 of each
-// element at most, independent over the sums of rows or vocabulary that the
-// results are, which are themselves rounded to bf16 once.
+// writer and its two readers), then dw of the piece is g^T x, and dx
+// grows by g W_piece in fp32.
+//
+// g is rounded to bf16 for the matrix cores: 2^-9 of each element at most,
+// independent from element to element, in sums that are rounded to bf16 once
+// themselves.  Of the upstream factors up_t = s 2^e m, with s the largest and
+// 1 <= |m| < 2, g holds m alone; 2^e goes into the x of dw's product, exactly,
+// s into dw in fp32, and up_t / m into dx in fp32.  So a mean's equal factors
+// (1 / rows, whose rounding would be the same error in every element) are
+// exact.  (All of up_t rounded inside g: dx and dw off by 0.34 % of their norm,
+// 0.17 % of it bf16 results' own.)
 //
 // Rows without a target take no part in the gradients: their g is 0, and the
 // x of dw's product is a copy with those rows as zeros, so that nothing an
@@ -48,7 +55,8 @@ struct GemmArgs {
   // entries from v0 on
   const uint32_t* target;
   const float* lse;
-  const float* up;
+  const float* mantissa;  // kEpiGrad: [m]
+  const float* scale;   // kEpiBf16: factor of the result
   float2* stats;        // [m][stat_tiles]
   float* target_logit;  // [m]
   uint32_t v0, vocab, stat_tiles, first;
@@ -145,11 +153,11 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
         if (row >= p.m) continue;
         const uint32_t target = p.target[row], at = p.v0 + col;
         float g = 0.0f;
-        if (target < p.vocab && col < p.n) g = p.up[row] * (expf(v - p.lse[row]) - (target == at ? 1.0f : 0.0f));
+        if (target < p.vocab && col < p.n) g = p.mantissa[row] * (expf(v - p.lse[row]) - (target == at ? 1.0f : 0.0f));
         static_cast<uint16_t*>(p.out)[(uint64_t)row * p.ldo + col] = (uint16_t)f32_to_bf16_bits(g);
       } else if (row < p.m && col < p.n) {
         const uint64_t o = (uint64_t)row * p.ldo + col;
-        if constexpr (EPI == kEpiBf16) static_cast<uint16_t*>(p.out)[o] = (uint16_t)f32_to_bf16_bits(v);
+        if constexpr (EPI == kEpiBf16) static_cast<uint16_t*>(p.out)[o] = (uint16_t)f32_to_bf16_bits(v * *p.scale);
         else static_cast<float*>(p.out)[o] = p.first ? v : static_cast<float*>(p.out)[o] + v;
       }
     }
@@ -192,7 +200,8 @@ struct BigArgs {
   uint64_t split_stride;   // kEpiAdd: elements between the splits' sums
   const uint32_t* target;
   const float* lse;
-  const float* up;
+  const float* mantissa;   // kEpiGrad: [m]
+  const float* scale;      // kEpiBf16: factor of the result
   float2* stats;
   float* target_logit;
   uint32_t v0, vocab, first;
@@ -235,7 +244,7 @@ struct BigShape {
   static constexpr int LA = ROWS / 32, LB = 8, NL = LA + LB;         // DMAs per wave and step
   static constexpr uint32_t kOutRow = 16 * NB * 2 + 16;              // a wave's staged output row
   static constexpr uint32_t kOut = ST * kStage;                      // 16 of them per wave
-  static constexpr uint32_t kMeta = kOut + 4 * 16 * kOutRow;         // per row: two tiles' targets, lse, up
+  static constexpr uint32_t kMeta = kOut + 4 * 16 * kOutRow;         // per row: two tiles' targets, lse, mantissas
   static constexpr uint32_t kLds = kMeta + 2 * ROWS * 12;
   static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -297,8 +306,8 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       dma16(sb, ob, lds + S::kA + i * 4096);
     }
   };
-  // tile t and its first steps sent for; its rows' targets and factors into
-  // half `which` of the panel (0 for a row that has no target: g is 0)
+  // tile t and its first steps sent for; its rows' targets, log-sum-exps and
+  // mantissas into half `which` of the panel (kNoTarget for every row whose g is 0)
   auto start = [&](uint32_t which) __attribute__((always_inline)) {
     split = t % p.splits;
     const uint32_t u = t / p.splits, strip = u / (8 * p.n_tiles), in_strip = u % (8 * p.n_tiles);
@@ -327,11 +336,10 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         const uint32_t row = m0 + tid;
         uint32_t* const meta = reinterpret_cast<uint32_t*>(smem + S::kMeta + which * ROWS * 12);
         const uint32_t y = row < p.m ? p.target[row] : kNoTarget;
-        meta[tid] = y;
+        meta[tid] = y < p.vocab ? y : kNoTarget;
         if constexpr (EPI == kEpiGrad) {
-          const bool live = y < p.vocab;
-          meta[ROWS + tid] = __float_as_uint(live ? p.lse[row] : 0.0f);
-          meta[2 * ROWS + tid] = __float_as_uint(live ? p.up[row] : 0.0f);
+          meta[ROWS + tid] = __float_as_uint(row < p.m ? p.lse[row] : 0.0f);
+          meta[2 * ROWS + tid] = __float_as_uint(row < p.m ? p.mantissa[row] : 1.0f);
         }
       }
     }
@@ -544,23 +552,33 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       constexpr uint32_t kLanes = 2 * NB, kRowsAt = 64 / kLanes;  // lanes per row, rows per instruction
       uint8_t* const st = smem + S::kOut + wave * 16 * S::kOutRow;
       const bool whole = cn + TB <= p.n;
+      const float scale = EPI == kEpiBf16 ? *p.scale : 1.0f;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
         if constexpr (EPI == kEpiGrad) {
-          const uint32_t at_row = lrow + 16 * i + lr, place = meta[at_row] - p.v0 - wcol;
-          const float shift = -__uint_as_float(meta[ROWS + at_row]) * kLog2e, up = __uint_as_float(meta[2 * ROWS + at_row]);
-          const bool here = place < 16u * NB;
+          const uint32_t at_row = lrow + 16 * i + lr, target = meta[at_row], place = target - p.v0 - wcol;
+          const float shift = -__uint_as_float(meta[ROWS + at_row]) * kLog2e;
 #pragma unroll
           for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              acc[i][j][e] = up * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, shift));
-          if (__builtin_amdgcn_ballot_w64(here)) {
+              acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, shift));
+          if (__builtin_amdgcn_ballot_w64(place < 16u * NB)) {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (place == 16u * j + 4 * lg + e) acc[i][j][e] -= up;
+                if (place == 16u * j + 4 * lg + e) acc[i][j][e] -= 1.0f;
+          }
+          const float m = __uint_as_float(meta[2 * ROWS + at_row]);
+          if (__builtin_amdgcn_ballot_w64(m != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = v4f{acc[i][j][0] * m, acc[i][j][1] * m, acc[i][j][2] * m, acc[i][j][3] * m};
+          }
+          if (__builtin_amdgcn_ballot_w64(target == kNoTarget)) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+              if (target == kNoTarget) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
           }
           if (!whole) {
 #pragma unroll
@@ -573,7 +591,8 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          const v4f v = acc[i][j];
+          v4f v = acc[i][j];
+          if constexpr (EPI == kEpiBf16) v = v4f{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
           *reinterpret_cast<uint2*>(st + lr * S::kOutRow + j * 32 + lg * 8) =
               uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
         }
@@ -643,28 +662,82 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* stats, con
   if (bad) atomicOr(err, bad);
 }
 
-// x with zeros for the rows without a target, [rows up to a multiple of 64]
-__global__ __launch_bounds__(256) void loss_live_rows_kernel(const uint16_t* x, const uint32_t* target, uint16_t* out,
-                                                             uint32_t* err, uint32_t rows, uint32_t vocab,
-                                                             uint32_t hidden) {
+// the largest upstream factor of the rows with a target, by one block; a NaN
+// among them is one
+__global__ __launch_bounds__(1024) void loss_factor_kernel(const float* up, const uint32_t* target, float* out,
+                                                           uint32_t rows, uint32_t vocab) {
+  __shared__ float tops[16];
+  float top = 0.0f;
+  bool nan = false;
+  for (uint32_t i = threadIdx.x; i < rows; i += 1024)
+    if (target[i] < vocab) {
+      const float v = fabsf(up[i]);
+      top = fmaxf(top, v);
+      nan |= v != v;
+    }
+  top = reduce_max_xor<64>(top);
+  if (__builtin_amdgcn_ballot_w64(nan)) top = __builtin_nanf("");
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w)
+      if (!(top >= tops[w]) && top == top) top = tops[w];
+    *out = top;
+  }
+}
+
+// up = factor 2^e m: m of every row, and 2^e x with zeros for the rows without
+// a target, [rows up to a multiple of 64].  Where up / factor is not a normal
+// number (0, NaN, or of no weight in dw) 2^e is that number and m is 1.
+__global__ __launch_bounds__(256) void loss_live_rows_kernel(const uint16_t* x, const uint32_t* target,
+                                                             const float* up, const float* factor, uint16_t* out,
+                                                             float* mantissa, uint32_t* err, uint32_t rows,
+                                                             uint32_t vocab, uint32_t hidden) {
   const uint32_t row = blockIdx.x;
   const uint32_t y = row < rows ? target[row] : kNoTarget;
-  if (threadIdx.x == 0 && y >= vocab && y != kNoTarget) atomicOr(err, kErrTarget);
+  float power = 0.0f, m = 1.0f;
+  if (y < vocab) {
+    power = *factor != 0.0f ? up[row] / *factor : 0.0f;
+    const uint32_t bits = __float_as_uint(power), exponent = bits & 0x7f800000u;
+    if (exponent != 0 && exponent != 0x7f800000u) {
+      m = __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
+      power = __uint_as_float(exponent);
+    }
+  }
+  if (threadIdx.x == 0) {
+    if (row < rows) mantissa[row] = m;
+    if (y >= vocab && y != kNoTarget) atomicOr(err, kErrTarget);
+  }
   for (uint32_t c = threadIdx.x * 8; c < hidden; c += 2048) {
     v4i v{0, 0, 0, 0};
-    if (y < vocab) v = *reinterpret_cast<const v4i*>(x + (uint64_t)row * hidden + c);
+    if (y < vocab) {
+      v = *reinterpret_cast<const v4i*>(x + (uint64_t)row * hidden + c);
+      if (power != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t bits = (uint32_t)v[i];
+          v[i] = (int)f32x2_to_bf16x2(power * bf16_bits_to_f32(bits & 0xffffu), power * bf16_bits_to_f32(bits >> 16));
+        }
+      }
+    }
     *reinterpret_cast<v4i*>(out + (uint64_t)row * hidden + c) = v;
   }
 }
 
-// dx: bf16 of the fp32 sums, the splits' added in order
-__global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, uint16_t* out, uint64_t count,
-                                                         uint32_t splits) {
+// dx: bf16 of up / m times the fp32 sums, the splits' added in order
+__global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, const uint32_t* target, const float* up,
+                                                         const float* mantissa, uint16_t* out, uint32_t hidden, uint32_t vocab,
+                                                         uint64_t count, uint32_t splits) {
   const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= count) return;
+  const uint32_t row = (uint32_t)(i / hidden);
+  const bool live = target[row] < vocab;
+  const float f = live ? up[row] / mantissa[row] : 0.0f;
   v4f v = *reinterpret_cast<const v4f*>(sums + i);
   for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(sums + s * count + i);
-  *reinterpret_cast<uint2*>(out + i) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+  // (a row without a target: 0, whatever the weights' infinities made of it)
+  if (!live) v = v4f{0.f, 0.f, 0.f, 0.f};
+  *reinterpret_cast<uint2*>(out + i) = uint2{f32x2_to_bf16x2(v[0] * f, v[1] * f), f32x2_to_bf16x2(v[2] * f, v[3] * f)};
 }
 
 template <bool AT, bool BT, int EPI>
@@ -691,7 +764,7 @@ bool big_takes(uint32_t hidden) { return hidden % KB == 0; }
 
 struct BackwardPlan {
   uint32_t piece, splits;
-  uint64_t g, live, sums, bytes;
+  uint64_t g, live, sums, factor, mantissa, bytes;
 };
 BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   BackwardPlan p{};
@@ -704,7 +777,9 @@ BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   // there is a tile for every CU, at 1024 columns a split or more
   const uint32_t tiles = ((rows + TB - 1) / TB) * ((hidden + TB - 1) / TB);
   p.splits = big_takes(hidden) ? std::max<uint32_t>(1, std::min<uint32_t>(kCus / tiles, p.piece / 1024)) : 1;
-  p.bytes = p.sums + padded((uint64_t)p.splits * rows * hidden * 4);
+  p.factor = p.sums + padded((uint64_t)p.splits * rows * hidden * 4);
+  p.mantissa = p.factor + padded(4);
+  p.bytes = p.mantissa + padded((uint64_t)rows * 4);
   return p;
 }
 
@@ -780,14 +855,18 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
   uint16_t* const live = reinterpret_cast<uint16_t*>(ws + plan.live);
   float* const sums = reinterpret_cast<float*>(ws + plan.sums);
   const uint32_t row_up = (a.rows + 63) / 64 * 64;
-  hipLaunchKernelGGL(loss_live_rows_kernel, dim3(row_up), dim3(256), 0, a.stream, a.x, a.target, live, a.error_flag,
-                     a.rows, a.vocab, a.hidden);
+  float* const factor = reinterpret_cast<float*>(ws + plan.factor);
+  float* const mantissa = reinterpret_cast<float*>(ws + plan.mantissa);
+  hipLaunchKernelGGL(loss_factor_kernel, dim3(1), dim3(1024), 0, a.stream, a.loss_grad, a.target, factor, a.rows,
+                     a.vocab);
+  hipLaunchKernelGGL(loss_live_rows_kernel, dim3(row_up), dim3(256), 0, a.stream, a.x, a.target, a.loss_grad, factor,
+                     live, mantissa, a.error_flag, a.rows, a.vocab, a.hidden);
   for (uint32_t v0 = 0; v0 < a.vocab; v0 += plan.piece) {
     const uint32_t cols = std::min(plan.piece, a.vocab - v0);
     const uint16_t* const w = a.w + (uint64_t)v0 * a.hidden;
     if (big_takes(a.hidden)) {
       BigArgs b{};
-      b.a = live;
+      b.a = a.x;
       b.b = w;
       b.m = a.rows;
       b.n = cols;
@@ -797,7 +876,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
       b.ldo = plan.piece;
       b.target = a.target;
       b.lse = a.lse;
-      b.up = a.loss_grad;
+      b.mantissa = mantissa;
       b.v0 = v0;
       b.vocab = a.vocab;
       launch_big<false, false, kEpiGrad>(b, a.stream);
@@ -811,6 +890,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
         b.lda = plan.piece;
         b.ldb = a.hidden;
         b.out = a.dw + (uint64_t)v0 * a.hidden;
+        b.scale = factor;
         b.ldo = a.hidden;
         launch_big<true, true, kEpiBf16>(b, a.stream);
       }
@@ -832,7 +912,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
       continue;
     }
     GemmArgs g{};
-    g.a = live;
+    g.a = a.x;
     g.b = w;
     g.m = a.rows;
     g.n = cols;
@@ -842,7 +922,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
     g.ldo = plan.piece;
     g.target = a.target;
     g.lse = a.lse;
-    g.up = a.loss_grad;
+    g.mantissa = mantissa;
     g.v0 = v0;
     g.vocab = a.vocab;
     launch_gemm<false, false, kEpiGrad>(g, a.stream);
@@ -856,6 +936,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
       d.lda = plan.piece;
       d.ldb = a.hidden;
       d.out = a.dw + (uint64_t)v0 * a.hidden;
+      d.scale = factor;
       d.ldo = a.hidden;
       launch_gemm<true, true, kEpiBf16>(d, a.stream);
     }
@@ -873,8 +954,8 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
     launch_gemm<false, true, kEpiAdd>(d, a.stream);
   }
   const uint64_t count = (uint64_t)a.rows * a.hidden;
-  hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, a.stream, sums, a.dx,
-                     count, plan.splits);
+  hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, a.stream, sums,
+                     a.target, a.loss_grad, mantissa, a.dx, a.hidden, a.vocab, count, plan.splits);
   return AfterLaunch("lm_head_loss_backward_launch_failed");
 }
 
