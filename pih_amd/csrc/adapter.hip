@@ -99,6 +99,10 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
 __device__ __forceinline__ v4i load16(const uint16_t* p) { return *reinterpret_cast<const v4i*>(p); }
+// (read once)
+__device__ __forceinline__ v4i load16_once(const uint16_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p));
+}
 __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
       for (uint32_t h = 0; h < 2; ++h) {
         v.b[r][h] = v4i{0, 0, 0, 0};
         const uint32_t c = c0 + 32 * h + 8 * lg;
-        if (p.base && c < p.cols) v.b[r][h] = load16(p.base + base_row[r] + c);
+        if (p.base && c < p.cols) v.b[r][h] = load16_once(p.base + base_row[r] + c);
       }
   };
   v4i hi[RB][KJ], lo[RB][KJ];

@@ -303,7 +303,9 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
           if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
         }
       }
-      dma16(sb, ob, lds + S::kA + i * 4096);
+      // (a single tile of rows: the weights are read once)
+      if constexpr (ROWS == 64 && !BT) dma16nt(sb, ob, lds + S::kA + i * 4096);
+      else dma16(sb, ob, lds + S::kA + i * 4096);
     }
   };
   // tile t and its first steps sent for; its rows' targets, log-sum-exps and
