@@ -215,24 +215,15 @@ __device__ __forceinline__ v4i join(v4s x, v4s y) {
   return v4i{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
 }
 
-// c += a . b with c kept where it is: with all 256 accumulator registers in
-// use the compiler's own form moved them about, 518 moves beside 128 MFMAs.
-// The compiler does not see an MFMA in it, so the wait states are kept here: an
-// operand written by a vector instruction is read two states later (s_nop 1;
-// the matrix pipe is busy with the MFMA before meanwhile), an accumulator is
-// used again no sooner than 15 MFMAs on, and settle() stands between the MFMAs
-// and anything else that touches accumulators, tied to them by its operands.
-__device__ __forceinline__ void mfma_in_place(v4f& c, v4i a, v4i b) {
-  asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-}
+// Accumulators held in their registers: with all 256 in use the compiler
+// otherwise moved them about, 518 moves beside 128 MFMAs (now none).
 template <int NB>
-__device__ __forceinline__ void settle(v4f (&c)[NB]) {
+__device__ __forceinline__ void pin(v4f (&c)[NB]) {
   static_assert(NB == 4 || NB == 8, "blocks");
   if constexpr (NB == 8)
-    asm volatile("s_nop 15\n\ts_nop 7"
-                 : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
+    asm volatile("" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
   else
-    asm volatile("s_nop 15\n\ts_nop 7" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]));
+    asm volatile("" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]));
 }
 
 template <int ROWS>
@@ -374,7 +365,10 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   };
   auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) mfma_in_place(acc[i][j], fb[from][j], fa[from][i]);
+    for (int j = 0; j < NB; ++j)
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fb[from][j]),
+                                                          __builtin_bit_cast(v8bf, fa[from][i]), acc[i][j], 0, 0, 0);
+    pin(acc[i]);
   };
   uint32_t s;  // the buffer of the step being multiplied
   // kNext: the next step exists, with kLeft further steps in flight behind it;
@@ -439,7 +433,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < MB; ++i) settle(acc[i]);
+    for (int i = 0; i < MB; ++i) pin(acc[i]);
     __builtin_amdgcn_s_waitcnt(kLdsRead);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -467,7 +461,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       start(which);
     }
 #pragma unroll
-    for (int i = 0; i < MB; ++i) settle(acc[i]);
+    for (int i = 0; i < MB; ++i) pin(acc[i]);
 
     // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of
     // the wave's part
