@@ -165,11 +165,11 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
 }
 
 // ------------------------------------------------ tiles fed by DMA
-// C [m][n] = A . B^T in tiles of 256 columns and 256 or (few rows) 64 rows.
-// Four waves: 2 x 2 quarters of 128 x 128, one wave per SIMD with 256
+// C [m][n] = A . B^T in tiles of 256 columns and 256, 128 or 64 rows.  Four
+// waves: 2 x 2 quarters of 128 x 128 (64 x 128), one wave per SIMD with 256
 // accumulator registers, or 1 x 4 of 64 x 64.  A K step is 64 deep and moved
-// into LDS by DMA, two (64 rows: three) steps resident.  Two layouts of an
-// operand:
+// into LDS by DMA, two (128 and 64 rows: three) steps resident.  Two layouts
+// of an operand:
 //   rows     [row][k] in memory: LDS rows of 128 bytes, 16-byte chunk c of row
 //            r in slot c ^ ((r >> 1) & 7); a fragment is one ds_read_b128
 //            (16 rows, one chunk each: all 64 banks once);
@@ -228,14 +228,15 @@ __device__ __forceinline__ void pin(v4f (&c)[NB]) {
 
 template <int ROWS>
 struct BigShape {
-  static constexpr int WM = ROWS == 256 ? 2 : 1, WN = 4 / WM;        // waves
+  static constexpr int WM = ROWS >= 128 ? 2 : 1, WN = 4 / WM;        // waves
   static constexpr int MB = ROWS / 16 / WM, NB = TB / 16 / WN;       // a wave's 16 x 16 blocks
   static constexpr int ST = ROWS == 256 ? 2 : 3;                     // steps resident
   static constexpr uint32_t kA = ROWS * KB * 2, kB = TB * KB * 2, kStage = kA + kB;
   static constexpr int LA = ROWS / 32, LB = 8, NL = LA + LB;         // DMAs per wave and step
   static constexpr uint32_t kOutRow = 16 * NB * 2 + 16;              // a wave's staged output row
-  static constexpr uint32_t kOut = ST * kStage;                      // 16 of them per wave
-  static constexpr uint32_t kMeta = kOut + 4 * 16 * kOutRow;         // per row: two tiles' targets, lse, mantissas
+  static constexpr uint32_t kOutRows = ROWS == 128 ? 8 : 16;         // staged at a time
+  static constexpr uint32_t kOut = ST * kStage;                      // kOutRows of them per wave
+  static constexpr uint32_t kMeta = kOut + 4 * kOutRows * kOutRow;   // per row: two tiles' targets, lse, mantissas
   static constexpr uint32_t kLds = kMeta + 2 * ROWS * 12;
   static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -352,16 +353,17 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   };
   v4f acc[MB][NB];
   v4i fa[2][MB], fb[2][NB];
-  // the fragments of a half, three beside each group of NB MFMAs: B's first,
-  // which the next half's first group needs, and all of them a group or two
-  // early
+  // the fragments of a half, three or four beside each group of NB MFMAs: B's
+  // first, which the next half's first group needs, and all of them a group or
+  // two early
+  constexpr uint32_t kReads = (MB + NB + MB - 2) / (MB - 1);
   auto read_one = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
     if (i < (uint32_t)NB) fb[to][i] = frag(bt, s * S::kStage + S::kA, wn * NB * 16 + 16 * i, q);
     else if (i < (uint32_t)(NB + MB)) fa[to][i - NB] = frag(at, s * S::kStage, wm * MB * 16 + 16 * (i - NB), q);
   };
   auto read_group = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t e = 3 * i; e < 3 * i + 3; ++e) read_one(s, q, to, e);
+    for (uint32_t e = kReads * i; e < kReads * i + kReads; ++e) read_one(s, q, to, e);
   };
   auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     if constexpr (EPI == kEpiStats) {
       // [column part][row]: maximum and sum
       float2* const parts = reinterpret_cast<float2*>(smem + S::kOut);
-      static_assert(S::WN * ROWS * 8 <= 4 * 16 * S::kOutRow, "parts");
+      static_assert(S::WN * ROWS * 8 <= 4 * S::kOutRows * S::kOutRow, "parts");
       const bool whole = cn + TB <= p.n;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -543,10 +545,10 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      // bf16 through the wave's own LDS, 16 rows at a time, so that a store
+      // bf16 through the wave's own LDS, 16 or 8 rows at a time, so that a store
       // instruction writes whole lines
       constexpr uint32_t kLanes = 2 * NB, kRowsAt = 64 / kLanes;  // lanes per row, rows per instruction
-      uint8_t* const st = smem + S::kOut + wave * 16 * S::kOutRow;
+      uint8_t* const st = smem + S::kOut + wave * S::kOutRows * S::kOutRow;
       const bool whole = cn + TB <= p.n;
       const float scale = EPI == kEpiBf16 ? *p.scale : 1.0f;
 #pragma unroll
@@ -586,23 +588,28 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
           if (i == 0) arrived();
         }
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          v4f v = acc[i][j];
-          if constexpr (EPI == kEpiBf16) v = v4f{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
-          *reinterpret_cast<uint2*>(st + lr * S::kOutRow + j * 32 + lg * 8) =
-              uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
-        }
-        wave_lds_order();
+        for (uint32_t r0 = 0; r0 < 16; r0 += S::kOutRows) {
+          if (lr - r0 < S::kOutRows) {
 #pragma unroll
-        for (uint32_t h = 0; h < 16 / kRowsAt; ++h) {
-          const uint32_t q = kRowsAt * h + lane / kLanes, r = wrow + 16 * i + q, c = wcol + 8 * (lane % kLanes);
-          const v4i o = *reinterpret_cast<const v4i*>(st + q * S::kOutRow + lane % kLanes * 16);
-          // the rows of g up to a multiple of 64 and its columns up to the
-          // tile's end are written as zeros: the products with g read them
-          const bool in = EPI == kEpiGrad ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
-          if (in) *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c) = o;
+            for (int j = 0; j < NB; ++j) {
+              v4f v = acc[i][j];
+              if constexpr (EPI == kEpiBf16) v = v4f{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
+              *reinterpret_cast<uint2*>(st + (lr - r0) * S::kOutRow + j * 32 + lg * 8) =
+                  uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+            }
+          }
+          wave_lds_order();
+#pragma unroll
+          for (uint32_t h = 0; h < S::kOutRows / kRowsAt; ++h) {
+            const uint32_t q = kRowsAt * h + lane / kLanes, r = wrow + 16 * i + r0 + q, c = wcol + 8 * (lane % kLanes);
+            const v4i o = *reinterpret_cast<const v4i*>(st + q * S::kOutRow + lane % kLanes * 16);
+            // the rows of g up to a multiple of 64 and its columns up to the
+            // tile's end are written as zeros: the products with g read them
+            const bool in = EPI == kEpiGrad ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
+            if (in) *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c) = o;
+          }
+          wave_lds_order();
         }
-        wave_lds_order();
       }
     }
     if (!more) return;
@@ -617,12 +624,29 @@ void launch_rows(BigArgs p, hipStream_t s) {
   const uint32_t grid = std::min((p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8, kCus);
   hipLaunchKernelGGL((loss_big_kernel<ROWS, AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
 }
-// products whose rows are the batch's: 64-row tiles while there is one of them
+// Rows of a tile by the time of the rounds of tiles on the CUs: a step and a
+// tile's own beginning and end cost (us)
+//   256 rows 1.45 and 9,  128 rows 0.95 and 7,  64 rows 0.70 and 6.
+inline uint32_t tile_rows(const BigArgs& p) {
+  const uint32_t steps = (p.k / KB + std::max(p.splits, 1u) - 1) / std::max(p.splits, 1u);
+  auto cost = [&](uint32_t rows, float step, float tile) {
+    const uint64_t tiles = (uint64_t)((p.m + rows - 1) / rows) * ((p.n + TB - 1) / TB) * std::max(p.splits, 1u);
+    return (float)((tiles + kCus - 1) / kCus) * (tile + step * (float)steps);
+  };
+  const float c256 = cost(256, 1.45f, 9.0f), c128 = cost(128, 0.95f, 7.0f), c64 = cost(64, 0.70f, 6.0f);
+  return c64 < c128 && c64 < c256 ? 64 : c128 < c256 ? 128 : 256;
+}
+// (the gradient of the weights has the vocabulary for rows: always many)
 template <bool AT, bool BT, int EPI>
 void launch_big(const BigArgs& p, hipStream_t s) {
   if constexpr (!AT) {
-    if (p.m <= 64) {
+    const uint32_t rows = tile_rows(p);
+    if (rows == 64) {
       launch_rows<64, AT, BT, EPI>(p, s);
+      return;
+    }
+    if (rows == 128) {
+      launch_rows<128, AT, BT, EPI>(p, s);
       return;
     }
   }
@@ -730,6 +754,7 @@ __global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, cons
   const bool live = target[row] < vocab;
   const float f = live ? up[row] / mantissa[row] : 0.0f;
   v4f v = *reinterpret_cast<const v4f*>(sums + i);
+#pragma unroll 8
   for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(sums + s * count + i);
   // (a row without a target: 0, whatever the weights' infinities made of it)
   if (!live) v = v4f{0.f, 0.f, 0.f, 0.f};
@@ -751,7 +776,7 @@ uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 // columns of a piece: 2^26 elements of g, in whole tiles
 uint32_t piece_columns(uint32_t rows, uint32_t vocab) {
   const uint32_t all = (vocab + 255) / 256 * 256;
-  const uint32_t fit = (uint32_t)std::min<uint64_t>((1ull << 26) / rows / 256 * 256, 65536);
+  const uint32_t fit = (uint32_t)((1ull << 26) / rows / 256 * 256);
   return std::min(all, std::max(fit, 4096u));
 }
 

@@ -55,8 +55,8 @@ def _ref(x, w, target):
     elog = e.max(1).values + (w.shape[0] / 64 + 48) * U + lse.abs() * 2 * U
     live = target >= 0
     at = target.clamp(min=0).long()
-    loss = torch.where(live, lse - logits[torch.arange(rows), at], torch.zeros((), dtype=torch.float64))
-    eloss = elog + e[torch.arange(rows), at] + loss.abs() * U
+    loss = torch.where(live, lse - logits[torch.arange(rows, device=x.device), at], torch.zeros((), dtype=torch.float64, device=x.device))
+    eloss = elog + e[torch.arange(rows, device=x.device), at] + loss.abs() * U
     return logits, e, lse, elog, loss, eloss, live, at
 
 
@@ -93,9 +93,9 @@ def _grads_ref(x, w, target, up, lse32):
     xd, wd = x.double(), w.double()
     rows, vocab = logits.shape
     p = torch.exp(logits - lse32.double()[:, None])
-    upd = torch.where(live, up.double(), torch.zeros((), dtype=torch.float64))[:, None]
+    upd = torch.where(live, up.double(), torch.zeros((), dtype=torch.float64, device=x.device))[:, None]
     g = p.clone()
-    g[torch.arange(rows), at] -= 1
+    g[torch.arange(rows, device=x.device), at] -= 1
     g *= upd
     arg = (logits - lse32.double()[:, None]).abs()
     eg = upd.abs() * p * (1.1 * e + (arg + 4) * U + 2.0 ** -21) + g.abs() * (2 * U + HALF_BF16) + upd.abs() * U
@@ -127,24 +127,24 @@ def test_backward(eng, rows, vocab, hidden):
 
 
 def test_several_pieces_of_the_vocabulary(eng):
-    """More columns than a piece holds (65536 at these few rows), the last
-    piece a short one."""
+    """More columns than a piece holds (2^26 elements: 60928 columns at these
+    rows), the last piece a short one; 64 bits on the GPU."""
     import torch
 
     from pih_amd.linear import lm_head_loss, lm_head_loss_backward
 
-    x, w, target, up = _case(3, 37, 65536 * 2 + 1003, 64)
-    target[0], target[1], target[2] = 65535, 65536, 65536 * 2 + 1002
-    _, _, lse, elog, loss, eloss, _, _ = _ref(x, w, target)
-    args = [t.cuda() for t in (x, w, target)]
-    got, glse, _ = lm_head_loss(*args)
-    _within(glse, lse, elog, "lse")
-    _within(got, loss, eloss, "loss")
-    (dx, ex), (dw, ew) = _grads_ref(x, w, target, up, glse.cpu())
-    gx, gw, flag = lm_head_loss_backward(*args, glse, up.cuda())
+    x, w, target, up = [t.cuda() for t in _case(3, 1100, 60928 * 2 + 1003, 64)]
+    target[0], target[1], target[2] = 60927, 60928, 60928 * 2 + 1002
+    logits, e, lse, elog, loss, eloss, _, _ = _ref(x, w, target)
+    del logits, e
+    got, glse, _ = lm_head_loss(x, w, target)
+    _within(glse, lse.cpu(), elog.cpu(), "lse")
+    _within(got, loss.cpu(), eloss.cpu(), "loss")
+    gx, gw, flag = lm_head_loss_backward(x, w, target, glse, up)
+    (dx, ex), (dw, ew) = _grads_ref(x, w, target, up, glse)
     assert int(flag.item()) == 0
-    _within(gx, dx, ex, "dx")
-    _within(gw, dw, ew, "dw")
+    _within(gx, dx.cpu(), ex.cpu(), "dx")
+    _within(gw, dw.cpu(), ew.cpu(), "dw")
 
 
 def test_gradients_are_the_differences(eng):
