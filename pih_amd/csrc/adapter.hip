@@ -640,8 +640,11 @@ void with_pow2(uint32_t n, F&& f) {
 
 template <bool kColumns>
 void launch_up(UpParams p, const AdapterArgs& a) {
-  // column blocks for three rounds of what the card holds: a wave then takes
-  // several groups where there are many tiles, and the last round costs little
+  // column blocks for as many blocks as the card holds at once (tiles of few
+  // rows: every further round repeats the search and the sum of h; 57 one-row
+  // requests 10.2 us against 12.7 with three rounds) or, with long segments,
+  // for three rounds of that, whose last costs little (8192 rows 117 us against
+  // 126 with one)
   const uint32_t blocks = tile_blocks(a) == 4 && p.rank <= 64 ? 2 : 1;
   const uint32_t tiles = tile_bound(a, 16 * blocks), all = (p.cols + 63) / 64;
   with_pow2((p.rank + 31) / 32, [&](auto kj) {
@@ -649,7 +652,7 @@ void launch_up(UpParams p, const AdapterArgs& a) {
     if constexpr (KJ <= 4) {
       auto launch = [&](auto rb) {
         constexpr int RB = decltype(rb)::value;
-        const uint32_t columns = std::max<uint32_t>(1, 3 * kCus * up_occupancy(KJ, RB) / tiles);
+        const uint32_t columns = std::max<uint32_t>(1, (RB == 1 ? 1 : 3) * kCus * up_occupancy(KJ, RB) / tiles);
         p.groups = std::max<uint32_t>(1, (all + 4 * columns - 1) / (4 * columns));
         const dim3 grid(tiles, (all + 4 * p.groups - 1) / (4 * p.groups));
         hipLaunchKernelGGL((adapter_up_kernel<KJ, RB, kColumns>), grid, dim3(256), 0, a.stream, p);

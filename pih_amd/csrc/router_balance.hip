@@ -210,37 +210,44 @@ __global__ __launch_bounds__(64 * kBalanceWaves) void router_balance_kernel(cons
   if (bad) atomicOr(err, bad);
 }
 
-// The blocks' partial sums, and the loss: one block, thread (e, part) adds
-// every parts-th block's partial of expert e.
+// The blocks' partial sums, and the loss: one block, whose thread (column,
+// part) adds every parts-th block's partials of V neighbouring experts.
+template <int V>
 __global__ __launch_bounds__(1024) void router_balance_finish_kernel(const float* part_sum, const uint32_t* part_count,
                                                                      float* loss, uint32_t* counts, float* mean,
                                                                      uint32_t blocks, uint32_t tokens,
                                                                      uint32_t experts, float weight) {
-  __shared__ float s_sum[1024];
-  __shared__ uint32_t s_count[1024];
+  typedef float Sums __attribute__((ext_vector_type(V)));
+  typedef uint32_t Counts __attribute__((ext_vector_type(V)));
+  __shared__ Sums s_sum[1024];
+  __shared__ Counts s_count[1024];
   __shared__ float s_term[16];
-  const uint32_t tid = threadIdx.x, parts = 1024 / experts, e = tid % experts, part = tid / experts;
-  float v = 0.0f;
-  uint32_t c = 0;
+  const uint32_t tid = threadIdx.x, columns = experts / V, parts = 1024 / columns, c = tid % columns, part = tid / columns;
+  Sums v = 0.0f;
+  Counts n = 0u;
   if (part < parts)
 #pragma unroll 8
     for (uint32_t i = part; i < blocks; i += parts) {
-      v += part_sum[(uint64_t)i * experts + e];
-      c += part_count[(uint64_t)i * experts + e];
+      v += *reinterpret_cast<const Sums*>(part_sum + (uint64_t)i * experts + V * c);
+      n += *reinterpret_cast<const Counts*>(part_count + (uint64_t)i * experts + V * c);
     }
   s_sum[tid] = v;
-  s_count[tid] = c;
+  s_count[tid] = n;
   __syncthreads();
   float term = 0.0f;
-  if (tid < experts) {
+  if (tid < columns) {
+#pragma unroll 4
     for (uint32_t q = 1; q < parts; ++q) {
-      v += s_sum[q * experts + tid];
-      c += s_count[q * experts + tid];
+      v += s_sum[q * columns + tid];
+      n += s_count[q * columns + tid];
     }
-    const float m = v / (float)tokens;
-    counts[tid] = c;
-    mean[tid] = m;
-    term = (float)c * m;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float m = v[e] / (float)tokens;
+      counts[V * tid + e] = n[e];
+      mean[V * tid + e] = m;
+      term += (float)n[e] * m;
+    }
   }
   term = reduce_sum_xor<64>(term);
   if ((tid & 63u) == 0) s_term[tid >> 6] = term;
@@ -381,7 +388,7 @@ St LaunchRouterBalance(const RouterBalanceArgs& a) {
   if (a.mode != kRouterSoftmax && a.mode != kRouterSqrtSoftplus) return Invalid("router_balance_mode_invalid");
   if (!__builtin_isfinite(a.coefficient)) return Invalid("router_balance_coefficient_invalid");
   if (a.workspace_bytes < RouterBalanceWorkspaceBytes(a.tokens, a.topk, a.experts) ||
-      reinterpret_cast<uintptr_t>(a.workspace) % 4)
+      !aligned16(a.workspace))
     return Invalid("router_balance_workspace_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
@@ -397,8 +404,9 @@ St LaunchRouterBalance(const RouterBalanceArgs& a) {
                        a.error_flag, a.tokens, a.experts, a.topk, vec);
   });
   const float weight = (float)((double)a.coefficient * a.experts / ((double)a.tokens * a.topk));
-  hipLaunchKernelGGL(router_balance_finish_kernel, dim3(1), dim3(1024), 0, a.stream, sums, counts, a.loss, a.counts,
-                     a.mean, blocks, a.tokens, a.experts, weight);
+  auto finish = a.experts % 4 == 0 ? router_balance_finish_kernel<4> : router_balance_finish_kernel<1>;
+  hipLaunchKernelGGL(finish, dim3(1), dim3(1024), 0, a.stream, sums, counts, a.loss, a.counts, a.mean, blocks,
+                     a.tokens, a.experts, weight);
   return AfterLaunch("router_balance_launch_failed");
 }
 
@@ -414,7 +422,7 @@ St LaunchRouterBackward(const RouterBackwardArgs& a) {
   if (!clean.ok()) return clean;
   // of a score's own term: the loss's weight over T
   const float weight = (float)((double)a.coefficient * a.experts / ((double)a.tokens * a.tokens * a.topk));
-  const uint32_t rows = kWaves * 64 / row_lanes(a.experts), blocks = std::min<uint32_t>(2048, (a.tokens + rows - 1) / rows);
+  const uint32_t rows = kWaves * 64 / row_lanes(a.experts), blocks = std::min<uint32_t>(1024, (a.tokens + rows - 1) / rows);
   const bool vec = a.experts % 4 == 0 && aligned16(a.scores) && aligned16(a.scores_grad);
   with_row(a.experts, [&](auto lanes, auto quads) {
     constexpr int L = decltype(lanes)::value, Q = decltype(quads)::value;
