@@ -95,6 +95,97 @@ __device__ __forceinline__ bool find_tile(const Segments& p, uint32_t height, ui
   return false;
 }
 
+// Tiles of 16 rows with one adapter picked from all segments: where segments
+// are a token or two, as in a decode batch, a tile per segment would read the
+// adapter again for every one of them.  Tiles go by adapter (without one last),
+// a tile's rows in the order of the segments.  Every block finds its tile by
+// itself: rows per adapter counted in LDS, the adapters' tiles and then the
+// adapter's rows by block scans (~2 us).
+constexpr uint32_t kGroupAdapters = 1023, kGroupSegments = 2048;
+struct GroupShared {
+  uint32_t count[kGroupAdapters + 1];
+  uint32_t wave[4];
+  uint32_t adapter, tile;
+  uint32_t rows[16];
+};
+// inclusive scan of a block's values, and their sum
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t& total, uint32_t* wave_sums) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (uint32_t d = 1; d < 64; d <<= 1) {
+    const uint32_t u = __shfl_up(v, d, 64);
+    if (lane >= d) v += u;
+  }
+  if (lane == 63) wave_sums[wave] = v;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < 4; ++w) {
+    if (w < wave) before += wave_sums[w];
+    total += wave_sums[w];
+  }
+  __syncthreads();
+  return v + before;
+}
+// Segment s: first row, rows (0 past the last and where the offsets are bad)
+// and its place in count[] (`adapters` without one, kNoAdapter a bad id).
+struct Segment {
+  uint32_t first, rows, place;
+};
+__device__ __forceinline__ Segment segment_at(const Segments& p, uint32_t s, bool report, uint32_t* err) {
+  Segment v{0, 0, kNoAdapter};
+  if (s >= p.segments) return v;
+  const uint32_t lo = p.offsets[s], hi = p.offsets[s + 1], a = p.adapter[s];
+  if (hi < lo || hi > p.rows) {
+    if (report) atomicOr(err, kErrOffsets);
+    return v;
+  }
+  v = Segment{lo, hi - lo, a < p.adapters ? a : a == kNoAdapter ? p.adapters : kNoAdapter};
+  if (report && v.place == kNoAdapter && v.rows) atomicOr(err, kErrAdapter);
+  return v;
+}
+__device__ __forceinline__ bool group_tile(const Segments& p, uint32_t index, Tile& t, GroupShared& g, uint32_t* err) {
+  const uint32_t tid = threadIdx.x, places = p.adapters + 1;
+  for (uint32_t i = tid; i < places; i += 256) g.count[i] = 0;
+  __syncthreads();
+  for (uint32_t s = tid; s < p.segments; s += 256) {
+    const Segment v = segment_at(p, s, index == 0, err);
+    if (v.rows && v.place != kNoAdapter) atomicAdd(&g.count[v.place], v.rows);
+  }
+  __syncthreads();
+  uint32_t before = 0;
+  bool found = false;
+  for (uint32_t b = 0; b < places && !found; b += 256) {
+    const uint32_t n = b + tid < places ? (g.count[b + tid] + 15) / 16 : 0;
+    uint32_t total;
+    const uint32_t upto = block_scan(n, total, g.wave);
+    const uint32_t at = index - before;
+    if (at < total && at < upto && at >= upto - n) {
+      g.adapter = b + tid;
+      g.tile = at - (upto - n);
+    }
+    found = at < total;
+    before += total;
+  }
+  if (!found) return false;
+  __syncthreads();
+  const uint32_t place = g.adapter, p0 = 16 * g.tile, rows = min(16u, g.count[place] - p0);
+  before = 0;
+  for (uint32_t s0 = 0; s0 < p.segments && before < p0 + rows; s0 += 256) {
+    const Segment v = segment_at(p, s0 + tid, false, err);
+    const uint32_t n = v.place == place ? v.rows : 0;
+    uint32_t total;
+    const uint32_t first = before + block_scan(n, total, g.wave) - n;
+    for (uint32_t q = max(first, p0); q < min(first + n, p0 + rows); ++q) g.rows[q - p0] = v.first + (q - first);
+    before += total;
+  }
+  __syncthreads();
+  t = Tile{0, rows, place < p.adapters ? place : kNoAdapter, 1.0f};
+  if (place < p.adapters && p.scale) t.scale = p.scale[place];
+  return true;
+}
+
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
@@ -144,9 +235,9 @@ struct DownParams {
 // of cols; the four waves take 128-column pieces in turn.  kColumns: 32 rows
 // of the weights (one contiguous piece of memory) go through the wave's LDS
 // and are read transposed.
-template <int NJ, int RB, bool kColumns>
-__device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d, const Tile& t, uint32_t split,
-                                          uint8_t* lds) {
+template <int NJ, int RB, bool kColumns, typename F>
+__device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d, const Tile& t, F&& row_of,
+                                          uint32_t split, uint8_t* lds) {
   constexpr uint32_t kSumRow = NJ * 16 + 4;
   float* const sums = reinterpret_cast<float*>(lds);  // [4][16][kSumRow]
   const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
@@ -159,7 +250,7 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
     for (int j = 0; j < NJ; ++j) acc[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
   const uint16_t* src[RB];
 #pragma unroll
-  for (int r = 0; r < RB; ++r) src[r] = d.src + (uint64_t)(t.row0 + min(16 * r + lr, t.rows - 1)) * d.stride;
+  for (int r = 0; r < RB; ++r) src[r] = d.src + (uint64_t)row_of(min(16 * r + lr, t.rows - 1)) * d.stride;
   const uint16_t* const w = d.w + (uint64_t)t.adapter * rank * d.cols;
   if constexpr (!kColumns) {
     const uint16_t* wr[NJ];
@@ -236,7 +327,7 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
     }
     __syncthreads();
   }
-  float* const out = d.out + ((uint64_t)split * p.seg.rows + t.row0) * rank;
+  float* const out = d.out + (uint64_t)split * p.seg.rows * rank;
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     if (16u * r >= t.rows) break;
@@ -247,7 +338,7 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
       const uint32_t row = i / (rank / 4), j = i % (rank / 4) * 4;
       const float* const from = sums + row * kSumRow + j;
       auto part = [&](uint32_t v) { return *reinterpret_cast<const v4f*>(from + v * 16 * kSumRow); };
-      *reinterpret_cast<v4f*>(out + (uint64_t)(16 * r + row) * rank + j) = (part(0) + part(1)) + (part(2) + part(3));
+      *reinterpret_cast<v4f*>(out + (uint64_t)row_of(16 * r + row) * rank + j) = (part(0) + part(1)) + (part(2) + part(3));
     }
     __syncthreads();
   }
@@ -267,13 +358,23 @@ __global__ __launch_bounds__(256, down_occupancy(NJ, RB)) void adapter_down_kern
   Tile t;
   const DownSide& d = p.side[blockIdx.z];
   if (blockIdx.y >= d.splits || !find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
+  auto row_of = [&](uint32_t r) { return t.row0 + r; };
   if constexpr (kBackward) {
     if (blockIdx.z) {
-      down_tile<NJ, RB, true>(p, d, t, blockIdx.y, lds);
+      down_tile<NJ, RB, true>(p, d, t, row_of, blockIdx.y, lds);
       return;
     }
   }
-  down_tile<NJ, RB, false>(p, d, t, blockIdx.y, lds);
+  down_tile<NJ, RB, false>(p, d, t, row_of, blockIdx.y, lds);
+}
+// the same on tiles of rows from several segments
+template <int NJ>
+__global__ __launch_bounds__(256, down_occupancy(NJ, 1)) void adapter_down_group_kernel(DownParams p) {
+  __shared__ __align__(16) uint8_t lds[4 * 16 * (NJ * 16 + 4) * 4];
+  __shared__ GroupShared group;
+  Tile t;
+  if (!group_tile(p.seg, blockIdx.x, t, group, p.err) || t.adapter >= p.seg.adapters) return;
+  down_tile<NJ, 1, false>(p, p.side[0], t, [&](uint32_t r) { return group.rows[r]; }, blockIdx.y, lds);
 }
 
 // -------------------------------------------------------------------- up
@@ -297,13 +398,23 @@ struct UpParams {
 // blocks of the up kernel that a CU holds, by its registers
 constexpr int up_occupancy(int kj, int rb) { return kj == 1 ? (rb == 1 ? 4 : 3) : kj == 2 && rb == 1 ? 3 : 2; }
 
-template <int KJ, int RB, bool kColumns>
+template <int KJ, int RB, bool kColumns, bool kGroup>
 __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(UpParams p) {
+  static_assert(!kGroup || RB == 1, "a group's tile has 16 rows");
   constexpr uint32_t kRow = KJ * 32 + 4, kPitch = 128 + 16;
   __shared__ __align__(16) float hs[16 * RB * kRow];
   __shared__ __align__(16) uint8_t staged[kColumns ? 4 * 32 * kPitch : 16];
+  __shared__ std::conditional_t<kGroup, GroupShared, char> group;
   Tile t;
-  if (!find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err)) return;
+  if constexpr (kGroup) {
+    if (!group_tile(p.seg, blockIdx.x, t, group, p.err)) return;
+  } else {
+    if (!find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err)) return;
+  }
+  auto row_of = [&](uint32_t r) -> uint32_t {
+    if constexpr (kGroup) return group.rows[r];
+    else return t.row0 + r;
+  };
   if (t.adapter >= p.seg.adapters && t.adapter != kNoAdapter) return;
   const bool live = t.adapter != kNoAdapter;
   if (!live && p.base == p.out) return;
@@ -314,7 +425,7 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
   uint64_t base_row[RB], out_row[RB];
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
-    const uint32_t row = t.row0 + min(16 * r + lr, t.rows - 1);
+    const uint32_t row = row_of(min(16 * r + lr, t.rows - 1));
     base_row[r] = (uint64_t)row * p.base_stride;
     out_row[r] = (uint64_t)row * p.out_stride;
   }
@@ -407,7 +518,7 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
       const uint32_t r = i / (KJ * 8), j = i % (KJ * 8) * 4;
       v4f v{0.f, 0.f, 0.f, 0.f};
       if (r < t.rows && j < rank) {
-        const float* from = p.h + (uint64_t)(t.row0 + r) * rank + j;
+        const float* from = p.h + (uint64_t)row_of(r) * rank + j;
         const uint64_t step = (uint64_t)p.seg.rows * rank;
 #pragma unroll 8
         for (uint32_t q = 0; q < p.splits; ++q) v += *reinterpret_cast<const v4f*>(from + q * step);
@@ -623,10 +734,13 @@ uint32_t tile_bound(const AdapterArgs& a, uint32_t height) {
   return (uint32_t)std::min<uint64_t>(t, a.rows);
 }
 // K splits of the down product: what the card holds at once (a short second
-// round costs as much as a full one), 256 columns each at least
+// round costs as much as a full one), 512 columns each at least: every block of
+// the up product adds the splits (64 one-row requests of rank 128 over 12288
+// columns 30 us against 43 with 256 columns; 1024 wins with one adapter, 29 us,
+// and loses with 16 at rank 64, 22.4 against 20.4)
 uint32_t down_splits(uint32_t tiles, uint32_t cols, uint32_t rank, uint32_t blocks, uint32_t sides) {
   const uint32_t held = kCus * down_occupancy((rank + 15) / 16, blocks);
-  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 255) / 256, held / std::max(sides * tiles, 1u)));
+  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 511) / 512, held / std::max(sides * tiles, 1u)));
 }
 uint32_t per_split(uint32_t cols, uint32_t splits) { return ((cols + splits - 1) / splits + 127) / 128 * 128; }
 
@@ -638,15 +752,31 @@ void with_pow2(uint32_t n, F&& f) {
   else f(std::integral_constant<int, 8>{});
 }
 
+// Whether tiles take the rows of one adapter from all segments: where segments
+// have a row or two and an adapter two segments or more, as many as a block's
+// scans hold.  256 one-row requests of 16 adapters of rank 128 over 12288
+// columns: 42 us against 130 with a tile per segment, 1024 of them 75 against
+// 496.  With an adapter of its own per request the scans are lost (256 requests
+// of rank 16 51 us against 41), and below 32 segments the tiles are few either
+// way (one request 19 us with both).
+bool grouped(const AdapterArgs& a) {
+  return a.segments >= 32 && a.segments <= kGroupSegments && a.rows / 2 <= a.segments &&
+         a.adapters <= std::min(a.segments / 2, kGroupAdapters);
+}
+// tiles of the groups at most: every adapter, and none, ends in a short one
+uint32_t group_bound(const AdapterArgs& a) {
+  return std::min<uint32_t>(a.rows, a.rows / 16 + std::min(a.adapters + 1, a.segments));
+}
+
 template <bool kColumns>
-void launch_up(UpParams p, const AdapterArgs& a) {
+void launch_up(UpParams p, const AdapterArgs& a, bool group) {
   // column blocks for as many blocks as the card holds at once (tiles of few
   // rows: every further round repeats the search and the sum of h; 57 one-row
   // requests 10.2 us against 12.7 with three rounds) or, with long segments,
   // for three rounds of that, whose last costs little (8192 rows 117 us against
   // 126 with one)
   const uint32_t blocks = tile_blocks(a) == 4 && p.rank <= 64 ? 2 : 1;
-  const uint32_t tiles = tile_bound(a, 16 * blocks), all = (p.cols + 63) / 64;
+  const uint32_t tiles = group ? group_bound(a) : tile_bound(a, 16 * blocks), all = (p.cols + 63) / 64;
   with_pow2((p.rank + 31) / 32, [&](auto kj) {
     constexpr int KJ = decltype(kj)::value;
     if constexpr (KJ <= 4) {
@@ -655,7 +785,13 @@ void launch_up(UpParams p, const AdapterArgs& a) {
         const uint32_t columns = std::max<uint32_t>(1, (RB == 1 ? 1 : 3) * kCus * up_occupancy(KJ, RB) / tiles);
         p.groups = std::max<uint32_t>(1, (all + 4 * columns - 1) / (4 * columns));
         const dim3 grid(tiles, (all + 4 * p.groups - 1) / (4 * p.groups));
-        hipLaunchKernelGGL((adapter_up_kernel<KJ, RB, kColumns>), grid, dim3(256), 0, a.stream, p);
+        if constexpr (RB == 1 && !kColumns) {
+          if (group) {
+            hipLaunchKernelGGL((adapter_up_kernel<KJ, 1, false, true>), grid, dim3(256), 0, a.stream, p);
+            return;
+          }
+        }
+        hipLaunchKernelGGL((adapter_up_kernel<KJ, RB, kColumns, false>), grid, dim3(256), 0, a.stream, p);
       };
       if constexpr (KJ <= 2) {
         if (blocks == 2) {
@@ -733,7 +869,8 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   if (!aligned16(a.x) || !aligned16(a.a) || !aligned16(a.b) || !aligned16(a.base) || !aligned16(a.out) ||
       !aligned4(a.scale) || !aligned4(a.offsets) || !aligned4(a.adapter) || !aligned4(a.error_flag))
     return Invalid("adapter_gemm_alignment_invalid");
-  const uint32_t blocks = tile_blocks(a), tiles = tile_bound(a, 16 * blocks);
+  const bool group = grouped(a);
+  const uint32_t blocks = tile_blocks(a), tiles = group ? group_bound(a) : tile_bound(a, 16 * blocks);
   const uint32_t splits = down_splits(tiles, a.k, a.rank, blocks, 1);
   if (a.workspace_bytes < AdapterGemmWorkspaceBytes(a.rows, a.rank, a.k) || !aligned16(a.workspace))
     return Invalid("adapter_gemm_workspace_invalid");
@@ -744,7 +881,12 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   d.side[0] = DownSide{a.x, a.a, static_cast<float*>(a.workspace), a.x_stride, a.k, per_split(a.k, splits), splits};
   d.err = a.error_flag;
   d.rank = a.rank;
-  launch_down<false>(d, tiles, blocks, splits, a.stream);
+  if (group)
+    with_pow2((a.rank + 15) / 16, [&](auto nj) {
+      hipLaunchKernelGGL((adapter_down_group_kernel<decltype(nj)::value>), dim3(tiles, splits), dim3(256), 0, a.stream,
+                         d);
+    });
+  else launch_down<false>(d, tiles, blocks, splits, a.stream);
   UpParams u{};
   u.seg = d.seg;
   u.h = d.side[0].out;
@@ -757,7 +899,7 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
   u.cols = a.n;
   u.base_stride = a.base_stride;
   u.out_stride = a.out_stride;
-  launch_up<false>(u, a);
+  launch_up<false>(u, a, group);
   return AfterLaunch("adapter_gemm_launch_failed");
 }
 
@@ -813,7 +955,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   u.base_stride = a.base_stride;
   u.out_stride = a.out_stride;
   u.scaled = 1;
-  launch_up<true>(u, a);
+  launch_up<true>(u, a, false);
   GradParams g{};
   g.seg = d.seg;
   g.rank = a.rank;

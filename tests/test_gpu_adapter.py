@@ -360,3 +360,105 @@ def test_other_streams_at_once(eng):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def _mix(seed, count, adapters, longest=2, none=8):
+    """Segments of 0 to `longest` rows and their adapters, every none-th without."""
+    g = np.random.default_rng(seed)
+    ids = g.integers(0, adapters, count)
+    ids[none - 1::none] = -1
+    return g.integers(0, longest + 1, count).tolist(), ids.tolist()
+
+
+# as CASES: short segments, whose tiles take an adapter's rows from all of them
+SHORT = [
+    ([1] * 33, [0] * 33, 16, 72, 520, 1, 0, 0),  # one adapter, two tiles and a row
+    ([1] * 300, [i % 3 for i in range(300)], 128, 136, 1032, 3, 0, 0),  # more segments than threads, tiles across them
+    ([2] * 40, [-1] * 40, 8, 64, 64, 4, 0, 0),  # no adapter at all
+    (*_mix(1, 900, 400), 8, 24, 40, 400, 7, 30),  # more adapters than threads, some without rows, empty segments
+    (*_mix(2, 2048, 5), 24, 40, 264, 6, 0, 0),  # the most segments
+    (*_mix(3, 2048, 1023), 8, 16, 24, 1023, 3, 0),  # and the most adapters
+    ([1, 60] + [0] * 60, [1, 0] * 31, 64, 200, 136, 2, 1, 2),  # one segment has all tiles
+    (*_mix(4, 2049, 9), 8, 32, 64, 9, 0, 0),  # one segment more than the groups take
+]
+
+
+@pytest.mark.parametrize("base", [True, False])
+@pytest.mark.parametrize("case", range(len(SHORT)))
+def test_short_segments(eng, case, base):
+    import torch
+
+    from pih_amd.linear import adapter_gemm
+
+    c = _case(300 + case, *SHORT[case])
+    ref, bound, written = _forward_ref(c, base)
+    d = _dev(c)
+    args = (d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"])
+    out = torch.full_like(d["base"], 7.0)
+    got, flag = adapter_gemm(*args, base=d["base"] if base else None, out=out)
+    w = torch.from_numpy(written)
+    again = adapter_gemm(*args, base=d["base"] if base else None)[0]
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    assert torch.all(got.cpu()[~w] == 7.0)
+    assert torch.equal(got[w.cuda()], again[w.cuda()])
+    _within(got[w.cuda()], ref[w], bound[w], f"case {case}")
+
+
+def test_short_segments_in_place_and_flagged(eng):
+    import torch
+
+    from pih_amd.linear import adapter_gemm
+
+    c = _case(331, [1] * 64, [i % 3 - (i % 3 == 2) * 3 for i in range(64)], 16, 72, 136, 2)
+    d = _dev(c)
+    args = (d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"])
+    want = adapter_gemm(*args, base=d["base"])[0]
+    y = d["base"].clone()
+    assert torch.equal(adapter_gemm(*args, base=y, out=y)[0], want)
+    d["adapters"][6] = 2  # past the stacks
+    out = torch.full_like(want, 7.0)
+    _, flag = adapter_gemm(*args, base=d["base"], out=out)
+    torch.cuda.synchronize()
+    rest = torch.arange(64, device="cuda") != 6
+    assert int(flag.item()) == 1 and torch.all(out[6] == 7.0) and torch.equal(out[rest], want[rest])
+    d["adapters"][6] = 0
+    d["offsets"][64] = 65  # past the rows
+    out.fill_(7.0)
+    _, flag = adapter_gemm(*args, base=d["base"], out=out)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 2 and torch.all(out[63] == 7.0) and torch.equal(out[:63], want[:63])
+    d["offsets"][64] = 62  # descends: the last two segments' rows are in question
+    out.fill_(7.0)
+    _, flag = adapter_gemm(*args, base=d["base"], out=out)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 2 and torch.equal(out[:62], want[:62])
+
+
+def test_short_segments_captured(eng):
+    """A decode batch whose segments change between replays."""
+    import torch
+
+    from pih_amd.linear import adapter_gemm
+
+    c = _case(341, [1] * 96, [i % 4 for i in range(96)], 32, 264, 520, 4)
+    d = _dev(c)
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    call = lambda: adapter_gemm(d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"],  # noqa: E731
+                                base=d["base"], flag=flag)[0]
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.current_stream()):
+        held = call()
+    for i in range(4):
+        g = torch.Generator().manual_seed(350 + i)
+        d["adapters"].copy_(torch.randint(-1, 4, (96,), generator=g).to(torch.int32))
+        d["offsets"].copy_((torch.rand(97, generator=g) * 97).long().sort().values.clamp(max=96).to(torch.int32))
+        d["offsets"][0], d["offsets"][96] = 0, 96
+        eager = call()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, eager)
+    assert int(flag.item()) == 0
