@@ -416,15 +416,16 @@ typedef struct pih_amd_v41_block_dequant_launch_v1 {
  * ascending; an empty segment is allowed) and has adapter a =
  * segment_adapter[s] (u32 [segments]; 0xFFFFFFFF: none, output = base).
  * Segments may share an adapter.  Rows outside every segment are neither
- * read nor written.  A bf16 [adapters][rank][k], B bf16 [adapters][n][rank],
- * scale f32 [adapters] (0: all 1).  base_bf16 may be the output itself (same
+ * read nor written.  Up to 2^26 rows, 65536 segments (every block reads the
+ * offsets) and 32767 adapters.
+ * A bf16 [adapters][rank][k], B bf16 [adapters][n][rank], scale f32 [adapters] (0: all 1).  base_bf16 may be the output itself (same
  * stride) or 0 (the rows start from zero).  input, base and output rows are
  * *_stride elements apart (k, n, n at least).
  * rank a multiple of 8 up to 128; n, k and the strides multiples of 8; every
  * address 16-byte aligned (the u32 and f32 arrays 4-byte).  The product with
  * A is summed in fp32 and enters the second product as the sum of two bf16
  * values (2^-16 relative), so the only rounding to bf16 is the output's.
- * workspace: query_workspace(ADAPTER_GEMM, row_count, rank, k).
+ * workspace (16-byte aligned): query_workspace(ADAPTER_GEMM, row_count, rank, k).
  * Error bits: 1 an adapter id that is neither 0xFFFFFFFF nor below
  * adapter_count (its rows are left unwritten), 2 offsets that descend or
  * pass row_count (the segment is left out). */
@@ -447,7 +448,8 @@ typedef struct pih_amd_adapter_gemm_launch_v1 {
  * base_bf16 (dx's own or 0) carries the shared projection's input gradient;
  * da f32 [adapters][rank][k] and db f32 [adapters][n][rank] are written for
  * every adapter, zero where it has no row.  dx rows outside every segment
- * are left as they are.  Sums run in a fixed order: the same call gives the
+ * are left as they are; dx may be base, but neither dy nor input, which are
+ * read after it is written.  Sums run in a fixed order: the same call gives the
  * same bits.  Conditions, alignment and error bits are those of
  * pih_amd_adapter_gemm_launch_v1.  query_adapter_backward_workspace writes
  * the byte count that `workspace` needs (from row_count, segment_count,
@@ -471,8 +473,8 @@ typedef struct pih_amd_adapter_backward_launch_v1 {
  * input bf16 [rows][hidden], weight bf16 [vocab][hidden], target u32 [rows]
  * (0xFFFFFFFF: the row has none, loss 0), loss f32 [rows], lse f32 [rows].
  * -loss is the target's log-probability.  Logits, maxima and sums are fp32.
- * hidden a multiple of 8, addresses 16-byte aligned (target, loss and lse
- * 4-byte).  workspace: query_workspace(LM_HEAD_LOSS, rows, vocab, hidden).
+ * hidden a multiple of 8, rows, vocab and hidden up to 2^20, addresses 16-byte
+ * aligned (target, loss and lse 4-byte).  workspace: query_workspace(LM_HEAD_LOSS, rows, vocab, hidden).
  * Error bits: 1 a target that is neither 0xFFFFFFFF nor below vocab (the row
  * counts as one without), 4 a non-finite loss (stored). */
 #define PIH_AMD_NO_TARGET_V1 0xFFFFFFFFU
@@ -488,11 +490,13 @@ typedef struct pih_amd_lm_head_loss_launch_v1 {
 /* Gradients of the above from lse (as launch_lm_head_loss wrote it) and the
  * losses' upstream gradient f32 [rows]: with
  *   g[t, v] = loss_grad[t] * (exp(logit[t, v] - lse[t]) - [v == target[t]])
- * rounded to bf16 as the operand of both products,
  *   input_grad  bf16 [rows][hidden]  = g . weight
  *   weight_grad bf16 [vocab][hidden] = g^T . input   (address 0: left out)
- * summed in fp32.  A row without a target gives zeros, whatever its input,
- * lse and loss_grad hold.  Conditions are those of
+ * summed in fp32.  Both products take g as bf16, of whose upstream factor it
+ * holds the mantissa alone (powers of two and the rows' largest factor enter
+ * in fp32 or exactly), so equal factors such as a mean's 1 / rows are not
+ * rounded.  A row without a target gives zeros, whatever its input, lse and
+ * loss_grad hold.  The results lie outside every input.  Conditions are those of
  * pih_amd_lm_head_loss_launch_v1; workspace:
  * query_workspace(LM_HEAD_LOSS_BACKWARD, rows, vocab, hidden).
  * Error bit 1 as above. */
@@ -513,10 +517,11 @@ typedef struct pih_amd_lm_head_loss_backward_launch_v1 {
  *   loss             = coefficient * E / (T * top_k) *
  *                      sum over e of counts[e] * mean_affinity[e]   f32 [1]
  * scores f32 [T, E], topk_ids u32 [T, top_k] (as launch_router_topk reads
- * and writes them); limits as there.  Error bits: 1 a non-finite score (the
+ * and writes them); limits as there, and fewer than 2^27 tokens.  An id
+ * twice in a row counts as two routes.  Error bits: 1 a non-finite score (the
  * row adds nothing to mean_affinity; its routes count), 2 an id >= E (not
  * counted), 4 a row whose affinities sum to 0 (adds nothing).
- * workspace: query_workspace(ROUTER_BALANCE, T, top_k, E). */
+ * workspace (16-byte aligned): query_workspace(ROUTER_BALANCE, T, top_k, E). */
 typedef struct pih_amd_router_balance_launch_v1 {
   uint32_t struct_size, abi_version;
   uintptr_t scores_f32, topk_ids_u32;
@@ -533,8 +538,8 @@ typedef struct pih_amd_router_balance_launch_v1 {
  * 0: none; topk_ids as that entry wrote them, route_scale as it was given):
  * scores_grad f32 [T, E], the sum of both.  The counts and the selection are
  * constants of the differentiation.  A row with error bit 1 or 4 gets zeros,
- * a route with error bit 2 (or an id a second time) adds its own term alone
- * or none. */
+ * a route with error bit 2 has no part in the row's sums; an id twice in a row
+ * is two routes. */
 typedef struct pih_amd_router_backward_launch_v1 {
   uint32_t struct_size, abi_version;
   uintptr_t scores_f32, topk_ids_u32, counts_u32, loss_grad_f32;

@@ -33,6 +33,8 @@ namespace {
 
 constexpr uint32_t kMaxRank = 128;
 constexpr uint32_t kMaxColumns = 1u << 20;
+constexpr uint32_t kMaxRows = 1u << 26;      // a grid has fewer than 2^32 threads
+constexpr uint32_t kMaxSegments = 1u << 16;  // every block reads the offsets
 constexpr uint32_t kErrAdapter = 1u, kErrOffsets = 2u;
 constexpr uint32_t kNoAdapter = 0xffffffffu;
 
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(256) void adapter_grad_reduce_kernel(GradParams p, 
 // ------------------------------------------------------------------ host
 bool shape_ok(const AdapterArgs& a) {
   return a.rows && a.segments && a.adapters && a.rank && a.rank <= kMaxRank && a.rank % 8 == 0 && a.n && a.k &&
-         a.n % 8 == 0 && a.k % 8 == 0 && a.rows <= 0x7fffffffu && a.segments <= 0x7fffffffu &&
+         a.n % 8 == 0 && a.k % 8 == 0 && a.rows <= kMaxRows && a.segments <= kMaxSegments &&
          a.adapters <= 0x7fffu && a.n <= kMaxColumns && a.k <= kMaxColumns;
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -851,7 +853,7 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
 }  // namespace
 
 uint64_t AdapterGemmWorkspaceBytes(uint32_t rows, uint32_t rank, uint32_t k) {
-  if (!rows || !rank || rank > kMaxRank || !k) return 0;
+  if (!rows || rows > kMaxRows || !rank || rank > kMaxRank || !k || k > kMaxColumns) return 0;
   // as many splits as any segments lead to: a tile per 64 or 16 rows at least
   const uint32_t splits = std::max(down_splits((rows + 63) / 64, k, rank, 4, 1), down_splits((rows + 15) / 16, k, rank, 1, 1));
   return (uint64_t)splits * rows * rank * 4;
@@ -916,6 +918,8 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
       !aligned16(a.out) || !aligned16(a.da) || !aligned16(a.db) || !aligned4(a.scale) || !aligned4(a.offsets) ||
       !aligned4(a.adapter) || !aligned4(a.error_flag))
     return Invalid("adapter_backward_alignment_invalid");
+  // (dx is written before the weights' gradients read x and dy)
+  if (a.out == a.x || a.out == a.dy) return Invalid("adapter_backward_alias_invalid");
   const BackwardPlan plan = backward_plan(a);
   if (a.workspace_bytes < plan.bytes || !aligned16(a.workspace)) return Invalid("adapter_backward_workspace_invalid");
   St clean = RequireCleanLastError();

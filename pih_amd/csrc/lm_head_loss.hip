@@ -748,17 +748,18 @@ __global__ __launch_bounds__(256) void loss_live_rows_kernel(const uint16_t* x, 
 __global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, const uint32_t* target, const float* up,
                                                          const float* mantissa, uint16_t* out, uint32_t hidden, uint32_t vocab,
                                                          uint64_t count, uint32_t splits) {
-  const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= count) return;
-  const uint32_t row = (uint32_t)(i / hidden);
-  const bool live = target[row] < vocab;
-  const float f = live ? up[row] / mantissa[row] : 0.0f;
-  v4f v = *reinterpret_cast<const v4f*>(sums + i);
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (uint64_t)gridDim.x * 1024) {
+    const uint32_t row = (uint32_t)(i / hidden);
+    const bool live = target[row] < vocab;
+    const float f = live ? up[row] / mantissa[row] : 0.0f;
+    v4f v = *reinterpret_cast<const v4f*>(sums + i);
 #pragma unroll 8
-  for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(sums + s * count + i);
-  // (a row without a target: 0, whatever the weights' infinities made of it)
-  if (!live) v = v4f{0.f, 0.f, 0.f, 0.f};
-  *reinterpret_cast<uint2*>(out + i) = uint2{f32x2_to_bf16x2(v[0] * f, v[1] * f), f32x2_to_bf16x2(v[2] * f, v[3] * f)};
+    for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(sums + s * count + i);
+    // (a row without a target: 0, whatever the weights' infinities made of it)
+    if (!live) v = v4f{0.f, 0.f, 0.f, 0.f};
+    *reinterpret_cast<uint2*>(out + i) =
+        uint2{f32x2_to_bf16x2(v[0] * f, v[1] * f), f32x2_to_bf16x2(v[2] * f, v[3] * f)};
+  }
 }
 
 template <bool AT, bool BT, int EPI>
@@ -866,6 +867,8 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
   if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.dx, 16) || !aligned(a.dw, 16) || !aligned(a.target, 4) ||
       !aligned(a.lse, 4) || !aligned(a.loss_grad, 4) || !aligned(a.error_flag, 4))
     return Invalid("lm_head_loss_backward_alignment_invalid");
+  // (the weights' gradient of a piece is written before dx reads its weights)
+  if (a.dw == a.w) return Invalid("lm_head_loss_backward_alias_invalid");
   const BackwardPlan plan = backward_plan(a.rows, a.vocab, a.hidden);
   if (a.workspace_bytes < plan.bytes || !aligned(a.workspace, 16))
     return Invalid("lm_head_loss_backward_workspace_invalid");
@@ -975,7 +978,8 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
     launch_gemm<false, true, kEpiAdd>(d, a.stream);
   }
   const uint64_t count = (uint64_t)a.rows * a.hidden;
-  hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, a.stream, sums,
+  hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 20)), dim3(256), 0,
+                     a.stream, sums,
                      a.target, a.loss_grad, mantissa, a.dx, a.hidden, a.vocab, count, plan.splits);
   return AfterLaunch("lm_head_loss_backward_launch_failed");
 }

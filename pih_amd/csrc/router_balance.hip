@@ -33,6 +33,7 @@ namespace pih_amd {
 namespace {
 
 constexpr uint32_t kMaxExperts = 1024, kMaxTopk = 32, kNoId = 0xffffffffu;
+constexpr uint32_t kMaxTokens = (1u << 27) - 1;  // times kMaxTopk below 2^32, the counts' range
 constexpr uint32_t kWaves = 4;          // of the gradient's blocks
 constexpr uint32_t kBalanceWaves = 16;  // of the loss's, whose partial sums one block adds up:
 constexpr uint32_t kBlocks = 128;       // few and large
@@ -338,6 +339,11 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
         for (int c = 0; c < 4; ++c) d[4 * q + c] += v[c];
       }
     }
+    // (0 times an upstream gradient that is not finite)
+    if (row.wrong) {
+#pragma unroll
+      for (int j = 0; j < R::N; ++j) d[j] = 0.0f;
+    }
     float* const out = scores_grad + (uint64_t)t * experts;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
 }
 
 bool shape_ok(uint32_t tokens, uint32_t topk, uint32_t experts) {
-  return tokens && experts && experts <= kMaxExperts && topk && topk <= kMaxTopk && topk <= experts;
+  return tokens && tokens <= kMaxTokens && experts && experts <= kMaxExperts && topk && topk <= kMaxTopk && topk <= experts;
 }
 
 // lanes of a row and float4s a lane holds
@@ -373,6 +379,10 @@ uint32_t balance_blocks(uint32_t tokens, uint32_t experts) {
   return std::min(kBlocks, (tokens + rows - 1) / rows);
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+template <typename... P>
+bool aligned4(P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % 4 == 0) && ...);
+}
 
 }  // namespace
 
@@ -387,6 +397,8 @@ St LaunchRouterBalance(const RouterBalanceArgs& a) {
   if (!shape_ok(a.tokens, a.topk, a.experts)) return Invalid("router_balance_shape_invalid");
   if (a.mode != kRouterSoftmax && a.mode != kRouterSqrtSoftplus) return Invalid("router_balance_mode_invalid");
   if (!__builtin_isfinite(a.coefficient)) return Invalid("router_balance_coefficient_invalid");
+  if (!aligned4(a.scores, a.ids, a.loss, a.counts, a.mean, a.error_flag))
+    return Invalid("router_balance_alignment_invalid");
   if (a.workspace_bytes < RouterBalanceWorkspaceBytes(a.tokens, a.topk, a.experts) ||
       !aligned16(a.workspace))
     return Invalid("router_balance_workspace_invalid");
@@ -418,6 +430,8 @@ St LaunchRouterBackward(const RouterBackwardArgs& a) {
   if (a.mode != kRouterSoftmax && a.mode != kRouterSqrtSoftplus) return Invalid("router_backward_mode_invalid");
   if (!__builtin_isfinite(a.coefficient)) return Invalid("router_backward_coefficient_invalid");
   if (!__builtin_isfinite(a.scale) || a.scale <= 0.0f) return Invalid("router_backward_scale_invalid");
+  if (!aligned4(a.scores, a.ids, a.counts, a.loss_grad, a.weights_grad, a.scores_grad, a.error_flag))
+    return Invalid("router_backward_alignment_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
   // of a score's own term: the loss's weight over T

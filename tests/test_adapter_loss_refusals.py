@@ -35,7 +35,8 @@ def _adapter_gemm(**over):
 
 def _adapter_backward(**over):
     f = dict(workspace_bytes=1 << 40, row_count=33, segment_count=2, adapter_count=3, rank=16, n=64, k=128,
-             output_grad_stride=64, input_stride=128, base_stride=128, input_grad_stride=128)
+             output_grad_stride=64, input_stride=128, base_stride=128, input_grad_stride=128, input_bf16=0x20000,
+             output_grad_bf16=0x30000)
     f.update(over)
     return "launch_adapter_backward", _fill("adapter_backward", **f)
 
@@ -47,7 +48,7 @@ def _loss(**over):
 
 
 def _loss_backward(**over):
-    f = dict(workspace_bytes=1 << 40, rows=5, vocab=100, hidden=64)
+    f = dict(workspace_bytes=1 << 40, rows=5, vocab=100, hidden=64, weight_bf16=0x20000)
     f.update(over)
     return "launch_lm_head_loss_backward", _fill("lm_head_loss_backward", **f)
 
@@ -100,6 +101,18 @@ BAD += [(_balance, {f: 0}) for f in ("loss_f32", "counts_u32", "mean_affinity_f3
 BAD += [(_router_backward, f) for f in ({"scores_grad_f32": 0}, {"counts_u32": 0},
                                         {"loss_grad_f32": 0, "topk_weights_grad_f32": 0}, {"route_scale": 0.0},
                                         {"route_scale": -1.0}, {"route_scale": INF})]
+# more tokens than the counts hold, rows than a grid has threads, segments than
+# a block's search ends in; addresses between two words; results over inputs
+BAD += [(make, {"token_count": 1 << 27}) for make in (_balance, _router_backward)]
+BAD += [(make, {f: v}) for make in (_adapter_gemm, _adapter_backward)
+        for f, v in (("row_count", (1 << 26) + 1), ("segment_count", (1 << 16) + 1))]
+BAD += [(_balance, {f: 0x10002}) for f in ("scores_f32", "topk_ids_u32", "loss_f32", "counts_u32", "mean_affinity_f32",
+                                           "error_flag_u32")]
+BAD += [(_router_backward, {f: 0x10002}) for f in ("scores_f32", "topk_ids_u32", "counts_u32", "loss_grad_f32",
+                                                   "topk_weights_grad_f32", "scores_grad_f32", "error_flag_u32")]
+BAD += [(_adapter_backward, {"input_grad_bf16": 0x20000, "base_bf16": 0}),
+        (_adapter_backward, {"input_grad_bf16": 0x30000, "base_bf16": 0}),
+        (_loss_backward, {"weight_grad_bf16": 0x20000})]
 
 
 @pytest.mark.parametrize("make,over", BAD, ids=lambda v: v.__name__ if callable(v) else str(v))
@@ -135,7 +148,9 @@ def test_workspace_one_byte_short():
                                         (abi.WORKSPACE_LM_HEAD_LOSS, (4, 0, 64)),
                                         (abi.WORKSPACE_LM_HEAD_LOSS, (4, 10, 60)),
                                         (abi.WORKSPACE_LM_HEAD_LOSS_BACKWARD, (0, 10, 64)),
-                                        (abi.WORKSPACE_ROUTER_BALANCE, (4, 9, 8))])
+                                        (abi.WORKSPACE_ROUTER_BALANCE, (4, 9, 8)),
+                                        (abi.WORKSPACE_ROUTER_BALANCE, (1 << 27, 4, 8)),
+                                        (abi.WORKSPACE_ADAPTER_GEMM, ((1 << 26) + 1, 16, 128))])
 def test_workspace_query_refuses_shapes(kind, shape):
     assert _query(kind, *shape)[0] == abi.INVALID_ARGUMENT
 

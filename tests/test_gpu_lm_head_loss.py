@@ -292,3 +292,51 @@ def test_captured_and_replayed(eng):
         for p, q in zip(held, eager):
             assert torch.equal(p, q)
     assert int(flag.item()) == 0
+
+
+# tiles of 128 and 256 rows (the sizes above take 64), of every product: the
+# logits' in the first two, dx's in the others, whose columns are split too
+@pytest.mark.parametrize("rows,vocab,hidden", [(1003, 8190, 64), (301, 29999, 64), (1000, 8200, 2048),
+                                               (190, 16380, 2048)])
+def test_taller_tiles(eng, rows, vocab, hidden):
+    import torch
+
+    from pih_amd.linear import lm_head_loss, lm_head_loss_backward
+
+    x, w, target, up = (t.cuda() for t in _case(rows + vocab, rows, vocab, hidden))
+    _, _, lse, elog, loss, eloss, live, _ = _ref(x, w, target)
+    got, glse, flag = lm_head_loss(x, w, target)
+    torch.cuda.synchronize()
+    _within(glse, lse.cpu(), elog.cpu(), "lse")
+    _within(got, loss.cpu(), eloss.cpu(), "loss")
+    (dx, ex), (dw, ew) = _grads_ref(x, w, target, up, lse.float())
+    gx, gw, _ = lm_head_loss_backward(x, w, target, lse.float(), up, flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.all(got[~live] == 0) and torch.all(gx[~live] == 0)
+    _within(gx, dx.cpu(), ex.cpu(), "dx")
+    _within(gw, dw.cpu(), ew.cpu(), "dw")
+
+
+def test_other_streams_at_once(eng):
+    """Forward and backward on two streams, each with the workspaces of its own calls."""
+    import torch
+
+    from pih_amd.linear import lm_head_loss, lm_head_loss_backward
+
+    cases = [[t.cuda() for t in _case(90 + i, 200, 3000, 256)] for i in range(2)]
+
+    def call(x, w, target, up):
+        loss, lse, flag = lm_head_loss(x, w, target)
+        return (loss,) + lm_head_loss_backward(x, w, target, lse, up, flag=flag)[:2]
+
+    want = [call(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(p, q) for g in got[i] for p, q in zip(g, want[i]))

@@ -235,3 +235,49 @@ def test_counts_are_the_route_plan_s(eng):
     torch.cuda.synchronize()
     assert int(flag.item()) == 0
     np.testing.assert_array_equal(np.diff(offsets.cpu().numpy()), counts.cpu().numpy())
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("t,e,k", [(33, 67, 3), (5, 2, 2), (129, 301, 7), (40, 515, 9), (9, 1023, 31), (9001, 63, 2)])
+def test_odd_expert_counts(eng, t, e, k, mode):
+    """Rows that are not 16-byte aligned, and more rows than a round of blocks."""
+    test_against_64_bits(eng, t, e, k, mode)
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_an_id_twice_is_two_routes(eng, mode):
+    import torch
+
+    from pih_amd.linear import router_backward, router_balance
+
+    scores, ids, dweights = _case(61, 50, 96, 5)
+    ids[:, 3] = ids[:, 1]
+    loss, counts, mean, grad, bound = _ref(scores, ids, mode, 0.05, 1.25, dweights, 2.0)
+    s, i = scores.cuda(), ids.cuda()
+    _, gc, _, flag = router_balance(s, i, mode, 0.05)
+    got, _ = router_backward(s, i, gc, mode, 0.05, torch.tensor([1.25], device="cuda"), dweights=dweights.cuda(),
+                             route_scale=2.0, flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.equal(gc.cpu().long(), counts)
+    # (the two routes' magnitudes add up in the bound as their terms do)
+    assert float(((got.cpu().double() - grad).abs() / bound).max()) <= 1.0
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_a_bad_row_is_zeros_whatever_its_upstream(eng, mode):
+    import torch
+
+    from pih_amd.linear import router_backward, router_balance
+
+    scores, ids, dweights = _case(67, 21, 64, 4)
+    want = _ref(scores, ids, mode, 0.1, 1.0, dweights, 1.0)[3]
+    scores[8, 5] = float("nan")
+    dweights[8] = torch.tensor([float("inf"), float("nan"), 1.0, -float("inf")])
+    s, i, dw = scores.cuda(), ids.cuda(), dweights.cuda()
+    _, counts, _, flag = router_balance(s, i, mode, 0.1)
+    got, _ = router_backward(s, i, None, mode, 0.0, None, dweights=dw, flag=flag)
+    nan, _ = router_backward(s, i, counts, mode, 0.1, torch.full((1,), float("nan"), device="cuda"), flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 1
+    assert torch.all(got[8] == 0) and torch.all(nan[8] == 0) and torch.all(nan[9].isnan())
+    assert bool(torch.isfinite(got).all()) and want.shape == got.shape
