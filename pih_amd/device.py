@@ -88,21 +88,25 @@ def ptr(t: Optional[torch.Tensor]) -> int:
     return t.data_ptr()
 
 
-def rows_ptr(t: Optional[torch.Tensor]) -> int:
-    """The address of a 2-D tensor whose rows are contiguous, at any distance
-    from one another (a column slice of a wider tensor)."""
-    if t is None:
-        return 0
-    if not t.is_cuda:
-        raise ValueError("pih_amd: tensor must live on the HIP device")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError("pih_amd: tensor rows must be contiguous")
-    return t.data_ptr()
+def device_ptrs(*tensors: Optional[torch.Tensor]) -> list:
+    """The addresses of contiguous tensors (None: 0), which all live on the
+    current device, to whose stream the launches go."""
+    current = torch._C._cuda_getDevice()
+    out = []
+    for t in tensors:
+        if t is None:
+            out.append(0)
+            continue
+        if t.get_device() != current:
+            raise ValueError("pih_amd: tensor must live on the current HIP device")
+        if not t.is_contiguous():
+            raise ValueError("pih_amd: tensor must be contiguous")
+        out.append(t.data_ptr())
+    return out
 
 
 def same_device(*tensors: Optional[torch.Tensor]) -> None:
-    """The launches go to the current device's stream: every tensor must live
-    there."""
+    """The same of tensors whose addresses are at hand."""
     current = torch._C._cuda_getDevice()
     for t in tensors:
         if t is not None and t.get_device() != current:

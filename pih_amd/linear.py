@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import abi
-from .device import error_flag, ptr, rows_ptr, same_device, stream_handle
+from .device import device_ptrs, error_flag, ptr, same_device, stream_handle
 
 
 class KernelError(RuntimeError):
@@ -537,10 +537,14 @@ def _adapter_stacks(a, b, scale, offsets, adapters):
     return count, rank, n, k
 
 
-def _rows(t, rows: int, cols: int, what: str) -> int:
+def _rows(t, rows: int, cols: int, what: str):
+    """Address and row stride of a tensor whose rows are contiguous."""
     if t.shape != (rows, cols) or t.dtype != torch.bfloat16:
         raise ValueError(f"pih_amd: {what} is bfloat16 [{rows}, {cols}]")
-    return t.stride(0) if rows > 1 else cols
+    row, col = t.stride()
+    if col != 1 and cols > 1:
+        raise ValueError("pih_amd: tensor rows must be contiguous")
+    return t.data_ptr(), row if rows > 1 else cols
 
 
 def adapter_gemm(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: Optional[torch.Tensor],
@@ -556,17 +560,17 @@ def adapter_gemm(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: Optio
     left as they are.  Returns (out, flag)."""
     count, rank, n, k = _adapter_stacks(a, b, scale, offsets, adapters)
     rows = x.shape[0]
-    xs = _rows(x, rows, k, "the adapters' input")
-    bs = 0 if base is None else _rows(base, rows, n, "the adapters' base")
+    px, xs = _rows(x, rows, k, "the adapters' input")
+    pbase, bs = (0, 0) if base is None else _rows(base, rows, n, "the adapters' base")
     if out is None:
         out = torch.empty(rows, n, dtype=torch.bfloat16, device=x.device)
-    os = _rows(out, rows, n, "the adapters' output")
+    pout, os = _rows(out, rows, n, "the adapters' output")
     flag = error_flag() if flag is None else flag
-    same_device(x, a, b, scale, offsets, adapters, base, out, flag)
+    same_device(x, base, out)
+    pa, pb, ps, po, pi, pflag = device_ptrs(a, b, scale, offsets, adapters, flag)
     ws = _workspace(abi.WORKSPACE_ADAPTER_GEMM, rows, rank, k, x.device)
-    _launch("launch_adapter_gemm", "adapter_gemm", rows_ptr(x), ptr(a), ptr(b), ptr(scale), ptr(offsets),
-            ptr(adapters), rows_ptr(base), rows_ptr(out), ws.data_ptr(), ws.numel(), ptr(flag), stream_handle(), rows,
-            adapters.shape[0], count, rank, n, k, xs, bs, os)
+    _launch("launch_adapter_gemm", "adapter_gemm", px, pa, pb, ps, po, pi, pbase, pout, ws.data_ptr(), ws.numel(),
+            pflag, stream_handle(), rows, adapters.shape[0], count, rank, n, k, xs, bs, os)
     return out, flag
 
 
@@ -590,20 +594,22 @@ def adapter_backward(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torc
     that share an adapter add up; an adapter without rows has zeros."""
     count, rank, n, k = _adapter_stacks(a, b, scale, offsets, adapters)
     rows = x.shape[0]
-    ys, xs = _rows(dy, rows, n, "the upstream gradient"), _rows(x, rows, k, "the adapters' input")
-    bs = 0 if base is None else _rows(base, rows, k, "the gradient's base")
+    pdy, ys = _rows(dy, rows, n, "the upstream gradient")
+    px, xs = _rows(x, rows, k, "the adapters' input")
+    pbase, bs = (0, 0) if base is None else _rows(base, rows, k, "the gradient's base")
     if out is None:
         out = torch.empty(rows, k, dtype=torch.bfloat16, device=x.device)
-    os = _rows(out, rows, k, "the input's gradient")
+    pout, os = _rows(out, rows, k, "the input's gradient")
     da = torch.empty(a.shape, dtype=torch.float32, device=x.device)
     db = torch.empty(b.shape, dtype=torch.float32, device=x.device)
     flag = error_flag() if flag is None else flag
-    same_device(dy, x, a, b, scale, offsets, adapters, base, out, flag)
+    same_device(dy, x, base, out)
+    pa, pb, ps, po, pi, pflag = device_ptrs(a, b, scale, offsets, adapters, flag)
     ws = torch.empty(_adapter_backward_bytes(rows, adapters.shape[0], count, rank, n, k), dtype=torch.uint8,
                      device=x.device)
-    _launch("launch_adapter_backward", "adapter_backward", rows_ptr(dy), rows_ptr(x), ptr(a), ptr(b), ptr(scale),
-            ptr(offsets), ptr(adapters), rows_ptr(base), rows_ptr(out), da.data_ptr(), db.data_ptr(), ws.data_ptr(),
-            ws.numel(), 0, ptr(flag), stream_handle(), rows, adapters.shape[0], count, rank, n, k, ys, xs, bs, os)
+    _launch("launch_adapter_backward", "adapter_backward", pdy, px, pa, pb, ps, po, pi, pbase, pout, da.data_ptr(),
+            db.data_ptr(), ws.data_ptr(), ws.numel(), 0, pflag, stream_handle(), rows, adapters.shape[0], count, rank,
+            n, k, ys, xs, bs, os)
     return out, da, db, flag
 
 
@@ -624,10 +630,10 @@ def lm_head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
     loss = torch.empty(rows, dtype=torch.float32, device=x.device)
     lse = torch.empty(rows, dtype=torch.float32, device=x.device)
     flag = error_flag() if flag is None else flag
-    same_device(x, weight, targets, flag)
+    px, pw, pt, pflag = device_ptrs(x, weight, targets, flag)
     ws = _workspace(abi.WORKSPACE_LM_HEAD_LOSS, rows, vocab, hidden, x.device)
-    _launch("launch_lm_head_loss", "lm_head_loss", ptr(x), ptr(weight), ptr(targets), loss.data_ptr(), lse.data_ptr(),
-            ws.data_ptr(), ws.numel(), ptr(flag), stream_handle(), rows, vocab, hidden)
+    _launch("launch_lm_head_loss", "lm_head_loss", px, pw, pt, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
+            pflag, stream_handle(), rows, vocab, hidden)
     return loss, lse, flag
 
 
@@ -640,13 +646,13 @@ def lm_head_loss_backward(x: torch.Tensor, weight: torch.Tensor, targets: torch.
     rows, vocab, hidden = _loss_inputs(x, weight, targets)
     _want(lse.dtype == dloss.dtype == torch.float32 and lse.shape == dloss.shape == x.shape[:1],
           "lse and dloss are float32 [rows]")
+    flag = error_flag() if flag is None else flag
+    px, pw, pt, pl, pd, pflag = device_ptrs(x, weight, targets, lse, dloss, flag)
     dx = torch.empty_like(x)
     dw = torch.empty_like(weight) if weight_gradient else None
-    flag = error_flag() if flag is None else flag
-    same_device(x, weight, targets, lse, dloss, flag)
     ws = _workspace(abi.WORKSPACE_LM_HEAD_LOSS_BACKWARD, rows, vocab, hidden, x.device)
-    _launch("launch_lm_head_loss_backward", "lm_head_loss_backward", ptr(x), ptr(weight), ptr(targets), ptr(lse),
-            ptr(dloss), ptr(dx), ptr(dw), ws.data_ptr(), ws.numel(), ptr(flag), stream_handle(), rows, vocab, hidden)
+    _launch("launch_lm_head_loss_backward", "lm_head_loss_backward", px, pw, pt, pl, pd, dx.data_ptr(),
+            0 if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel(), pflag, stream_handle(), rows, vocab, hidden)
     return dx, dw, flag
 
 
@@ -669,11 +675,10 @@ def router_balance(scores: torch.Tensor, topk_ids: torch.Tensor, mode: int, coef
     counts = torch.empty(experts, dtype=torch.int32, device=dev)
     mean = torch.empty(experts, dtype=torch.float32, device=dev)
     flag = error_flag() if flag is None else flag
-    same_device(scores, topk_ids, flag)
+    ps, pi, pflag = device_ptrs(scores, topk_ids, flag)
     ws = _workspace(abi.WORKSPACE_ROUTER_BALANCE, tokens, topk, experts, dev)
-    _launch("launch_router_balance", "router_balance", ptr(scores), ptr(topk_ids), loss.data_ptr(), counts.data_ptr(),
-            mean.data_ptr(), ws.data_ptr(), ws.numel(), ptr(flag), stream_handle(), tokens, experts, topk, mode,
-            coefficient)
+    _launch("launch_router_balance", "router_balance", ps, pi, loss.data_ptr(), counts.data_ptr(), mean.data_ptr(),
+            ws.data_ptr(), ws.numel(), pflag, stream_handle(), tokens, experts, topk, mode, coefficient)
     return loss, counts, mean, flag
 
 
@@ -691,10 +696,9 @@ def router_backward(scores: torch.Tensor, topk_ids: torch.Tensor, counts: Option
           "dloss is float32 [1] and comes with counts int32 [experts]")
     _want(dweights is None or (dweights.dtype == torch.float32 and dweights.shape == topk_ids.shape),
           "dweights is float32 [tokens, top_k]")
-    dscores = torch.empty_like(scores)
     flag = error_flag() if flag is None else flag
-    same_device(scores, topk_ids, counts, dloss, dweights, flag)
-    _launch("launch_router_backward", "router_backward", ptr(scores), ptr(topk_ids), ptr(counts), ptr(dloss),
-            ptr(dweights), dscores.data_ptr(), ptr(flag), stream_handle(), tokens, experts, topk, mode, coefficient,
-            route_scale)
+    ps, pi, pc, pl, pw, pflag = device_ptrs(scores, topk_ids, counts, dloss, dweights, flag)
+    dscores = torch.empty_like(scores)
+    _launch("launch_router_backward", "router_backward", ps, pi, pc, pl, pw, dscores.data_ptr(), pflag,
+            stream_handle(), tokens, experts, topk, mode, coefficient, route_scale)
     return dscores, flag
