@@ -297,34 +297,41 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
       const uint32_t e = min(64 * i + lane, pieces - 1);
       put[i] = e / per_row * pitch + e % per_row * 16;
     }
+    // (as many columns' loads together as registers hold, as above)
+    constexpr int Q = NJ + RB <= 6 ? 4 : NJ + RB <= 8 ? 2 : 1;
     for (uint32_t c = c0 + 128 * wave; c < c1; c += 512) {
 #pragma unroll
-      for (uint32_t q = 0; q < 4; ++q) {
-        const uint32_t cq = c + 32 * q;
-        if (cq >= c1) break;
-        const uint32_t at = cq + 8 * lg, valid = min(32u, c1 - cq) * per_row;
-        v4i x[RB], m[NJ];
+      for (uint32_t q0 = 0; q0 < 4; q0 += Q) {
+        v4i x[Q][RB], m[Q][NJ];
 #pragma unroll
-        for (int r = 0; r < RB; ++r) {
-          x[r] = v4i{0, 0, 0, 0};
-          if (at < c1) x[r] = load16(src[r] + at);
+        for (uint32_t q = 0; q < Q; ++q) {
+          const uint32_t cq = c + 32 * (q0 + q), at = cq + 8 * lg, valid = cq < c1 ? min(32u, c1 - cq) * per_row : 0;
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            x[q][r] = v4i{0, 0, 0, 0};
+            if (at < c1) x[q][r] = load16(src[r] + at);
+          }
+#pragma unroll
+          for (int i = 0; i < NJ; ++i) {
+            m[q][i] = v4i{0, 0, 0, 0};
+            if (64u * i + lane < valid) m[q][i] = load16(w + (uint64_t)cq * rank + 8 * (64 * i + lane));
+          }
         }
 #pragma unroll
-        for (int i = 0; i < NJ; ++i) {
-          m[i] = v4i{0, 0, 0, 0};
-          if (64u * i + lane < valid) m[i] = load16(w + (uint64_t)cq * rank + 8 * (64 * i + lane));
+        for (uint32_t q = 0; q < Q; ++q) {
+          if (c + 32 * (q0 + q) >= c1) break;
+#pragma unroll
+          for (int i = 0; i < NJ; ++i)
+            if (64u * i + lane < pieces) *reinterpret_cast<v4i*>(st + put[i]) = m[q][i];
+          wave_lds_order();
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            const v4i a = transposed(st + (8 * lg + (lr >> 2)) * pitch + 32 * j + 8 * (lr & 3), pitch);
+#pragma unroll
+            for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a, x[q][r], acc[r][j]);
+          }
+          wave_lds_order();
         }
-#pragma unroll
-        for (int i = 0; i < NJ; ++i)
-          if (64u * i + lane < pieces) *reinterpret_cast<v4i*>(st + put[i]) = m[i];
-        wave_lds_order();
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const v4i a = transposed(st + (8 * lg + (lr >> 2)) * pitch + 32 * j + 8 * (lr & 3), pitch);
-#pragma unroll
-          for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a, x[r], acc[r][j]);
-        }
-        wave_lds_order();
       }
     }
     __syncthreads();
@@ -403,8 +410,9 @@ constexpr int up_occupancy(int kj, int rb) { return kj == 1 ? (rb == 1 ? 4 : 3) 
 template <int KJ, int RB, bool kColumns, bool kGroup>
 __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(UpParams p) {
   static_assert(!kGroup || RB == 1, "a group's tile has 16 rows");
-  constexpr uint32_t kRow = KJ * 32 + 4, kPitch = 128 + 16;
+  constexpr uint32_t kRow = KJ * 32 + 4, kPitch = 128 + 16, kSumRow = 64 + 4;
   __shared__ __align__(16) float hs[16 * RB * kRow];
+  __shared__ __align__(16) float sums[4 * 16 * kSumRow];
   __shared__ __align__(16) uint8_t staged[kColumns ? 4 * 32 * kPitch : 16];
   __shared__ std::conditional_t<kGroup, GroupShared, char> group;
   Tile t;
@@ -424,13 +432,17 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), rank = p.rank;
   const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * rank * p.cols;
   uint8_t* const st = staged + (kColumns ? wave * 32 * kPitch : 0);
-  uint64_t base_row[RB], out_row[RB];
+  float* const mine = sums + wave * 16 * kSumRow;
+  // base and out: rows 8 h + (lane >> 3) of 16, 8 columns a lane
+  uint64_t base_row[RB][2], out_row[RB][2];
 #pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const uint32_t row = row_of(min(16 * r + lr, t.rows - 1));
-    base_row[r] = (uint64_t)row * p.base_stride;
-    out_row[r] = (uint64_t)row * p.out_stride;
-  }
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t row = row_of(min(16 * r + 8 * h + (lane >> 3), t.rows - 1));
+      base_row[r][h] = (uint64_t)row * p.base_stride;
+      out_row[r][h] = (uint64_t)row * p.out_stride;
+    }
 
   struct Group {
     v4i x[KJ][4], b[RB][2];
@@ -456,8 +468,8 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {
         v.b[r][h] = v4i{0, 0, 0, 0};
-        const uint32_t c = c0 + 32 * h + 8 * lg;
-        if (p.base && c < p.cols) v.b[r][h] = load16_once(p.base + base_row[r] + c);
+        const uint32_t c = c0 + 8 * (lane & 7);
+        if (p.base && c < p.cols) v.b[r][h] = load16_once(p.base + base_row[r][h] + c);
       }
   };
   v4i hi[RB][KJ], lo[RB][KJ];
@@ -492,21 +504,33 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
       }
     }
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int r = 0; r < RB; ++r) {
+      // through the wave's LDS, so that a load or store has whole lines
+      if (live) {
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+          *reinterpret_cast<v4f*>(mine + lr * kSumRow + 32 * (u >> 1) + 8 * lg + 4 * (u & 1)) = acc[r][u];
+        wave_lds_order();
+      }
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t c = c0 + 32 * h + 8 * lg;
-        v4i o;
+        const uint32_t row = 8 * h + (lane >> 3), c = 8 * (lane & 7);
+        v4i o = v.b[r][h];  // (without an adapter base goes through bit for bit, a -0 too)
+        if (live) {
+          const v4f y0 = *reinterpret_cast<const v4f*>(mine + row * kSumRow + c);
+          const v4f y1 = *reinterpret_cast<const v4f*>(mine + row * kSumRow + c + 4);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t bits = (uint32_t)v.b[r][h][i];
-          const v4f y = acc[r][2 * h + i / 2];
-          o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y[2 * (i & 1)],
-                                      bf16_bits_to_f32(bits >> 16) + y[2 * (i & 1) + 1]);
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t bits = (uint32_t)v.b[r][h][i];
+            const v4f y = i < 2 ? y0 : y1;
+            o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y[2 * (i & 1)],
+                                        bf16_bits_to_f32(bits >> 16) + y[2 * (i & 1) + 1]);
+          }
         }
-        // (without an adapter base goes through bit for bit, a -0 too)
-        if (16 * r + lr < t.rows && c < p.cols) *reinterpret_cast<v4i*>(p.out + out_row[r] + c) = live ? o : v.b[r][h];
+        if (16 * r + row < t.rows && c0 + c < p.cols) *reinterpret_cast<v4i*>(p.out + out_row[r][h] + c0 + c) = o;
       }
+      if (live) wave_lds_order();
+    }
   };
 
   // the wave's groups: wave, wave + 4, .. of the block's
