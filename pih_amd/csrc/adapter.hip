@@ -233,6 +233,14 @@ struct DownParams {
   uint32_t rank;
 };
 
+// a wave's LDS: 16 rows of 64 columns, and (kColumns) 32 rows of the weights
+constexpr uint32_t kTurnPitch = 128 + 16, kTurn = 16 * kTurnPitch;
+template <int NJ, bool kColumns>
+constexpr uint32_t kDownWave = kTurn + (kColumns ? 32 * (NJ * 32 + 16) : 0);
+// a block's: that, or the sums of its waves
+template <int NJ, bool kColumns>
+constexpr uint32_t kDownLds = std::max(4 * kDownWave<NJ, kColumns>, 4u * 16 * (NJ * 16 + 4) * 4);
+
 // One tile of 16 RB rows times the rank columns of its adapter over a range
 // of cols; the four waves take 128-column pieces in turn.  kColumns: 32 rows
 // of the weights (one contiguous piece of memory) go through the wave's LDS
@@ -250,47 +258,75 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
   for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  const uint16_t* src[RB];
+  // 64 columns of 16 rows at a time: rows 8 h + (lane >> 3), 8 columns a lane,
+  // so that a load has whole lines; turned in the wave's LDS to a row per lane
+  const uint16_t* src[RB][2];
 #pragma unroll
-  for (int r = 0; r < RB; ++r) src[r] = d.src + (uint64_t)row_of(min(16 * r + lr, t.rows - 1)) * d.stride;
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+      src[r][h] = d.src + (uint64_t)row_of(min(16 * r + 8 * h + (lane >> 3), t.rows - 1)) * d.stride;
+  uint8_t* const turn = lds + wave * kDownWave<NJ, kColumns>;
+  auto turned = [&](const v4i (&v)[2], v4i (&to)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+      *reinterpret_cast<v4i*>(turn + (8 * h + (lane >> 3)) * kTurnPitch + (lane & 7) * 16) = v[h];
+    wave_lds_order();
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q) to[q] = *reinterpret_cast<const v4i*>(turn + lr * kTurnPitch + 64 * q + 16 * lg);
+    wave_lds_order();
+  };
   const uint16_t* const w = d.w + (uint64_t)t.adapter * rank * d.cols;
   if constexpr (!kColumns) {
-    const uint16_t* wr[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) wr[j] = w + (uint64_t)min(16 * j + lr, rank - 1) * d.cols;
+    // 128 columns together while registers hold them, else 64
+    constexpr uint32_t U = NJ + RB <= 6 ? 2 : 1;
+    const uint16_t* const wl = w + (uint64_t)(lane >> 3) * d.cols;
     for (uint32_t c = c0 + 128 * wave; c < c1; c += 512) {
-      // 128 columns together while registers hold them, else 32
-      constexpr int Q = NJ + RB <= 6 ? 4 : 2;
 #pragma unroll
-      for (uint32_t q0 = 0; q0 < 4; q0 += Q) {
-        v4i x[Q][RB], a[Q][NJ];
+      for (uint32_t u0 = 0; u0 < 2; u0 += U) {
+        v4i x[U][RB][2], a[U][NJ][2];
 #pragma unroll
-        for (uint32_t q = 0; q < Q; ++q) {
-          const uint32_t at = c + 32 * (q0 + q) + 8 * lg;
+        for (uint32_t u = 0; u < U; ++u) {
+          const uint32_t at = c + 64 * (u0 + u) + 8 * (lane & 7);
 #pragma unroll
-          for (int r = 0; r < RB; ++r) {
-            x[q][r] = v4i{0, 0, 0, 0};
-            if (at < c1) x[q][r] = load16(src[r] + at);
-          }
+          for (uint32_t h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            a[q][j] = v4i{0, 0, 0, 0};
-            if (at < c1) a[q][j] = load16(wr[j] + at);
+            for (int r = 0; r < RB; ++r) {
+              x[u][r][h] = v4i{0, 0, 0, 0};
+              if (at < c1) x[u][r][h] = load16(src[r][h] + at);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+              // (rows past the rank repeat its last eight)
+              a[u][j][h] = v4i{0, 0, 0, 0};
+              if (at < c1) a[u][j][h] = load16(wl + (uint64_t)min(16u * j + 8 * h, rank - 8) * d.cols + at);
+            }
           }
         }
 #pragma unroll
-        for (uint32_t q = 0; q < Q; ++q)
+        for (uint32_t u = 0; u < U; ++u) {
+          if (c + 64 * (u0 + u) >= c1) break;
+          v4i at[NJ][2];
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+          for (int j = 0; j < NJ; ++j) turned(a[u][j], at[j]);
 #pragma unroll
-            for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a[q][j], x[q][r], acc[r][j]);
+          for (int r = 0; r < RB; ++r) {
+            v4i xt[2];
+            turned(x[u][r], xt);
+#pragma unroll
+            for (uint32_t q = 0; q < 2; ++q)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) acc[r][j] = mfma(at[j][q], xt[q], acc[r][j]);
+          }
+        }
       }
     }
+    __syncthreads();
   } else {
     // LDS rows of 2 rank + 16 bytes; 16-byte piece i of a lane is number
     // 64 i + lane of the 4 rank pieces of 32 rows
     const uint32_t pitch = 2 * rank + 16, per_row = rank / 8, pieces = 32 * per_row;
-    uint8_t* const st = lds + wave * 32 * (NJ * 32 + 16);
+    uint8_t* const st = turn + kTurn;
     uint32_t put[NJ];
 #pragma unroll
     for (int i = 0; i < NJ; ++i) {
@@ -298,39 +334,49 @@ __device__ __forceinline__ void down_tile(const DownParams& p, const DownSide& d
       put[i] = e / per_row * pitch + e % per_row * 16;
     }
     // (as many columns' loads together as registers hold, as above)
-    constexpr int Q = NJ + RB <= 6 ? 4 : NJ + RB <= 8 ? 2 : 1;
+    constexpr int U = NJ + RB <= 6 ? 2 : 1;
     for (uint32_t c = c0 + 128 * wave; c < c1; c += 512) {
 #pragma unroll
-      for (uint32_t q0 = 0; q0 < 4; q0 += Q) {
-        v4i x[Q][RB], m[Q][NJ];
+      for (uint32_t u0 = 0; u0 < 2; u0 += U) {
+        v4i x[U][RB][2], m[U][2][NJ];
 #pragma unroll
-        for (uint32_t q = 0; q < Q; ++q) {
-          const uint32_t cq = c + 32 * (q0 + q), at = cq + 8 * lg, valid = cq < c1 ? min(32u, c1 - cq) * per_row : 0;
+        for (uint32_t u = 0; u < U; ++u) {
+          const uint32_t cu = c + 64 * (u0 + u), at = cu + 8 * (lane & 7);
 #pragma unroll
-          for (int r = 0; r < RB; ++r) {
-            x[q][r] = v4i{0, 0, 0, 0};
-            if (at < c1) x[q][r] = load16(src[r] + at);
-          }
+          for (uint32_t h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int i = 0; i < NJ; ++i) {
-            m[q][i] = v4i{0, 0, 0, 0};
-            if (64u * i + lane < valid) m[q][i] = load16(w + (uint64_t)cq * rank + 8 * (64 * i + lane));
+            for (int r = 0; r < RB; ++r) {
+              x[u][r][h] = v4i{0, 0, 0, 0};
+              if (at < c1) x[u][r][h] = load16(src[r][h] + at);
+            }
+            const uint32_t cq = cu + 32 * h, valid = cq < c1 ? min(32u, c1 - cq) * per_row : 0;
+#pragma unroll
+            for (int i = 0; i < NJ; ++i) {
+              m[u][h][i] = v4i{0, 0, 0, 0};
+              if (64u * i + lane < valid) m[u][h][i] = load16(w + (uint64_t)cq * rank + 8 * (64 * i + lane));
+            }
           }
         }
 #pragma unroll
-        for (uint32_t q = 0; q < Q; ++q) {
-          if (c + 32 * (q0 + q) >= c1) break;
+        for (uint32_t u = 0; u < U; ++u) {
+          if (c + 64 * (u0 + u) >= c1) break;
+          v4i xt[RB][2];
 #pragma unroll
-          for (int i = 0; i < NJ; ++i)
-            if (64u * i + lane < pieces) *reinterpret_cast<v4i*>(st + put[i]) = m[q][i];
-          wave_lds_order();
+          for (int r = 0; r < RB; ++r) turned(x[u][r], xt[r]);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const v4i a = transposed(st + (8 * lg + (lr >> 2)) * pitch + 32 * j + 8 * (lr & 3), pitch);
+          for (uint32_t q = 0; q < 2; ++q) {
 #pragma unroll
-            for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a, x[q][r], acc[r][j]);
+            for (int i = 0; i < NJ; ++i)
+              if (64u * i + lane < pieces) *reinterpret_cast<v4i*>(st + put[i]) = m[u][q][i];
+            wave_lds_order();
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+              const v4i a = transposed(st + (8 * lg + (lr >> 2)) * pitch + 32 * j + 8 * (lr & 3), pitch);
+#pragma unroll
+              for (int r = 0; r < RB; ++r) acc[r][j] = mfma(a, xt[r][q], acc[r][j]);
+            }
+            wave_lds_order();
           }
-          wave_lds_order();
         }
       }
     }
@@ -362,8 +408,7 @@ constexpr int down_occupancy(int nj, int rb) {
 
 template <int NJ, int RB, bool kBackward>
 __global__ __launch_bounds__(256, down_occupancy(NJ, RB)) void adapter_down_kernel(DownParams p) {
-  constexpr uint32_t kSums = 4 * 16 * (NJ * 16 + 4) * 4, kStaged = kBackward ? 4 * 32 * (NJ * 32 + 16) : 0;
-  __shared__ __align__(16) uint8_t lds[kSums > kStaged ? kSums : kStaged];
+  __shared__ __align__(16) uint8_t lds[kDownLds<NJ, kBackward>];
   Tile t;
   const DownSide& d = p.side[blockIdx.z];
   if (blockIdx.y >= d.splits || !find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
@@ -379,7 +424,7 @@ __global__ __launch_bounds__(256, down_occupancy(NJ, RB)) void adapter_down_kern
 // the same on tiles of rows from several segments
 template <int NJ>
 __global__ __launch_bounds__(256, down_occupancy(NJ, 1)) void adapter_down_group_kernel(DownParams p) {
-  __shared__ __align__(16) uint8_t lds[4 * 16 * (NJ * 16 + 4) * 4];
+  __shared__ __align__(16) uint8_t lds[kDownLds<NJ, false>];
   __shared__ GroupShared group;
   Tile t;
   if (!group_tile(p.seg, blockIdx.x, t, group, p.err) || t.adapter >= p.seg.adapters) return;
