@@ -219,6 +219,19 @@ __device__ __forceinline__ void split8(const float* v, v4i& hi, v4i& lo) {
   }
 }
 
+// eight bf16 and as many fp32 sums, rounded once
+__device__ __forceinline__ v4i added(v4i base, const float* sums) {
+  const v4f y[2] = {*reinterpret_cast<const v4f*>(sums), *reinterpret_cast<const v4f*>(sums + 4)};
+  v4i o;
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    const uint32_t bits = (uint32_t)base[i];
+    o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y[i / 2][2 * (i & 1)],
+                                bf16_bits_to_f32(bits >> 16) + y[i / 2][2 * (i & 1) + 1]);
+  }
+  return o;
+}
+
 // ------------------------------------------------------------------ down
 struct DownSide {
   const uint16_t* src;  // [rows][cols]
@@ -450,7 +463,9 @@ struct UpParams {
 // kColumns: the weights' rows of the 64 columns go through the wave's LDS and
 // are read transposed.
 // blocks of the up kernel that a CU holds, by its registers
-constexpr int up_occupancy(int kj, int rb) { return kj == 1 ? (rb == 1 ? 4 : 3) : kj == 2 && rb == 1 ? 3 : 2; }
+constexpr int up_occupancy(int kj, int rb) { return kj == 1 ? (rb == 1 ? 4 : 3) : kj == 2 ? 3 : 2; }
+
+constexpr int tall_occupancy(int kj) { return kj == 4 ? 2 : 4; }
 
 template <int KJ, int RB, bool kColumns, bool kGroup>
 __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(UpParams p) {
@@ -561,17 +576,7 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
       for (uint32_t h = 0; h < 2; ++h) {
         const uint32_t row = 8 * h + (lane >> 3), c = 8 * (lane & 7);
         v4i o = v.b[r][h];  // (without an adapter base goes through bit for bit, a -0 too)
-        if (live) {
-          const v4f y0 = *reinterpret_cast<const v4f*>(mine + row * kSumRow + c);
-          const v4f y1 = *reinterpret_cast<const v4f*>(mine + row * kSumRow + c + 4);
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t bits = (uint32_t)v.b[r][h][i];
-            const v4f y = i < 2 ? y0 : y1;
-            o[i] = (int)f32x2_to_bf16x2(bf16_bits_to_f32(bits & 0xffffu) + y[2 * (i & 1)],
-                                        bf16_bits_to_f32(bits >> 16) + y[2 * (i & 1) + 1]);
-          }
-        }
+        if (live) o = added(o, mine + row * kSumRow + c);
         if (16 * r + row < t.rows && c0 + c < p.cols) *reinterpret_cast<v4i*>(p.out + out_row[r][h] + c0 + c) = o;
       }
       if (live) wave_lds_order();
@@ -610,6 +615,140 @@ __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(U
     if (g + 8 < end) load(g + 8, even);
     finish(g + 4, odd);
     g += 8;
+  }
+}
+
+// The same for tiles of 64 rows, 16 a wave, whose weights the waves share: the
+// block's 64 columns of them lie in LDS (the next ones' loads under way), so
+// that they are read once per 64 rows.
+template <int KJ, bool kColumns>
+__global__ __launch_bounds__(256, tall_occupancy(KJ)) void adapter_up_tall_kernel(UpParams p) {
+  constexpr uint32_t kSumRow = 64 + 4, kPitch = kColumns ? 128 + 16 : KJ * 64 + 16, kStage = (kColumns ? KJ * 32 : 64) * kPitch;
+  __shared__ __align__(16) uint8_t staged[2 * kStage];
+  __shared__ __align__(16) float sums[4 * 16 * kSumRow];
+  Tile t;
+  if (!find_tile(p.seg, 64, blockIdx.x, t, p.err)) return;
+  if (t.adapter >= p.seg.adapters && t.adapter != kNoAdapter) return;
+  const bool live = t.adapter != kNoAdapter;
+  if (!live && p.base == p.out) return;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), rank = p.rank;
+  const uint16_t* const w = p.w + (uint64_t)(live ? t.adapter : 0) * rank * p.cols;
+  float* const mine = sums + wave * 16 * kSumRow;
+  const bool some = 16 * wave < t.rows;  // rows for this wave
+  // base and out: rows 8 h + (lane >> 3) of 16, 8 columns a lane
+  uint64_t base_row[2], out_row[2];
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h) {
+    const uint64_t row = t.row0 + min(16 * wave + 8 * h + (lane >> 3), t.rows - 1);
+    base_row[h] = row * p.base_stride;
+    out_row[h] = row * p.out_stride;
+  }
+  // 16-byte piece 256 i + tid of the 64 columns' weights: kColumns 8 of every
+  // rank row, else rank / 8 of every column, contiguous
+  const uint32_t per_row = kColumns ? 8 : rank / 8;
+  uint32_t put[KJ];
+#pragma unroll
+  for (int i = 0; i < KJ; ++i) {
+    const uint32_t e = 256 * i + tid;
+    put[i] = e / per_row * kPitch + e % per_row * 16;
+  }
+  struct Group {
+    v4i x[KJ], b[2];
+  };
+  auto load = [&](uint32_t g, Group& v) __attribute__((always_inline)) {
+    const uint32_t c0 = g * 64, valid = min(64u, p.cols - c0);
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < KJ; ++i) {
+        const uint32_t e = 256 * i + tid;
+        v.x[i] = v4i{0, 0, 0, 0};
+        if constexpr (kColumns) {
+          if (e < 8 * rank && 8 * (e & 7) < valid) v.x[i] = load16(w + (uint64_t)(e >> 3) * p.cols + c0 + 8 * (e & 7));
+        } else {
+          if (e < valid * per_row) v.x[i] = load16(w + (uint64_t)c0 * rank + 8 * e);
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      v.b[h] = v4i{0, 0, 0, 0};
+      if (p.base && some && 8 * (lane & 7) < valid) v.b[h] = load16_once(p.base + base_row[h] + c0 + 8 * (lane & 7));
+    }
+  };
+  auto stage = [&](uint32_t to, const Group& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < KJ; ++i)
+      if (256u * i + tid < (kColumns ? 8 * rank : 64 * per_row))
+        *reinterpret_cast<v4i*>(staged + to * kStage + put[i]) = v.x[i];
+  };
+  const uint32_t all = (p.cols + 63) / 64, end = min((blockIdx.y + 1) * p.groups, all);
+  uint32_t g = blockIdx.y * p.groups;
+  Group now, next;
+  load(g, now);
+  v4i hi[KJ], lo[KJ];
+  if (live) {
+    // (ranks past the last: zeros on both sides)
+    if (rank < KJ * 32u)
+      for (uint32_t i = tid; i < 2 * kStage / 16; i += 256) *reinterpret_cast<v4i*>(staged + 16 * i) = v4i{0, 0, 0, 0};
+    const float s = p.scaled ? 1.0f : t.scale;
+    const uint64_t step = (uint64_t)p.seg.rows * rank;
+    const float* const from = p.h + (t.row0 + min(16 * wave + lr, t.rows - 1)) * (uint64_t)rank + 8 * lg;
+#pragma unroll
+    for (int q = 0; q < KJ; ++q) {
+      v4f v0{0.f, 0.f, 0.f, 0.f}, v1 = v0;
+      if (32 * q + 8 * lg < rank) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < p.splits; ++i) {
+          v0 += *reinterpret_cast<const v4f*>(from + i * step + 32 * q);
+          v1 += *reinterpret_cast<const v4f*>(from + i * step + 32 * q + 4);
+        }
+      }
+      const float f[8] = {v0[0] * s, v0[1] * s, v0[2] * s, v0[3] * s, v1[0] * s, v1[1] * s, v1[2] * s, v1[3] * s};
+      split8(f, hi[q], lo[q]);
+    }
+    __syncthreads();
+    stage(0, now);
+  }
+  __syncthreads();
+  for (uint32_t at = 0; g < end; ++g, at ^= 1) {
+    if (g + 1 < end) load(g + 1, next);
+    if (some) {
+      const uint32_t c0 = g * 64;
+      if (live) {
+        v4f acc[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) acc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+        const uint8_t* const st = staged + at * kStage;
+#pragma unroll
+        for (int q = 0; q < KJ; ++q)
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) {
+            v4i x;
+            if constexpr (kColumns)
+              x = transposed(st + (32 * q + 8 * lg + (lr >> 2)) * kPitch + 2 * (32 * (u >> 1) + 8 * (lr & 3) + 4 * (u & 1)), kPitch);
+            else
+              x = *reinterpret_cast<const v4i*>(st + (32 * (u >> 1) + 8 * (lr >> 2) + 4 * (u & 1) + (lr & 3)) * kPitch + 64 * q + 16 * lg);
+            acc[u] = mfma(x, lo[q], acc[u]);
+            acc[u] = mfma(x, hi[q], acc[u]);
+          }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+          *reinterpret_cast<v4f*>(mine + lr * kSumRow + 32 * (u >> 1) + 8 * lg + 4 * (u & 1)) = acc[u];
+        wave_lds_order();
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t row = 8 * h + (lane >> 3), c = 8 * (lane & 7);
+        v4i o = now.b[h];  // (without an adapter base goes through bit for bit, a -0 too)
+        if (live) o = added(o, mine + row * kSumRow + c);
+        if (16 * wave + row < t.rows && c0 + c < p.cols) *reinterpret_cast<v4i*>(p.out + out_row[h] + c0 + c) = o;
+      }
+      if (live) wave_lds_order();
+    }
+    if (live && g + 1 < end) stage(at ^ 1, next);
+    now = next;
+    __syncthreads();
   }
 }
 
@@ -804,16 +943,38 @@ uint32_t tile_bound(const AdapterArgs& a, uint32_t height) {
   const uint64_t t = ((uint64_t)a.rows + (uint64_t)std::min(a.segments, a.rows) * (height - 1)) / height;
   return (uint32_t)std::min<uint64_t>(t, a.rows);
 }
-// K splits of the down product: what the card holds at once (a short second
-// round costs as much as a full one), 512 columns each at least: every block of
-// the up product adds the splits (64 one-row requests of rank 128 over 12288
-// columns 30 us against 43 with 256 columns; 1024 wins with one adapter, 29 us,
-// and loses with 16 at rank 64, 22.4 against 20.4)
-uint32_t down_splits(uint32_t tiles, uint32_t cols, uint32_t rank, uint32_t blocks, uint32_t sides) {
-  const uint32_t held = kCus * down_occupancy((rank + 15) / 16, blocks);
-  return std::max<uint32_t>(1, std::min<uint32_t>((cols + 511) / 512, held / std::max(sides * tiles, 1u)));
+// Columns of a K split of the down product, of one side or both: of one to
+// three rounds of the blocks that the card holds at once the cheapest by the
+// rounds' columns and 512 more for a round's beginning and end (a short second
+// round costs as much as a full one); 512 at least, since every block of the up
+// product adds the splits (64 one-row requests of rank 128 over 12288 columns 30
+// us against 43 with 256 columns; 1024 wins with one adapter, 29 us, and loses
+// with 16 at rank 64, 22.4 against 20.4).
+constexpr uint32_t kRounds = 3, kSplitColumns = 512;
+uint32_t held_blocks(uint32_t rank, uint32_t blocks) { return kCus * down_occupancy((rank + 15) / 16, blocks); }
+uint32_t split_columns(uint32_t tiles, uint32_t cols, uint32_t other, uint32_t rank, uint32_t blocks) {
+  const uint32_t held = held_blocks(rank, blocks), most = std::max(cols, other);
+  auto parts = [&](uint32_t at) { return (uint64_t)tiles * ((cols + at - 1) / at + (other + at - 1) / at); };
+  uint32_t best = (most + 127) / 128;  // in 128 columns, as the waves take them
+  uint64_t cost = (parts(128 * best) + held - 1) / held * (128 * best + 512);
+  for (uint32_t r = 1; r <= kRounds; ++r) {
+    // the shortest split whose blocks fit r rounds
+    uint32_t low = kSplitColumns / 128, high = (most + 127) / 128;
+    if (low >= high || parts(128 * high) > (uint64_t)r * held) continue;
+    while (low < high) {
+      const uint32_t mid = (low + high) / 2;
+      if (parts(128 * mid) <= (uint64_t)r * held) high = mid;
+      else low = mid + 1;
+    }
+    const uint64_t c = (uint64_t)r * (128 * high + 512);
+    if (c < cost) {
+      cost = c;
+      best = high;
+    }
+  }
+  return 128 * best;
 }
-uint32_t per_split(uint32_t cols, uint32_t splits) { return ((cols + splits - 1) / splits + 127) / 128 * 128; }
+uint32_t splits_of(uint32_t cols, uint32_t at) { return (cols + at - 1) / at; }
 
 template <typename F>
 void with_pow2(uint32_t n, F&& f) {
@@ -841,12 +1002,29 @@ uint32_t group_bound(const AdapterArgs& a) {
 
 template <bool kColumns>
 void launch_up(UpParams p, const AdapterArgs& a, bool group) {
+  const bool tall = tile_blocks(a) == 4;
+  if (tall && p.rank > 32) {
+    // two blocks a CU, each with as many groups as there are splits of h, which
+    // every block adds up (4099 x 4096 outputs of rank 64: 25 us; one block a CU
+    // 32, four 29; tiles of 32 rows that read the weights themselves 31.  4099 x
+    // 12288 of rank 128: 60 us, 213 with 16-row tiles)
+    with_pow2((p.rank + 31) / 32, [&](auto kj) {
+      constexpr int KJ = decltype(kj)::value;
+      if constexpr (KJ == 2 || KJ == 4) {
+        const uint32_t tiles = tile_bound(a, 64), all = (p.cols + 63) / 64, columns = std::max(1u, 2 * kCus / tiles);
+        p.groups = std::max((all + columns - 1) / columns, p.splits);
+        hipLaunchKernelGGL((adapter_up_tall_kernel<KJ, kColumns>), dim3(tiles, (all + p.groups - 1) / p.groups),
+                           dim3(256), 0, a.stream, p);
+      }
+    });
+    return;
+  }
   // column blocks for as many blocks as the card holds at once (tiles of few
   // rows: every further round repeats the search and the sum of h; 57 one-row
   // requests 10.2 us against 12.7 with three rounds) or, with long segments,
-  // for three rounds of that, whose last costs little (8192 rows 117 us against
-  // 126 with one)
-  const uint32_t blocks = tile_blocks(a) == 4 && p.rank <= 64 ? 2 : 1;
+  // for three rounds of that, whose last costs little (8192 rows 117 us a
+  // backward call against 126 with one)
+  const uint32_t blocks = tall ? 2 : 1;
   const uint32_t tiles = group ? group_bound(a) : tile_bound(a, 16 * blocks), all = (p.cols + 63) / 64;
   with_pow2((p.rank + 31) / 32, [&](auto kj) {
     constexpr int KJ = decltype(kj)::value;
@@ -864,7 +1042,7 @@ void launch_up(UpParams p, const AdapterArgs& a, bool group) {
         }
         hipLaunchKernelGGL((adapter_up_kernel<KJ, RB, kColumns, false>), grid, dim3(256), 0, a.stream, p);
       };
-      if constexpr (KJ <= 2) {
+      if constexpr (KJ == 1) {
         if (blocks == 2) {
           launch(std::integral_constant<int, 2>{});
           return;
@@ -890,7 +1068,7 @@ void launch_down(const DownParams& d, uint32_t tiles, uint32_t blocks, uint32_t 
 }
 
 struct BackwardPlan {
-  uint32_t blocks, tiles, finish_tiles, splits[2], row_pitch, grad_splits;
+  uint32_t blocks, tiles, finish_tiles, per_split, splits[2], row_pitch, grad_splits;
   uint64_t part[2], dh, parts[2], grads[2], bytes;
 };
 BackwardPlan backward_plan(const AdapterArgs& a) {
@@ -898,8 +1076,9 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   p.blocks = tile_blocks(a);
   p.tiles = tile_bound(a, 16 * p.blocks);
   p.finish_tiles = tile_bound(a, kFinishRows);
-  p.splits[0] = down_splits(p.tiles, a.k, a.rank, p.blocks, 2);
-  p.splits[1] = down_splits(p.tiles, a.n, a.rank, p.blocks, 2);
+  p.per_split = split_columns(p.tiles, a.k, a.n, a.rank, p.blocks);
+  p.splits[0] = splits_of(a.k, p.per_split);
+  p.splits[1] = splits_of(a.n, p.per_split);
   p.row_pitch = (a.rows + 31) / 32 * 32;
   // row splits of the gradients: two rounds of blocks, 256 rows each at least
   const uint64_t blocks = (uint64_t)a.adapters * ((a.n + 63) / 64 + (a.k + 63) / 64);
@@ -923,9 +1102,12 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
 
 uint64_t AdapterGemmWorkspaceBytes(uint32_t rows, uint32_t rank, uint32_t k) {
   if (!rows || rows > kMaxRows || !rank || rank > kMaxRank || !k || k > kMaxColumns) return 0;
-  // as many splits as any segments lead to: a tile per 64 or 16 rows at least
-  const uint32_t splits = std::max(down_splits((rows + 63) / 64, k, rank, 4, 1), down_splits((rows + 15) / 16, k, rank, 1, 1));
-  return (uint64_t)splits * rows * rank * 4;
+  // as many splits as any segments lead to: every block has a tile of 64 rows at
+  // most, or of 16
+  const uint64_t tall = (uint64_t)kRounds * held_blocks(rank, 4) / ((rows + 63) / 64);
+  const uint64_t low = (uint64_t)kRounds * held_blocks(rank, 1) / ((rows + 15) / 16);
+  const uint64_t splits = std::min<uint64_t>(splits_of(k, kSplitColumns), std::max<uint64_t>(1, std::max(tall, low)));
+  return splits * rows * rank * 4;
 }
 
 uint64_t AdapterBackwardWorkspaceBytes(const AdapterArgs& a) { return shape_ok(a) ? backward_plan(a).bytes : 0; }
@@ -942,14 +1124,14 @@ St LaunchAdapterGemm(const AdapterArgs& a) {
     return Invalid("adapter_gemm_alignment_invalid");
   const bool group = grouped(a);
   const uint32_t blocks = tile_blocks(a), tiles = group ? group_bound(a) : tile_bound(a, 16 * blocks);
-  const uint32_t splits = down_splits(tiles, a.k, a.rank, blocks, 1);
+  const uint32_t per_split = split_columns(tiles, a.k, 0, a.rank, blocks), splits = splits_of(a.k, per_split);
   if (a.workspace_bytes < AdapterGemmWorkspaceBytes(a.rows, a.rank, a.k) || !aligned16(a.workspace))
     return Invalid("adapter_gemm_workspace_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
   DownParams d{};
   d.seg = segments_of(a);
-  d.side[0] = DownSide{a.x, a.a, static_cast<float*>(a.workspace), a.x_stride, a.k, per_split(a.k, splits), splits};
+  d.side[0] = DownSide{a.x, a.a, static_cast<float*>(a.workspace), a.x_stride, a.k, per_split, splits};
   d.err = a.error_flag;
   d.rank = a.rank;
   if (group)
@@ -998,8 +1180,8 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   auto u16 = [&](uint64_t at) { return reinterpret_cast<uint16_t*>(ws + at); };
   DownParams d{};
   d.seg = segments_of(a);
-  d.side[0] = DownSide{a.x,   a.a, f32(plan.part[0]), a.x_stride, a.k, per_split(a.k, plan.splits[0]), plan.splits[0]};
-  d.side[1] = DownSide{a.dy,  a.b, f32(plan.part[1]), a.dy_stride, a.n, per_split(a.n, plan.splits[1]), plan.splits[1]};
+  d.side[0] = DownSide{a.x,   a.a, f32(plan.part[0]), a.x_stride, a.k, plan.per_split, plan.splits[0]};
+  d.side[1] = DownSide{a.dy,  a.b, f32(plan.part[1]), a.dy_stride, a.n, plan.per_split, plan.splits[1]};
   d.err = a.error_flag;
   d.rank = a.rank;
   launch_down<true>(d, plan.tiles, plan.blocks, std::max(plan.splits[0], plan.splits[1]), a.stream);
