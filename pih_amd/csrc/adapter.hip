@@ -753,34 +753,49 @@ __global__ __launch_bounds__(256, tall_occupancy(KJ)) void adapter_up_tall_kerne
 }
 
 // ---------------------------------------------------- splits of a backward
+// h and dh from the splits: dh in fp32 for dx, and both as three bf16 that add
+// up to the value, in the order of the gradients' MFMA operands, so that a wave
+// loads 1 KB in one piece: [32 rows][part][16 ranks][lane (rank lr, rows 8 lg
+// ..)][8 rows].
 constexpr uint32_t kFinishRows = 16;
 struct FinishParams {
   Segments seg;
   const float* part[2];   // [splits][rows][rank]: x A^T, dy B
   float* dh;              // [rows][rank], scaled
-  uint16_t* parts[2];     // [3][rank][row_pitch], scaled: three bf16 that add up to the value
+  uint16_t* parts[2];
   uint32_t* err;
   uint32_t splits[2];
-  uint32_t rank, row_pitch;
+  uint32_t rank;
 };
 __global__ __launch_bounds__(256) void adapter_finish_kernel(FinishParams p) {
+  __shared__ float sums[kFinishRows][kMaxRank + 1];
   Tile t;
   if (!find_tile(p.seg, kFinishRows, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
-  const uint32_t side = blockIdx.y;
+  const uint32_t side = blockIdx.y, pieces = p.rank / 4;
+  for (uint32_t i = threadIdx.x; i < t.rows * pieces; i += 256) {
+    const uint32_t r = i / pieces, j = i % pieces * 4;
+    const uint64_t at = (uint64_t)(t.row0 + r) * p.rank + j, step = (uint64_t)p.seg.rows * p.rank;
+    v4f v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (uint32_t q = 0; q < p.splits[side]; ++q) v += *reinterpret_cast<const v4f*>(p.part[side] + q * step + at);
+    v = v4f{v[0] * t.scale, v[1] * t.scale, v[2] * t.scale, v[3] * t.scale};
+    if (side) *reinterpret_cast<v4f*>(p.dh + at) = v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[r][j + e] = v[e];
+  }
+  __syncthreads();
+  const uint32_t blocks = (p.rank + 15) / 16;
   for (uint32_t i = threadIdx.x; i < kFinishRows * p.rank; i += 256) {
     const uint32_t r = i & (kFinishRows - 1), j = i / kFinishRows;
     if (r >= t.rows) continue;
-    const uint64_t row = t.row0 + r;
-    float v = 0.0f;
-#pragma unroll 8
-    for (uint32_t q = 0; q < p.splits[side]; ++q) v += p.part[side][((uint64_t)q * p.seg.rows + row) * p.rank + j];
-    v *= t.scale;
-    if (side) p.dh[row * p.rank + j] = v;
-    uint16_t* const part = p.parts[side] + (uint64_t)j * p.row_pitch + row;
+    const uint32_t row = t.row0 + r;
+    float v = sums[r][j];
+    uint16_t* const part = p.parts[side] + ((uint64_t)(row / 32) * 3 * blocks + j / 16) * 512 +
+                           (row / 8 % 4 * 16 + j % 16) * 8 + row % 8;
 #pragma unroll
     for (uint32_t q = 0; q < 3; ++q) {
       const uint32_t h = f32_to_bf16_bits(v);
-      part[(uint64_t)q * p.rank * p.row_pitch] = (uint16_t)h;
+      part[q * blocks * 512] = (uint16_t)h;
       v -= bf16_bits_to_f32(h);
     }
   }
@@ -789,7 +804,7 @@ __global__ __launch_bounds__(256) void adapter_finish_kernel(FinishParams p) {
 // ------------------------------------------------- gradients of A and of B
 struct GradSide {
   const uint16_t* src;   // [rows][cols]: x for A, dy for B
-  const uint16_t* parts; // [3][rank][row_pitch]
+  const uint16_t* parts; // as above
   float* out;            // [adapters][rank][cols], or (B) [adapters][cols][rank]
   float* part;           // [splits] of those when the rows are split
   uint32_t stride, cols;
@@ -797,7 +812,7 @@ struct GradSide {
 struct GradParams {
   Segments seg;
   GradSide side[2];
-  uint32_t rank, row_pitch, splits;
+  uint32_t rank, splits;
 };
 
 // 64 columns of one adapter's gradient over its rows, in blocks of 32 rows at
@@ -841,9 +856,13 @@ __device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d
                   (r + 2 * q + 1 >= lo_row && r + 2 * q + 1 < hi_row ? (int)0xffff0000 : 0);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const uint16_t* const from = d.parts + (uint64_t)min(16 * j + lr, p.rank - 1) * p.row_pitch + r;
+        // (a rank of less than 16 j + 16: what its places hold goes to results
+        // that are not written)
+        const uint32_t blocks = (p.rank + 15) / 16;
+        const uint16_t* const from =
+            d.parts + ((uint64_t)(first + i) * 3 * blocks + min((uint32_t)j, blocks - 1)) * 512 + 8 * lane;
 #pragma unroll
-        for (uint32_t q = 0; q < 3; ++q) h[q][j] = load16(from + (uint64_t)q * p.rank * p.row_pitch) & mask;
+        for (uint32_t q = 0; q < 3; ++q) h[q][j] = load16(from + q * blocks * 512) & mask;
       }
 #pragma unroll
       for (uint32_t q = 0; q < 4; ++q)
@@ -1068,7 +1087,7 @@ void launch_down(const DownParams& d, uint32_t tiles, uint32_t blocks, uint32_t 
 }
 
 struct BackwardPlan {
-  uint32_t blocks, tiles, finish_tiles, per_split, splits[2], row_pitch, grad_splits;
+  uint32_t blocks, tiles, finish_tiles, per_split, splits[2], grad_splits;
   uint64_t part[2], dh, parts[2], grads[2], bytes;
 };
 BackwardPlan backward_plan(const AdapterArgs& a) {
@@ -1079,7 +1098,6 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   p.per_split = split_columns(p.tiles, a.k, a.n, a.rank, p.blocks);
   p.splits[0] = splits_of(a.k, p.per_split);
   p.splits[1] = splits_of(a.n, p.per_split);
-  p.row_pitch = (a.rows + 31) / 32 * 32;
   // row splits of the gradients: two rounds of blocks, 256 rows each at least
   const uint64_t blocks = (uint64_t)a.adapters * ((a.n + 63) / 64 + (a.k + 63) / 64);
   p.grad_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((a.rows + 255) / 256, 1024 / blocks));
@@ -1091,7 +1109,7 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   };
   for (int s = 0; s < 2; ++s) p.part[s] = take((uint64_t)p.splits[s] * a.rows * a.rank * 4);
   p.dh = take((uint64_t)a.rows * a.rank * 4);
-  for (int s = 0; s < 2; ++s) p.parts[s] = take(3ull * a.rank * p.row_pitch * 2);
+  for (int s = 0; s < 2; ++s) p.parts[s] = take(3ull * ((a.rank + 15) / 16 * 16) * ((a.rows + 31ull) / 32 * 32) * 2);
   if (p.grad_splits > 1)
     for (int s = 0; s < 2; ++s) p.grads[s] = take((uint64_t)p.grad_splits * a.adapters * a.rank * (s ? a.n : a.k) * 4);
   p.bytes = at;
@@ -1195,7 +1213,6 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   }
   f.err = a.error_flag;
   f.rank = a.rank;
-  f.row_pitch = plan.row_pitch;
   hipLaunchKernelGGL(adapter_finish_kernel, dim3(plan.finish_tiles, 2), dim3(256), 0, a.stream, f);
   UpParams u{};
   u.seg = d.seg;
@@ -1214,7 +1231,6 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   GradParams g{};
   g.seg = d.seg;
   g.rank = a.rank;
-  g.row_pitch = plan.row_pitch;
   g.splits = plan.grad_splits;
   // da = dh^T x, db = dy^T h
   g.side[0] = GradSide{a.x, f.parts[1], a.da, f32(plan.grads[0]), a.x_stride, a.k};
