@@ -9,8 +9,8 @@
 // tile, and the target's logit where they hold it; a second launch joins a
 // row's pairs.  Backward: pieces of the vocabulary.  For a piece the logits
 // are computed again and leave as g, bf16 [rows][piece] in the workspace
-// (128 MB at most, so that it stays in the memory-side cache between its
-// writer and its two readers), then dw of the piece is g^T x, and dx
+// (128 MB, so that it stays in the memory-side cache between its writer and its
+// two readers; 4096 columns at least, which is more above 16384 rows), then dw of the piece is g^T x, and dx
 // grows by g W_piece in fp32.
 //
 // g is rounded to bf16 for the matrix cores: 2^-9 of each element at most,
@@ -42,55 +42,39 @@ typedef uint16_t Tile16[TS][kPitch];
 
 enum : int { kEpiStats = 0, kEpiGrad = 1, kEpiBf16 = 2, kEpiAdd = 3 };
 
-// C [m][n] = A . B^T over k.  A: [m][k] with row stride lda, or (AT) [k][m];
-// B: [n][k], or (BT) [k][n].
+// C [m][n] = A . B^T over k.  A: [m][k] with row stride lda, B: [n][k].
 struct GemmArgs {
   const uint16_t* a;
   const uint16_t* b;
   uint32_t m, n, k;
   uint64_t lda, ldb;
-  void* out;            // kEpiBf16: bf16, kEpiAdd: f32, kEpiGrad: bf16
+  void* out;            // kEpiGrad: bf16
   uint64_t ldo;
-  // kEpiStats, kEpiGrad: rows of the result are x rows, columns vocabulary
-  // entries from v0 on
+  // rows of the result are x rows, columns vocabulary entries from v0 on
   const uint32_t* target;
   const float* lse;
   const float* mantissa;  // kEpiGrad: [m]
-  const float* scale;   // kEpiBf16: factor of the result
   float2* stats;        // [m][stat_tiles]
   float* target_logit;  // [m]
-  uint32_t v0, vocab, stat_tiles, first;
+  uint32_t v0, vocab, stat_tiles;
 };
 
-// 64 x 64 elements of an operand into LDS as [row][k], zeros outside
-template <bool kT>
+// 64 x 64 elements of an operand into LDS, zeros outside
 __device__ __forceinline__ void stage(Tile16& s, const uint16_t* p, uint64_t ld, uint32_t r0, uint32_t rows, uint32_t k0,
                                       uint32_t k) {
   for (uint32_t i = threadIdx.x; i < TS * KS / 8; i += 256) {
     const uint32_t r = i / 8, c = i % 8 * 8;
     v4i v{0, 0, 0, 0};
-    if constexpr (kT) {
-      // source row k0 + r, columns r0 + c ..
-      if (k0 + r < k && r0 + c < rows) {
-        const uint16_t* src = p + (uint64_t)(k0 + r) * ld + r0 + c;
-        if (r0 + c + 8 <= rows) {
-          v = *reinterpret_cast<const v4i*>(src);
-        } else {
-          for (uint32_t q = 0; q < rows - r0 - c; ++q) v[q / 2] |= (int)((uint32_t)src[q] << (16 * (q & 1)));
-        }
-      }
-#pragma unroll
-      for (uint32_t q = 0; q < 8; ++q) s[c + q][r] = (uint16_t)((uint32_t)v[q / 2] >> (16 * (q & 1)));
-    } else {
-      if (r0 + r < rows && k0 + c < k) v = *reinterpret_cast<const v4i*>(p + (uint64_t)(r0 + r) * ld + k0 + c);
-      *reinterpret_cast<v4i*>(&s[r][c]) = v;
-    }
+    if (r0 + r < rows && k0 + c < k) v = *reinterpret_cast<const v4i*>(p + (uint64_t)(r0 + r) * ld + k0 + c);
+    *reinterpret_cast<v4i*>(&s[r][c]) = v;
   }
 }
 
-// Tile of 64 x 64: four waves of 32 x 32.  The MFMA's first operand is B, so
-// that a lane's four results are consecutive columns of one row.
-template <bool AT, bool BT, int EPI>
+// The logits' product for hidden sizes that are no multiple of 64.  Tile of
+// 64 x 64: four waves of 32 x 32.  The MFMA's first operand is B, so that a
+// lane's four results are consecutive columns of one row.  1024 rows, 32768
+// entries: 267 us at hidden 1000 (251 TFLOP/s), the tiles below 70 us at 1024.
+template <int EPI>
 __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
   __shared__ __align__(16) Tile16 sa, sb;
   __shared__ float tile[TS][TS + 1];
@@ -100,8 +84,8 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = v4f{0.f, 0.f, 0.f, 0.f};
   for (uint32_t k0 = 0; k0 < p.k; k0 += KS) {
-    stage<AT>(sa, p.a, p.lda, m0, p.m, k0, p.k);
-    stage<BT>(sb, p.b, p.ldb, n0, p.n, k0, p.k);
+    stage(sa, p.a, p.lda, m0, p.m, k0, p.k);
+    stage(sb, p.b, p.ldb, n0, p.n, k0, p.k);
     __syncthreads();
 #pragma unroll
     for (uint32_t q = 0; q < KS; q += 32) {
@@ -149,17 +133,14 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
     for (uint32_t i = tid; i < TS * TS; i += 256) {
       const uint32_t r = i / TS, c = i % TS, row = m0 + r, col = n0 + c;
       float v = tile[r][c];
-      if constexpr (EPI == kEpiGrad) {
-        if (row >= p.m) continue;
+      // (rows and columns past the last up to the tile's end are read as zeros
+      // by the products with g)
+      float g = 0.0f;
+      if (row < p.m && col < p.n) {
         const uint32_t target = p.target[row], at = p.v0 + col;
-        float g = 0.0f;
-        if (target < p.vocab && col < p.n) g = p.mantissa[row] * (expf(v - p.lse[row]) - (target == at ? 1.0f : 0.0f));
-        static_cast<uint16_t*>(p.out)[(uint64_t)row * p.ldo + col] = (uint16_t)f32_to_bf16_bits(g);
-      } else if (row < p.m && col < p.n) {
-        const uint64_t o = (uint64_t)row * p.ldo + col;
-        if constexpr (EPI == kEpiBf16) static_cast<uint16_t*>(p.out)[o] = (uint16_t)f32_to_bf16_bits(v * *p.scale);
-        else static_cast<float*>(p.out)[o] = p.first ? v : static_cast<float*>(p.out)[o] + v;
+        if (target < p.vocab) g = p.mantissa[row] * (expf(v - p.lse[row]) - (target == at ? 1.0f : 0.0f));
       }
+      static_cast<uint16_t*>(p.out)[(uint64_t)row * p.ldo + col] = (uint16_t)f32_to_bf16_bits(g);
     }
   }
 }
@@ -762,9 +743,9 @@ __global__ __launch_bounds__(256) void loss_round_kernel(const float* sums, cons
   }
 }
 
-template <bool AT, bool BT, int EPI>
+template <int EPI>
 void launch_gemm(const GemmArgs& g, hipStream_t s) {
-  hipLaunchKernelGGL((loss_gemm_kernel<AT, BT, EPI>), dim3((g.m + TS - 1) / TS, (g.n + TS - 1) / TS), dim3(256), 0, s,
+  hipLaunchKernelGGL((loss_gemm_kernel<EPI>), dim3((g.m + TS - 1) / TS, (g.n + TS - 1) / TS), dim3(256), 0, s,
                      g);
 }
 
@@ -781,7 +762,7 @@ uint32_t piece_columns(uint32_t rows, uint32_t vocab) {
   return std::min(all, std::max(fit, 4096u));
 }
 
-// the 256 x 256 tiles take 64-deep steps
+// the tiles fed by DMA take 64-deep steps
 bool big_takes(uint32_t hidden) { return hidden % KB == 0; }
 
 struct BackwardPlan {
@@ -798,7 +779,7 @@ BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   // dx has few tiles: its contraction, a piece's columns, is split until
   // there is a tile for every CU, at 1024 columns a split or more
   const uint32_t tiles = ((rows + TB - 1) / TB) * ((hidden + TB - 1) / TB);
-  p.splits = big_takes(hidden) ? std::max<uint32_t>(1, std::min<uint32_t>(kCus / tiles, p.piece / 1024)) : 1;
+  p.splits = std::max<uint32_t>(1, std::min<uint32_t>(kCus / tiles, p.piece / 1024));
   p.factor = p.sums + padded((uint64_t)p.splits * rows * hidden * 4);
   p.mantissa = p.factor + padded(4);
   p.bytes = p.mantissa + padded((uint64_t)rows * 4);
@@ -853,7 +834,7 @@ St LaunchLmHeadLoss(const LmHeadLossArgs& a) {
     launch_big<false, false, kEpiStats>(b, a.stream);
     g.stat_tiles = (a.vocab + TB - 1) / TB;
   } else {
-    launch_gemm<false, false, kEpiStats>(g, a.stream);
+    launch_gemm<kEpiStats>(g, a.stream);
   }
   hipLaunchKernelGGL(loss_join_kernel, dim3((a.rows + 3) / 4), dim3(256), 0, a.stream, g.stats, g.target_logit,
                      a.target, a.loss, a.lse, a.error_flag, a.rows, a.vocab, g.stat_tiles);
@@ -904,78 +885,52 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
       b.v0 = v0;
       b.vocab = a.vocab;
       launch_big<false, false, kEpiGrad>(b, a.stream);
-      if (a.dw) {
-        b = BigArgs{};
-        b.a = grad;
-        b.b = live;
-        b.m = cols;
-        b.n = a.hidden;
-        b.k = b.k_valid = row_up;
-        b.lda = plan.piece;
-        b.ldb = a.hidden;
-        b.out = a.dw + (uint64_t)v0 * a.hidden;
-        b.scale = factor;
-        b.ldo = a.hidden;
-        launch_big<true, true, kEpiBf16>(b, a.stream);
-      }
-      b = BigArgs{};
+    } else {
+      GemmArgs g{};
+      g.a = a.x;
+      g.b = w;
+      g.m = a.rows;
+      g.n = cols;
+      g.k = a.hidden;
+      g.lda = g.ldb = a.hidden;
+      g.out = grad;
+      g.ldo = plan.piece;
+      g.target = a.target;
+      g.lse = a.lse;
+      g.mantissa = mantissa;
+      g.v0 = v0;
+      g.vocab = a.vocab;
+      launch_gemm<kEpiGrad>(g, a.stream);
+    }
+    if (a.dw) {
+      BigArgs b{};
       b.a = grad;
-      b.b = w;
-      b.m = a.rows;
+      b.b = live;
+      b.m = cols;
       b.n = a.hidden;
-      b.k = (cols + KB - 1) / KB * KB;
-      b.k_valid = cols;
+      b.k = b.k_valid = row_up;
       b.lda = plan.piece;
       b.ldb = a.hidden;
-      b.out = sums;
+      b.out = a.dw + (uint64_t)v0 * a.hidden;
+      b.scale = factor;
       b.ldo = a.hidden;
-      b.splits = plan.splits;
-      b.split_stride = (uint64_t)a.rows * a.hidden;
-      b.first = v0 == 0;
-      launch_big<false, true, kEpiAdd>(b, a.stream);
-      continue;
+      launch_big<true, true, kEpiBf16>(b, a.stream);
     }
-    GemmArgs g{};
-    g.a = a.x;
-    g.b = w;
-    g.m = a.rows;
-    g.n = cols;
-    g.k = a.hidden;
-    g.lda = g.ldb = a.hidden;
-    g.out = grad;
-    g.ldo = plan.piece;
-    g.target = a.target;
-    g.lse = a.lse;
-    g.mantissa = mantissa;
-    g.v0 = v0;
-    g.vocab = a.vocab;
-    launch_gemm<false, false, kEpiGrad>(g, a.stream);
-    if (a.dw) {
-      GemmArgs d{};
-      d.a = grad;
-      d.b = live;
-      d.m = cols;
-      d.n = a.hidden;
-      d.k = a.rows;
-      d.lda = plan.piece;
-      d.ldb = a.hidden;
-      d.out = a.dw + (uint64_t)v0 * a.hidden;
-      d.scale = factor;
-      d.ldo = a.hidden;
-      launch_gemm<true, true, kEpiBf16>(d, a.stream);
-    }
-    GemmArgs d{};
-    d.a = grad;
-    d.b = w;
-    d.m = a.rows;
-    d.n = a.hidden;
-    d.k = cols;
-    d.lda = plan.piece;
-    d.ldb = a.hidden;
-    d.out = sums;
-    d.ldo = a.hidden;
-    d.first = v0 == 0;
-    launch_gemm<false, true, kEpiAdd>(d, a.stream);
+    BigArgs b{};
+    b.a = grad;
+    b.b = w;
+    b.m = a.rows;
+    b.n = a.hidden;
+    b.k = (cols + KB - 1) / KB * KB;
+    b.k_valid = cols;
+    b.lda = plan.piece;
+    b.ldb = a.hidden;
+    b.out = sums;
+    b.ldo = a.hidden;
+    b.splits = plan.splits;
+    b.split_stride = (uint64_t)a.rows * a.hidden;
+    b.first = v0 == 0;
+    launch_big<false, true, kEpiAdd>(b, a.stream);
   }
   const uint64_t count = (uint64_t)a.rows * a.hidden;
   hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 20)), dim3(256), 0,
