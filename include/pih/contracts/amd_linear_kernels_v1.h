@@ -417,10 +417,11 @@ typedef struct pih_amd_v41_block_dequant_launch_v1 {
  * segment_adapter[s] (u32 [segments]; 0xFFFFFFFF: none, output = base).
  * Segments may share an adapter.  Rows outside every segment are neither
  * read nor written.  Up to 2^26 rows, 65536 segments (every block reads the
- * offsets) and 32767 adapters.
- * A bf16 [adapters][rank][k], B bf16 [adapters][n][rank], scale f32 [adapters] (0: all 1).  base_bf16 may be the output itself (same
- * stride) or 0 (the rows start from zero).  input, base and output rows are
- * *_stride elements apart (k, n, n at least).
+ * offsets) and 32767 adapters.  A bf16 [adapters][rank][k], B bf16
+ * [adapters][n][rank], scale f32 [adapters] (0: all 1).  base_bf16 may be the
+ * output itself (same stride) or 0 (the rows start from zero); the output lies
+ * outside input.  input, base and output rows are *_stride elements apart (k, n,
+ * n at least).
  * rank a multiple of 8 up to 128; n, k and the strides multiples of 8; every
  * address 16-byte aligned (the u32 and f32 arrays 4-byte).  The product with
  * A is summed in fp32 and enters the second product as the sum of two bf16

@@ -4,21 +4,35 @@
 //   dx = base + dh A_a,  da = dh^T x,  db = dy^T h
 //   with  h = s_a x A_a^T,  dh = s_a dy B_a   (rank <= 128 columns).
 //
-// Two launches forward.  The first ("down") multiplies a 16-row tile of a
-// segment with A and leaves fp32 sums [split][row][rank]: K is split over
-// the blocks until they fill the card, since a decode batch has few rows.
-// The second ("up") adds the splits, scales, and multiplies with B on top of
-// base.  Tiles never cross a segment, so a tile has one adapter and no row
-// permutation is needed; a tile finds its segment by a wave scan over the
-// offsets.  The product between the two stays fp32 up to the second MFMA,
-// which takes it as two bf16 values hi + lo (2^-16 of the value at most is
-// lost): twice the MFMAs of a product that is bound by bytes, and the output
-// is off by its own rounding only.
+// Two launches forward.  The first ("down") multiplies a tile of a segment's
+// rows with A and leaves fp32 sums [split][row][rank]: K is split over the
+// blocks until they fill the card, since a decode batch has few rows.  The
+// second ("up") adds the splits, scales, and multiplies with B on top of base.
+// The product between the two stays fp32 up to the second MFMA, which takes it
+// as two bf16 values hi + lo (2^-16 of the value at most is lost): twice the
+// MFMAs of a product that is bound by bytes, and the output is off by its own
+// rounding only.  (One launch, every block with the whole product with A for
+// itself: 57 requests 17.9 us of GPU time against 13.1, since a CU then takes in
+// all of A.)
+//
+// A tile has one adapter: rows of one segment, found by a wave scan over the
+// offsets, 16 or (segments of 64 rows) 64 in the product with A, 16, 32 or 64 in
+// the product with B; or, where segments are a row or two, 16 rows of an adapter
+// from all segments, so that the adapter is read once for them.
+//
+// Both products move bytes: rows of 64 columns and fewer are taken through LDS,
+// so that every load and store of a wave has whole 128-byte lines (half lines
+// ran at 3.3 TB/s where whole ones reach 4.9).  Measured, us of GPU time:
+//   1 row, rank 16, 4096 x 4096                4.4 + 4.4   (latency)
+//   57 one-row requests, 16 adapters, rank 32, 12288 x 4096   6.0 + 6.8
+//   4099 rows, rank 64, 4096 x 12288           26 (4.1 TB/s) + 25 (2.7 TB/s)
+//   8000 rows, rank 32, 12288 outputs          up 81 (4.9 TB/s)
+//   backward, 8192 rows, rank 16, 4096 x 4096  36 (3.7 TB/s) + 5 + 30 (4.5) + 27 (4.9) + 5
 //
 // The backward runs both downs (x A^T and dy B) in one launch, then sums the
 // splits once, into [row][rank] for the up product with A and into three bf16
-// parts (all 24 bits: these gradients are fp32) with the rows innermost for
-// the gradients of A and B, whose contraction runs over the rows.
+// parts (all 24 bits: these gradients are fp32) for the gradients of A and B,
+// whose contraction runs over the rows.
 //
 // MFMA operands: the weights (or the rows' side for da) come first, so that a
 // lane's four results are consecutive in memory.
@@ -456,17 +470,16 @@ struct UpParams {
   uint32_t scaled;      // h holds the scale
 };
 
-// out rows of a tile of 16 RB: 64 columns ("a group") at a time per wave, the
-// next group's loads under way.  Row rho of MFMA u holds column
-// 32 (u >> 1) + 8 (rho >> 2) + 4 (u & 1) + (rho & 3), so that a lane's results
-// of two MFMAs are 8 consecutive columns and its row's four lanes' 64 bytes.
-// kColumns: the weights' rows of the 64 columns go through the wave's LDS and
-// are read transposed.
-// blocks of the up kernel that a CU holds, by its registers
+// blocks of the up kernels that a CU holds, by registers and LDS (kj: 32-column
+// pieces of the rank)
 constexpr int up_occupancy(int kj, int rb) { return kj == 1 ? (rb == 1 ? 4 : 3) : kj == 2 ? 3 : 2; }
-
 constexpr int tall_occupancy(int kj) { return kj == 4 ? 2 : 4; }
 
+// out rows of a tile of 16 RB: 64 columns ("a group") at a time per wave, the
+// next group's loads under way.  Row rho of MFMA u holds column
+// 32 (u >> 1) + 8 (rho >> 2) + 4 (u & 1) + (rho & 3): a lane's results of two
+// MFMAs are 8 consecutive columns.  kColumns: the weights' rows of the 64
+// columns go through the wave's LDS and are read transposed.
 template <int KJ, int RB, bool kColumns, bool kGroup>
 __global__ __launch_bounds__(256, up_occupancy(KJ, RB)) void adapter_up_kernel(UpParams p) {
   static_assert(!kGroup || RB == 1, "a group's tile has 16 rows");

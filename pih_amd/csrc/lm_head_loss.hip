@@ -22,6 +22,13 @@
 // exact.  (All of up_t rounded inside g: dx and dw off by 0.34 % of their norm,
 // 0.17 % of it bf16 results' own.)
 //
+// Measured: 4096 rows, 129280 x 4096 3.12-3.28 ms (1.32-1.39 PFLOP/s; a library
+// product of that shape alone 3.25 ms) and 9.7-10.1 ms for the gradients, bound
+// by the matrix pipe, 68 % busy, and the power it takes (1.9 GHz); 33 rows, 151936
+// x 1024 67 us, of which the weights' 311 MB take 61 at 5.1 TB/s; the gradients
+// of 1021 rows there 1.03-1.07 ms (0.93 PFLOP/s: of a 256 x 256 tile's 32 us 9
+// are the exponentials and the stores).
+//
 // Rows without a target take no part in the gradients: their g is 0, and the
 // x of dw's product is a copy with those rows as zeros, so that nothing an
 // unused row holds (infinities, NaN) reaches dw.
@@ -634,7 +641,8 @@ void launch_big(const BigArgs& p, hipStream_t s) {
   launch_rows<256, AT, BT, EPI>(p, s);
 }
 
-// A row's pairs joined, by a wave: lse = M + log(sum of s exp(m - M))
+// A row's pairs joined, by a wave: lse = M + log(sum of s exp(m - M)).  33 rows
+// of 594 pairs 6 us, 4096 rows of 505 9 us.
 __global__ __launch_bounds__(256) void loss_join_kernel(const float2* stats, const float* target_logit,
                                                         const uint32_t* target, float* loss, float* lse, uint32_t* err,
                                                         uint32_t rows, uint32_t vocab, uint32_t tiles) {
