@@ -618,33 +618,55 @@ void launch_rows(BigArgs p, hipStream_t s) {
   const uint32_t grid = std::min((p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8, kCus);
   hipLaunchKernelGGL((loss_big_kernel<ROWS, AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
 }
-// Rows of a tile by the time of the rounds of tiles on the CUs: a step and a
-// tile's own beginning and end cost (us)
+// Time (us) of m rows in tiles of `rows`: the rounds of tiles on the CUs, each a
+// step's time and a tile's own beginning and end
 //   256 rows 1.45 and 9,  128 rows 0.95 and 7,  64 rows 0.70 and 6.
-inline uint32_t tile_rows(const BigArgs& p) {
-  const uint32_t steps = (p.k / KB + std::max(p.splits, 1u) - 1) / std::max(p.splits, 1u);
-  auto cost = [&](uint32_t rows, float step, float tile) {
-    const uint64_t tiles = (uint64_t)((p.m + rows - 1) / rows) * ((p.n + TB - 1) / TB) * std::max(p.splits, 1u);
-    return (float)((tiles + kCus - 1) / kCus) * (tile + step * (float)steps);
-  };
-  const float c256 = cost(256, 1.45f, 9.0f), c128 = cost(128, 0.95f, 7.0f), c64 = cost(64, 0.70f, 6.0f);
+inline float rows_cost(const BigArgs& p, uint32_t m, uint32_t rows) {
+  const uint32_t splits = std::max(p.splits, 1u), steps = (p.k / KB + splits - 1) / splits;
+  const uint64_t tiles = (uint64_t)((m + rows - 1) / rows) * ((p.n + TB - 1) / TB) * splits;
+  const float tile = rows == 256 ? 9.0f + 1.45f * steps : rows == 128 ? 7.0f + 0.95f * steps : 6.0f + 0.70f * steps;
+  return (float)((tiles + kCus - 1) / kCus) * tile;
+}
+inline uint32_t tile_rows(const BigArgs& p, uint32_t m) {
+  const float c256 = rows_cost(p, m, 256), c128 = rows_cost(p, m, 128), c64 = rows_cost(p, m, 64);
   return c64 < c128 && c64 < c256 ? 64 : c128 < c256 ? 128 : 256;
+}
+template <bool AT, bool BT, int EPI>
+void launch_any(const BigArgs& p, hipStream_t s) {
+  const uint32_t rows = tile_rows(p, p.m);
+  if (rows == 64) launch_rows<64, AT, BT, EPI>(p, s);
+  else if (rows == 128) launch_rows<128, AT, BT, EPI>(p, s);
+  else launch_rows<256, AT, BT, EPI>(p, s);
 }
 // (the gradient of the weights has the vocabulary for rows: always many)
 template <bool AT, bool BT, int EPI>
-void launch_big(const BigArgs& p, hipStream_t s) {
-  if constexpr (!AT) {
-    const uint32_t rows = tile_rows(p);
-    if (rows == 64) {
-      launch_rows<64, AT, BT, EPI>(p, s);
-      return;
+void launch_big(BigArgs p, hipStream_t s) {
+  if constexpr (AT) {
+    launch_rows<256, AT, BT, EPI>(p, s);
+  } else {
+    // the rows behind the last whole 256 in a launch of their own where that is
+    // cheaper, although B is read once more (at 5 TB/s) and the launch costs 3
+    // us: 800 rows over 151936 x 1024 309 -> 283 us; 257 rows would go 154 -> 171
+    const uint32_t whole = p.m / 256 * 256, rest = p.m - whole;
+    const float again = std::max(rows_cost(p, rest, tile_rows(p, rest)), (float)p.n * (float)p.k * (2.0f / 5.0e6f)) + 3.0f;
+    if (whole && rest && rows_cost(p, whole, 256) + again < rows_cost(p, p.m, tile_rows(p, p.m))) {
+      BigArgs q = p;
+      q.m = whole;
+      launch_rows<256, AT, BT, EPI>(q, s);
+      p.m = rest;
+      p.a += whole * p.lda;
+      p.target += whole;
+      if constexpr (EPI == kEpiStats) {
+        p.stats += (uint64_t)whole * ((p.n + TB - 1) / TB);
+        p.target_logit += whole;
+      } else {
+        p.lse += whole;
+        p.mantissa += whole;
+        p.out = static_cast<uint8_t*>(p.out) + whole * p.ldo * (EPI == kEpiAdd ? 4 : 2);
+      }
     }
-    if (rows == 128) {
-      launch_rows<128, AT, BT, EPI>(p, s);
-      return;
-    }
+    launch_any<AT, BT, EPI>(p, s);
   }
-  launch_rows<256, AT, BT, EPI>(p, s);
 }
 
 // A row's pairs joined, by a wave: lse = M + log(sum of s exp(m - M)).  33 rows

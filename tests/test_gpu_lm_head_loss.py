@@ -295,9 +295,10 @@ def test_captured_and_replayed(eng):
 
 
 # tiles of 128 and 256 rows (the sizes above take 64), of every product: the
-# logits' in the first two, dx's in the others, whose columns are split too
+# logits' in the first two, dx's in the next two, whose columns are split too;
+# and the logits in two launches, of 768 rows and the 22 behind them
 @pytest.mark.parametrize("rows,vocab,hidden", [(1003, 8190, 64), (301, 29999, 64), (1000, 8200, 2048),
-                                               (190, 16380, 2048)])
+                                               (190, 16380, 2048), (790, 20400, 128)])
 def test_taller_tiles(eng, rows, vocab, hidden):
     import torch
 
