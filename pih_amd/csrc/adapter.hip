@@ -1111,9 +1111,9 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   p.per_split = split_columns(p.tiles, a.k, a.n, a.rank, p.blocks);
   p.splits[0] = splits_of(a.k, p.per_split);
   p.splits[1] = splits_of(a.n, p.per_split);
-  // row splits of the gradients: two rounds of blocks, 256 rows each at least
+  // row splits of the gradients: two rounds of blocks, 512 rows each at least
   const uint64_t blocks = (uint64_t)a.adapters * ((a.n + 63) / 64 + (a.k + 63) / 64);
-  p.grad_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((a.rows + 255) / 256, 1024 / blocks));
+  p.grad_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((a.rows + 511) / 512, 1024 / blocks));
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;

@@ -9,8 +9,8 @@
 // tile, and the target's logit where they hold it; a second launch joins a
 // row's pairs.  Backward: pieces of the vocabulary.  For a piece the logits
 // are computed again and leave as g, bf16 [rows][piece] in the workspace
-// (128 MB, so that it stays in the memory-side cache between its writer and its
-// two readers; 4096 columns at least, which is more above 16384 rows), then dw of the piece is g^T x, and dx
+// (128 MB or so, so that it stays in the memory-side cache between its writer and
+// its two readers; 4096 columns or so, which is more, above 16384 rows), then dw of the piece is g^T x, and dx
 // grows by g W_piece in fp32.
 //
 // g is rounded to bf16 for the matrix cores: 2^-9 of each element at most,
@@ -791,11 +791,31 @@ bool shape_ok(uint32_t rows, uint32_t vocab, uint32_t hidden) {
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// columns of a piece: 2^26 elements of g, in whole tiles
-uint32_t piece_columns(uint32_t rows, uint32_t vocab) {
-  const uint32_t all = (vocab + 255) / 256 * 256;
-  const uint32_t fit = (uint32_t)((1ull << 26) / rows / 256 * 256);
-  return std::min(all, std::max(fit, 4096u));
+// Columns of a piece, in whole tiles: 2/3 to 4/3 of 2^26 elements of g (of 4096
+// columns at least, or all columns), by the rounds of tiles that a piece's logits
+// and weights' gradient take and 25 us of its own (three launches, and dx's sums
+// read and written once more).  1021 rows over 151936 x 1024: two pieces, 990 us,
+// three of 2^26 elements 1031; 4096 rows: pieces of whole rounds 3476 us, nine
+// even ones 4284.
+uint32_t piece_columns(uint32_t rows, uint32_t vocab, uint32_t hidden) {
+  const uint32_t all = (vocab + TB - 1) / TB, tall = (rows + 255) / 256, wide = (hidden + TB - 1) / TB;
+  const uint32_t fit = (uint32_t)std::max<uint64_t>((1ull << 26) / rows, 4096) / TB;
+  const uint32_t most = std::max(1u, fit + fit / 3);
+  if (all <= most) return all * TB;
+  auto time = [&](uint64_t tiles, uint32_t k) {
+    return (float)((tiles + kCus - 1) / kCus) * (9.0f + 1.45f * (float)k / KB);
+  };
+  auto piece = [&](uint64_t c) { return c ? time(tall * c, hidden) + time(wide * c, rows) + 25.0f : 0.0f; };
+  uint32_t best = most;
+  float least = INFINITY;
+  for (uint32_t c = most; c >= std::max(1u, fit - fit / 3); --c) {
+    const float cost = (float)(all / c) * piece(c) + piece(all % c);
+    if (cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best * TB;
 }
 
 // the tiles fed by DMA take 64-deep steps
@@ -807,7 +827,7 @@ struct BackwardPlan {
 };
 BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   BackwardPlan p{};
-  p.piece = piece_columns(rows, vocab);
+  p.piece = piece_columns(rows, vocab, hidden);
   const uint64_t row_up = (rows + 63) / 64 * 64;
   p.g = 0;
   p.live = p.g + padded(row_up * p.piece * 2);

@@ -127,8 +127,8 @@ def test_backward(eng, rows, vocab, hidden):
 
 
 def test_several_pieces_of_the_vocabulary(eng):
-    """More columns than a piece holds (2^26 elements: 60928 columns at these
-    rows), the last piece a short one; 64 bits on the GPU."""
+    """More columns than a piece holds (about 2^26 elements, 60928 columns at
+    these rows); 64 bits on the GPU."""
     import torch
 
     from pih_amd.linear import lm_head_loss, lm_head_loss_backward
