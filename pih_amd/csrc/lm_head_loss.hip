@@ -655,14 +655,16 @@ void launch_big(BigArgs p, hipStream_t s) {
       launch_rows<256, AT, BT, EPI>(q, s);
       p.m = rest;
       p.a += whole * p.lda;
-      p.target += whole;
       if constexpr (EPI == kEpiStats) {
         p.stats += (uint64_t)whole * ((p.n + TB - 1) / TB);
         p.target_logit += whole;
       } else {
+        p.out = static_cast<uint8_t*>(p.out) + whole * p.ldo * (EPI == kEpiAdd ? 4 : 2);
+      }
+      if constexpr (EPI != kEpiAdd) p.target += whole;
+      if constexpr (EPI == kEpiGrad) {
         p.lse += whole;
         p.mantissa += whole;
-        p.out = static_cast<uint8_t*>(p.out) + whole * p.ldo * (EPI == kEpiAdd ? 4 : 2);
       }
     }
     launch_any<AT, BT, EPI>(p, s);

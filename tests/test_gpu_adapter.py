@@ -462,3 +462,49 @@ def test_short_segments_captured(eng):
         torch.cuda.synchronize()
         assert torch.equal(held, eager)
     assert int(flag.item()) == 0
+
+
+def test_rows_more_than_4_gib_apart(eng):
+    """x, base and output (in place), dy and dx as rows of one buffer each,
+    whose last row lies past 2^32 bytes."""
+    import torch
+
+    from pih_amd.linear import adapter_backward, adapter_gemm
+
+    c = _case(401, [2, 1], [1, 0], 16, 72, 136, 2)
+    d = _dev(c)
+    apart = (1 << 30) + 64
+    far = {}
+    for name in ("x", "base", "dy", "dbase"):
+        flat = torch.empty(2 * apart + d[name].shape[1], dtype=torch.bfloat16, device="cuda")
+        far[name] = flat.as_strided(d[name].shape, (apart, 1))
+        far[name].copy_(d[name])
+    args = (d["a"], d["b"], d["scale"], d["offsets"], d["adapters"])
+    want = adapter_gemm(d["x"], *args, base=d["base"])[0]
+    grads = adapter_backward(d["dy"], d["x"], *args, base=d["dbase"])
+    got, flag = adapter_gemm(far["x"], *args, base=far["base"], out=far["base"])
+    out = adapter_backward(far["dy"], far["x"], *args, base=far["dbase"], out=far["dbase"], flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    assert torch.equal(got, want)
+    assert all(torch.equal(p, q) for p, q in zip(out[:3], grads[:3]))
+
+
+def test_stacks_past_4_gib(eng):
+    """The last of 530 adapters of 4.4 GB of A and of B (only two are filled)."""
+    import torch
+
+    from pih_amd.linear import adapter_gemm
+
+    c = _case(409, [17, 30], [0, 1], 128, 32768, 32768, 2)
+    d = _dev(c)
+    want = adapter_gemm(d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"], base=d["base"])[0]
+    a = torch.empty(530, 128, 32768, dtype=torch.bfloat16, device="cuda")
+    b = torch.empty(530, 32768, 128, dtype=torch.bfloat16, device="cuda")
+    scale = torch.zeros(530, device="cuda")
+    for at, i in ((529, 0), (3, 1)):
+        a[at], b[at], scale[at] = d["a"][i], d["b"][i], d["scale"][i]
+    ids = torch.tensor([529, 3], dtype=torch.int32, device="cuda")
+    got, flag = adapter_gemm(d["x"], a, b, scale, d["offsets"], ids, base=d["base"])
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.equal(got, want)

@@ -341,3 +341,40 @@ def test_other_streams_at_once(eng):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(p, q) for g in got[i] for p, q in zip(g, want[i]))
+
+
+def test_weights_past_4_gib(eng):
+    """2^20 vocabulary entries of 2112 (4.4 GB), 1009 different ones over and
+    over: the sums follow from those, each so many times."""
+    import torch
+
+    from pih_amd.linear import lm_head_loss, lm_head_loss_backward
+
+    vocab, hidden, rows, kinds = 1 << 20, 2112, 5, 1009
+    x, few, _, up = (t.cuda() for t in _case(97, rows, kinds, hidden))
+    w = few.repeat((vocab + kinds - 1) // kinds, 1)[:vocab].contiguous()
+    target = torch.tensor([0, vocab - 1, 123456, vocab // 2 + 7, vocab - 300], dtype=torch.int32, device="cuda")
+    logits, e, _, _, _, _, _, _ = _ref(x, few, target % kinds)
+    times = torch.bincount(torch.arange(vocab, device="cuda") % kinds, minlength=kinds).double()
+    lse = torch.logsumexp(logits + times.log(), 1)
+    elog = e.max(1).values + (vocab / 64 + 48) * U + lse.abs() * 2 * U
+    at = (target.long() % kinds)[:, None]
+    loss = lse - logits.gather(1, at)[:, 0]
+    got, glse, flag = lm_head_loss(x, w, target)
+    _within(glse, lse.cpu(), elog.cpu(), "lse")
+    _within(got, loss.cpu(), (elog + e.gather(1, at)[:, 0] + loss.abs() * U).cpu(), "loss")
+    gx, gw, _ = lm_head_loss_backward(x, w, target, glse, up, flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    # (an entry's gradient in the last 1009 of them and around the targets)
+    for first in (0, 123456 - 4, vocab // 2, vocab - kinds):
+        take = torch.arange(first, min(first + kinds, vocab), device="cuda")
+        g = torch.exp(logits - glse.double()[:, None])[:, take % kinds]
+        eg = up.double().abs()[:, None] * g * (1.1 * e[:, take % kinds] + 64 * U + 2.0 ** -21)
+        g = (g - (take == target[:, None]).double()) * up.double()[:, None]
+        eg += g.abs() * (2 * U + HALF_BF16) + up.double().abs()[:, None] * U
+        ref = g.T @ x.double()
+        err = eg.T @ x.double().abs() * 1.01
+        err += ref.abs() * HALF_BF16 + 1e-37
+        _within(gw[take], ref.cpu(), (err + 256 * U * (g.abs().T @ x.double().abs())).cpu(), f"dw from {first}")
+    assert bool(torch.isfinite(gx).all())
