@@ -26,8 +26,8 @@
 // product of that shape alone 3.25 ms) and 9.7-10.1 ms for the gradients, bound
 // by the matrix pipe, 68 % busy, and the power it takes (1.9 GHz); 33 rows, 151936
 // x 1024 67 us, of which the weights' 311 MB take 61 at 5.1 TB/s; the gradients
-// of 1021 rows there 1.03-1.07 ms (0.93 PFLOP/s: of a 256 x 256 tile's 32 us 9
-// are the exponentials and the stores).
+// of 1021 rows there 0.99 ms (0.96 PFLOP/s: of a 256 x 256 tile's 32 us 9 are the
+// exponentials and the stores).
 //
 // Rows without a target take no part in the gradients: their g is 0, and the
 // x of dw's product is a copy with those rows as zeros, so that nothing an
