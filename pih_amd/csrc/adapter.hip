@@ -761,7 +761,7 @@ __global__ __launch_bounds__(256, tall_occupancy(KJ)) void adapter_up_tall_kerne
     }
     if (live && g + 1 < end) stage(at ^ 1, next);
     now = next;
-    __syncthreads();
+    block_lds_barrier();
   }
 }
 
@@ -827,6 +827,32 @@ struct GradParams {
   GradSide side[2];
   uint32_t rank, splits;
 };
+
+// the block's sums, [64 columns][rank], to the gradient or the split's part
+template <int NJ, bool kB>
+__device__ __forceinline__ void write_grads(const GradParams& p, const GradSide& d, uint32_t adapter, uint32_t c0,
+                                            const float* sums) {
+  constexpr uint32_t kSumRow = NJ * 16 + 4;
+  const uint32_t tid = threadIdx.x;
+  float* const out = p.splits > 1 ? d.part + (uint64_t)blockIdx.y * p.seg.adapters * p.rank * d.cols : d.out;
+  const uint32_t cols = min(64u, d.cols - c0);
+  if constexpr (kB) {
+    // one contiguous piece: columns c0 .., rank values each
+    float* const o = out + ((uint64_t)adapter * d.cols + c0) * p.rank;
+    for (uint32_t i = tid; i < cols * (p.rank / 4); i += 256) {
+      const uint32_t col = i / (p.rank / 4), j = i % (p.rank / 4) * 4;
+      *reinterpret_cast<v4f*>(o + 4 * (uint64_t)i) = *reinterpret_cast<const v4f*>(sums + col * kSumRow + j);
+    }
+  } else {
+    for (uint32_t i = tid; i < p.rank * 16; i += 256) {
+      const uint32_t j = i / 16, col = i % 16 * 4;
+      if (col >= cols) continue;
+      const float* const from = sums + col * kSumRow + j;
+      *reinterpret_cast<v4f*>(out + ((uint64_t)adapter * p.rank + j) * d.cols + c0 + col) =
+          v4f{from[0], from[kSumRow], from[2 * kSumRow], from[3 * kSumRow]};
+    }
+  }
+}
 
 // 64 columns of one adapter's gradient over its rows, in blocks of 32 rows at
 // multiples of 32; with several splits, every splits-th group of four blocks.
@@ -916,33 +942,134 @@ __device__ __forceinline__ void grad_tile(const GradParams& p, const GradSide& d
       }
   }
   __syncthreads();
-  float* const out = p.splits > 1 ? d.part + (uint64_t)blockIdx.y * p.seg.adapters * p.rank * d.cols : d.out;
-  const uint32_t cols = min(64u, d.cols - c0);
-  if constexpr (kB) {
-    // one contiguous piece: columns c0 .., rank values each
-    float* const o = out + ((uint64_t)adapter * d.cols + c0) * p.rank;
-    for (uint32_t i = tid; i < cols * (p.rank / 4); i += 256) {
-      const uint32_t col = i / (p.rank / 4), j = i % (p.rank / 4) * 4;
-      *reinterpret_cast<v4f*>(o + 4 * (uint64_t)i) = *reinterpret_cast<const v4f*>(sums + col * kSumRow + j);
+  write_grads<NJ, kB>(p, d, adapter, c0, sums);
+}
+
+// The same for ranks above 64 and 128 columns: the waves take NJ / 4 of the
+// 16-rank pieces each and all the rows, whose columns they share in LDS, two
+// pieces' loads under way: nothing is added up between them, and the parts of h,
+// six times the rows' bytes, are read once for 128 columns.  Rank 128, 300 rows,
+// 12288 + 4096 columns 44 -> 16 us, 4099 rows 92 -> 74; at rank 64 the waves' own
+// rows are faster (4099 rows: 51 us against 68).
+template <int NJ, bool kB>
+__device__ __forceinline__ void grad_ranks_tile(const GradParams& p, const GradSide& d, uint32_t adapter, uint8_t* lds) {
+  constexpr uint32_t kPitch = 256 + 16, kStage = 32 * kPitch, kSumRow = NJ * 16 + 4, JW = NJ / 4;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t c0 = blockIdx.x * 128, c = c0 + 8 * (tid & 7), blocks16 = (p.rank + 15) / 16;
+  if (c0 >= d.cols) return;
+  // the block's 32-row pieces: every splits-th of the adapter's
+  uint32_t s = 0, lo = 0, hi = 0, first = 0, blocks = 0, at = blockIdx.y;
+  auto find = [&]() -> bool {
+    while (at >= blocks) {
+      at -= blocks;
+      blocks = 0;
+      for (; s < p.seg.segments; ++s) {
+        if (p.seg.adapter[s] != adapter) continue;
+        lo = p.seg.offsets[s], hi = p.seg.offsets[s + 1];
+        if (hi > lo && hi <= p.seg.rows) break;
+      }
+      if (s >= p.seg.segments) return false;
+      ++s;
+      first = lo / 32;
+      blocks = (hi + 31) / 32 - first;
     }
-  } else {
-    for (uint32_t i = tid; i < p.rank * 16; i += 256) {
-      const uint32_t j = i / 16, col = i % 16 * 4;
-      if (col >= cols) continue;
-      const float* const from = sums + col * kSumRow + j;
-      *reinterpret_cast<v4f*>(out + ((uint64_t)adapter * p.rank + j) * d.cols + c0 + col) =
-          v4f{from[0], from[kSumRow], from[2 * kSumRow], from[3 * kSumRow]};
+    return true;
+  };
+  struct Rows {
+    v4i x[2], h[JW][3];
+  };
+  auto load = [&](Rows& v) __attribute__((always_inline)) {
+    const uint32_t r0 = (first + at) * 32, row = r0 + (tid >> 3), r = r0 + 8 * lg;
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q) {
+      v.x[q] = v4i{0, 0, 0, 0};
+      if (row >= lo && row < hi && c + 64 * q < d.cols) v.x[q] = load16(d.src + (uint64_t)row * d.stride + c + 64 * q);
     }
+    v4i mask;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      mask[q] = (r + 2 * q >= lo && r + 2 * q < hi ? 0xffff : 0) |
+                (r + 2 * q + 1 >= lo && r + 2 * q + 1 < hi ? (int)0xffff0000 : 0);
+#pragma unroll
+    for (uint32_t j = 0; j < JW; ++j) {
+      const uint16_t* const from =
+          d.parts + ((uint64_t)(first + at) * 3 * blocks16 + min(JW * wave + j, blocks16 - 1)) * 512 + 8 * lane;
+#pragma unroll
+      for (uint32_t q = 0; q < 3; ++q) v.h[j][q] = load16(from + q * blocks16 * 512) & mask;
+    }
+  };
+  v4f acc[8][JW];
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+#pragma unroll
+    for (uint32_t j = 0; j < JW; ++j) acc[u][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  // two pieces' loads under way
+  Rows now, next, after;
+  bool more = find(), later = false;
+  if (more) {
+    load(now);
+    at += p.splits;
+    later = find();
+    if (later) load(next);
+  }
+  for (uint32_t b = 0; more; b ^= 1) {
+    more = later;
+    if (later) {
+      at += p.splits;
+      later = find();
+      if (later) load(after);
+    }
+    uint8_t* const st = lds + b * kStage;
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q)
+      *reinterpret_cast<v4i*>(st + (tid >> 3) * kPitch + 16 * (tid & 7) + 128 * q) = now.x[q];
+    block_lds_barrier();
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) {
+      const v4i x = transposed(st + (8 * lg + (lr >> 2)) * kPitch + 2 * (16 * u + 4 * (lr & 3)), kPitch);
+#pragma unroll
+      for (uint32_t j = 0; j < JW; ++j)
+#pragma unroll
+        for (int q = 2; q >= 0; --q) acc[u][j] = kB ? mfma(now.h[j][q], x, acc[u][j]) : mfma(x, now.h[j][q], acc[u][j]);
+    }
+    now = next;
+    next = after;
+  }
+  float* const sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (uint32_t half = 0; half < 2; ++half) {
+    __syncthreads();
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+      for (uint32_t j = 0; j < JW; ++j) {
+        const uint32_t rank16 = 16 * (JW * wave + j);
+        const v4f v = acc[4 * half + u][j];
+        if constexpr (kB) {  // lane: column 16 u + lr, ranks 4 lg ..
+          *reinterpret_cast<v4f*>(sums + (16 * u + lr) * kSumRow + rank16 + 4 * lg) = v;
+        } else {  // lane: rank lr, columns 16 u + 4 lg ..
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sums[(16 * u + 4 * lg + e) * kSumRow + rank16 + lr] = v[e];
+        }
+      }
+    __syncthreads();
+    if (c0 + 64 * half < d.cols) write_grads<NJ, kB>(p, d, adapter, c0 + 64 * half, sums);
   }
 }
 
 template <int NJ>
 __global__ __launch_bounds__(256) void adapter_grad_kernel(GradParams p) {
-  constexpr uint32_t kStaged = 4 * 32 * 144, kSums = 64 * (NJ * 16 + 4) * 4;
+  constexpr uint32_t kStaged = NJ == 8 ? 2 * 32 * 272 : 4 * 32 * 144, kSums = 64 * (NJ * 16 + 4) * 4;
   __shared__ __align__(16) uint8_t lds[kSums > kStaged ? kSums : kStaged];
   const uint32_t adapter = blockIdx.z >> 1;
-  if (blockIdx.z & 1) grad_tile<NJ, true>(p, p.side[1], adapter, lds);
-  else grad_tile<NJ, false>(p, p.side[0], adapter, lds);
+  if constexpr (NJ == 8) {
+    if (blockIdx.z & 1) grad_ranks_tile<NJ, true>(p, p.side[1], adapter, lds);
+    else grad_ranks_tile<NJ, false>(p, p.side[0], adapter, lds);
+  } else {
+    if (blockIdx.z & 1) grad_tile<NJ, true>(p, p.side[1], adapter, lds);
+    else grad_tile<NJ, false>(p, p.side[0], adapter, lds);
+  }
 }
 
 // the splits of the gradients, in order: of A, then (blocks from `first_b`
@@ -1099,6 +1226,9 @@ void launch_down(const DownParams& d, uint32_t tiles, uint32_t blocks, uint32_t 
   });
 }
 
+// columns of a block of the gradients
+uint32_t grad_columns(const AdapterArgs& a) { return a.rank > 64 ? 128 : 64; }
+
 struct BackwardPlan {
   uint32_t blocks, tiles, finish_tiles, per_split, splits[2], grad_splits;
   uint64_t part[2], dh, parts[2], grads[2], bytes;
@@ -1111,9 +1241,11 @@ BackwardPlan backward_plan(const AdapterArgs& a) {
   p.per_split = split_columns(p.tiles, a.k, a.n, a.rank, p.blocks);
   p.splits[0] = splits_of(a.k, p.per_split);
   p.splits[1] = splits_of(a.n, p.per_split);
-  // row splits of the gradients: two rounds of blocks, 512 rows each at least
-  const uint64_t blocks = (uint64_t)a.adapters * ((a.n + 63) / 64 + (a.k + 63) / 64);
-  p.grad_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((a.rows + 511) / 512, 1024 / blocks));
+  // row splits of the gradients: two rounds of blocks (of 128 columns: one), 512
+  // rows each at least
+  const uint32_t width = grad_columns(a);
+  const uint64_t blocks = (uint64_t)a.adapters * ((a.n + width - 1) / width + (a.k + width - 1) / width);
+  p.grad_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((a.rows + 511) / 512, (a.rank > 64 ? 512 : 1024) / blocks));
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -1250,7 +1382,7 @@ St LaunchAdapterBackward(const AdapterArgs& a) {
   g.side[1] = GradSide{a.dy, f.parts[0], a.db, f32(plan.grads[1]), a.dy_stride, a.n};
   with_pow2((a.rank + 15) / 16, [&](auto nj) {
     hipLaunchKernelGGL((adapter_grad_kernel<decltype(nj)::value>),
-                       dim3((std::max(a.n, a.k) + 63) / 64, plan.grad_splits, 2 * a.adapters), dim3(256), 0, a.stream,
+                       dim3((std::max(a.n, a.k) + grad_columns(a) - 1) / grad_columns(a), plan.grad_splits, 2 * a.adapters), dim3(256), 0, a.stream,
                        g);
   });
   if (plan.grad_splits > 1) {

@@ -266,6 +266,15 @@ constexpr int kLdsRead = 0xC07F;
 // from forwarding a lane's own writes).
 __device__ __forceinline__ void wave_lds_order() { asm volatile("" ::: "memory"); }
 
+// A block's barrier between LDS writes and reads that leaves global loads and
+// stores under way (__syncthreads waits for them).
+__device__ __forceinline__ void block_lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(kLdsRead);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <int kWidth>
 __device__ __forceinline__ float reduce_max_xor(float v) {
 #pragma unroll

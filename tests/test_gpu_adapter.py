@@ -508,3 +508,40 @@ def test_stacks_past_4_gib(eng):
     got, flag = adapter_gemm(d["x"], a, b, scale, d["offsets"], ids, base=d["base"])
     torch.cuda.synchronize()
     assert int(flag.item()) == 0 and torch.equal(got, want)
+
+
+# as CASES: segments long enough for the tall tiles, ranks that fill none of
+# their 32-rank pieces, rows enough for several splits of the gradients
+LONG = [
+    ([600, 3, 700, 0, 41], [1, 0, 1, 2, 0], 104, 136, 264, 3, 9, 5),
+    ([130, 70, 65], [0, 1, -1], 40, 328, 72, 2, 0, 0),
+    ([1100, 64], [1, 1], 128, 72, 520, 2, 0, 3),
+    ([90, 200], [0, 0], 72, 40, 1032, 1, 1, 0),
+]
+
+
+@pytest.mark.parametrize("base", [True, False])
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_long_segments_of_odd_ranks(eng, case, base):
+    import torch
+
+    from pih_amd.linear import adapter_backward, adapter_gemm
+
+    c = _case(500 + case, *LONG[case])
+    ref, bound, written = _forward_ref(c, base)
+    (dx, ex), (da, ea), (db, eb) = _backward_ref(c, base)
+    d = _dev(c)
+    w = torch.from_numpy(written)
+    got, flag = adapter_gemm(d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"],
+                             base=d["base"] if base else None, out=torch.full_like(d["base"], 7.0))
+    args = (d["dy"], d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"])
+    grads = adapter_backward(*args, base=d["dbase"] if base else None, out=torch.full_like(d["dbase"], 7.0), flag=flag)
+    again = adapter_backward(*args, base=d["dbase"] if base else None, out=torch.full_like(d["dbase"], 7.0))
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    assert torch.all(got.cpu()[~w] == 7.0) and torch.all(grads[0].cpu()[~w] == 7.0)
+    _within(got[w.cuda()], ref[w], bound[w], f"case {case}")
+    _within(grads[0][w.cuda()], dx[w], ex[w], f"dx {case}")
+    _within(grads[1], da, ea, f"da {case}")
+    _within(grads[2], db, eb, f"db {case}")
+    assert all(torch.equal(p, q) for p, q in zip(grads[:3], again[:3]))
