@@ -1164,14 +1164,16 @@ void launch_up(UpParams p, const AdapterArgs& a, bool group) {
   const bool tall = tile_blocks(a) == 4;
   if (tall && p.rank > 32) {
     // two blocks a CU, each with as many groups as there are splits of h, which
-    // every block adds up (4099 x 4096 outputs of rank 64: 25 us; one block a CU
-    // 32, four 29; tiles of 32 rows that read the weights themselves 31.  4099 x
-    // 12288 of rank 128: 60 us, 213 with 16-row tiles)
+    // every block adds up, while that leaves a block for every other CU (4099 x
+    // 4096 outputs of rank 64: 25 us; one block a CU 32, four 29; tiles of 32 rows
+    // that read the weights themselves 31.  4099 x 12288 of rank 128: 60 us, 213
+    // with 16-row tiles.  1000 x 1024 of rank 128: 13 us; 20 with fewer blocks, 19
+    // with one for every CU)
     with_pow2((p.rank + 31) / 32, [&](auto kj) {
       constexpr int KJ = decltype(kj)::value;
       if constexpr (KJ == 2 || KJ == 4) {
         const uint32_t tiles = tile_bound(a, 64), all = (p.cols + 63) / 64, columns = std::max(1u, 2 * kCus / tiles);
-        p.groups = std::max((all + columns - 1) / columns, p.splits);
+        p.groups = std::max((all + columns - 1) / columns, std::min(p.splits, std::max(1u, 2 * all * tiles / kCus)));
         hipLaunchKernelGGL((adapter_up_tall_kernel<KJ, kColumns>), dim3(tiles, (all + p.groups - 1) / p.groups),
                            dim3(256), 0, a.stream, p);
       }
