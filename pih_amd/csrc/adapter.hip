@@ -64,9 +64,19 @@ struct Tile {
   float scale;
 };
 
+// Offsets that descend or pass the rows, of the segments from `from` on.
+__device__ __forceinline__ void report_offsets(const Segments& p, uint32_t from, uint32_t* err) {
+  for (uint32_t s = from + threadIdx.x; s < p.segments; s += blockDim.x)
+    if (p.offsets[s + 1] < p.offsets[s] || p.offsets[s + 1] > p.rows) atomicOr(err, kErrOffsets);
+}
+
 // Tile `index` of the segments' tiles of `height` rows, in order; false past
 // the last.  A segment whose offsets descend or pass the rows counts as empty.
-__device__ __forceinline__ bool find_tile(const Segments& p, uint32_t height, uint32_t index, Tile& t, uint32_t* err) {
+// The first tile's block reports such segments among the 64 that its search
+// ends in and before, with all_offsets (one launch
+// of a call) also those behind.
+__device__ __forceinline__ bool find_tile(const Segments& p, uint32_t height, uint32_t index, Tile& t, uint32_t* err,
+                                          bool all_offsets = false) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t before = 0;
   for (uint32_t s0 = 0; s0 < p.segments; s0 += 64) {
@@ -104,6 +114,7 @@ __device__ __forceinline__ bool find_tile(const Segments& p, uint32_t height, ui
       } else if (t.adapter != kNoAdapter) {
         if (threadIdx.x == 0) atomicOr(err, kErrAdapter);
       }
+      if (all_offsets && index == 0) report_offsets(p, s0 + 64, err);
       return true;
     }
     before += all;
@@ -438,7 +449,9 @@ __global__ __launch_bounds__(256, down_occupancy(NJ, RB)) void adapter_down_kern
   __shared__ __align__(16) uint8_t lds[kDownLds<NJ, kBackward>];
   Tile t;
   const DownSide& d = p.side[blockIdx.z];
-  if (blockIdx.y >= d.splits || !find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err) || t.adapter >= p.seg.adapters) return;
+  if (blockIdx.y >= d.splits || !find_tile(p.seg, 16 * RB, blockIdx.x, t, p.err, blockIdx.y + blockIdx.z == 0) ||
+      t.adapter >= p.seg.adapters)
+    return;
   auto row_of = [&](uint32_t r) { return t.row0 + r; };
   if constexpr (kBackward) {
     if (blockIdx.z) {

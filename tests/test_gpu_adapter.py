@@ -545,3 +545,41 @@ def test_long_segments_of_odd_ranks(eng, case, base):
     _within(grads[1], da, ea, f"da {case}")
     _within(grads[2], db, eb, f"db {case}")
     assert all(torch.equal(p, q) for p, q in zip(grads[:3], again[:3]))
+
+
+# segment length, rank: tiles of 16 rows, and of 64 in each of the two products with B
+@pytest.mark.parametrize("length,rank", [(1, 8), (40, 16), (70, 16), (70, 64), (66, 128)])
+@pytest.mark.parametrize("bad", [64, 70, 98, 99])
+def test_bad_offsets_behind_many_segments_are_flagged(eng, bad, length, rank):
+    """Bit 2 for an offset that the block of the first tile need not read to
+    find it, forward and backward: the end of segment `bad` of 100 passes the
+    rows, and the next one's descends from there.  What is left out, and all
+    else, is as with no adapter on those segments."""
+    import torch
+
+    from pih_amd.linear import adapter_backward, adapter_gemm
+
+    stacks = 100 if length == 1 else 3  # (an adapter each: no tiles across segments)
+    c = _case(600 + bad, [length] * 100, [i % stacks for i in range(100)], rank, 40, 72, stacks)
+    d = _dev(c)
+    args = (d["a"], d["b"], d["scale"])
+    none = d["adapters"].clone()
+    none[bad:bad + 2] = -1
+    left = slice(bad * length, min(bad + 2, 100) * length)
+
+    def calls(offsets, adapters):
+        out, dx = torch.full_like(d["base"], 7.0), torch.full_like(d["dbase"], 7.0)
+        _, flag = adapter_gemm(d["x"], *args, offsets, adapters, base=d["base"], out=out)
+        _, da, db, back = adapter_backward(d["dy"], d["x"], *args, offsets, adapters, base=d["dbase"], out=dx)
+        torch.cuda.synchronize()
+        return out, dx, da, db, int(flag.item()), int(back.item())
+
+    want = calls(d["offsets"], none)
+    assert want[4:] == (0, 0)
+    want[0][left], want[1][left] = 7.0, 7.0
+    offsets = d["offsets"].clone()
+    offsets[bad + 1] = 100 * length + 1
+    got = calls(offsets, d["adapters"])
+    assert got[4:] == (2, 2)
+    for p, q in zip(got[:4], want[:4]):
+        assert torch.equal(p, q)
