@@ -512,7 +512,9 @@ def _workspace(kind: int, m: int, n: int, k: int, device) -> torch.Tensor:
 @functools.lru_cache(maxsize=None)
 def _entry(entry: str, name: str):
     t = abi.LN[name]
-    return getattr(_ln().table, entry), t, abi.C.sizeof(t)
+    # (the 32-bit sizes and strides, which follow one another in every request)
+    words = [i for i, (_, kind) in enumerate(t._fields_[2:]) if kind is abi.U32]
+    return getattr(_ln().table, entry), t, abi.C.sizeof(t), slice(words[0], words[-1] + 1)
 
 
 _byref = abi.C.byref
@@ -521,7 +523,9 @@ _byref = abi.C.byref
 def _launch(entry: str, name: str, *fields) -> None:
     """The entry called with its request's fields in order (one constructor
     call: 2 us less of host time than setting twenty fields by name)."""
-    call, t, size = _entry(entry, name)
+    call, t, size, words = _entry(entry, name)
+    if max(fields[words]) > 0xFFFFFFFF:  # (a request's field would keep the lower half)
+        raise ValueError(f"pih_amd: {name} takes sizes and strides of 32 bits")
     status = call(_byref(t(size, 1, *fields)))
     if status.code:
         _check(status, name)

@@ -187,3 +187,100 @@ def test_python_callers_refuse_host_tensors_and_wrong_types():
     with pytest.raises(ValueError, match="counts"):
         linear.router_backward(torch.zeros(4, 64), i32(4, 2), None, abi.ROUTER_SOFTMAX, 0.01, torch.ones(1),
                                flag=i32(1))
+
+
+class _Recorded:
+    """The linear pack with its launches recorded in place of made."""
+
+    def __init__(self):
+        self.table, self.launched = self, []
+
+    def call(self, entry, request):
+        return abi.linear_pack().call(entry, request)
+
+    def __getattr__(self, entry):
+        def launch(request):
+            self.launched.append(entry)
+            return abi.Status(struct_size=C.sizeof(abi.Status), abi_version=1, code=abi.OK)
+        return launch
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """Python callers over tensors that have sizes and strides but no memory."""
+    from pih_amd import linear
+
+    pack = _Recorded()
+    monkeypatch.setattr(linear, "_ln", lambda: pack)
+    monkeypatch.setattr(linear, "same_device", lambda *t: None)
+    monkeypatch.setattr(linear, "device_ptrs", lambda *t: [0x10000 if v is not None else 0 for v in t])
+    monkeypatch.setattr(linear, "stream_handle", lambda: 0x10000)
+    linear._entry.cache_clear()
+    yield pack
+    linear._entry.cache_clear()
+
+
+def _sizes_past_32_bits():
+    import torch
+
+    from pih_amd import linear
+
+    def meta(*shape, dtype=torch.bfloat16, stride=None):
+        if stride is None:
+            return torch.empty(shape, dtype=dtype, device="meta")
+        return torch.empty_strided(shape, (stride, 1), dtype=dtype, device="meta")
+
+    i32, f32 = torch.int32, torch.float32
+    a, b, flag, big = meta(2, 8, 64), meta(2, 32, 8), meta(1, dtype=i32), 1 << 32
+
+    def gemm(rows=3, segments=1, x=None, base=None, out=None):
+        return lambda: linear.adapter_gemm(meta(rows, 64, stride=x), a, b, None, meta(segments + 1, dtype=i32),
+                                           meta(segments, dtype=i32), base=base and meta(rows, 32, stride=base),
+                                           out=meta(rows, 32, stride=out or 32), flag=flag)
+
+    def backward(rows=3, dy=None, x=None, base=None, out=None):
+        return lambda: linear.adapter_backward(meta(rows, 32, stride=dy), meta(rows, 64, stride=x), a, b, None,
+                                               meta(2, dtype=i32), meta(1, dtype=i32),
+                                               base=base and meta(rows, 64, stride=base),
+                                               out=meta(rows, 64, stride=out or 64), flag=flag)
+
+    def loss(rows, vocab):
+        return lambda: linear.lm_head_loss(meta(rows, 64), meta(vocab, 64), meta(rows, dtype=i32), flag=flag)
+
+    def loss_backward(rows, vocab):
+        return lambda: linear.lm_head_loss_backward(meta(rows, 64), meta(vocab, 64), meta(rows, dtype=i32),
+                                                    meta(rows, dtype=f32), meta(rows, dtype=f32), flag=flag)
+
+    def balance(tokens, mode):
+        return lambda: linear.router_balance(meta(tokens, 8, dtype=f32), meta(tokens, 2, dtype=i32), mode, 0.1,
+                                             flag=flag)
+
+    def router_backward(tokens, mode):
+        return lambda: linear.router_backward(meta(tokens, 8, dtype=f32), meta(tokens, 2, dtype=i32), None, mode, 0.1,
+                                              None, dweights=meta(tokens, 2, dtype=f32), flag=flag)
+
+    good = [gemm(x=64, base=32), backward(dy=32, x=64, base=64), loss(3, 5), loss_backward(3, 5), balance(3, 1),
+            router_backward(3, 1)]
+    bad = [gemm(x=big + 64), gemm(base=big + 40), gemm(out=big + 32), gemm(rows=big + 3), gemm(segments=big + 1),
+           backward(dy=big + 32), backward(x=big + 72), backward(base=big + 64), backward(out=big + 64),
+           backward(rows=big + 3), loss(big + 3, 5), loss(3, big + 5), loss_backward(big + 3, 5),
+           loss_backward(3, big + 5), balance(big + 3, 1), balance(3, big + 1), router_backward(big + 3, 1),
+           router_backward(3, big + 1)]
+    return good, bad
+
+
+@pytest.mark.parametrize("case", range(18))
+def test_sizes_past_32_bits_are_refused(recorded, case):
+    """Sizes and strides whose lower 32 bits alone are valid."""
+    good, bad = _sizes_past_32_bits()
+    assert len(bad) == 18
+    with pytest.raises(ValueError, match="32 bits"):
+        bad[case]()
+    assert not recorded.launched
+
+
+def test_sizes_within_32_bits_are_launched(recorded):
+    good, _ = _sizes_past_32_bits()
+    for call in good:
+        call()
+    assert len(recorded.launched) == len(good)
