@@ -425,7 +425,9 @@ typedef struct pih_amd_v41_block_dequant_launch_v1 {
  * rank a multiple of 8 up to 128; n, k and the strides multiples of 8; every
  * address 16-byte aligned (the u32 and f32 arrays 4-byte).  The product with
  * A is summed in fp32 and enters the second product as the sum of two bf16
- * values (2^-16 relative), so the only rounding to bf16 is the output's.
+ * values (2^-16 relative), so the only rounding to bf16 is the output's.  An
+ * infinite value of it stays one; an infinite weight of B may give NaN where
+ * the formula gives an infinity.
  * workspace (16-byte aligned): query_workspace(ADAPTER_GEMM, row_count, rank, k).
  * Error bits: 1 an adapter id that is neither 0xFFFFFFFF nor below
  * adapter_count (its rows are left unwritten), 2 offsets that descend or
@@ -451,8 +453,9 @@ typedef struct pih_amd_adapter_gemm_launch_v1 {
  * every adapter, zero where it has no row.  dx rows outside every segment
  * are left as they are; dx may be base, but neither dy nor input, which are
  * read after it is written.  Sums run in a fixed order: the same call gives the
- * same bits.  Conditions, alignment and error bits are those of
- * pih_amd_adapter_gemm_launch_v1.  query_adapter_backward_workspace writes
+ * same bits.  An infinite weight of A (in dx), input (in da) or dy (in db) may
+ * give NaN where the formula gives an infinity.  Conditions, alignment and error
+ * bits are those of pih_amd_adapter_gemm_launch_v1.  query_adapter_backward_workspace writes
  * the byte count that `workspace` needs (from row_count, segment_count,
  * adapter_count, rank, n and k) to *required_bytes_u64, a host address. */
 typedef struct pih_amd_adapter_backward_launch_v1 {

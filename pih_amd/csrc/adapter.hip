@@ -233,11 +233,15 @@ __device__ __forceinline__ v4i transposed(const uint8_t* x, uint32_t pitch) {
   const uint2 u = __builtin_bit_cast(uint2, a), v = __builtin_bit_cast(uint2, b);
   return v4i{(int)u.x, (int)u.y, (int)v.x, (int)v.y};
 }
+// A part of a value in bf16 that leaves the rest to the next: at most the
+// largest bf16, so that an infinity stays in the rest (infinite parts would
+// leave inf - inf), as does what a value past that number has above it.
+__device__ __forceinline__ float part_of(float v) { return __builtin_amdgcn_fmed3f(v, -0x1.fep127f, 0x1.fep127f); }
 // fp32 values as bf16 hi + lo, eight of them
 __device__ __forceinline__ void split8(const float* v, v4i& hi, v4i& lo) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t h = f32x2_to_bf16x2(v[2 * i], v[2 * i + 1]);
+    const uint32_t h = f32x2_to_bf16x2(part_of(v[2 * i]), part_of(v[2 * i + 1]));
     const float l0 = v[2 * i] - bf16_bits_to_f32(h & 0xffffu), l1 = v[2 * i + 1] - bf16_bits_to_f32(h >> 16);
     hi[i] = (int)h;
     lo[i] = (int)f32x2_to_bf16x2(l0, l1);
@@ -820,7 +824,7 @@ __global__ __launch_bounds__(256) void adapter_finish_kernel(FinishParams p) {
                            (row / 8 % 4 * 16 + j % 16) * 8 + row % 8;
 #pragma unroll
     for (uint32_t q = 0; q < 3; ++q) {
-      const uint32_t h = f32_to_bf16_bits(v);
+      const uint32_t h = f32_to_bf16_bits(q < 2 ? part_of(v) : v);
       part[q * blocks * 512] = (uint16_t)h;
       v -= bf16_bits_to_f32(h);
     }

@@ -583,3 +583,102 @@ def test_bad_offsets_behind_many_segments_are_flagged(eng, bad, length, rank):
     assert got[4:] == (2, 2)
     for p, q in zip(got[:4], want[:4]):
         assert torch.equal(p, q)
+
+
+# each kernel of the product with B: tiles of 16, 32 and 64 rows, of rows from all segments
+@pytest.mark.parametrize("lengths,adapters,rank", [([9, 4], [1, 0], 24), ([70, 81], [1, 0], 16), ([70, 81], [0, 1], 72),
+                                                   ([1] * 40, [i % 2 for i in range(40)], 16)])
+def test_infinite_and_largest_products_with_a(eng, lengths, adapters, rank):
+    """An infinite x . A (and dy . B) is infinite in out (dx) and in db (da),
+    and a finite one past the largest bf16 stays finite: three rows with
+    x[0] = +-inf or with x[:2] of the largest bf16 and 2^119 (a sum of
+    0x1.ff * 2^127, which bf16 rounds to infinity), A[:, :2] = 1, B >= 0."""
+    import torch
+
+    from pih_amd.linear import adapter_backward, adapter_gemm
+
+    c = _case(700 + rank, lengths, adapters, rank, 40, 72, 2, scale=False)
+    rows = sum(lengths)
+    plus, minus, large = 1, rows // 2, rows - 1
+    for t in (c["x"], c["dy"]):
+        t[plus, 0], t[minus, 0] = float("inf"), float("-inf")
+        t[large] = 0
+        t[large, 0], t[large, 1] = torch.finfo(torch.bfloat16).max, 2.0 ** 119
+    # dx and db of the rows with infinite dy take A and x of one sign
+    c["a"], c["b"] = c["a"].abs() + 2.0 ** -10, c["b"].abs() + 2.0 ** -10
+    forward = {**c, "a": c["a"].clone()}
+    forward["a"][:, :, :2] = 1
+    forward["b"] = (c["b"] * 2.0 ** -4 / rank).to(torch.bfloat16)
+    d = _dev(forward)
+    args = (d["x"], d["a"], d["b"], None, d["offsets"], d["adapters"])
+    out, flag = adapter_gemm(*args, base=d["base"])
+    finite = c["dy"].clone()
+    finite[[plus, minus, large]] = 1
+    dx, da, db, _ = adapter_backward(finite.cuda(), *args, flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    out, dx, db = out.cpu(), dx.cpu(), db.cpu()
+    assert torch.all(out[plus] == float("inf")) and torch.all(out[minus] == float("-inf"))
+    rest = torch.ones(rows, dtype=torch.bool)
+    rest[[plus, minus]] = False
+    plain = {**forward, "x": forward["x"].clone(), "dy": finite}
+    plain["x"][[plus, minus]] = 0
+    ref, bound, _ = _forward_ref(plain, True)
+    assert torch.isfinite(out[large]).all()
+    _within(out[rest], ref[rest], bound[rest], "out")
+    assert torch.isfinite(dx).all()  # (x takes no part in it)
+    owner = {a: [r for lo, hi, i in _segments(c) if i == a for r in (plus, minus, large) if lo <= r < hi] for a in (0, 1)}
+    for a, held in owner.items():
+        if held and set(held) <= {plus}:
+            assert torch.all(db[a] == float("inf"))
+        if held and set(held) <= {minus}:
+            assert torch.all(db[a] == float("-inf"))
+        if held == [large]:
+            assert torch.isfinite(db[a]).all()
+    # the same of dy . B: dx and da
+    back = {**c, "b": c["b"].clone(), "x": torch.ones_like(c["x"])}
+    back["b"][:, :2] = 1
+    back["a"] = (c["a"] * 2.0 ** -4 / rank).to(torch.bfloat16)
+    d = _dev(back)
+    dx, da, db, flag = adapter_backward(d["dy"], d["x"], d["a"], d["b"], None, d["offsets"], d["adapters"])
+    torch.cuda.synchronize()
+    dx, da = dx.cpu(), da.cpu()
+    assert int(flag.item()) == 0
+    assert torch.all(dx[plus] == float("inf")) and torch.all(dx[minus] == float("-inf"))
+    assert torch.isfinite(dx[rest]).all()
+    for a, held in owner.items():
+        if held and set(held) <= {plus}:
+            assert torch.all(da[a] == float("inf"))
+        if held and set(held) <= {minus}:
+            assert torch.all(da[a] == float("-inf"))
+        if held == [large]:
+            assert torch.isfinite(da[a]).all()
+
+
+@pytest.mark.parametrize("lengths,rank", [([9], 24), ([140], 16), ([140], 72)])
+def test_a_nan_stays_in_its_row_and_adapter(eng, lengths, rank):
+    """NaN in x reaches all of its row's output and its adapter's db; in dy
+    its row's dx and its adapter's da; and nothing else."""
+    import torch
+
+    from pih_amd.linear import adapter_backward, adapter_gemm
+
+    c = _case(730 + rank, lengths + [5], [0, 1], rank, 40, 72, 2)
+    c["a"], c["b"] = c["a"].abs() + 2.0 ** -10, c["b"].abs() + 2.0 ** -10
+    for t in ("x", "dy"):
+        bad = {**c, t: c[t].clone()}
+        bad[t][3, 7] = float("nan")
+        d = _dev(bad)
+        args = (d["x"], d["a"], d["b"], d["scale"], d["offsets"], d["adapters"])
+        out, flag = adapter_gemm(*args)
+        dx, da, db, _ = adapter_backward(d["dy"], *args, flag=flag)
+        torch.cuda.synchronize()
+        assert int(flag.item()) == 0
+        row = out if t == "x" else dx
+        assert row[3].isnan().all() and torch.isfinite(row[:3]).all() and torch.isfinite(row[4:]).all()
+        assert torch.isfinite(dx if t == "x" else out).all()
+        whole, column = (db, da) if t == "x" else (da, db.transpose(1, 2))
+        assert whole[0].isnan().all() and torch.isfinite(whole[1]).all()
+        assert column[0, :, 7].isnan().all() and torch.isfinite(column[1]).all()
+        rest = torch.arange(column.shape[2], device="cuda") != 7
+        assert torch.isfinite(column[0][:, rest]).all()
