@@ -61,7 +61,9 @@ __device__ __forceinline__ float log1p01(float e) {
 
 // b(s) and its derivative.  2^(s log2 e) by the hardware exponential: off by
 // 2^-23 of itself and |s| 2^-24 from the exponent's rounding.
-template <int MODE>
+// kFar: for scores below -80 too.
+constexpr float kFarScore = -80.0f;
+template <int MODE, bool kFar>
 __device__ __forceinline__ void affinity(float s, float top, float& b, float& slope) {
   if constexpr (MODE == kRouterSoftmax) {
     b = __builtin_amdgcn_exp2f((s - top) * kLog2e);
@@ -73,6 +75,13 @@ __device__ __forceinline__ void affinity(float s, float top, float& b, float& sl
     b = __builtin_amdgcn_sqrtf(sp);
     // sigmoid / softplus tends to 1 where both underflow
     slope = sp > 1e-30f ? 0.5f * sig * __builtin_amdgcn_rcpf(b) : 0.5f * b;
+    if constexpr (kFar) {
+      // e^s leaves the normal numbers at -87, its root e^(s/2), which is b there
+      // (to 2^-117 of itself below -80), at -174
+      const float x = 0.5f * kLog2e * s, far = x >= -126.0f ? __builtin_amdgcn_exp2f(x) : 0.0f;
+      b = s < kFarScore ? far : b;
+      slope = s < kFarScore ? 0.5f * far : slope;
+    }
   }
 }
 
@@ -109,6 +118,7 @@ struct Row {
   static constexpr int N = 4 * Q;
   float b[N], slope[N], top, sum;
   uint32_t wrong;
+  bool far;  // some row of the wave has far scores
 
   static __device__ __forceinline__ uint32_t expert(int j) {
     return 4 * (LANES * (j / 4) + (threadIdx.x & (LANES - 1))) + j % 4;
@@ -147,14 +157,24 @@ struct Row {
       bad += expert(j) < experts ? nan : 0.0f;
     }
     sum = 0.0f;
+    auto all = [&](auto FAR) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float s = slope[j];
-      affinity<MODE>(s, top, b[j], slope[j]);
-      // (outside the row: -inf, whose derivative is a NaN)
-      if (expert(j) >= experts) b[j] = slope[j] = 0.0f;
-      sum += b[j];
+      for (int j = 0; j < N; ++j) {
+        const float s = slope[j];
+        affinity<MODE, decltype(FAR)::value>(s, top, b[j], slope[j]);
+        // (outside the row: -inf, whose derivative is a NaN)
+        if (expert(j) >= experts) b[j] = slope[j] = 0.0f;
+        sum += b[j];
+      }
+    };
+    float least = 0.0f;
+    if constexpr (MODE == kRouterSqrtSoftplus) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) least = fminf(least, expert(j) < experts ? slope[j] : 0.0f);
     }
+    far = MODE == kRouterSqrtSoftplus && __builtin_amdgcn_ballot_w64(least < kFarScore);
+    if (far) all(std::true_type{});
+    else all(std::false_type{});
     sum = row_sum<LANES>(sum);
     wrong = row_sum<LANES>(bad) == 0.0f ? (sum == 0.0f ? 4u : 0u) : 1u;
     if (wrong) {
@@ -347,7 +367,8 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
       float cb[kRoutes], cs[kRoutes], sum = 0.0f, back = 0.0f;
 #pragma unroll
       for (uint32_t r = 0; r < kRoutes; ++r) {
-        affinity<MODE>(chosen[r], row.top, cb[r], cs[r]);
+        if (row.far) affinity<MODE, true>(chosen[r], row.top, cb[r], cs[r]);
+        else affinity<MODE, false>(chosen[r], row.top, cb[r], cs[r]);
         if (id[r] == kNoId || row.wrong) cb[r] = cs[r] = 0.0f;
         sum += cb[r];
         back += dw[r] * cb[r];
@@ -360,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
       wave_lds_order();
 #pragma unroll
       for (uint32_t r = 0; r < kRoutes; ++r)
-        if (id[r] != kNoId) atomicAdd(mine + id[r], cs[r] * (scale * per * (dw[r] - mean)));
+        if (id[r] != kNoId) atomicAdd(mine + id[r], cs[r] * per * (scale * (dw[r] - mean)));
       wave_lds_order();
 #pragma unroll
       for (int q = 0; q < Q; ++q) {

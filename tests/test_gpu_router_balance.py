@@ -281,3 +281,37 @@ def test_a_bad_row_is_zeros_whatever_its_upstream(eng, mode):
     assert int(flag.item()) == 1
     assert torch.all(got[8] == 0) and torch.all(nan[8] == 0) and torch.all(nan[9].isnan())
     assert bool(torch.isfinite(got).all()) and want.shape == got.shape
+
+
+def test_affinities_far_below_the_normal_exponentials(eng):
+    """sqrt(softplus(s)) = e^(s/2) keeps its bits where e^s has none left
+    (s < -87): rows that launch_router_topk takes, and lower ones."""
+    import torch
+
+    from pih_amd.linear import router_backward, router_balance, router_topk
+
+    mode = abi.ROUTER_SQRT_SOFTPLUS
+    g = torch.Generator().manual_seed(71)
+    scores = torch.randn(96, 64, generator=g) * 3 - 95  # about -106 to -84
+    scores[64:] -= 60
+    assert float(scores.min()) > -172 and float(scores[:64].max()) > -90
+    scores[1], scores[2, 5] = -100.0, -20.0
+    dweights = torch.randn(96, 4, generator=g)
+    s = scores.cuda()
+    ids, _, flag = router_topk(s[:64].contiguous(), 4, mode)
+    assert int(flag.item()) == 0
+    ids = torch.cat((ids.cpu(), torch.topk(scores[64:], 4, dim=1).indices.to(torch.int32)))
+    loss, counts, mean, grad, bound = _ref(scores, ids, mode, 0.02, 1.0, dweights, 1.5)
+    i = ids.cuda()
+    gl, gc, gm, _ = router_balance(s, i, mode, 0.02, flag=flag)
+    got, _ = router_backward(s, i, gc, mode, 0.02, torch.ones(1, device="cuda"), dweights=dweights.cuda(),
+                             route_scale=1.5, flag=flag)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.equal(gc.cpu().long(), counts)
+    # an exponent of s / 2 log2 e is rounded twice: its affinity is off by |s| 2^-24
+    far = 172 * 2.0 ** -24
+    rel = 2.0 ** -19 + 2 * far + 324 * 2.0 ** -24
+    assert float(((gm.cpu().double() - mean).abs() / mean).max()) <= rel
+    assert abs(float(gl) - float(loss)) <= (rel + 64 * 2.0 ** -23) * float(loss)
+    # (slope, sum, selected sum and their products: four such factors at most)
+    assert float(((got.cpu().double() - grad).abs() / (bound * (1 + 4 * far * 2 ** 18))).max()) <= 1.0
