@@ -543,7 +543,9 @@ typedef struct pih_amd_router_balance_launch_v1 {
  * scores_grad f32 [T, E], the sum of both.  The counts and the selection are
  * constants of the differentiation.  A row with error bit 1 or 4 gets zeros,
  * a route with error bit 2 has no part in the row's sums; an id twice in a row
- * is two routes. */
+ * is two routes.  Where the affinities of a row's routes alone sum to 0 (bit 4 of
+ * launch_router_topk too), topk_weights_grad adds nothing to it and bit 4 is
+ * set. */
 typedef struct pih_amd_router_backward_launch_v1 {
   uint32_t struct_size, abi_version;
   uintptr_t scores_f32, topk_ids_u32, counts_u32, loss_grad_f32;

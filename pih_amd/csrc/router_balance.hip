@@ -27,7 +27,8 @@
 // (3.7 TB/s), where the 7 sums and the exponentials of a row take as long as its
 // bytes; 57 rows 6.6 us, one launch.
 //
-// Error bits: 1 non-finite score, 2 id >= E, 4 affinities that sum to 0.
+// Error bits: 1 non-finite score, 2 id >= E, 4 affinities that sum to 0 (with the
+// route weights' gradient also those of a row's routes).
 #include <algorithm>
 #include <type_traits>
 
@@ -375,7 +376,13 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
       }
       sum = row_sum<LANES>(sum);
       back = row_sum<LANES>(back);
-      const float per = sum > 0.0f ? 1.0f / sum : 0.0f, mean = back * per;
+      // (below the normal numbers 1 / sum could be infinite)
+      const bool none = sum < 0x1p-126f;
+      if (none && !row.wrong) {
+#pragma unroll
+        for (uint32_t r = 0; r < kRoutes; ++r) bad |= id[r] != kNoId ? 4u : 0u;
+      }
+      const float per = none ? 0.0f : 1.0f / sum, mean = back * per;
 #pragma unroll
       for (int q = 0; q < Q; ++q) *reinterpret_cast<v4f*>(mine + R::expert(4 * q)) = v4f{0.f, 0.f, 0.f, 0.f};
       wave_lds_order();

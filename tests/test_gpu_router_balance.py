@@ -315,3 +315,38 @@ def test_affinities_far_below_the_normal_exponentials(eng):
     assert abs(float(gl) - float(loss)) <= (rel + 64 * 2.0 ** -23) * float(loss)
     # (slope, sum, selected sum and their products: four such factors at most)
     assert float(((got.cpu().double() - grad).abs() / (bound * (1 + 4 * far * 2 ** 18))).max()) <= 1.0
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_routes_without_affinity_are_flagged(eng, mode):
+    """A row whose routes have affinities of 0 has no route weights (bit 4 of
+    launch_router_topk too, where a bias selects them): that part of its
+    gradient is zeros, the balance loss's stays."""
+    import torch
+
+    from pih_amd.linear import router_backward, router_balance, router_topk
+
+    scores, ids, dweights = _case(73, 30, 64, 4)
+    scores[7, :8] = -1e30
+    ids[7] = torch.tensor([0, 3, 5, 6], dtype=torch.int32)
+    s, i, dw = scores.cuda(), ids.cuda(), dweights.cuda()
+    one = torch.ones(1, device="cuda")
+    _, counts, _, flag = router_balance(s, i, mode, 0.02)
+    balance, _ = router_backward(s, i, counts, mode, 0.02, one, flag=flag)
+    assert int(flag.item()) == 0  # (the whole row has affinities)
+    both, flag = router_backward(s, i, counts, mode, 0.02, one, dweights=dw)
+    part, flag2 = router_backward(s, i, None, mode, 0.0, None, dweights=dw)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == int(flag2.item()) == 4
+    assert not part[7].any() and torch.equal(both[7], balance[7])
+    assert part[[6, 8]].any(1).all() and torch.isfinite(part).all()
+    if mode == abi.ROUTER_SQRT_SOFTPLUS:
+        bias = torch.zeros(64, device="cuda")
+        bias[:8] = 100.0
+        chosen, _, flag = router_topk(s[7:8].contiguous(), 4, mode, bias=bias)
+        assert int(flag.item()) == 4 and int(chosen.max()) < 8
+    # ids past the experts alone leave no route: bit 2, not 4
+    i[7] = 64
+    part, flag = router_backward(s, i, None, mode, 0.0, None, dweights=dw)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 2 and not part[7].any()
