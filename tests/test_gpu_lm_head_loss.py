@@ -378,3 +378,31 @@ def test_weights_past_4_gib(eng):
         err += ref.abs() * HALF_BF16 + 1e-37
         _within(gw[take], ref.cpu(), (err + 256 * U * (g.abs().T @ x.double().abs())).cpu(), f"dw from {first}")
     assert bool(torch.isfinite(gx).all())
+
+
+@pytest.mark.parametrize("hidden", [64, 72])
+def test_targets_beside_every_tile_s_edge(eng, hidden):
+    """Targets in the last and the first column of every 256-column tile, and
+    so on either side of wherever a piece of the vocabulary ends (a piece is
+    whole tiles; these sizes have more columns than one holds: (4/3) 2^26
+    elements, 81152 columns at 1100 rows).  64 bits on the GPU."""
+    import torch
+
+    from pih_amd.linear import lm_head_loss, lm_head_loss_backward
+
+    rows, vocab = 1100, 122859
+    x, w, target, up = [t.cuda() for t in _case(7, rows, vocab, hidden, masked=0.0)]
+    edges = torch.arange(256, vocab, 256, dtype=torch.int32, device="cuda")
+    target[:2 * len(edges)] = torch.stack((edges - 1, edges), 1).reshape(-1)
+    target[-1] = vocab - 1
+    _, e, lse, elog, loss, eloss, _, _ = _ref(x, w, target)
+    got, glse, _ = lm_head_loss(x, w, target)
+    _within(glse, lse.cpu(), elog.cpu(), "lse")
+    _within(got, loss.cpu(), eloss.cpu(), "loss")
+    del e
+    gx, gw, flag = lm_head_loss_backward(x, w, target, glse, up)
+    (dx, ex), (dw, ew) = _grads_ref(x, w, target, up, glse)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    _within(gx, dx.cpu(), ex.cpu(), "dx")
+    _within(gw, dw.cpu(), ew.cpu(), "dw")
