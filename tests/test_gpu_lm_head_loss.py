@@ -406,3 +406,67 @@ def test_targets_beside_every_tile_s_edge(eng, hidden):
     assert int(flag.item()) == 0
     _within(gx, dx.cpu(), ex.cpu(), "dx")
     _within(gw, dw.cpu(), ew.cpu(), "dw")
+
+
+# one piece of the vocabulary, and two whose sums of dx are added up
+@pytest.mark.parametrize("vocab", [5000, 30011])
+def test_input_gradient_in_two_launches(eng, vocab):
+    """dx of 4096 rows and the 4 behind them: a round of 256 tiles of 256 x
+    256, where one more row of tiles would cost a second round."""
+    import torch
+
+    from pih_amd.linear import lm_head_loss_backward
+
+    x, w, target, up = [t.cuda() for t in _case(11, 4100, vocab, 4096)]
+    lse = torch.logsumexp(x.double() @ w.double().T, 1).float()
+    gx, gw, flag = lm_head_loss_backward(x, w, target, lse, up)
+    (dx, ex), (dw, ew) = _grads_ref(x, w, target, up, lse)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.all(gx[target < 0] == 0)
+    _within(gx, dx.cpu(), ex.cpu(), "dx")
+    _within(gx[4090:], dx[4090:].cpu(), ex[4090:].cpu(), "dx around row 4096")
+    _within(gw, dw.cpu(), ew.cpu(), "dw")
+
+
+def test_input_gradient_of_weights_past_4_gib(eng):
+    """dx over 2^20 entries of 2112 where two thirds of every row's probability
+    lie past 2^32 bytes: 1009 different entries over and over up to there, 211
+    others behind it, each five of which point along one of the rows of x.
+
+    A term of dx is off as in _grads_ref, without up 2^-23 but for the target,
+    whose 1 is subtracted; the sum runs in 16 parts or more."""
+    import torch
+
+    from pih_amd.linear import lm_head_loss_backward
+
+    vocab, hidden, rows, kinds, late = 1 << 20, 2112, 5, 1009, 211
+    x, few, _, up = (t.cuda() for t in _case(101, rows, kinds, hidden))
+    g = torch.Generator(device="cuda").manual_seed(103)
+    along = x[torch.arange(late, device="cuda") % rows].float() * 0.004
+    along = (along + torch.randn(late, hidden, device="cuda", generator=g) * 0.002).to(torch.bfloat16)
+    first = (1 << 32) // (2 * hidden) + 1
+    every = torch.cat((few, along))
+    v = torch.arange(vocab, device="cuda")
+    kind = torch.where(v < first, v % kinds, kinds + v % late)
+    w = every[kind].contiguous()
+    target = torch.tensor([0, vocab - 1, first - 1, first, vocab - 300], dtype=torch.int32, device="cuda")
+    times = torch.bincount(kind, minlength=kinds + late).double()
+    logits, e, _, _, _, _, _, _ = _ref(x, every, kind[target.long()])
+    lse = torch.logsumexp(logits + times.log(), 1).float()
+    p = torch.exp(logits - lse.double()[:, None])
+    assert float((p * times)[:, kinds:].sum(1).min()) > 0.3
+    gx, none, flag = lm_head_loss_backward(x, w, target, lse, up, weight_gradient=False)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and none is None
+    u = up.double()[:, None]
+    of = every[kind[target.long()]].double()
+    ref = (u * p * times) @ every.double() - u * of
+    arg = (logits - lse.double()[:, None]).abs()
+    terms = u.abs() * p * (1 + 1.1 * e)
+    eg = u.abs() * p * (1.1 * e + (arg + 4) * U + 2.0 ** -21) + terms * (2 * U + HALF_BF16)
+    size = (terms * times) @ every.double().abs() + u.abs() * of.abs()
+    err = (eg * times) @ every.double().abs() + u.abs() * of.abs() * (3 * U + HALF_BF16) + size * (vocab / 16 + 64) * U
+    _within(gx, ref.cpu(), (err + (ref.abs() + err) * HALF_BF16 + 1e-37).cpu(), "dx")
+    # (what lies past 2^32 bytes is most of the value: the bound holds it apart)
+    lost = (u * (p * times)[:, kinds:]) @ along.double()
+    assert float((lost.abs() / err).max()) > 4
