@@ -824,6 +824,11 @@ uint32_t piece_columns(uint32_t rows, uint32_t vocab, uint32_t hidden) {
 
 // the tiles fed by DMA take 64-deep steps
 bool big_takes(uint32_t hidden) { return hidden % KB == 0; }
+// a row's pairs of the forward pass: one per column tile
+uint32_t stat_tiles(uint32_t vocab, uint32_t hidden) {
+  const uint32_t columns = big_takes(hidden) ? TB : TS;
+  return (vocab + columns - 1) / columns;
+}
 
 struct BackwardPlan {
   uint32_t piece, splits;
@@ -850,7 +855,7 @@ BackwardPlan backward_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
 
 uint64_t LmHeadLossWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   if (!shape_ok(rows, vocab, hidden)) return 0;
-  return padded((uint64_t)rows * ((vocab + TS - 1) / TS) * 8) + padded((uint64_t)rows * 4);
+  return padded((uint64_t)rows * stat_tiles(vocab, hidden) * 8) + padded((uint64_t)rows * 4);
 }
 
 uint64_t LmHeadLossBackwardWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden) {
@@ -876,7 +881,7 @@ St LaunchLmHeadLoss(const LmHeadLossArgs& a) {
   g.k = a.hidden;
   g.lda = g.ldb = a.hidden;
   g.target = a.target;
-  g.stat_tiles = (a.vocab + TS - 1) / TS;
+  g.stat_tiles = stat_tiles(a.vocab, a.hidden);
   g.stats = static_cast<float2*>(a.workspace);
   g.target_logit = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) +
                                             padded((uint64_t)a.rows * g.stat_tiles * 8));
@@ -892,7 +897,6 @@ St LaunchLmHeadLoss(const LmHeadLossArgs& a) {
     b.stats = g.stats;
     b.target_logit = g.target_logit;
     launch_big<false, false, kEpiStats>(b, a.stream);
-    g.stat_tiles = (a.vocab + TB - 1) / TB;
   } else {
     launch_gemm<kEpiStats>(g, a.stream);
   }

@@ -284,3 +284,14 @@ def test_sizes_within_32_bits_are_launched(recorded):
     for call in good:
         call()
     assert len(recorded.launched) == len(good)
+
+
+@pytest.mark.parametrize("rows,vocab,hidden", [(1, 1, 64), (33, 151936, 1024), (32768, 151936, 1024), (4096, 129281, 4096),
+                                               (17, 1000, 72), (4096, 129280, 1000)])
+def test_loss_workspace_is_what_is_written(rows, vocab, hidden):
+    """A pair of 4-byte words per row and tile, of 256 columns or (hidden no
+    multiple of 64) 64, and a word per row, each array in whole 256 bytes."""
+    tile = 64 if hidden % 64 else 256
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    assert _query(abi.WORKSPACE_LM_HEAD_LOSS, rows, vocab, hidden) == (
+        abi.OK, up(rows * ((vocab + tile - 1) // tile) * 8) + up(rows * 4))

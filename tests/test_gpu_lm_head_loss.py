@@ -470,3 +470,23 @@ def test_input_gradient_of_weights_past_4_gib(eng):
     # (what lies past 2^32 bytes is most of the value: the bound holds it apart)
     lost = (u * (p * times)[:, kinds:]) @ along.double()
     assert float((lost.abs() / err).max()) > 4
+
+
+@pytest.mark.parametrize("rows,vocab,hidden", [(33, 1000, 128), (300, 5000, 128), (1003, 8190, 64), (790, 20400, 128),
+                                               (70, 1000, 72)])
+def test_forward_stays_in_its_workspace(eng, rows, vocab, hidden):
+    import torch
+
+    from pih_amd import linear
+
+    x, w, target, _ = (t.cuda() for t in _case(111, rows, vocab, hidden))
+    want = linear.lm_head_loss(x, w, target)
+    need = linear._workspace_bytes(abi.WORKSPACE_LM_HEAD_LOSS, rows, vocab, hidden)
+    ws = torch.full((need + 65536,), 0x5A, dtype=torch.uint8, device="cuda")
+    loss, lse = (torch.empty(rows, dtype=torch.float32, device="cuda") for _ in range(2))
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    linear._launch("launch_lm_head_loss", "lm_head_loss", x.data_ptr(), w.data_ptr(), target.data_ptr(), loss.data_ptr(),
+                   lse.data_ptr(), ws.data_ptr(), need, flag.data_ptr(), linear.stream_handle(), rows, vocab, hidden)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.all(ws[need:] == 0x5A)
+    assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
