@@ -727,9 +727,10 @@ __global__ __launch_bounds__(1024) void loss_factor_kernel(const float* up, cons
   }
 }
 
-// up = factor 2^e m: m of every row, and 2^e x with zeros for the rows without
-// a target, [rows up to a multiple of 64].  Where up / factor is not a normal
-// number (0, NaN, or of no weight in dw) 2^e is that number and m is 1.
+// up = factor 2^e m: m of every row, and for dw's product 2^e x with zeros for
+// the rows without a target, [rows up to a multiple of 64] (out null: without
+// dw).  Where up / factor is not a normal number (0, NaN, or of no weight in dw)
+// 2^e is that number and m is 1.
 __global__ __launch_bounds__(256) void loss_live_rows_kernel(const uint16_t* x, const uint32_t* target,
                                                              const float* up, const float* factor, uint16_t* out,
                                                              float* mantissa, uint32_t* err, uint32_t rows,
@@ -749,6 +750,7 @@ __global__ __launch_bounds__(256) void loss_live_rows_kernel(const uint16_t* x, 
     if (row < rows) mantissa[row] = m;
     if (y >= vocab && y != kNoTarget) atomicOr(err, kErrTarget);
   }
+  if (!out) return;
   for (uint32_t c = threadIdx.x * 8; c < hidden; c += 2048) {
     v4i v{0, 0, 0, 0};
     if (y < vocab) {
@@ -929,7 +931,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
   hipLaunchKernelGGL(loss_factor_kernel, dim3(1), dim3(1024), 0, a.stream, a.loss_grad, a.target, factor, a.rows,
                      a.vocab);
   hipLaunchKernelGGL(loss_live_rows_kernel, dim3(row_up), dim3(256), 0, a.stream, a.x, a.target, a.loss_grad, factor,
-                     live, mantissa, a.error_flag, a.rows, a.vocab, a.hidden);
+                     a.dw ? live : nullptr, mantissa, a.error_flag, a.rows, a.vocab, a.hidden);
   for (uint32_t v0 = 0; v0 < a.vocab; v0 += plan.piece) {
     const uint32_t cols = std::min(plan.piece, a.vocab - v0);
     const uint16_t* const w = a.w + (uint64_t)v0 * a.hidden;

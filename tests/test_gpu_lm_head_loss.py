@@ -490,3 +490,29 @@ def test_forward_stays_in_its_workspace(eng, rows, vocab, hidden):
     torch.cuda.synchronize()
     assert int(flag.item()) == 0 and torch.all(ws[need:] == 0x5A)
     assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("rows,vocab,hidden", [(70, 300, 1024), (65, 500, 1000)])
+def test_a_frozen_head_leaves_the_copy_of_the_rows_out(eng, rows, vocab, hidden):
+    """Without dw the workspace's scaled copy of x, which only dw reads, is not
+    written (its bytes, of rows up to a multiple of 64, keep their pattern), and
+    dx has the bits that it has beside dw."""
+    import torch
+
+    from pih_amd import linear
+
+    x, w, target, up = (t.cuda() for t in _case(113, rows, vocab, hidden))
+    lse = torch.logsumexp(x.double() @ w.double().T, 1).float()
+    target[5] = -1
+    want = linear.lm_head_loss_backward(x, w, target, lse, up)[0]
+    need = linear._workspace_bytes(abi.WORKSPACE_LM_HEAD_LOSS_BACKWARD, rows, vocab, hidden)
+    ws = torch.full((need,), 0x5A, dtype=torch.uint8, device="cuda")
+    dx, flag = torch.empty_like(x), torch.zeros(1, dtype=torch.int32, device="cuda")
+    target[5] = vocab + 3
+    linear._launch("launch_lm_head_loss_backward", "lm_head_loss_backward", x.data_ptr(), w.data_ptr(), target.data_ptr(),
+                   lse.data_ptr(), up.data_ptr(), dx.data_ptr(), 0, ws.data_ptr(), need, flag.data_ptr(),
+                   linear.stream_handle(), rows, vocab, hidden)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 1  # (a bad target is reported as ever)
+    assert int((ws == 0x5A).sum()) >= (rows + 63) // 64 * 64 * hidden * 2
+    assert torch.equal(dx, want)
