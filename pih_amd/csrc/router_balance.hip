@@ -219,8 +219,8 @@ __global__ __launch_bounds__(64 * kBalanceWaves) void router_balance_kernel(cons
   using R = Row<MODE, LANES, Q>;
   constexpr uint32_t kRows = 64 / LANES, kAll = LANES * R::N;  // rows of a wave, experts held
   constexpr uint32_t kParts = kBalanceWaves * kRows;
-  constexpr uint32_t kFold = kParts * kAll > 16384 ? 16384 / kAll : kParts;  // partial sums in LDS at a time
-  __shared__ float sums[kFold][kAll];
+  static_assert(kParts * kAll <= 16384, "64 KB of partial sums");
+  __shared__ float sums[kParts][kAll];
   __shared__ uint32_t counts[kAll];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, part = wave * kRows + lane / LANES;
   for (uint32_t e = tid; e < kAll; e += 64 * kBalanceWaves) counts[e] = 0;
@@ -243,18 +243,13 @@ __global__ __launch_bounds__(64 * kBalanceWaves) void router_balance_kernel(cons
 #pragma unroll
     for (int j = 0; j < R::N; ++j) acc[j] += row.b[j] * inv;
   }
-  // kFold parts at a time, each time added up by expert
+  // the parts' sums, added up by expert
   float total = 0.0f;
-  for (uint32_t p0 = 0; p0 < kParts; p0 += kFold) {
-    __syncthreads();
-    if (part >= p0 && part < p0 + kFold) {
 #pragma unroll
-      for (int j = 0; j < R::N; ++j) sums[part - p0][R::expert(j)] = acc[j];
-    }
-    __syncthreads();
-    if (tid < experts)
-      for (uint32_t i = 0; i < kFold; ++i) total += sums[i][tid];
-  }
+  for (int j = 0; j < R::N; ++j) sums[part][R::expert(j)] = acc[j];
+  __syncthreads();
+  if (tid < experts)
+    for (uint32_t i = 0; i < kParts; ++i) total += sums[i][tid];
   if (bad) atomicOr(err, bad);
   if (gridDim.x == 1) {
     float term = 0.0f;
