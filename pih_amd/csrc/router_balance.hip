@@ -62,9 +62,7 @@ __device__ __forceinline__ float log1p01(float e) {
 
 // b(s) and its derivative.  2^(s log2 e) by the hardware exponential: off by
 // 2^-23 of itself and |s| 2^-24 from the exponent's rounding.
-// kFar: for scores below -80 too.
-constexpr float kFarScore = -80.0f;
-template <int MODE, bool kFar>
+template <int MODE>
 __device__ __forceinline__ void affinity(float s, float top, float& b, float& slope) {
   if constexpr (MODE == kRouterSoftmax) {
     b = __builtin_amdgcn_exp2f((s - top) * kLog2e);
@@ -76,14 +74,15 @@ __device__ __forceinline__ void affinity(float s, float top, float& b, float& sl
     b = __builtin_amdgcn_sqrtf(sp);
     // sigmoid / softplus tends to 1 where both underflow
     slope = sp > 1e-30f ? 0.5f * sig * __builtin_amdgcn_rcpf(b) : 0.5f * b;
-    if constexpr (kFar) {
-      // e^s leaves the normal numbers at -87, its root e^(s/2), which is b there
-      // (to 2^-117 of itself below -80), at -174
-      const float x = 0.5f * kLog2e * s, far = x >= -126.0f ? __builtin_amdgcn_exp2f(x) : 0.0f;
-      b = s < kFarScore ? far : b;
-      slope = s < kFarScore ? 0.5f * far : slope;
-    }
   }
+}
+// The same for sqrt(softplus) of a score below -80: e^s leaves the normal
+// numbers at -87, its root e^(s/2), which b is there to 2^-117 of itself, at -174.
+constexpr float kFarScore = -80.0f;
+__device__ __forceinline__ void far_affinity(float s, float& b, float& slope) {
+  const float x = 0.5f * kLog2e * s;
+  b = x >= -126.0f ? __builtin_amdgcn_exp2f(x) : 0.0f;
+  slope = 0.5f * b;
 }
 
 // the sum or maximum over a row's lanes, in every one of them
@@ -119,7 +118,9 @@ struct Row {
   static constexpr int N = 4 * Q;
   float b[N], slope[N], top, sum;
   uint32_t wrong;
-  bool far;  // some row of the wave has far scores
+  bool far;  // some row of the wave has scores below kFarScore
+  // scores outside the row
+  static constexpr float kOutside = MODE == kRouterSoftmax ? -INFINITY : 0.0f;
 
   static __device__ __forceinline__ uint32_t expert(int j) {
     return 4 * (LANES * (j / 4) + (threadIdx.x & (LANES - 1))) + j % 4;
@@ -130,52 +131,57 @@ struct Row {
     for (int q = 0; q < Q; ++q) {
       const uint32_t e = expert(4 * q);
       if (vec) {
-        v4f v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        v4f v{kOutside, kOutside, kOutside, kOutside};
         if (e < experts) v = *reinterpret_cast<const v4f*>(s + e);
 #pragma unroll
         for (int c = 0; c < 4; ++c) slope[4 * q + c] = v[c];
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) slope[4 * q + c] = e + c < experts ? s[e + c] : -INFINITY;
+        for (int c = 0; c < 4; ++c) slope[4 * q + c] = e + c < experts ? s[e + c] : kOutside;
       }
     }
   }
-  // the affinities, their derivatives and sum; what is wrong with the row
-  // (then the sum is 1 and every affinity 0)
-  __device__ __forceinline__ void work(uint32_t experts) {
-    float bad = 0.0f;
+  // the affinities, their derivatives and sum of the row s; what is wrong with
+  // it (then the sum is 1 and every affinity 0)
+  __device__ __forceinline__ void work(const float* s, uint32_t experts) {
+    float bad = 0.0f, least = 0.0f;
     top = 0.0f;
     if constexpr (MODE == kRouterSoftmax) {
       top = slope[0];
 #pragma unroll
       for (int j = 1; j < N; ++j) top = fmaxf(top, slope[j]);
       top = row_max<LANES>(top);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) least = fminf(least, slope[j]);
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       // 0 for a finite score, else NaN
       const float nan = slope[j] * 0.0f;
-      bad += expert(j) < experts ? nan : 0.0f;
+      bad += kOutside == 0.0f || expert(j) < experts ? nan : 0.0f;
     }
     sum = 0.0f;
-    auto all = [&](auto FAR) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float s = slope[j];
-        affinity<MODE, decltype(FAR)::value>(s, top, b[j], slope[j]);
-        // (outside the row: -inf, whose derivative is a NaN)
-        if (expert(j) >= experts) b[j] = slope[j] = 0.0f;
-        sum += b[j];
-      }
-    };
-    float least = 0.0f;
-    if constexpr (MODE == kRouterSqrtSoftplus) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) least = fminf(least, expert(j) < experts ? slope[j] : 0.0f);
+    for (int j = 0; j < N; ++j) {
+      const float score = slope[j];
+      affinity<MODE>(score, top, b[j], slope[j]);
+      // (outside the row; of -inf the derivative is a NaN)
+      if (expert(j) >= experts) b[j] = slope[j] = 0.0f;
+      sum += b[j];
     }
     far = MODE == kRouterSqrtSoftplus && __builtin_amdgcn_ballot_w64(least < kFarScore);
-    if (far) all(std::true_type{});
-    else all(std::false_type{});
+    if (far) {
+      // (rare: the scores again, one at a time, for registers of no more)
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float score = expert(j) < experts ? s[expert(j)] : 0.0f;
+        if (score < kFarScore) far_affinity(score, b[j], slope[j]);
+        sum += b[j];
+        asm volatile("" ::: "memory");
+      }
+    }
     sum = row_sum<LANES>(sum);
     wrong = row_sum<LANES>(bad) == 0.0f ? (sum == 0.0f ? 4u : 0u) : 1u;
     if (wrong) {
@@ -237,7 +243,7 @@ __global__ __launch_bounds__(64 * kBalanceWaves) void router_balance_kernel(cons
       if (id < experts) atomicAdd(&counts[id], 1u);
       else bad |= 2u;
     }
-    row.work(experts);
+    row.work(scores + (uint64_t)t * experts, experts);
     bad |= row.wrong;
     const float inv = 1.0f / row.sum;
 #pragma unroll
@@ -349,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
       for (uint32_t k = i; k < topk; k += LANES)
         if (ids[(uint64_t)t * topk + k] >= experts) bad |= 2u;
     }
-    row.work(experts);
+    row.work(s, experts);
     bad |= row.wrong;
     const float inv = 1.0f / row.sum;
     float dot = 0.0f;
@@ -363,8 +369,8 @@ __global__ __launch_bounds__(64 * kWaves) void router_backward_kernel(
       float cb[kRoutes], cs[kRoutes], sum = 0.0f, back = 0.0f;
 #pragma unroll
       for (uint32_t r = 0; r < kRoutes; ++r) {
-        if (row.far) affinity<MODE, true>(chosen[r], row.top, cb[r], cs[r]);
-        else affinity<MODE, false>(chosen[r], row.top, cb[r], cs[r]);
+        affinity<MODE>(chosen[r], row.top, cb[r], cs[r]);
+        if (row.far && chosen[r] < kFarScore) far_affinity(chosen[r], cb[r], cs[r]);
         if (id[r] == kNoId || row.wrong) cb[r] = cs[r] = 0.0f;
         sum += cb[r];
         back += dw[r] * cb[r];
