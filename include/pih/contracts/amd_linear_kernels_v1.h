@@ -500,7 +500,8 @@ typedef struct pih_amd_lm_head_loss_launch_v1 {
  * holds the mantissa alone (powers of two and the rows' largest factor enter
  * in fp32 or exactly), so equal factors such as a mean's 1 / rows are not
  * rounded.  A row without a target gives zeros, whatever its input, lse and
- * loss_grad hold.  The results lie outside every input.  Conditions are those of
+ * loss_grad hold; an infinite loss_grad of another makes weight_grad NaN, also
+ * where the formula gives an infinity.  The results lie outside every input.  Conditions are those of
  * pih_amd_lm_head_loss_launch_v1; workspace:
  * query_workspace(LM_HEAD_LOSS_BACKWARD, rows, vocab, hidden).
  * Error bit 1 as above. */

@@ -13,21 +13,24 @@
 // its two readers; 4096 columns or so, which is more, above 16384 rows), then dw of the piece is g^T x, and dx
 // grows by g W_piece in fp32.
 //
-// g is rounded to bf16 for the matrix cores: 2^-9 of each element at most,
-// independent from element to element, in sums that are rounded to bf16 once
-// themselves.  Of the upstream factors up_t = s 2^e m, with s the largest and
+// g is rounded to bf16 for the matrix cores, which costs half the MFMAs of two
+// parts: 2^-8 of each element at most, independent from element to element, in
+// sums that are rounded to bf16 once themselves (4096 rows over 129280 x 4096:
+// dx and dw 0.20 % of their norm off 64 bits, 0.17 % of it their own rounding).
+// Of the upstream factors up_t = s 2^e m, with s the largest and
 // 1 <= |m| < 2, g holds m alone; 2^e goes into the x of dw's product, exactly,
 // s into dw in fp32, and up_t / m into dx in fp32.  So a mean's equal factors
 // (1 / rows, whose rounding would be the same error in every element) are
-// exact.  (All of up_t rounded inside g: dx and dw off by 0.34 % of their norm,
-// 0.17 % of it bf16 results' own.)
+// exact (all of up_t rounded inside g: 0.34 %).
 //
 // Measured: 4096 rows, 129280 x 4096 3.12-3.28 ms (1.32-1.39 PFLOP/s; a library
 // product of that shape alone 3.25 ms) and 9.7-10.1 ms for the gradients, bound
 // by the matrix pipe, 68 % busy, and the power it takes (1.9 GHz); 33 rows, 151936
-// x 1024 67 us, of which the weights' 311 MB take 61 at 5.1 TB/s; the gradients
+// x 1024 64.5 us, of which the weights' 311 MB take 61 at 5.1 TB/s; the gradients
 // of 1021 rows there 0.99 ms (0.96 PFLOP/s: of a 256 x 256 tile's 32 us 9 are the
-// exponentials and the stores).
+// exponentials and the stores).  dx alone, for a frozen head: 33 rows 148 us over
+// 151936 x 1024 and 373 over 129280 x 4096 (the weights twice from HBM), 4096 rows
+// 6.6 ms over 129280 x 4096 (1.32 PFLOP/s).
 //
 // Rows without a target take no part in the gradients: their g is 0, and the
 // x of dw's product is a copy with those rows as zeros, so that nothing an
@@ -283,8 +286,11 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
           if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
         }
       }
-      // (few rows: the weights are read once, past the caches.  dx of 33 rows
-      // over 151936 x 1024 92 -> 72 us, the loss of 128 rows 84 -> 79)
+      // (few rows: the weights past the caches.  Of one row tile they are read
+      // once: dx of 33 rows over 151936 x 1024 92 -> 72 us, the loss of 128 rows
+      // 84 -> 79.  With two or three row tiles it still gains: the loss of 300
+      // rows 150 -> 135 there, 435 -> 392 over 129280 x 4096, of 200 rows over
+      // 32768 x 1024 26 -> 25; the other way dx of 128 rows there, 60 -> 67)
       if constexpr (ROWS <= 128) dma16nt(sb, ob, lds + S::kA + i * 4096);
       else dma16(sb, ob, lds + S::kA + i * 4096);
     }

@@ -22,10 +22,10 @@
 // are integer adds, whose order does not show.  The route weights' part of the
 // gradient is added up per row in LDS, since its places are any experts.
 //
-// Measured at 256 experts: 32768 rows (34 MB) 13.5 us for the loss's pass and 5 for
+// Measured at 256 experts: 32768 rows (34 MB) 12.7 us for the loss's pass and 5 for
 // the block that finishes it, 18 us for the gradient with the route weights'
 // (3.7 TB/s), where the 7 sums and the exponentials of a row take as long as its
-// bytes; 57 rows 6.6 us, one launch.
+// bytes; 57 rows 6.5 us, one launch.
 //
 // Error bits: 1 non-finite score, 2 id >= E, 4 affinities that sum to 0 (with the
 // route weights' gradient also those of a row's routes).

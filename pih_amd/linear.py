@@ -572,7 +572,8 @@ def adapter_gemm(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: Optio
     adapters[s]`` (-1: none).  ``x`` [rows, k], ``base`` and ``out``
     [rows, n] may be column slices of wider tensors; ``out`` may be ``base``
     itself; ``base`` None starts from zero.  Rows outside every segment are
-    left as they are.  Returns (out, flag)."""
+    left as they are (in a new ``out`` they hold anything).  Returns (out,
+    flag)."""
     count, rank, n, k = _adapter_stacks(a, b, scale, offsets, adapters)
     rows = x.shape[0]
     px, xs = _rows(x, rows, k, "the adapters' input")
@@ -606,7 +607,8 @@ def adapter_backward(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torc
     n] (``launch_adapter_backward``): (dx bf16 [rows, k], da f32 like ``a``,
     db f32 like ``b``, flag).  ``base`` is the shared projection's gradient of
     x, on top of which dx comes (``out`` may be ``base`` itself).  Segments
-    that share an adapter add up; an adapter without rows has zeros."""
+    that share an adapter add up; an adapter without rows has zeros.  Rows of
+    dx outside every segment are left as they are, as in ``adapter_gemm``."""
     count, rank, n, k = _adapter_stacks(a, b, scale, offsets, adapters)
     rows = x.shape[0]
     pdy, ys = _rows(dy, rows, n, "the upstream gradient")
