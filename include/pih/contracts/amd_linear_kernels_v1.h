@@ -78,7 +78,15 @@
  *                          output, the LM head's softmax cross entropy, the
  *                          router's balance loss and the gradients of all
  *                          three (no reference counterpart: the reference
- *                          serves one set of weights and does not train).
+ *                          serves one set of weights and does not train);
+ *   launch_gated_mlp, launch_gated_mlp_backward,
+ *   launch_lm_head_distill, launch_lm_head_distill_backward,
+ *   launch_draft_verify
+ *                          the gated feed-forward block and an LM head's
+ *                          divergence from a teacher's top logits with their
+ *                          gradients, and the verification of drafted tokens:
+ *                          a draft model's training and its use (no reference
+ *                          counterpart: it decodes one token at a time).
  *
  * Conventions are those of the reference's pack tables: one request pointer
  * in, pih_status_v1 by value out; a NULL request, wrong struct_size or wrong
@@ -127,6 +135,11 @@ extern "C" {
 #define PIH_AMD_WORKSPACE_LM_HEAD_LOSS_V1 5U
 #define PIH_AMD_WORKSPACE_LM_HEAD_LOSS_BACKWARD_V1 6U
 #define PIH_AMD_WORKSPACE_ROUTER_BALANCE_V1 7U
+#define PIH_AMD_WORKSPACE_GATED_MLP_V1 8U
+#define PIH_AMD_WORKSPACE_GATED_MLP_BACKWARD_V1 9U
+#define PIH_AMD_WORKSPACE_LM_HEAD_DISTILL_V1 10U
+#define PIH_AMD_WORKSPACE_LM_HEAD_DISTILL_BACKWARD_V1 11U
+#define PIH_AMD_WORKSPACE_DRAFT_VERIFY_V1 12U
 
 /* Scratch size query (host only; touches no device). */
 typedef struct pih_amd_workspace_query_v1 {
@@ -556,6 +569,152 @@ typedef struct pih_amd_router_backward_launch_v1 {
   float coefficient, route_scale;
 } pih_amd_router_backward_launch_v1;
 
+/* The gated feed-forward block of a layer, with L = limit (<= 0: no clamp):
+ *   gate = input . gate_weight^T, up = input . up_weight^T   [rows][intermediate]
+ *   h    = silu(min(gate, L)) * min(max(up, -L), L)
+ *   output = h . down_weight^T                               [rows][hidden]
+ * input, output bf16 [rows][hidden]; gate_weight, up_weight bf16
+ * [intermediate][hidden] (the halves of a fused weight will do), down_weight
+ * bf16 [hidden][intermediate].  gate and up bf16 [rows][intermediate], before
+ * the clamp, are what the backward pass needs: both or neither (0).  The
+ * activation takes gate and up from their fp32 sums; h is rounded to bf16 once
+ * and summed in fp32.  The results lie outside every input.  hidden and
+ * intermediate multiples of 8 up to 2^17, rows up to 2^20, limit finite, addresses
+ * 16-byte aligned.  workspace: query_workspace(GATED_MLP, rows, intermediate,
+ * hidden). */
+typedef struct pih_amd_gated_mlp_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t input_bf16, gate_weight_bf16, up_weight_bf16, down_weight_bf16;
+  uintptr_t output_bf16, gate_bf16, up_bf16, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t stream;
+  uint32_t rows, hidden, intermediate;
+  float limit;
+} pih_amd_gated_mlp_launch_v1;
+
+/* Gradients of the above for an upstream gradient of the output, with gate
+ * and up as launch_gated_mlp wrote them:
+ *   dh = output_grad . down_weight
+ *   dup   = dh * silu(min(gate, L))              (0 where |up| > L)
+ *   dgate = dh * clamped up * silu'(gate)        (0 where gate > L)
+ *   input_grad       = dgate . gate_weight + dup . up_weight
+ *   gate_weight_grad = dgate^T . input, up_weight_grad = dup^T . input
+ *   down_weight_grad = output_grad^T . h
+ * all bf16, shaped like what they belong to; any of the four may be left out
+ * (0), not all.  dh is not rounded; dgate, dup and h are rounded to bf16 once
+ * for the products behind them, which sum in fp32.  Sums run in a fixed order:
+ * the same call gives the same bits.  The results lie outside every input and
+ * one another.  Conditions are those of pih_amd_gated_mlp_launch_v1; workspace:
+ * query_workspace(GATED_MLP_BACKWARD, rows, intermediate, hidden). */
+typedef struct pih_amd_gated_mlp_backward_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t output_grad_bf16, input_bf16, gate_weight_bf16, up_weight_bf16, down_weight_bf16;
+  uintptr_t gate_bf16, up_bf16;
+  uintptr_t input_grad_bf16, gate_weight_grad_bf16, up_weight_grad_bf16, down_weight_grad_bf16;
+  uintptr_t workspace;
+  uint64_t workspace_bytes;
+  uintptr_t stream;
+  uint32_t rows, hidden, intermediate;
+  float limit;
+} pih_amd_gated_mlp_backward_launch_v1;
+
+/* Divergence of an LM head from a teacher's top logits, without the head's own
+ * logits in memory.  With z[t, v] = input[t, :] . weight[v, :], T = temperature
+ * and the teacher's entries k of a row, (id, s) in teacher_ids u32 and
+ * teacher_logits f32 [rows][top_k]:
+ *   lse[t]  = log(sum over v of exp(z[t, v] / T))
+ *   q[t, k] = exp(s / T) / sum over the row's entries of exp(s / T), or where
+ *             teacher_lse f32 [rows] is given exp(s / T - teacher_lse[t])
+ *             (the log-sum-exp of ALL the teacher's logits over T)
+ *   loss[t] = T^2 * sum over k of q * (log(q) - z[t, id] / T + lse[t])
+ * logits f32 [rows][top_k] takes z[t, id] (0 for an entry that is not there).
+ * An id of 0xFFFFFFFF is no entry, a teacher logit of -infinity one of
+ * probability 0, which adds nothing; a row without any other has loss 0.  An
+ * id twice in a row is two entries.  Logits, maxima and sums are fp32.
+ * input bf16 [rows][hidden], weight bf16 [vocab][hidden].  hidden a multiple of
+ * 8, rows, vocab and hidden up to 2^20, top_k up to 256, temperature positive
+ * and finite, addresses 16-byte aligned (the u32 and f32 arrays 4-byte).
+ * workspace: query_workspace(LM_HEAD_DISTILL, rows, vocab, hidden).
+ * Error bits: 1 an id that is neither 0xFFFFFFFF nor below vocab (no entry),
+ * 4 a non-finite loss (stored). */
+#define PIH_AMD_NO_TEACHER_ENTRY_V1 0xFFFFFFFFU
+typedef struct pih_amd_lm_head_distill_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t input_bf16, weight_bf16, teacher_ids_u32, teacher_logits_f32, teacher_lse_f32;
+  uintptr_t loss_f32, lse_f32, logits_f32, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t rows, vocab, hidden, top_k;
+  float temperature;
+} pih_amd_lm_head_distill_launch_v1;
+
+/* Gradients of the above from lse and logits (as launch_lm_head_distill wrote
+ * them) and the losses' upstream gradient f32 [rows]: with Q[t] the sum of the
+ * row's q
+ *   g[t, v] = loss_grad[t] * T * (Q[t] * exp(z[t, v] / T - lse[t])
+ *                                 - sum of q[t, k] over the entries with id v)
+ *   input_grad  bf16 [rows][hidden]  = g . weight
+ *   weight_grad bf16 [vocab][hidden] = g^T . input   (address 0: left out)
+ * summed in fp32, g as pih_amd_lm_head_loss_backward_launch_v1 takes it: its
+ * upstream factor's powers of two and the rows' largest one enter in fp32 or
+ * exactly.  A row without entries of a probability above 0 gives zeros,
+ * whatever its input, lse and loss_grad hold.  The results lie outside every
+ * input.  workspace: query_workspace(LM_HEAD_DISTILL_BACKWARD, rows, vocab,
+ * hidden).  Conditions and error bit 1 are those of
+ * pih_amd_lm_head_distill_launch_v1. */
+typedef struct pih_amd_lm_head_distill_backward_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t input_bf16, weight_bf16, teacher_ids_u32, teacher_logits_f32, teacher_lse_f32;
+  uintptr_t lse_f32, logits_f32, loss_grad_f32, input_grad_bf16, weight_grad_bf16, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t rows, vocab, hidden, top_k;
+  float temperature;
+} pih_amd_lm_head_distill_backward_launch_v1;
+
+/* Drafted tokens of many sequences verified against the target model's logits.
+ * Sequence s has n = draft_offsets[s + 1] - draft_offsets[s] drafted tokens
+ * d[0..n), entries draft_offsets[s] .. of draft_tokens u32 [draft_count] and
+ * accept_random f32 [draft_count], rows of the draft model's logits
+ * [draft_count][vocab] (0: the drafts were looked up, not drawn), and n + 1
+ * rows from draft_offsets[s] + s on of the target's logits [draft_count +
+ * sequence_count][vocab].  Logits are f32 or bf16 (logits_type
+ * PIH_AMD_OUTPUT_*), their rows *_stride elements apart.  With T =
+ * temperature[s] (f32; address 0: all 1) and p, q the softmax of a target and a
+ * draft row over T (q all at d[i] for looked-up drafts):
+ *   token i is accepted while accept_random[i] * q(d[i]) < p(d[i]), as far as
+ *     the first that is not;
+ *   the token behind the accepted ones is the smallest v whose sum of w up to
+ *     and with v passes sample_random[s] times the sum of all w, w = max(0, p -
+ *     q) at the rejected place (p where that is 0 throughout), p behind n
+ *     accepted tokens.
+ * T = 0: greedy, token i is accepted if it is the target row's first largest
+ * logit, which else takes its place.  tokens u32 [sequence_count][max_drafts
+ * + 1] holds the accepted tokens, the one behind them and 0xFFFFFFFF from
+ * there on, accepted u32 [sequence_count] their count.  Probabilities and sums
+ * are 64-bit.  Logits of -infinity have probability 0.
+ * draft_count may be 0 (its arrays are then not read); up to 2^20, sequences up
+ * to 2^14, at least 1; max_drafts up to 255, vocab up to 2^20, and sequences *
+ * (2 max_drafts + 1) * vocab / 4096 (rounded up) below 2^24.  Addresses are
+ * aligned to their elements, the results outside every input, workspace 16-byte:
+ * query_workspace(DRAFT_VERIFY, sequence_count, max_drafts, vocab).
+ * Error bits: 1 a drafted token that is reached and not below vocab (rejected,
+ * as of probability 0); 2 offsets that descend, pass draft_count or leave more
+ * than max_drafts for a sequence (it accepts 0 and has no token); 4 a row that
+ * is reached and whose probabilities do not exist (a NaN, +infinity but for the
+ * greedy, or no logit above -infinity), or a temperature that is negative, NaN
+ * or infinite: nothing from that place on is accepted and no token follows. */
+typedef struct pih_amd_draft_verify_launch_v1 {
+  uint32_t struct_size, abi_version;
+  uintptr_t target_logits, draft_logits, draft_tokens_u32, draft_offsets_u32;
+  uintptr_t accept_random_f32, sample_random_f32, temperature_f32;
+  uintptr_t tokens_u32, accepted_u32, workspace;
+  uint64_t workspace_bytes;
+  uintptr_t error_flag_u32, stream;
+  uint32_t sequence_count, draft_count, max_drafts, vocab;
+  uint32_t target_stride, draft_stride, logits_type;
+} pih_amd_draft_verify_launch_v1;
+
 typedef struct pih_amd_linear_kernels_api_v1 {
   uint32_t struct_size;
   uint32_t contract_version;
@@ -607,6 +766,13 @@ typedef struct pih_amd_linear_kernels_api_v1 {
   pih_status_v1 (*launch_lm_head_loss_backward)(const pih_amd_lm_head_loss_backward_launch_v1*);
   pih_status_v1 (*launch_router_balance)(const pih_amd_router_balance_launch_v1*);
   pih_status_v1 (*launch_router_backward)(const pih_amd_router_backward_launch_v1*);
+  /* The feed-forward block, distillation and draft verification (the five
+   * structs above; no counterpart in the reference). */
+  pih_status_v1 (*launch_gated_mlp)(const pih_amd_gated_mlp_launch_v1*);
+  pih_status_v1 (*launch_gated_mlp_backward)(const pih_amd_gated_mlp_backward_launch_v1*);
+  pih_status_v1 (*launch_lm_head_distill)(const pih_amd_lm_head_distill_launch_v1*);
+  pih_status_v1 (*launch_lm_head_distill_backward)(const pih_amd_lm_head_distill_backward_launch_v1*);
+  pih_status_v1 (*launch_draft_verify)(const pih_amd_draft_verify_launch_v1*);
 } pih_amd_linear_kernels_api_v1;
 
 #define PIH_AMD_ROUTE_PLAN_NOALLOC_MAX_SCRATCH_V1 (1ULL << 20)

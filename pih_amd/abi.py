@@ -265,7 +265,27 @@ LN["router_backward"] = _struct("RouterBackward", _hdr(
     *_u("scores_f32", "topk_ids_u32", "counts_u32", "loss_grad_f32", "topk_weights_grad_f32", "scores_grad_f32",
         "error_flag_u32", "stream"), *_i("token_count", "expert_count", "top_k", "mode"), ("coefficient", F32),
     ("route_scale", F32)))
-NO_ADAPTER = NO_TARGET = 0xFFFFFFFF
+LN["gated_mlp"] = _struct("GatedMlp", _hdr(
+    *_u("input_bf16", "gate_weight_bf16", "up_weight_bf16", "down_weight_bf16", "output_bf16", "gate_bf16", "up_bf16",
+        "workspace"), ("workspace_bytes", U64), *_u("stream"), *_i("rows", "hidden", "intermediate"), ("limit", F32)))
+LN["gated_mlp_backward"] = _struct("GatedMlpBackward", _hdr(
+    *_u("output_grad_bf16", "input_bf16", "gate_weight_bf16", "up_weight_bf16", "down_weight_bf16", "gate_bf16",
+        "up_bf16", "input_grad_bf16", "gate_weight_grad_bf16", "up_weight_grad_bf16", "down_weight_grad_bf16",
+        "workspace"), ("workspace_bytes", U64), *_u("stream"), *_i("rows", "hidden", "intermediate"), ("limit", F32)))
+LN["lm_head_distill"] = _struct("LmHeadDistill", _hdr(
+    *_u("input_bf16", "weight_bf16", "teacher_ids_u32", "teacher_logits_f32", "teacher_lse_f32", "loss_f32", "lse_f32",
+        "logits_f32", "workspace"), ("workspace_bytes", U64), *_u("error_flag_u32", "stream"),
+    *_i("rows", "vocab", "hidden", "top_k"), ("temperature", F32)))
+LN["lm_head_distill_backward"] = _struct("LmHeadDistillBackward", _hdr(
+    *_u("input_bf16", "weight_bf16", "teacher_ids_u32", "teacher_logits_f32", "teacher_lse_f32", "lse_f32",
+        "logits_f32", "loss_grad_f32", "input_grad_bf16", "weight_grad_bf16", "workspace"), ("workspace_bytes", U64),
+    *_u("error_flag_u32", "stream"), *_i("rows", "vocab", "hidden", "top_k"), ("temperature", F32)))
+LN["draft_verify"] = _struct("DraftVerify", _hdr(
+    *_u("target_logits", "draft_logits", "draft_tokens_u32", "draft_offsets_u32", "accept_random_f32",
+        "sample_random_f32", "temperature_f32", "tokens_u32", "accepted_u32", "workspace"), ("workspace_bytes", U64),
+    *_u("error_flag_u32", "stream"), *_i("sequence_count", "draft_count", "max_drafts", "vocab", "target_stride",
+                                         "draft_stride", "logits_type")))
+NO_ADAPTER = NO_TARGET = NO_TEACHER_ENTRY = 0xFFFFFFFF
 WEIGHT_FP8, WEIGHT_MXFP4 = 1, 2
 # pih_amd_w4a16_problem_v1: one entry of the grouped launch's host array
 W4A16_PROBLEM = _struct("W4a16Problem", _u("input_bf16", "qweight", "scales", "zeros", "output_bf16") +
@@ -284,7 +304,10 @@ LN_ORDER = [("query_workspace", "workspace_query"), ("launch_route_plan", "route
             ("launch_adapter_gemm", "adapter_gemm"), ("query_adapter_backward_workspace", "adapter_backward"),
             ("launch_adapter_backward", "adapter_backward"),
             ("launch_lm_head_loss", "lm_head_loss"), ("launch_lm_head_loss_backward", "lm_head_loss_backward"),
-            ("launch_router_balance", "router_balance"), ("launch_router_backward", "router_backward")]
+            ("launch_router_balance", "router_balance"), ("launch_router_backward", "router_backward"),
+            ("launch_gated_mlp", "gated_mlp"), ("launch_gated_mlp_backward", "gated_mlp_backward"),
+            ("launch_lm_head_distill", "lm_head_distill"),
+            ("launch_lm_head_distill_backward", "lm_head_distill_backward"), ("launch_draft_verify", "draft_verify")]
 LN_API = _struct("AmdLinearKernelsApi", [("struct_size", U32), ("contract_version", U32),
                                          ("identity", C.POINTER(Identity))] +
                  [(f, C.CFUNCTYPE(Status, C.POINTER(LN[s]))) for f, s in LN_ORDER])
@@ -352,6 +375,8 @@ ACTIVATION_E4M3, ACTIVATION_BF16 = 1, 2
 W4A16_SYMMETRIC, W4A16_ASYMMETRIC = 1, 2
 WORKSPACE_ROUTE_PLAN, WORKSPACE_BF16_GEMM, WORKSPACE_W4A16 = 1, 2, 3
 WORKSPACE_ADAPTER_GEMM, WORKSPACE_LM_HEAD_LOSS, WORKSPACE_LM_HEAD_LOSS_BACKWARD, WORKSPACE_ROUTER_BALANCE = 4, 5, 6, 7
+WORKSPACE_GATED_MLP, WORKSPACE_GATED_MLP_BACKWARD = 8, 9
+WORKSPACE_LM_HEAD_DISTILL, WORKSPACE_LM_HEAD_DISTILL_BACKWARD, WORKSPACE_DRAFT_VERIFY = 10, 11, 12
 ROUTER_SOFTMAX, ROUTER_SQRT_SOFTPLUS = 1, 2
 
 

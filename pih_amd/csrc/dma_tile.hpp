@@ -1,0 +1,553 @@
+// Product tiles of bf16 operands fed by DMA, shared by the LM head's losses and
+// the feed-forward block: C [m][n] = A . B^T on the MFMAs, summed in fp32, with
+// what becomes of C chosen by EPI.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "device_common.hpp"
+#include "kernels.hpp"
+
+namespace pih_amd {
+namespace {
+
+// an entry of a list of vocabulary ids that is none
+constexpr uint32_t kNoTarget = 0xffffffffu;
+
+// kEpiStats: maximum and sum of exponentials of every row's columns, and the
+// target's logit; kEpiGrad: the logits' gradient in bf16; kEpiBf16: a scaled
+// result in bf16; kEpiAdd: added to fp32 sums; kEpiTeacherStats, kEpiTeacherGrad: the
+// first two of logits over a temperature, without a target (whose part the
+// caller adds)
+enum : int { kEpiStats = 0, kEpiGrad = 1, kEpiBf16 = 2, kEpiAdd = 3, kEpiTeacherStats = 4, kEpiTeacherGrad = 5 };
+constexpr bool has_stats(int epi) { return epi == kEpiStats || epi == kEpiTeacherStats; }
+constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherGrad; }
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ------------------------------------------------ tiles fed by DMA
+// C [m][n] = A . B^T in tiles of 256 columns and 256, 128 or 64 rows.  Four
+// waves: 2 x 2 quarters of 128 x 128 (64 x 128), one wave per SIMD with 256
+// accumulator registers, or 1 x 4 of 64 x 64.  A K step is 64 deep and moved
+// into LDS by DMA, two (128 and 64 rows: three) steps resident.  Two layouts
+// of an operand:
+//   rows     [row][k] in memory: LDS rows of 128 bytes, 16-byte chunk c of row
+//            r in slot c ^ ((r >> 1) & 7); a fragment is one ds_read_b128
+//            (16 rows, one chunk each: all 64 banks once);
+//   columns  [k][row] in memory: LDS rows of 512 bytes (one k each), chunk c
+//            of k row r in slot c ^ 2 f(r), f(r) = (r & 3) + 4 (r >> 3 & 1); a
+//            fragment is two transposing reads (ds_read_b64_tr_b16: lane l of
+//            16 gives the address of 4 values of k row l / 4 and receives
+//            column l of the four rows), whose 8 k rows per half wave lie in
+//            different 32-byte slots.
+// The step's two 32-deep halves: while the MFMAs of the first run, the second
+// half's fragments are read; then one wait and one barrier (every wave has
+// read the step, and the next one has arrived), and while the MFMAs of the
+// second run, the next step's first fragments are read and another step is
+// sent for, into the buffer just freed.  A block per CU walks its tiles; the
+// next tile's first steps are sent for before the results of this one are
+// worked on.
+constexpr uint32_t TB = 256, KB = 64;
+
+struct BigArgs {
+  const uint16_t* a;
+  const uint16_t* b;
+  uint32_t m, n, k;        // k a multiple of 64
+  uint32_t k_valid;        // columns layout of B: k rows that exist (the others repeat the last)
+  uint64_t lda, ldb;
+  void* out;
+  uint64_t ldo;
+  uint32_t m_tiles, n_tiles, splits;
+  uint64_t split_stride;   // kEpiAdd: elements between the splits' sums
+  const uint32_t* target;
+  const float* lse;
+  const float* mantissa;   // kEpiGrad: [m]
+  const float* scale;      // kEpiBf16: factor of the result
+  float2* stats;
+  float* target_logit;
+  uint32_t v0, vocab, first;
+  float exponent;          // kEpiTeacher*: log2(e) / temperature
+};
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+
+__device__ __forceinline__ v4i join(v4s x, v4s y) {
+  const uint2 a = __builtin_bit_cast(uint2, x), b = __builtin_bit_cast(uint2, y);
+  return v4i{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
+}
+
+// Accumulators held in their registers: with all 256 in use the compiler
+// otherwise moved them about, 518 moves beside 128 MFMAs (now none).
+template <int NB>
+__device__ __forceinline__ void pin(v4f (&c)[NB]) {
+  static_assert(NB == 4 || NB == 8, "blocks");
+  if constexpr (NB == 8)
+    asm volatile("" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
+  else
+    asm volatile("" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]));
+}
+
+template <int ROWS>
+struct BigShape {
+  static constexpr int WM = ROWS >= 128 ? 2 : 1, WN = 4 / WM;        // waves
+  static constexpr int MB = ROWS / 16 / WM, NB = TB / 16 / WN;       // a wave's 16 x 16 blocks
+  static constexpr int ST = ROWS == 256 ? 2 : 3;                     // steps resident
+  static constexpr uint32_t kA = ROWS * KB * 2, kB = TB * KB * 2, kStage = kA + kB;
+  static constexpr int LA = ROWS / 32, LB = 8, NL = LA + LB;         // DMAs per wave and step
+  static constexpr uint32_t kOutRow = 16 * NB * 2 + 16;              // a wave's staged output row
+  static constexpr uint32_t kOutRows = ROWS == 128 ? 8 : 16;         // staged at a time
+  static constexpr uint32_t kOut = ST * kStage;                      // kOutRows of them per wave
+  static constexpr uint32_t kMeta = kOut + 4 * kOutRows * kOutRow;   // per row: two tiles' targets, lse, mantissas
+  static constexpr uint32_t kLds = kMeta + 2 * ROWS * 12;
+  static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+template <int ROWS, bool AT, bool BT, int EPI>
+__global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
+  using S = BigShape<ROWS>;
+  constexpr int MB = S::MB, NB = S::NB, ST = S::ST, LA = S::LA, LB = S::LB, NL = S::NL;
+  __shared__ __align__(16) uint8_t smem[S::kLds];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const uint32_t lds0 = lds_addr(smem);
+
+  // tiles: strips of 8 M tiles, M fastest, so that the 32 tiles an XCD works
+  // on are 8 x 4 (each operand tile is shared by several of them in its L2);
+  // the splits of a tile side by side
+  const uint32_t total = p.m_tiles * p.n_tiles * p.splits, per = (total + 7) / 8, stride = gridDim.x >> 3;
+  const uint32_t end = min(((blockIdx.x & 7) + 1) * per, total);
+  const uint32_t all_steps = p.k / KB, per_split = (all_steps + p.splits - 1) / p.splits;
+  uint32_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  uint32_t m0, n0, split, s0, steps;
+
+  // ---- DMA: instruction i of a wave moves 1 KB: rows 32 i + 8 wave + (l >> 3)
+  // of a rows layout, k rows 8 i + 2 wave + (l >> 5) of a columns layout
+  uint32_t off_a[LA], off_b[LB];
+  const uint8_t* base_a;
+  const uint8_t* base_b;
+  auto offset = [&](auto T, uint32_t i, uint32_t r0, uint32_t rows, uint64_t ld) __attribute__((always_inline)) {
+    if constexpr (decltype(T)::value) {
+      const uint32_t r = 8 * i + 2 * wave + (lane >> 5), f = (r & 3) + 4 * ((r >> 3) & 1);
+      const uint32_t c = min((r0 >> 3) + ((lane & 31) ^ (2 * f)), (rows - 1) >> 3);
+      return (uint32_t)(r * ld * 2) + (c << 4);
+    } else {
+      const uint32_t r = 32 * i + 8 * wave + (lane >> 3);
+      return (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+    }
+  };
+  auto source = [&](auto T, const uint8_t* base, uint64_t ld, uint32_t step) __attribute__((always_inline)) {
+    return uniform_ptr(base + (decltype(T)::value ? (uint64_t)step * KB * ld * 2 : (uint64_t)step * KB * 2));
+  };
+  constexpr std::bool_constant<AT> at{};
+  constexpr std::bool_constant<BT> bt{};
+  // DMA i of a step (A's first) into buffer s
+  auto issue = [&](const uint8_t* sa, const uint8_t* sb, uint32_t s, uint32_t i, bool short_b,
+                   uint32_t step) __attribute__((always_inline)) {
+    const uint32_t lds = lds0 + s * S::kStage + wave * 1024;
+    if (i < (uint32_t)LA) {
+      dma16(sa, off_a[i], lds + i * 4096);
+    } else {
+      i -= LA;
+      uint32_t ob = off_b[i];
+      if constexpr (BT) {
+        if (short_b) {
+          // k rows past the last repeat it (their factors in A are 0)
+          const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.k_valid - 1 - step * KB;
+          if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
+        }
+      }
+      // (few rows: the weights past the caches.  Of one row tile they are read
+      // once: dx of 33 rows over 151936 x 1024 92 -> 72 us, the loss of 128 rows
+      // 84 -> 79.  With two or three row tiles it still gains: the loss of 300
+      // rows 150 -> 135 there, 435 -> 392 over 129280 x 4096, of 200 rows over
+      // 32768 x 1024 26 -> 25; the other way dx of 128 rows there, 60 -> 67)
+      if constexpr (ROWS <= 128) dma16nt(sb, ob, lds + S::kA + i * 4096);
+      else dma16(sb, ob, lds + S::kA + i * 4096);
+    }
+  };
+  // tile t and its first steps sent for; its rows' targets, log-sum-exps and
+  // mantissas into half `which` of the panel (kNoTarget for every row whose g is 0)
+  auto start = [&](uint32_t which) __attribute__((always_inline)) {
+    split = t % p.splits;
+    const uint32_t u = t / p.splits, strip = u / (8 * p.n_tiles), in_strip = u % (8 * p.n_tiles);
+    const uint32_t high = min(8u, p.m_tiles - strip * 8);
+    m0 = (strip * 8 + in_strip % high) * ROWS;
+    n0 = in_strip / high * TB;
+    s0 = min(split * per_split, all_steps);
+    steps = min(s0 + per_split, all_steps) - s0;
+    base_a = reinterpret_cast<const uint8_t*>(AT ? p.a : p.a + m0 * p.lda);
+    base_b = reinterpret_cast<const uint8_t*>(BT ? p.b : p.b + n0 * p.ldb);
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)LA; ++i) off_a[i] = offset(at, i, m0, p.m, p.lda);
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)LB; ++i) off_b[i] = offset(bt, i, n0, p.n, p.ldb);
+#pragma unroll
+    for (uint32_t q = 0; q < (uint32_t)ST; ++q) {
+      if (q >= steps) break;
+      const uint8_t* sa = source(at, base_a, p.lda, s0 + q);
+      const uint8_t* sb = source(bt, base_b, p.ldb, s0 + q);
+      const bool short_b = BT && (s0 + q + 1) * KB > p.k_valid;
+#pragma unroll
+      for (uint32_t i = 0; i < (uint32_t)NL; ++i) issue(sa, sb, q, i, short_b, s0 + q);
+    }
+    if constexpr (EPI == kEpiStats || has_grad(EPI)) {
+      if (tid < ROWS) {
+        const uint32_t row = m0 + tid;
+        uint32_t* const meta = reinterpret_cast<uint32_t*>(smem + S::kMeta + which * ROWS * 12);
+        const uint32_t y = row < p.m ? p.target[row] : kNoTarget;
+        meta[tid] = y < p.vocab ? y : kNoTarget;
+        if constexpr (has_grad(EPI)) {
+          meta[ROWS + tid] = __float_as_uint(row < p.m ? p.lse[row] : 0.0f);
+          meta[2 * ROWS + tid] = __float_as_uint(row < p.m ? p.mantissa[row] : 1.0f);
+        }
+      }
+    }
+  };
+
+  // ---- fragments: 16 rows of the wave's, half q of the step
+  auto frag = [&](auto T, uint32_t stage, uint32_t first, uint32_t q) __attribute__((always_inline)) -> v4i {
+    const uint8_t* const from = smem + stage;
+    if constexpr (decltype(T)::value) {
+      const uint32_t r = 32 * q + 8 * lg + (lr >> 2), f = (lr >> 2) + 4 * (lg & 1);
+      const uint8_t* const x = from + r * 512 + ((2 * first + 8 * (lr & 3)) ^ (32 * f));
+      return join(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)x),
+                  __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x + 4 * 512)));
+    } else {
+      return *reinterpret_cast<const v4i*>(from + (first + lr) * 128 + (((4 * q + lg) ^ ((lr >> 1) & 7)) << 4));
+    }
+  };
+  v4f acc[MB][NB];
+  v4i fa[2][MB], fb[2][NB];
+  // the fragments of a half, three or four beside each group of NB MFMAs: B's
+  // first, which the next half's first group needs, and all of them a group or
+  // two early
+  constexpr uint32_t kReads = (MB + NB + MB - 2) / (MB - 1);
+  auto read_one = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
+    if (i < (uint32_t)NB) fb[to][i] = frag(bt, s * S::kStage + S::kA, wn * NB * 16 + 16 * i, q);
+    else if (i < (uint32_t)(NB + MB)) fa[to][i - NB] = frag(at, s * S::kStage, wm * MB * 16 + 16 * (i - NB), q);
+  };
+  auto read_group = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t e = kReads * i; e < kReads * i + kReads; ++e) read_one(s, q, to, e);
+  };
+  auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fb[from][j]),
+                                                          __builtin_bit_cast(v8bf, fa[from][i]), acc[i][j], 0, 0, 0);
+    pin(acc[i]);
+  };
+  uint32_t s;  // the buffer of the step being multiplied
+  // kNext: the next step exists, with kLeft further steps in flight behind it;
+  // kMore: step j + ST exists and is sent for (kLast: it is the last one,
+  // whose k rows may be short)
+  auto body = [&](uint32_t j, auto NEXT, auto LEFT, auto MORE, auto LAST) __attribute__((always_inline)) {
+    constexpr bool kNext = decltype(NEXT)::value, kMore = decltype(MORE)::value, kLast = decltype(LAST)::value;
+    const uint32_t ns = s + 1 == ST ? 0 : s + 1;
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
+      // (the first MFMAs wait for every LDS read before them)
+      if (i == 0) {
+        multiply(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      read_group(s, 1, 1, i);
+      if (i) multiply(0, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // this step read by this wave, the next one arrived for it (the first ST
+    // had before the tile was begun); then by all
+    __builtin_amdgcn_s_waitcnt(kLdsRead);
+    if (j + 1 >= (uint32_t)ST) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(decltype(LEFT)::value * NL));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const uint32_t step = s0 + j + ST;
+    const uint8_t* sa = nullptr;
+    const uint8_t* sb = nullptr;
+    if constexpr (kMore) {
+      sa = source(at, base_a, p.lda, step);
+      sb = source(bt, base_b, p.ldb, step);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
+      if constexpr (kNext) read_group(ns, 0, 0, i);
+      if constexpr (kMore) {
+#pragma unroll
+        for (uint32_t e = i * NL / MB; e < (i + 1) * NL / MB; ++e)
+          issue(sa, sb, s, e, kLast && (step + 1) * KB > p.k_valid, step);
+      }
+      multiply(1, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    s = ns;
+  };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  constexpr std::integral_constant<int, 0> none;
+  constexpr std::integral_constant<int, ST - 2> full;
+
+  if (t >= end) return;
+  uint32_t which = 0;
+  start(which);
+  // a tile's first steps have arrived before it is begun; for the tiles after
+  // the first that is waited for ahead of the results' stores, which so drain
+  // while the next tile is multiplied
+  auto arrived = []() __attribute__((always_inline)) { __builtin_amdgcn_s_waitcnt(vmcnt_at_most(0)); };
+  arrived();
+  while (true) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < MB; ++i) pin(acc[i]);
+    __builtin_amdgcn_s_waitcnt(kLdsRead);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (steps) {
+      s = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < (uint32_t)(MB + NB); ++i) read_one(0, 0, 0, i);
+      uint32_t j = 0;
+#pragma unroll 1
+      for (; j + ST + (BT ? 1 : 0) < steps; ++j) body(j, yes, full, yes, no);
+      if constexpr (BT)
+        if (j + ST < steps) body(j++, yes, full, yes, yes);
+      if constexpr (ST == 3)
+        if (j + 2 < steps) body(j++, yes, std::integral_constant<int, 1>{}, no, no);
+      if (j + 1 < steps) body(j++, yes, none, no, no);
+      body(j, no, none, no, no);
+    }
+    const uint32_t cm = m0, cn = n0, csplit = split;
+    const uint32_t* const meta = reinterpret_cast<const uint32_t*>(smem + S::kMeta + which * ROWS * 12);
+    const bool more = t + stride < end;
+    which ^= 1;
+    if (more) {
+      // (every wave is past the barrier after its last read of a buffer)
+      t += stride;
+      start(which);
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) pin(acc[i]);
+
+    // ---- results: acc[i][j][e] is row 16 i + lr, column 16 j + 4 lg + e of
+    // the wave's part
+    if constexpr (!has_grad(EPI)) arrived();
+    const uint32_t lrow = wm * MB * 16, wrow = cm + lrow, wcol = cn + wn * NB * 16;
+    const float exponent = EPI == kEpiTeacherStats || EPI == kEpiTeacherGrad ? p.exponent : kLog2e;
+    if constexpr (has_stats(EPI)) {
+      // [column part][row]: maximum and sum
+      float2* const parts = reinterpret_cast<float2*>(smem + S::kOut);
+      static_assert(S::WN * ROWS * 8 <= 4 * S::kOutRows * S::kOutRow, "parts");
+      const bool whole = cn + TB <= p.n;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = -INFINITY;
+        }
+        if constexpr (EPI == kEpiStats) {
+          const uint32_t target = meta[lrow + 16 * i + lr], place = target - wcol;
+          if (place < 16u * NB && ((place >> 2) & 3) == lg && target < p.n) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v = (uint32_t)j == place >> 4 && (uint32_t)e == (place & 3) ? acc[i][j][e] : v;
+            p.target_logit[wrow + 16 * i + lr] = v;
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float from = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          float part = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part += __builtin_amdgcn_exp2f((acc[i][j][e] - from) * exponent);
+          sum += part;
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lg == 0) parts[wn * ROWS + lrow + 16 * i + lr] = float2{top, sum};
+      }
+      __syncthreads();
+      if (tid < ROWS && cm + tid < p.m) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < S::WN; ++w) top = fmaxf(top, parts[w * ROWS + tid].x);
+#pragma unroll
+        for (int w = 0; w < S::WN; ++w) {
+          const float2 x = parts[w * ROWS + tid];
+          sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * exponent);
+        }
+        p.stats[(uint64_t)(cm + tid) * p.n_tiles + cn / TB] = float2{top, sum};
+      }
+    } else if constexpr (EPI == kEpiAdd) {
+      float* const out = static_cast<float*>(p.out) + csplit * p.split_stride + wcol + 4 * lg;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const uint32_t row = wrow + 16 * i + lr;
+        v4f* const o = reinterpret_cast<v4f*>(out + (uint64_t)min(row, p.m - 1) * p.ldo);
+        v4f before[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          before[j] = v4f{0.f, 0.f, 0.f, 0.f};
+          if (!p.first && wcol + 16 * j + 4 * lg < p.n) before[j] = o[4 * j];
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          if (row < p.m && wcol + 16 * j + 4 * lg < p.n) o[4 * j] = before[j] + acc[i][j];
+        // (16 rows at a time: registers for no more)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      // bf16 through the wave's own LDS, 16 or 8 rows at a time, so that a store
+      // instruction writes whole lines
+      constexpr uint32_t kLanes = 2 * NB, kRowsAt = 64 / kLanes;  // lanes per row, rows per instruction
+      uint8_t* const st = smem + S::kOut + wave * S::kOutRows * S::kOutRow;
+      const bool whole = cn + TB <= p.n;
+      const float scale = EPI == kEpiBf16 ? *p.scale : 1.0f;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        if constexpr (has_grad(EPI)) {
+          const uint32_t at_row = lrow + 16 * i + lr, target = meta[at_row], place = target - p.v0 - wcol;
+          const float shift = -__uint_as_float(meta[ROWS + at_row]) * kLog2e;
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], exponent, shift));
+          if (EPI == kEpiGrad && __builtin_amdgcn_ballot_w64(place < 16u * NB)) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (place == 16u * j + 4 * lg + e) acc[i][j][e] -= 1.0f;
+          }
+          const float m = __uint_as_float(meta[2 * ROWS + at_row]);
+          if (__builtin_amdgcn_ballot_w64(m != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = v4f{acc[i][j][0] * m, acc[i][j][1] * m, acc[i][j][2] * m, acc[i][j][3] * m};
+          }
+          if (__builtin_amdgcn_ballot_w64(target == kNoTarget)) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+              if (target == kNoTarget) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+          }
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = 0.0f;
+          }
+          if (i == 0) arrived();
+        }
+#pragma unroll
+        for (uint32_t r0 = 0; r0 < 16; r0 += S::kOutRows) {
+          if (lr - r0 < S::kOutRows) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+              v4f v = acc[i][j];
+              if constexpr (EPI == kEpiBf16) v = v4f{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
+              *reinterpret_cast<uint2*>(st + (lr - r0) * S::kOutRow + j * 32 + lg * 8) =
+                  uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+            }
+          }
+          wave_lds_order();
+#pragma unroll
+          for (uint32_t h = 0; h < S::kOutRows / kRowsAt; ++h) {
+            const uint32_t q = kRowsAt * h + lane / kLanes, r = wrow + 16 * i + r0 + q, c = wcol + 8 * (lane % kLanes);
+            const v4i o = *reinterpret_cast<const v4i*>(st + q * S::kOutRow + lane % kLanes * 16);
+            // the rows of g up to a multiple of 64 and its columns up to the
+            // tile's end are written as zeros: the products with g read them
+            const bool in = has_grad(EPI) ? r < (p.m + 63) / 64 * 64 : r < p.m && c < p.n;
+            if (!in) continue;
+            v4i* const to = reinterpret_cast<v4i*>(static_cast<uint16_t*>(p.out) + (uint64_t)r * p.ldo + c);
+            // (the weights' gradient is not read here again: past the caches,
+            // 33 rows 614 -> 574 us over 129280 x 4096)
+            if constexpr (EPI == kEpiBf16) __builtin_nontemporal_store(o, to);
+            else *to = o;
+          }
+          wave_lds_order();
+        }
+      }
+    }
+    if (!more) return;
+  }
+}
+
+template <int ROWS, bool AT, bool BT, int EPI>
+void launch_rows(BigArgs p, hipStream_t s) {
+  p.m_tiles = (p.m + ROWS - 1) / ROWS;
+  p.n_tiles = (p.n + TB - 1) / TB;
+  if (p.splits == 0) p.splits = 1;
+  const uint32_t grid = std::min((p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8, kCus);
+  hipLaunchKernelGGL((loss_big_kernel<ROWS, AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
+}
+// Time (us) of m rows in tiles of `rows`: the rounds of tiles on the CUs, each a
+// step's time and a tile's own beginning and end
+//   256 rows 1.45 and 9,  128 rows 0.95 and 7,  64 rows 0.70 and 6.
+inline float rows_cost(const BigArgs& p, uint32_t m, uint32_t rows) {
+  const uint32_t splits = std::max(p.splits, 1u), steps = (p.k / KB + splits - 1) / splits;
+  const uint64_t tiles = (uint64_t)((m + rows - 1) / rows) * ((p.n + TB - 1) / TB) * splits;
+  const float tile = rows == 256 ? 9.0f + 1.45f * steps : rows == 128 ? 7.0f + 0.95f * steps : 6.0f + 0.70f * steps;
+  return (float)((tiles + kCus - 1) / kCus) * tile;
+}
+inline uint32_t tile_rows(const BigArgs& p, uint32_t m) {
+  const float c256 = rows_cost(p, m, 256), c128 = rows_cost(p, m, 128), c64 = rows_cost(p, m, 64);
+  return c64 < c128 && c64 < c256 ? 64 : c128 < c256 ? 128 : 256;
+}
+template <bool AT, bool BT, int EPI>
+void launch_any(const BigArgs& p, hipStream_t s) {
+  const uint32_t rows = tile_rows(p, p.m);
+  if (rows == 64) launch_rows<64, AT, BT, EPI>(p, s);
+  else if (rows == 128) launch_rows<128, AT, BT, EPI>(p, s);
+  else launch_rows<256, AT, BT, EPI>(p, s);
+}
+// (the gradient of the weights has the vocabulary for rows: always many)
+template <bool AT, bool BT, int EPI>
+void launch_big(BigArgs p, hipStream_t s) {
+  if constexpr (AT) {
+    launch_rows<256, AT, BT, EPI>(p, s);
+  } else {
+    // the rows behind the last whole 256 in a launch of their own where that is
+    // cheaper, although B is read once more (at 5 TB/s) and the launch costs 3
+    // us: 800 rows over 151936 x 1024 309 -> 283 us; 257 rows would go 154 -> 171
+    const uint32_t whole = p.m / 256 * 256, rest = p.m - whole;
+    const float again = std::max(rows_cost(p, rest, tile_rows(p, rest)), (float)p.n * (float)p.k * (2.0f / 5.0e6f)) + 3.0f;
+    if (whole && rest && rows_cost(p, whole, 256) + again < rows_cost(p, p.m, tile_rows(p, p.m))) {
+      BigArgs q = p;
+      q.m = whole;
+      launch_rows<256, AT, BT, EPI>(q, s);
+      p.m = rest;
+      p.a += whole * p.lda;
+      if constexpr (has_stats(EPI)) {
+        p.stats += (uint64_t)whole * ((p.n + TB - 1) / TB);
+        if constexpr (EPI == kEpiStats) p.target_logit += whole;
+      } else {
+        p.out = static_cast<uint8_t*>(p.out) + whole * p.ldo * (EPI == kEpiAdd ? 4 : 2);
+      }
+      if constexpr (EPI == kEpiStats || has_grad(EPI)) p.target += whole;
+      if constexpr (has_grad(EPI)) {
+        p.lse += whole;
+        p.mantissa += whole;
+      }
+    }
+    launch_any<AT, BT, EPI>(p, s);
+  }
+}
+
+}  // namespace
+}  // namespace pih_amd

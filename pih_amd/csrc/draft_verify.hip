@@ -1,0 +1,510 @@
+// Verification of drafted tokens against a target model's logits for gfx950.
+// With p and q the softmax of a target and a draft row over the sequence's
+// temperature T, u and r given uniform numbers: drafted token d is accepted
+// while u q(d) < p(d); behind the accepted ones comes the smallest v with
+//   sum over v' <= v of w(v') > r sum of w,   w = max(0, p - q) at the rejected
+// place, w = p behind the last one.  (The tokens so put out are distributed as
+// the target's own.)
+//
+// Which token passes the threshold is decided among sums over the whole
+// vocabulary, whose neighbours may differ by 1e-8 and less; exponentials and
+// sums are therefore in 64 bits (of which the vector units do as many a clock
+// as of 32), so that the order of the sums moves no token.
+//
+// Launches: the largest logit and the sum of exponentials of every row and
+// chunk of the vocabulary; a block per sequence that joins them and walks the
+// drafts; the chunks' sums of w at the rejected places; a block per sequence
+// that finds the chunk and in it the token.
+#include "device_common.hpp"
+#include "kernels.hpp"
+
+namespace pih_amd {
+namespace {
+
+constexpr uint32_t kChunk = 4096, kPer = kChunk / 256;
+constexpr uint32_t kMaxVocab = 1u << 20, kMaxSequences = 1u << 14, kMostDrafts = 255;
+constexpr uint32_t kNone = 0xffffffffu;
+constexpr uint32_t kErrToken = 1u, kErrOffsets = 2u, kErrRow = 4u;
+static_assert(kMaxVocab / kChunk <= 256, "a thread per chunk");
+
+struct Stat {
+  double sum;      // of exp((logit - top) / T)
+  float top;       // largest logit
+  uint32_t index;  // greedy: its first place
+};
+// What the walk over a sequence's drafts leaves to be drawn
+struct Plan {
+  double p_inverse, q_inverse, k;  // 1 / sums of the rows, log2(e) / T
+  float p_top, q_top;
+  uint32_t place;   // of the target row, kNone: nothing to draw
+  uint32_t rejected;  // draft row `place` or token `without` is taken off
+  uint32_t without;   // looked-up drafts: the rejected token
+  uint32_t pad;
+};
+
+struct VerifyArgs {
+  const void* target;
+  const void* draft;
+  const uint32_t* tokens;
+  const uint32_t* offsets;
+  const float* accept;
+  const float* sample;
+  const float* temperature;
+  uint32_t* out;
+  uint32_t* accepted;
+  uint32_t* err;
+  Stat* stats;   // [sequences][rows][chunks]
+  Plan* plans;   // [sequences]
+  double* rest;  // [sequences][chunks]
+  uint64_t target_stride, draft_stride;
+  uint32_t sequences, drafts, most, vocab, chunks, rows;
+};
+
+// 2^y for y <= 0 (below -1100: 0; a NaN stays one): 2^f of |f| <= 1/2 by its
+// Taylor polynomial of degree 11 in f ln 2 (6e-15 of it), times 2^n
+__device__ __forceinline__ double exp2_64(double y) {
+  y = y < -1100.0 ? -1100.0 : y;
+  const double n = __builtin_rint(y), t = (y - n) * 0.693147180559945309417;
+  double e = 1.0 / 39916800.0;
+  e = __builtin_fma(e, t, 1.0 / 3628800.0);
+  e = __builtin_fma(e, t, 1.0 / 362880.0);
+  e = __builtin_fma(e, t, 1.0 / 40320.0);
+  e = __builtin_fma(e, t, 1.0 / 5040.0);
+  e = __builtin_fma(e, t, 1.0 / 720.0);
+  e = __builtin_fma(e, t, 1.0 / 120.0);
+  e = __builtin_fma(e, t, 1.0 / 24.0);
+  e = __builtin_fma(e, t, 1.0 / 6.0);
+  e = __builtin_fma(e, t, 0.5);
+  e = __builtin_fma(e, t, 1.0);
+  e = __builtin_fma(e, t, 1.0);
+  return __builtin_amdgcn_ldexp(e, (int)n);
+}
+
+// 16 logits from column c on, -inf past the vocabulary
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void load16(float (&v)[16], const void* row, uint32_t c, uint32_t vocab) {
+  if (WIDE && c + 16 <= vocab) {
+    if constexpr (BF16) {
+      const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 x = p[i];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * i + e] = bf16_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+      }
+    } else {
+      const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(row) + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v4f x = p[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * i + e] = x[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      v[i] = -INFINITY;
+      if (c + i < vocab)
+        v[i] = BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[c + i]) : static_cast<const float*>(row)[c + i];
+    }
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ const void* row_of(const void* base, uint64_t stride, uint64_t row) {
+  return static_cast<const uint8_t*>(base) + row * stride * (BF16 ? 2 : 4);
+}
+template <bool BF16>
+__device__ __forceinline__ float logit_at(const void* row, uint32_t c) {
+  return BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[c]) : static_cast<const float*>(row)[c];
+}
+
+struct Sequence {
+  uint32_t first, count;
+  float temperature;
+  bool offsets_ok;
+};
+__device__ __forceinline__ Sequence sequence_of(const VerifyArgs& p, uint32_t s) {
+  const uint32_t lo = p.offsets[s], hi = p.offsets[s + 1];
+  const float t = p.temperature ? p.temperature[s] : 1.0f;
+  return {lo, hi - lo, t, lo <= hi && hi <= p.drafts && hi - lo <= p.most};
+}
+// (what is left of these stops the sequence at its first place)
+__device__ __forceinline__ bool temperature_ok(float t) { return t >= 0.0f && t < INFINITY; }
+
+template <bool BF16, bool WIDE>
+__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
+  __shared__ double sums[4];
+  __shared__ float tops[4];
+  __shared__ uint32_t indexes[4];
+  const uint32_t chunk = blockIdx.x % p.chunks, at = blockIdx.x / p.chunks, y = at % p.rows, s = at / p.rows;
+  const Sequence q = sequence_of(p, s);
+  const bool greedy = q.temperature == 0.0f, of_draft = y > p.most;
+  const uint32_t place = of_draft ? y - p.most - 1 : y;
+  if (!q.offsets_ok || !temperature_ok(q.temperature) || place > q.count || (of_draft && (greedy || place == q.count)))
+    return;
+  const void* const row = of_draft ? row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + place)
+                                   : row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + place);
+  const uint32_t c = chunk * kChunk + threadIdx.x * kPer, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float v[kPer];
+  load16<BF16, WIDE>(v, row, c, p.vocab);
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < (int)kPer; ++i) top = fmaxf(top, v[i]);
+  top = reduce_max_xor<64>(top);
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  double sum = 0.0;
+  uint32_t index = kNone;
+  if (greedy) {
+#pragma unroll
+    for (int i = (int)kPer - 1; i >= 0; --i) {
+      if (v[i] == top) index = c + i;
+      if (v[i] != v[i]) sum = v[i];
+    }
+    if (index >= p.vocab) index = kNone;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) index = min(index, (uint32_t)__shfl_xor((int)index, off, 64));
+  } else {
+    const double k = 1.44269504088896340736 / (double)q.temperature, from = top == -INFINITY ? 0.0 : (double)top;
+#pragma unroll
+    for (int i = 0; i < (int)kPer; ++i) sum += exp2_64(((double)v[i] - from) * k);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) {
+    sums[wave] = sum;
+    indexes[wave] = index;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    p.stats[(uint64_t)at * p.chunks + chunk] = Stat{sums[0] + sums[1] + sums[2] + sums[3], top,
+                                                    min(min(indexes[0], indexes[1]), min(indexes[2], indexes[3]))};
+}
+
+// The walk over a sequence's drafts
+template <bool BF16>
+__global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
+  __shared__ double row_sum[2 * kMostDrafts + 1];
+  __shared__ float row_top[2 * kMostDrafts + 1];
+  __shared__ uint32_t row_index[kMostDrafts + 1];
+  __shared__ uint32_t stop, why;
+  const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Sequence q = sequence_of(p, s);
+  uint32_t* const out = p.out + (uint64_t)s * (p.most + 1);
+  const bool usable = q.offsets_ok && temperature_ok(q.temperature), greedy = q.temperature == 0.0f;
+  if (!usable) {
+    for (uint32_t i = tid; i <= p.most; i += 256) out[i] = kNone;
+    if (tid == 0) {
+      p.accepted[s] = 0;
+      p.plans[s].place = kNone;
+      atomicOr(p.err, q.offsets_ok ? kErrRow : kErrOffsets);
+    }
+    return;
+  }
+  const double k = 1.44269504088896340736 / (double)(greedy ? 1.0f : q.temperature);
+  const bool soft = p.draft && !greedy;
+  // rows 0 .. count of the target, then the draft's
+  const uint32_t rows = q.count + 1 + (soft ? q.count : 0);
+  for (uint32_t r = wave; r < rows; r += 4) {
+    const uint32_t y = r <= q.count ? r : p.most + 1 + r - (q.count + 1);
+    const Stat* const st = p.stats + ((uint64_t)s * p.rows + y) * p.chunks;
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < p.chunks; i += 64) top = fmaxf(top, st[i].top);
+    top = reduce_max_xor<64>(top);
+    double sum = 0.0;
+    uint32_t index = kNone;
+    for (uint32_t i = lane; i < p.chunks; i += 64) {
+      // (a chunk of -inf alone has the sum 0, or NaN)
+      if (greedy || st[i].top == -INFINITY) sum += st[i].sum;
+      else sum += st[i].sum * exp2_64(((double)st[i].top - (double)top) * k);
+      if (st[i].top == top) index = min(index, st[i].index);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      sum += __shfl_xor(sum, off, 64);
+      index = min(index, (uint32_t)__shfl_xor((int)index, off, 64));
+    }
+    // greedy: a sum of 1 stands for a row that has a largest logit
+    if (greedy && sum == 0.0) sum = top == -INFINITY ? 0.0 : 1.0;
+    if (lane == 0) {
+      row_sum[r] = sum;
+      row_top[r] = top;
+      if (r <= q.count) row_index[r] = index;
+    }
+  }
+  if (tid == 0) stop = q.count;
+  __syncthreads();
+  // a row's sum is above 0 and finite, or the row has no probabilities
+  auto usable_row = [&](uint32_t r) { return row_sum[r] > 0.0 && row_sum[r] < (double)INFINITY; };
+  bool ok = true, bad_token = false, bad_row = false;
+  if (tid <= q.count) bad_row = !usable_row(tid) || (soft && tid < q.count && !usable_row(q.count + 1 + tid));
+  if (tid < q.count) {
+    const uint32_t d = p.tokens[q.first + tid];
+    bad_token = d >= p.vocab;
+    if (greedy) {
+      ok = d == row_index[tid];
+    } else if (bad_token) {
+      ok = false;
+    } else {
+      const void* const target = row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + tid);
+      const double pd = exp2_64(((double)logit_at<BF16>(target, d) - (double)row_top[tid]) * k) / row_sum[tid];
+      double qd = 1.0;
+      if (soft) {
+        const void* const draft = row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + tid);
+        const uint32_t r = q.count + 1 + tid;
+        qd = exp2_64(((double)logit_at<BF16>(draft, d) - (double)row_top[r]) * k) / row_sum[r];
+      }
+      ok = (double)p.accept[q.first + tid] * qd < pd;
+    }
+    if (!ok || bad_row) atomicMin(&stop, tid);
+  }
+  __syncthreads();
+  const uint32_t j = stop;
+  if (tid == j) why = (bad_row ? kErrRow : 0) | (bad_token ? kErrToken : 0);
+  __syncthreads();
+  const uint32_t bits = why;
+  for (uint32_t i = tid; i <= p.most; i += 256) {
+    uint32_t t = kNone;
+    if (i < j) t = p.tokens[q.first + i];
+    else if (i == j && greedy && !(bits & kErrRow)) t = row_index[j];
+    out[i] = t;
+  }
+  if (tid == 0) {
+    p.accepted[s] = j;
+    Plan plan{};
+    plan.place = greedy || (bits & kErrRow) ? kNone : j;
+    if (plan.place != kNone) {
+      plan.k = k;
+      plan.p_top = row_top[j];
+      plan.p_inverse = 1.0 / row_sum[j];
+      plan.rejected = j < q.count;
+      if (plan.rejected) {
+        plan.without = p.tokens[q.first + j];
+        if (soft) {
+          plan.q_top = row_top[q.count + 1 + j];
+          plan.q_inverse = 1.0 / row_sum[q.count + 1 + j];
+        }
+      }
+    }
+    p.plans[s] = plan;
+    if (bits) atomicOr(p.err, bits);
+  }
+}
+
+// w of a thread's 16 columns of a chunk; `whole`: p alone
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void weights(double (&w)[16], const VerifyArgs& p, const Plan& plan, const Sequence& q, uint32_t s,
+                                        uint32_t c, bool whole) {
+  float v[16];
+  load16<BF16, WIDE>(v, row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + plan.place), c, p.vocab);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = exp2_64(((double)v[i] - (double)plan.p_top) * plan.k) * plan.p_inverse;
+  if (whole) return;
+  if (p.draft) {
+    load16<BF16, WIDE>(v, row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + plan.place), c, p.vocab);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const double d = w[i] - exp2_64(((double)v[i] - (double)plan.q_top) * plan.k) * plan.q_inverse;
+      w[i] = d > 0.0 ? d : 0.0;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i == plan.without) w[i] = 0.0;
+  }
+}
+
+// Sums of w over the chunks, at the rejected places
+template <bool BF16, bool WIDE>
+__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs p) {
+  __shared__ double sums[4];
+  const uint32_t chunk = blockIdx.x % p.chunks, s = blockIdx.x / p.chunks;
+  const Plan plan = p.plans[s];
+  if (plan.place == kNone || !plan.rejected) return;
+  double w[16];
+  weights<BF16, WIDE>(w, p, plan, sequence_of(p, s), s, chunk * kChunk + threadIdx.x * kPer, false);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum += w[i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) p.rest[(uint64_t)s * p.chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+// Running sum over the block's threads, in order; `parts` [4]
+__device__ __forceinline__ double running_sum(double v, double* parts) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const double from = __shfl_up(v, off, 64);
+    if (lane >= (uint32_t)off) v += from;
+  }
+  if (lane == 63) parts[wave] = v;
+  __syncthreads();
+  for (uint32_t i = 0; i < wave; ++i) v += parts[i];
+  return v;
+}
+
+template <bool BF16, bool WIDE>
+__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs p) {
+  __shared__ double parts[3][4];
+  __shared__ double all, before;
+  __shared__ uint32_t found, last;
+  const uint32_t s = blockIdx.x, tid = threadIdx.x;
+  const Plan plan = p.plans[s];
+  if (plan.place == kNone) return;
+  if (tid == 0) {
+    found = kNone;
+    last = 0;
+  }
+  // the chunks' sums of w; where they are 0 throughout, of p
+  double own = plan.rejected && tid < p.chunks ? p.rest[(uint64_t)s * p.chunks + tid] : 0.0;
+  double run = running_sum(own, parts[0]);
+  if (tid == 255) all = run;
+  __syncthreads();
+  const bool whole = !(all > 0.0);
+  if (whole) {
+    own = 0.0;
+    if (tid < p.chunks) {
+      const Stat st = p.stats[((uint64_t)s * p.rows + plan.place) * p.chunks + tid];
+      if (st.top != -INFINITY) own = st.sum * exp2_64(((double)st.top - (double)plan.p_top) * plan.k) * plan.p_inverse;
+    }
+    run = running_sum(own, parts[1]);
+    if (tid == 255) all = run;
+    __syncthreads();
+  }
+  const double threshold = (double)p.sample[s] * all;
+  // (where rounding leaves none above the threshold, the last that has a sum)
+  if (own > 0.0) {
+    if (run > threshold) atomicMin(&found, tid);
+    atomicMax(&last, tid);
+  }
+  __syncthreads();
+  const uint32_t chunk = found != kNone ? found : last;
+  if (tid == chunk) before = run - own;
+  __syncthreads();
+  if (tid == 0) {
+    found = kNone;
+    last = 0;
+  }
+  const double left = threshold - before;
+  double w[16];
+  weights<BF16, WIDE>(w, p, plan, sequence_of(p, s), s, chunk * kChunk + tid * kPer, whole);
+  own = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) own += w[i];
+  run = running_sum(own, parts[2]);
+  if (own > 0.0) {
+    if (run > left) atomicMin(&found, tid);
+    atomicMax(&last, tid);
+  }
+  __syncthreads();
+  if (tid != (found != kNone ? found : last)) return;
+  double sum = run - own;
+  uint32_t token = 0;
+  bool done = false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (done || !(w[i] > 0.0)) continue;
+    sum += w[i];
+    token = chunk * kChunk + tid * kPer + i;
+    done = sum > left;
+  }
+  p.out[(uint64_t)s * (p.most + 1) + plan.place] = token;
+}
+
+bool sizes_ok(uint32_t sequences, uint32_t most, uint32_t vocab) {
+  return sequences && sequences <= kMaxSequences && most <= kMostDrafts && vocab && vocab <= kMaxVocab;
+}
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
+uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
+
+struct VerifyPlan {
+  uint64_t plans, rest, bytes;
+};
+VerifyPlan verify_plan(uint32_t sequences, uint32_t most, uint32_t vocab) {
+  VerifyPlan v{};
+  v.plans = padded((uint64_t)sequences * (2 * most + 1) * chunks_of(vocab) * sizeof(Stat));
+  v.rest = v.plans + padded((uint64_t)sequences * sizeof(Plan));
+  v.bytes = v.rest + padded((uint64_t)sequences * chunks_of(vocab) * 8);
+  return v;
+}
+
+template <bool BF16, bool WIDE>
+void launch(const VerifyArgs& p, hipStream_t s) {
+  hipLaunchKernelGGL((verify_stats_kernel<BF16, WIDE>), dim3(p.sequences * p.rows * p.chunks), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((verify_walk_kernel<BF16>), dim3(p.sequences), dim3(256), 0, s, p);
+  if (p.drafts) hipLaunchKernelGGL((verify_rest_kernel<BF16, WIDE>), dim3(p.sequences * p.chunks), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((verify_pick_kernel<BF16, WIDE>), dim3(p.sequences), dim3(256), 0, s, p);
+}
+
+}  // namespace
+
+uint64_t DraftVerifyWorkspaceBytes(uint32_t sequences, uint32_t max_drafts, uint32_t vocab) {
+  return sizes_ok(sequences, max_drafts, vocab) ? verify_plan(sequences, max_drafts, vocab).bytes : 0;
+}
+
+St LaunchDraftVerify(const DraftVerifyArgs& a) {
+  if (!a.target || !a.offsets || !a.sample || !a.out || !a.accepted || !a.workspace || !a.error_flag || !a.stream ||
+      (a.drafts && (!a.tokens || !a.accept)))
+    return Invalid("draft_verify_null_argument");
+  if (!sizes_ok(a.sequences, a.max_drafts, a.vocab) || a.drafts > (1u << 20) || a.target_stride < a.vocab ||
+      (a.draft && a.draft_stride < a.vocab))
+    return Invalid("draft_verify_shape_invalid");
+  const uint32_t size = a.kind == kOutBf16 ? 2 : 4;
+  if (!aligned(a.target, size) || !aligned(a.draft, size) || !aligned(a.tokens, 4) || !aligned(a.offsets, 4) ||
+      !aligned(a.accept, 4) || !aligned(a.sample, 4) || !aligned(a.temperature, 4) || !aligned(a.out, 4) ||
+      !aligned(a.accepted, 4) || !aligned(a.error_flag, 4))
+    return Invalid("draft_verify_alignment_invalid");
+  // (the accepted tokens are written before the rejected one is read)
+  if (a.out == a.tokens || a.accepted == a.offsets || a.out == a.accepted) return Invalid("draft_verify_alias_invalid");
+  const VerifyPlan plan = verify_plan(a.sequences, a.max_drafts, a.vocab);
+  const uint32_t chunks = chunks_of(a.vocab), rows = a.max_drafts + 1 + (a.draft ? a.max_drafts : 0);
+  if (a.workspace_bytes < plan.bytes || !aligned(a.workspace, 16)) return Invalid("draft_verify_workspace_invalid");
+  if ((uint64_t)a.sequences * rows * chunks > (1u << 24) - 1) return Invalid("draft_verify_shape_invalid");
+  St clean = RequireCleanLastError();
+  if (!clean.ok()) return clean;
+  uint8_t* const ws = static_cast<uint8_t*>(a.workspace);
+  VerifyArgs p{};
+  p.target = a.target;
+  p.draft = a.draft;
+  p.tokens = a.tokens;
+  p.offsets = a.offsets;
+  p.accept = a.accept;
+  p.sample = a.sample;
+  p.temperature = a.temperature;
+  p.out = a.out;
+  p.accepted = a.accepted;
+  p.err = a.error_flag;
+  p.stats = reinterpret_cast<Stat*>(ws);
+  p.plans = reinterpret_cast<Plan*>(ws + plan.plans);
+  p.rest = reinterpret_cast<double*>(ws + plan.rest);
+  p.target_stride = a.target_stride;
+  p.draft_stride = a.draft_stride;
+  p.sequences = a.sequences;
+  p.drafts = a.drafts;
+  p.most = a.max_drafts;
+  p.vocab = a.vocab;
+  p.chunks = chunks;
+  p.rows = rows;
+  // 16-byte reads of whole rows
+  const bool wide = aligned(a.target, 16) && a.target_stride * size % 16 == 0 &&
+                    (!a.draft || (aligned(a.draft, 16) && a.draft_stride * size % 16 == 0));
+  if (a.kind == kOutBf16) {
+    if (wide) launch<true, true>(p, a.stream);
+    else launch<true, false>(p, a.stream);
+  } else {
+    if (wide) launch<false, true>(p, a.stream);
+    else launch<false, false>(p, a.stream);
+  }
+  return AfterLaunch("draft_verify_launch_failed");
+}
+
+}  // namespace pih_amd

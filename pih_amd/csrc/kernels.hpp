@@ -366,6 +366,84 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a);
 uint64_t LmHeadLossWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden);
 uint64_t LmHeadLossBackwardWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden);
 
+// ------------------------------------------- LM head against a teacher
+// (lm_head_distill.hip)
+struct LmHeadDistillArgs {
+  const uint16_t* x = nullptr;            // [rows, hidden]
+  const uint16_t* w = nullptr;            // [vocab, hidden]
+  const uint32_t* ids = nullptr;          // [rows, top_k], 0xffffffff: none
+  const float* teacher = nullptr;         // [rows, top_k]
+  const float* teacher_lse = nullptr;     // [rows] (nullptr: over the entries)
+  float* loss = nullptr;                  // forward: [rows]
+  float* lse = nullptr;                   // [rows]; forward: written; backward: read
+  float* logits = nullptr;                // [rows, top_k]; the same
+  const float* loss_grad = nullptr;       // backward: [rows]
+  uint16_t* dx = nullptr;                 // backward: [rows, hidden]
+  uint16_t* dw = nullptr;                 // backward: [vocab, hidden] (nullptr: left out)
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  uint32_t* error_flag = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t rows = 0, vocab = 0, hidden = 0, top_k = 0;
+  float temperature = 1.0f;
+};
+St LaunchLmHeadDistill(const LmHeadDistillArgs& a);
+St LaunchLmHeadDistillBackward(const LmHeadDistillArgs& a);
+// 0 for a shape that the launcher refuses
+uint64_t LmHeadDistillWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden);
+uint64_t LmHeadDistillBackwardWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden);
+
+// ------------------------------------------------ gated feed-forward block
+// (gated_mlp.hip)
+struct GatedMlpArgs {
+  const uint16_t* x = nullptr;      // [rows, hidden]
+  const uint16_t* wg = nullptr;     // [inter, hidden]
+  const uint16_t* wu = nullptr;     // [inter, hidden]
+  const uint16_t* wd = nullptr;     // [hidden, inter]
+  uint16_t* y = nullptr;            // forward: [rows, hidden]
+  uint16_t* gate = nullptr;         // [rows, inter]; forward: written (nullptr: not kept); backward: read
+  uint16_t* up = nullptr;           // the same
+  const uint16_t* dy = nullptr;     // backward: [rows, hidden]
+  uint16_t* dx = nullptr;           // backward, nullptr: left out; [rows, hidden]
+  uint16_t* dwg = nullptr;          // [inter, hidden]
+  uint16_t* dwu = nullptr;          // [inter, hidden]
+  uint16_t* dwd = nullptr;          // [hidden, inter]
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  hipStream_t stream = nullptr;
+  uint32_t rows = 0, hidden = 0, inter = 0;
+  float limit = 0.0f;
+};
+St LaunchGatedMlp(const GatedMlpArgs& a);
+St LaunchGatedMlpBackward(const GatedMlpArgs& a);
+// 0 for a shape that the launcher refuses
+uint64_t GatedMlpWorkspaceBytes(uint32_t rows, uint32_t inter, uint32_t hidden);
+uint64_t GatedMlpBackwardWorkspaceBytes(uint32_t rows, uint32_t inter, uint32_t hidden);
+
+// --------------------------------------------- verification of drafts
+// (draft_verify.hip)
+struct DraftVerifyArgs {
+  const void* target = nullptr;        // [drafts + sequences, vocab]
+  const void* draft = nullptr;         // [drafts, vocab] (nullptr: looked up)
+  const uint32_t* tokens = nullptr;    // [drafts]
+  const uint32_t* offsets = nullptr;   // [sequences + 1]
+  const float* accept = nullptr;       // [drafts]
+  const float* sample = nullptr;       // [sequences]
+  const float* temperature = nullptr;  // [sequences] (nullptr: 1)
+  uint32_t* out = nullptr;             // [sequences, max_drafts + 1]
+  uint32_t* accepted = nullptr;        // [sequences]
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  uint32_t* error_flag = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t sequences = 0, drafts = 0, max_drafts = 0, vocab = 0;
+  uint32_t target_stride = 0, draft_stride = 0;
+  OutKind kind = kOutF32;              // of the logits
+};
+St LaunchDraftVerify(const DraftVerifyArgs& a);
+// 0 for a shape that the launcher refuses
+uint64_t DraftVerifyWorkspaceBytes(uint32_t sequences, uint32_t max_drafts, uint32_t vocab);
+
 // --------------------------------------------------------------- MoE glue
 struct RoutePlanArgs {
   const uint32_t* topk_ids = nullptr;     // [tokens, topk]

@@ -56,6 +56,26 @@ St QueryWorkspace(const pih_amd_workspace_query_v1* r) {
       bytes = RouterBalanceWorkspaceBytes(r->m, r->n, r->k);
       if (bytes == 0) return Invalid("workspace_query_shape_invalid");
       break;
+    case PIH_AMD_WORKSPACE_GATED_MLP_V1:
+      bytes = GatedMlpWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_GATED_MLP_BACKWARD_V1:
+      bytes = GatedMlpBackwardWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_LM_HEAD_DISTILL_V1:
+      bytes = LmHeadDistillWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_LM_HEAD_DISTILL_BACKWARD_V1:
+      bytes = LmHeadDistillBackwardWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
+    case PIH_AMD_WORKSPACE_DRAFT_VERIFY_V1:
+      bytes = DraftVerifyWorkspaceBytes(r->m, r->n, r->k);
+      if (bytes == 0) return Invalid("workspace_query_shape_invalid");
+      break;
     default:
       return Invalid("workspace_query_kind_invalid");
   }
@@ -636,6 +656,126 @@ St RouterBackward(const pih_amd_router_backward_launch_v1* r) {
   return LaunchRouterBackward(a);
 }
 
+St GatedMlp(const pih_amd_gated_mlp_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("gated_mlp_request_invalid");
+  GatedMlpArgs a;
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.wg = Ptr<const uint16_t>(r->gate_weight_bf16);
+  a.wu = Ptr<const uint16_t>(r->up_weight_bf16);
+  a.wd = Ptr<const uint16_t>(r->down_weight_bf16);
+  a.y = Ptr<uint16_t>(r->output_bf16);
+  a.gate = Ptr<uint16_t>(r->gate_bf16);
+  a.up = Ptr<uint16_t>(r->up_bf16);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.stream = AsStream(r->stream);
+  a.rows = r->rows;
+  a.hidden = r->hidden;
+  a.inter = r->intermediate;
+  a.limit = r->limit;
+  return LaunchGatedMlp(a);
+}
+
+St GatedMlpBackward(const pih_amd_gated_mlp_backward_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("gated_mlp_backward_request_invalid");
+  GatedMlpArgs a;
+  a.dy = Ptr<const uint16_t>(r->output_grad_bf16);
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.wg = Ptr<const uint16_t>(r->gate_weight_bf16);
+  a.wu = Ptr<const uint16_t>(r->up_weight_bf16);
+  a.wd = Ptr<const uint16_t>(r->down_weight_bf16);
+  a.gate = Ptr<uint16_t>(r->gate_bf16);
+  a.up = Ptr<uint16_t>(r->up_bf16);
+  a.dx = Ptr<uint16_t>(r->input_grad_bf16);
+  a.dwg = Ptr<uint16_t>(r->gate_weight_grad_bf16);
+  a.dwu = Ptr<uint16_t>(r->up_weight_grad_bf16);
+  a.dwd = Ptr<uint16_t>(r->down_weight_grad_bf16);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.stream = AsStream(r->stream);
+  a.rows = r->rows;
+  a.hidden = r->hidden;
+  a.inter = r->intermediate;
+  a.limit = r->limit;
+  return LaunchGatedMlpBackward(a);
+}
+
+St LmHeadDistill(const pih_amd_lm_head_distill_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("lm_head_distill_request_invalid");
+  LmHeadDistillArgs a;
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.w = Ptr<const uint16_t>(r->weight_bf16);
+  a.ids = Ptr<const uint32_t>(r->teacher_ids_u32);
+  a.teacher = Ptr<const float>(r->teacher_logits_f32);
+  a.teacher_lse = Ptr<const float>(r->teacher_lse_f32);
+  a.loss = Ptr<float>(r->loss_f32);
+  a.lse = Ptr<float>(r->lse_f32);
+  a.logits = Ptr<float>(r->logits_f32);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.rows = r->rows;
+  a.vocab = r->vocab;
+  a.hidden = r->hidden;
+  a.top_k = r->top_k;
+  a.temperature = r->temperature;
+  return LaunchLmHeadDistill(a);
+}
+
+St LmHeadDistillBackward(const pih_amd_lm_head_distill_backward_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("lm_head_distill_backward_request_invalid");
+  LmHeadDistillArgs a;
+  a.x = Ptr<const uint16_t>(r->input_bf16);
+  a.w = Ptr<const uint16_t>(r->weight_bf16);
+  a.ids = Ptr<const uint32_t>(r->teacher_ids_u32);
+  a.teacher = Ptr<const float>(r->teacher_logits_f32);
+  a.teacher_lse = Ptr<const float>(r->teacher_lse_f32);
+  a.lse = Ptr<float>(r->lse_f32);
+  a.logits = Ptr<float>(r->logits_f32);
+  a.loss_grad = Ptr<const float>(r->loss_grad_f32);
+  a.dx = Ptr<uint16_t>(r->input_grad_bf16);
+  a.dw = Ptr<uint16_t>(r->weight_grad_bf16);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.rows = r->rows;
+  a.vocab = r->vocab;
+  a.hidden = r->hidden;
+  a.top_k = r->top_k;
+  a.temperature = r->temperature;
+  return LaunchLmHeadDistillBackward(a);
+}
+
+St DraftVerify(const pih_amd_draft_verify_launch_v1* r) {
+  if (!HeaderOk(r, kAbi)) return Invalid("draft_verify_request_invalid");
+  if (r->logits_type != PIH_AMD_OUTPUT_BF16_V1 && r->logits_type != PIH_AMD_OUTPUT_F32_V1)
+    return Invalid("draft_verify_logits_type_invalid");
+  DraftVerifyArgs a;
+  a.target = Ptr<const void>(r->target_logits);
+  a.draft = Ptr<const void>(r->draft_logits);
+  a.tokens = Ptr<const uint32_t>(r->draft_tokens_u32);
+  a.offsets = Ptr<const uint32_t>(r->draft_offsets_u32);
+  a.accept = Ptr<const float>(r->accept_random_f32);
+  a.sample = Ptr<const float>(r->sample_random_f32);
+  a.temperature = Ptr<const float>(r->temperature_f32);
+  a.out = Ptr<uint32_t>(r->tokens_u32);
+  a.accepted = Ptr<uint32_t>(r->accepted_u32);
+  a.workspace = Ptr<void>(r->workspace);
+  a.workspace_bytes = r->workspace_bytes;
+  a.error_flag = Ptr<uint32_t>(r->error_flag_u32);
+  a.stream = AsStream(r->stream);
+  a.sequences = r->sequence_count;
+  a.drafts = r->draft_count;
+  a.max_drafts = r->max_drafts;
+  a.vocab = r->vocab;
+  a.target_stride = r->target_stride;
+  a.draft_stride = r->draft_stride;
+  a.kind = static_cast<OutKind>(r->logits_type);
+  return LaunchDraftVerify(a);
+}
+
 PIH_AMD_CONTAINED(CQueryWorkspace, QueryWorkspace, pih_amd_workspace_query_v1)
 PIH_AMD_CONTAINED(CRoutePlan, RoutePlan, pih_amd_route_plan_launch_v1)
 PIH_AMD_CONTAINED(CFp8Quant, Fp8Quant, pih_amd_fp8_quant_launch_v1)
@@ -664,6 +804,11 @@ PIH_AMD_CONTAINED(CLmHeadLoss, LmHeadLoss, pih_amd_lm_head_loss_launch_v1)
 PIH_AMD_CONTAINED(CLmHeadLossBackward, LmHeadLossBackward, pih_amd_lm_head_loss_backward_launch_v1)
 PIH_AMD_CONTAINED(CRouterBalance, RouterBalance, pih_amd_router_balance_launch_v1)
 PIH_AMD_CONTAINED(CRouterBackward, RouterBackward, pih_amd_router_backward_launch_v1)
+PIH_AMD_CONTAINED(CGatedMlp, GatedMlp, pih_amd_gated_mlp_launch_v1)
+PIH_AMD_CONTAINED(CGatedMlpBackward, GatedMlpBackward, pih_amd_gated_mlp_backward_launch_v1)
+PIH_AMD_CONTAINED(CLmHeadDistill, LmHeadDistill, pih_amd_lm_head_distill_launch_v1)
+PIH_AMD_CONTAINED(CLmHeadDistillBackward, LmHeadDistillBackward, pih_amd_lm_head_distill_backward_launch_v1)
+PIH_AMD_CONTAINED(CDraftVerify, DraftVerify, pih_amd_draft_verify_launch_v1)
 
 const pih_amd_linear_kernels_api_v1 kContract = {
     sizeof(pih_amd_linear_kernels_api_v1), kAbi, &kIdentity, &CQueryWorkspace, &CRoutePlan,
@@ -671,7 +816,7 @@ const pih_amd_linear_kernels_api_v1 kContract = {
     &CSiluMul, &CSwiGlu, &CMxfp4Decode, &CW4a16Dequant, &CW4a16Grouped, &CQueryMoeLayer, &CMoeLayer,
     &CRoutePlanNoAlloc, &CRouterTopk, &CV41Linear, &CV41Fp4ToFp8, &CV41BlockDequant,
     &CAdapterGemm, &CQueryAdapterBackward, &CAdapterBackward, &CLmHeadLoss, &CLmHeadLossBackward, &CRouterBalance,
-    &CRouterBackward};
+    &CRouterBackward, &CGatedMlp, &CGatedMlpBackward, &CLmHeadDistill, &CLmHeadDistillBackward, &CDraftVerify};
 
 pih_status_v1 BindOrigin(const char* path) noexcept {
   return ToAbi(path && path[0] == '/' ? Ok() : Invalid("bind_origin_path_not_absolute"));

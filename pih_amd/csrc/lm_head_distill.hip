@@ -1,0 +1,323 @@
+// Divergence of an LM head from a teacher's top logits and its gradients for
+// gfx950, without the head's own logits in memory.  With z_tv = x_t . w_v, the
+// temperature T and a row's teacher entries k of id i_k and probability q_k:
+//   lse_t = log sum_v exp(z_tv / T),
+//   loss_t = T^2 sum_k q_k (log q_k - z_{t i_k} / T + lse_t),
+//   g_tv = up_t T (Q_t exp(z_tv / T - lse_t) - sum of q_k over i_k = v),
+//   dx = g W,  dw = g^T x,  Q_t = sum_k q_k.
+//
+// The products are those of the cross entropy (lm_head_loss.hip) without a
+// target.  The teacher's entries are few against the vocabulary, so they come
+// in launches of their own: forward the row's logits at them and the sum over
+// them, backward the elements of g at them, which the tiles have written
+// without their q.
+#include "lm_head_common.hpp"
+
+namespace pih_amd {
+namespace {
+
+constexpr uint32_t kTopMax = 256;
+
+// Teacher entries of a row, by a wave: lane l holds entries l, l + 64, ..
+struct Entries {
+  uint32_t id[kTopMax / 64];  // kNoTarget: none
+  float s[kTopMax / 64];      // logit over the temperature, -inf: none
+};
+__device__ __forceinline__ bool load_entries(Entries& e, const uint32_t* ids, const float* teacher, uint64_t at,
+                                             uint32_t top_k, uint32_t vocab, float inverse) {
+  const uint32_t lane = threadIdx.x & 63;
+  bool bad = false;
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    const uint32_t k = lane + 64 * i;
+    e.id[i] = k < top_k ? ids[at + k] : kNoTarget;
+    bad |= e.id[i] >= vocab && e.id[i] != kNoTarget;
+    if (e.id[i] >= vocab) e.id[i] = kNoTarget;
+    e.s[i] = e.id[i] != kNoTarget ? teacher[at + k] * inverse : -INFINITY;
+  }
+  return bad;
+}
+// log of what exp(s) is divided by, of a row; -inf where no entry has a
+// probability (its q are then 0 by probability())
+__device__ __forceinline__ float normalizer(const Entries& e, const float* teacher_lse, uint32_t row) {
+  if (teacher_lse) return teacher_lse[row];
+  float top = -INFINITY, sum = 0.0f;
+  bool nan = false;
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    top = fmaxf(top, e.s[i]);
+    nan |= e.s[i] != e.s[i];
+  }
+  top = reduce_max_xor<64>(top);
+  if (__builtin_amdgcn_ballot_w64(nan)) return __builtin_nanf("");
+  if (top == -INFINITY) return top;
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) sum += expf(e.s[i] - top);
+  return top + logf(reduce_sum_xor<64>(sum));
+}
+__device__ __forceinline__ float probability(float s, float normalizer) {
+  return s == -INFINITY ? 0.0f : expf(s - normalizer);
+}
+
+// z of every entry, by a wave: a dot product over the hidden size
+__global__ __launch_bounds__(256) void distill_gather_kernel(const uint16_t* x, const uint16_t* w, const uint32_t* ids,
+                                                             float* logits, uint64_t entries, uint32_t top_k,
+                                                             uint32_t vocab, uint32_t hidden) {
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); at < entries; at += (uint64_t)gridDim.x * 4) {
+    const uint32_t id = ids[at];
+    float sum = 0.0f;
+    if (id < vocab) {
+      const uint16_t* const a = x + at / top_k * hidden;
+      const uint16_t* const b = w + (uint64_t)id * hidden;
+      for (uint32_t c = lane * 8; c < hidden; c += 512) {
+        const v4i u = *reinterpret_cast<const v4i*>(a + c), v = *reinterpret_cast<const v4i*>(b + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t p = (uint32_t)u[i], q = (uint32_t)v[i];
+          sum = __builtin_fmaf(bf16_bits_to_f32(p & 0xffffu), bf16_bits_to_f32(q & 0xffffu), sum);
+          sum = __builtin_fmaf(bf16_bits_to_f32(p >> 16), bf16_bits_to_f32(q >> 16), sum);
+        }
+      }
+      sum = reduce_sum_xor<64>(sum);
+    }
+    if (lane == 0) logits[at] = sum;
+  }
+}
+
+// A row's pairs joined and its loss, by a wave
+__global__ __launch_bounds__(256) void distill_join_kernel(const float2* stats, const uint32_t* ids,
+                                                           const float* teacher, const float* teacher_lse,
+                                                           const float* logits, float* loss, float* lse, uint32_t* err,
+                                                           uint32_t rows, uint32_t vocab, uint32_t tiles, uint32_t top_k,
+                                                           float temperature) {
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const float2* s = stats + (uint64_t)row * tiles;
+  const float inverse = 1.0f / temperature;
+  float top = -INFINITY, sum = 0.0f;
+#pragma unroll 8
+  for (uint32_t i = lane; i < tiles; i += 64) top = fmaxf(top, s[i].x);
+  top = reduce_max_xor<64>(top);
+  // (a tile of -inf or NaN alone has the sum 0 or NaN, whatever the factor)
+#pragma unroll 8
+  for (uint32_t i = lane; i < tiles; i += 64) sum += s[i].x == -INFINITY ? s[i].y : s[i].y * expf((s[i].x - top) * inverse);
+  sum = reduce_sum_xor<64>(sum);
+  const float l = top * inverse + logf(sum);
+  Entries e;
+  const uint64_t at = (uint64_t)row * top_k;
+  const bool bad = load_entries(e, ids, teacher, at, top_k, vocab, inverse);
+  const float norm = normalizer(e, teacher_lse, row);
+  float total = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    const float q = probability(e.s[i], norm);
+    // (an entry of probability 0 adds nothing, whatever its logit)
+    if (q != 0.0f) total += q * ((e.s[i] - norm) - (logits[at + lane + 64 * i] * inverse - l));
+  }
+  total = reduce_sum_xor<64>(total) * temperature * temperature;
+  uint32_t bits = __builtin_amdgcn_ballot_w64(bad) ? kErrTarget : 0;
+  if (!__builtin_isfinite(total)) bits |= kErrLoss;
+  if (lane) return;
+  lse[row] = l;
+  loss[row] = total;
+  if (bits) atomicOr(err, bits);
+}
+
+// What the backward pass needs of a row's teacher, by a wave: live 0
+// (kNoTarget where no entry has a probability), the normalizer, Q, lse - log Q
+// and the upstream factor up T
+struct TeacherRows {
+  uint32_t* live;
+  float *norm, *total, *shift, *up;
+};
+__global__ __launch_bounds__(256) void distill_teacher_kernel(const uint32_t* ids, const float* teacher,
+                                                              const float* teacher_lse, const float* lse,
+                                                              const float* loss_grad, TeacherRows out, uint32_t* err,
+                                                              uint32_t rows, uint32_t vocab, uint32_t top_k,
+                                                              float temperature) {
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  Entries e;
+  const bool bad = load_entries(e, ids, teacher, (uint64_t)row * top_k, top_k, vocab, 1.0f / temperature);
+  const float norm = normalizer(e, teacher_lse, row);
+  float total = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) total += probability(e.s[i], norm);
+  total = reduce_sum_xor<64>(total);
+  const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+  if (lane) return;
+  out.live[row] = total == 0.0f ? kNoTarget : 0;
+  out.norm[row] = norm;
+  out.total[row] = total;
+  out.shift[row] = lse[row] - logf(total);
+  out.up[row] = loss_grad[row] * temperature;
+  if (any_bad) atomicOr(err, kErrTarget);
+}
+
+// g at the teacher's entries whose id lies in the piece [v0, v0 + cols), a
+// wave a row; an id twice in a row gets the sum of its entries twice, the same
+__global__ __launch_bounds__(256) void distill_entries_kernel(const uint32_t* ids, const float* teacher,
+                                                              const float* logits, const float* lse, TeacherRows in,
+                                                              const float* mantissa, uint16_t* g, uint64_t ldg,
+                                                              uint32_t rows, uint32_t vocab, uint32_t top_k, uint32_t v0,
+                                                              uint32_t cols, float temperature) {
+  __shared__ uint32_t all_id[4][kTopMax];
+  __shared__ float all_q[4][kTopMax];
+  const uint32_t wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
+  if (row >= rows || in.live[row] == kNoTarget) return;
+  Entries e;
+  const float inverse = 1.0f / temperature;
+  const uint64_t at = (uint64_t)row * top_k;
+  load_entries(e, ids, teacher, at, top_k, vocab, inverse);
+  const float norm = in.norm[row];
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    all_id[wave][lane + 64 * i] = e.id[i];
+    all_q[wave][lane + 64 * i] = probability(e.s[i], norm);
+  }
+  wave_lds_order();
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    const uint32_t id = e.id[i], place = id - v0;
+    if (id == kNoTarget || place >= cols) continue;
+    float q = 0.0f;
+    for (uint32_t k = 0; k < top_k; ++k) q += all_id[wave][k] == id ? all_q[wave][k] : 0.0f;
+    const float p = in.total[row] * expf(logits[at + lane + 64 * i] * inverse - lse[row]);
+    g[row * ldg + place] = (uint16_t)f32_to_bf16_bits(mantissa[row] * (p - q));
+  }
+}
+
+bool distill_ok(const LmHeadDistillArgs& a) {
+  return shape_ok(a.rows, a.vocab, a.hidden) && a.top_k && a.top_k <= kTopMax;
+}
+bool temperature_ok(float t) { return t > 0.0f && __builtin_isfinite(t) && __builtin_isfinite(1.0f / t); }
+
+struct DistillPlan {
+  BackwardPlan loss;
+  uint64_t live, norm, total, shift, up, bytes;
+};
+DistillPlan distill_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
+  DistillPlan p{};
+  p.loss = backward_plan(rows, vocab, hidden);
+  const uint64_t each = padded((uint64_t)rows * 4);
+  p.live = p.loss.bytes;
+  p.norm = p.live + each;
+  p.total = p.norm + each;
+  p.shift = p.total + each;
+  p.up = p.shift + each;
+  p.bytes = p.up + each;
+  return p;
+}
+
+}  // namespace
+
+uint64_t LmHeadDistillWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden) {
+  if (!shape_ok(rows, vocab, hidden)) return 0;
+  return padded((uint64_t)rows * stat_tiles(vocab, hidden) * 8);
+}
+
+uint64_t LmHeadDistillBackwardWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden) {
+  return shape_ok(rows, vocab, hidden) ? distill_plan(rows, vocab, hidden).bytes : 0;
+}
+
+St LaunchLmHeadDistill(const LmHeadDistillArgs& a) {
+  if (!a.x || !a.w || !a.ids || !a.teacher || !a.loss || !a.lse || !a.logits || !a.workspace || !a.error_flag ||
+      !a.stream)
+    return Invalid("lm_head_distill_null_argument");
+  if (!distill_ok(a)) return Invalid("lm_head_distill_shape_invalid");
+  if (!temperature_ok(a.temperature)) return Invalid("lm_head_distill_temperature_invalid");
+  if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.ids, 4) || !aligned(a.teacher, 4) ||
+      !aligned(a.teacher_lse, 4) || !aligned(a.loss, 4) || !aligned(a.lse, 4) || !aligned(a.logits, 4) ||
+      !aligned(a.error_flag, 4))
+    return Invalid("lm_head_distill_alignment_invalid");
+  // (the logits are written before the teacher's are read)
+  if (a.logits == a.teacher || (const void*)a.logits == a.ids || a.logits == a.teacher_lse)
+    return Invalid("lm_head_distill_alias_invalid");
+  if (a.workspace_bytes < LmHeadDistillWorkspaceBytes(a.rows, a.vocab, a.hidden) || !aligned(a.workspace, 16))
+    return Invalid("lm_head_distill_workspace_invalid");
+  St clean = RequireCleanLastError();
+  if (!clean.ok()) return clean;
+  const uint32_t tiles = stat_tiles(a.vocab, a.hidden);
+  float2* const stats = static_cast<float2*>(a.workspace);
+  if (big_takes(a.hidden)) {
+    BigArgs b{};
+    b.a = a.x;
+    b.b = a.w;
+    b.m = a.rows;
+    b.n = b.vocab = a.vocab;
+    b.k = a.hidden;
+    b.lda = b.ldb = a.hidden;
+    b.stats = stats;
+    b.exponent = kLog2e / a.temperature;
+    launch_big<false, false, kEpiTeacherStats>(b, a.stream);
+  } else {
+    GemmArgs g{};
+    g.a = a.x;
+    g.b = a.w;
+    g.m = a.rows;
+    g.n = g.vocab = a.vocab;
+    g.k = a.hidden;
+    g.lda = g.ldb = a.hidden;
+    g.stat_tiles = tiles;
+    g.stats = stats;
+    g.inverse = 1.0f / a.temperature;
+    launch_gemm<kEpiTeacherStats>(g, a.stream);
+  }
+  const uint64_t entries = (uint64_t)a.rows * a.top_k;
+  hipLaunchKernelGGL(distill_gather_kernel, dim3((uint32_t)std::min<uint64_t>((entries + 3) / 4, 1u << 20)), dim3(256), 0,
+                     a.stream, a.x, a.w, a.ids, a.logits, entries, a.top_k, a.vocab, a.hidden);
+  hipLaunchKernelGGL(distill_join_kernel, dim3((a.rows + 3) / 4), dim3(256), 0, a.stream, stats, a.ids, a.teacher,
+                     a.teacher_lse, a.logits, a.loss, a.lse, a.error_flag, a.rows, a.vocab, tiles, a.top_k,
+                     a.temperature);
+  return AfterLaunch("lm_head_distill_launch_failed");
+}
+
+St LaunchLmHeadDistillBackward(const LmHeadDistillArgs& a) {
+  if (!a.x || !a.w || !a.ids || !a.teacher || !a.lse || !a.logits || !a.loss_grad || !a.dx || !a.workspace ||
+      !a.error_flag || !a.stream)
+    return Invalid("lm_head_distill_backward_null_argument");
+  if (!distill_ok(a)) return Invalid("lm_head_distill_backward_shape_invalid");
+  if (!temperature_ok(a.temperature)) return Invalid("lm_head_distill_backward_temperature_invalid");
+  if (!aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.dx, 16) || !aligned(a.dw, 16) || !aligned(a.ids, 4) ||
+      !aligned(a.teacher, 4) || !aligned(a.teacher_lse, 4) || !aligned(a.lse, 4) || !aligned(a.logits, 4) ||
+      !aligned(a.loss_grad, 4) || !aligned(a.error_flag, 4))
+    return Invalid("lm_head_distill_backward_alignment_invalid");
+  // (the weights' gradient of a piece is written before dx reads its weights)
+  if (a.dw == a.w) return Invalid("lm_head_distill_backward_alias_invalid");
+  const DistillPlan plan = distill_plan(a.rows, a.vocab, a.hidden);
+  if (a.workspace_bytes < plan.bytes || !aligned(a.workspace, 16))
+    return Invalid("lm_head_distill_backward_workspace_invalid");
+  St clean = RequireCleanLastError();
+  if (!clean.ok()) return clean;
+  uint8_t* const ws = static_cast<uint8_t*>(a.workspace);
+  uint16_t* const grad = reinterpret_cast<uint16_t*>(ws + plan.loss.g);
+  float* const mantissa = reinterpret_cast<float*>(ws + plan.loss.mantissa);
+  const TeacherRows rows{reinterpret_cast<uint32_t*>(ws + plan.live), reinterpret_cast<float*>(ws + plan.norm),
+                         reinterpret_cast<float*>(ws + plan.total), reinterpret_cast<float*>(ws + plan.shift),
+                         reinterpret_cast<float*>(ws + plan.up)};
+  const dim3 row_grid((a.rows + 3) / 4);
+  hipLaunchKernelGGL(distill_teacher_kernel, row_grid, dim3(256), 0, a.stream, a.ids, a.teacher, a.teacher_lse, a.lse,
+                     a.loss_grad, rows, a.error_flag, a.rows, a.vocab, a.top_k, a.temperature);
+  BackwardCall call{};
+  call.x = a.x;
+  call.w = a.w;
+  call.target = rows.live;
+  call.lse = rows.shift;
+  call.up = rows.up;
+  call.dx = a.dx;
+  call.dw = a.dw;
+  call.error_flag = a.error_flag;
+  call.stream = a.stream;
+  call.rows = a.rows;
+  call.vocab = a.vocab;
+  call.hidden = a.hidden;
+  call.temperature = a.temperature;
+  launch_backward<kEpiTeacherGrad>(call, plan.loss, ws, [&](uint32_t v0, uint32_t cols) {
+    hipLaunchKernelGGL(distill_entries_kernel, row_grid, dim3(256), 0, a.stream, a.ids, a.teacher, a.logits, a.lse, rows,
+                       mantissa, grad, (uint64_t)plan.loss.piece, a.rows, a.vocab, a.top_k, v0, cols, a.temperature);
+  });
+  return AfterLaunch("lm_head_distill_backward_launch_failed");
+}
+
+}  // namespace pih_amd

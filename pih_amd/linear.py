@@ -719,3 +719,174 @@ def router_backward(scores: torch.Tensor, topk_ids: torch.Tensor, counts: Option
     _launch("launch_router_backward", "router_backward", ps, pi, pc, pl, pw, dscores.data_ptr(), pflag,
             stream_handle(), tokens, experts, topk, mode, coefficient, route_scale)
     return dscores, flag
+
+
+# ------------------- feed-forward block, distillation, drafted tokens
+def _mlp_inputs(x, w_gate, w_up, w_down):
+    _want(x.dim() == w_gate.dim() == w_down.dim() == 2 and
+          x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype == torch.bfloat16,
+          "the feed-forward block is x [rows, hidden] and three weights, bfloat16")
+    rows, hidden = x.shape
+    inter = w_gate.shape[0]
+    _want(w_gate.shape == w_up.shape == (inter, hidden) and w_down.shape == (hidden, inter),
+          "the block's weights are gate and up [intermediate, hidden] and down [hidden, intermediate]")
+    return rows, hidden, inter
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, limit: float = 0.0,
+              keep: bool = False, out: Optional[torch.Tensor] = None):
+    """The gated feed-forward block ``(silu(x . w_gate^T) * (x . w_up^T)) .
+    w_down^T`` (``launch_gated_mlp``): y bf16 [rows, hidden], or with
+    ``keep`` (y, gate, up) with the two projections' outputs bf16 [rows,
+    intermediate] that ``gated_mlp_backward`` takes.  ``limit`` above 0 clamps
+    the gate from above and up from both sides.  Unlike ``QwenMlpBlock``,
+    which issues the projections and the activation one by one as the
+    reference's model does, the activation takes its inputs in fp32."""
+    rows, hidden, inter = _mlp_inputs(x, w_gate, w_up, w_down)
+    if out is None:
+        out = torch.empty_like(x)
+    _want(out.shape == x.shape and out.dtype == torch.bfloat16, "the block's output is bfloat16 [rows, hidden]")
+    gate = up = None
+    if keep:
+        gate = torch.empty(rows, inter, dtype=torch.bfloat16, device=x.device)
+        up = torch.empty(rows, inter, dtype=torch.bfloat16, device=x.device)
+    px, pg, pu, pd, po = device_ptrs(x, w_gate, w_up, w_down, out)
+    ws = _workspace(abi.WORKSPACE_GATED_MLP, rows, inter, hidden, x.device)
+    _launch("launch_gated_mlp", "gated_mlp", px, pg, pu, pd, po, gate.data_ptr() if keep else 0,
+            up.data_ptr() if keep else 0, ws.data_ptr(), ws.numel(), stream_handle(), rows, hidden, inter, limit)
+    return (out, gate, up) if keep else out
+
+
+def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                       w_down: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, limit: float = 0.0,
+                       weight_gradients: bool = True):
+    """Gradients of ``gated_mlp`` for the upstream gradient ``dy`` of its
+    output (``launch_gated_mlp_backward``), with ``gate`` and ``up`` as it
+    kept them: (dx, dw_gate, dw_up, dw_down), bf16, the last three None
+    without ``weight_gradients`` (frozen weights)."""
+    rows, hidden, inter = _mlp_inputs(x, w_gate, w_up, w_down)
+    _want(dy.shape == x.shape and dy.dtype == torch.bfloat16, "the upstream gradient is bfloat16 [rows, hidden]")
+    _want(gate.shape == up.shape == (rows, inter) and gate.dtype == up.dtype == torch.bfloat16,
+          "gate and up are bfloat16 [rows, intermediate]")
+    py, px, pg, pu, pd, pa, pb = device_ptrs(dy, x, w_gate, w_up, w_down, gate, up)
+    dx = torch.empty_like(x)
+    grads = tuple(torch.empty_like(w) if weight_gradients else None for w in (w_gate, w_up, w_down))
+    ws = _workspace(abi.WORKSPACE_GATED_MLP_BACKWARD, rows, inter, hidden, x.device)
+    _launch("launch_gated_mlp_backward", "gated_mlp_backward", py, px, pg, pu, pd, pa, pb, dx.data_ptr(),
+            *(0 if g is None else g.data_ptr() for g in grads), ws.data_ptr(), ws.numel(), stream_handle(), rows,
+            hidden, inter, limit)
+    return (dx,) + grads
+
+
+def _teacher_inputs(x, weight, teacher_ids, teacher_logits, teacher_lse):
+    _want(x.dim() == 2 and weight.dim() == 2 and x.shape[1] == weight.shape[1] and
+          x.dtype == weight.dtype == torch.bfloat16, "the LM head is x [rows, hidden] . weight [vocab, hidden], bfloat16")
+    _want(teacher_ids.dim() == 2 and teacher_ids.shape[0] == x.shape[0] and teacher_ids.dtype == torch.int32 and
+          teacher_logits.shape == teacher_ids.shape and teacher_logits.dtype == torch.float32,
+          "the teacher's entries are ids int32 and logits float32 [rows, top_k]")
+    _want(teacher_lse is None or (teacher_lse.shape == x.shape[:1] and teacher_lse.dtype == torch.float32),
+          "teacher_lse is float32 [rows]")
+    return x.shape[0], weight.shape[0], x.shape[1], teacher_ids.shape[1]
+
+
+def lm_head_distill(x: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                    temperature: float = 1.0, teacher_lse: Optional[torch.Tensor] = None,
+                    flag: Optional[torch.Tensor] = None):
+    """Divergence of an LM head from a teacher's top logits, without the
+    head's own logits in memory (``launch_lm_head_distill``): (loss f32
+    [rows], lse f32 [rows], logits f32 [rows, top_k], flag).  ``loss`` is
+    ``temperature^2 * KL(teacher || head)`` of the softmaxes over
+    ``temperature``, the teacher's over its entries, or with ``teacher_lse``
+    (the log-sum-exp of all its logits over ``temperature``) over its whole
+    vocabulary, of which the entries' part is summed.  An id of -1 is no
+    entry; a row without entries has loss 0.  ``lse`` and ``logits`` (the
+    head's, at the entries) are what the backward pass needs."""
+    rows, vocab, hidden, top_k = _teacher_inputs(x, weight, teacher_ids, teacher_logits, teacher_lse)
+    loss = torch.empty(rows, dtype=torch.float32, device=x.device)
+    lse = torch.empty(rows, dtype=torch.float32, device=x.device)
+    logits = torch.empty(rows, top_k, dtype=torch.float32, device=x.device)
+    flag = error_flag() if flag is None else flag
+    px, pw, pi, pt, pl, pflag = device_ptrs(x, weight, teacher_ids, teacher_logits, teacher_lse, flag)
+    ws = _workspace(abi.WORKSPACE_LM_HEAD_DISTILL, rows, vocab, hidden, x.device)
+    _launch("launch_lm_head_distill", "lm_head_distill", px, pw, pi, pt, pl, loss.data_ptr(), lse.data_ptr(),
+            logits.data_ptr(), ws.data_ptr(), ws.numel(), pflag, stream_handle(), rows, vocab, hidden, top_k, temperature)
+    return loss, lse, logits, flag
+
+
+def lm_head_distill_backward(x: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
+                             teacher_logits: torch.Tensor, lse: torch.Tensor, logits: torch.Tensor,
+                             dloss: torch.Tensor, temperature: float = 1.0,
+                             teacher_lse: Optional[torch.Tensor] = None, weight_gradient: bool = True,
+                             flag: Optional[torch.Tensor] = None):
+    """Gradients of ``lm_head_distill`` for the losses' upstream gradient
+    ``dloss`` f32 [rows], from the ``lse`` and ``logits`` it returned
+    (``launch_lm_head_distill_backward``): (dx bf16 like ``x``, dweight bf16
+    like ``weight``, or None without ``weight_gradient``, flag)."""
+    rows, vocab, hidden, top_k = _teacher_inputs(x, weight, teacher_ids, teacher_logits, teacher_lse)
+    _want(lse.dtype == dloss.dtype == torch.float32 and lse.shape == dloss.shape == x.shape[:1],
+          "lse and dloss are float32 [rows]")
+    _want(logits.dtype == torch.float32 and logits.shape == teacher_ids.shape, "logits are float32 [rows, top_k]")
+    flag = error_flag() if flag is None else flag
+    px, pw, pi, pt, pl, pe, pz, pd, pflag = device_ptrs(x, weight, teacher_ids, teacher_logits, teacher_lse, lse,
+                                                        logits, dloss, flag)
+    dx = torch.empty_like(x)
+    dw = torch.empty_like(weight) if weight_gradient else None
+    ws = _workspace(abi.WORKSPACE_LM_HEAD_DISTILL_BACKWARD, rows, vocab, hidden, x.device)
+    _launch("launch_lm_head_distill_backward", "lm_head_distill_backward", px, pw, pi, pt, pl, pe, pz, pd, dx.data_ptr(),
+            0 if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel(), pflag, stream_handle(), rows, vocab, hidden,
+            top_k, temperature)
+    return dx, dw, flag
+
+
+def _logit_rows(t, rows: int, vocab: int, dtype, what: str):
+    """Address and row stride of logits whose rows are contiguous."""
+    if t.shape != (rows, vocab) or t.dtype is not dtype:
+        raise ValueError(f"pih_amd: {what} are {dtype} [{rows}, {vocab}]")
+    row, col = t.stride()
+    if col != 1 and vocab > 1:
+        raise ValueError("pih_amd: tensor rows must be contiguous")
+    return t.data_ptr(), row if rows > 1 else vocab
+
+
+def draft_verify(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft_offsets: torch.Tensor,
+                 accept_random: torch.Tensor, sample_random: torch.Tensor, max_drafts: int,
+                 draft_logits: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None,
+                 flag: Optional[torch.Tensor] = None):
+    """Drafted tokens of many sequences against the target model's logits
+    (``launch_draft_verify``): (tokens int32 [sequences, max_drafts + 1],
+    accepted int32 [sequences], flag).  Sequence s drafted
+    ``draft_tokens[draft_offsets[s]:draft_offsets[s + 1]]``, at most
+    ``max_drafts``; its rows of ``target_logits`` [drafts + sequences, vocab]
+    start at ``draft_offsets[s] + s``, one for each of them and one more.
+    ``draft_logits`` [drafts, vocab] are what the drafts were drawn from (None:
+    they were looked up); ``temperature`` f32 [sequences] (None: 1; 0: greedy)
+    holds for both models.  ``accept_random`` f32 [drafts] and
+    ``sample_random`` f32 [sequences] are uniform in [0, 1).  A row of
+    ``tokens`` holds the accepted tokens, the one that follows them, and -1.
+    Logits are float32 or bfloat16; their rows may be slices of wider ones."""
+    _want(target_logits.dim() == 2 and target_logits.dtype in (torch.float32, torch.bfloat16),
+          "logits are float32 or bfloat16 [rows, vocab]")
+    _want(draft_tokens.dim() == 1 and draft_offsets.dim() == 1 and draft_offsets.shape[0] > 1 and
+          draft_tokens.dtype == draft_offsets.dtype == torch.int32,
+          "drafted tokens are int32 [drafts], their offsets int32 [sequences + 1]")
+    drafts, sequences, vocab = draft_tokens.shape[0], draft_offsets.shape[0] - 1, target_logits.shape[1]
+    _want(accept_random.dtype == sample_random.dtype == torch.float32 and accept_random.shape == (drafts,) and
+          sample_random.shape == (sequences,), "random numbers are float32 [drafts] and [sequences]")
+    _want(temperature is None or (temperature.dtype == torch.float32 and temperature.shape == (sequences,)),
+          "temperatures are float32 [sequences]")
+    _want(max_drafts >= 0, "max_drafts is not negative")
+    pt, ts = _logit_rows(target_logits, drafts + sequences, vocab, target_logits.dtype, "the target's logits")
+    pd, ds = 0, 0
+    if draft_logits is not None and drafts:
+        pd, ds = _logit_rows(draft_logits, drafts, vocab, target_logits.dtype, "the draft model's logits")
+    dev = target_logits.device
+    tokens = torch.empty(sequences, max_drafts + 1, dtype=torch.int32, device=dev)
+    accepted = torch.empty(sequences, dtype=torch.int32, device=dev)
+    flag = error_flag() if flag is None else flag
+    same_device(target_logits, draft_logits)
+    pk, po, pa, ps, pm, pflag = device_ptrs(draft_tokens, draft_offsets, accept_random, sample_random, temperature, flag)
+    ws = _workspace(abi.WORKSPACE_DRAFT_VERIFY, sequences, max_drafts, vocab, dev)
+    _launch("launch_draft_verify", "draft_verify", pt, pd, pk, po, pa, ps, pm, tokens.data_ptr(), accepted.data_ptr(),
+            ws.data_ptr(), ws.numel(), pflag, stream_handle(), sequences, drafts, max_drafts, vocab, ts, ds,
+            abi.OUTPUT_F32 if target_logits.dtype == torch.float32 else abi.OUTPUT_BF16)
+    return tokens, accepted, flag
