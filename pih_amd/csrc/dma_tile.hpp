@@ -19,8 +19,14 @@ constexpr uint32_t kNoTarget = 0xffffffffu;
 // target's logit; kEpiGrad: the logits' gradient in bf16; kEpiBf16: a scaled
 // result in bf16; kEpiAdd: added to fp32 sums; kEpiTeacherStats, kEpiTeacherGrad: the
 // first two of logits over a temperature, without a target (whose part the
-// caller adds)
-enum : int { kEpiStats = 0, kEpiGrad = 1, kEpiBf16 = 2, kEpiAdd = 3, kEpiTeacherStats = 4, kEpiTeacherGrad = 5 };
+// caller adds).  The feed-forward block's: kEpiStore: bf16; kEpiSum: fp32, a plane
+// per split; kEpiGlu: two products side by side, gate and up, joined to h;
+// kEpiGluSum: the same two as kEpiSum; kEpiGluGrad: dh, joined with gate and up
+enum : int {
+  kEpiStats = 0, kEpiGrad = 1, kEpiBf16 = 2, kEpiAdd = 3, kEpiTeacherStats = 4, kEpiTeacherGrad = 5,
+  kEpiStore = 6, kEpiSum = 7, kEpiGlu = 8, kEpiGluSum = 9, kEpiGluGrad = 10
+};
+constexpr bool has_pair(int epi) { return epi == kEpiGlu || epi == kEpiGluSum; }
 constexpr bool has_stats(int epi) { return epi == kEpiStats || epi == kEpiTeacherStats; }
 constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherGrad; }
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -67,7 +73,44 @@ struct BigArgs {
   float* target_logit;
   uint32_t v0, vocab, first;
   float exponent;          // kEpiTeacher*: log2(e) / temperature
+  // the feed-forward block's products
+  const uint16_t* b2;      // kEpiGlu*: up's weights; kEpiStore, kEpiSum: B behind step b_steps
+  uint16_t* out2;          // kEpiStore: rows of the result from out_rows on
+  uint32_t a_valid;        // kEpiStore, columns layout of A: as k_valid
+  uint32_t b_steps, out_rows;
+  uint16_t* gate;          // kEpiGlu: written where not null; kEpiGluGrad: read; [m][n or n / 2]
+  uint16_t* up;
+  uint16_t* h;             // kEpiGluGrad: beside out, which has dgate and n columns on dup
+  uint64_t ldh;
+  float limit;
 };
+
+// With s the logistic function of g = min(gate, limit) and u the clamped up:
+// silu(g) = g s, silu'(g) = s + g s (1 - s).
+__device__ __forceinline__ float logistic(float g) {
+  // (g -> -inf: exp -> inf, 1 / inf = 0)
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
+}
+// (not fminf, which drops a NaN)
+__device__ __forceinline__ float at_most(float v, float limit) { return v > limit ? limit : v; }
+__device__ __forceinline__ float within(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
+__device__ __forceinline__ float activated(float gate, float up, float limit) {
+  const float g = at_most(gate, limit);
+  return g * logistic(g) * within(up, limit);
+}
+// from dh, gate and up: dgate, dup and h
+struct GluGrad {
+  float dgate, dup, h;
+};
+__device__ __forceinline__ GluGrad glu_grad(float dh, float gate, float up, float limit) {
+  const float g = at_most(gate, limit), u = within(up, limit), s = logistic(g), silu = g * s;
+  return {gate > limit ? 0.0f : dh * u * (s + silu * (1.0f - s)), up > limit || up < -limit ? 0.0f : dh * silu, silu * u};
+}
+// four bf16 values of a uint2
+__device__ __forceinline__ v4f bf16x4_to_f32(uint2 v) {
+  return v4f{bf16_bits_to_f32(v.x & 0xffffu), bf16_bits_to_f32(v.x >> 16), bf16_bits_to_f32(v.y & 0xffffu),
+             bf16_bits_to_f32(v.y >> 16)};
+}
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
@@ -139,6 +182,23 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   auto source = [&](auto T, const uint8_t* base, uint64_t ld, uint32_t step) __attribute__((always_inline)) {
     return uniform_ptr(base + (decltype(T)::value ? (uint64_t)step * KB * ld * 2 : (uint64_t)step * KB * 2));
   };
+  // B's part of a step: the feed-forward block's has two sources, gate's and up's
+  // weights, for alternate 16 rows of a tile (each wave's DMAs read one of them)
+  // or for the two halves of k
+  auto offset_b = [&](uint32_t i) __attribute__((always_inline)) {
+    if constexpr (has_pair(EPI)) {
+      const uint32_t r = 32 * i + 8 * wave + (lane >> 3), row = 16 * i + 8 * (wave & 1) + (lane >> 3);
+      return (uint32_t)((min(n0 / 2 + row, p.n / 2 - 1) - n0 / 2) * p.ldb * 2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+    } else {
+      return offset(std::bool_constant<BT>{}, i, n0, p.n, p.ldb);
+    }
+  };
+  auto source_b = [&](uint32_t step) __attribute__((always_inline)) {
+    if constexpr (BT && (EPI == kEpiStore || EPI == kEpiSum)) {
+      if (step >= p.b_steps) return source(std::true_type{}, reinterpret_cast<const uint8_t*>(p.b2), p.ldb, step - p.b_steps);
+    }
+    return source(std::bool_constant<BT>{}, base_b, p.ldb, step);
+  };
   constexpr std::bool_constant<AT> at{};
   constexpr std::bool_constant<BT> bt{};
   // DMA i of a step (A's first) into buffer s
@@ -146,7 +206,14 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
                    uint32_t step) __attribute__((always_inline)) {
     const uint32_t lds = lds0 + s * S::kStage + wave * 1024;
     if (i < (uint32_t)LA) {
-      dma16(sa, off_a[i], lds + i * 4096);
+      uint32_t oa = off_a[i];
+      if constexpr (AT && EPI == kEpiStore) {
+        if ((step + 1) * KB > p.a_valid) {
+          const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.a_valid - 1 - step * KB;
+          if (r > last) oa -= (uint32_t)((r - last) * p.lda * 2);
+        }
+      }
+      dma16(sa, oa, lds + i * 4096);
     } else {
       i -= LA;
       uint32_t ob = off_b[i];
@@ -177,16 +244,17 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     s0 = min(split * per_split, all_steps);
     steps = min(s0 + per_split, all_steps) - s0;
     base_a = reinterpret_cast<const uint8_t*>(AT ? p.a : p.a + m0 * p.lda);
-    base_b = reinterpret_cast<const uint8_t*>(BT ? p.b : p.b + n0 * p.ldb);
+    if constexpr (has_pair(EPI)) base_b = reinterpret_cast<const uint8_t*>((wave & 2 ? p.b2 : p.b) + n0 / 2 * p.ldb);
+    else base_b = reinterpret_cast<const uint8_t*>(BT ? p.b : p.b + n0 * p.ldb);
 #pragma unroll
     for (uint32_t i = 0; i < (uint32_t)LA; ++i) off_a[i] = offset(at, i, m0, p.m, p.lda);
 #pragma unroll
-    for (uint32_t i = 0; i < (uint32_t)LB; ++i) off_b[i] = offset(bt, i, n0, p.n, p.ldb);
+    for (uint32_t i = 0; i < (uint32_t)LB; ++i) off_b[i] = offset_b(i);
 #pragma unroll
     for (uint32_t q = 0; q < (uint32_t)ST; ++q) {
       if (q >= steps) break;
       const uint8_t* sa = source(at, base_a, p.lda, s0 + q);
-      const uint8_t* sb = source(bt, base_b, p.ldb, s0 + q);
+      const uint8_t* sb = source_b(s0 + q);
       const bool short_b = BT && (s0 + q + 1) * KB > p.k_valid;
 #pragma unroll
       for (uint32_t i = 0; i < (uint32_t)NL; ++i) issue(sa, sb, q, i, short_b, s0 + q);
@@ -267,7 +335,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     const uint8_t* sb = nullptr;
     if constexpr (kMore) {
       sa = source(at, base_a, p.lda, step);
-      sb = source(bt, base_b, p.ldb, step);
+      sb = source_b(step);
     }
 #pragma unroll
     for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
@@ -392,7 +460,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         }
         p.stats[(uint64_t)(cm + tid) * p.n_tiles + cn / TB] = float2{top, sum};
       }
-    } else if constexpr (EPI == kEpiAdd) {
+    } else if constexpr (EPI == kEpiAdd || EPI == kEpiSum || EPI == kEpiGluSum) {
       float* const out = static_cast<float*>(p.out) + csplit * p.split_stride + wcol + 4 * lg;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -402,7 +470,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           before[j] = v4f{0.f, 0.f, 0.f, 0.f};
-          if (!p.first && wcol + 16 * j + 4 * lg < p.n) before[j] = o[4 * j];
+          if (EPI == kEpiAdd && !p.first && wcol + 16 * j + 4 * lg < p.n) before[j] = o[4 * j];
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -410,6 +478,99 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         // (16 rows at a time: registers for no more)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
+      }
+    } else if constexpr (EPI == kEpiStore || EPI == kEpiGlu || EPI == kEpiGluGrad) {
+      // 16 rows of BLOCKS 16-column blocks in bf16 through the wave's own LDS,
+      // so that a store instruction writes whole lines
+      uint8_t* const st = smem + S::kOut + wave * S::kOutRows * S::kOutRow;
+      auto put = [&](auto BLOCKS, auto&& value, auto&& row_at, uint32_t row0, uint32_t col0, uint32_t rows,
+                     uint32_t cols) __attribute__((always_inline)) {
+        constexpr uint32_t kBlocks = decltype(BLOCKS)::value, kLanes = 2 * kBlocks;
+        constexpr uint32_t kRowsAt = 64 / kLanes < S::kOutRows ? 64 / kLanes : S::kOutRows;
+#pragma unroll
+        for (uint32_t r0 = 0; r0 < 16; r0 += S::kOutRows) {
+          if (lr - r0 < S::kOutRows) {
+#pragma unroll
+            for (uint32_t j = 0; j < kBlocks; ++j) {
+              const v4f v = value(j);
+              *reinterpret_cast<uint2*>(st + (lr - r0) * S::kOutRow + j * 32 + lg * 8) =
+                  uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+            }
+          }
+          wave_lds_order();
+#pragma unroll
+          for (uint32_t h = 0; h < S::kOutRows / kRowsAt; ++h) {
+            const uint32_t q = kRowsAt * h + lane / kLanes, r = row0 + r0 + q, c = col0 + 8 * (lane % kLanes);
+            if (lane / kLanes >= kRowsAt) continue;
+            const v4i o = *reinterpret_cast<const v4i*>(st + q * S::kOutRow + lane % kLanes * 16);
+            if (r < rows && c < cols) *reinterpret_cast<v4i*>(row_at(r) + c) = o;
+          }
+          wave_lds_order();
+        }
+      };
+      if constexpr (EPI == kEpiStore) {
+        uint16_t* const out = static_cast<uint16_t*>(p.out);
+        auto row_at = [&](uint32_t r) {
+          return r < p.out_rows ? out + (uint64_t)r * p.ldo : p.out2 + (uint64_t)(r - p.out_rows) * p.ldo;
+        };
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+          put(std::integral_constant<int, NB>{}, [&](uint32_t j) { return acc[i][j]; }, row_at, wrow + 16 * i, wcol, p.m,
+              p.n);
+      } else if constexpr (EPI == kEpiGlu) {
+        constexpr std::integral_constant<int, NB / 2> half;
+        const uint32_t gcol = wcol / 2, cols = p.n / 2;
+        auto plane = [&](uint16_t* base) { return [&, base](uint32_t r) { return base + (uint64_t)r * p.ldo; }; };
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          if (p.gate) {
+            put(half, [&](uint32_t j) { return acc[i][2 * j]; }, plane(p.gate), wrow + 16 * i, gcol, p.m, cols);
+            put(half, [&](uint32_t j) { return acc[i][2 * j + 1]; }, plane(p.up), wrow + 16 * i, gcol, p.m, cols);
+          }
+          put(half, [&](uint32_t j) {
+            v4f h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = activated(acc[i][2 * j][e], acc[i][2 * j + 1][e], p.limit);
+            return h;
+          }, plane(static_cast<uint16_t*>(p.out)), wrow + 16 * i, gcol, p.m, cols);
+        }
+      } else {
+        // (the rows up to a multiple of 64 are written as zeros: the weights'
+        // gradients read them)
+        const uint32_t rows = (p.m + 63) / 64 * 64;
+        constexpr std::integral_constant<int, NB> all;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const uint32_t row = wrow + 16 * i + lr;
+          const uint64_t at_row = (uint64_t)min(row, p.m - 1) * p.n;
+          uint2 gate[NB], up[NB];
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            const uint64_t from = at_row + min(wcol + 16 * j + 4 * lg, p.n - 4);
+            gate[j] = *reinterpret_cast<const uint2*>(p.gate + from);
+            up[j] = *reinterpret_cast<const uint2*>(p.up + from);
+          }
+          v4f du[NB], h[NB];
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            const v4f g = bf16x4_to_f32(gate[j]), u = bf16x4_to_f32(up[j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              GluGrad d = glu_grad(acc[i][j][e], g[e], u[e], p.limit);
+              if (row >= p.m) d = GluGrad{0.0f, 0.0f, 0.0f};
+              acc[i][j][e] = d.dgate;
+              du[j][e] = d.dup;
+              h[j][e] = d.h;
+            }
+          }
+          uint16_t* const out = static_cast<uint16_t*>(p.out);
+          put(all, [&](uint32_t j) { return acc[i][j]; }, [&](uint32_t r) { return out + (uint64_t)r * p.ldo; },
+              wrow + 16 * i, wcol, rows, p.n);
+          put(all, [&](uint32_t j) { return du[j]; }, [&](uint32_t r) { return out + (uint64_t)r * p.ldo + p.n; },
+              wrow + 16 * i, wcol, rows, p.n);
+          put(all, [&](uint32_t j) { return h[j]; }, [&](uint32_t r) { return p.h + (uint64_t)r * p.ldh; }, wrow + 16 * i,
+              wcol, rows, p.n);
+        }
       }
     } else {
       // bf16 through the wave's own LDS, 16 or 8 rows at a time, so that a store

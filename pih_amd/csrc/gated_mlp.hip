@@ -9,28 +9,11 @@
 // element at most, independent from element to element, in sums that are
 // rounded to bf16 once themselves.  gate, up and dh stay in fp32 between
 // their product and the activation.
-#include <algorithm>
-
-#include "kernels.hpp"
+#include "dma_tile.hpp"
 #include "tile64.hpp"
 
 namespace pih_amd {
 namespace {
-
-// With s the logistic function of g = min(gate, limit) and u the clamped up:
-// silu(g) = g s, silu'(g) = s + g s (1 - s).
-__device__ __forceinline__ float logistic(float g) {
-  // (g -> -inf: exp -> inf, 1 / inf = 0)
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g));
-}
-// (not fminf, which drops a NaN)
-__device__ __forceinline__ float at_most(float v, float limit) { return v > limit ? limit : v; }
-__device__ __forceinline__ float within(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
-
-__device__ __forceinline__ float activated(float gate, float up, float limit) {
-  const float g = at_most(gate, limit);
-  return g * logistic(g) * within(up, limit);
-}
 
 struct MlpArgs {
   const uint16_t* a;
@@ -89,21 +72,164 @@ __global__ __launch_bounds__(256) void mlp_dh64_kernel(MlpArgs p) {
   each64(m0, n0, [&](uint32_t r, uint32_t c, int i, int j) {
     if (r >= p.m || c >= p.n) return;
     const uint64_t at = (uint64_t)r * p.n + c;
-    const uint2 gw = *reinterpret_cast<const uint2*>(p.gate + at), uw = *reinterpret_cast<const uint2*>(p.up + at);
+    const v4f gate = bf16x4_to_f32(*reinterpret_cast<const uint2*>(p.gate + at));
+    const v4f up = bf16x4_to_f32(*reinterpret_cast<const uint2*>(p.up + at));
     v4f dg, du, h;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float gate = bf16_bits_to_f32(((e < 2 ? gw.x : gw.y) >> (16 * (e & 1))) & 0xffffu);
-      const float up = bf16_bits_to_f32(((e < 2 ? uw.x : uw.y) >> (16 * (e & 1))) & 0xffffu);
-      const float g = at_most(gate, p.limit), u = within(up, p.limit), s = logistic(g), silu = g * s, d = dh[i][j][e];
-      dg[e] = gate > p.limit ? 0.0f : d * u * (s + silu * (1.0f - s));
-      du[e] = up > p.limit || up < -p.limit ? 0.0f : d * silu;
-      h[e] = silu * u;
+      const GluGrad d = glu_grad(dh[i][j][e], gate[e], up[e], p.limit);
+      dg[e] = d.dgate;
+      du[e] = d.dup;
+      h[e] = d.h;
     }
     *reinterpret_cast<uint2*>(p.dgate + at) = bf16x4(dg);
     *reinterpret_cast<uint2*>(p.dup + at) = bf16x4(du);
     *reinterpret_cast<uint2*>(p.out + at) = bf16x4(h);
   });
+}
+
+// ------------------------------------------- products split over k
+// A product with too few tiles for the CUs leaves fp32 sums, a plane per split,
+// which these join in order.
+
+// h, and gate and up where they are kept: the sums' columns are 16 of gate and 16
+// of up in turn
+__global__ __launch_bounds__(256) void mlp_join_glu_kernel(const float* sums, uint32_t splits, uint64_t plane,
+                                                           uint16_t* h, uint16_t* gate, uint16_t* up, uint64_t count,
+                                                           uint32_t inter, float limit) {
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (uint64_t)gridDim.x * 1024) {
+    const uint32_t c = (uint32_t)(i % inter);
+    const float* const from = sums + i / inter * (2 * (uint64_t)inter) + c / 16 * 32 + c % 16;
+    v4f g = *reinterpret_cast<const v4f*>(from), u = *reinterpret_cast<const v4f*>(from + 16);
+#pragma unroll 4
+    for (uint32_t s = 1; s < splits; ++s) {
+      g += *reinterpret_cast<const v4f*>(from + s * plane);
+      u += *reinterpret_cast<const v4f*>(from + s * plane + 16);
+    }
+    v4f v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = activated(g[e], u[e], limit);
+    *reinterpret_cast<uint2*>(h + i) = bf16x4(v);
+    if (gate) {
+      *reinterpret_cast<uint2*>(gate + i) = bf16x4(g);
+      *reinterpret_cast<uint2*>(up + i) = bf16x4(u);
+    }
+  }
+}
+
+// dgate, dup (side by side, rows 2 inter long) and h of dh; zeros for the rows
+// from count / inter up to a multiple of 64
+__global__ __launch_bounds__(256) void mlp_join_dh_kernel(const float* sums, uint32_t splits, uint64_t plane,
+                                                          const uint16_t* gate, const uint16_t* up, uint16_t* dgu,
+                                                          uint16_t* h, uint64_t count, uint64_t padded, uint32_t inter,
+                                                          float limit) {
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < padded; i += (uint64_t)gridDim.x * 1024) {
+    v4f dg{0.f, 0.f, 0.f, 0.f}, du = dg, v = dg;
+    if (i < count) {
+      v4f dh = *reinterpret_cast<const v4f*>(sums + i);
+#pragma unroll 4
+      for (uint32_t s = 1; s < splits; ++s) dh += *reinterpret_cast<const v4f*>(sums + s * plane + i);
+      const v4f g = bf16x4_to_f32(*reinterpret_cast<const uint2*>(gate + i));
+      const v4f u = bf16x4_to_f32(*reinterpret_cast<const uint2*>(up + i));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const GluGrad d = glu_grad(dh[e], g[e], u[e], limit);
+        dg[e] = d.dgate;
+        du[e] = d.dup;
+        v[e] = d.h;
+      }
+    }
+    uint16_t* const row = dgu + i / inter * (2 * (uint64_t)inter) + i % inter;
+    *reinterpret_cast<uint2*>(row) = bf16x4(dg);
+    *reinterpret_cast<uint2*>(row + inter) = bf16x4(du);
+    *reinterpret_cast<uint2*>(h + i) = bf16x4(v);
+  }
+}
+
+__global__ __launch_bounds__(256) void mlp_join_kernel(const float* sums, uint32_t splits, uint64_t plane, uint16_t* out,
+                                                       uint64_t count) {
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (uint64_t)gridDim.x * 1024) {
+    v4f v = *reinterpret_cast<const v4f*>(sums + i);
+#pragma unroll 4
+    for (uint32_t s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(sums + s * plane + i);
+    *reinterpret_cast<uint2*>(out + i) = bf16x4(v);
+  }
+}
+dim3 join_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 16)); }
+
+// ------------------------------------------- which tiles
+// How the rows of a product [m][n] over k run: tiles of `rows` rows, k in
+// `splits` parts.  Time (us): the rounds of tiles on the CUs, each its beginning
+// and end and a step's time (rows_cost in dma_tile.hpp), and for splits the sums
+// written and read at 4 TB/s and a launch.
+struct Tiling {
+  uint32_t rows, splits;
+  float us;
+};
+Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
+  BigArgs p{};
+  p.n = n;
+  p.k = k;
+  Tiling best{256, 1, INFINITY};
+  for (uint32_t rows : {256u, 128u, 64u})
+    for (uint32_t splits = 1; splits <= 16 && k / KB / splits >= 4; ++splits) {
+      // (no split is empty)
+      const uint32_t steps = k / KB, part = (steps + splits - 1) / splits;
+      if ((steps + part - 1) / part != splits) continue;
+      p.splits = splits;
+      const float us = rows_cost(p, m, rows) + (splits > 1 ? 4.0f + (float)splits * m * n * (8.0f / 4.0e6f) : 0.0f);
+      if (us < best.us) best = {rows, splits, us};
+    }
+  return best;
+}
+// All rows alike, or the whole 256 without splits and the rest by itself, where B
+// is read once more (at 5 TB/s) and the launch costs 3 us
+struct Route {
+  uint32_t whole;  // rows in tiles of 256, unsplit
+  Tiling rest;     // of those behind
+  uint64_t sums;   // fp32 elements
+};
+Route route_of(uint32_t m, uint32_t n, uint32_t k) {
+  const Tiling all = tiling_of(m, n, k);
+  const uint32_t whole = m / 256 * 256, rest = m - whole;
+  Route r{0, all, all.splits > 1 ? (uint64_t)all.splits * m * n : 0};
+  if (whole && rest) {
+    BigArgs p{};
+    p.n = n;
+    p.k = k;
+    const Tiling last = tiling_of(rest, n, k);
+    const float again = std::max(last.us, (float)n * k * (2.0f / 5.0e6f)) + 3.0f;
+    if (rows_cost(p, whole, 256) + again < all.us) r = {whole, last, last.splits > 1 ? (uint64_t)last.splits * rest * n : 0};
+  }
+  return r;
+}
+// EPI for the rows in one part, SUM and join(sums, first row, rows, splits,
+// elements of a plane) for those in several
+template <bool BT, int EPI, int SUM, typename A, typename J>
+void run_route(const Route& r, BigArgs p, float* sums, hipStream_t s, A&& advance, J&& join) {
+  const uint32_t m = p.m;
+  p.splits = 1;
+  if (r.whole) {
+    p.m = r.whole;
+    launch_rows<256, false, BT, EPI>(p, s);
+    if (r.whole == m) return;
+    advance(p, r.whole);
+    p.m = m - r.whole;
+  }
+  if (r.rest.splits > 1) {
+    p.splits = r.rest.splits;
+    p.split_stride = (uint64_t)p.m * p.n;
+    p.out = sums;
+    p.ldo = p.n;
+    if (r.rest.rows == 64) launch_rows<64, false, BT, SUM>(p, s);
+    else if (r.rest.rows == 128) launch_rows<128, false, BT, SUM>(p, s);
+    else launch_rows<256, false, BT, SUM>(p, s);
+    join(r.whole, p.m, p.splits, p.split_stride);
+  } else {
+    if (r.rest.rows == 64) launch_rows<64, false, BT, EPI>(p, s);
+    else if (r.rest.rows == 128) launch_rows<128, false, BT, EPI>(p, s);
+    else launch_rows<256, false, BT, EPI>(p, s);
+  }
 }
 
 bool shape_ok(uint32_t rows, uint32_t inter, uint32_t hidden) {
@@ -113,6 +239,37 @@ bool shape_ok(uint32_t rows, uint32_t inter, uint32_t hidden) {
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 dim3 tiles64(uint32_t m, uint32_t n) { return dim3((n + kT64 - 1) / kT64, (m + kT64 - 1) / kT64); }
+// the tiles fed by DMA take 64-deep steps of every product
+bool dma_takes(uint32_t inter, uint32_t hidden) { return inter % KB == 0 && hidden % KB == 0; }
+struct ForwardPlan {
+  Route up, down;
+  uint64_t sums, bytes;
+};
+ForwardPlan forward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
+  ForwardPlan p{};
+  p.sums = padded((uint64_t)rows * inter * 2);
+  p.bytes = p.sums;
+  if (!dma_takes(inter, hidden)) return p;
+  p.up = route_of(rows, 2 * inter, hidden);
+  p.down = route_of(rows, hidden, inter);
+  p.bytes += padded(std::max(p.up.sums, p.down.sums) * 4);
+  return p;
+}
+struct BackwardPlan {
+  Route dh, dx;
+  uint64_t h, sums, bytes;
+};
+BackwardPlan backward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
+  BackwardPlan p{};
+  const uint64_t plane = (uint64_t)(rows + 63) / 64 * 64 * inter * 2;
+  p.h = padded(2 * plane);
+  p.bytes = p.sums = p.h + padded(plane);
+  if (!dma_takes(inter, hidden)) return p;
+  p.dh = route_of(rows, inter, hidden);
+  p.dx = route_of(rows, hidden, 2 * inter);
+  p.bytes += padded(std::max(p.dh.sums, p.dx.sums) * 4);
+  return p;
+}
 // (a clamp that nothing passes; infinities stay what they are)
 float limit_of(const GatedMlpArgs& a) { return a.limit > 0.0f ? a.limit : INFINITY; }
 
@@ -120,12 +277,12 @@ float limit_of(const GatedMlpArgs& a) { return a.limit > 0.0f ? a.limit : INFINI
 
 uint64_t GatedMlpWorkspaceBytes(uint32_t rows, uint32_t inter, uint32_t hidden) {
   if (!shape_ok(rows, inter, hidden)) return 0;
-  return padded((uint64_t)rows * inter * 2);
+  return forward_plan(rows, inter, hidden).bytes;
 }
 
 uint64_t GatedMlpBackwardWorkspaceBytes(uint32_t rows, uint32_t inter, uint32_t hidden) {
   if (!shape_ok(rows, inter, hidden)) return 0;
-  return 3 * padded((uint64_t)rows * inter * 2);
+  return backward_plan(rows, inter, hidden).bytes;
 }
 
 St LaunchGatedMlp(const GatedMlpArgs& a) {
@@ -142,6 +299,62 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
     return Invalid("gated_mlp_alias_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
+  const ForwardPlan plan = forward_plan(a.rows, a.inter, a.hidden);
+  uint16_t* const h = static_cast<uint16_t*>(a.workspace);
+  if (dma_takes(a.inter, a.hidden)) {
+    float* const sums = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + plan.sums);
+    BigArgs p{};
+    p.a = a.x;
+    p.b = a.wg;
+    p.b2 = a.wu;
+    p.m = a.rows;
+    p.n = 2 * a.inter;
+    p.k = p.k_valid = a.hidden;
+    p.lda = p.ldb = a.hidden;
+    p.out = h;
+    p.ldo = a.inter;
+    p.gate = a.gate;
+    p.up = a.up;
+    p.limit = limit_of(a);
+    run_route<false, kEpiGlu, kEpiGluSum>(
+        plan.up, p, sums, a.stream,
+        [&](BigArgs& q, uint32_t rows) {
+          q.a += (uint64_t)rows * a.hidden;
+          q.out = h + (uint64_t)rows * a.inter;
+          if (a.gate) {
+            q.gate += (uint64_t)rows * a.inter;
+            q.up += (uint64_t)rows * a.inter;
+          }
+        },
+        [&](uint32_t first, uint32_t rows, uint32_t splits, uint64_t plane) {
+          const uint64_t from = (uint64_t)first * a.inter, count = (uint64_t)rows * a.inter;
+          hipLaunchKernelGGL(mlp_join_glu_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane, h + from,
+                             a.gate ? a.gate + from : nullptr, a.up ? a.up + from : nullptr, count, a.inter, p.limit);
+        });
+    BigArgs q{};
+    q.a = h;
+    q.b = a.wd;
+    q.m = a.rows;
+    q.n = a.hidden;
+    q.out_rows = a.rows;
+    q.k = q.k_valid = a.inter;
+    q.lda = q.ldb = a.inter;
+    q.out = a.y;
+    q.ldo = a.hidden;
+    q.b_steps = 0xffffffffu;
+    run_route<false, kEpiStore, kEpiSum>(
+        plan.down, q, sums, a.stream,
+        [&](BigArgs& r, uint32_t rows) {
+          r.a += (uint64_t)rows * a.inter;
+          r.out = a.y + (uint64_t)rows * a.hidden;
+        },
+        [&](uint32_t first, uint32_t rows, uint32_t splits, uint64_t plane) {
+          const uint64_t count = (uint64_t)rows * a.hidden;
+          hipLaunchKernelGGL(mlp_join_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane,
+                             a.y + (uint64_t)first * a.hidden, count);
+        });
+    return AfterLaunch("gated_mlp_launch_failed");
+  }
   MlpArgs p{};
   p.a = a.x;
   p.b = a.wg;
@@ -149,7 +362,7 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
   p.m = a.rows;
   p.n = a.inter;
   p.k = a.hidden;
-  p.out = static_cast<uint16_t*>(a.workspace);
+  p.out = h;
   p.gate = a.gate;
   p.up = a.up;
   p.limit = limit_of(a);
@@ -186,11 +399,96 @@ St LaunchGatedMlpBackward(const GatedMlpArgs& a) {
     return Invalid("gated_mlp_backward_workspace_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
+  const BackwardPlan plan = backward_plan(a.rows, a.inter, a.hidden);
   uint8_t* const ws = static_cast<uint8_t*>(a.workspace);
-  const uint64_t plane = padded((uint64_t)a.rows * a.inter * 2);
+  uint16_t* const h = reinterpret_cast<uint16_t*>(ws + plan.h);
+  if (dma_takes(a.inter, a.hidden)) {
+    uint16_t* const dgu = reinterpret_cast<uint16_t*>(ws);  // [rows up to a multiple of 64][dgate, dup]
+    float* const sums = reinterpret_cast<float*>(ws + plan.sums);
+    const uint32_t row_up = (a.rows + 63) / 64 * 64;
+    BigArgs p{};
+    p.a = a.dy;
+    p.b = a.wd;
+    p.m = a.rows;
+    p.n = a.inter;
+    p.k = p.k_valid = a.hidden;
+    p.lda = a.hidden;
+    p.ldb = a.inter;
+    p.out = dgu;
+    p.ldo = 2 * a.inter;
+    p.h = h;
+    p.ldh = a.inter;
+    p.gate = a.gate;
+    p.up = a.up;
+    p.b_steps = 0xffffffffu;
+    p.limit = limit_of(a);
+    run_route<true, kEpiGluGrad, kEpiSum>(
+        plan.dh, p, sums, a.stream,
+        [&](BigArgs& q, uint32_t rows) {
+          q.a += (uint64_t)rows * a.hidden;
+          q.out = dgu + (uint64_t)rows * 2 * a.inter;
+          q.h += (uint64_t)rows * a.inter;
+          q.gate += (uint64_t)rows * a.inter;
+          q.up += (uint64_t)rows * a.inter;
+        },
+        [&](uint32_t first, uint32_t rows, uint32_t splits, uint64_t plane) {
+          const uint64_t from = (uint64_t)first * a.inter, count = (uint64_t)rows * a.inter;
+          const uint64_t up_to = (uint64_t)(row_up - first) * a.inter;
+          hipLaunchKernelGGL(mlp_join_dh_kernel, join_grid(up_to), dim3(256), 0, a.stream, sums, splits, plane,
+                             a.gate + from, a.up + from, dgu + 2 * from, h + from, count, up_to, a.inter, p.limit);
+        });
+    if (a.dx) {
+      BigArgs q{};
+      q.a = dgu;
+      q.b = a.wg;
+      q.b2 = a.wu;
+      q.b_steps = a.inter / KB;
+      q.m = q.out_rows = a.rows;
+      q.n = a.hidden;
+      q.k = q.k_valid = 2 * a.inter;
+      q.lda = 2 * a.inter;
+      q.ldb = a.hidden;
+      q.out = a.dx;
+      q.ldo = a.hidden;
+      run_route<true, kEpiStore, kEpiSum>(
+          plan.dx, q, sums, a.stream,
+          [&](BigArgs& r, uint32_t rows) {
+            r.a += (uint64_t)rows * 2 * a.inter;
+            r.out = a.dx + (uint64_t)rows * a.hidden;
+          },
+          [&](uint32_t first, uint32_t rows, uint32_t splits, uint64_t plane) {
+            const uint64_t count = (uint64_t)rows * a.hidden;
+            hipLaunchKernelGGL(mlp_join_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane,
+                               a.dx + (uint64_t)first * a.hidden, count);
+          });
+    }
+    // the weights' gradients, columns of A against columns of B over the rows
+    auto weight = [&](const uint16_t* from, uint32_t ld, uint32_t from_valid, uint32_t m, const uint16_t* with,
+                      uint32_t with_valid, uint32_t n, uint16_t* out, uint16_t* out2, uint32_t out_rows) {
+      BigArgs q{};
+      q.a = from;
+      q.b = with;
+      q.m = m;
+      q.n = n;
+      q.k = row_up;
+      q.a_valid = from_valid;
+      q.k_valid = with_valid;
+      q.lda = ld;
+      q.ldb = q.ldo = n;
+      q.out = out;
+      q.out2 = out2;
+      q.out_rows = out_rows;
+      q.b_steps = 0xffffffffu;
+      launch_rows<256, true, true, kEpiStore>(q, a.stream);
+    };
+    if (a.dwg && a.dwu) weight(dgu, 2 * a.inter, row_up, 2 * a.inter, a.x, a.rows, a.hidden, a.dwg, a.dwu, a.inter);
+    else if (a.dwg) weight(dgu, 2 * a.inter, row_up, a.inter, a.x, a.rows, a.hidden, a.dwg, nullptr, a.inter);
+    else if (a.dwu) weight(dgu + a.inter, 2 * a.inter, row_up, a.inter, a.x, a.rows, a.hidden, a.dwu, nullptr, a.inter);
+    if (a.dwd) weight(a.dy, a.hidden, a.rows, a.hidden, h, row_up, a.inter, a.dwd, nullptr, a.hidden);
+    return AfterLaunch("gated_mlp_backward_launch_failed");
+  }
   uint16_t* const dgate = reinterpret_cast<uint16_t*>(ws);
-  uint16_t* const dup = reinterpret_cast<uint16_t*>(ws + plane);
-  uint16_t* const h = reinterpret_cast<uint16_t*>(ws + 2 * plane);
+  uint16_t* const dup = dgate + (uint64_t)a.rows * a.inter;
   MlpArgs p{};
   p.a = a.dy;
   p.b = a.wd;
