@@ -159,6 +159,8 @@ __device__ __forceinline__ void store_nonfinite(const TileParams& p, uint32_t ro
 __device__ __forceinline__ void raise(const TileParams& p, uint32_t bad) {
   const uint32_t bits = ((bad & kErrCode) ? p.err_code : 0u) | ((bad & kErrScale) ? p.err_scale : 0u) |
                         ((bad & kErrNonFinite) ? p.err_nonfinite : 0u);
+  // (no bits: no flag either, in a call that reports nothing)
+  if (!bits) return;
   // (the waves of a whole output may have the same to say: only one that
   // finds it unsaid adds to the queue at the flag)
   if (bits & ~__hip_atomic_load(p.err, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicOr(p.err, bits);
