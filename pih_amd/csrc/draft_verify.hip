@@ -14,7 +14,8 @@
 // Launches: the largest logit and the sum of exponentials of every row and
 // chunk of the vocabulary; a block per sequence that joins them and walks the
 // drafts; the chunks' sums of w at the rejected places; a block per sequence
-// that finds the chunk and in it the token.
+// that finds the chunk and in it the token.  (The last two in one, the token found
+// by the last of a sequence's blocks: 57 sequences 21 -> 24 us, 256 46 -> 58.)
 #include "device_common.hpp"
 #include "kernels.hpp"
 
@@ -36,9 +37,10 @@ struct Stat {
 struct Plan {
   double p_inverse, q_inverse, k;  // 1 / sums of the rows, log2(e) / T
   float p_top, q_top;
-  uint32_t place;   // of the target row, kNone: nothing to draw
-  uint32_t rejected;  // draft row `place` or token `without` is taken off
-  uint32_t without;   // looked-up drafts: the rejected token
+  uint32_t place;       // in the sequence, kNone: nothing to draw
+  uint32_t rejected;    // the draft row or token `without` is taken off
+  uint32_t without;     // looked-up drafts: the rejected token
+  uint32_t target_row, draft_row;
   uint32_t pad;
 };
 
@@ -60,43 +62,63 @@ struct VerifyArgs {
   uint32_t sequences, drafts, most, vocab, chunks, rows;
 };
 
-// 2^y for y <= 0 (below -1100: 0; a NaN stays one): 2^f of |f| <= 1/2 by its
-// Taylor polynomial of degree 11 in f ln 2 (6e-15 of it), times 2^n
-__device__ __forceinline__ double exp2_64(double y) {
-  y = y < -1100.0 ? -1100.0 : y;
-  const double n = __builtin_rint(y), t = (y - n) * 0.693147180559945309417;
-  double e = 1.0 / 39916800.0;
-  e = __builtin_fma(e, t, 1.0 / 3628800.0);
-  e = __builtin_fma(e, t, 1.0 / 362880.0);
-  e = __builtin_fma(e, t, 1.0 / 40320.0);
-  e = __builtin_fma(e, t, 1.0 / 5040.0);
-  e = __builtin_fma(e, t, 1.0 / 720.0);
-  e = __builtin_fma(e, t, 1.0 / 120.0);
-  e = __builtin_fma(e, t, 1.0 / 24.0);
-  e = __builtin_fma(e, t, 1.0 / 6.0);
-  e = __builtin_fma(e, t, 0.5);
-  e = __builtin_fma(e, t, 1.0);
-  e = __builtin_fma(e, t, 1.0);
-  return __builtin_amdgcn_ldexp(e, (int)n);
+// 2^y for y <= 0, 2^-1021 for all below that (and -inf): 2^f of |f| <= 1/2 by the
+// polynomial of degree 9 whose largest relative error, 1.4e-14, is least (Remez
+// exchange), times 2^n by an addition to the exponent; n = rint(y) by adding and
+// taking off 1.5 * 2^52, whose sum's lower word is n.  So all of it but the
+// conversion of y's float issues at the full rate, which rounding and ldexp do
+// not (16 exponentials a thread with those and degree 11: 194e6 logits in 202 us).
+// `lead`: lead_coefficient(), once for many
+__device__ __forceinline__ double lead_coefficient() {
+  double e = 0x1.b3f4221448a2ap-24;
+  asm("" : "+v"(e));  // (in registers: an FMA takes one constant from elsewhere)
+  return e;
 }
+__device__ __forceinline__ double exp2_64(double y, double lead) {
+  constexpr double kRound = 6755399441055744.0;
+  y = __builtin_fmax(y, -1021.0);
+  const double n = y + kRound, f = y - (n - kRound);
+  double e = __builtin_fma(lead, f, 0x1.63edf10ad3737p-20);
+  e = __builtin_fma(e, f, 0x1.ffce246029cbcp-17);
+  e = __builtin_fma(e, f, 0x1.43088fca94b5ep-13);
+  e = __builtin_fma(e, f, 0x1.5d87fd9012504p-10);
+  e = __builtin_fma(e, f, 0x1.3b2ab72a109c3p-7);
+  e = __builtin_fma(e, f, 0x1.c6b08d70d1fffp-5);
+  e = __builtin_fma(e, f, 0x1.ebfbdff81570dp-3);
+  e = __builtin_fma(e, f, 0x1.62e42fefa3752p-1);
+  e = __builtin_fma(e, f, 0x1.0000000000039p+0);
+  uint2 v = __builtin_bit_cast(uint2, e);
+  asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(v.y) : "v"(__builtin_bit_cast(uint2, n).x));
+  return __builtin_bit_cast(double, v);
+}
+// the same, and 0 below 2^-1021
+__device__ __forceinline__ double exp2_or_0(double y, double lead) { return y < -1021.0 ? 0.0 : exp2_64(y, lead); }
+__device__ __forceinline__ double exp2_or_0(double y) { return exp2_or_0(y, lead_coefficient()); }
 
-// 16 logits from column c on, -inf past the vocabulary
-template <bool BF16, bool WIDE>
-__device__ __forceinline__ void load16(float (&v)[16], const void* row, uint32_t c, uint32_t vocab) {
-  if (WIDE && c + 16 <= vocab) {
+// N logits from column c on, -inf past the vocabulary
+template <bool BF16, bool WIDE, int N>
+__device__ __forceinline__ void load_logits(float (&v)[N], const void* row, uint32_t c, uint32_t vocab) {
+  static_assert(N == 4 || N == 16, "a thread's logits");
+  if (WIDE && c + N <= vocab) {
     if constexpr (BF16) {
-      const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+      uint32_t w[N / 2];
+      if constexpr (N == 16) {
+        const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+        const uint4 x = p[0], y = p[1];
+        const uint32_t all[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 x = p[i];
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * i + e] = bf16_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+        for (int i = 0; i < N / 2; ++i) w[i] = all[i];
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + c);
+        w[0] = x.x;
+        w[1] = x.y;
       }
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = bf16_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
     } else {
       const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(row) + c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < N / 4; ++i) {
         const v4f x = p[i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * i + e] = x[e];
@@ -104,7 +126,7 @@ __device__ __forceinline__ void load16(float (&v)[16], const void* row, uint32_t
     }
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
+    for (uint32_t i = 0; i < N; ++i) {
       v[i] = -INFINITY;
       if (c + i < vocab)
         v[i] = BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[c + i]) : static_cast<const float*>(row)[c + i];
@@ -149,7 +171,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
                                    : row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + place);
   const uint32_t c = chunk * kChunk + threadIdx.x * kPer, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float v[kPer];
-  load16<BF16, WIDE>(v, row, c, p.vocab);
+  load_logits<BF16, WIDE>(v, row, c, p.vocab);
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < (int)kPer; ++i) top = fmaxf(top, v[i]);
@@ -159,20 +181,28 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   double sum = 0.0;
   uint32_t index = kNone;
+  bool bad = false;
   if (greedy) {
 #pragma unroll
     for (int i = (int)kPer - 1; i >= 0; --i) {
       if (v[i] == top) index = c + i;
-      if (v[i] != v[i]) sum = v[i];
+      bad |= v[i] != v[i];
     }
     if (index >= p.vocab) index = kNone;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) index = min(index, (uint32_t)__shfl_xor((int)index, off, 64));
   } else {
-    const double k = 1.44269504088896340736 / (double)q.temperature, from = top == -INFINITY ? 0.0 : (double)top;
+    // (the argument in one FMA: -top k, rounded, is off by the same for all)
+    const double k = 1.44269504088896340736 / (double)q.temperature, shift = -(double)top * k;
+    const double lead = lead_coefficient();
 #pragma unroll
-    for (int i = 0; i < (int)kPer; ++i) sum += exp2_64(((double)v[i] - from) * k);
+    for (int i = 0; i < (int)kPer; ++i) {
+      sum += exp2_64(__builtin_fma((double)v[i], k, shift), lead);
+      bad |= !(v[i] < INFINITY);  // +inf or NaN
+    }
+    if (top == -INFINITY) sum = 0.0;
   }
+  if (bad) sum = __builtin_nan("");
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if (lane == 0) {
@@ -207,6 +237,17 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
   }
   const double k = 1.44269504088896340736 / (double)(greedy ? 1.0f : q.temperature);
   const bool soft = p.draft && !greedy;
+  // (a draft's own logits, on their way while the rows are joined)
+  uint32_t token = kNone;
+  float target_logit = 0.0f, draft_logit = 0.0f, number = 0.0f;
+  if (tid < q.count) {
+    token = p.tokens[q.first + tid];
+    number = p.accept[q.first + tid];
+    if (token < p.vocab) {
+      target_logit = logit_at<BF16>(row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + tid), token);
+      if (soft) draft_logit = logit_at<BF16>(row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + tid), token);
+    }
+  }
   // rows 0 .. count of the target, then the draft's
   const uint32_t rows = q.count + 1 + (soft ? q.count : 0);
   for (uint32_t r = wave; r < rows; r += 4) {
@@ -220,7 +261,7 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
     for (uint32_t i = lane; i < p.chunks; i += 64) {
       // (a chunk of -inf alone has the sum 0, or NaN)
       if (greedy || st[i].top == -INFINITY) sum += st[i].sum;
-      else sum += st[i].sum * exp2_64(((double)st[i].top - (double)top) * k);
+      else sum += st[i].sum * exp2_or_0(((double)st[i].top - (double)top) * k);
       if (st[i].top == top) index = min(index, st[i].index);
     }
 #pragma unroll
@@ -243,22 +284,16 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
   bool ok = true, bad_token = false, bad_row = false;
   if (tid <= q.count) bad_row = !usable_row(tid) || (soft && tid < q.count && !usable_row(q.count + 1 + tid));
   if (tid < q.count) {
-    const uint32_t d = p.tokens[q.first + tid];
-    bad_token = d >= p.vocab;
+    bad_token = token >= p.vocab;
     if (greedy) {
-      ok = d == row_index[tid];
+      ok = token == row_index[tid];
     } else if (bad_token) {
       ok = false;
     } else {
-      const void* const target = row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + tid);
-      const double pd = exp2_64(((double)logit_at<BF16>(target, d) - (double)row_top[tid]) * k) / row_sum[tid];
-      double qd = 1.0;
-      if (soft) {
-        const void* const draft = row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + tid);
-        const uint32_t r = q.count + 1 + tid;
-        qd = exp2_64(((double)logit_at<BF16>(draft, d) - (double)row_top[r]) * k) / row_sum[r];
-      }
-      ok = (double)p.accept[q.first + tid] * qd < pd;
+      const double pd = exp2_or_0(((double)target_logit - (double)row_top[tid]) * k) / row_sum[tid];
+      const uint32_t r = q.count + 1 + tid;
+      const double qd = soft ? exp2_or_0(((double)draft_logit - (double)row_top[r]) * k) / row_sum[r] : 1.0;
+      ok = (double)number * qd < pd;
     }
     if (!ok || bad_row) atomicMin(&stop, tid);
   }
@@ -282,6 +317,8 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
       plan.p_top = row_top[j];
       plan.p_inverse = 1.0 / row_sum[j];
       plan.rejected = j < q.count;
+      plan.target_row = q.first + s + j;
+      plan.draft_row = q.first + j;
       if (plan.rejected) {
         plan.without = p.tokens[q.first + j];
         if (soft) {
@@ -295,26 +332,24 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
   }
 }
 
-// w of a thread's 16 columns of a chunk; `whole`: p alone
-template <bool BF16, bool WIDE>
-__device__ __forceinline__ void weights(double (&w)[16], const VerifyArgs& p, const Plan& plan, const Sequence& q, uint32_t s,
-                                        uint32_t c, bool whole) {
-  float v[16];
-  load16<BF16, WIDE>(v, row_of<BF16>(p.target, p.target_stride, (uint64_t)q.first + s + plan.place), c, p.vocab);
+// w of a thread's N columns of a chunk; `whole`: p alone
+template <bool BF16, bool WIDE, int N>
+__device__ __forceinline__ void weights(double (&w)[N], const VerifyArgs& p, const Plan& plan, uint32_t c, bool whole) {
+  float v[N], d[N];
+  const double lead = lead_coefficient();
+  load_logits<BF16, WIDE>(v, row_of<BF16>(p.target, p.target_stride, plan.target_row), c, p.vocab);
+  const bool soft = p.draft && !whole;
+  if (soft) load_logits<BF16, WIDE>(d, row_of<BF16>(p.draft, p.draft_stride, plan.draft_row), c, p.vocab);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = exp2_64(((double)v[i] - (double)plan.p_top) * plan.k) * plan.p_inverse;
-  if (whole) return;
-  if (p.draft) {
-    load16<BF16, WIDE>(v, row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + plan.place), c, p.vocab);
+  for (int i = 0; i < N; ++i) {
+    w[i] = exp2_or_0(((double)v[i] - (double)plan.p_top) * plan.k, lead) * plan.p_inverse;
+    if (!whole && !p.draft && c + i == plan.without) w[i] = 0.0;
+  }
+  if (!soft) return;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const double d = w[i] - exp2_64(((double)v[i] - (double)plan.q_top) * plan.k) * plan.q_inverse;
-      w[i] = d > 0.0 ? d : 0.0;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (c + i == plan.without) w[i] = 0.0;
+  for (int i = 0; i < N; ++i) {
+    const double e = w[i] - exp2_or_0(((double)d[i] - (double)plan.q_top) * plan.k, lead) * plan.q_inverse;
+    w[i] = e > 0.0 ? e : 0.0;
   }
 }
 
@@ -325,11 +360,11 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs p) {
   const uint32_t chunk = blockIdx.x % p.chunks, s = blockIdx.x / p.chunks;
   const Plan plan = p.plans[s];
   if (plan.place == kNone || !plan.rejected) return;
-  double w[16];
-  weights<BF16, WIDE>(w, p, plan, sequence_of(p, s), s, chunk * kChunk + threadIdx.x * kPer, false);
+  double w[kPer];
+  weights<BF16, WIDE>(w, p, plan, chunk * kChunk + threadIdx.x * kPer, false);
   double sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum += w[i];
+  for (int i = 0; i < (int)kPer; ++i) sum += w[i];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
@@ -337,7 +372,7 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs p) {
   if (threadIdx.x == 0) p.rest[(uint64_t)s * p.chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
-// Running sum over the block's threads, in order; `parts` [4]
+// Running sum over the block's threads, in order; `parts`: one per wave
 __device__ __forceinline__ double running_sum(double v, double* parts) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -351,9 +386,11 @@ __device__ __forceinline__ double running_sum(double v, double* parts) {
   return v;
 }
 
+// (1024 threads of 4 columns each: 10.4 -> 11.7 us for one sequence)
+constexpr uint32_t kPick = 256, kPickPer = kChunk / kPick;
 template <bool BF16, bool WIDE>
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs p) {
-  __shared__ double parts[3][4];
+__global__ __launch_bounds__(kPick) void verify_pick_kernel(VerifyArgs p) {
+  __shared__ double parts[3][kPick / 64];
   __shared__ double all, before;
   __shared__ uint32_t found, last;
   const uint32_t s = blockIdx.x, tid = threadIdx.x;
@@ -364,22 +401,25 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs p) {
     last = 0;
   }
   // the chunks' sums of w; where they are 0 throughout, of p
-  double own = plan.rejected && tid < p.chunks ? p.rest[(uint64_t)s * p.chunks + tid] : 0.0;
-  double run = running_sum(own, parts[0]);
-  if (tid == 255) all = run;
+  const float number = p.sample[s];
+  double own = 0.0, of_p = 0.0;
+  if (tid < p.chunks) {
+    const Stat st = p.stats[((uint64_t)s * p.rows + plan.place) * p.chunks + tid];
+    if (plan.rejected) own = p.rest[(uint64_t)s * p.chunks + tid];
+    if (st.top != -INFINITY) of_p = st.sum * exp2_or_0(((double)st.top - (double)plan.p_top) * plan.k) * plan.p_inverse;
+  }
+  bool whole = !plan.rejected;
+  double run = running_sum(whole ? of_p : own, parts[0]);
+  if (tid == kPick - 1) all = run;
   __syncthreads();
-  const bool whole = !(all > 0.0);
-  if (whole) {
-    own = 0.0;
-    if (tid < p.chunks) {
-      const Stat st = p.stats[((uint64_t)s * p.rows + plan.place) * p.chunks + tid];
-      if (st.top != -INFINITY) own = st.sum * exp2_64(((double)st.top - (double)plan.p_top) * plan.k) * plan.p_inverse;
-    }
-    run = running_sum(own, parts[1]);
-    if (tid == 255) all = run;
+  if (!whole && !(all > 0.0)) {
+    whole = true;
+    run = running_sum(of_p, parts[1]);
+    if (tid == kPick - 1) all = run;
     __syncthreads();
   }
-  const double threshold = (double)p.sample[s] * all;
+  if (whole) own = of_p;
+  const double threshold = (double)number * all;
   // (where rounding leaves none above the threshold, the last that has a sum)
   if (own > 0.0) {
     if (run > threshold) atomicMin(&found, tid);
@@ -394,11 +434,12 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs p) {
     last = 0;
   }
   const double left = threshold - before;
-  double w[16];
-  weights<BF16, WIDE>(w, p, plan, sequence_of(p, s), s, chunk * kChunk + tid * kPer, whole);
+  const uint32_t first = chunk * kChunk + tid * kPickPer;
+  double w[kPickPer];
+  weights<BF16, WIDE>(w, p, plan, first, whole);
   own = 0.0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) own += w[i];
+  for (int i = 0; i < (int)kPickPer; ++i) own += w[i];
   run = running_sum(own, parts[2]);
   if (own > 0.0) {
     if (run > left) atomicMin(&found, tid);
@@ -410,10 +451,10 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs p) {
   uint32_t token = 0;
   bool done = false;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < (int)kPickPer; ++i) {
     if (done || !(w[i] > 0.0)) continue;
     sum += w[i];
-    token = chunk * kChunk + tid * kPer + i;
+    token = first + i;
     done = sum > left;
   }
   p.out[(uint64_t)s * (p.most + 1) + plan.place] = token;
@@ -442,7 +483,7 @@ void launch(const VerifyArgs& p, hipStream_t s) {
   hipLaunchKernelGGL((verify_stats_kernel<BF16, WIDE>), dim3(p.sequences * p.rows * p.chunks), dim3(256), 0, s, p);
   hipLaunchKernelGGL((verify_walk_kernel<BF16>), dim3(p.sequences), dim3(256), 0, s, p);
   if (p.drafts) hipLaunchKernelGGL((verify_rest_kernel<BF16, WIDE>), dim3(p.sequences * p.chunks), dim3(256), 0, s, p);
-  hipLaunchKernelGGL((verify_pick_kernel<BF16, WIDE>), dim3(p.sequences), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((verify_pick_kernel<BF16, WIDE>), dim3(p.sequences), dim3(kPick), 0, s, p);
 }
 
 }  // namespace
