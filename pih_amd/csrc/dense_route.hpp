@@ -63,6 +63,7 @@ inline uint32_t DenseTileRows(uint32_t m, uint32_t n, uint32_t problems, uint32_
 struct TilePick {
   uint32_t mb = 0, nb = 0;
   bool grid = false;
+  double us = 0.0;  // the estimate it was chosen by
 };
 
 // The tile for a shape, by an estimate of its time: the rounds of tiles on the
@@ -72,11 +73,14 @@ struct TilePick {
 // at a time: their weights were measured to stream at 7 TB/s (12288 x 4096
 // bf16 at m 8: 16.5 us, 18.4 with 16 x 48 tiles) and a round is 512 of them,
 // 1.1 us apart.
-inline TilePick PickTile(bool bf16, uint32_t m, uint32_t n, uint32_t row_bytes, uint32_t problems) {
+// `pair`: tiles of an even number of 16-row weight blocks, not walked (the
+// feed-forward block's gate and up).
+inline TilePick PickTile(bool bf16, uint32_t m, uint32_t n, uint32_t row_bytes, uint32_t problems, bool pair = false) {
   TilePick best;
   double best_ns = 0.0;
   const double w_bytes = (double)n * problems * row_bytes;
   auto consider = [&](uint32_t mb, uint32_t nb, bool grid) {
+    if (pair && nb % 2) return;
     if (n % (16 * nb) || (mb > 1 && 16 * (mb - 1) >= m && mb < 8)) return;
     const uint64_t tiles = (uint64_t)((m + 16 * mb - 1) / (16 * mb)) * (n / (16 * nb)) * problems;
     const bool paired = mb == 1 && nb == 1;
@@ -91,7 +95,7 @@ inline TilePick PickTile(bool bf16, uint32_t m, uint32_t n, uint32_t row_bytes, 
     const bool tie = ns < best_ns + 1e-6 && (std::min(mb, nb) > std::min(best.mb, best.nb) ||
                                              (std::min(mb, nb) == std::min(best.mb, best.nb) && mb > best.mb));
     if (!best.mb || ns < best_ns - 1e-6 || tie) {
-      best = TilePick{mb, nb, grid};
+      best = TilePick{mb, nb, grid, ns * 1e-3};
       best_ns = ns;
     }
   };
@@ -100,7 +104,7 @@ inline TilePick PickTile(bool bf16, uint32_t m, uint32_t n, uint32_t row_bytes, 
       if ((bf16 || nb != 3) && (nb != 8 || mb <= 4)) consider(mb, nb, false);
   // (a tile's scale panel is reused two tiles later: the ring must not run
   // further ahead than one tile)
-  if (row_bytes / kWalkStep >= 8) {
+  if (row_bytes / kWalkStep >= 8 && !pair) {
     consider(8, 8, true);
     consider(12, 8, true);
     if (bf16) consider(16, 8, true);

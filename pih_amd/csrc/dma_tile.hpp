@@ -6,7 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "device_common.hpp"
+#include "glu.hpp"
 #include "kernels.hpp"
 
 namespace pih_amd {
@@ -29,7 +29,6 @@ enum : int {
 constexpr bool has_pair(int epi) { return epi == kEpiGlu || epi == kEpiGluSum; }
 constexpr bool has_stats(int epi) { return epi == kEpiStats || epi == kEpiTeacherStats; }
 constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherGrad; }
-constexpr float kLog2e = 1.44269504088896340736f;
 
 // ------------------------------------------------ tiles fed by DMA
 // C [m][n] = A . B^T in tiles of 256 columns and 256, 128 or 64 rows.  Four
@@ -84,33 +83,6 @@ struct BigArgs {
   uint64_t ldh;
   float limit;
 };
-
-// With s the logistic function of g = min(gate, limit) and u the clamped up:
-// silu(g) = g s, silu'(g) = s + g s (1 - s).
-__device__ __forceinline__ float logistic(float g) {
-  // (g -> -inf: exp -> inf, 1 / inf = 0)
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
-}
-// (not fminf, which drops a NaN)
-__device__ __forceinline__ float at_most(float v, float limit) { return v > limit ? limit : v; }
-__device__ __forceinline__ float within(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
-__device__ __forceinline__ float activated(float gate, float up, float limit) {
-  const float g = at_most(gate, limit);
-  return g * logistic(g) * within(up, limit);
-}
-// from dh, gate and up: dgate, dup and h
-struct GluGrad {
-  float dgate, dup, h;
-};
-__device__ __forceinline__ GluGrad glu_grad(float dh, float gate, float up, float limit) {
-  const float g = at_most(gate, limit), u = within(up, limit), s = logistic(g), silu = g * s;
-  return {gate > limit ? 0.0f : dh * u * (s + silu * (1.0f - s)), up > limit || up < -limit ? 0.0f : dh * silu, silu * u};
-}
-// four bf16 values of a uint2
-__device__ __forceinline__ v4f bf16x4_to_f32(uint2 v) {
-  return v4f{bf16_bits_to_f32(v.x & 0xffffu), bf16_bits_to_f32(v.x >> 16), bf16_bits_to_f32(v.y & 0xffffu),
-             bf16_bits_to_f32(v.y >> 16)};
-}
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;

@@ -9,6 +9,7 @@
 // element at most, independent from element to element, in sums that are
 // rounded to bf16 once themselves.  gate, up and dh stay in fp32 between
 // their product and the activation.
+#include "dense_route.hpp"
 #include "dma_tile.hpp"
 #include "tile64.hpp"
 
@@ -160,8 +161,8 @@ dim3 join_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count
 // ------------------------------------------- which tiles
 // How the rows of a product [m][n] over k run: tiles of `rows` rows, k in
 // `splits` parts.  Time (us): the rounds of tiles on the CUs, each its beginning
-// and end and a step's time (rows_cost in dma_tile.hpp), and for splits the sums
-// written and read at 4 TB/s and a launch.
+// and end and a step's time (rows_cost in dma_tile.hpp), no less than B takes at
+// 5.1 TB/s, and for splits the sums written and read at 4 TB/s and a launch.
 struct Tiling {
   uint32_t rows, splits;
   float us;
@@ -177,7 +178,8 @@ Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
       const uint32_t steps = k / KB, part = (steps + splits - 1) / splits;
       if ((steps + part - 1) / part != splits) continue;
       p.splits = splits;
-      const float us = rows_cost(p, m, rows) + (splits > 1 ? 4.0f + (float)splits * m * n * (8.0f / 4.0e6f) : 0.0f);
+      const float us = std::max(rows_cost(p, m, rows), (float)n * k * (2.0f / 5.1e6f)) +
+                       (splits > 1 ? 7.0f + (float)splits * m * n * (8.0f / 4.0e6f) : 0.0f);
       if (us < best.us) best = {rows, splits, us};
     }
   return best;
@@ -188,18 +190,19 @@ struct Route {
   uint32_t whole;  // rows in tiles of 256, unsplit
   Tiling rest;     // of those behind
   uint64_t sums;   // fp32 elements
+  float us;
 };
 Route route_of(uint32_t m, uint32_t n, uint32_t k) {
   const Tiling all = tiling_of(m, n, k);
   const uint32_t whole = m / 256 * 256, rest = m - whole;
-  Route r{0, all, all.splits > 1 ? (uint64_t)all.splits * m * n : 0};
+  Route r{0, all, all.splits > 1 ? (uint64_t)all.splits * m * n : 0, all.us};
   if (whole && rest) {
     BigArgs p{};
     p.n = n;
     p.k = k;
     const Tiling last = tiling_of(rest, n, k);
-    const float again = std::max(last.us, (float)n * k * (2.0f / 5.0e6f)) + 3.0f;
-    if (rows_cost(p, whole, 256) + again < all.us) r = {whole, last, last.splits > 1 ? (uint64_t)last.splits * rest * n : 0};
+    const float us = rows_cost(p, whole, 256) + last.us + 3.0f;
+    if (us < all.us) r = {whole, last, last.splits > 1 ? (uint64_t)last.splits * rest * n : 0, us};
   }
   return r;
 }
@@ -241,8 +244,18 @@ uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 dim3 tiles64(uint32_t m, uint32_t n) { return dim3((n + kT64 - 1) / kT64, (m + kT64 - 1) / kT64); }
 // the tiles fed by DMA take 64-deep steps of every product
 bool dma_takes(uint32_t inter, uint32_t hidden) { return inter % KB == 0 && hidden % KB == 0; }
+// Few rows: the tiles of gemm_tile.hip, chosen per shape for all CUs without
+// splits, against the route here, by both estimates (what those tiles take is
+// underestimated by 15 % against these).  Forward pass, us, route -> tiles for
+// gate and up -> for down too: 1 row of 4096 x 2048 23.8 -> 19.1 -> 15.9, of 4096
+// x 12288 64.9 -> 57.1 -> 52.0; 57 rows 35.0 -> 25.0 -> 19.1 and 78.9 -> 67.4 ->
+// 58.7; 512 rows 59.2 -> 51.6 -> 43.0, but 157.9 -> 209.4 -> 223.8.
+bool tiles_faster(uint32_t m, uint32_t n, uint32_t k, bool pair, const Route& r) {
+  return 1.15 * PickTile(true, m, n, 2 * k, 1, pair).us < r.us;
+}
 struct ForwardPlan {
   Route up, down;
+  bool up_tiles, down_tiles;
   uint64_t sums, bytes;
 };
 ForwardPlan forward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
@@ -252,7 +265,14 @@ ForwardPlan forward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
   if (!dma_takes(inter, hidden)) return p;
   p.up = route_of(rows, 2 * inter, hidden);
   p.down = route_of(rows, hidden, inter);
-  p.bytes += padded(std::max(p.up.sums, p.down.sums) * 4);
+  TileGluArgs t;
+  t.m = rows;
+  t.inter = inter;
+  t.k = hidden;
+  p.up_tiles = TileGluTakes(t) && tiles_faster(rows, 2 * inter, hidden, true, p.up);
+  // (LaunchBf16Gemm, which takes whole 128 columns above 64 rows)
+  p.down_tiles = (rows <= 64 || hidden % 128 == 0) && tiles_faster(rows, hidden, inter, false, p.down);
+  p.bytes += padded(std::max(p.up_tiles ? 0 : p.up.sums, p.down_tiles ? 0 : p.down.sums) * 4);
   return p;
 }
 struct BackwardPlan {
@@ -303,34 +323,62 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
   uint16_t* const h = static_cast<uint16_t*>(a.workspace);
   if (dma_takes(a.inter, a.hidden)) {
     float* const sums = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + plan.sums);
-    BigArgs p{};
-    p.a = a.x;
-    p.b = a.wg;
-    p.b2 = a.wu;
-    p.m = a.rows;
-    p.n = 2 * a.inter;
-    p.k = p.k_valid = a.hidden;
-    p.lda = p.ldb = a.hidden;
-    p.out = h;
-    p.ldo = a.inter;
-    p.gate = a.gate;
-    p.up = a.up;
-    p.limit = limit_of(a);
-    run_route<false, kEpiGlu, kEpiGluSum>(
-        plan.up, p, sums, a.stream,
-        [&](BigArgs& q, uint32_t rows) {
-          q.a += (uint64_t)rows * a.hidden;
-          q.out = h + (uint64_t)rows * a.inter;
-          if (a.gate) {
-            q.gate += (uint64_t)rows * a.inter;
-            q.up += (uint64_t)rows * a.inter;
-          }
-        },
-        [&](uint32_t first, uint32_t rows, uint32_t splits, uint64_t plane) {
-          const uint64_t from = (uint64_t)first * a.inter, count = (uint64_t)rows * a.inter;
-          hipLaunchKernelGGL(mlp_join_glu_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane, h + from,
-                             a.gate ? a.gate + from : nullptr, a.up ? a.up + from : nullptr, count, a.inter, p.limit);
-        });
+    if (plan.up_tiles) {
+      TileGluArgs t;
+      t.x = a.x;
+      t.wg = a.wg;
+      t.wu = a.wu;
+      t.h = h;
+      t.gate = a.gate;
+      t.up = a.up;
+      t.stream = a.stream;
+      t.m = a.rows;
+      t.inter = a.inter;
+      t.k = a.hidden;
+      t.limit = limit_of(a);
+      const St up = LaunchTileGlu(t);
+      if (!up.ok()) return up;
+    } else {
+      BigArgs p{};
+      p.a = a.x;
+      p.b = a.wg;
+      p.b2 = a.wu;
+      p.m = a.rows;
+      p.n = 2 * a.inter;
+      p.k = p.k_valid = a.hidden;
+      p.lda = p.ldb = a.hidden;
+      p.out = h;
+      p.ldo = a.inter;
+      p.gate = a.gate;
+      p.up = a.up;
+      p.limit = limit_of(a);
+      run_route<false, kEpiGlu, kEpiGluSum>(
+          plan.up, p, sums, a.stream,
+          [&](BigArgs& q, uint32_t rows) {
+            q.a += (uint64_t)rows * a.hidden;
+            q.out = h + (uint64_t)rows * a.inter;
+            if (a.gate) {
+              q.gate += (uint64_t)rows * a.inter;
+              q.up += (uint64_t)rows * a.inter;
+            }
+          },
+          [&](uint32_t first, uint32_t rows, uint32_t splits, uint64_t plane) {
+            const uint64_t from = (uint64_t)first * a.inter, count = (uint64_t)rows * a.inter;
+            hipLaunchKernelGGL(mlp_join_glu_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane, h + from,
+                               a.gate ? a.gate + from : nullptr, a.up ? a.up + from : nullptr, count, a.inter, p.limit);
+          });
+    }
+    if (plan.down_tiles) {
+      Bf16GemmArgs g;
+      g.a = h;
+      g.w = a.wd;
+      g.out = a.y;
+      g.stream = a.stream;
+      g.m = a.rows;
+      g.n = a.hidden;
+      g.k = a.inter;
+      return LaunchBf16Gemm(g);
+    }
     BigArgs q{};
     q.a = h;
     q.b = a.wd;

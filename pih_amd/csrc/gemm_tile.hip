@@ -37,7 +37,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "device_common.hpp"
+#include "glu.hpp"
 #include "kernels.hpp"
 
 namespace pih_amd {
@@ -66,6 +66,10 @@ struct TileParams {
   uint32_t out_prob_col;
   uint32_t out_f32, write_nonfinite, check_codes;
   uint32_t err_code, err_scale, err_nonfinite;
+  // the feed-forward block's gate and up (PAIR)
+  const uint8_t* w2;
+  uint16_t *gate, *up;
+  float limit;
 };
 
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
@@ -200,8 +204,12 @@ struct TileShape {
   static constexpr uint32_t kRing = kStages * kStage > kSums ? kStages * kStage : kSums;
 };
 
-template <int OP, int MB, int NB>
+// PAIR (bf16): two weights of n / 2 rows, w and w2, of which a tile has 16 rows in
+// turn; a row's results come out as h = silu(gate) up, [m][n / 2], and where
+// p.gate is not null gate and up themselves.
+template <int OP, int MB, int NB, bool PAIR = false>
 __global__ __launch_bounds__(kThreads, 1) void tile_gemm_kernel(TileParams p) {
+  static_assert(!PAIR || (OP == kTileBf16 && NB % 2 == 0), "pairs of weight blocks");
   using S = TileShape<OP, MB, NB>;
   constexpr uint32_t TM = S::TM, TN = S::TN;
   constexpr int ST = S::kStages, NL = S::kLoads;
@@ -232,7 +240,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_gemm_kernel(TileParams p) {
   auto a_row = [&](uint32_t r) -> uint64_t {
     return (uint64_t)min(row0 + r, p.m - 1) * p.a_row_stride + (uint64_t)prob * p.a_prob_row;
   };
-  const uint8_t* const w_base = p.w + ((uint64_t)prob * p.n + col0) * RB;
+  const uint64_t w_row = PAIR ? col0 / 2 : (uint64_t)prob * p.n + col0;
+  const uint8_t* const w_base = p.w + w_row * RB;
 
   // ---- DMA sources: instruction i of wave w moves rows 16 i + 4 w + (l >> 4),
   // lane l's 16 bytes to slot l & 15 (chunk (l & 15) ^ (row & 15))
@@ -241,15 +250,17 @@ __global__ __launch_bounds__(kThreads, 1) void tile_gemm_kernel(TileParams p) {
 #pragma unroll
   for (int i = 0; i < MB; ++i) a_off[i] = (uint32_t)(a_row(16 * i + drow) * RB) + dchunk;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) w_off[i] = (16 * i + drow) * RB + dchunk;
+  for (int i = 0; i < NB; ++i) w_off[i] = (16 * (PAIR ? i / 2 : i) + drow) * RB + dchunk;
   auto issue = [&](uint32_t stage, uint32_t j, auto NT) __attribute__((always_inline)) {
     const uint32_t lds = lds0 + stage * S::kStage + wv * 1024;
     const uint8_t* ab = uniform_ptr(p.a + (uint64_t)j * SB);
     const uint8_t* wb = uniform_ptr(w_base + (uint64_t)j * SB);
+    const uint8_t* wb2 = PAIR ? uniform_ptr(p.w2 + w_row * RB + (uint64_t)j * SB) : wb;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      if constexpr (decltype(NT)::value) dma16nt(wb, w_off[i], lds + TM * SB + i * 4096);
-      else dma16(wb, w_off[i], lds + TM * SB + i * 4096);
+      const uint8_t* const from = i % 2 ? wb2 : wb;
+      if constexpr (decltype(NT)::value) dma16nt(from, w_off[i], lds + TM * SB + i * 4096);
+      else dma16(from, w_off[i], lds + TM * SB + i * 4096);
     }
 #pragma unroll
     for (int i = 0; i < MB; ++i) dma16(ab, a_off[i], lds + i * 4096);
@@ -456,6 +467,24 @@ __global__ __launch_bounds__(kThreads, 1) void tile_gemm_kernel(TileParams p) {
   auto pick4 = [](v4f v, uint32_t i) __attribute__((always_inline)) -> float {
     return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
   };
+  if constexpr (PAIR) {
+#pragma unroll 1
+    for (uint32_t it = tid; it < TM * (QR / 2); it += kThreads) {
+      const uint32_t row = it / (QR / 2), cq = it % (QR / 2);
+      if (row0 + row >= p.m) continue;
+      const v4f gate = sum4(row, cq / 4 * 8 + cq % 4), up = sum4(row, cq / 4 * 8 + 4 + cq % 4);
+      const uint64_t o = (uint64_t)(row0 + row) * (p.n / 2) + col0 / 2 + cq * 4;
+      v4f h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = activated(gate[e], up[e], p.limit);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = bf16x4(h);
+      if (p.gate) {
+        *reinterpret_cast<uint2*>(p.gate + o) = bf16x4(gate);
+        *reinterpret_cast<uint2*>(p.up + o) = bf16x4(up);
+      }
+    }
+    return;
+  }
 #pragma unroll 1
   for (uint32_t it = tid; it < TM * QR; it += kThreads) {
     const uint32_t row = it / QR, cq = it % QR;
@@ -817,12 +846,12 @@ __global__ __launch_bounds__(kThreads, 1) void tile_grid_kernel(TileParams p) {
   if (bad) raise(p, bad);
 }
 
-template <int OP, int MB, int NB>
+template <int OP, int MB, int NB, bool PAIR = false>
 void launch_tile(TileParams p, hipStream_t s) {
   p.m_tiles = (p.m + 16 * MB - 1) / (16 * MB);
   p.n_tiles = p.n / (16 * NB);
   const uint32_t grid = (p.m_tiles * p.n_tiles * p.problems + 7) / 8 * 8;
-  hipLaunchKernelGGL((tile_gemm_kernel<OP, MB, NB>), dim3(grid), dim3(kThreads), 0, s, p);
+  hipLaunchKernelGGL((tile_gemm_kernel<OP, MB, NB, PAIR>), dim3(grid), dim3(kThreads), 0, s, p);
 }
 
 template <int OP, int MB, int NB, int SBW>
@@ -867,7 +896,48 @@ void launch_pick(const TilePick& t, const TileParams& p, hipStream_t s) {
   }
 }
 
+template <int MB>
+void launch_pair(int nb, const TileParams& p, hipStream_t s) {
+  if (nb == 2) launch_tile<kTileBf16, MB, 2, true>(p, s);
+  else if (nb == 4) launch_tile<kTileBf16, MB, 4, true>(p, s);
+  else if constexpr (MB <= 4) launch_tile<kTileBf16, MB, 8, true>(p, s);
+}
+
 }  // namespace
+
+bool TileGluTakes(const TileGluArgs& a) {
+  return a.m && a.inter && a.k && a.k % (SB / 2) == 0 && a.inter % 16 == 0 && (uint64_t)a.m * a.k * 2 <= 0xffffffffull &&
+         (uint64_t)a.inter / 16 * ((a.m + 15) / 16) <= 0x3fffffffull;
+}
+
+St LaunchTileGlu(const TileGluArgs& a) {
+  if (!a.x || !a.wg || !a.wu || !a.h || !a.stream || !a.gate != !a.up) return Invalid("tile_glu_null_argument");
+  if (!TileGluTakes(a)) return Invalid("tile_glu_shape_invalid");
+  TileParams p{};
+  p.a = reinterpret_cast<const uint8_t*>(a.x);
+  p.w = reinterpret_cast<const uint8_t*>(a.wg);
+  p.w2 = reinterpret_cast<const uint8_t*>(a.wu);
+  p.out = a.h;
+  p.gate = a.gate;
+  p.up = a.up;
+  p.limit = a.limit;
+  p.m = a.m;
+  p.n = 2 * a.inter;
+  p.row_bytes = 2 * a.k;
+  p.problems = 1;
+  p.a_row_stride = 1;
+  const TilePick t = PickTile(true, a.m, p.n, p.row_bytes, 1, true);
+  switch (t.mb) {
+    case 1: launch_pair<1>(t.nb, p, a.stream); break;
+    case 2: launch_pair<2>(t.nb, p, a.stream); break;
+    case 3: launch_pair<3>(t.nb, p, a.stream); break;
+    case 4: launch_pair<4>(t.nb, p, a.stream); break;
+    case 5: launch_pair<5>(t.nb, p, a.stream); break;
+    case 6: launch_pair<6>(t.nb, p, a.stream); break;
+    case 8: launch_pair<8>(t.nb, p, a.stream); break;
+  }
+  return AfterLaunch("tile_glu_launch_failed");
+}
 
 bool TileGemmTakes(const TileGemmArgs& a) {
   const uint64_t rb = a.bf16 ? 2ull * a.k : a.k, osz = a.out_kind == kOutF32 ? 4 : 2;

@@ -218,6 +218,22 @@ struct TileGemmArgs {
 };
 bool TileGemmTakes(const TileGemmArgs& a);
 St LaunchTileGemm(const TileGemmArgs& a, const TilePick& tile);
+// The feed-forward block's gate and up on the same tiles: h = silu(x . wg^T) (x .
+// wu^T) with the clamp of glu.hpp (limit infinite: none); gate and up themselves
+// where not null
+struct TileGluArgs {
+  const uint16_t* x = nullptr;   // [m, k]
+  const uint16_t* wg = nullptr;  // [inter, k]
+  const uint16_t* wu = nullptr;
+  uint16_t* h = nullptr;         // [m, inter]
+  uint16_t* gate = nullptr;
+  uint16_t* up = nullptr;
+  hipStream_t stream = nullptr;
+  uint32_t m = 0, inter = 0, k = 0;
+  float limit = 0.0f;
+};
+bool TileGluTakes(const TileGluArgs& a);
+St LaunchTileGlu(const TileGluArgs& a);
 // out[m, n] = sum over the splits in order of ws[q][m][n] (bf16 or fp32)
 St LaunchSplitKReduce(const float* ws, uint32_t splits, uint32_t m, uint32_t n, void* out, OutKind out_kind,
                       uint32_t* err, uint32_t bit, hipStream_t stream);

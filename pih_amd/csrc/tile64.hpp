@@ -79,7 +79,5 @@ __device__ __forceinline__ void each64(uint32_t m0, uint32_t n0, F&& f) {
     for (int j = 0; j < 2; ++j) f(m0 + wm + 16 * i + lr, n0 + wn + 16 * j + 4 * lg, i, j);
 }
 
-__device__ __forceinline__ uint2 bf16x4(v4f v) { return uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])}; }
-
 }  // namespace
 }  // namespace pih_amd
