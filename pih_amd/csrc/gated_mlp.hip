@@ -158,54 +158,6 @@ __global__ __launch_bounds__(256) void mlp_join_kernel(const float* sums, uint32
 }
 dim3 join_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 16)); }
 
-// ------------------------------------------- which tiles
-// How the rows of a product [m][n] over k run: tiles of `rows` rows, k in
-// `splits` parts.  Time (us): the rounds of tiles on the CUs, each its beginning
-// and end and a step's time (rows_cost in dma_tile.hpp), no less than B takes at
-// 5.1 TB/s, and for splits the sums written and read at 4 TB/s and a launch.
-struct Tiling {
-  uint32_t rows, splits;
-  float us;
-};
-Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
-  BigArgs p{};
-  p.n = n;
-  p.k = k;
-  Tiling best{256, 1, INFINITY};
-  for (uint32_t rows : {256u, 128u, 64u})
-    for (uint32_t splits = 1; splits <= 16 && k / KB / splits >= 4; ++splits) {
-      // (no split is empty)
-      const uint32_t steps = k / KB, part = (steps + splits - 1) / splits;
-      if ((steps + part - 1) / part != splits) continue;
-      p.splits = splits;
-      const float us = std::max(rows_cost(p, m, rows), (float)n * k * (2.0f / 5.1e6f)) +
-                       (splits > 1 ? 7.0f + (float)splits * m * n * (8.0f / 4.0e6f) : 0.0f);
-      if (us < best.us) best = {rows, splits, us};
-    }
-  return best;
-}
-// All rows alike, or the whole 256 without splits and the rest by itself, where B
-// is read once more (at 5 TB/s) and the launch costs 3 us
-struct Route {
-  uint32_t whole;  // rows in tiles of 256, unsplit
-  Tiling rest;     // of those behind
-  uint64_t sums;   // fp32 elements
-  float us;
-};
-Route route_of(uint32_t m, uint32_t n, uint32_t k) {
-  const Tiling all = tiling_of(m, n, k);
-  const uint32_t whole = m / 256 * 256, rest = m - whole;
-  Route r{0, all, all.splits > 1 ? (uint64_t)all.splits * m * n : 0, all.us};
-  if (whole && rest) {
-    BigArgs p{};
-    p.n = n;
-    p.k = k;
-    const Tiling last = tiling_of(rest, n, k);
-    const float us = rows_cost(p, whole, 256) + last.us + 3.0f;
-    if (us < all.us) r = {whole, last, last.splits > 1 ? (uint64_t)last.splits * rest * n : 0, us};
-  }
-  return r;
-}
 // EPI for the rows in one part, SUM and join(sums, first row, rows, splits,
 // elements of a plane) for those in several
 template <bool BT, int EPI, int SUM, typename A, typename J>

@@ -288,9 +288,37 @@ struct BackwardCall {
   float temperature = 1.0f;  // kEpiTeacherGrad
 };
 
-// after_logits(v0, cols): enqueues what g of a piece still needs
+// dx of a piece on a route of its own: the rows in whole tiles of 256 and the
+// rest each with the splits that suit them, whose sums lie behind one another
+struct DxRoute {
+  Tiling whole, rest;
+  uint32_t whole_rows;
+  uint64_t sums;  // fp32 elements
+};
+DxRoute dx_route(uint32_t rows, uint32_t hidden, uint32_t columns) {
+  const Tiling all = tiling_of(rows, hidden, columns);
+  DxRoute r{all, {}, rows, (uint64_t)all.splits * rows * hidden};
+  const uint32_t whole = rows / 256 * 256;
+  if (whole && whole < rows) {
+    const Tiling first = tiling_of(whole, hidden, columns), last = tiling_of(rows - whole, hidden, columns);
+    if (first.us + last.us + 3.0f < all.us)
+      r = {first, last, whole, ((uint64_t)first.splits * whole + (uint64_t)last.splits * (rows - whole)) * hidden};
+  }
+  return r;
+}
+inline void launch_dx(const Tiling& t, BigArgs b, hipStream_t s) {
+  b.splits = t.splits;
+  b.split_stride = (uint64_t)b.m * b.n;
+  if (t.rows == 64) launch_rows<64, false, true, kEpiAdd>(b, s);
+  else if (t.rows == 128) launch_rows<128, false, true, kEpiAdd>(b, s);
+  else launch_rows<256, false, true, kEpiAdd>(b, s);
+}
+
+// after_logits(v0, cols): enqueues what g of a piece still needs.  route: dx's
+// (null: all rows alike, in plan.splits parts)
 template <int EPI, typename F>
-void launch_backward(const BackwardCall& a, const BackwardPlan& plan, uint8_t* ws, F&& after_logits) {
+void launch_backward(const BackwardCall& a, const BackwardPlan& plan, const DxRoute* route, uint8_t* ws,
+                     F&& after_logits) {
   uint16_t* const grad = reinterpret_cast<uint16_t*>(ws + plan.g);
   uint16_t* const live = reinterpret_cast<uint16_t*>(ws + plan.live);
   float* const sums = reinterpret_cast<float*>(ws + plan.sums);
@@ -364,14 +392,36 @@ void launch_backward(const BackwardCall& a, const BackwardPlan& plan, uint8_t* w
     b.ldb = a.hidden;
     b.out = sums;
     b.ldo = a.hidden;
-    b.splits = plan.splits;
-    b.split_stride = (uint64_t)a.rows * a.hidden;
     b.first = v0 == 0;
-    launch_big<false, true, kEpiAdd>(b, a.stream);
+    if (route) {
+      b.m = route->whole_rows;
+      launch_dx(route->whole, b, a.stream);
+      if (route->whole_rows < a.rows) {
+        b.m = a.rows - route->whole_rows;
+        b.a += (uint64_t)route->whole_rows * plan.piece;
+        b.out = sums + (uint64_t)route->whole.splits * route->whole_rows * a.hidden;
+        launch_dx(route->rest, b, a.stream);
+      }
+    } else {
+      b.splits = plan.splits;
+      b.split_stride = (uint64_t)a.rows * a.hidden;
+      launch_big<false, true, kEpiAdd>(b, a.stream);
+    }
   }
-  const uint64_t count = (uint64_t)a.rows * a.hidden;
-  hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 20)), dim3(256), 0,
-                     a.stream, sums, a.target, a.up, mantissa, a.dx, a.hidden, a.vocab, count, plan.splits);
+  auto round = [&](const float* from, uint32_t first, uint32_t rows, uint32_t splits) {
+    const uint64_t count = (uint64_t)rows * a.hidden;
+    hipLaunchKernelGGL(loss_round_kernel, dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 20)), dim3(256),
+                       0, a.stream, from, a.target + first, a.up + first, mantissa + first,
+                       a.dx + (uint64_t)first * a.hidden, a.hidden, a.vocab, count, splits);
+  };
+  if (!route) {
+    round(sums, 0, a.rows, plan.splits);
+  } else {
+    round(sums, 0, route->whole_rows, route->whole.splits);
+    if (route->whole_rows < a.rows)
+      round(sums + (uint64_t)route->whole.splits * route->whole_rows * a.hidden, route->whole_rows,
+            a.rows - route->whole_rows, route->rest.splits);
+  }
 }
 
 }  // namespace

@@ -195,13 +195,18 @@ bool temperature_ok(float t) { return t > 0.0f && __builtin_isfinite(t) && __bui
 
 struct DistillPlan {
   BackwardPlan loss;
+  DxRoute dx;
   uint64_t live, norm, total, shift, up, bytes;
 };
 DistillPlan distill_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   DistillPlan p{};
   p.loss = backward_plan(rows, vocab, hidden);
+  // (dx has its own sums)
+  p.dx = dx_route(rows, hidden, (std::min(p.loss.piece, vocab) + KB - 1) / KB * KB);
   const uint64_t each = padded((uint64_t)rows * 4);
-  p.live = p.loss.bytes;
+  p.loss.factor = p.loss.sums + padded(p.dx.sums * 4);
+  p.loss.mantissa = p.loss.factor + padded(4);
+  p.live = p.loss.mantissa + each;
   p.norm = p.live + each;
   p.total = p.norm + each;
   p.shift = p.total + each;
@@ -313,7 +318,7 @@ St LaunchLmHeadDistillBackward(const LmHeadDistillArgs& a) {
   call.vocab = a.vocab;
   call.hidden = a.hidden;
   call.temperature = a.temperature;
-  launch_backward<kEpiTeacherGrad>(call, plan.loss, ws, [&](uint32_t v0, uint32_t cols) {
+  launch_backward<kEpiTeacherGrad>(call, plan.loss, &plan.dx, ws, [&](uint32_t v0, uint32_t cols) {
     hipLaunchKernelGGL(distill_entries_kernel, row_grid, dim3(256), 0, a.stream, a.ids, a.teacher, a.logits, a.lse, rows,
                        mantissa, grad, (uint64_t)plan.loss.piece, a.rows, a.vocab, a.top_k, v0, cols, a.temperature);
   });

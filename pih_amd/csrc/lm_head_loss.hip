@@ -153,7 +153,7 @@ St LaunchLmHeadLossBackward(const LmHeadLossArgs& a) {
   call.rows = a.rows;
   call.vocab = a.vocab;
   call.hidden = a.hidden;
-  launch_backward<kEpiGrad>(call, plan, static_cast<uint8_t*>(a.workspace), [](uint32_t, uint32_t) {});
+  launch_backward<kEpiGrad>(call, plan, nullptr, static_cast<uint8_t*>(a.workspace), [](uint32_t, uint32_t) {});
   return AfterLaunch("lm_head_loss_backward_launch_failed");
 }
 
