@@ -18,8 +18,8 @@ constexpr uint32_t kNoTarget = 0xffffffffu;
 // kEpiStats: maximum and sum of exponentials of every row's columns, and the
 // target's logit; kEpiGrad: the logits' gradient in bf16; kEpiBf16: a scaled
 // result in bf16; kEpiAdd: added to fp32 sums; kEpiTeacherStats, kEpiTeacherGrad: the
-// first two of logits over a temperature, without a target (whose part the
-// caller adds).  The feed-forward block's: kEpiStore: bf16; kEpiSum: fp32, a plane
+// first two of logits over a temperature, without a target, the first with the
+// logits at a list of columns that every row has.  The feed-forward block's: kEpiStore: bf16; kEpiSum: fp32, a plane
 // per split; kEpiGlu: two products side by side, gate and up, joined to h;
 // kEpiGluSum: the same two as kEpiSum; kEpiGluGrad: dh, joined with gate and up
 enum : int {
@@ -72,6 +72,13 @@ struct BigArgs {
   float* target_logit;
   uint32_t v0, vocab, first;
   float exponent;          // kEpiTeacher*: log2(e) / temperature
+  // kEpiTeacherStats: a row's columns in order, id << 8 | place in its list
+  // ([m][top_k]), how many of them lie before each tile ([m][n_tiles + 1]; null: no
+  // lists), and where their logits go ([m][top_k])
+  const uint32_t* sorted;
+  const uint16_t* before;
+  float* logits;
+  uint32_t top_k;
   // the feed-forward block's products
   const uint16_t* b2;      // kEpiGlu*: up's weights; kEpiStore, kEpiSum: B behind step b_steps
   uint16_t* out2;          // kEpiStore: rows of the result from out_rows on
@@ -122,7 +129,9 @@ template <int ROWS, bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   using S = BigShape<ROWS>;
   constexpr int MB = S::MB, NB = S::NB, ST = S::ST, LA = S::LA, LB = S::LB, NL = S::NL;
-  __shared__ __align__(16) uint8_t smem[S::kLds];
+  // (kEpiTeacherStats: the waves' parts of a row beside the staged logits)
+  constexpr uint32_t kParts = EPI == kEpiTeacherStats ? S::kLds : S::kOut;
+  __shared__ __align__(16) uint8_t smem[S::kLds + (EPI == kEpiTeacherStats ? S::WN * ROWS * 8 : 0)];
   const uint32_t tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
   const uint32_t lds0 = lds_addr(smem);
@@ -205,6 +214,9 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       else dma16(sb, ob, lds + S::kA + i * 4096);
     }
   };
+  // kEpiTeacherStats: of row tid of the tile the first and the end of its listed
+  // columns (low and high half), and the first two of them
+  uint32_t range = 0, key0 = 0, key1 = 0;
   // tile t and its first steps sent for; its rows' targets, log-sum-exps and
   // mantissas into half `which` of the panel (kNoTarget for every row whose g is 0)
   auto start = [&](uint32_t which) __attribute__((always_inline)) {
@@ -241,6 +253,13 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
           meta[ROWS + tid] = __float_as_uint(row < p.m ? p.lse[row] : 0.0f);
           meta[2 * ROWS + tid] = __float_as_uint(row < p.m ? p.mantissa[row] : 1.0f);
         }
+      }
+    }
+    if constexpr (EPI == kEpiTeacherStats) {
+      range = 0;
+      if (p.before && tid < ROWS && m0 + tid < p.m) {
+        const uint16_t* const b = p.before + (uint64_t)(m0 + tid) * (p.n_tiles + 1) + n0 / TB;
+        range = b[0] | (uint32_t)b[1] << 16;
       }
     }
   };
@@ -327,9 +346,19 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   constexpr std::integral_constant<int, 0> none;
   constexpr std::integral_constant<int, ST - 2> full;
 
+  // (on their way beside the K loop)
+  auto fetch_keys = [&]() __attribute__((always_inline)) {
+    if (EPI == kEpiTeacherStats && p.before) {
+      const uint32_t from = range & 0xffffu, count = (range >> 16) - from;
+      const uint32_t* const list = p.sorted + (uint64_t)(m0 + tid) * p.top_k + from;
+      key0 = count > 0 ? list[0] : 0u;
+      key1 = count > 1 ? list[1] : 0u;
+    }
+  };
   if (t >= end) return;
   uint32_t which = 0;
   start(which);
+  fetch_keys();
   // a tile's first steps have arrived before it is begun; for the tiles after
   // the first that is waited for ahead of the results' stores, which so drain
   // while the next tile is multiplied
@@ -359,7 +388,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       if (j + 1 < steps) body(j++, yes, none, no, no);
       body(j, no, none, no, no);
     }
-    const uint32_t cm = m0, cn = n0, csplit = split;
+    const uint32_t cm = m0, cn = n0, csplit = split, listed = range;
     const uint32_t* const meta = reinterpret_cast<const uint32_t*>(smem + S::kMeta + which * ROWS * 12);
     const bool more = t + stride < end;
     which ^= 1;
@@ -378,17 +407,55 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     const float exponent = EPI == kEpiTeacherStats || EPI == kEpiTeacherGrad ? p.exponent : kLog2e;
     if constexpr (has_stats(EPI)) {
       // [column part][row]: maximum and sum
-      float2* const parts = reinterpret_cast<float2*>(smem + S::kOut);
+      float2* const parts = reinterpret_cast<float2*>(smem + kParts);
       static_assert(S::WN * ROWS * 8 <= 4 * S::kOutRows * S::kOutRow, "parts");
       const bool whole = cn + TB <= p.n;
+      uint32_t* const lists = reinterpret_cast<uint32_t*>(smem + S::kMeta);  // [range, first, second][ROWS]
+      if (EPI == kEpiTeacherStats && p.before) {
+        if (tid < ROWS) {
+          lists[tid] = listed;
+          lists[ROWS + tid] = key0;
+          lists[2 * ROWS + tid] = key1;
+        }
+        __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
+        v4f (&l)[NB] = acc[i];
+        if (EPI == kEpiTeacherStats && p.before) {
+          // the row's listed columns: 16 or 8 rows x half of the wave's columns at a
+          // time through its LDS, where the four lanes of a row take theirs in turn
+          const uint32_t at_row = lrow + 16 * i + lr, mine = lists[at_row], from = mine & 0xffffu, count = (mine >> 16) - from;
+          if (__builtin_amdgcn_ballot_w64(count != 0)) {
+            const uint64_t list = (uint64_t)(cm + at_row) * p.top_k;
+            uint8_t* const st = smem + S::kOut + wave * S::kOutRows * S::kOutRow;
+#pragma unroll
+            for (uint32_t r0 = 0; r0 < 16; r0 += S::kOutRows) {
+              uint8_t* const row = st + (lr - r0) * S::kOutRow;
+              const bool staged = lr - r0 < S::kOutRows;
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                if (staged) {
+#pragma unroll
+                  for (int j = 0; j < NB / 2; ++j) *reinterpret_cast<v4f*>(row + j * 64 + lg * 16) = l[half * NB / 2 + j];
+                }
+                wave_lds_order();
+                for (uint32_t h = lg; staged && h < count; h += 4) {
+                  const uint32_t k = h < 2 ? lists[(h + 1) * ROWS + at_row] : p.sorted[list + from + h];
+                  const uint32_t place = (k >> 8) - (wcol + half * 8 * NB);
+                  if (place < 8u * NB) p.logits[list + (k & 0xffu)] = *reinterpret_cast<const float*>(row + place * 4);
+                }
+                wave_lds_order();
+              }
+            }
+          }
+        }
         if (!whole) {
 #pragma unroll
           for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (wcol + 16 * j + 4 * lg + e >= p.n) acc[i][j][e] = -INFINITY;
+              if (wcol + 16 * j + 4 * lg + e >= p.n) l[j][e] = -INFINITY;
         }
         if constexpr (EPI == kEpiStats) {
           const uint32_t target = meta[lrow + 16 * i + lr], place = target - wcol;
@@ -397,14 +464,14 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v = (uint32_t)j == place >> 4 && (uint32_t)e == (place & 3) ? acc[i][j][e] : v;
+              for (int e = 0; e < 4; ++e) v = (uint32_t)j == place >> 4 && (uint32_t)e == (place & 3) ? l[j][e] : v;
             p.target_logit[wrow + 16 * i + lr] = v;
           }
         }
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-          top = fmaxf(top, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+          top = fmaxf(top, fmaxf(fmaxf(l[j][0], l[j][1]), fmaxf(l[j][2], l[j][3])));
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float from = top == -INFINITY ? 0.0f : top;
@@ -413,7 +480,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
         for (int j = 0; j < NB; ++j) {
           float part = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) part += __builtin_amdgcn_exp2f((acc[i][j][e] - from) * exponent);
+          for (int e = 0; e < 4; ++e) part += __builtin_amdgcn_exp2f((l[j][e] - from) * exponent);
           sum += part;
         }
         sum += __shfl_xor(sum, 16, 64);
@@ -618,6 +685,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       }
     }
     if (!more) return;
+    fetch_keys();
   }
 }
 
@@ -668,7 +736,13 @@ void launch_big(BigArgs p, hipStream_t s) {
       p.a += whole * p.lda;
       if constexpr (has_stats(EPI)) {
         p.stats += (uint64_t)whole * ((p.n + TB - 1) / TB);
-        if constexpr (EPI == kEpiStats) p.target_logit += whole;
+        if constexpr (EPI == kEpiStats) {
+          p.target_logit += whole;
+        } else {
+          p.sorted += (uint64_t)whole * p.top_k;
+          if (p.before) p.before += (uint64_t)whole * ((p.n + TB - 1) / TB + 1);
+          p.logits += (uint64_t)whole * p.top_k;
+        }
       } else {
         p.out = static_cast<uint8_t*>(p.out) + whole * p.ldo * (EPI == kEpiAdd ? 4 : 2);
       }

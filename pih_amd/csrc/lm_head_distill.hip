@@ -7,10 +7,11 @@
 //   dx = g W,  dw = g^T x,  Q_t = sum_k q_k.
 //
 // The products are those of the cross entropy (lm_head_loss.hip) without a
-// target.  The teacher's entries are few against the vocabulary, so they come
-// in launches of their own: forward the row's logits at them and the sum over
-// them, backward the elements of g at them, which the tiles have written
-// without their q.
+// target.  The teacher's entries are few against the vocabulary: forward their
+// logits are dot products of their own, or where that is much (listed()) every row's
+// entries come in order, with how many lie before each tile, and the tile that
+// has an entry's logit writes it out; backward the elements of g at them, which
+// the tiles have written without their q, are written once more.
 #include "lm_head_common.hpp"
 
 namespace pih_amd {
@@ -57,6 +58,52 @@ __device__ __forceinline__ float normalizer(const Entries& e, const float* teach
 }
 __device__ __forceinline__ float probability(float s, float normalizer) {
   return s == -INFINITY ? 0.0f : expf(s - normalizer);
+}
+
+// The entries of a row in order of their ids, by a wave (an entry's place is how
+// many are less; no two are equal), how many lie before each tile of the
+// vocabulary, and 0 for the logits of those that are not there
+__global__ __launch_bounds__(256) void distill_sort_kernel(const uint32_t* ids, uint32_t* sorted, uint16_t* before,
+                                                           float* logits, uint32_t rows, uint32_t vocab, uint32_t tiles,
+                                                           uint32_t top_k) {
+  __shared__ uint32_t all[4][kTopMax], ordered[4][kTopMax];
+  const uint32_t wave = threadIdx.x >> 6, row = blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const uint64_t at = (uint64_t)row * top_k;
+  uint32_t key[kTopMax / 64], there = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    const uint32_t k = lane + 64 * i, id = k < top_k ? ids[at + k] : kNoTarget;
+    // (those that are not there last, in order of their places too)
+    key[i] = (id < vocab ? id << 8 : 1u << 28) | k;
+    there += __popcll(__builtin_amdgcn_ballot_w64(id < vocab));
+    if (k < top_k) {
+      all[wave][k] = key[i];
+      if (id >= vocab) logits[at + k] = 0.0f;
+    }
+  }
+  wave_lds_order();
+#pragma unroll
+  for (uint32_t i = 0; i < kTopMax / 64; ++i) {
+    if (64 * i >= top_k) break;
+    uint32_t less = 0;
+    for (uint32_t k = 0; k < top_k; ++k) less += all[wave][k] < key[i];
+    if (lane + 64 * i < top_k) {
+      ordered[wave][less] = key[i];
+      sorted[at + less] = key[i];
+    }
+  }
+  wave_lds_order();
+  uint16_t* const out = before + (uint64_t)row * (tiles + 1);
+  for (uint32_t t = lane; t <= tiles; t += 64) {
+    uint32_t low = 0, high = there;
+    while (low < high) {
+      const uint32_t mid = (low + high) / 2;
+      if (ordered[wave][mid] >> 8 < t * TB) low = mid + 1;
+      else high = mid;
+    }
+    out[t] = (uint16_t)low;
+  }
 }
 
 // z of every entry, by a wave: a dot product over the hidden size
@@ -193,6 +240,28 @@ bool distill_ok(const LmHeadDistillArgs& a) {
 }
 bool temperature_ok(float t) { return t > 0.0f && __builtin_isfinite(t) && __builtin_isfinite(1.0f / t); }
 
+// Whether the tiles write the entries' logits: 4 us a round of tiles and 6 for the
+// sort, against the dot products' bytes at 8 TB/s.  64 entries, 4096 rows over
+// 129280 x 4096: 3499 us with dot products, 3330 so; 20 entries, 33 rows over
+// 151936 x 1024: 68 and 74.
+bool listed(uint32_t rows, uint32_t vocab, uint32_t hidden, uint32_t top_k) {
+  const float rounds = (float)rows * vocab / (65536.0f * kCus);
+  return big_takes(hidden) && (float)rows * top_k * hidden * (2.0f / 8.0e6f) > 6.0f + 4.0f * rounds;
+}
+// the forward pass's workspace: the rows' pairs, and for the tiles fed by DMA the
+// entries in order and how many lie before each tile
+struct DistillForward {
+  uint64_t sorted, before, bytes;
+};
+DistillForward distill_forward(uint32_t rows, uint32_t vocab, uint32_t hidden) {
+  DistillForward f{};
+  f.bytes = f.sorted = padded((uint64_t)rows * stat_tiles(vocab, hidden) * 8);
+  if (!big_takes(hidden)) return f;
+  f.before = f.sorted + padded((uint64_t)rows * kTopMax * 4);
+  f.bytes = f.before + padded((uint64_t)rows * (stat_tiles(vocab, hidden) + 1) * 2);
+  return f;
+}
+
 struct DistillPlan {
   BackwardPlan loss;
   DxRoute dx;
@@ -219,7 +288,7 @@ DistillPlan distill_plan(uint32_t rows, uint32_t vocab, uint32_t hidden) {
 
 uint64_t LmHeadDistillWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden) {
   if (!shape_ok(rows, vocab, hidden)) return 0;
-  return padded((uint64_t)rows * stat_tiles(vocab, hidden) * 8);
+  return distill_forward(rows, vocab, hidden).bytes;
 }
 
 uint64_t LmHeadDistillBackwardWorkspaceBytes(uint32_t rows, uint32_t vocab, uint32_t hidden) {
@@ -245,7 +314,15 @@ St LaunchLmHeadDistill(const LmHeadDistillArgs& a) {
   if (!clean.ok()) return clean;
   const uint32_t tiles = stat_tiles(a.vocab, a.hidden);
   float2* const stats = static_cast<float2*>(a.workspace);
+  const bool in_tiles = listed(a.rows, a.vocab, a.hidden, a.top_k);
   if (big_takes(a.hidden)) {
+    const DistillForward plan = distill_forward(a.rows, a.vocab, a.hidden);
+    uint8_t* const ws = static_cast<uint8_t*>(a.workspace);
+    uint32_t* const sorted = reinterpret_cast<uint32_t*>(ws + plan.sorted);
+    uint16_t* const before = reinterpret_cast<uint16_t*>(ws + plan.before);
+    if (in_tiles)
+      hipLaunchKernelGGL(distill_sort_kernel, dim3((a.rows + 3) / 4), dim3(256), 0, a.stream, a.ids, sorted, before, a.logits,
+                         a.rows, a.vocab, tiles, a.top_k);
     BigArgs b{};
     b.a = a.x;
     b.b = a.w;
@@ -255,6 +332,10 @@ St LaunchLmHeadDistill(const LmHeadDistillArgs& a) {
     b.lda = b.ldb = a.hidden;
     b.stats = stats;
     b.exponent = kLog2e / a.temperature;
+    b.sorted = sorted;
+    b.before = in_tiles ? before : nullptr;
+    b.logits = a.logits;
+    b.top_k = a.top_k;
     launch_big<false, false, kEpiTeacherStats>(b, a.stream);
   } else {
     GemmArgs g{};
@@ -269,9 +350,11 @@ St LaunchLmHeadDistill(const LmHeadDistillArgs& a) {
     g.inverse = 1.0f / a.temperature;
     launch_gemm<kEpiTeacherStats>(g, a.stream);
   }
-  const uint64_t entries = (uint64_t)a.rows * a.top_k;
-  hipLaunchKernelGGL(distill_gather_kernel, dim3((uint32_t)std::min<uint64_t>((entries + 3) / 4, 1u << 20)), dim3(256), 0,
-                     a.stream, a.x, a.w, a.ids, a.logits, entries, a.top_k, a.vocab, a.hidden);
+  if (!in_tiles) {
+    const uint64_t entries = (uint64_t)a.rows * a.top_k;
+    hipLaunchKernelGGL(distill_gather_kernel, dim3((uint32_t)std::min<uint64_t>((entries + 3) / 4, 1u << 20)), dim3(256), 0,
+                       a.stream, a.x, a.w, a.ids, a.logits, entries, a.top_k, a.vocab, a.hidden);
+  }
   hipLaunchKernelGGL(distill_join_kernel, dim3((a.rows + 3) / 4), dim3(256), 0, a.stream, stats, a.ids, a.teacher,
                      a.teacher_lse, a.logits, a.loss, a.lse, a.error_flag, a.rows, a.vocab, tiles, a.top_k,
                      a.temperature);

@@ -326,3 +326,27 @@ def test_captured(eng):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want))
     assert int(flag.item()) == 0
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,top_k", [(70, 600, 4096, 256), (190, 700, 2048, 200), (300, 300, 2048, 255),
+                                                     (420, 5000, 2048, 100), (1000, 513, 1024, 128)])
+def test_many_entries_in_a_tile(eng, rows, vocab, hidden, top_k):
+    """Lists long enough for the tiles to write their logits, with many entries
+    of a row in one tile, equal ones, none at all, and a certain id in all."""
+    import torch
+
+    from pih_amd.linear import lm_head_distill
+
+    case = [t.cuda() for t in _case(rows, rows, vocab, hidden, top_k)]
+    x, w, ids, teacher, more, _ = case
+    ids[:, 3] = 255
+    ids[1::4, 5:9] = vocab - 1
+    ids[2] = 7
+    _, loss, lse, z = _forward_ref(x, w, ids, teacher, more, 1.3, False)
+    for n in (1 << 12, 1 << 16, 1 << 20):
+        torch.full((n,), float("nan"), device="cuda")
+    got = lm_head_distill(x, w, ids, teacher, 1.3)
+    assert int(got[3].item()) == 0
+    for what, a, b in (("logits", got[2], z), ("lse", got[1], lse), ("loss", got[0], loss)):
+        _within(a, b, what)
+    assert torch.all(got[2][ids < 0] == 0)
