@@ -770,8 +770,8 @@ Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
   p.n = n;
   p.k = k;
   Tiling best{256, 1, INFINITY};
-  for (uint32_t rows : {256u, 128u, 64u})
-    for (uint32_t splits = 1; splits <= 16 && k / KB / splits >= 4; ++splits) {
+  for (uint32_t rows : {64u, 128u, 256u})
+    for (uint32_t splits = 1; splits <= 64 && k / KB / splits >= 4; ++splits) {
       // (no split is empty)
       const uint32_t steps = k / KB, part = (steps + splits - 1) / splits;
       if ((steps + part - 1) / part != splits) continue;
