@@ -159,15 +159,17 @@ __global__ __launch_bounds__(256) void mlp_join_kernel(const float* sums, uint32
 dim3 join_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 1023) / 1024, 1u << 16)); }
 
 // EPI for the rows in one part, SUM and join(sums, first row, rows, splits,
-// elements of a plane) for those in several
-template <bool BT, int EPI, int SUM, typename A, typename J>
-void run_route(const Route& r, BigArgs p, float* sums, hipStream_t s, A&& advance, J&& join) {
+// elements of a plane) for those in several; rest(first row, rows) does the rows
+// behind the whole 256 where rest_apart
+template <bool BT, int EPI, int SUM, typename A, typename J, typename R>
+St run_route(const Route& r, BigArgs p, float* sums, hipStream_t s, A&& advance, J&& join, bool rest_apart, R&& rest) {
   const uint32_t m = p.m;
   p.splits = 1;
   if (r.whole) {
     p.m = r.whole;
     launch_rows<256, false, BT, EPI>(p, s);
-    if (r.whole == m) return;
+    if (r.whole == m) return Ok();
+    if (rest_apart) return rest(r.whole, m - r.whole);
     advance(p, r.whole);
     p.m = m - r.whole;
   }
@@ -185,6 +187,7 @@ void run_route(const Route& r, BigArgs p, float* sums, hipStream_t s, A&& advanc
     else if (r.rest.rows == 128) launch_rows<128, false, BT, EPI>(p, s);
     else launch_rows<256, false, BT, EPI>(p, s);
   }
+  return Ok();
 }
 
 bool shape_ok(uint32_t rows, uint32_t inter, uint32_t hidden) {
@@ -201,13 +204,16 @@ bool dma_takes(uint32_t inter, uint32_t hidden) { return inter % KB == 0 && hidd
 // underestimated by 15 % against these).  Forward pass, us, route -> tiles for
 // gate and up -> for down too: 1 row of 4096 x 2048 23.8 -> 19.1 -> 15.9, of 4096
 // x 12288 64.9 -> 57.1 -> 52.0; 57 rows 35.0 -> 25.0 -> 19.1 and 78.9 -> 67.4 ->
-// 58.7; 512 rows 59.2 -> 51.6 -> 43.0, but 157.9 -> 209.4 -> 223.8.
-bool tiles_faster(uint32_t m, uint32_t n, uint32_t k, bool pair, const Route& r) {
-  return 1.15 * PickTile(true, m, n, 2 * k, 1, pair).us < r.us;
+// 58.7; 512 rows 59.2 -> 51.6 -> 43.0, but 157.9 -> 209.4 -> 223.8.  The same
+// choice for the rows behind the whole 256 of a route: 1030 rows of 4096 x 12288
+// 334 -> 321, 4099 rows 964 -> 943.
+bool tiles_faster(uint32_t m, uint32_t n, uint32_t k, bool pair, float route_us) {
+  return 1.15 * PickTile(true, m, n, 2 * k, 1, pair).us < route_us;
 }
 struct ForwardPlan {
   Route up, down;
-  bool up_tiles, down_tiles;
+  bool up_tiles, down_tiles;            // all rows
+  bool up_rest_tiles, down_rest_tiles;  // the rows behind the whole 256 of the route
   uint64_t sums, bytes;
 };
 ForwardPlan forward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
@@ -217,14 +223,24 @@ ForwardPlan forward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
   if (!dma_takes(inter, hidden)) return p;
   p.up = route_of(rows, 2 * inter, hidden);
   p.down = route_of(rows, hidden, inter);
-  TileGluArgs t;
-  t.m = rows;
-  t.inter = inter;
-  t.k = hidden;
-  p.up_tiles = TileGluTakes(t) && tiles_faster(rows, 2 * inter, hidden, true, p.up);
-  // (LaunchBf16Gemm, which takes whole 128 columns above 64 rows)
-  p.down_tiles = (rows <= 64 || hidden % 128 == 0) && tiles_faster(rows, hidden, inter, false, p.down);
-  p.bytes += padded(std::max(p.up_tiles ? 0 : p.up.sums, p.down_tiles ? 0 : p.down.sums) * 4);
+  auto up_tiles = [&](uint32_t m, float us) {
+    TileGluArgs t;
+    t.m = m;
+    t.inter = inter;
+    t.k = hidden;
+    return TileGluTakes(t) && tiles_faster(m, 2 * inter, hidden, true, us);
+  };
+  // (LaunchBf16Gemm, which takes whole 128 columns above 64 rows, and 32-bit offsets into h)
+  auto down_tiles = [&](uint32_t m, float us) {
+    return (m <= 64 || hidden % 128 == 0) && (uint64_t)m * inter * 2 <= 0xffffffffull &&
+           tiles_faster(m, hidden, inter, false, us);
+  };
+  p.up_tiles = up_tiles(rows, p.up.us);
+  p.down_tiles = down_tiles(rows, p.down.us);
+  p.up_rest_tiles = p.up.whole && p.up.whole < rows && up_tiles(rows - p.up.whole, p.up.rest.us);
+  p.down_rest_tiles = p.down.whole && p.down.whole < rows && down_tiles(rows - p.down.whole, p.down.rest.us);
+  p.bytes += padded(std::max(p.up_tiles || p.up_rest_tiles ? 0 : p.up.sums,
+                             p.down_tiles || p.down_rest_tiles ? 0 : p.down.sums) * 4);
   return p;
 }
 struct BackwardPlan {
@@ -275,21 +291,36 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
   uint16_t* const h = static_cast<uint16_t*>(a.workspace);
   if (dma_takes(a.inter, a.hidden)) {
     float* const sums = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + plan.sums);
-    if (plan.up_tiles) {
+    auto up_on_tiles = [&](uint32_t first, uint32_t rows) {
+      const uint64_t from = (uint64_t)first * a.inter;
       TileGluArgs t;
-      t.x = a.x;
+      t.x = a.x + (uint64_t)first * a.hidden;
       t.wg = a.wg;
       t.wu = a.wu;
-      t.h = h;
-      t.gate = a.gate;
-      t.up = a.up;
+      t.h = h + from;
+      t.gate = a.gate ? a.gate + from : nullptr;
+      t.up = a.up ? a.up + from : nullptr;
       t.stream = a.stream;
-      t.m = a.rows;
+      t.m = rows;
       t.inter = a.inter;
       t.k = a.hidden;
       t.limit = limit_of(a);
-      const St up = LaunchTileGlu(t);
-      if (!up.ok()) return up;
+      return LaunchTileGlu(t);
+    };
+    auto down_on_tiles = [&](uint32_t first, uint32_t rows) {
+      Bf16GemmArgs g;
+      g.a = h + (uint64_t)first * a.inter;
+      g.w = a.wd;
+      g.out = a.y + (uint64_t)first * a.hidden;
+      g.stream = a.stream;
+      g.m = rows;
+      g.n = a.hidden;
+      g.k = a.inter;
+      return LaunchBf16Gemm(g);
+    };
+    St up = Ok();
+    if (plan.up_tiles) {
+      up = up_on_tiles(0, a.rows);
     } else {
       BigArgs p{};
       p.a = a.x;
@@ -304,7 +335,7 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
       p.gate = a.gate;
       p.up = a.up;
       p.limit = limit_of(a);
-      run_route<false, kEpiGlu, kEpiGluSum>(
+      up = run_route<false, kEpiGlu, kEpiGluSum>(
           plan.up, p, sums, a.stream,
           [&](BigArgs& q, uint32_t rows) {
             q.a += (uint64_t)rows * a.hidden;
@@ -318,19 +349,11 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
             const uint64_t from = (uint64_t)first * a.inter, count = (uint64_t)rows * a.inter;
             hipLaunchKernelGGL(mlp_join_glu_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane, h + from,
                                a.gate ? a.gate + from : nullptr, a.up ? a.up + from : nullptr, count, a.inter, p.limit);
-          });
+          },
+          plan.up_rest_tiles, up_on_tiles);
     }
-    if (plan.down_tiles) {
-      Bf16GemmArgs g;
-      g.a = h;
-      g.w = a.wd;
-      g.out = a.y;
-      g.stream = a.stream;
-      g.m = a.rows;
-      g.n = a.hidden;
-      g.k = a.inter;
-      return LaunchBf16Gemm(g);
-    }
+    if (!up.ok()) return up;
+    if (plan.down_tiles) return down_on_tiles(0, a.rows);
     BigArgs q{};
     q.a = h;
     q.b = a.wd;
@@ -342,7 +365,7 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
     q.out = a.y;
     q.ldo = a.hidden;
     q.b_steps = 0xffffffffu;
-    run_route<false, kEpiStore, kEpiSum>(
+    const St down = run_route<false, kEpiStore, kEpiSum>(
         plan.down, q, sums, a.stream,
         [&](BigArgs& r, uint32_t rows) {
           r.a += (uint64_t)rows * a.inter;
@@ -352,8 +375,9 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
           const uint64_t count = (uint64_t)rows * a.hidden;
           hipLaunchKernelGGL(mlp_join_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane,
                              a.y + (uint64_t)first * a.hidden, count);
-        });
-    return AfterLaunch("gated_mlp_launch_failed");
+        },
+        plan.down_rest_tiles, down_on_tiles);
+    return down.ok() ? AfterLaunch("gated_mlp_launch_failed") : down;
   }
   MlpArgs p{};
   p.a = a.x;
@@ -436,7 +460,8 @@ St LaunchGatedMlpBackward(const GatedMlpArgs& a) {
           const uint64_t up_to = (uint64_t)(row_up - first) * a.inter;
           hipLaunchKernelGGL(mlp_join_dh_kernel, join_grid(up_to), dim3(256), 0, a.stream, sums, splits, plane,
                              a.gate + from, a.up + from, dgu + 2 * from, h + from, count, up_to, a.inter, p.limit);
-        });
+        },
+        false, [](uint32_t, uint32_t) { return Ok(); });
     if (a.dx) {
       BigArgs q{};
       q.a = dgu;
@@ -460,7 +485,8 @@ St LaunchGatedMlpBackward(const GatedMlpArgs& a) {
             const uint64_t count = (uint64_t)rows * a.hidden;
             hipLaunchKernelGGL(mlp_join_kernel, join_grid(count), dim3(256), 0, a.stream, sums, splits, plane,
                                a.dx + (uint64_t)first * a.hidden, count);
-          });
+          },
+          false, [](uint32_t, uint32_t) { return Ok(); });
     }
     // the weights' gradients, columns of A against columns of B over the rows
     auto weight = [&](const uint16_t* from, uint32_t ld, uint32_t from_valid, uint32_t m, const uint16_t* with,

@@ -164,7 +164,7 @@ def test_backward(eng, rows, hidden, inter, limit):
 
 
 LARGE = [(1, 4096, 2048), (7, 7168, 2048), (16, 4096, 12288), (40, 4096, 12288), (57, 4096, 2048), (128, 4096, 12288),
-         (200, 7168, 2048), (509, 4096, 12288), (1021, 4096, 2048), (2100, 4096, 4096)]
+         (200, 7168, 2048), (509, 4096, 12288), (1021, 4096, 2048), (1030, 4096, 12288), (2100, 4096, 4096)]
 
 
 @pytest.mark.parametrize("rows,hidden,inter", LARGE)
@@ -301,3 +301,56 @@ def test_captured(eng, rows, hidden, inter):
             want = step(*case)
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("rows,hidden,inter", [(40, 256, 512), (300, 320, 192), (7, 72, 136)])
+def test_any_part_of_the_gradients(eng, rows, hidden, inter):
+    """The entry's results that are left out (null) change nothing of the others."""
+    import torch
+
+    from pih_amd import abi, linear
+    from pih_amd.device import stream_handle
+
+    x, wg, wu, wd, dy = (t.cuda() for t in _case(12, rows, hidden, inter))
+    _, gate, up = linear.gated_mlp(x, wg, wu, wd, keep=True)
+    want = linear.gated_mlp_backward(dy, x, wg, wu, wd, gate, up)
+    ws = linear._workspace(abi.WORKSPACE_GATED_MLP_BACKWARD, rows, inter, hidden, x.device)
+    for parts in range(1, 16):
+        got = [torch.full_like(w, 7.0) for w in want]
+        linear._launch("launch_gated_mlp_backward", "gated_mlp_backward",
+                       *(t.data_ptr() for t in (dy, x, wg, wu, wd, gate, up)),
+                       *(t.data_ptr() if parts >> i & 1 else 0 for i, t in enumerate(got)), ws.data_ptr(), ws.numel(),
+                       stream_handle(), rows, hidden, inter, 0.0)
+        for i, (g, w) in enumerate(zip(got, want)):
+            assert torch.equal(g, w if parts >> i & 1 else torch.full_like(w, 7.0)), (parts, i)
+
+
+@pytest.mark.parametrize("hidden,inter", [(4096, 128), (128, 4096)])
+def test_rows_past_4_gib(eng, hidden, inter):
+    """2^20 rows, whose x and y or gate, up and h have more than 2^32 bytes.  All
+    rows repeat the first 8191: y, gate, up and dx with them, and the weights'
+    gradients, of an upstream gradient that is zero before the last 8191 rows, are
+    those of as many rows."""
+    import torch
+
+    from pih_amd.linear import gated_mlp, gated_mlp_backward
+
+    rows, few = 1 << 20, 8191
+    x, wg, wu, wd, dy = _case(21, few, hidden, inter, "cuda")
+    times = -(-rows // few)
+    # (the last rows are the first ones, in order)
+    long_x = x.repeat(times, 1)[-rows:].contiguous()
+    assert long_x.numel() * 2 > 1 << 32 or rows * inter * 2 > 1 << 32
+    y, gate, up = gated_mlp(long_x, wg, wu, wd, keep=True)
+    for what, t, w in zip(("y", "gate", "up"), (y, gate, up), _forward_ref(x, wg, wu, wd, 0.0)):
+        for at in (rows - few, rows - few * (times - 1)):
+            _within(t[at:at + few], w, what)
+    del y
+    long_dy = torch.zeros_like(long_x)
+    long_dy[-few:] = dy
+    got = gated_mlp_backward(long_dy, long_x, wg, wu, wd, gate, up)
+    want = _backward_ref(dy, x, wg, wu, wd, gate[-few:], up[-few:], 0.0)
+    assert torch.all(got[0][:-few] == 0)
+    # (their sums run over all rows, most of them zeros)
+    for what, g, w in zip(("dx", "dw_gate", "dw_up", "dw_down"), (got[0][-few:],) + got[1:], want):
+        _within(g, w, what)

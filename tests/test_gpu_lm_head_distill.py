@@ -350,3 +350,53 @@ def test_many_entries_in_a_tile(eng, rows, vocab, hidden, top_k):
     for what, a, b in (("logits", got[2], z), ("lse", got[1], lse), ("loss", got[0], loss)):
         _within(a, b, what)
     assert torch.all(got[2][ids < 0] == 0)
+
+
+def test_rows_past_4_gib(eng):
+    """2^20 rows, whose x has more than 2^32 bytes, that repeat 2047: so do the
+    losses and dx, and the weights' gradient, of an upstream gradient that is zero
+    before the last 2047 rows, is that of as many rows."""
+    import torch
+
+    from pih_amd.linear import lm_head_distill, lm_head_distill_backward
+
+    rows, few, vocab, hidden, top_k = 1 << 20, 2047, 500, 4096, 8
+    x, w, ids, teacher, more, up = _case(31, few, vocab, hidden, top_k, "cuda")
+    times = -(-rows // few)
+    long_x, long_ids, long_teacher = (t.repeat(times, 1)[-rows:].contiguous() for t in (x, ids, teacher))
+    assert long_x.numel() * 2 > 1 << 32
+    got = lm_head_distill(long_x, w, long_ids, long_teacher, 1.5)
+    assert int(got[3].item()) == 0
+    _, *want = _forward_ref(x, w, ids, teacher, more, 1.5, False)
+    for at in (rows - few, rows - few * (times - 1)):
+        for what, a, b in zip(("loss", "lse", "logits"), got, want):
+            _within(a[at:at + few], b, what)
+    long_up = torch.zeros(rows, device="cuda")
+    long_up[-few:] = up
+    dx, dw, _ = lm_head_distill_backward(long_x, w, long_ids, long_teacher, got[1], got[2], long_up, 1.5)
+    want = _grads_ref(x, w, ids, teacher, more, up, got[1][-few:], 1.5, False)
+    assert torch.all(dx[:-few] == 0)
+    _within(dx[-few:], want[0], "dx")
+    _within(dw, want[1], "dw")
+
+
+def test_weights_past_4_gib(eng):
+    """The largest vocabulary, whose weights and their gradient have more than
+    2^32 bytes; entries at both ends of it."""
+    import torch
+
+    from pih_amd.linear import lm_head_distill, lm_head_distill_backward
+
+    rows, vocab, hidden, top_k = 20, 1 << 20, 2112, 16
+    x, w, ids, teacher, more, up = _case(32, rows, vocab, hidden, top_k, "cuda", std=1.0)
+    assert w.numel() * 2 > 1 << 32
+    ids[:, 2], ids[:, 7] = vocab - 1, 0
+    got = lm_head_distill(x, w, ids, teacher)
+    assert int(got[3].item()) == 0
+    _, *want = _forward_ref(x, w, ids, teacher, more, 1.0, False)
+    for what, a, b in zip(("loss", "lse", "logits"), got, want):
+        _within(a, b, what)
+    want = _grads_ref(x, w, ids, teacher, more, up, got[1], 1.0, False)
+    dx, dw, _ = lm_head_distill_backward(x, w, ids, teacher, got[1], got[2], up)
+    _within(dx, want[0], "dx")
+    _within(dw, want[1], "dw")
