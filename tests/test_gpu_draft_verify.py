@@ -237,6 +237,30 @@ def test_masked_logits(eng):
         np.testing.assert_array_equal(got[0] < 700, True)
 
 
+@pytest.mark.parametrize("soft", [True, False])
+def test_extreme_temperatures(eng, soft):
+    """Temperatures so low that the largest logit alone has a probability, or
+    that a logit over it exceeds 64 bits' integers, and so high that all have the
+    same; logits of every size."""
+    import numpy as np
+
+    for seed, spread in ((1, 1.0), (2, 50.0), (3, 1e-3)):
+        t = [1e-45, 1e-38, 1e-30, 1e-20, 1e-12, 1e-8, 1e-5, 1e-3, 0.03, 30.0, 1e4, 1e20, 3e38]
+        case = _case(seed, [3] * len(t), 9000, soft=soft, spread=spread, near=0.1 * spread, temperature=t)
+        case["accept"][::4] = np.float32(1 - 2.0 ** -24)
+        got = _check(case, 3)
+        assert got[2] == 0
+        # (equal models accept everything, at any of them)
+        if soft:
+            case["draft"] = case["target"][[4 * s + i for s in range(len(t)) for i in range(3)]].clone()
+            tau = np.repeat(np.asarray(t, np.float32), 3)
+            cold = tau < 0.1  # (a draft of probability 0 is rejected)
+            case["tokens"][cold] = case["draft"].numpy()[cold].argmax(1)
+            case["accept"][:] = np.float32(1 - 2.0 ** -24)
+            got = _check(case, 3)
+            assert (got[1] == 3).all()
+
+
 def test_greedy_takes_the_first_of_equals(eng):
     case = _case(3, [3, 3], 9000, temperature=[0.0, 0.0])
     t = case["target"]
