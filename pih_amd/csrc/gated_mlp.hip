@@ -281,13 +281,12 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
   if (!aligned(a.x) || !aligned(a.wg) || !aligned(a.wu) || !aligned(a.wd) || !aligned(a.y) || !aligned(a.gate) ||
       !aligned(a.up))
     return Invalid("gated_mlp_alignment_invalid");
-  if (a.workspace_bytes < GatedMlpWorkspaceBytes(a.rows, a.inter, a.hidden) || !aligned(a.workspace))
-    return Invalid("gated_mlp_workspace_invalid");
+  const ForwardPlan plan = forward_plan(a.rows, a.inter, a.hidden);
+  if (a.workspace_bytes < plan.bytes || !aligned(a.workspace)) return Invalid("gated_mlp_workspace_invalid");
   if (a.y == a.x || (a.gate && (a.gate == a.x || a.up == a.x || a.gate == a.up || a.gate == a.y || a.up == a.y)))
     return Invalid("gated_mlp_alias_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
-  const ForwardPlan plan = forward_plan(a.rows, a.inter, a.hidden);
   uint16_t* const h = static_cast<uint16_t*>(a.workspace);
   if (dma_takes(a.inter, a.hidden)) {
     float* const sums = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + plan.sums);
@@ -419,11 +418,10 @@ St LaunchGatedMlpBackward(const GatedMlpArgs& a) {
     for (int s = 0; s < r; ++s)
       if (results[r] && results[r] == results[s]) return Invalid("gated_mlp_backward_alias_invalid");
   }
-  if (a.workspace_bytes < GatedMlpBackwardWorkspaceBytes(a.rows, a.inter, a.hidden) || !aligned(a.workspace))
-    return Invalid("gated_mlp_backward_workspace_invalid");
+  const BackwardPlan plan = backward_plan(a.rows, a.inter, a.hidden);
+  if (a.workspace_bytes < plan.bytes || !aligned(a.workspace)) return Invalid("gated_mlp_backward_workspace_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
-  const BackwardPlan plan = backward_plan(a.rows, a.inter, a.hidden);
   uint8_t* const ws = static_cast<uint8_t*>(a.workspace);
   uint16_t* const h = reinterpret_cast<uint16_t*>(ws + plan.h);
   if (dma_takes(a.inter, a.hidden)) {
