@@ -11,11 +11,14 @@
 // sums are therefore in 64 bits (of which the vector units do as many a clock
 // as of 32), so that the order of the sums moves no token.
 //
-// Launches: the largest logit and the sum of exponentials of every row and
-// chunk of the vocabulary; a block per sequence that joins them and walks the
-// drafts; the chunks' sums of w at the rejected places; a block per sequence
-// that finds the chunk and in it the token.  (The last two in one, the token found
-// by the last of a sequence's blocks: 57 sequences 21 -> 24 us, 256 46 -> 58.)
+// Launches: the largest logit and the sum of exponentials of every row and chunk
+// of the vocabulary; then for few sequences one launch, a block per sequence and
+// chunk, that does the three others' work: a block per sequence that joins the
+// rows and walks the drafts; the chunks' sums of w at the rejected places; a block
+// per sequence that finds the chunk and in it the token.  (The last two in one for
+// many, the token found by the last of a sequence's blocks: 57 sequences 21 -> 24
+// us, 256 46 -> 58.)
+#include "dense_route.hpp"
 #include "device_common.hpp"
 #include "kernels.hpp"
 
@@ -58,6 +61,7 @@ struct VerifyArgs {
   Stat* stats;   // [sequences][rows][chunks]
   Plan* plans;   // [sequences]
   double* rest;  // [sequences][chunks]
+  uint32_t* done;  // [sequences]: blocks that have written theirs
   uint64_t target_stride, draft_stride;
   uint32_t sequences, drafts, most, vocab, chunks, rows;
 };
@@ -143,6 +147,45 @@ __device__ __forceinline__ float logit_at(const void* row, uint32_t c) {
   return BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[c]) : static_cast<const float*>(row)[c];
 }
 
+// Running sums and largest values over a wave by lane moves: within 16 lanes, then
+// from the last lane of one 16 to the next, then from the 32nd to the upper half;
+// lane 63 has all.  (~25 cycles a step of a 64-bit sum; through LDS ~130.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v, uint32_t other) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double plus_moved(double v) {
+  const uint2 x = __builtin_bit_cast(uint2, v);
+  return v + __builtin_bit_cast(double, uint2{moved<CTRL, ROWS>(x.x, 0u), moved<CTRL, ROWS>(x.y, 0u)});
+}
+__device__ __forceinline__ double wave_running_sum(double v) {
+  v = plus_moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = plus_moved<0x112, 0xf>(v);
+  v = plus_moved<0x114, 0xf>(v);
+  v = plus_moved<0x118, 0xf>(v);
+  v = plus_moved<0x142, 0xa>(v);  // row_bcast 15
+  return plus_moved<0x143, 0xc>(v);  // row_bcast 31
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  const uint2 x = __builtin_bit_cast(uint2, wave_running_sum(v));
+  return __builtin_bit_cast(double, uint2{(uint32_t)__builtin_amdgcn_readlane((int)x.x, 63),
+                                          (uint32_t)__builtin_amdgcn_readlane((int)x.y, 63)});
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_moved(float v) {
+  return fmaxf(v, __uint_as_float(moved<CTRL, ROWS>(__float_as_uint(v), 0xff800000u)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = max_moved<0x111, 0xf>(v);
+  v = max_moved<0x112, 0xf>(v);
+  v = max_moved<0x114, 0xf>(v);
+  v = max_moved<0x118, 0xf>(v);
+  v = max_moved<0x142, 0xa>(v);
+  v = max_moved<0x143, 0xc>(v);
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+
 struct Sequence {
   uint32_t first, count;
   float temperature;
@@ -163,6 +206,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   __shared__ uint32_t indexes[4];
   const uint32_t chunk = blockIdx.x % p.chunks, at = blockIdx.x / p.chunks, y = at % p.rows, s = at / p.rows;
   const Sequence q = sequence_of(p, s);
+  if (y == 0 && chunk == 0 && threadIdx.x == 0) p.done[s] = 0;
   const bool greedy = q.temperature == 0.0f, of_draft = y > p.most;
   const uint32_t place = of_draft ? y - p.most - 1 : y;
   if (!q.offsets_ok || !temperature_ok(q.temperature) || place > q.count || (of_draft && (greedy || place == q.count)))
@@ -175,7 +219,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < (int)kPer; ++i) top = fmaxf(top, v[i]);
-  top = reduce_max_xor<64>(top);
+  top = wave_max(top);
   if (lane == 0) tops[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -210,8 +254,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
     if (top == -INFINITY) sum = 0.0;
   }
   if (bad) sum = __builtin_nan("");
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  sum = wave_sum(sum);
   if (lane == 0) {
     sums[wave] = sum;
     indexes[wave] = index;
@@ -222,28 +265,49 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
                                                     min(min(indexes[0], indexes[1]), min(indexes[2], indexes[3]))};
 }
 
-// The walk over a sequence's drafts
+struct WalkRows {
+  double sum[2 * kMostDrafts + 1];
+  float top[2 * kMostDrafts + 1];
+  uint32_t index[kMostDrafts + 1];
+  uint32_t stop, why;
+};
+// The walk over a sequence's drafts by a block: what is left to be drawn into
+// `plan` (in LDS too; to be read behind a barrier), the tokens and the count written
+// by the one block that `writes`
 template <bool BF16>
-__global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
-  __shared__ double row_sum[2 * kMostDrafts + 1];
-  __shared__ float row_top[2 * kMostDrafts + 1];
-  __shared__ uint32_t row_index[kMostDrafts + 1];
-  __shared__ uint32_t stop, why;
-  const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ void walk(const VerifyArgs& p, uint32_t s, bool writes, WalkRows& row, Plan& plan) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Sequence q = sequence_of(p, s);
   uint32_t* const out = p.out + (uint64_t)s * (p.most + 1);
   const bool usable = q.offsets_ok && temperature_ok(q.temperature), greedy = q.temperature == 0.0f;
   if (!usable) {
-    for (uint32_t i = tid; i <= p.most; i += 256) out[i] = kNone;
+    for (uint32_t i = tid; writes && i <= p.most; i += 256) out[i] = kNone;
     if (tid == 0) {
-      p.accepted[s] = 0;
-      p.plans[s].place = kNone;
-      atomicOr(p.err, q.offsets_ok ? kErrRow : kErrOffsets);
+      plan.place = kNone;
+      if (writes) {
+        p.accepted[s] = 0;
+        atomicOr(p.err, q.offsets_ok ? kErrRow : kErrOffsets);
+      }
     }
     return;
   }
   const double k = 1.44269504088896340736 / (double)(greedy ? 1.0f : q.temperature);
   const bool soft = p.draft && !greedy;
+  // rows 0 .. count of the target, then the draft's; four of a wave's at a time
+  const uint32_t rows = q.count + 1 + (soft ? q.count : 0);
+  auto stats_of = [&](uint32_t r) {
+    const uint32_t y = r <= q.count ? r : p.most + 1 + r - (q.count + 1);
+    return p.stats + ((uint64_t)s * p.rows + y) * p.chunks;
+  };
+  Stat ahead[4];
+  auto load_rows = [&](uint32_t r0) {
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) {
+      ahead[b] = Stat{0.0, -INFINITY, kNone};
+      if (r0 + 4 * b < rows && lane < p.chunks) ahead[b] = stats_of(r0 + 4 * b)[lane];
+    }
+  };
+  load_rows(wave);
   // (a draft's own logits, on their way while the rows are joined)
   uint32_t token = kNone;
   float target_logit = 0.0f, draft_logit = 0.0f, number = 0.0f;
@@ -255,88 +319,116 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
       if (soft) draft_logit = logit_at<BF16>(row_of<BF16>(p.draft, p.draft_stride, (uint64_t)q.first + tid), token);
     }
   }
-  // rows 0 .. count of the target, then the draft's
-  const uint32_t rows = q.count + 1 + (soft ? q.count : 0);
-  for (uint32_t r = wave; r < rows; r += 4) {
-    const uint32_t y = r <= q.count ? r : p.most + 1 + r - (q.count + 1);
-    const Stat* const st = p.stats + ((uint64_t)s * p.rows + y) * p.chunks;
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < p.chunks; i += 64) top = fmaxf(top, st[i].top);
-    top = reduce_max_xor<64>(top);
-    double sum = 0.0;
-    uint32_t index = kNone;
-    for (uint32_t i = lane; i < p.chunks; i += 64) {
-      // (a chunk of -inf alone has the sum 0, or NaN)
-      if (greedy || st[i].top == -INFINITY) sum += st[i].sum;
-      else sum += st[i].sum * exp2_or_0(((double)st[i].top - (double)top) * k);
-      if (st[i].top == top) index = min(index, st[i].index);
+  for (uint32_t r0 = wave; r0 < rows; r0 += 16) {
+    if (r0 != wave) load_rows(r0);
+    float top[4];
+    double sum[4];
+    // (the four in step, for the waits in between)
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) {
+      top[b] = ahead[b].top;
+      for (uint32_t i = lane + 64; r0 + 4 * b < rows && i < p.chunks; i += 64)
+        top[b] = fmaxf(top[b], stats_of(r0 + 4 * b)[i].top);
     }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      sum += __shfl_xor(sum, off, 64);
-      index = min(index, (uint32_t)__shfl_xor((int)index, off, 64));
+    for (uint32_t b = 0; b < 4; ++b) top[b] = wave_max(top[b]);
+    // (a chunk of -inf alone has the sum 0, or NaN)
+    auto part = [&](const Stat& x, float largest) {
+      if (greedy || x.top == -INFINITY) return x.sum;
+      return x.sum * exp2_or_0(((double)x.top - (double)largest) * k);
+    };
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) {
+      sum[b] = part(ahead[b], top[b]);
+      for (uint32_t i = lane + 64; r0 + 4 * b < rows && i < p.chunks; i += 64)
+        sum[b] += part(stats_of(r0 + 4 * b)[i], top[b]);
     }
-    // greedy: a sum of 1 stands for a row that has a largest logit
-    if (greedy && sum == 0.0) sum = top == -INFINITY ? 0.0 : 1.0;
-    if (lane == 0) {
-      row_sum[r] = sum;
-      row_top[r] = top;
-      if (r <= q.count) row_index[r] = index;
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) {
+      sum[b] = wave_sum(sum[b]);
+      // greedy: a sum of 1 stands for a row that has a largest logit
+      if (greedy && sum[b] == 0.0) sum[b] = top[b] == -INFINITY ? 0.0 : 1.0;
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < 4; ++b) {
+      const uint32_t r = r0 + 4 * b;
+      if (r >= rows) break;
+      if (lane == 0) {
+        row.sum[r] = sum[b];
+        row.top[r] = top[b];
+      }
+      if (!greedy) continue;
+      uint32_t index = ahead[b].top == top[b] ? ahead[b].index : kNone;
+      for (uint32_t i = lane + 64; i < p.chunks; i += 64) {
+        const Stat x = stats_of(r)[i];
+        if (x.top == top[b]) index = min(index, x.index);
+      }
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) index = min(index, (uint32_t)__shfl_xor((int)index, off, 64));
+      if (lane == 0) row.index[r] = index;
     }
   }
-  if (tid == 0) stop = q.count;
+  if (tid == 0) row.stop = q.count;
   __syncthreads();
   // a row's sum is above 0 and finite, or the row has no probabilities
-  auto usable_row = [&](uint32_t r) { return row_sum[r] > 0.0 && row_sum[r] < (double)INFINITY; };
+  auto usable_row = [&](uint32_t r) { return row.sum[r] > 0.0 && row.sum[r] < (double)INFINITY; };
   bool ok = true, bad_token = false, bad_row = false;
   if (tid <= q.count) bad_row = !usable_row(tid) || (soft && tid < q.count && !usable_row(q.count + 1 + tid));
   if (tid < q.count) {
     bad_token = token >= p.vocab;
     if (greedy) {
-      ok = token == row_index[tid];
+      ok = token == row.index[tid];
     } else if (bad_token) {
       ok = false;
     } else {
-      const double pd = exp2_or_0(((double)target_logit - (double)row_top[tid]) * k) / row_sum[tid];
+      const double pd = exp2_or_0(((double)target_logit - (double)row.top[tid]) * k) / row.sum[tid];
       const uint32_t r = q.count + 1 + tid;
-      const double qd = soft ? exp2_or_0(((double)draft_logit - (double)row_top[r]) * k) / row_sum[r] : 1.0;
+      const double qd = soft ? exp2_or_0(((double)draft_logit - (double)row.top[r]) * k) / row.sum[r] : 1.0;
       ok = (double)number * qd < pd;
     }
-    if (!ok || bad_row) atomicMin(&stop, tid);
+    if (!ok || bad_row) atomicMin(&row.stop, tid);
   }
   __syncthreads();
-  const uint32_t j = stop;
-  if (tid == j) why = (bad_row ? kErrRow : 0) | (bad_token ? kErrToken : 0);
+  const uint32_t j = row.stop;
+  // the thread of the place has its token at hand
+  if (tid == j) {
+    const uint32_t bits = (bad_row ? kErrRow : 0) | (bad_token ? kErrToken : 0);
+    row.why = bits;
+    plan.place = greedy || (bits & kErrRow) ? kNone : j;
+    plan.k = k;
+    plan.p_top = row.top[j];
+    plan.p_inverse = 1.0 / row.sum[j];
+    plan.rejected = j < q.count;
+    plan.target_row = q.first + s + j;
+    plan.draft_row = q.first + j;
+    plan.without = token;
+    const bool with_draft = soft && j < q.count;
+    plan.q_top = with_draft ? row.top[q.count + 1 + j] : 0.0f;
+    plan.q_inverse = with_draft ? 1.0 / row.sum[q.count + 1 + j] : 0.0;
+    if (writes) {
+      p.accepted[s] = j;
+      if (bits) atomicOr(p.err, bits);
+    }
+  }
+  if (!writes) return;
   __syncthreads();
-  const uint32_t bits = why;
+  const uint32_t bits = row.why;
   for (uint32_t i = tid; i <= p.most; i += 256) {
     uint32_t t = kNone;
-    if (i < j) t = p.tokens[q.first + i];
-    else if (i == j && greedy && !(bits & kErrRow)) t = row_index[j];
-    out[i] = t;
+    if (i < j) t = token;  // (i is tid: j <= count < 256)
+    else if (i == j && greedy && !(bits & kErrRow)) t = row.index[j];
+    // (the place to be drawn is written by who draws it, in another block perhaps)
+    if (i != j || plan.place == kNone) out[i] = t;
   }
-  if (tid == 0) {
-    p.accepted[s] = j;
-    Plan plan{};
-    plan.place = greedy || (bits & kErrRow) ? kNone : j;
-    if (plan.place != kNone) {
-      plan.k = k;
-      plan.p_top = row_top[j];
-      plan.p_inverse = 1.0 / row_sum[j];
-      plan.rejected = j < q.count;
-      plan.target_row = q.first + s + j;
-      plan.draft_row = q.first + j;
-      if (plan.rejected) {
-        plan.without = p.tokens[q.first + j];
-        if (soft) {
-          plan.q_top = row_top[q.count + 1 + j];
-          plan.q_inverse = 1.0 / row_sum[q.count + 1 + j];
-        }
-      }
-    }
-    p.plans[s] = plan;
-    if (bits) atomicOr(p.err, bits);
-  }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
+  __shared__ WalkRows rows;
+  __shared__ Plan plan;
+  walk<BF16>(p, blockIdx.x, true, rows, plan);
+  __syncthreads();
+  if (threadIdx.x == 0) p.plans[blockIdx.x] = plan;
 }
 
 // w of a thread's N columns of a chunk; `whole`: p alone
@@ -360,6 +452,20 @@ __device__ __forceinline__ void weights(double (&w)[N], const VerifyArgs& p, con
   }
 }
 
+// Sum of w over a chunk, in thread 0
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ double chunk_rest(const VerifyArgs& p, const Plan& plan, uint32_t chunk, double (&sums)[4]) {
+  double w[kPer];
+  weights<BF16, WIDE>(w, p, plan, chunk * kChunk + threadIdx.x * kPer, false);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < (int)kPer; ++i) sum += w[i];
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  return sums[0] + sums[1] + sums[2] + sums[3];
+}
+
 // Sums of w over the chunks, at the rejected places
 template <bool BF16, bool WIDE>
 __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs p) {
@@ -367,93 +473,83 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs p) {
   const uint32_t chunk = blockIdx.x % p.chunks, s = blockIdx.x / p.chunks;
   const Plan plan = p.plans[s];
   if (plan.place == kNone || !plan.rejected) return;
-  double w[kPer];
-  weights<BF16, WIDE>(w, p, plan, chunk * kChunk + threadIdx.x * kPer, false);
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < (int)kPer; ++i) sum += w[i];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) p.rest[(uint64_t)s * p.chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
+  const double sum = chunk_rest<BF16, WIDE>(p, plan, chunk, sums);
+  if (threadIdx.x == 0) p.rest[(uint64_t)s * p.chunks + chunk] = sum;
 }
 
 // Running sum over the block's threads, in order; `parts`: one per wave
-__device__ __forceinline__ double running_sum(double v, double* parts) {
+__device__ __forceinline__ double running_sum(double v, double (&parts)[4]) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double from = __shfl_up(v, off, 64);
-    if (lane >= (uint32_t)off) v += from;
-  }
+  v = wave_running_sum(v);
   if (lane == 63) parts[wave] = v;
   __syncthreads();
   for (uint32_t i = 0; i < wave; ++i) v += parts[i];
   return v;
 }
 
-// (1024 threads of 4 columns each: 10.4 -> 11.7 us for one sequence)
-constexpr uint32_t kPick = 256, kPickPer = kChunk / kPick;
+// The token behind the accepted ones, by a block
+constexpr uint32_t kPickPer = kChunk / 256;
+struct PickRows {
+  double parts[3][4];
+  double all, before;
+  uint32_t found, last;
+};
+// the sum of p over chunk threadIdx.x
+__device__ __forceinline__ double chunk_of_p(const VerifyArgs& p, uint32_t s, const Plan& plan) {
+  if (threadIdx.x >= p.chunks) return 0.0;
+  const Stat st = p.stats[((uint64_t)s * p.rows + plan.place) * p.chunks + threadIdx.x];
+  if (st.top == -INFINITY) return 0.0;
+  return st.sum * exp2_or_0(((double)st.top - (double)plan.p_top) * plan.k) * plan.p_inverse;
+}
+// own: the sum of w over it
 template <bool BF16, bool WIDE>
-__global__ __launch_bounds__(kPick) void verify_pick_kernel(VerifyArgs p) {
-  __shared__ double parts[3][kPick / 64];
-  __shared__ double all, before;
-  __shared__ uint32_t found, last;
-  const uint32_t s = blockIdx.x, tid = threadIdx.x;
-  const Plan plan = p.plans[s];
-  if (plan.place == kNone) return;
+__device__ __forceinline__ void pick(const VerifyArgs& p, uint32_t s, const Plan& plan, PickRows& lds, float number,
+                                     double of_p, double own) {
+  const uint32_t tid = threadIdx.x;
   if (tid == 0) {
-    found = kNone;
-    last = 0;
+    lds.found = kNone;
+    lds.last = 0;
   }
-  // the chunks' sums of w; where they are 0 throughout, of p
-  const float number = p.sample[s];
-  double own = 0.0, of_p = 0.0;
-  if (tid < p.chunks) {
-    const Stat st = p.stats[((uint64_t)s * p.rows + plan.place) * p.chunks + tid];
-    if (plan.rejected) own = p.rest[(uint64_t)s * p.chunks + tid];
-    if (st.top != -INFINITY) of_p = st.sum * exp2_or_0(((double)st.top - (double)plan.p_top) * plan.k) * plan.p_inverse;
-  }
+  // where the sums of w are 0 throughout, of p
   bool whole = !plan.rejected;
-  double run = running_sum(whole ? of_p : own, parts[0]);
-  if (tid == kPick - 1) all = run;
+  double run = running_sum(whole ? of_p : own, lds.parts[0]);
+  if (tid == 255) lds.all = run;
   __syncthreads();
-  if (!whole && !(all > 0.0)) {
+  if (!whole && !(lds.all > 0.0)) {
     whole = true;
-    run = running_sum(of_p, parts[1]);
-    if (tid == kPick - 1) all = run;
+    run = running_sum(of_p, lds.parts[1]);
+    if (tid == 255) lds.all = run;
     __syncthreads();
   }
   if (whole) own = of_p;
-  const double threshold = (double)number * all;
+  const double threshold = (double)number * lds.all;
   // (where rounding leaves none above the threshold, the last that has a sum)
   if (own > 0.0) {
-    if (run > threshold) atomicMin(&found, tid);
-    atomicMax(&last, tid);
+    if (run > threshold) atomicMin(&lds.found, tid);
+    atomicMax(&lds.last, tid);
   }
   __syncthreads();
-  const uint32_t chunk = found != kNone ? found : last;
-  if (tid == chunk) before = run - own;
+  const uint32_t chunk = lds.found != kNone ? lds.found : lds.last;
+  if (tid == chunk) lds.before = run - own;
   __syncthreads();
   if (tid == 0) {
-    found = kNone;
-    last = 0;
+    lds.found = kNone;
+    lds.last = 0;
   }
-  const double left = threshold - before;
+  const double left = threshold - lds.before;
   const uint32_t first = chunk * kChunk + tid * kPickPer;
   double w[kPickPer];
   weights<BF16, WIDE>(w, p, plan, first, whole);
   own = 0.0;
 #pragma unroll
   for (int i = 0; i < (int)kPickPer; ++i) own += w[i];
-  run = running_sum(own, parts[2]);
+  run = running_sum(own, lds.parts[2]);
   if (own > 0.0) {
-    if (run > left) atomicMin(&found, tid);
-    atomicMax(&last, tid);
+    if (run > left) atomicMin(&lds.found, tid);
+    atomicMax(&lds.last, tid);
   }
   __syncthreads();
-  if (tid != (found != kNone ? found : last)) return;
+  if (tid != (lds.found != kNone ? lds.found : lds.last)) return;
   double sum = run - own;
   uint32_t token = 0;
   bool done = false;
@@ -467,6 +563,49 @@ __global__ __launch_bounds__(kPick) void verify_pick_kernel(VerifyArgs p) {
   p.out[(uint64_t)s * (p.most + 1) + plan.place] = token;
 }
 
+// (1024 threads of 4 columns each: 10.4 -> 11.7 us for one sequence)
+template <bool BF16, bool WIDE>
+__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs p) {
+  __shared__ PickRows lds;
+  const uint32_t s = blockIdx.x;
+  const Plan plan = p.plans[s];
+  if (plan.place == kNone) return;
+  const float number = p.sample[s];
+  const double own = plan.rejected && threadIdx.x < p.chunks ? p.rest[(uint64_t)s * p.chunks + threadIdx.x] : 0.0;
+  pick<BF16, WIDE>(p, s, plan, lds, number, chunk_of_p(p, s, plan), own);
+}
+
+// The three in one: every block of a sequence walks its drafts, the last that has
+// its chunk's sum written finds the token
+template <bool BF16, bool WIDE>
+__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
+  __shared__ WalkRows rows;
+  __shared__ Plan plan;
+  __shared__ PickRows lds;
+  __shared__ double sums[4];
+  __shared__ uint32_t order;
+  const uint32_t chunk = blockIdx.x % p.chunks, s = blockIdx.x / p.chunks;
+  const float number = p.sample[s];
+  walk<BF16>(p, s, chunk == 0, rows, plan);
+  __syncthreads();
+  if (plan.place == kNone || (!plan.rejected && chunk)) return;
+  double* const rest = p.rest + (uint64_t)s * p.chunks;
+  // (on its way before the chunk's sum is worked out)
+  const double of_p = chunk_of_p(p, s, plan);
+  double own = 0.0;
+  if (plan.rejected) {
+    const double sum = chunk_rest<BF16, WIDE>(p, plan, chunk, sums);
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(rest + chunk, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      order = __hip_atomic_fetch_add(p.done + s, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (order != p.chunks - 1) return;
+    if (threadIdx.x < p.chunks) own = __hip_atomic_load(rest + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  pick<BF16, WIDE>(p, s, plan, lds, number, of_p, own);
+}
+
 bool sizes_ok(uint32_t sequences, uint32_t most, uint32_t vocab) {
   return sequences && sequences <= kMaxSequences && most <= kMostDrafts && vocab && vocab <= kMaxVocab;
 }
@@ -475,22 +614,32 @@ uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 struct VerifyPlan {
-  uint64_t plans, rest, bytes;
+  uint64_t plans, rest, done, bytes;
 };
 VerifyPlan verify_plan(uint32_t sequences, uint32_t most, uint32_t vocab) {
   VerifyPlan v{};
   v.plans = padded((uint64_t)sequences * (2 * most + 1) * chunks_of(vocab) * sizeof(Stat));
   v.rest = v.plans + padded((uint64_t)sequences * sizeof(Plan));
-  v.bytes = v.rest + padded((uint64_t)sequences * chunks_of(vocab) * 8);
+  v.done = v.rest + padded((uint64_t)sequences * chunks_of(vocab) * 8);
+  v.bytes = v.done + padded((uint64_t)sequences * 4);
   return v;
 }
 
 template <bool BF16, bool WIDE>
 void launch(const VerifyArgs& p, hipStream_t s) {
   hipLaunchKernelGGL((verify_stats_kernel<BF16, WIDE>), dim3(p.sequences * p.rows * p.chunks), dim3(256), 0, s, p);
+  // One launch behind the first where its blocks, which repeat the walk, are at most
+  // three for two CUs; us, three -> one: 151936 columns of fp32 with a draft
+  // model's, 1 sequence (38 blocks) 25.5 -> 23.0, 4 27.2 -> 23.9, 32 (1216) 53.5 ->
+  // 56.3; 129280 of bf16, 8 (256) 28.3 -> 27.4, 12 (384) 30.5 -> 30.9, 16 31.9 -> 33.6;
+  // 32000, 1 (8) 23.7 -> 20.1, 32 (256) 30.9 -> 27.6
+  if (p.sequences * p.chunks <= kCus * 3 / 2) {
+    hipLaunchKernelGGL((verify_draw_kernel<BF16, WIDE>), dim3(p.sequences * p.chunks), dim3(256), 0, s, p);
+    return;
+  }
   hipLaunchKernelGGL((verify_walk_kernel<BF16>), dim3(p.sequences), dim3(256), 0, s, p);
   if (p.drafts) hipLaunchKernelGGL((verify_rest_kernel<BF16, WIDE>), dim3(p.sequences * p.chunks), dim3(256), 0, s, p);
-  hipLaunchKernelGGL((verify_pick_kernel<BF16, WIDE>), dim3(p.sequences), dim3(kPick), 0, s, p);
+  hipLaunchKernelGGL((verify_pick_kernel<BF16, WIDE>), dim3(p.sequences), dim3(256), 0, s, p);
 }
 
 }  // namespace
@@ -534,6 +683,7 @@ St LaunchDraftVerify(const DraftVerifyArgs& a) {
   p.stats = reinterpret_cast<Stat*>(ws);
   p.plans = reinterpret_cast<Plan*>(ws + plan.plans);
   p.rest = reinterpret_cast<double*>(ws + plan.rest);
+  p.done = reinterpret_cast<uint32_t*>(ws + plan.done);
   p.target_stride = a.target_stride;
   p.draft_stride = a.draft_stride;
   p.sequences = a.sequences;

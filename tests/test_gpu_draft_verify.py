@@ -177,6 +177,26 @@ def test_large_vocabulary(eng, dtype, soft):
     assert accepted > 0
 
 
+@pytest.mark.parametrize("vocab,sequences", [(9000, 127), (9000, 129), (9000, 200), (300, 500), (40960, 45)])
+@pytest.mark.parametrize("dtype,soft", [("float32", True), ("bfloat16", False)])
+def test_many_sequences(eng, vocab, sequences, dtype, soft):
+    """Enough of them that the walk and the draw are launches of their own, and
+    just not: masks, greedy ones, hardly any randomness, tokens outside and broken
+    rows among them."""
+    import numpy as np
+
+    counts = [i % 6 for i in range(sequences)]
+    t = [(1.0, 0.0, 0.6, 1e-3, 1.4, 0.8, 1e5)[i % 7] for i in range(sequences)]
+    case = _case(vocab + sequences, counts, vocab, dtype=dtype, soft=soft, temperature=t)
+    case["target"][::5, 20:] = float("-inf")
+    case["target"][3::17, 1:] = float("-inf")
+    case["tokens"][5::40] = vocab
+    case["target"][61] = float("-inf")
+    case["target"][90, 7] = float("nan")
+    case["accept"][1::9] = np.float32(1 - 2.0 ** -24)
+    assert _check(case, 6)[2] == 5
+
+
 def test_random_numbers_at_their_ends(eng):
     """0 accepts what has a probability and takes the first token that has one;
     the largest number below 1 the last."""
