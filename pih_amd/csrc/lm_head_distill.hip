@@ -106,42 +106,36 @@ __global__ __launch_bounds__(256) void distill_sort_kernel(const uint32_t* ids, 
   }
 }
 
-// z of every entry, by a wave: a dot product over the hidden size
+// z of an entry, by a wave: a dot product over the hidden size; 0 for none
+__device__ __forceinline__ float entry_logit(const uint16_t* a, const uint16_t* w, uint32_t id, uint32_t vocab,
+                                             uint32_t hidden) {
+  if (id >= vocab) return 0.0f;
+  const uint16_t* const b = w + (uint64_t)id * hidden;
+  float sum = 0.0f;
+  for (uint32_t c = (threadIdx.x & 63) * 8; c < hidden; c += 512) {
+    const v4i u = *reinterpret_cast<const v4i*>(a + c), v = *reinterpret_cast<const v4i*>(b + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t p = (uint32_t)u[i], q = (uint32_t)v[i];
+      sum = __builtin_fmaf(bf16_bits_to_f32(p & 0xffffu), bf16_bits_to_f32(q & 0xffffu), sum);
+      sum = __builtin_fmaf(bf16_bits_to_f32(p >> 16), bf16_bits_to_f32(q >> 16), sum);
+    }
+  }
+  return reduce_sum_xor<64>(sum);
+}
+
 __global__ __launch_bounds__(256) void distill_gather_kernel(const uint16_t* x, const uint16_t* w, const uint32_t* ids,
                                                              float* logits, uint64_t entries, uint32_t top_k,
                                                              uint32_t vocab, uint32_t hidden) {
-  const uint32_t lane = threadIdx.x & 63;
   for (uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); at < entries; at += (uint64_t)gridDim.x * 4) {
-    const uint32_t id = ids[at];
-    float sum = 0.0f;
-    if (id < vocab) {
-      const uint16_t* const a = x + at / top_k * hidden;
-      const uint16_t* const b = w + (uint64_t)id * hidden;
-      for (uint32_t c = lane * 8; c < hidden; c += 512) {
-        const v4i u = *reinterpret_cast<const v4i*>(a + c), v = *reinterpret_cast<const v4i*>(b + c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t p = (uint32_t)u[i], q = (uint32_t)v[i];
-          sum = __builtin_fmaf(bf16_bits_to_f32(p & 0xffffu), bf16_bits_to_f32(q & 0xffffu), sum);
-          sum = __builtin_fmaf(bf16_bits_to_f32(p >> 16), bf16_bits_to_f32(q >> 16), sum);
-        }
-      }
-      sum = reduce_sum_xor<64>(sum);
-    }
-    if (lane == 0) logits[at] = sum;
+    const float v = entry_logit(x + at / top_k * hidden, w, ids[at], vocab, hidden);
+    if ((threadIdx.x & 63) == 0) logits[at] = v;
   }
 }
 
-// A row's pairs joined and its loss, by a wave
-__global__ __launch_bounds__(256) void distill_join_kernel(const float2* stats, const uint32_t* ids,
-                                                           const float* teacher, const float* teacher_lse,
-                                                           const float* logits, float* loss, float* lse, uint32_t* err,
-                                                           uint32_t rows, uint32_t vocab, uint32_t tiles, uint32_t top_k,
-                                                           float temperature) {
-  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  const float2* s = stats + (uint64_t)row * tiles;
-  const float inverse = 1.0f / temperature;
+// A row's pairs joined to its log-sum-exp, by a wave
+__device__ __forceinline__ float joined(const float2* s, uint32_t tiles, float inverse) {
+  const uint32_t lane = threadIdx.x & 63;
   float top = -INFINITY, sum = 0.0f;
 #pragma unroll 8
   for (uint32_t i = lane; i < tiles; i += 64) top = fmaxf(top, s[i].x);
@@ -149,18 +143,19 @@ __global__ __launch_bounds__(256) void distill_join_kernel(const float2* stats, 
   // (a tile of -inf or NaN alone has the sum 0 or NaN, whatever the factor)
 #pragma unroll 8
   for (uint32_t i = lane; i < tiles; i += 64) sum += s[i].x == -INFINITY ? s[i].y : s[i].y * expf((s[i].x - top) * inverse);
-  sum = reduce_sum_xor<64>(sum);
-  const float l = top * inverse + logf(sum);
-  Entries e;
-  const uint64_t at = (uint64_t)row * top_k;
-  const bool bad = load_entries(e, ids, teacher, at, top_k, vocab, inverse);
-  const float norm = normalizer(e, teacher_lse, row);
+  return top * inverse + logf(reduce_sum_xor<64>(sum));
+}
+// A row's loss, by a wave; z: its entries' logits
+__device__ __forceinline__ void row_loss(const Entries& e, bool bad, const float* teacher_lse, const float* z, float l,
+                                         float* loss, float* lse, uint32_t* err, uint32_t row, float temperature) {
+  const uint32_t lane = threadIdx.x & 63;
+  const float inverse = 1.0f / temperature, norm = normalizer(e, teacher_lse, row);
   float total = 0.0f;
 #pragma unroll
   for (uint32_t i = 0; i < kTopMax / 64; ++i) {
     const float q = probability(e.s[i], norm);
     // (an entry of probability 0 adds nothing, whatever its logit)
-    if (q != 0.0f) total += q * ((e.s[i] - norm) - (logits[at + lane + 64 * i] * inverse - l));
+    if (q != 0.0f) total += q * ((e.s[i] - norm) - (z[lane + 64 * i] * inverse - l));
   }
   total = reduce_sum_xor<64>(total) * temperature * temperature;
   uint32_t bits = __builtin_amdgcn_ballot_w64(bad) ? kErrTarget : 0;
@@ -169,6 +164,47 @@ __global__ __launch_bounds__(256) void distill_join_kernel(const float2* stats, 
   lse[row] = l;
   loss[row] = total;
   if (bits) atomicOr(err, bits);
+}
+
+// Rows whose entries' logits are there, a wave each
+__global__ __launch_bounds__(256) void distill_join_kernel(const float2* stats, const uint32_t* ids,
+                                                           const float* teacher, const float* teacher_lse,
+                                                           const float* logits, float* loss, float* lse, uint32_t* err,
+                                                           uint32_t rows, uint32_t vocab, uint32_t tiles, uint32_t top_k,
+                                                           float temperature) {
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const uint64_t at = (uint64_t)row * top_k;
+  const float l = joined(stats + (uint64_t)row * tiles, tiles, 1.0f / temperature);
+  Entries e;
+  const bool bad = load_entries(e, ids, teacher, at, top_k, vocab, 1.0f / temperature);
+  row_loss(e, bad, teacher_lse, logits + at, l, loss, lse, err, row, temperature);
+}
+
+// A row by eight waves: one joins its pairs while the others work out its entries'
+// logits
+__global__ __launch_bounds__(512) void distill_row_kernel(const uint16_t* x, const uint16_t* w, const float2* stats,
+                                                          const uint32_t* ids, const float* teacher,
+                                                          const float* teacher_lse, float* logits, float* loss, float* lse,
+                                                          uint32_t* err, uint32_t vocab, uint32_t hidden, uint32_t tiles,
+                                                          uint32_t top_k, float temperature) {
+  __shared__ float z[kTopMax];
+  const uint32_t row = blockIdx.x, wave = threadIdx.x >> 6;
+  const uint64_t at = (uint64_t)row * top_k;
+  float l = 0.0f;
+  bool bad = false;
+  Entries e;
+  if (wave == 0) {
+    l = joined(stats + (uint64_t)row * tiles, tiles, 1.0f / temperature);
+    bad = load_entries(e, ids, teacher, at, top_k, vocab, 1.0f / temperature);
+  } else {
+    for (uint32_t k = wave - 1; k < top_k; k += 7) {
+      const float v = entry_logit(x + (uint64_t)row * hidden, w, ids[at + k], vocab, hidden);
+      if ((threadIdx.x & 63) == 0) z[k] = logits[at + k] = v;
+    }
+  }
+  __syncthreads();
+  if (wave == 0) row_loss(e, bad, teacher_lse, z, l, loss, lse, err, row, temperature);
 }
 
 // What the backward pass needs of a row's teacher, by a wave: live 0
@@ -248,6 +284,10 @@ bool listed(uint32_t rows, uint32_t vocab, uint32_t hidden, uint32_t top_k) {
   const float rounds = (float)rows * vocab / (65536.0f * kCus);
   return big_takes(hidden) && (float)rows * top_k * hidden * (2.0f / 8.0e6f) > 6.0f + 4.0f * rounds;
 }
+// Whether a row's entries are few enough for the waves beside the one that joins it,
+// us, two launches -> one: 33 rows over 151936 x 1024, 20 entries 68.5 -> 65.1, 64
+// 69.2 -> 71.9; over 129280 x 4096, 1 entry 200 -> 196, 20 199 -> 201.5
+bool by_row(uint32_t hidden, uint32_t top_k) { return top_k * hidden <= 1u << 15; }
 // the forward pass's workspace: the rows' pairs, and for the tiles fed by DMA the
 // entries in order and how many lie before each tile
 struct DistillForward {
@@ -349,6 +389,12 @@ St LaunchLmHeadDistill(const LmHeadDistillArgs& a) {
     g.stats = stats;
     g.inverse = 1.0f / a.temperature;
     launch_gemm<kEpiTeacherStats>(g, a.stream);
+  }
+  if (!in_tiles && by_row(a.hidden, a.top_k)) {
+    hipLaunchKernelGGL(distill_row_kernel, dim3(a.rows), dim3(512), 0, a.stream, a.x, a.w, stats, a.ids, a.teacher,
+                       a.teacher_lse, a.logits, a.loss, a.lse, a.error_flag, a.vocab, a.hidden, tiles, a.top_k,
+                       a.temperature);
+    return AfterLaunch("lm_head_distill_launch_failed");
   }
   if (!in_tiles) {
     const uint64_t entries = (uint64_t)a.rows * a.top_k;
