@@ -18,6 +18,11 @@
 // per sequence that finds the chunk and in it the token.  (The last two in one for
 // many, the token found by the last of a sequence's blocks: 57 sequences 21 -> 24
 // us, 256 46 -> 58.)
+//
+// Measured: 1 sequence of 5 drafts over 151936 columns of fp32 23 us (two launches of
+// 5 and 18, dependent loads), 57 of up to 7 over 129280 of bf16, looked up, 52-54, 256
+// of up to 4 over 151936 of fp32 200-215 (the statistics 778 MB at 4.4 TB/s with the
+// vector units busy in 85 % of the cycles).
 #include "dense_route.hpp"
 #include "device_common.hpp"
 #include "kernels.hpp"

@@ -5,10 +5,28 @@
 // with gate clamped from above and up from both sides where there is a limit
 // (no gradient beyond it).
 //
-// h, dgate and dup are rounded to bf16 for the matrix cores: 2^-9 of each
+// h, dgate and dup are rounded to bf16 for the matrix cores: 2^-8 of each
 // element at most, independent from element to element, in sums that are
-// rounded to bf16 once themselves.  gate, up and dh stay in fp32 between
-// their product and the activation.
+// rounded to bf16 once themselves (y, dx and the weights' gradients 0.23 % of
+// their norm off 64 bits, 0.17 % of it their own rounding).  gate, up and dh stay
+// in fp32 between their product and the activation.
+//
+// Forward two products, backward four, of which a product with too few tiles for
+// the CUs has k in parts, joined by a launch of its own.  Gate and up are one
+// product whose tile holds 16 columns of each in turn, so that a wave has both of
+// an element and leaves h; dh's tile reads gate and up and leaves dgate and dup
+// side by side, so that dx is one product over both weights and their gradients
+// one over both halves, and h for dWd.
+//
+// Measured: 1 row of 4096 x 2048 15 us (50 MB; the host's time of a call), 57 rows
+// of 4096 x 12288 69 us (302 MB at 4.4 TB/s: gate and up 5.4, down 4.6), 4099 rows
+// with gate and up kept 0.98 ms (1.27 PFLOP/s); gradients of 4096 rows 2.08 ms (1.19
+// PFLOP/s), of 509 rows of 7168 x 2048 146 us (0.62 PFLOP/s).  Many rows: the matrix
+// pipe at the clock that power leaves (1.9 GHz; a library product of 4096 x 24576 x
+// 4096 650-750 us over and over, 550 with pauses, gate and up here 730-780), and in
+// the gradients what the tiles of a round write at once (dh's 165 MB, ~50 us of a
+// round) and the transposing reads of the weights' gradients (12 % more cycles).
+// Few rows: the weights' bytes; 509 rows: 64-row tiles, bound by what a CU takes in.
 #include "dense_route.hpp"
 #include "dma_tile.hpp"
 #include "tile64.hpp"
@@ -197,7 +215,9 @@ bool shape_ok(uint32_t rows, uint32_t inter, uint32_t hidden) {
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 dim3 tiles64(uint32_t m, uint32_t n) { return dim3((n + kT64 - 1) / kT64, (m + kT64 - 1) / kT64); }
-// the tiles fed by DMA take 64-deep steps of every product
+// The tiles fed by DMA take 64-deep steps of every product; other sizes run on 64 x 64
+// tiles, us at 1024 rows of 1024 x 4096 -> of 1000 x 4008: forward 41 -> 178, gradients
+// 131 -> 507; at 1 row 13 -> 116 and 42 -> 224
 bool dma_takes(uint32_t inter, uint32_t hidden) { return inter % KB == 0 && hidden % KB == 0; }
 // Few rows: the tiles of gemm_tile.hip, chosen per shape for all CUs without
 // splits, against the route here, by both estimates (what those tiles take is
