@@ -220,15 +220,18 @@ dim3 tiles64(uint32_t m, uint32_t n) { return dim3((n + kT64 - 1) / kT64, (m + k
 // 131 -> 507; at 1 row 13 -> 116 and 42 -> 224
 bool dma_takes(uint32_t inter, uint32_t hidden) { return inter % KB == 0 && hidden % KB == 0; }
 // Few rows: the tiles of gemm_tile.hip, chosen per shape for all CUs without
-// splits, against the route here, by both estimates (what those tiles take is
-// underestimated by 15 % against these).  Forward pass, us, route -> tiles for
+// splits, against the route here, by both estimates (what those tiles take, in pairs
+// or walked by a block per CU, is underestimated by 15 % against these: 4096 x 12288,
+// down on them in spite of it at 180 rows 106 -> 97 us, at 257 147 -> 139, but walked
+// at 2049 552 -> 585, and gate and up at 180 rows 106 -> 114).  Forward pass, us, route -> tiles for
 // gate and up -> for down too: 1 row of 4096 x 2048 23.8 -> 19.1 -> 15.9, of 4096
 // x 12288 64.9 -> 57.1 -> 52.0; 57 rows 35.0 -> 25.0 -> 19.1 and 78.9 -> 67.4 ->
 // 58.7; 512 rows 59.2 -> 51.6 -> 43.0, but 157.9 -> 209.4 -> 223.8.  The same
 // choice for the rows behind the whole 256 of a route: 1030 rows of 4096 x 12288
 // 334 -> 321, 4099 rows 964 -> 943.
 bool tiles_faster(uint32_t m, uint32_t n, uint32_t k, bool pair, float route_us) {
-  return 1.15 * PickTile(true, m, n, 2 * k, 1, pair).us < route_us;
+  const TilePick t = PickTile(true, m, n, 2 * k, 1, pair);
+  return (pair || t.grid ? 1.15 : 1.0) * t.us < route_us;
 }
 struct ForwardPlan {
   Route up, down;
