@@ -777,7 +777,8 @@ Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
   p.n = n;
   p.k = k;
   Tiling best{256, 1, INFINITY};
-  for (uint32_t rows : {64u, 128u, 256u})
+  for (uint32_t rows : {64u, 128u, 256u}) {
+    if (m <= rows / 2 && rows > 64) break;  // (as many tiles as of half the rows, each slower)
     for (uint32_t splits = 1; splits <= 64 && k / KB / splits >= 4; ++splits) {
       // (no split is empty)
       const uint32_t steps = k / KB, part = (steps + splits - 1) / splits;
@@ -789,6 +790,7 @@ Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
                        (splits > 1 ? 7.0f + (float)splits * m * n * (8.0f / 4.0e6f) : 0.0f);
       if (us < best.us) best = {rows, splits, us};
     }
+  }
   return best;
 }
 // All rows alike, or the whole 256 without splits and the rest by itself, where B
