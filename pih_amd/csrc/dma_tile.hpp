@@ -49,7 +49,15 @@ constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherG
 // half's fragments are read; then one wait and one barrier (every wave has
 // read the step, and the next one has arrived), and while the MFMAs of the
 // second run, the next step's first fragments are read and another step is
-// sent for, into the buffer just freed.  A block per CU walks its tiles; the
+// sent for, into the buffer just freed.  With two steps resident the wait for
+// the next one stands, with a barrier of its own, in the middle of the second
+// half, and its fragments are read in the rest.  Reads and DMAs are issued one
+// by one between MFMAs, which run for four issues each: in front of a group's
+// eight the matrix pipe ran dry.  (Both together: the block's forward pass of 4099
+// rows of 4096 x 12288 958 -> 920 us, its gradients of 4096 2046 -> 1964; the loss of
+// 4096 rows over 129280 x 4096 3100 -> 2960, its gradients 9706 -> 9335; a half of it
+// from the order of issue, a half from the wait.  The wait three, five or six eighths
+// into the half: no better; DMAs all at its start: 4-8 % slower.)  A block per CU walks its tiles; the
 // next tile's first steps are sent for before the results of this one are
 // worked on.
 // (Eight waves, two to a SIMD, that take turns on 32-deep halves, so that one's
@@ -283,21 +291,24 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   v4i fa[2][MB], fb[2][NB];
   // the fragments of a half, three or four beside each group of NB MFMAs: B's
   // first, which the next half's first group needs, and all of them a group or
-  // two early
+  // two early (kLate: of the next step where two are resident, beside the last half
+  // of the groups)
+  constexpr uint32_t kLate = (MB + NB) / (MB / 2);
   constexpr uint32_t kReads = (MB + NB + MB - 2) / (MB - 1);
   auto read_one = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
     if (i < (uint32_t)NB) fb[to][i] = frag(bt, s * S::kStage + S::kA, wn * NB * 16 + 16 * i, q);
     else if (i < (uint32_t)(NB + MB)) fa[to][i - NB] = frag(at, s * S::kStage, wm * MB * 16 + 16 * (i - NB), q);
   };
-  auto read_group = [&](uint32_t s, uint32_t q, int to, uint32_t i) __attribute__((always_inline)) {
+  // NB MFMAs, with beside(j) issued while MFMA j runs
+  auto multiply = [&](int from, uint32_t i, auto&& beside) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t e = kReads * i; e < kReads * i + kReads; ++e) read_one(s, q, to, e);
-  };
-  auto multiply = [&](int from, uint32_t i) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int j = 0; j < NB; ++j) {
       acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, fb[from][j]),
                                                           __builtin_bit_cast(v8bf, fa[from][i]), acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      beside((uint32_t)j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     pin(acc[i]);
   };
   uint32_t s;  // the buffer of the step being multiplied
@@ -309,19 +320,14 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     const uint32_t ns = s + 1 == ST ? 0 : s + 1;
 #pragma unroll
     for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
-      // (the first MFMAs wait for every LDS read before them)
-      if (i == 0) {
-        multiply(0, i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      read_group(s, 1, 1, i);
-      if (i) multiply(0, i);
-      __builtin_amdgcn_sched_barrier(0);
+      multiply(0, i, [&](uint32_t j) __attribute__((always_inline)) {
+        if (j < kReads) read_one(s, 1, 1, kReads * i + j);
+      });
     }
-    // this step read by this wave, the next one arrived for it (the first ST
-    // had before the tile was begun); then by all
+    // this step read by this wave (and three resident: the next one arrived for it;
+    // the first ST had before the tile was begun); then by all
     __builtin_amdgcn_s_waitcnt(kLdsRead);
-    if (j + 1 >= (uint32_t)ST) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(decltype(LEFT)::value * NL));
+    if (ST != 2 && j + 1 >= (uint32_t)ST) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(decltype(LEFT)::value * NL));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     const uint32_t step = s0 + j + ST;
@@ -333,14 +339,32 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     }
 #pragma unroll
     for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
-      if constexpr (kNext) read_group(ns, 0, 0, i);
-      if constexpr (kMore) {
-#pragma unroll
-        for (uint32_t e = i * NL / MB; e < (i + 1) * NL / MB; ++e)
-          issue(sa, sb, s, e, kLast && (step + 1) * KB > p.k_valid, step);
+      if constexpr (kNext && ST == 2) {
+        if (i == MB / 2) {
+          // the next step arrived for this wave (half of the one after it is sent
+          // for), then for all
+          if (j + 1 >= (uint32_t)ST) __builtin_amdgcn_s_waitcnt(vmcnt_at_most(kMore ? NL / 2 : 0));
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
       }
-      multiply(1, i);
-      __builtin_amdgcn_sched_barrier(0);
+      multiply(1, i, [&](uint32_t j) __attribute__((always_inline)) {
+        if constexpr (kNext) {
+          if constexpr (ST == 2) {
+            if (i >= MB / 2 && j < kLate) read_one(ns, 0, 0, kLate * (i - MB / 2) + j);
+          } else {
+            if (j < kReads) read_one(ns, 0, 0, kReads * i + j);
+          }
+        }
+        if constexpr (kMore) {
+          // (DMAs behind the reads, MFMAs between them)
+          const uint32_t first = i * NL / MB, count = (i + 1) * NL / MB - first;
+#pragma unroll
+          for (uint32_t e = 0; e < count; ++e)
+            if (j == min(kReads + 2 * e, (uint32_t)NB - 1))
+              issue(sa, sb, s, first + e, kLast && (step + 1) * KB > p.k_valid, step);
+        }
+      });
     }
     s = ns;
   };
