@@ -37,7 +37,7 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // order, and the compiler's count, which omits the DMA, only waits longer).
 // M0 is written here only; nothing else in these kernels uses it.
 // The address is a wave-uniform base (SGPRs) plus a per-lane 32-bit offset,
-// or (dma4v) a per-lane 64-bit address.
+// or (dma4v, dma16v) a per-lane 64-bit address.
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
                : "memory");
@@ -52,6 +52,10 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 }
 __device__ __forceinline__ void dma4v(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
+}
+
+__device__ __forceinline__ void dma16v(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
 typedef int v8i __attribute__((ext_vector_type(8)));

@@ -65,11 +65,14 @@ constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherG
 // and over, with more LDS traffic: power sets the clock, 1.9 GHz of 2.4.)
 constexpr uint32_t TB = 256, KB = 64;
 
+// 16 bytes of a row that is not there
+__device__ const v4i kNoRow{0, 0, 0, 0};
+
 struct BigArgs {
   const uint16_t* a;
   const uint16_t* b;
   uint32_t m, n, k;        // k a multiple of 64
-  uint32_t k_valid;        // columns layout of B: k rows that exist (the others repeat the last)
+  uint32_t k_valid;        // columns layout of B: k rows that exist (kEpiAdd, kEpiStore; the others are zeros)
   uint64_t lda, ldb;
   void* out;
   uint64_t ldo;
@@ -193,36 +196,33 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   };
   constexpr std::bool_constant<AT> at{};
   constexpr std::bool_constant<BT> bt{};
-  // DMA i of a step (A's first) into buffer s
-  auto issue = [&](const uint8_t* sa, const uint8_t* sb, uint32_t s, uint32_t i, bool short_b,
+  // a step may have fewer than 64 k rows of an operand, the last one
+  constexpr bool kShort = BT && (EPI == kEpiAdd || (AT && EPI == kEpiStore));
+  const uint32_t k_whole = AT && EPI == kEpiStore ? min(p.a_valid, p.k_valid) : p.k_valid;
+  // DMA i of a step (A's first) into buffer s; CUT: such a step.  The rows that are
+  // not there are read as zeros: the other operand's are, but a repeated row that
+  // holds an infinity would make NaN of them.
+  auto issue = [&](const uint8_t* sa, const uint8_t* sb, uint32_t s, uint32_t i, auto CUT,
                    uint32_t step) __attribute__((always_inline)) {
+    constexpr bool kCut = decltype(CUT)::value;
     const uint32_t lds = lds0 + s * S::kStage + wave * 1024;
+    auto source_of = [&](const uint8_t* base, uint32_t off, uint32_t i, uint32_t valid) __attribute__((always_inline)) {
+      const uint32_t row = step * KB + 8 * i + 2 * wave + (lane >> 5);
+      return row < valid ? base + off : reinterpret_cast<const uint8_t*>(&kNoRow);
+    };
     if (i < (uint32_t)LA) {
-      uint32_t oa = off_a[i];
-      if constexpr (AT && EPI == kEpiStore) {
-        if ((step + 1) * KB > p.a_valid) {
-          const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.a_valid - 1 - step * KB;
-          if (r > last) oa -= (uint32_t)((r - last) * p.lda * 2);
-        }
-      }
-      dma16(sa, oa, lds + i * 4096);
+      if constexpr (kCut && AT) dma16v(source_of(sa, off_a[i], i, p.a_valid), lds + i * 4096);
+      else dma16(sa, off_a[i], lds + i * 4096);
     } else {
       i -= LA;
-      uint32_t ob = off_b[i];
-      if constexpr (BT) {
-        if (short_b) {
-          // k rows past the last repeat it (their factors in A are 0)
-          const uint32_t r = 8 * i + 2 * wave + (lane >> 5), last = p.k_valid - 1 - step * KB;
-          if (r > last) ob -= (uint32_t)((r - last) * p.ldb * 2);
-        }
-      }
       // (few rows: the weights past the caches.  Of one row tile they are read
       // once: dx of 33 rows over 151936 x 1024 92 -> 72 us, the loss of 128 rows
       // 84 -> 79.  With two or three row tiles it still gains: the loss of 300
       // rows 150 -> 135 there, 435 -> 392 over 129280 x 4096, of 200 rows over
       // 32768 x 1024 26 -> 25; the other way dx of 128 rows there, 60 -> 67)
-      if constexpr (ROWS <= 128) dma16nt(sb, ob, lds + S::kA + i * 4096);
-      else dma16(sb, ob, lds + S::kA + i * 4096);
+      if constexpr (kCut) dma16v(source_of(sb, off_b[i], i, p.k_valid), lds + S::kA + i * 4096);
+      else if constexpr (ROWS <= 128) dma16nt(sb, off_b[i], lds + S::kA + i * 4096);
+      else dma16(sb, off_b[i], lds + S::kA + i * 4096);
     }
   };
   // kEpiTeacherStats: of row tid of the tile the first and the end of its listed
@@ -250,9 +250,12 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       if (q >= steps) break;
       const uint8_t* sa = source(at, base_a, p.lda, s0 + q);
       const uint8_t* sb = source_b(s0 + q);
-      const bool short_b = BT && (s0 + q + 1) * KB > p.k_valid;
+      auto all = [&](auto CUT) __attribute__((always_inline)) {
 #pragma unroll
-      for (uint32_t i = 0; i < (uint32_t)NL; ++i) issue(sa, sb, q, i, short_b, s0 + q);
+        for (uint32_t i = 0; i < (uint32_t)NL; ++i) issue(sa, sb, q, i, CUT, s0 + q);
+      };
+      if (kShort && (s0 + q + 1) * KB > k_whole) all(std::bool_constant<kShort>{});
+      else all(std::false_type{});
     }
     if constexpr (EPI == kEpiStats || has_grad(EPI)) {
       if (tid < ROWS) {
@@ -313,10 +316,9 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
   };
   uint32_t s;  // the buffer of the step being multiplied
   // kNext: the next step exists, with kLeft further steps in flight behind it;
-  // kMore: step j + ST exists and is sent for (kLast: it is the last one,
-  // whose k rows may be short)
-  auto body = [&](uint32_t j, auto NEXT, auto LEFT, auto MORE, auto LAST) __attribute__((always_inline)) {
-    constexpr bool kNext = decltype(NEXT)::value, kMore = decltype(MORE)::value, kLast = decltype(LAST)::value;
+  // kMore: step j + ST exists and is sent for (CUT: it is cut short)
+  auto body = [&](uint32_t j, auto NEXT, auto LEFT, auto MORE, auto CUT) __attribute__((always_inline)) {
+    constexpr bool kNext = decltype(NEXT)::value, kMore = decltype(MORE)::value;
     const uint32_t ns = s + 1 == ST ? 0 : s + 1;
 #pragma unroll
     for (uint32_t i = 0; i < (uint32_t)MB; ++i) {
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
 #pragma unroll
           for (uint32_t e = 0; e < count; ++e)
             if (j == min(kReads + 2 * e, (uint32_t)NB - 1))
-              issue(sa, sb, s, first + e, kLast && (step + 1) * KB > p.k_valid, step);
+              issue(sa, sb, s, first + e, CUT, step);
         }
       });
     }
@@ -409,8 +411,8 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
       for (uint32_t i = 0; i < (uint32_t)(MB + NB); ++i) read_one(0, 0, 0, i);
       uint32_t j = 0;
 #pragma unroll 1
-      for (; j + ST + (BT ? 1 : 0) < steps; ++j) body(j, yes, full, yes, no);
-      if constexpr (BT)
+      for (; j + ST + (kShort && (s0 + steps) * KB > k_whole ? 1 : 0) < steps; ++j) body(j, yes, full, yes, no);
+      if constexpr (kShort)
         if (j + ST < steps) body(j++, yes, full, yes, yes);
       if constexpr (ST == 3)
         if (j + 2 < steps) body(j++, yes, std::integral_constant<int, 1>{}, no, no);

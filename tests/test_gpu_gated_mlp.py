@@ -354,3 +354,32 @@ def test_rows_past_4_gib(eng, hidden, inter):
     # (their sums run over all rows, most of them zeros)
     for what, g, w in zip(("dx", "dw_gate", "dw_up", "dw_down"), (got[0][-few:],) + got[1:], want):
         _within(g, w, what)
+
+
+def _same_nonfinite(got, want, what):
+    """NaN and infinities where the 64-bit form has them, and nowhere else."""
+    import torch
+
+    for name, mask in (("NaN", torch.isnan), ("inf", torch.isposinf), ("-inf", torch.isneginf)):
+        assert torch.equal(mask(got).cpu(), mask(want)), (what, name)
+
+
+@pytest.mark.parametrize("rows,hidden,inter", [(1, 64, 64), (3, 64, 128), (70, 256, 512), (129, 320, 192), (300, 512, 256),
+                                               (509, 1024, 512), (64, 64, 128), (5, 72, 136)])
+@pytest.mark.parametrize("where", ["dy", "x"])
+def test_infinity_in_the_last_row_of_the_weights_gradients(eng, rows, hidden, inter, where):
+    """An infinite element of the last row: what the sums over the rows make of it is
+    theirs alone, also where the rows are no multiple of the products' steps."""
+    import torch
+
+    from pih_amd.linear import gated_mlp_backward
+
+    x, wg, wu, wd, dy = _case(rows + inter, rows, hidden, inter)
+    gate, up = ((x.double() @ w.double().T).to(torch.bfloat16) for w in (wg, wu))
+    (dy if where == "dy" else x)[-1, hidden // 3] = float("inf")
+    want = _backward_ref(dy, x, wg, wu, wd, gate, up, 0.0)
+    got = gated_mlp_backward(*(t.cuda() for t in (dy, x, wg, wu, wd, gate, up)))
+    torch.cuda.synchronize()
+    for what, g, (w, _) in zip(("dx", "dw_gate", "dw_up", "dw_down"), got, want):
+        _same_nonfinite(g, w, what)
+    assert torch.isinf(want[3][0] if where == "dy" else want[1][0]).any()

@@ -400,3 +400,42 @@ def test_weights_past_4_gib(eng):
     dx, dw, _ = lm_head_distill_backward(x, w, ids, teacher, got[1], got[2], up)
     _within(dx, want[0], "dx")
     _within(dw, want[1], "dw")
+
+
+@pytest.mark.parametrize("rows,vocab,hidden", [(1, 70, 64), (33, 1000, 128), (130, 2050, 192), (300, 5000, 256), (40, 777, 72),
+                                               (16, 1024, 64)])
+@pytest.mark.parametrize("loss", ["teacher", "target"])
+def test_infinite_last_weight(eng, rows, vocab, hidden, loss):
+    """The last vocabulary entry's weight holds an infinity at a column that is
+    negative in every row: its logit is -inf, its probability 0.  Of the row whose
+    teacher (or target) is sure of that entry, dx is -up times the weight there, an
+    infinity; in the column 0 x inf of the other rows is NaN, and everything else is
+    finite."""
+    import torch
+
+    from pih_amd.linear import (lm_head_distill, lm_head_distill_backward, lm_head_loss, lm_head_loss_backward)
+
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    x = torch.randn(rows, hidden, generator=g, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(vocab, hidden, generator=g, device="cuda") * hidden ** -0.5).to(torch.bfloat16)
+    up = torch.rand(rows, generator=g, device="cuda") + 0.5
+    column, row = hidden // 3, rows // 2
+    x[:, column] = -x[:, column].abs() - 0.1
+    w[-1, column] = float("inf")
+    target = torch.arange(rows, device="cuda", dtype=torch.int32) % (vocab - 1)
+    target[row] = vocab - 1
+    if loss == "target":
+        _, lse, flag = lm_head_loss(x, w, target)
+        dx, dw, _ = lm_head_loss_backward(x, w, target, lse, up)
+    else:
+        entries = target[:, None].contiguous(), torch.zeros(rows, 1, device="cuda")
+        _, lse, z, flag = lm_head_distill(x, w, *entries)
+        dx, dw, _ = lm_head_distill_backward(x, w, *entries, lse, z, up)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 4  # (that row's loss is infinite)
+    assert torch.isfinite(lse).all() and torch.isfinite(dw).all()
+    rest = torch.arange(hidden, device="cuda") != column
+    assert torch.isfinite(dx[:, rest]).all()
+    assert torch.isneginf(dx[row, column])
+    others = torch.arange(rows, device="cuda") != row
+    assert torch.isnan(dx[others, column]).all()
