@@ -219,6 +219,24 @@ inline bool Bf16OnTiles(uint32_t m, uint32_t n, uint32_t k, bool f32_out, bool b
   return m <= 64 || !big || !BigTilesFaster(true, m, n, k, 1, f32_out, t, k_splits);
 }
 
+// Whether a BF16 GEMM that has no workspace, its operands on 16-byte borders, runs
+// on the tile that PickTile chooses, or up to 128 rows on the 128 x 256 tiles of
+// very wide weights, whose time is that of the weights too: PickTile's estimate
+// holds for it
+inline bool Bf16EstimateHolds(uint32_t m, uint32_t n, uint32_t k) {
+  if (m >= 2 && m <= 128 && Bf16Wide(m, n, k)) return true;
+  if (k % 128 || n % 16 || (uint64_t)m * k * 2 > 0xffffffffull) return false;
+  const bool big = (Bf16BigTiles(m, n, k) || Bf16Wide(m, n, k)) && (uint64_t)n * k * 2 <= 0xffffffffull;
+  return Bf16OnTiles(m, n, k, false, big, 1, PickTile(true, m, n, 2 * k, 1));
+}
+// Estimate of the BF16 GEMV (m <= 64), us: the weights, from HBM at 6.2 TB/s or into
+// a CU at 32 KB/us, and the rows, which a CU reads again from L2 for every 16 weight
+// rows at 17 KB/us (those of 32 KB stay in its L1)
+inline double Bf16GemvUs(uint32_t m, uint32_t n, uint32_t k) {
+  const double rounds = (n / 16 + kCus - 1) / kCus, rows = 2.0 * m * k;
+  return std::max((double)n * k * 2.0 / 6.2e6, rounds * k / 1e3) + (rows > 32768.0 ? rounds * rows / 17e3 : 0.0);
+}
+
 // W4A16 (w4a16_tile.hip), count problems of n[i] rows, shapes that it runs (k %
 // 512 == 0): the 16-row weight blocks of a tile, or 0 for the GEMV kernels.  By
 // measurement (one MI355X, asymmetric, us GEMV -> here; blocks: 16-row weight

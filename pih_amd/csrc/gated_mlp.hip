@@ -253,10 +253,16 @@ ForwardPlan forward_plan(uint32_t rows, uint32_t inter, uint32_t hidden) {
     t.k = hidden;
     return TileGluTakes(t) && tiles_faster(m, 2 * inter, hidden, true, us);
   };
-  // (LaunchBf16Gemm, which takes whole 128 columns above 64 rows, and 32-bit offsets into h)
+  // LaunchBf16Gemm, where it runs those tiles, or up to 64 rows the GEMV, which takes
+  // the intermediate sizes that those do not (inter % 128 == 64).  Forward pass, us,
+  // route -> GEMV for down at 8, 17, 33 and 64 rows: 12352 -> 4096 53.6 -> 51.8, 55.6 ->
+  // 59.8, 59.8 -> 71.0, 64.3 -> 91; 4160 -> 1024 16.5 -> 14.8, 17.5 -> 17.8, 19.0 -> 22.4,
+  // 21.5 -> 30.7; 2112 -> 4096 20.5 -> 15.7, 22.5 -> 18.0, 25.4 -> 22.3, 30.9 -> 29.0.  Above
+  // 64 rows it would run them on the 128 x 256 tiles without splits: 12352 -> 4096
+  // at 192 rows 104 on the route, 152 there, 5696 -> 2048 at 65 rows 32 and 68.
   auto down_tiles = [&](uint32_t m, float us) {
-    return (m <= 64 || hidden % 128 == 0) && (uint64_t)m * inter * 2 <= 0xffffffffull &&
-           tiles_faster(m, hidden, inter, false, us);
+    if (Bf16EstimateHolds(m, hidden, inter)) return tiles_faster(m, hidden, inter, false, us);
+    return m <= 64 && Bf16GemvUs(m, hidden, inter) < us;
   };
   p.up_tiles = up_tiles(rows, p.up.us);
   p.down_tiles = down_tiles(rows, p.down.us);

@@ -383,3 +383,20 @@ def test_infinity_in_the_last_row_of_the_weights_gradients(eng, rows, hidden, in
     for what, g, (w, _) in zip(("dx", "dw_gate", "dw_up", "dw_down"), got, want):
         _same_nonfinite(g, w, what)
     assert torch.isinf(want[3][0] if where == "dy" else want[1][0]).any()
+
+
+@pytest.mark.parametrize("rows,hidden,inter", [(1, 64, 16448), (8, 512, 2112), (24, 2048, 5696), (33, 1024, 4160), (64, 64, 16448),
+                                               (65, 256, 4160), (130, 1024, 4160), (320, 512, 2112)])
+def test_intermediate_sizes_off_128(eng, rows, hidden, inter):
+    """Half a step of 128 behind the last whole one, on the kernels that take it."""
+    import torch
+
+    from pih_amd.linear import gated_mlp
+
+    x, wg, wu, wd, _ = _case(rows + inter, rows, hidden, inter, "cuda")
+    _poison()
+    got = gated_mlp(x, wg, wu, wd, keep=True)
+    alone = gated_mlp(x, wg, wu, wd)
+    for what, g, w in zip(("y", "gate", "up"), got, _forward_ref(x, wg, wu, wd, 0.0)):
+        _within(g, w, what)
+    assert torch.equal(alone, got[0])
