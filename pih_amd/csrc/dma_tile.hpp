@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "dma_route.hpp"
 #include "glu.hpp"
 #include "kernels.hpp"
 
@@ -63,7 +64,6 @@ constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherG
 // (Eight waves, two to a SIMD, that take turns on 32-deep halves, so that one's
 // LDS reads run under the other's MFMAs: fewer cycles, but 5-10 % more time over
 // and over, with more LDS traffic: power sets the clock, 1.9 GHz of 2.4.)
-constexpr uint32_t TB = 256, KB = 64;
 
 // 16 bytes of a row that is not there
 __device__ const v4i kNoRow{0, 0, 0, 0};
@@ -730,14 +730,8 @@ void launch_rows(BigArgs p, hipStream_t s) {
   const uint32_t grid = std::min((p.m_tiles * p.n_tiles * p.splits + 7) / 8 * 8, kCus);
   hipLaunchKernelGGL((loss_big_kernel<ROWS, AT, BT, EPI>), dim3(grid), dim3(256), 0, s, p);
 }
-// Time (us) of m rows in tiles of `rows`: the rounds of tiles on the CUs, each a
-// step's time and a tile's own beginning and end
-//   256 rows 1.45 and 9,  128 rows 0.95 and 7,  64 rows 0.70 and 6.
 inline float rows_cost(const BigArgs& p, uint32_t m, uint32_t rows) {
-  const uint32_t splits = std::max(p.splits, 1u), steps = (p.k / KB + splits - 1) / splits;
-  const uint64_t tiles = (uint64_t)((m + rows - 1) / rows) * ((p.n + TB - 1) / TB) * splits;
-  const float tile = rows == 256 ? 9.0f + 1.45f * steps : rows == 128 ? 7.0f + 0.95f * steps : 6.0f + 0.70f * steps;
-  return (float)((tiles + kCus - 1) / kCus) * tile;
+  return DmaRowsUs(m, p.n, p.k, std::max(p.splits, 1u), rows);
 }
 inline uint32_t tile_rows(const BigArgs& p, uint32_t m) {
   const float c256 = rows_cost(p, m, 256), c128 = rows_cost(p, m, 128), c64 = rows_cost(p, m, 64);
@@ -787,59 +781,6 @@ void launch_big(BigArgs p, hipStream_t s) {
     }
     launch_any<AT, BT, EPI>(p, s);
   }
-}
-
-// ------------------------------------------- which tiles
-// How the rows of a product [m][n] over k run: tiles of `rows` rows, k in
-// `splits` parts.  Time (us): the rounds of tiles on the CUs, each its beginning
-// and end and a step's time (rows_cost), no less than B takes at
-// the CUs' share of 5.1 TB/s, and for splits the sums written and read at 4 TB/s and a launch.
-struct Tiling {
-  uint32_t rows, splits;
-  float us;
-};
-Tiling tiling_of(uint32_t m, uint32_t n, uint32_t k) {
-  BigArgs p{};
-  p.n = n;
-  p.k = k;
-  Tiling best{256, 1, INFINITY};
-  for (uint32_t rows : {64u, 128u, 256u}) {
-    if (m <= rows / 2 && rows > 64) break;  // (as many tiles as of half the rows, each slower)
-    for (uint32_t splits = 1; splits <= 64 && k / KB / splits >= 4; ++splits) {
-      // (no split is empty)
-      const uint32_t steps = k / KB, part = (steps + splits - 1) / splits;
-      if ((steps + part - 1) / part != splits) continue;
-      p.splits = splits;
-      const uint64_t tiles = (uint64_t)((m + rows - 1) / rows) * ((n + TB - 1) / TB) * splits;
-      const float busy = (float)std::min<uint64_t>(tiles, kCus) / kCus;
-      const float us = std::max(rows_cost(p, m, rows), (float)n * k * (2.0f / 5.1e6f) / busy) +
-                       (splits > 1 ? 7.0f + (float)splits * m * n * (8.0f / 4.0e6f) : 0.0f);
-      if (us < best.us) best = {rows, splits, us};
-    }
-  }
-  return best;
-}
-// All rows alike, or the whole 256 without splits and the rest by itself, where B
-// is read once more (at 5 TB/s) and the launch costs 3 us
-struct Route {
-  uint32_t whole;  // rows in tiles of 256, unsplit
-  Tiling rest;     // of those behind
-  uint64_t sums;   // fp32 elements
-  float us;
-};
-Route route_of(uint32_t m, uint32_t n, uint32_t k) {
-  const Tiling all = tiling_of(m, n, k);
-  const uint32_t whole = m / 256 * 256, rest = m - whole;
-  Route r{0, all, all.splits > 1 ? (uint64_t)all.splits * m * n : 0, all.us};
-  if (whole && rest) {
-    BigArgs p{};
-    p.n = n;
-    p.k = k;
-    const Tiling last = tiling_of(rest, n, k);
-    const float us = rows_cost(p, whole, 256) + last.us + 3.0f;
-    if (us < all.us) r = {whole, last, last.splits > 1 ? (uint64_t)last.splits * rest * n : 0, us};
-  }
-  return r;
 }
 
 }  // namespace
