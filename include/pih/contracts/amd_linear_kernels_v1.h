@@ -631,6 +631,8 @@ typedef struct pih_amd_gated_mlp_backward_launch_v1 {
  * An id of 0xFFFFFFFF is no entry, a teacher logit of -infinity one of
  * probability 0, which adds nothing; a row without any other has loss 0.  An
  * id twice in a row is two entries.  Logits, maxima and sums are fp32.
+ * The results lie outside every input and one another; loss or lse may stand
+ * in the place of teacher_lse.
  * input bf16 [rows][hidden], weight bf16 [vocab][hidden].  hidden a multiple of
  * 8, rows, vocab and hidden up to 2^20, top_k up to 256, temperature positive
  * and finite, addresses 16-byte aligned (the u32 and f32 arrays 4-byte).

@@ -618,6 +618,16 @@ bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p
 uint64_t padded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 
+// whether a result overlaps one of the logits' rows (what lies between them is the
+// caller's)
+bool overlaps_rows(Span result, const void* base, uint64_t rows, uint64_t bytes, uint64_t stride) {
+  if (!rows || !Overlap(result, {base, (rows - 1) * stride + bytes})) return false;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(result.p), first = reinterpret_cast<uintptr_t>(base);
+  if (from < first) return true;
+  const uint64_t row = (from - first) / stride, within = (from - first) % stride;
+  return within < bytes || (row + 1 < rows && within + result.bytes > stride);
+}
+
 struct VerifyPlan {
   uint64_t plans, rest, done, bytes;
 };
@@ -665,8 +675,16 @@ St LaunchDraftVerify(const DraftVerifyArgs& a) {
       !aligned(a.accept, 4) || !aligned(a.sample, 4) || !aligned(a.temperature, 4) || !aligned(a.out, 4) ||
       !aligned(a.accepted, 4) || !aligned(a.error_flag, 4))
     return Invalid("draft_verify_alignment_invalid");
-  // (the accepted tokens are written before the rejected one is read)
-  if (a.out == a.tokens || a.accepted == a.offsets || a.out == a.accepted) return Invalid("draft_verify_alias_invalid");
+  const uint64_t of_drafts = (uint64_t)a.drafts * 4, of_sequences = (uint64_t)a.sequences * 4;
+  const Span results[] = {{a.out, of_sequences * (a.max_drafts + 1)}, {a.accepted, of_sequences}};
+  const Span inputs[] = {{a.tokens, of_drafts},    {a.offsets, of_sequences + 4},   {a.accept, of_drafts},
+                         {a.sample, of_sequences}, {a.temperature, of_sequences}};
+  bool alias = ResultsOverlap(results, inputs);
+  for (const Span& r : results)
+    alias |= overlaps_rows(r, a.target, (uint64_t)a.drafts + a.sequences, (uint64_t)a.vocab * size,
+                           (uint64_t)a.target_stride * size) ||
+             overlaps_rows(r, a.draft, a.drafts, (uint64_t)a.vocab * size, (uint64_t)a.draft_stride * size);
+  if (alias) return Invalid("draft_verify_alias_invalid");
   const VerifyPlan plan = verify_plan(a.sequences, a.max_drafts, a.vocab);
   const uint32_t chunks = chunks_of(a.vocab), rows = a.max_drafts + 1 + (a.draft ? a.max_drafts : 0);
   if (a.workspace_bytes < plan.bytes || !aligned(a.workspace, 16)) return Invalid("draft_verify_workspace_invalid");

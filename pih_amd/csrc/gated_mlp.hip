@@ -312,8 +312,11 @@ St LaunchGatedMlp(const GatedMlpArgs& a) {
     return Invalid("gated_mlp_alignment_invalid");
   const ForwardPlan plan = forward_plan(a.rows, a.inter, a.hidden);
   if (a.workspace_bytes < plan.bytes || !aligned(a.workspace)) return Invalid("gated_mlp_workspace_invalid");
-  if (a.y == a.x || (a.gate && (a.gate == a.x || a.up == a.x || a.gate == a.up || a.gate == a.y || a.up == a.y)))
-    return Invalid("gated_mlp_alias_invalid");
+  const uint64_t of_rows = (uint64_t)a.rows * a.hidden * 2, of_inter = (uint64_t)a.rows * a.inter * 2,
+                 of_weight = (uint64_t)a.inter * a.hidden * 2;
+  const Span results[] = {{a.y, of_rows}, {a.gate, of_inter}, {a.up, of_inter}};
+  const Span inputs[] = {{a.x, of_rows}, {a.wg, of_weight}, {a.wu, of_weight}, {a.wd, of_weight}};
+  if (ResultsOverlap(results, inputs)) return Invalid("gated_mlp_alias_invalid");
   St clean = RequireCleanLastError();
   if (!clean.ok()) return clean;
   uint16_t* const h = static_cast<uint16_t*>(a.workspace);
@@ -436,17 +439,16 @@ St LaunchGatedMlpBackward(const GatedMlpArgs& a) {
     return Invalid("gated_mlp_backward_null_argument");
   if (!shape_ok(a.rows, a.inter, a.hidden)) return Invalid("gated_mlp_backward_shape_invalid");
   if (!__builtin_isfinite(a.limit)) return Invalid("gated_mlp_backward_limit_invalid");
-  const void* const inputs[] = {a.dy, a.x, a.wg, a.wu, a.wd, a.gate, a.up};
-  const void* const results[] = {a.dx, a.dwg, a.dwu, a.dwd};
-  for (const void* i : inputs)
-    if (!aligned(i)) return Invalid("gated_mlp_backward_alignment_invalid");
-  for (int r = 0; r < 4; ++r) {
-    if (!aligned(results[r])) return Invalid("gated_mlp_backward_alignment_invalid");
-    for (const void* i : inputs)
-      if (results[r] == i) return Invalid("gated_mlp_backward_alias_invalid");
-    for (int s = 0; s < r; ++s)
-      if (results[r] && results[r] == results[s]) return Invalid("gated_mlp_backward_alias_invalid");
-  }
+  const uint64_t of_rows = (uint64_t)a.rows * a.hidden * 2, of_inter = (uint64_t)a.rows * a.inter * 2,
+                 of_weight = (uint64_t)a.inter * a.hidden * 2;
+  const Span inputs[] = {{a.dy, of_rows},   {a.x, of_rows},     {a.wg, of_weight}, {a.wu, of_weight},
+                         {a.wd, of_weight}, {a.gate, of_inter}, {a.up, of_inter}};
+  const Span results[] = {{a.dx, of_rows}, {a.dwg, of_weight}, {a.dwu, of_weight}, {a.dwd, of_weight}};
+  for (const Span& i : inputs)
+    if (!aligned(i.p)) return Invalid("gated_mlp_backward_alignment_invalid");
+  for (const Span& r : results)
+    if (!aligned(r.p)) return Invalid("gated_mlp_backward_alignment_invalid");
+  if (ResultsOverlap(results, inputs)) return Invalid("gated_mlp_backward_alias_invalid");
   const BackwardPlan plan = backward_plan(a.rows, a.inter, a.hidden);
   if (a.workspace_bytes < plan.bytes || !aligned(a.workspace)) return Invalid("gated_mlp_backward_workspace_invalid");
   St clean = RequireCleanLastError();

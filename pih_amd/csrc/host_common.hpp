@@ -55,6 +55,29 @@ inline T* Ptr(uintptr_t p) {
   return reinterpret_cast<T*>(p);
 }
 
+// Memory of a call's argument, for the entries whose results may not overlap what
+// they read; empty where the argument is left out
+struct Span {
+  const void* p = nullptr;
+  uint64_t bytes = 0;
+};
+inline bool Overlap(Span a, Span b) {
+  if (!a.p || !b.p || !a.bytes || !b.bytes) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return x < y ? y - x < a.bytes : x - y < b.bytes;
+}
+// whether a result overlaps another one or an input
+template <size_t R, size_t I>
+inline bool ResultsOverlap(const Span (&results)[R], const Span (&inputs)[I]) {
+  for (size_t r = 0; r < R; ++r) {
+    for (const Span& i : inputs)
+      if (Overlap(results[r], i)) return true;
+    for (size_t s = 0; s < r; ++s)
+      if (Overlap(results[r], results[s])) return true;
+  }
+  return false;
+}
+
 // A one-time host step per device (raising a kernel's LDS limit): run()
 // performs the step on the current device until it has succeeded there
 // once.  Host threads that arrive together may both perform it (every such

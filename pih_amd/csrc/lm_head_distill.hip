@@ -351,9 +351,15 @@ St LaunchLmHeadDistill(const LmHeadDistillArgs& a) {
       !aligned(a.teacher_lse, 4) || !aligned(a.loss, 4) || !aligned(a.lse, 4) || !aligned(a.logits, 4) ||
       !aligned(a.error_flag, 4))
     return Invalid("lm_head_distill_alignment_invalid");
-  // (the logits are written before the teacher's are read)
-  if (a.logits == a.teacher || (const void*)a.logits == a.ids || a.logits == a.teacher_lse)
-    return Invalid("lm_head_distill_alias_invalid");
+  const uint64_t each = (uint64_t)a.rows * 4, entries = each * a.top_k;
+  const Span x{a.x, (uint64_t)a.rows * a.hidden * 2}, w{a.w, (uint64_t)a.vocab * a.hidden * 2};
+  const Span results[] = {{a.loss, each}, {a.lse, each}, {a.logits, entries}};
+  const Span inputs[] = {x, w, {a.ids, entries}, {a.teacher, entries}};
+  const Span teacher_lse{a.teacher_lse, each};
+  bool alias = ResultsOverlap(results, inputs) || Overlap(results[2], teacher_lse);
+  // (a row's own place in it is read before its loss and lse are written)
+  for (int r = 0; r < 2; ++r) alias |= results[r].p != teacher_lse.p && Overlap(results[r], teacher_lse);
+  if (alias) return Invalid("lm_head_distill_alias_invalid");
   if (a.workspace_bytes < LmHeadDistillWorkspaceBytes(a.rows, a.vocab, a.hidden) || !aligned(a.workspace, 16))
     return Invalid("lm_head_distill_workspace_invalid");
   St clean = RequireCleanLastError();
@@ -423,8 +429,14 @@ St LaunchLmHeadDistillBackward(const LmHeadDistillArgs& a) {
       !aligned(a.teacher, 4) || !aligned(a.teacher_lse, 4) || !aligned(a.lse, 4) || !aligned(a.logits, 4) ||
       !aligned(a.loss_grad, 4) || !aligned(a.error_flag, 4))
     return Invalid("lm_head_distill_backward_alignment_invalid");
-  // (the weights' gradient of a piece is written before dx reads its weights)
-  if (a.dw == a.w) return Invalid("lm_head_distill_backward_alias_invalid");
+  // (a piece's weights' gradient is written before dx reads its weights, and before
+  // the other pieces read the rest)
+  const uint64_t each = (uint64_t)a.rows * 4, entries = each * a.top_k;
+  const uint64_t of_rows = (uint64_t)a.rows * a.hidden * 2, of_weight = (uint64_t)a.vocab * a.hidden * 2;
+  const Span results[] = {{a.dx, of_rows}, {a.dw, of_weight}};
+  const Span inputs[] = {{a.x, of_rows},          {a.w, of_weight}, {a.ids, entries},    {a.teacher, entries},
+                         {a.teacher_lse, each}, {a.lse, each},    {a.logits, entries}, {a.loss_grad, each}};
+  if (ResultsOverlap(results, inputs)) return Invalid("lm_head_distill_backward_alias_invalid");
   const DistillPlan plan = distill_plan(a.rows, a.vocab, a.hidden);
   if (a.workspace_bytes < plan.bytes || !aligned(a.workspace, 16))
     return Invalid("lm_head_distill_backward_workspace_invalid");

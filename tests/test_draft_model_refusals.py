@@ -242,3 +242,56 @@ def test_table_entries_follow_the_earlier_ones():
     assert last == ["launch_gated_mlp", "launch_gated_mlp_backward", "launch_lm_head_distill",
                     "launch_lm_head_distill_backward", "launch_draft_verify"]
     assert table.launch_gated_mlp.offset == table.launch_router_backward.offset + C.sizeof(C.c_void_p)
+
+
+def _overlaps():
+    """A result that begins inside an input or another result, or ends there."""
+    # (rows 5, hidden 64, intermediate 128: 640 bytes of rows, 1280 of gate and up, 16384 of a weight)
+    x, inter, weight = 640, 1280, 16384
+    out = []
+
+    def pairs(make, results, inputs):
+        for i, (r, size) in enumerate(results):
+            for other, length in inputs + results[:i]:
+                # (multiples of 16 for the rows, of 4 for the u32 and f32 arrays)
+                step = 16 if "bf16" in r else 4
+                out.extend((make, r, other, d) for d in (0, (length - 1) // step * step, -((size - 1) // step * step)))
+
+    weights = [("gate_weight_bf16", weight), ("up_weight_bf16", weight), ("down_weight_bf16", weight)]
+    kept = [("gate_bf16", inter), ("up_bf16", inter)]
+    pairs(_mlp, [("output_bf16", x)] + kept, [("input_bf16", x)] + weights)
+    pairs(_mlp_backward, [("input_grad_bf16", x)] + [(w.replace("_bf16", "_grad_bf16"), n) for w, n in weights],
+          [("output_grad_bf16", x), ("input_bf16", x)] + weights + kept)
+    # (5 rows of 4 entries, 100 x 64 weights)
+    rows, entries, head = 20, 80, 12800
+    teacher = [("teacher_ids_u32", entries), ("teacher_logits_f32", entries)]
+    shared = [("input_bf16", x), ("weight_bf16", head)] + teacher
+    pairs(_distill, [("loss_f32", rows), ("lse_f32", rows), ("logits_f32", entries)], shared)
+    out.extend((_distill, r, "teacher_lse_f32", d) for r, d in
+               (("loss_f32", 16), ("loss_f32", -16), ("lse_f32", 4), ("logits_f32", 0), ("logits_f32", -64)))
+    pairs(_distill_backward, [("input_grad_bf16", x), ("weight_grad_bf16", head)],
+          shared + [("teacher_lse_f32", rows), ("lse_f32", rows), ("logits_f32", entries), ("loss_grad_f32", rows)])
+    # (3 sequences, 7 drafts, at most 4 a sequence, 100 columns of fp32)
+    pairs(_verify, [("tokens_u32", 60), ("accepted_u32", 12)],
+          [("target_logits", 4000), ("draft_logits", 2800), ("draft_tokens_u32", 28), ("draft_offsets_u32", 16),
+           ("accept_random_f32", 28), ("sample_random_f32", 12), ("temperature_f32", 12)])
+    return out
+
+
+@pytest.mark.parametrize("make,result,other,offset", _overlaps(), ids=lambda v: v.__name__ if callable(v) else str(v))
+def test_overlapping_results_are_refused(make, result, other, offset):
+    entry, r = make()
+    setattr(r, result, getattr(r, other) + offset)
+    st = abi.linear_pack().call(entry, r)
+    assert st.code == abi.INVALID_ARGUMENT and b"alias" in st.message, st.message
+
+
+@pytest.mark.parametrize("offset", [396, 744])
+def test_results_that_reach_into_strided_logits_are_refused(offset):
+    """Rows 800 bytes apart, of which 400 are logits: 60 bytes of tokens from the
+    last logit of a row on, or up to the first of the next (between them:
+    test_gpu_draft_verify.py)."""
+    entry, r = _verify(target_stride=200)
+    r.tokens_u32 = r.target_logits + offset
+    st = abi.linear_pack().call(entry, r)
+    assert st.code == abi.INVALID_ARGUMENT and b"alias" in st.message, st.message

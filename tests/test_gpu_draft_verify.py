@@ -461,3 +461,31 @@ def test_rows_past_4_gib(eng):
     tokens, accepted, flag = draft_verify(target, empty, torch.zeros(sequences + 1, dtype=torch.int32, device="cuda"),
                                           empty.float(), torch.full((sequences,), 0.5, device="cuda"), most)
     assert int(flag.item()) == 0 and torch.equal(tokens[:, 0].long(), best) and torch.all(accepted == 0)
+
+
+def test_results_between_strided_rows(eng):
+    """The tokens and counts in the columns behind the logits of a wider tensor."""
+    import torch
+
+    from pih_amd import abi, linear
+    from pih_amd.device import error_flag, stream_handle
+
+    most, vocab = 4, 100
+    case = _case(31, [3, 0, 4], vocab, soft=False)
+    target = case["target"].cuda()
+    tokens, offsets, accept, sample = (torch.from_numpy(case[n]).cuda() for n in ("tokens", "offsets", "accept", "sample"))
+    drafts, sequences = tokens.shape[0], sample.shape[0]
+    want = linear.draft_verify(target, tokens, offsets, accept, sample, most)
+    wide = torch.zeros(drafts + sequences, 200, device="cuda")
+    wide[:, :vocab] = target
+    out, count = wide[0, vocab:].view(torch.int32), wide[1, vocab:].view(torch.int32)
+    flag = error_flag()
+    ws = linear._workspace(abi.WORKSPACE_DRAFT_VERIFY, sequences, most, vocab, target.device)
+    linear._launch("launch_draft_verify", "draft_verify", wide.data_ptr(), 0,
+                   *(t.data_ptr() for t in (tokens, offsets, accept, sample)), 0, out.data_ptr(), count.data_ptr(),
+                   ws.data_ptr(), ws.numel(), flag.data_ptr(), stream_handle(), sequences, drafts, most, vocab, 200, 0,
+                   abi.OUTPUT_F32)
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0 and torch.equal(wide[:, :vocab], target)
+    assert torch.equal(out[:sequences * (most + 1)].view(sequences, most + 1), want[0])
+    assert torch.equal(count[:sequences], want[1])

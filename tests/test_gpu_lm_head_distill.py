@@ -439,3 +439,26 @@ def test_infinite_last_weight(eng, rows, vocab, hidden, loss):
     assert torch.isneginf(dx[row, column])
     others = torch.arange(rows, device="cuda") != row
     assert torch.isnan(dx[others, column]).all()
+
+
+def test_lse_in_the_place_of_the_teachers(eng):
+    """A row's place in teacher_lse is read before its lse (or loss) is written there."""
+    import torch
+
+    from pih_amd import abi, linear
+    from pih_amd.device import error_flag, stream_handle
+
+    rows, vocab, hidden, top_k = 70, 1000, 128, 5
+    x, w, ids, teacher, _, _ = (t.cuda() for t in _case(8, rows, vocab, hidden, top_k))
+    tail = torch.full((rows,), 4.0, device="cuda")
+    want = linear.lm_head_distill(x, w, ids, teacher, 1.5, teacher_lse=tail)
+    ws = linear._workspace(abi.WORKSPACE_LM_HEAD_DISTILL, rows, vocab, hidden, x.device)
+    for place in (0, 1):
+        out, flag = [torch.empty(rows, device="cuda") for _ in range(2)], error_flag()
+        out[place] = tail.clone()
+        z = torch.empty(rows, top_k, device="cuda")
+        linear._launch("launch_lm_head_distill", "lm_head_distill",
+                       *(t.data_ptr() for t in (x, w, ids, teacher, out[place], out[0], out[1], z, ws)), ws.numel(),
+                       flag.data_ptr(), stream_handle(), rows, vocab, hidden, top_k, 1.5)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out + [z], want))
