@@ -400,3 +400,54 @@ def test_intermediate_sizes_off_128(eng, rows, hidden, inter):
     for what, g, w in zip(("y", "gate", "up"), got, _forward_ref(x, wg, wu, wd, 0.0)):
         _within(g, w, what)
     assert torch.equal(alone, got[0])
+
+
+def test_gradient_against_differences_along_the_formulas(eng):
+    """The backward pass against the forward one's own change along directions
+    that do not come from it: the 64-bit gradient on a quarter of the tensor, for
+    x also each of its two terms.  A value v = sum of y dy is off by y's and h's
+    roundings, independent and at most 2^-8 of each element: six standard
+    deviations of the two values' difference are 6 sqrt(2 / 3) 2^-8 sqrt(|y dy|^2 +
+    |h dh|^2).  What the change has beyond the first order is taken from the 64-bit
+    form, and the gradient's own error from its bound."""
+    import torch
+
+    from pih_amd.linear import gated_mlp, gated_mlp_backward
+
+    x, wg, wu, wd, dy = (t.cuda() for t in _case(5, 64, 256, 512, spread=1.0))
+    y, gate, up = gated_mlp(x, wg, wu, wd, keep=True)
+    grads = gated_mlp_backward(dy, x, wg, wu, wd, gate, up)
+    refs = _backward_ref(dy, x, wg, wu, wd, gate, up, 0.0)
+
+    def value64(args):
+        return (_forward_ref(*args, 0.0)[0][0] * dy.double()).sum()
+
+    g, u, dh = gate.double(), up.double(), dy.double() @ wd.double()
+    s = torch.sigmoid(g)
+    h = g * s * u
+    noise = 6 * (2 / 3) ** 0.5 * HALF_BF16 * ((y.double() * dy.double()).norm() ** 2 + (h * dh).norm() ** 2).sqrt()
+    terms = ((dh * u * (s + g * s * (1 - s))) @ wg.double(), (dh * g * s) @ wu.double())
+    for i, (t, d) in enumerate(zip((x, wg, wu, wd), grads)):
+        ref, bound = refs[i]
+        quarters = []
+        for rows in (0, 1):
+            for columns in (0, 1):
+                part = torch.zeros_like(ref)
+                part[rows::2, columns::2] = ref[rows::2, columns::2]
+                quarters.append(part)
+        for j, direction in enumerate(quarters + (list(terms) if i == 0 else [])):
+            step = direction / direction.norm() * t.double().norm() * 0.05
+            values, exact = [], []
+            low, high = (t.double() - step).to(torch.bfloat16), (t.double() + step).to(torch.bfloat16)
+            for v in (low, high):
+                args = [x, wg, wu, wd]
+                args[i] = v
+                values.append((gated_mlp(*args).double() * dy.double()).sum())
+                exact.append(value64(args))
+            moved = high.double() - low.double()
+            first, change = (moved * d.double()).sum(), values[1] - values[0]
+            beyond = (exact[1] - exact[0] - (moved * ref).sum()).abs()
+            tolerance = noise + beyond + (moved.abs() * bound).sum()
+            print(f"{i}.{j}: {change.item():.6f} against {first.item():.6f}, tolerance {tolerance.item():.6f}", flush=True)
+            assert tolerance < 0.2 * first.abs()
+            assert (change - first).abs() <= tolerance

@@ -462,3 +462,69 @@ def test_lse_in_the_place_of_the_teachers(eng):
                        flag.data_ptr(), stream_handle(), rows, vocab, hidden, top_k, 1.5)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out + [z], want))
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,top_k", [(1100, 122859, 64, 128), (1021, 151936, 256, 8), (2053, 70001, 320, 3)])
+def test_entries_at_every_tiles_border(eng, rows, vocab, hidden, top_k):
+    """Ids on either side of every border of the tiles of 256 columns, those of the
+    backward pass's pieces among them (2^26 elements of g or so in each, of the rows'
+    135, 155 and 144 million), each in several rows."""
+    import torch
+
+    from pih_amd.linear import lm_head_distill, lm_head_distill_backward
+
+    assert rows * vocab > (1 << 26) * 4 // 3  # more than a piece
+    x, w, ids, teacher, more, up = _case(rows + 1, rows, vocab, hidden, top_k, "cuda", empty=0.0)
+    edges = torch.arange(256, vocab, 256, device="cuda", dtype=torch.int32)
+    edges = torch.cat((edges - 1, edges, torch.tensor([0, vocab - 1], device="cuda", dtype=torch.int32)))
+    times = rows * top_k // edges.numel()
+    assert times >= 2
+    ids.view(-1)[:times * edges.numel()] = edges.repeat(times)
+    teacher_lse, loss, lse, z = _forward_ref(x, w, ids, teacher, more, 1.5, True)
+    got = lm_head_distill(x, w, ids, teacher, 1.5, teacher_lse=teacher_lse)
+    for what, a, b in (("loss", got[0], loss), ("lse", got[1], lse), ("logits", got[2], z)):
+        _within(a, b, what)
+    assert int(got[3].item()) == 0
+    want = _grads_ref(x, w, ids, teacher, more, up, got[1], 1.5, True)
+    grads = lm_head_distill_backward(x, w, ids, teacher, got[1], got[2], up, 1.5, teacher_lse=teacher_lse)
+    _within(grads[0], want[0], "dx")
+    _within(grads[1], want[1], "dw")
+
+
+def test_gradient_against_differences_along_the_formulas(eng):
+    """The backward pass against the loss's own change along directions that do not
+    come from it: the 64-bit gradient on a quarter of the tensor.  The losses are off
+    by their bounds; what the change has beyond the first order is taken from the
+    64-bit form, and the gradient's own error from its bound."""
+    import torch
+
+    from pih_amd.linear import lm_head_distill, lm_head_distill_backward
+
+    case = [t.cuda() for t in _case(21, 40, 2000, 256, 16)]
+    x, w, ids, teacher, more, up = case
+    _, lse, z, _ = lm_head_distill(x, w, ids, teacher, 2.0)
+    grads = lm_head_distill_backward(x, w, ids, teacher, lse, z, up, 2.0)
+    refs = _grads_ref(x, w, ids, teacher, more, up, lse, 2.0, False)
+    for i, (t, d) in enumerate(((x, grads[0]), (w, grads[1]))):
+        ref, bound = refs[i]
+        for rows in (0, 1):
+            for columns in (0, 1):
+                step = torch.zeros_like(ref)
+                step[rows::2, columns::2] = ref[rows::2, columns::2]
+                step *= t.double().norm() * 0.02 / step.norm()
+                low, high = (t.double() - step).to(torch.bfloat16), (t.double() + step).to(torch.bfloat16)
+                values, exact, noise = [], [], 0.0
+                for v in (low, high):
+                    xv, wv = (v, w) if i == 0 else (x, v)
+                    values.append((lm_head_distill(xv, wv, ids, teacher, 2.0)[0].double() * up.double()).sum())
+                    loss, eloss = _forward_ref(xv, wv, ids, teacher, more, 2.0, False)[1]
+                    exact.append((loss * up.double()).sum())
+                    noise = noise + (eloss * up.double().abs()).sum()
+                moved = high.double() - low.double()
+                first, change = (moved * d.double()).sum(), values[1] - values[0]
+                beyond = (exact[1] - exact[0] - (moved * ref).sum()).abs()
+                tolerance = noise + beyond + (moved.abs() * bound).sum()
+                print(f"{i}.{rows}{columns}: {change.item():.6f} against {first.item():.6f}, tolerance "
+                      f"{tolerance.item():.6f}", flush=True)
+                assert tolerance < 0.2 * first.abs()
+                assert (change - first).abs() <= tolerance
