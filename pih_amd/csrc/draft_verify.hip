@@ -30,7 +30,7 @@
 namespace pih_amd {
 namespace {
 
-constexpr uint32_t kChunk = 4096, kPer = kChunk / 256;
+constexpr uint32_t kChunk = 4096, kPer = kChunk / 256;  // a block's columns, a thread's
 constexpr uint32_t kMaxVocab = 1u << 20, kMaxSequences = 1u << 14, kMostDrafts = 255;
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr uint32_t kErrToken = 1u, kErrOffsets = 2u, kErrRow = 4u;
@@ -104,38 +104,28 @@ __device__ __forceinline__ double exp2_64(double y, double lead) {
 __device__ __forceinline__ double exp2_or_0(double y, double lead) { return y < -1021.0 ? 0.0 : exp2_64(y, lead); }
 __device__ __forceinline__ double exp2_or_0(double y) { return exp2_or_0(y, lead_coefficient()); }
 
-// N logits from column c on, -inf past the vocabulary
-template <bool BF16, bool WIDE, int N>
-__device__ __forceinline__ void load_logits(float (&v)[N], const void* row, uint32_t c, uint32_t vocab) {
-  static_assert(N == 4 || N == 16, "a thread's logits");
-  if (WIDE && c + N <= vocab) {
+// A thread's logits from column c on, -inf past the vocabulary
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void load_logits(float (&v)[kPer], const void* row, uint32_t c, uint32_t vocab) {
+  if (WIDE && c + kPer <= vocab) {
     if constexpr (BF16) {
-      uint32_t w[N / 2];
-      if constexpr (N == 16) {
-        const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
-        const uint4 x = p[0], y = p[1];
-        const uint32_t all[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+      const uint4 x = p[0], y = p[1];
+      const uint32_t w[kPer / 2] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) w[i] = all[i];
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + c);
-        w[0] = x.x;
-        w[1] = x.y;
-      }
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = bf16_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+      for (uint32_t e = 0; e < kPer; ++e) v[e] = bf16_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
     } else {
       const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(row) + c);
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
+      for (uint32_t i = 0; i < kPer / 4; ++i) {
         const v4f x = p[i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * i + e] = x[e];
+        for (uint32_t e = 0; e < 4; ++e) v[4 * i + e] = x[e];
       }
     }
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
+    for (uint32_t i = 0; i < kPer; ++i) {
       v[i] = -INFINITY;
       if (c + i < vocab)
         v[i] = BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[c + i]) : static_cast<const float*>(row)[c + i];
@@ -436,22 +426,22 @@ __global__ __launch_bounds__(256) void verify_walk_kernel(VerifyArgs p) {
   if (threadIdx.x == 0) p.plans[blockIdx.x] = plan;
 }
 
-// w of a thread's N columns of a chunk; `whole`: p alone
-template <bool BF16, bool WIDE, int N>
-__device__ __forceinline__ void weights(double (&w)[N], const VerifyArgs& p, const Plan& plan, uint32_t c, bool whole) {
-  float v[N], d[N];
+// w of a thread's columns of a chunk; `whole`: p alone
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void weights(double (&w)[kPer], const VerifyArgs& p, const Plan& plan, uint32_t c, bool whole) {
+  float v[kPer], d[kPer];
   const double lead = lead_coefficient();
   load_logits<BF16, WIDE>(v, row_of<BF16>(p.target, p.target_stride, plan.target_row), c, p.vocab);
   const bool soft = p.draft && !whole;
   if (soft) load_logits<BF16, WIDE>(d, row_of<BF16>(p.draft, p.draft_stride, plan.draft_row), c, p.vocab);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < (int)kPer; ++i) {
     w[i] = exp2_or_0(((double)v[i] - (double)plan.p_top) * plan.k, lead) * plan.p_inverse;
     if (!whole && !p.draft && c + i == plan.without) w[i] = 0.0;
   }
   if (!soft) return;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < (int)kPer; ++i) {
     const double e = w[i] - exp2_or_0(((double)d[i] - (double)plan.q_top) * plan.k, lead) * plan.q_inverse;
     w[i] = e > 0.0 ? e : 0.0;
   }
@@ -493,7 +483,6 @@ __device__ __forceinline__ double running_sum(double v, double (&parts)[4]) {
 }
 
 // The token behind the accepted ones, by a block
-constexpr uint32_t kPickPer = kChunk / 256;
 struct PickRows {
   double parts[3][4];
   double all, before;
@@ -542,12 +531,12 @@ __device__ __forceinline__ void pick(const VerifyArgs& p, uint32_t s, const Plan
     lds.last = 0;
   }
   const double left = threshold - lds.before;
-  const uint32_t first = chunk * kChunk + tid * kPickPer;
-  double w[kPickPer];
+  const uint32_t first = chunk * kChunk + tid * kPer;
+  double w[kPer];
   weights<BF16, WIDE>(w, p, plan, first, whole);
   own = 0.0;
 #pragma unroll
-  for (int i = 0; i < (int)kPickPer; ++i) own += w[i];
+  for (int i = 0; i < (int)kPer; ++i) own += w[i];
   run = running_sum(own, lds.parts[2]);
   if (own > 0.0) {
     if (run > left) atomicMin(&lds.found, tid);
@@ -559,7 +548,7 @@ __device__ __forceinline__ void pick(const VerifyArgs& p, uint32_t s, const Plan
   uint32_t token = 0;
   bool done = false;
 #pragma unroll
-  for (int i = 0; i < (int)kPickPer; ++i) {
+  for (int i = 0; i < (int)kPer; ++i) {
     if (done || !(w[i] > 0.0)) continue;
     sum += w[i];
     token = first + i;
