@@ -21,8 +21,9 @@
 //
 // Measured: 1 sequence of 5 drafts over 151936 columns of fp32 23 us (two launches of
 // 5 and 18, dependent loads), 57 of up to 7 over 129280 of bf16, looked up, 52-54, 256
-// of up to 4 over 151936 of fp32 200-215 (the statistics 778 MB at 4.4 TB/s with the
-// vector units busy in 85 % of the cycles).
+// of up to 4 over 151936 of fp32 205-220.  The statistics are bound by the 64-bit
+// arithmetic of their exponentials: 1.0 G logits a ms in bf16 (33 M in 34 us, 2.0 TB/s)
+// as in fp32 (194 M in 185-202, 3.9-4.2 TB/s, the vector units busy in 85 % of the cycles).
 #include "dense_route.hpp"
 #include "device_common.hpp"
 #include "kernels.hpp"

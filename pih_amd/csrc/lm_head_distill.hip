@@ -7,10 +7,10 @@
 //   dx = g W,  dw = g^T x,  Q_t = sum_k q_k.
 //
 // Measured: 33 rows over 151936 x 1024, 20 entries, 65 us (the weights' 311 MB in 59,
-// 5.3 TB/s), 4096 rows over 129280 x 4096, 64 entries, 3.09 ms (1.40 PFLOP/s: the matrix
-// pipe at the clock that power leaves); gradients of 1021 rows over 151936 x 1024
-// 0.95 ms (1.00 PFLOP/s: of a tile's 31 us 9 are exponentials and stores), of 2053 over
-// 129280 x 4096 5.26 ms (1.24 PFLOP/s), of 33 over 151936 x 1024 228 us.
+// 5.3 TB/s), 4096 rows over 129280 x 4096, 64 entries, 3.09-3.16 ms (1.38 PFLOP/s: the
+// matrix pipe at the clock that power leaves); gradients of 1021 rows over 151936 x 1024
+// 0.95-0.97 ms (0.99 PFLOP/s: of a tile's 31 us 9 are exponentials and stores), of 2053
+// over 129280 x 4096 5.26-5.40 ms (1.22 PFLOP/s), of 33 over 151936 x 1024 228 us.
 //
 // The products are those of the cross entropy (lm_head_loss.hip) without a
 // target.  The teacher's entries are few against the vocabulary: forward their

@@ -23,14 +23,14 @@
 // (1 / rows, whose rounding would be the same error in every element) are
 // exact (all of up_t rounded inside g: 0.34 %).
 //
-// Measured: 4096 rows, 129280 x 4096 2.95-2.97 ms (1.46 PFLOP/s; a library
-// product of that shape alone 3.25 ms) and 9.34 ms for the gradients, bound
+// Measured: 4096 rows, 129280 x 4096 2.95-3.04 ms (1.45 PFLOP/s; a library
+// product of that shape alone 3.25 ms) and 9.3-9.5 ms for the gradients, bound
 // by the matrix pipe, 70 % busy, and the power it takes (1.9 GHz); 33 rows, 151936
 // x 1024 64.4 us, of which the weights' 311 MB take 61 at 5.1 TB/s; the gradients
 // of 1021 rows there 0.93 ms (1.02 PFLOP/s: of a 256 x 256 tile's 31 us 9 are the
-// exponentials and the stores).  dx alone, for a frozen head: 33 rows 148 us over
-// 151936 x 1024 and 375 over 129280 x 4096 (the weights twice from HBM), 4096 rows
-// 6.17 ms over 129280 x 4096 (1.41 PFLOP/s).
+// exponentials and the stores).  dx alone, for a frozen head: 33 rows 136 us over
+// 151936 x 1024 and 374 over 129280 x 4096 (the weights twice from HBM), 4096 rows
+// 6.2 ms over 129280 x 4096 (1.41 PFLOP/s).
 //
 // Rows without a target take no part in the gradients: their g is 0, and the
 // x of dw's product is a copy with those rows as zeros, so that nothing an
