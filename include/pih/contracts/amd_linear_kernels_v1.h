@@ -634,8 +634,8 @@ typedef struct pih_amd_gated_mlp_backward_launch_v1 {
  * The results lie outside every input and one another; loss or lse may stand
  * in the place of teacher_lse.
  * input bf16 [rows][hidden], weight bf16 [vocab][hidden].  hidden a multiple of
- * 8, rows, vocab and hidden up to 2^20, top_k up to 256, temperature positive
- * and finite, addresses 16-byte aligned (the u32 and f32 arrays 4-byte).
+ * 8, rows, vocab and hidden up to 2^20, top_k up to 256, temperature finite
+ * and above 4.24e-39 (log2(e) over it is finite), addresses 16-byte aligned (the u32 and f32 arrays 4-byte).
  * workspace: query_workspace(LM_HEAD_DISTILL, rows, vocab, hidden).
  * Error bits: 1 an id that is neither 0xFFFFFFFF nor below vocab (no entry),
  * 4 a non-finite loss (stored). */

@@ -280,7 +280,8 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(const uint32_t* id
 bool distill_ok(const LmHeadDistillArgs& a) {
   return shape_ok(a.rows, a.vocab, a.hidden) && a.top_k && a.top_k <= kTopMax;
 }
-bool temperature_ok(float t) { return t > 0.0f && __builtin_isfinite(t) && __builtin_isfinite(1.0f / t); }
+// (log2(e) / t multiplies the logits' differences, 0 among them)
+bool temperature_ok(float t) { return t > 0.0f && __builtin_isfinite(t) && __builtin_isfinite(kLog2e / t); }
 
 // Whether the tiles write the entries' logits: 4 us a round of tiles and 6 for the
 // sort, against the dot products' bytes at 8 TB/s.  64 entries, 4096 rows over

@@ -295,3 +295,13 @@ def test_results_that_reach_into_strided_logits_are_refused(offset):
     r.tokens_u32 = r.target_logits + offset
     st = abi.linear_pack().call(entry, r)
     assert st.code == abi.INVALID_ARGUMENT and b"alias" in st.message, st.message
+
+
+@pytest.mark.parametrize("make", [_distill, _distill_backward])
+@pytest.mark.parametrize("temperature", [2.9e-39, 3.5e-39, 4.2e-39])
+def test_temperatures_whose_exponents_have_no_scale_are_refused(make, temperature):
+    """1 / T is finite from 2.94e-39 on, log2(e) / T, which the logits' differences
+    are multiplied with, from 4.24e-39 on: below, 0 times it would be NaN."""
+    entry, r = make(temperature=temperature)
+    st = abi.linear_pack().call(entry, r)
+    assert st.code == abi.INVALID_ARGUMENT and b"temperature" in st.message, st.message
