@@ -659,7 +659,10 @@ typedef struct pih_amd_lm_head_distill_launch_v1 {
  *   weight_grad bf16 [vocab][hidden] = g^T . input   (address 0: left out)
  * summed in fp32, g as pih_amd_lm_head_loss_backward_launch_v1 takes it: its
  * upstream factor's powers of two and the rows' largest one enter in fp32 or
- * exactly.  A row without entries of a probability above 0 gives zeros,
+ * exactly.  exp(z / T - lse) is taken from the fp32 lse: at low temperatures,
+ * |lse| above 1e5 or so, off by a factor of exp(|lse| 2^-22) (below T = 2^-10 1 at
+ * most).
+ * A row without entries of a probability above 0 gives zeros,
  * whatever its input, lse and loss_grad hold.  The results lie outside every
  * input.  workspace: query_workspace(LM_HEAD_DISTILL_BACKWARD, rows, vocab,
  * hidden).  Conditions and error bit 1 are those of

@@ -20,16 +20,18 @@ constexpr uint32_t kNoTarget = 0xffffffffu;
 // target's logit; kEpiGrad: the logits' gradient in bf16; kEpiBf16: a scaled
 // result in bf16; kEpiAdd: added to fp32 sums; kEpiTeacherStats, kEpiTeacherGrad: the
 // first two of logits over a temperature, without a target, the first with the
-// logits at a list of columns that every row has.  The feed-forward block's: kEpiStore: bf16; kEpiSum: fp32, a plane
+// logits at a list of columns that every row has; kEpiTeacherGradLow: the second at
+// low temperatures.  The feed-forward block's: kEpiStore: bf16; kEpiSum: fp32, a plane
 // per split; kEpiGlu: two products side by side, gate and up, joined to h;
 // kEpiGluSum: the same two as kEpiSum; kEpiGluGrad: dh, joined with gate and up
 enum : int {
   kEpiStats = 0, kEpiGrad = 1, kEpiBf16 = 2, kEpiAdd = 3, kEpiTeacherStats = 4, kEpiTeacherGrad = 5,
-  kEpiStore = 6, kEpiSum = 7, kEpiGlu = 8, kEpiGluSum = 9, kEpiGluGrad = 10
+  kEpiStore = 6, kEpiSum = 7, kEpiGlu = 8, kEpiGluSum = 9, kEpiGluGrad = 10, kEpiTeacherGradLow = 11
 };
 constexpr bool has_pair(int epi) { return epi == kEpiGlu || epi == kEpiGluSum; }
 constexpr bool has_stats(int epi) { return epi == kEpiStats || epi == kEpiTeacherStats; }
-constexpr bool has_grad(int epi) { return epi == kEpiGrad || epi == kEpiTeacherGrad; }
+constexpr bool has_teacher_grad(int epi) { return epi == kEpiTeacherGrad || epi == kEpiTeacherGradLow; }
+constexpr bool has_grad(int epi) { return epi == kEpiGrad || has_teacher_grad(epi); }
 
 // ------------------------------------------------ tiles fed by DMA
 // C [m][n] = A . B^T in tiles of 256 columns and 256, 128 or 64 rows.  Four
@@ -86,6 +88,7 @@ struct BigArgs {
   float* target_logit;
   uint32_t v0, vocab, first;
   float exponent;          // kEpiTeacher*: log2(e) / temperature
+  const float* most;       // kEpiTeacherGradLow: what a row's exponentials sum to
   // kEpiTeacherStats: a row's columns in order, id << 8 | place in its list
   // ([m][top_k]), how many of them lie before each tile ([m][n_tiles + 1]; null: no
   // lists), and where their logits go ([m][top_k])
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
     // the wave's part
     if constexpr (!has_grad(EPI) && !has_stats(EPI)) arrived();
     const uint32_t lrow = wm * MB * 16, wrow = cm + lrow, wcol = cn + wn * NB * 16;
-    const float exponent = EPI == kEpiTeacherStats || EPI == kEpiTeacherGrad ? p.exponent : kLog2e;
+    const float exponent = EPI == kEpiTeacherStats || has_teacher_grad(EPI) ? p.exponent : kLog2e;
     if constexpr (has_stats(EPI)) {
       // [column part][row]: maximum and sum
       float2* const parts = reinterpret_cast<float2*>(smem + kParts);
@@ -659,6 +662,14 @@ __global__ __launch_bounds__(256, 1) void loss_big_kernel(BigArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], exponent, shift));
+          if constexpr (EPI == kEpiTeacherGradLow) {
+            // none exceeds their sum (but for the rounding of a large log-sum-exp)
+            const float most = p.most[min(cm + at_row, p.m - 1)];
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][e] = at_most(acc[i][j][e], most);
+          }
           if (EPI == kEpiGrad && __builtin_amdgcn_ballot_w64(place < 16u * NB)) {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
@@ -778,6 +789,7 @@ void launch_big(BigArgs p, hipStream_t s) {
         p.lse += whole;
         p.mantissa += whole;
       }
+      if constexpr (EPI == kEpiTeacherGradLow) p.most += whole;
     }
     launch_any<AT, BT, EPI>(p, s);
   }

@@ -29,6 +29,7 @@ struct GemmArgs {
   float* target_logit;  // [m]
   uint32_t v0, vocab, stat_tiles;
   float inverse;        // kEpiTeacher*: 1 / temperature
+  const float* most;    // kEpiTeacherGrad: what a row's exponentials sum to
 };
 
 // 64 x 64 elements of an operand into LDS, zeros outside
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(256) void loss_gemm_kernel(GemmArgs p) {
         const uint32_t target = p.target[row], at = p.v0 + col;
         if (target < p.vocab) {
           if constexpr (EPI == kEpiGrad) g = p.mantissa[row] * (expf(v - p.lse[row]) - (target == at ? 1.0f : 0.0f));
-          else g = p.mantissa[row] * expf(v * p.inverse - p.lse[row]);
+          else g = p.mantissa[row] * at_most(expf(v * p.inverse - p.lse[row]), p.most[row]);
         }
       }
       static_cast<uint16_t*>(p.out)[(uint64_t)row * p.ldo + col] = (uint16_t)f32_to_bf16_bits(g);
@@ -286,6 +287,7 @@ struct BackwardCall {
   hipStream_t stream;
   uint32_t rows, vocab, hidden;
   float temperature = 1.0f;  // kEpiTeacherGrad
+  const float* most = nullptr;  // the same: what a row's exponentials sum to
 };
 
 // dx of a piece on a route of its own: the rows in whole tiles of 256 and the
@@ -351,6 +353,7 @@ void launch_backward(const BackwardCall& a, const BackwardPlan& plan, const DxRo
       b.v0 = v0;
       b.vocab = a.vocab;
       b.exponent = kLog2e / a.temperature;
+      b.most = a.most;
       launch_big<false, false, EPI>(b, a.stream);
     } else {
       GemmArgs g{};
@@ -368,7 +371,8 @@ void launch_backward(const BackwardCall& a, const BackwardPlan& plan, const DxRo
       g.v0 = v0;
       g.vocab = a.vocab;
       g.inverse = 1.0f / a.temperature;
-      launch_gemm<EPI>(g, a.stream);
+      g.most = a.most;
+      launch_gemm<has_teacher_grad(EPI) ? kEpiTeacherGrad : EPI>(g, a.stream);
     }
     after_logits(v0, cols);
     if (a.dw) {

@@ -528,3 +528,55 @@ def test_gradient_against_differences_along_the_formulas(eng):
                       f"{tolerance.item():.6f}", flush=True)
                 assert tolerance < 0.2 * first.abs()
                 assert (change - first).abs() <= tolerance
+
+
+@pytest.mark.parametrize("rows,hidden", [(40, 64), (40, 72), (300, 128)])
+@pytest.mark.parametrize("temperature", [4.25e-39, 1e-30, 1e-9])
+def test_low_temperatures(eng, rows, hidden, temperature):
+    """The head's and the teacher's softmax are their largest logits alone, which
+    agree: no loss.  Of the gradients' two sides, each at most the temperature, the
+    head's is as far off as its fp32 log-sum-exp over it, but never above that."""
+    import torch
+
+    from pih_amd.linear import lm_head_distill, lm_head_distill_backward
+
+    vocab = 300
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(rows, hidden, generator=g, device="cuda") * 0.02).to(torch.bfloat16)
+    w = (torch.randn(vocab, hidden, generator=g, device="cuda") * 0.02).to(torch.bfloat16)
+    best, second = (x.double() @ w.double().T).topk(2).indices.unbind(1)
+    ids = torch.stack((best, second), 1).to(torch.int32)
+    teacher = torch.tensor([0.25, 0.125], device="cuda").repeat(rows, 1)
+    loss, lse, z, flag = lm_head_distill(x, w, ids, teacher, temperature)
+    assert int(flag.item()) == 0 and torch.isfinite(lse).all()
+    # (a row's loss is T^2 times a difference of numbers like lse)
+    assert torch.all(loss.abs().double() <= temperature ** 2 * lse.abs().double() * 4 * U)
+    dx, dw, flag = lm_head_distill_backward(x, w, ids, teacher, lse, z, torch.ones(rows, device="cuda"), temperature)
+    assert int(flag.item()) == 0 and torch.isfinite(dx).all() and torch.isfinite(dw).all()
+    # (two sides, rounded to bf16 twice)
+    most = 2 * temperature * (1 + 4 * HALF_BF16)
+    assert torch.all(dx.double().abs() <= most * w.double().abs().max())
+    assert torch.all(dw.double().abs() <= most * x.double().abs().sum(0))
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,top_k", [(33, 65, 128, 7), (17, 64, 200, 65), (130, 2050, 192, 32),
+                                                     (300, 5000, 128, 64), (515, 300, 64, 4)])
+@pytest.mark.parametrize("temperature,tail", [(9e-4, False), (5e-4, True)])
+def test_backward_below_a_thousandth(eng, rows, vocab, hidden, top_k, temperature, tail):
+    import torch
+
+    from pih_amd.linear import lm_head_distill_backward
+
+    case = _case(rows * 3 + vocab, rows, vocab, hidden, top_k, std=0.02)
+    # (the teacher's logits as far apart over the temperature as the head's)
+    case = case[:3] + (case[3] * 0.01, case[4] * 0.01) + case[5:]
+    teacher_lse, _, lse, z = _forward_ref(*case[:5], temperature, tail)
+    lse, z = lse[0].float(), z[0].float()
+    dx, dw = _grads_ref(*case[:5], case[5], lse, temperature, tail)
+    x, w, ids, teacher = (t.cuda() for t in case[:4])
+    gx, gw, flag = lm_head_distill_backward(x, w, ids, teacher, lse.cuda(), z.cuda(), case[5].cuda(), temperature,
+                                            teacher_lse=None if teacher_lse is None else teacher_lse.cuda())
+    torch.cuda.synchronize()
+    assert int(flag.item()) == 0
+    _within(gx, dx, "dx")
+    _within(gw, dw, "dw")
