@@ -20,7 +20,7 @@
 //
 // Measured: 1 row of 4096 x 2048 15 us (50 MB; the host's time of a call), 57 rows
 // of 4096 x 12288 69 us (302 MB at 4.4 TB/s: gate and up 5.4, down 4.6), 4099 rows
-// with gate and up kept 0.92-0.94 ms (1.33 PFLOP/s); gradients of 4096 rows 1.96-2.01 ms
+// with gate and up kept 0.92-0.94 ms (1.33 PFLOP/s); gradients of 4096 rows 1.93-2.01 ms
 // (1.25 PFLOP/s), of 509 rows of 7168 x 2048 142-145 us (0.62 PFLOP/s).  Many rows: the matrix
 // pipe at the clock that power leaves (1.9 GHz; a library product of 4096 x 24576 x
 // 4096 takes 650-750 us over and over, 550 with pauses), and in the gradients what the
